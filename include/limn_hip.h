@@ -4,8 +4,8 @@
  *
  * limn reaches its GPU kernels through ctypes (reference limn/backend_cuda.py:54-151 binds the
  * CUDA driver and NVRTC the same way). The generated loop-nest kernels go through hipRTC and
- * hipModuleLaunchKernel directly; the three fused-attention CUSTOM kernels and the dense
- * contraction are hand-written and exported here.
+ * hipModuleLaunchKernel directly; the three fused-attention CUSTOM kernels, the dense
+ * contraction, attention with score rules and the head's cross entropy are hand-written and exported here.
  *
  * Conventions for every entry point:
  *  - pointers are device pointers (hipMalloc'd), row-major and contiguous;
@@ -199,13 +199,76 @@ int64_t limn_hip_contract_workspace(int dtype, int64_t batch, int64_t M, int64_t
 int limn_hip_contract_pays(int dtype, int64_t batch, int64_t M, int64_t N, int64_t K);
 
 /*
+ * Attention with score rules. Query i of a sequence with L live keys (lengths[b], or t_k) sits at position
+ * p(i) = L - t_q + i: the queries are the last of its positions. Query head h reads key head
+ * h / (heads / kv_heads), and
+ *   s[i, j] = cap(scale q_i . k_j) - slopes[h] |p(i) - j|,  cap(x) = softcap tanh(x / softcap), or x at 0
+ *   out_i = sum_j softmax_j(s[i, j]) v_j over the keys j that query i sees: j < L; where the call is causal,
+ *   j <= p(i) or j < prefix[b]; where documents are given, documents[b][p(i)] == documents[b][j] >= 0.
+ * A query that sees no key gets a row of zeros, an lse of -inf and no gradient; a hidden key gets zero
+ * gradients. A hidden key's values, infinities and NaN among them, change nothing in the rows that do not
+ * see it, and keys from L on are not read.
+ *   q (batch, heads, t_q, hd), k (batch, kv_heads, t_k, hd), v (batch, kv_heads, t_k, hd_v) -> out (batch,
+ *   heads, t_q, hd_v) of float32, float16 or bfloat16, lse (batch, heads, t_q) float32; slopes (heads)
+ *   float32, documents (batch, t_k), prefix (batch) and lengths (batch) int32, each NULL for none. A length
+ *   outside [0, t_k] is taken as the nearest end. t_q <= t_k where the call is causal or has documents or
+ *   lengths. hd and hd_v at most 256.
+ * `workspace` must hold limn_hip_attend_workspace(...) bytes, 16-byte aligned, for this call alone: calls
+ * that may overlap, and captured graphs that may run at once, need one each. Every result is deterministic.
+ * No counterpart in the reference (its attention has a causal and a key mask, limn/tensor.py:509-575);
+ * composed there, the scores are a tensor in memory.
+ */
+int limn_hip_attend_fwd(const void* q, const void* k, const void* v, const void* slopes, const void* documents,
+                        const void* prefix, const void* lengths, void* out, void* lse, int dtype, int64_t batch,
+                        int64_t heads, int64_t kv_heads, int64_t t_q, int64_t t_k, int64_t hd, int64_t hd_v, int causal,
+                        double scale, double softcap, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Its gradients for the cotangent dout of out, from the forward's out and lse: dq of q's shape, dk and dv of
+ * k's and v's (summed over the query heads that share a key head). */
+int limn_hip_attend_bwd(const void* q, const void* k, const void* v, const void* slopes, const void* documents,
+                        const void* prefix, const void* lengths, const void* out, const void* lse, const void* dout,
+                        void* dq, void* dk, void* dv, int dtype, int64_t batch, int64_t heads, int64_t kv_heads,
+                        int64_t t_q, int64_t t_k, int64_t hd, int64_t hd_v, int causal, double scale, double softcap,
+                        void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Workspace bytes of limn_hip_attend_fwd (backward = 0) or limn_hip_attend_bwd; 0 when it needs none, or has
+ * no kernel for such a call (which then says so). */
+int64_t limn_hip_attend_workspace(int dtype, int64_t batch, int64_t heads, int64_t kv_heads, int64_t t_q, int64_t t_k,
+                                  int64_t hd, int64_t hd_v, int backward);
+
+/*
+ * The softmax cross entropy of a language model's head, straight from its input rows and weight: with
+ * z[n, v] = x[n] . w[v],
+ *   loss[n] = lse[n] - z[n, targets[n]], lse[n] = logsumexp_v z[n, v]
+ * The logits are never kept: the vocabulary goes by in pieces. A target outside [0, vocab) leaves its row
+ * out: loss 0, no gradient, and what the row holds reaches nothing.
+ *   x (rows, width) and w (vocab, width) of float32, float16 or bfloat16, targets (rows) int32; loss and lse
+ *   (rows) float32. Sums and statistics are float32.
+ * Workspace as for limn_hip_attend_fwd, of limn_hip_xent_workspace(...) bytes. No counterpart in the reference,
+ * whose training example takes log_softmax of the logits (examples/train_stories.py:61-64).
+ */
+int limn_hip_xent_fwd(const void* x, const void* w, const void* targets, void* loss, void* lse, int dtype, int64_t rows,
+                      int64_t width, int64_t vocab, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Its gradients for the cotangents g (rows, float32) of loss: dx = dz w and dw = dz^T x, with
+ * dz[n, v] = g[n] (exp(z[n, v] - lse[n]) - [v = targets[n]]); a half width rounds dz to its own type, as the
+ * operand of both products. */
+int limn_hip_xent_bwd(const void* x, const void* w, const void* targets, const void* lse, const void* g, void* dx, void* dw,
+                      int dtype, int64_t rows, int64_t width, int64_t vocab, void* workspace, int64_t workspace_bytes,
+                      void* stream);
+
+int64_t limn_hip_xent_workspace(int dtype, int64_t rows, int64_t width, int64_t vocab, int backward);
+
+/*
  * A pre-bound launch list: the kernels of one recorded execution of a plan, replayed against new
  * buffers. Each step is one launch: a hipRTC module kernel (`function`, `grid` x `block`
  * threads, its arguments the kernel's parameters in order), a zero fill (pointer, bytes), or one
  * call of limn_hip_matmul (its 20 arguments before `stream`), limn_hip_matmul_add or
  * limn_hip_contract (27), limn_hip_sdpa_fwd (13 before `scale`), limn_hip_sdpa_bwd_q (15),
  * limn_hip_sdpa_bwd_kv (16) or limn_hip_sdpa_bwd (17 before `scale`, then passes, workspace and
- * its size: 20), with `scale` in the step. An
+ * its size: 20), limn_hip_attend_fwd (18 before `scale`, then softcap as the bits of a double, workspace and
+ * its size: 21), limn_hip_attend_bwd (22, then the same: 25), with `scale` in the step, limn_hip_xent_fwd (11)
+ * or limn_hip_xent_bwd (13). An
  * argument is `value` when `slot` < 0, else slots[slot] + value: a byte offset into the buffer
  * this replay binds to that slot. Steps run in order on `stream`; the first failing one stops the
  * list and its status is returned. No counterpart in the reference: its capture replays a plan
@@ -221,6 +284,10 @@ enum {
   LIMN_HIP_STEP_MATMUL_ADD = 6,
   LIMN_HIP_STEP_SDPA_BWD = 7,
   LIMN_HIP_STEP_CONTRACT = 8,
+  LIMN_HIP_STEP_ATTEND_FWD = 9,
+  LIMN_HIP_STEP_ATTEND_BWD = 10,
+  LIMN_HIP_STEP_XENT_FWD = 11,
+  LIMN_HIP_STEP_XENT_BWD = 12,
 };
 
 typedef struct {

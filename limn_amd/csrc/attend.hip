@@ -1,0 +1,176 @@
+// The C ABI of attention with score rules (include/limn_hip.h): argument checks, choice of kernels, workspaces;
+// and the kernel that joins partial results of a call whose keys are split over workgroups.
+
+#include <math.h>
+
+#include "attend_rules.h"
+
+namespace limn {
+
+int attend_general_fwd_f32(const AttendArgs& a, int64_t splits);
+int attend_general_fwd_f16(const AttendArgs& a, int64_t splits);
+int attend_general_fwd_bf16(const AttendArgs& a, int64_t splits);
+int attend_general_bwd_f32(const AttendArgs& a);
+int attend_general_bwd_f16(const AttendArgs& a);
+int attend_general_bwd_bf16(const AttendArgs& a);
+
+namespace {
+
+// One wave per packed row: the splits' reference points brought to the largest, their sums and totals added
+// in split order, so that the result does not depend on which workgroup ended first.
+template <typename T>
+__global__ __launch_bounds__(64) void attend_join(const float* __restrict__ totals, const float* __restrict__ stats,
+                                                  typename T::Storage* __restrict__ out, float* __restrict__ lse, int64_t rows_all,
+                                                  int splits, int group, int kv_heads, int t_q, int hd_v) {
+  const int64_t row = blockIdx.x;
+  const int64_t per = (int64_t)group * t_q, bk = row / per, r = row % per;
+  float top = -__builtin_inff(), total = 0.f;
+  for (int s = 0; s < splits; s++) top = fmaxf(top, stats[(s * rows_all + row) * 2]);
+  const float base = top == -__builtin_inff() ? 0.f : top;
+  for (int s = 0; s < splits; s++) {
+    const float* st = stats + (s * rows_all + row) * 2;
+    total += st[0] == -__builtin_inff() ? st[1] : st[1] * fast_exp2(st[0] - base);
+  }
+  // bk = b * kv_heads + kvh; head kvh * group + r % group of sequence b
+  const int64_t at = (bk * group + r % group) * t_q + r / group;
+  const float inv = total == 0.f ? 0.f : 1.f / total;
+  for (int d = threadIdx.x; d < hd_v; d += 64) {
+    float x = 0.f;
+    for (int s = 0; s < splits; s++) {
+      const float m = stats[(s * rows_all + row) * 2];
+      x += totals[(s * rows_all + row) * hd_v + d] * (m == -__builtin_inff() ? 1.f : fast_exp2(m - base));
+    }
+    T::store(out + at * hd_v, d, total == 0.f ? 0.f : x * inv);
+  }
+  if (threadIdx.x == 0) lse[at] = total == 0.f ? -__builtin_inff() : base * ATT_LN2 + logf(total);
+}
+
+template <typename T>
+int join(const AttendArgs& a, const float* totals, const float* stats, int64_t splits) {
+  const int64_t rows_all = a.batch * a.heads * a.t_q;
+  if (rows_all > 0x7fffffff) return fail(LIMN_HIP_EUNSUPPORTED, "attend: %lld rows exceed one launch", (long long)rows_all);
+  hipLaunchKernelGGL((attend_join<T>), dim3((unsigned)rows_all), dim3(64), 0, a.stream, totals, stats, (typename T::Storage*)a.o0, (float*)a.o1,
+                     rows_all, (int)splits, (int)a.group(), (int)a.kv_heads, (int)a.t_q, (int)a.hd_v);
+  return check_hip(hipGetLastError(), "joining attention's splits");
+}
+
+constexpr int64_t FILL = 512;  // workgroups that give every CU two
+
+// Parts of the keys a general forward is cut into: rows in too few tiles to fill the GPU walk long
+// sequences in parts of at least 8 key tiles (two a wave).
+int64_t general_splits(const AttendArgs& a) {
+  const int64_t blocks = a.batch * a.kv_heads * ((a.group() * a.t_q + 31) / 32), tiles = (a.t_k + 31) / 32;
+  int64_t splits = (FILL + blocks - 1) / blocks;
+  splits = splits < tiles / 8 ? splits : tiles / 8;
+  return splits > 1 ? splits : 1;
+}
+
+int64_t split_bytes(const AttendArgs& a, int64_t splits) {
+  const int64_t rows = a.batch * a.heads * a.t_q;
+  return splits > 1 ? attend_align(splits * rows * a.hd_v * 4) + attend_align(splits * rows * 8) : 0;
+}
+
+int check_attend(const char* name, const AttendArgs& a) {
+  if (a.dtype != LIMN_HIP_FLOAT32 && a.dtype != LIMN_HIP_FLOAT16 && a.dtype != LIMN_HIP_BFLOAT16)
+    return fail(LIMN_HIP_EUNSUPPORTED, "%s: takes float32, float16 or bfloat16, not dtype code %d", name, a.dtype);
+  if (a.batch < 1 || a.heads < 1 || a.kv_heads < 1 || a.t_q < 1 || a.t_k < 1 || a.hd < 1 || a.hd_v < 1)
+    return fail(LIMN_HIP_EINVAL, "%s: sizes must be positive (batch %lld, heads %lld, kv_heads %lld, t_q %lld, t_k %lld, hd %lld, hd_v %lld)", name,
+                (long long)a.batch, (long long)a.heads, (long long)a.kv_heads, (long long)a.t_q, (long long)a.t_k, (long long)a.hd, (long long)a.hd_v);
+  if (a.heads % a.kv_heads != 0)
+    return fail(LIMN_HIP_EINVAL, "%s: %lld query heads do not share %lld key heads evenly", name, (long long)a.heads, (long long)a.kv_heads);
+  if (a.t_q > a.t_k && (a.causal || a.documents != nullptr || a.lengths != nullptr))
+    return fail(LIMN_HIP_EINVAL, "%s: the queries are the last of the keys' positions: %lld queries and %lld keys", name, (long long)a.t_q, (long long)a.t_k);
+  if (!isfinite(a.scale)) return fail(LIMN_HIP_EINVAL, "%s: scale must be finite", name);
+  if (!isfinite(a.softcap) || a.softcap < 0) return fail(LIMN_HIP_EINVAL, "%s: softcap must be finite, and positive or 0 for none", name);
+  if (a.prefix != nullptr && !a.causal) return fail(LIMN_HIP_EINVAL, "%s: a prefix opens keys that causality hides; the call is not causal", name);
+  if (a.hd > 256 || a.hd_v > 256) return fail(LIMN_HIP_EUNSUPPORTED, "%s: no kernel for head dims %lld and %lld (at most 256)", name, (long long)a.hd, (long long)a.hd_v);
+  // positions and packed rows are 32-bit in the kernels; element offsets are 64-bit
+  const int64_t most = (int64_t)1 << 30;
+  if (a.t_k > most || a.t_q > most / a.group() || a.heads > most || a.batch > ((int64_t)1 << 40) / a.heads / (a.t_q > a.t_k ? a.t_q : a.t_k))
+    return fail(LIMN_HIP_EUNSUPPORTED, "%s: sizes out of range", name);
+  return LIMN_HIP_OK;
+}
+
+int check_pointers(const char* name, const AttendArgs& a, bool backward) {
+  if (a.q == nullptr || a.k == nullptr || a.v == nullptr || a.o0 == nullptr || a.o1 == nullptr) return fail(LIMN_HIP_EINVAL, "%s: null buffer", name);
+  if (backward && (a.out == nullptr || a.lse == nullptr || a.dout == nullptr || a.o2 == nullptr)) return fail(LIMN_HIP_EINVAL, "%s: null buffer", name);
+  const uintptr_t size = a.dtype == LIMN_HIP_FLOAT32 ? 4 : 2;
+  const uintptr_t typed = (uintptr_t)a.q | (uintptr_t)a.k | (uintptr_t)a.v | (uintptr_t)a.o0 | (uintptr_t)a.out | (uintptr_t)a.dout | (uintptr_t)a.o2 | (backward ? (uintptr_t)a.o1 : 0);
+  const uintptr_t words = (uintptr_t)a.slopes | (uintptr_t)a.documents | (uintptr_t)a.prefix | (uintptr_t)a.lengths | (uintptr_t)a.lse | (backward ? 0 : (uintptr_t)a.o1);
+  if (typed % size != 0 || words % 4 != 0) return fail(LIMN_HIP_EINVAL, "%s: buffers must be aligned to their element size", name);
+  if (a.workspace_bytes < 0) return fail(LIMN_HIP_EINVAL, "%s: negative workspace size", name);
+  return LIMN_HIP_OK;
+}
+
+int64_t workspace_of(const AttendArgs& a, bool backward) { return attend_general_workspace(a, backward); }
+
+int check_workspace(const char* name, const AttendArgs& a, bool backward) {
+  const int64_t need = workspace_of(a, backward);
+  if (need > 0 && (a.workspace == nullptr || a.workspace_bytes < need || (uintptr_t)a.workspace % 16 != 0))
+    return fail(LIMN_HIP_EINVAL, "%s: needs a workspace of %lld bytes, 16-byte aligned", name, (long long)need);
+  return LIMN_HIP_OK;
+}
+
+}  // namespace
+
+int launch_attend_join(const AttendArgs& a, const float* totals, const float* stats, int64_t splits) {
+  if (a.dtype == LIMN_HIP_FLOAT32) return join<F32>(a, totals, stats, splits);
+  return a.dtype == LIMN_HIP_FLOAT16 ? join<F16>(a, totals, stats, splits) : join<BF16>(a, totals, stats, splits);
+}
+
+int64_t attend_general_workspace(const AttendArgs& a, bool backward) {
+  return backward ? attend_align(a.batch * a.heads * a.t_q * 4) : split_bytes(a, general_splits(a));
+}
+
+int launch_attend_general_fwd(const AttendArgs& a) {
+  const int64_t splits = general_splits(a);
+  if (a.dtype == LIMN_HIP_FLOAT32) return attend_general_fwd_f32(a, splits);
+  return a.dtype == LIMN_HIP_FLOAT16 ? attend_general_fwd_f16(a, splits) : attend_general_fwd_bf16(a, splits);
+}
+
+int launch_attend_general_bwd(const AttendArgs& a) {
+  if (a.dtype == LIMN_HIP_FLOAT32) return attend_general_bwd_f32(a);
+  return a.dtype == LIMN_HIP_FLOAT16 ? attend_general_bwd_f16(a) : attend_general_bwd_bf16(a);
+}
+
+}  // namespace limn
+
+using namespace limn;
+
+extern "C" {
+
+int64_t limn_hip_attend_workspace(int dtype, int64_t batch, int64_t heads, int64_t kv_heads, int64_t t_q, int64_t t_k, int64_t hd,
+                                  int64_t hd_v, int backward) {
+  AttendArgs a = {};
+  a.dtype = dtype, a.batch = batch, a.heads = heads, a.kv_heads = kv_heads, a.t_q = t_q, a.t_k = t_k, a.hd = hd, a.hd_v = hd_v;
+  if (check_attend("attend_workspace", a) != LIMN_HIP_OK) return 0;
+  return workspace_of(a, backward != 0);
+}
+
+int limn_hip_attend_fwd(const void* q, const void* k, const void* v, const void* slopes, const void* documents, const void* prefix,
+                        const void* lengths, void* out, void* lse, int dtype, int64_t batch, int64_t heads, int64_t kv_heads, int64_t t_q,
+                        int64_t t_k, int64_t hd, int64_t hd_v, int causal, double scale, double softcap, void* workspace,
+                        int64_t workspace_bytes, void* stream) {
+  AttendArgs a = {q, k, v, (const float*)slopes, (const int*)documents, (const int*)prefix, (const int*)lengths, nullptr, nullptr, nullptr,
+                  out, lse, nullptr, dtype, batch, heads, kv_heads, t_q, t_k, hd, hd_v, causal != 0, scale, softcap, workspace, workspace_bytes,
+                  (hipStream_t)stream};
+  int rc = check_attend("attend_fwd", a);
+  if (rc == LIMN_HIP_OK) rc = check_pointers("attend_fwd", a, false);
+  if (rc == LIMN_HIP_OK) rc = check_workspace("attend_fwd", a, false);
+  return rc != LIMN_HIP_OK ? rc : launch_attend_general_fwd(a);
+}
+
+int limn_hip_attend_bwd(const void* q, const void* k, const void* v, const void* slopes, const void* documents, const void* prefix,
+                        const void* lengths, const void* out, const void* lse, const void* dout, void* dq, void* dk, void* dv, int dtype,
+                        int64_t batch, int64_t heads, int64_t kv_heads, int64_t t_q, int64_t t_k, int64_t hd, int64_t hd_v, int causal,
+                        double scale, double softcap, void* workspace, int64_t workspace_bytes, void* stream) {
+  AttendArgs a = {q, k, v, (const float*)slopes, (const int*)documents, (const int*)prefix, (const int*)lengths, out, (const float*)lse, dout,
+                  dq, dk, dv, dtype, batch, heads, kv_heads, t_q, t_k, hd, hd_v, causal != 0, scale, softcap, workspace, workspace_bytes,
+                  (hipStream_t)stream};
+  int rc = check_attend("attend_bwd", a);
+  if (rc == LIMN_HIP_OK) rc = check_pointers("attend_bwd", a, true);
+  if (rc == LIMN_HIP_OK) rc = check_workspace("attend_bwd", a, true);
+  return rc != LIMN_HIP_OK ? rc : launch_attend_general_bwd(a);
+}
+
+}  // extern "C"

@@ -7,6 +7,7 @@
 // on one stream; nothing is looked up or rebuilt per launch.
 
 #include <stdio.h>
+#include <string.h>
 
 #include <vector>
 
@@ -137,6 +138,44 @@ int run_step(const limn_hip_replay_step& s, int64_t i, const limn_hip_replay_arg
                                (const void*)(intptr_t)v[6], (void*)(intptr_t)v[7], (void*)(intptr_t)v[8], (void*)(intptr_t)v[9],
                                (int)v[10], v[11], v[12], v[13], v[14], v[15], (int)v[16], s.scale, (int)v[17], (void*)(intptr_t)v[18],
                                v[19], stream);
+    }
+    case LIMN_HIP_STEP_ATTEND_FWD: {
+      int rc = expect(s, i, 21, "attend_fwd");
+      if (rc != LIMN_HIP_OK) return rc;
+      int64_t v[21];
+      for (int k = 0; k < 21; k++) v[k] = bound(a[k], slots);
+      auto at = [&](int k) { return (void*)(intptr_t)v[k]; };
+      double softcap;
+      memcpy(&softcap, &v[18], sizeof softcap);
+      return limn_hip_attend_fwd(at(0), at(1), at(2), at(3), at(4), at(5), at(6), at(7), at(8), (int)v[9], v[10], v[11], v[12], v[13], v[14], v[15],
+                                 v[16], (int)v[17], s.scale, softcap, at(19), v[20], stream);
+    }
+    case LIMN_HIP_STEP_ATTEND_BWD: {
+      int rc = expect(s, i, 25, "attend_bwd");
+      if (rc != LIMN_HIP_OK) return rc;
+      int64_t v[25];
+      for (int k = 0; k < 25; k++) v[k] = bound(a[k], slots);
+      auto at = [&](int k) { return (void*)(intptr_t)v[k]; };
+      double softcap;
+      memcpy(&softcap, &v[22], sizeof softcap);
+      return limn_hip_attend_bwd(at(0), at(1), at(2), at(3), at(4), at(5), at(6), at(7), at(8), at(9), at(10), at(11), at(12), (int)v[13], v[14],
+                                 v[15], v[16], v[17], v[18], v[19], v[20], (int)v[21], s.scale, softcap, at(23), v[24], stream);
+    }
+    case LIMN_HIP_STEP_XENT_FWD: {
+      int rc = expect(s, i, 11, "xent_fwd");
+      if (rc != LIMN_HIP_OK) return rc;
+      int64_t v[11];
+      for (int k = 0; k < 11; k++) v[k] = bound(a[k], slots);
+      auto at = [&](int k) { return (void*)(intptr_t)v[k]; };
+      return limn_hip_xent_fwd(at(0), at(1), at(2), at(3), at(4), (int)v[5], v[6], v[7], v[8], at(9), v[10], stream);
+    }
+    case LIMN_HIP_STEP_XENT_BWD: {
+      int rc = expect(s, i, 13, "xent_bwd");
+      if (rc != LIMN_HIP_OK) return rc;
+      int64_t v[13];
+      for (int k = 0; k < 13; k++) v[k] = bound(a[k], slots);
+      auto at = [&](int k) { return (void*)(intptr_t)v[k]; };
+      return limn_hip_xent_bwd(at(0), at(1), at(2), at(3), at(4), at(5), at(6), (int)v[7], v[8], v[9], v[10], at(11), v[12], stream);
     }
     default:
       return fail(LIMN_HIP_EINVAL, "replay step %lld: unknown kind %d", (long long)i, s.kind);

@@ -8,7 +8,8 @@ this GPU rather than translated:
 - lowered loop nests are rendered by limn_amd/hip/emit.py into gfx950 kernels, compiled by
   hipRTC once per program and launched with hipModuleLaunchKernel on the null stream;
 - the CUSTOM attention kernels `sdpa`, `sdpa_bwd_q` and `sdpa_bwd_kv` are the hand-written
-  MFMA/LDS kernels of liblimn_hip.so, reached through its C ABI (include/limn_hip.h);
+  MFMA/LDS kernels of liblimn_hip.so, reached through its C ABI (include/limn_hip.h), and so are
+  `attend_fwd`/`attend_bwd` (limn_amd/attend.py) and `xent_fwd`/`xent_bwd` (limn_amd/xent.py);
 - host arrays handed in are uploaded per batch (`prepare`), and an ASSIGN whose target is a host
   array is written back (`commit`), as the reference device does;
 - `finish()` synchronizes once per batch, which pins an asynchronous failure to its batch.
@@ -21,6 +22,8 @@ import ctypes
 import dataclasses
 import math
 import time
+import weakref
+from collections.abc import Callable
 from typing import Any
 
 import numpy as np
@@ -28,11 +31,12 @@ import numpy as np
 from limn_amd.dtypes import ABI_CODE
 from limn_amd.hip import replay, runtime
 from limn_amd.hip.runtime import DEVICE_TO_DEVICE, DEVICE_TO_HOST, HOST_TO_DEVICE, check, check_limn
-from limn_amd.seam import FLOATS, CompiledDevice, LoopNest, Node, Op, Runner, accumulate_in, realized
+from limn_amd.seam import FLOATS, CompiledDevice, LoopNest, Node, Op, Runner, accumulate_in, float32, int32, realized
 
 Buffer = Any
 
 SDPA, SDPA_BWD_Q, SDPA_BWD_KV = "sdpa", "sdpa_bwd_q", "sdpa_bwd_kv"
+ATTEND_FWD, ATTEND_BWD, XENT_FWD, XENT_BWD = "attend_fwd", "attend_bwd", "xent_fwd", "xent_bwd"  # limn_amd/attend.py, limn_amd/xent.py
 BWD_BOTH = 3  # LIMN_HIP_BWD_BOTH: limn_hip_sdpa_bwd runs both passes
 
 
@@ -69,7 +73,7 @@ def plan_context(order: list[Node], sinks: list[Node]) -> tuple[set, set]:
 class HipBuffer:
     """Device bytes; the pointer returns to its device's pool when the last reference drops."""
 
-    __slots__ = ("ptr", "nbytes", "pool")
+    __slots__ = ("ptr", "nbytes", "pool", "__weakref__")
 
     def __init__(self, ptr: int, nbytes: int, pool: dict[int, list[int]]):
         self.ptr = ptr
@@ -138,9 +142,12 @@ class HipDevice(CompiledDevice):
         self._committed: list[tuple[Buffer, Buffer]] = []  # launched, kept alive until the barrier
         self._commit_table: tuple[int, int, Buffer] | None = None  # (pinned host ptr, rows, device copy)
         self._commit_kernel: int | None = None
+        self._workspaces: weakref.WeakValueDictionary[int, HipBuffer] = weakref.WeakValueDictionary()  # by bytes, see _held
         self.custom[SDPA] = self._sdpa_runner
         self.custom[SDPA_BWD_Q] = self._sdpa_runner
         self.custom[SDPA_BWD_KV] = self._sdpa_runner
+        self.custom[ATTEND_FWD] = self.custom[ATTEND_BWD] = self._attend_runner
+        self.custom[XENT_FWD] = self.custom[XENT_BWD] = self._xent_runner
         # pre-bound launch lists: id(plan) -> [plan, Program or None, refused], least recently
         # run first, at most replay.PLANS_KEPT; `tape` collects the launches of the run that
         # records one (every launch site appends while it is set)
@@ -515,5 +522,98 @@ class HipDevice(CompiledDevice):
             check_limn(lib.limn_hip_sdpa_bwd(*args, scale, BWD_BOTH, ws.ptr, ws.nbytes, None))
             if self.tape is not None:
                 self.tape.append(replay.Launch(replay.STEP_SDPA_BWD, (*args, BWD_BOTH, ws.ptr, ws.nbytes), scale=scale))
+
+        return run
+
+    def _held(self, need: int) -> Callable[[], tuple[int | None, int]]:
+        """A runner's workspace as (pointer, bytes): taken on its first run and kept with it, so a replayed
+        or graph-captured list sees the same pointer every time. Runners that need as many bytes share one
+        (the layers of a model, say): every launch of the device is on the null stream, one runner's after
+        another's."""
+        held: list = []
+
+        def workspace() -> tuple[int | None, int]:
+            if need <= 0:
+                return None, 0
+            if not held:
+                shared = self._workspaces.get(need)
+                if shared is None:
+                    shared = self._workspaces[need] = self._alloc(need)
+                held.append(shared)
+            return held[0].ptr, held[0].nbytes
+
+        return workspace
+
+    # ---- attention with score rules, the head's cross entropy ----
+
+    def _attend_runner(self, node: Node) -> Runner:
+        """CUSTOM attend_fwd (srcs q, k, v, the rules given) and attend_bwd (and then out, lse, dout), bound
+        to limn_hip_attend_fwd and limn_hip_attend_bwd. params: (causal, scale, softcap, which of slopes,
+        documents, prefix, lengths are given)."""
+        name = node.arg.name
+        causal, scale, softcap, given = node.arg.params
+        backward, count = name == ATTEND_BWD, 3 + sum(given)
+        if len(node.srcs) != count + 3 * backward:
+            raise ValueError(f"{name}: expected {count + 3 * backward} srcs, got {len(node.srcs)}")
+        q, k, v = node.srcs[:3]
+        if q.dtype not in ABI_CODE or q.dtype not in FLOATS or any(s.dtype != q.dtype for s in (k, v)):
+            raise NotImplementedError(f"{name}: no kernel for dtypes {q.dtype}, {k.dtype}, {v.dtype}")
+        lead, (heads, t_q, hd) = q.shape[:-3], q.shape[-3:]
+        kv_heads, t_k = k.shape[-3:-1]
+        hd_v = v.shape[-1]
+        batch = math.prod(lead)
+        if k.shape != lead + (kv_heads, t_k, hd) or v.shape != lead + (kv_heads, t_k, hd_v):
+            raise ValueError(f"{name} shape mismatch: {q.shape}, {k.shape}, {v.shape}")
+        rules = iter(node.srcs[3:count])
+        for on, shape, dtype in zip(given, ((heads,), lead + (t_k,), lead, lead), (float32, int32, int32, int32)):
+            rule = next(rules) if on else None
+            if rule is not None and (rule.shape != shape or rule.dtype != dtype):
+                raise ValueError(f"{name}: a rule must be {shape} {dtype}, got {rule.shape} {rule.dtype}")
+        if backward:
+            out, lse, do = node.srcs[count:]
+            rows = lead + (heads, t_q)
+            if out.shape != rows + (hd_v,) or do.shape != rows + (hd_v,) or do.dtype != q.dtype or math.prod(lse.shape) != math.prod(rows):
+                raise ValueError(f"{name} shape mismatch: out {out.shape}, dout {do.shape} {do.dtype}, lse {lse.shape}")
+        code, sizes = ABI_CODE[q.dtype], (batch, heads, kv_heads, t_q, t_k, hd, hd_v)
+        flags, scale, softcap = int(bool(causal)), float(scale), float(softcap)
+        workspace = self._held(int(self.lib.limn_hip_attend_workspace(code, *sizes, int(backward))))
+        entry = self.lib.limn_hip_attend_bwd if backward else self.lib.limn_hip_attend_fwd
+        kind = replay.STEP_ATTEND_BWD if backward else replay.STEP_ATTEND_FWD
+        cap_bits = ctypes.c_int64.from_buffer_copy(ctypes.c_double(softcap)).value
+
+        def run(inputs: list[Buffer], outs: list[Buffer]) -> None:
+            ptrs = [b.ptr for b in inputs]
+            rules = iter(ptrs[3:count])
+            args = (*ptrs[:3], *(next(rules) if on else None for on in given), *ptrs[count:], *(b.ptr for b in outs), code, *sizes, flags)
+            ws, room = workspace()
+            check_limn(entry(*args, scale, softcap, ws, room, None))
+            if self.tape is not None:
+                self.tape.append(replay.Launch(kind, (*args, cap_bits, ws, room), scale=scale))
+
+        return run
+
+    def _xent_runner(self, node: Node) -> Runner:
+        """CUSTOM xent_fwd (srcs x, weight, targets) and xent_bwd (and then lse and the losses' cotangents),
+        bound to limn_hip_xent_fwd and limn_hip_xent_bwd."""
+        name = node.arg.name
+        backward = name == XENT_BWD
+        if len(node.srcs) != 3 + 2 * backward:
+            raise ValueError(f"{name}: expected {3 + 2 * backward} srcs, got {len(node.srcs)}")
+        x, w, targets = node.srcs[:3]
+        if x.dtype not in ABI_CODE or x.dtype not in FLOATS or w.dtype != x.dtype:
+            raise NotImplementedError(f"{name}: no kernel for dtypes {x.dtype} and {w.dtype}")
+        if len(x.shape) != 2 or len(w.shape) != 2 or x.shape[1] != w.shape[1] or any(math.prod(s.shape) != x.shape[0] for s in (targets, *node.srcs[3:])):
+            raise ValueError(f"{name} shape mismatch: {[s.shape for s in node.srcs]}")
+        code, sizes = ABI_CODE[x.dtype], (x.shape[0], x.shape[1], w.shape[0])
+        workspace = self._held(int(self.lib.limn_hip_xent_workspace(code, *sizes, int(backward))))
+        entry = self.lib.limn_hip_xent_bwd if backward else self.lib.limn_hip_xent_fwd
+        kind = replay.STEP_XENT_BWD if backward else replay.STEP_XENT_FWD
+
+        def run(inputs: list[Buffer], outs: list[Buffer]) -> None:
+            args = (*(b.ptr for b in inputs), *(b.ptr for b in outs), code, *sizes)
+            ws, room = workspace()
+            check_limn(entry(*args, ws, room, None))
+            if self.tape is not None:
+                self.tape.append(replay.Launch(kind, (*args, ws, room)))
 
         return run

@@ -28,7 +28,7 @@ from dataclasses import dataclass, field
 import numpy as np
 
 (STEP_KERNEL, STEP_ZERO, STEP_MATMUL, STEP_SDPA_FWD, STEP_SDPA_BWD_Q, STEP_SDPA_BWD_KV, STEP_MATMUL_ADD,
- STEP_SDPA_BWD, STEP_CONTRACT) = range(9)
+ STEP_SDPA_BWD, STEP_CONTRACT, STEP_ATTEND_FWD, STEP_ATTEND_BWD, STEP_XENT_FWD, STEP_XENT_BWD) = range(13)
 
 # which arguments of each step kind are device pointers (the rest are sizes, codes and flags)
 POINTER_ARGS = {
@@ -40,7 +40,13 @@ POINTER_ARGS = {
     STEP_SDPA_BWD_Q: frozenset(range(8)),
     STEP_SDPA_BWD_KV: frozenset(range(9)),
     STEP_SDPA_BWD: frozenset(range(10)) | {18},
+    STEP_ATTEND_FWD: frozenset(range(9)) | {19},
+    STEP_ATTEND_BWD: frozenset(range(13)) | {23},
+    STEP_XENT_FWD: frozenset(range(5)) | {9},
+    STEP_XENT_BWD: frozenset(range(7)) | {11},
 }
+
+LAUNCHES = {STEP_SDPA_BWD: 2, STEP_ATTEND_BWD: 2, STEP_XENT_FWD: 3, STEP_XENT_BWD: 5}
 
 ARG = np.dtype([("value", np.int64), ("slot", np.int32), ("reserved", np.int32)])
 STEP = np.dtype([("kind", np.int32), ("nargs", np.int32), ("first", np.int64), ("function", np.uint64),
@@ -86,7 +92,8 @@ class Program:
     @functools.cached_property
     def launches(self) -> int:
         """Kernel launches of the list, at most: a contraction given a workspace may fold k slices, one of
-        half widths copy its operands as well; a paired attention backward is two."""
+        half widths copy its operands as well; attention given a workspace may join parts; LAUNCHES has the
+        kinds of several (a cross entropy's for one piece of the vocabulary)."""
         total = 0
         for kind, first in zip(self.steps["kind"].tolist(), self.steps["first"].tolist()):
             value = lambda k: int(self.args["value"][first + k])
@@ -94,8 +101,10 @@ class Program:
                 total += 1 + (value(19 if kind == STEP_MATMUL else 26) > 0)
             elif kind == STEP_CONTRACT:
                 total += 1 + (value(26) > 0) * (1 if value(3) == 1 else 2)
+            elif kind == STEP_ATTEND_FWD:
+                total += 1 + (value(20) > 0)
             else:
-                total += 2 if kind == STEP_SDPA_BWD else 1
+                total += LAUNCHES.get(kind, 1)
         return total
 
     def launch(self, lib, slots: np.ndarray, stream=None) -> int:

@@ -113,6 +113,12 @@ _LIMN = {
         [c_void_p] * 10 + [c_int, _I64, _I64, _I64, _I64, _I64, c_int, ctypes.c_double, c_int, c_void_p, _I64, c_void_p],
     ),
     "limn_hip_sdpa_bwd_workspace": (_I64, [c_int, _I64, _I64, _I64, _I64, _I64, c_int, c_int]),
+    "limn_hip_attend_fwd": (c_int, [c_void_p] * 9 + [c_int] + [_I64] * 7 + [c_int, ctypes.c_double, ctypes.c_double, c_void_p, _I64, c_void_p]),
+    "limn_hip_attend_bwd": (c_int, [c_void_p] * 13 + [c_int] + [_I64] * 7 + [c_int, ctypes.c_double, ctypes.c_double, c_void_p, _I64, c_void_p]),
+    "limn_hip_attend_workspace": (_I64, [c_int] + [_I64] * 7 + [c_int]),
+    "limn_hip_xent_fwd": (c_int, [c_void_p] * 5 + [c_int, _I64, _I64, _I64, c_void_p, _I64, c_void_p]),
+    "limn_hip_xent_bwd": (c_int, [c_void_p] * 7 + [c_int, _I64, _I64, _I64, c_void_p, _I64, c_void_p]),
+    "limn_hip_xent_workspace": (_I64, [c_int, _I64, _I64, _I64, c_int]),
 }
 
 # The C ABI's status codes (include/limn_hip.h) and the Python exception each maps to.
