@@ -3,7 +3,7 @@
 
 #include <math.h>
 
-#include "attend_rules.h"
+#include "attend_fast.h"
 
 namespace limn {
 
@@ -102,7 +102,80 @@ int check_pointers(const char* name, const AttendArgs& a, bool backward) {
   return LIMN_HIP_OK;
 }
 
-int64_t workspace_of(const AttendArgs& a, bool backward) { return attend_general_workspace(a, backward); }
+// ---- the half-width kernels ----
+
+int64_t granules_of(const AttendArgs& a) { return (a.t_k + 31) / 32; }
+int64_t row_blocks(const AttendArgs& a) { return a.batch * a.heads * ((a.t_q + ATT_ROWS - 1) / ATT_ROWS); }
+int64_t key_blocks(const AttendArgs& a) { return a.batch * a.kv_heads * ((a.t_k + ATT_ROWS - 1) / ATT_ROWS); }
+
+// Sizes the half-width kernels serve: 16-byte rows, a head's rows within 32-bit byte offsets, few enough
+// streamed tiles for a block's list of them.
+bool fast_sizes(const AttendArgs& a) {
+  return a.dtype != LIMN_HIP_FLOAT32 && a.hd == a.hd_v && a.hd % 8 == 0 && a.hd <= 128 && a.t_q <= (1 << 17) && a.t_k <= (1 << 17);
+}
+
+// A call of such sizes goes to them where every buffer is 16-byte aligned and the scale positive (the forward's
+// reference point is taken over unscaled scores).
+bool fast_call(const AttendArgs& a, bool backward) {
+  const uintptr_t at = (uintptr_t)a.q | (uintptr_t)a.k | (uintptr_t)a.v | (uintptr_t)a.o0 | (backward ? (uintptr_t)a.o1 | (uintptr_t)a.o2 | (uintptr_t)a.out | (uintptr_t)a.dout : 0);
+  return fast_sizes(a) && a.scale > 0 && at % 16 == 0;
+}
+
+// flags of the blocks, the documents' ranges, and for the backward delta
+int64_t fast_workspace(const AttendArgs& a, bool backward) {
+  if (!fast_sizes(a)) return 0;
+  int64_t need = attend_align(row_blocks(a) * 4) + attend_align(a.batch * granules_of(a) * 8);
+  if (backward) need += attend_align(key_blocks(a) * 4) + attend_align(a.batch * a.heads * a.t_q * 4);
+  return need;
+}
+
+#define LIMN_ATTEND_WIDTH(PASS) \
+  (a.hd <= 64 ? launch_attend_##PASS##_64 : a.hd <= 96 ? launch_attend_##PASS##_96 : launch_attend_##PASS##_128)
+
+int launch_fast(const AttendArgs& a, bool backward) {
+  const RuleArgs ra = rule_args(a);
+  char* at = (char*)a.workspace;
+  auto take = [&](int64_t bytes) {
+    char* p = at;
+    at += attend_align(bytes);
+    return p;
+  };
+  int* odd = (int*)take(row_blocks(a) * 4);
+  int2* ranges = (int2*)take(a.batch * granules_of(a) * 8);
+  FastArgs g = {};
+  g.q = (const u16*)a.q, g.k = (const u16*)a.k, g.v = (const u16*)a.v, g.out = (const u16*)a.out, g.dout = (const u16*)a.dout;
+  g.lse_in = a.lse, g.o0 = (u16*)a.o0, g.odd = odd, g.ranges = a.documents != nullptr ? ranges : nullptr;
+  g.batch = a.batch, g.heads = (int)a.heads, g.kv_heads = (int)a.kv_heads, g.hd = (int)a.hd, g.granules = (int)granules_of(a), g.scale = (float)a.scale;
+  int rc = LIMN_HIP_OK;
+  if (a.documents != nullptr && (rc = launch_attend_ranges(ra, ranges, a.batch, g.granules, a.stream)) != LIMN_HIP_OK) return rc;
+  // without causality and documents a hidden key is one past the live ones, which reads as zeros
+  const bool mend = a.causal || a.documents != nullptr;
+  if (!backward) {
+    g.lse = (float*)a.o1;
+    rc = LIMN_ATTEND_WIDTH(fwd)(g, ra, a.dtype, a.stream);
+    return rc != LIMN_HIP_OK || !mend ? rc : launch_attend_mend_fwd(g, ra, a.dtype, a.stream);
+  }
+  FastArgs kv = g;
+  kv.odd = (int*)take(key_blocks(a) * 4);
+  g.delta = kv.delta = (float*)take(a.batch * a.heads * a.t_q * 4);
+  kv.o0 = (u16*)a.o1;
+  kv.o1 = (u16*)a.o2;
+  if ((rc = LIMN_ATTEND_WIDTH(dq)(g, ra, a.dtype, a.stream)) != LIMN_HIP_OK) return rc;
+  rc = LIMN_ATTEND_WIDTH(dkv)(kv, ra, a.dtype, a.stream);
+  return rc != LIMN_HIP_OK || !mend ? rc : launch_attend_mend_bwd(g, kv, ra, a.dtype, a.stream);
+}
+
+// Enough for whichever kernels the call's buffers and scale allow.
+int64_t workspace_of(const AttendArgs& a, bool backward) {
+  const int64_t general = attend_general_workspace(a, backward), fast = fast_workspace(a, backward);
+  return general > fast ? general : fast;
+}
+
+// Few rows take the general kernels, which pack a key head's rows into one tile and split its keys.
+int launch(const AttendArgs& a, bool backward) {
+  if (fast_call(a, backward) && (backward || a.t_q >= 64)) return launch_fast(a, backward);
+  return backward ? launch_attend_general_bwd(a) : launch_attend_general_fwd(a);
+}
 
 int check_workspace(const char* name, const AttendArgs& a, bool backward) {
   const int64_t need = workspace_of(a, backward);
@@ -157,7 +230,7 @@ int limn_hip_attend_fwd(const void* q, const void* k, const void* v, const void*
   int rc = check_attend("attend_fwd", a);
   if (rc == LIMN_HIP_OK) rc = check_pointers("attend_fwd", a, false);
   if (rc == LIMN_HIP_OK) rc = check_workspace("attend_fwd", a, false);
-  return rc != LIMN_HIP_OK ? rc : launch_attend_general_fwd(a);
+  return rc != LIMN_HIP_OK ? rc : launch(a, false);
 }
 
 int limn_hip_attend_bwd(const void* q, const void* k, const void* v, const void* slopes, const void* documents, const void* prefix,
@@ -170,7 +243,7 @@ int limn_hip_attend_bwd(const void* q, const void* k, const void* v, const void*
   int rc = check_attend("attend_bwd", a);
   if (rc == LIMN_HIP_OK) rc = check_pointers("attend_bwd", a, true);
   if (rc == LIMN_HIP_OK) rc = check_workspace("attend_bwd", a, true);
-  return rc != LIMN_HIP_OK ? rc : launch_attend_general_bwd(a);
+  return rc != LIMN_HIP_OK ? rc : launch(a, true);
 }
 
 }  // extern "C"

@@ -1,0 +1,43 @@
+// Arguments of the half-width kernels of attention with score rules (attend_mfma.h), of the kernel that finds
+// documents' ranges and of the one that mends blocks with non-finite totals (attend_mend.hip).
+#pragma once
+
+#include "attend_rules.h"
+
+namespace limn {
+
+constexpr int ATT_ROWS = 128;  // resident rows of a workgroup
+
+struct FastArgs {
+  const u16* q;
+  const u16* k;
+  const u16* v;
+  const u16* out;
+  const u16* dout;
+  const float* lse_in;
+  float* delta;
+  const int2* ranges;  // (batch, granules): documents of 32 positions, see attend_ranges; nullptr without
+  u16* o0;             // out / dq / dk
+  u16* o1;             // dv
+  float* lse;
+  int* odd;            // one flag a block of resident rows: its totals were not all finite
+  int64_t batch;
+  int heads, kv_heads, hd, granules;
+  float scale;
+};
+
+int launch_attend_ranges(const RuleArgs& ra, int2* ranges, int64_t batch, int granules, hipStream_t stream);
+int launch_attend_mend_fwd(const FastArgs& g, const RuleArgs& ra, int dtype, hipStream_t stream);
+// blocks of the dQ pass (g.odd) and of the dK/dV pass (kv.odd) that are to be computed again
+int launch_attend_mend_bwd(const FastArgs& g, const FastArgs& kv, const RuleArgs& ra, int dtype, hipStream_t stream);
+
+#define LIMN_ATTEND_PASSES(D)                                                                              \
+  int launch_attend_fwd_##D(const FastArgs& g, const RuleArgs& ra, int dtype, hipStream_t stream);         \
+  int launch_attend_dq_##D(const FastArgs& g, const RuleArgs& ra, int dtype, hipStream_t stream);          \
+  int launch_attend_dkv_##D(const FastArgs& g, const RuleArgs& ra, int dtype, hipStream_t stream);
+LIMN_ATTEND_PASSES(64)
+LIMN_ATTEND_PASSES(96)
+LIMN_ATTEND_PASSES(128)
+#undef LIMN_ATTEND_PASSES
+
+}  // namespace limn

@@ -374,9 +374,6 @@ struct GenBwd {
   float scale;
 };
 
-// log2 of the row's normalizer; infinite for a row that sees nothing, so that its probabilities are 0
-__device__ __forceinline__ float gen_l2(float lse) { return lse == -__builtin_inff() ? __builtin_inff() : lse * ATT_LOG2E; }
-
 // dq of packed rows [row0, row0 + 32), and their delta.
 template <typename T, int DT>
 __device__ __forceinline__ void gen_dq_block(const GenBwd& g, const RuleArgs& ra, const RowMap& map, int64_t b, int kvh, int row0,
@@ -410,7 +407,7 @@ __device__ __forceinline__ void gen_dq_block(const GenBwd& g, const RuleArgs& ra
   for (int dt = 0; dt < DT; dt++) acc[dt] = gen_zero();
   delta = gen_pair_sum(delta);
   if (write_delta && wave == 0 && h == 0 && there) g.delta[first + here] = delta;
-  const float l2 = there ? gen_l2(g.lse[first + here]) : __builtin_inff();
+  const float l2 = there ? att_l2(g.lse[first + here]) : __builtin_inff();
 
   int kend = r.len;
   if (r.causal) kend = min(kend, max(t.pmax + 1, r.pre));
@@ -513,7 +510,7 @@ __device__ __forceinline__ void gen_dkv_block(const GenBwd& g, const RuleArgs& r
     if (gen_none(r, t, key0, kd)) continue;
     const bool whole = gen_whole(r, t, row0 + 32 <= map.rows, key0, kd);
     const int64_t here = row_there ? map.at(row, r.t_q, 1) : 0;
-    const float l2 = row_there ? gen_l2(g.lse[first + here]) : __builtin_inff(), delta = row_there ? g.delta[first + here] : 0.f;
+    const float l2 = row_there ? att_l2(g.lse[first + here]) : __builtin_inff(), delta = row_there ? g.delta[first + here] : 0.f;
     f32x16 s = gen_zero(), dp = gen_zero();
 #pragma unroll
     for (int c = 0; c < CH; c++) {

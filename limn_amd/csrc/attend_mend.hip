@@ -1,0 +1,124 @@
+// Beside the half-width kernels of attention with score rules (attend_mfma.h): the ranges of documents that
+// let them skip tiles, and the blocks that hidden infinities or NaN spoiled, computed again in float.
+
+#include "attend_fast.h"
+#include "attend_general.h"
+
+namespace limn {
+namespace {
+
+// The least and greatest document of each 32 positions, padding and positions past the live keys left out
+// (an empty range if there is nothing else); the sign bit of y: some were left out.
+__global__ __launch_bounds__(256) void attend_ranges(RuleArgs ra, int2* __restrict__ ranges, int64_t batch, int granules) {
+  const int64_t id = blockIdx.x * (int64_t)8 + (threadIdx.x >> 5), b = id / granules;
+  if (b >= batch) return;  // a half wave at a time: the shuffles below stay inside it
+  const int g = (int)(id - b * granules), n = threadIdx.x & 31, p = g * 32 + n;
+  const int len = ra.lengths ? ra.lengths[b] : ra.t_k;
+  int doc = -1;
+  if (p < ra.t_k && p < len) doc = ra.documents[b * ra.t_k + p];
+  int lo = doc < 0 ? 0x7fffffff : doc, hi = doc < 0 ? -1 : doc, none = doc < 0;
+#pragma unroll
+  for (int m = 1; m < 32; m <<= 1) {
+    lo = min(lo, __shfl_xor(lo, m));
+    hi = max(hi, __shfl_xor(hi, m));
+    none |= __shfl_xor(none, m);
+  }
+  // an empty range has hi = 0 and lo above it
+  if (n == 0) ranges[id] = make_int2(lo, (hi < 0 ? 0 : hi) | (none ? (int)0x80000000 : 0));
+}
+
+// The flagged blocks among those of this workgroup (every gridDim.x-th), found 256 flags at a time.
+template <typename F>
+__device__ __forceinline__ void each_odd(const int* odd, int64_t blocks, F f) {
+  for (int64_t first = blockIdx.x; first < blocks; first += (int64_t)gridDim.x * 256) {
+    const int64_t mine = first + (int64_t)threadIdx.x * gridDim.x;
+    if (!__syncthreads_or(mine < blocks && odd[mine] != 0)) continue;
+    for (int j = 0; j < 256; j++) {
+      const int64_t id = first + (int64_t)j * gridDim.x;
+      if (id >= blocks) break;
+      if (odd[id] != 0) f(id);  // the same for every thread
+    }
+  }
+}
+
+template <typename T, int DT>
+__global__ __launch_bounds__(GEN_THREADS, 1) void attend_mend_fwd(FastArgs g, RuleArgs ra, int64_t blocks) {
+  __shared__ float lds[GEN_LDS];
+  const int64_t nqb = (ra.t_q + ATT_ROWS - 1) / ATT_ROWS;
+  each_odd(g.odd, blocks, [&](int64_t id) {
+    const int64_t bh = id / nqb, b = bh / g.heads;
+    const int head = (int)(bh - b * g.heads), q0 = (int)(id - bh * nqb) * ATT_ROWS;
+    const GenFwd gen = {g.q, g.k, g.v, g.o0, g.lse, nullptr, nullptr, g.batch, g.heads, g.kv_heads, g.hd, g.hd, 1, 1};
+    for (int j = 0; j < ATT_ROWS && q0 + j < ra.t_q; j += 32)
+      gen_fwd_block<T, DT>(gen, ra, RowMap{1, head, ra.t_q}, b, head / (g.heads / g.kv_heads), q0 + j, 0, lds);
+  });
+}
+
+template <typename T, int DT>
+__global__ __launch_bounds__(GEN_THREADS, 1) void attend_mend_dq(FastArgs g, RuleArgs ra, int64_t blocks) {
+  __shared__ float lds[GEN_LDS];
+  const int64_t nqb = (ra.t_q + ATT_ROWS - 1) / ATT_ROWS;
+  each_odd(g.odd, blocks, [&](int64_t id) {
+    const int64_t bh = id / nqb, b = bh / g.heads;
+    const int head = (int)(bh - b * g.heads), q0 = (int)(id - bh * nqb) * ATT_ROWS;
+    const GenBwd gen = {g.q, g.k, g.v, g.out, g.dout, g.lse_in, g.delta, g.o0, nullptr, nullptr, g.heads, g.kv_heads, g.hd, g.hd, 1, g.scale};
+    for (int j = 0; j < ATT_ROWS && q0 + j < ra.t_q; j += 32)
+      gen_dq_block<T, DT>(gen, ra, RowMap{1, head, ra.t_q}, b, head / (g.heads / g.kv_heads), q0 + j, false, lds);
+  });
+}
+
+template <typename T, int DT>
+__global__ __launch_bounds__(GEN_THREADS, 1) void attend_mend_dkv(FastArgs g, RuleArgs ra, int64_t blocks) {
+  __shared__ float lds[GEN_LDS];
+  const int64_t nkb = (ra.t_k + ATT_ROWS - 1) / ATT_ROWS;
+  const int group = g.heads / g.kv_heads;
+  each_odd(g.odd, blocks, [&](int64_t id) {
+    const int64_t bk = id / nkb, b = bk / g.kv_heads;
+    const int kvh = (int)(bk - b * g.kv_heads), k0 = (int)(id - bk * nkb) * ATT_ROWS;
+    const GenBwd gen = {g.q, g.k, g.v, g.out, g.dout, g.lse_in, g.delta, nullptr, g.o0, g.o1, g.heads, g.kv_heads, g.hd, g.hd, 1, g.scale};
+    for (int j = 0; j < ATT_ROWS && k0 + j < ra.t_k; j += 32)
+      gen_dkv_block<T, DT>(gen, ra, RowMap{group, kvh * group, group * ra.t_q}, b, kvh, k0 + j, lds);
+  });
+}
+
+constexpr int64_t MEND_GROUPS = 256;
+
+unsigned mend_grid(int64_t blocks) { return (unsigned)(blocks < MEND_GROUPS ? blocks : MEND_GROUPS); }
+
+template <typename T, int DT>
+int mend_fwd(const FastArgs& g, const RuleArgs& ra, hipStream_t stream) {
+  const int64_t blocks = g.batch * g.heads * ((ra.t_q + ATT_ROWS - 1) / ATT_ROWS);
+  hipLaunchKernelGGL((attend_mend_fwd<T, DT>), dim3(mend_grid(blocks)), dim3(GEN_THREADS), 0, stream, g, ra, blocks);
+  return check_hip(hipGetLastError(), "launching attention's mending");
+}
+
+template <typename T, int DT>
+int mend_bwd(const FastArgs& g, const FastArgs& kv, const RuleArgs& ra, hipStream_t stream) {
+  const int64_t blocks = g.batch * g.heads * ((ra.t_q + ATT_ROWS - 1) / ATT_ROWS), kv_blocks = g.batch * g.kv_heads * ((ra.t_k + ATT_ROWS - 1) / ATT_ROWS);
+  hipLaunchKernelGGL((attend_mend_dq<T, DT>), dim3(mend_grid(blocks)), dim3(GEN_THREADS), 0, stream, g, ra, blocks);
+  const int rc = check_hip(hipGetLastError(), "launching attention's mending");
+  if (rc != LIMN_HIP_OK) return rc;
+  hipLaunchKernelGGL((attend_mend_dkv<T, DT>), dim3(mend_grid(kv_blocks)), dim3(GEN_THREADS), 0, stream, kv, ra, kv_blocks);
+  return check_hip(hipGetLastError(), "launching attention's mending");
+}
+
+}  // namespace
+
+int launch_attend_ranges(const RuleArgs& ra, int2* ranges, int64_t batch, int granules, hipStream_t stream) {
+  const int64_t blocks = (batch * granules + 7) / 8;
+  if (blocks > 0x7fffffff) return fail(LIMN_HIP_EUNSUPPORTED, "attend: %lld workgroups exceed one launch", (long long)blocks);
+  hipLaunchKernelGGL(attend_ranges, dim3((unsigned)blocks), dim3(256), 0, stream, ra, ranges, batch, granules);
+  return check_hip(hipGetLastError(), "launching the documents' ranges");
+}
+
+int launch_attend_mend_fwd(const FastArgs& g, const RuleArgs& ra, int dtype, hipStream_t stream) {
+  if (dtype == LIMN_HIP_BFLOAT16) return g.hd <= 64 ? mend_fwd<BF16, 2>(g, ra, stream) : mend_fwd<BF16, 4>(g, ra, stream);
+  return g.hd <= 64 ? mend_fwd<F16, 2>(g, ra, stream) : mend_fwd<F16, 4>(g, ra, stream);
+}
+
+int launch_attend_mend_bwd(const FastArgs& g, const FastArgs& kv, const RuleArgs& ra, int dtype, hipStream_t stream) {
+  if (dtype == LIMN_HIP_BFLOAT16) return g.hd <= 64 ? mend_bwd<BF16, 2>(g, kv, ra, stream) : mend_bwd<BF16, 4>(g, kv, ra, stream);
+  return g.hd <= 64 ? mend_bwd<F16, 2>(g, kv, ra, stream) : mend_bwd<F16, 4>(g, kv, ra, stream);
+}
+
+}  // namespace limn

@@ -11,6 +11,21 @@
 #include "attend.h"
 
 namespace limn {
+
+struct RuleArgs {
+  const float* slopes;
+  const int* documents;
+  const int* prefix;
+  const int* lengths;
+  int t_q, t_k;
+  int causal;
+  float scale, softcap;
+};
+
+inline RuleArgs rule_args(const AttendArgs& a) {
+  return RuleArgs{a.slopes, a.documents, a.prefix, a.lengths, (int)a.t_q, (int)a.t_k, a.causal, (float)a.scale, (float)a.softcap};
+}
+
 namespace {
 
 constexpr float ATT_LOG2E = 1.4426950408889634f, ATT_LN2 = 0.6931471805599453f;
@@ -23,16 +38,6 @@ struct Rules {
   bool causal;
   float c2;              // scale * log2(e)
   float cap_in, cap_out; // 2 log2(e) scale / cap and cap log2(e); cap_out = 0: no cap
-};
-
-struct RuleArgs {
-  const float* slopes;
-  const int* documents;
-  const int* prefix;
-  const int* lengths;
-  int t_q, t_k;
-  int causal;
-  float scale, softcap;
 };
 
 __device__ __forceinline__ Rules rules_of(const RuleArgs& a, int64_t b) {
@@ -64,9 +69,8 @@ __device__ __forceinline__ bool sees(const Rules& r, int p, int key) {
   return ok;
 }
 
-inline RuleArgs rule_args(const AttendArgs& a) {
-  return RuleArgs{a.slopes, a.documents, a.prefix, a.lengths, (int)a.t_q, (int)a.t_k, a.causal, (float)a.scale, (float)a.softcap};
-}
+// log2 of a row's normalizer; infinite for a row that sees nothing, so that its probabilities are 0
+__device__ __forceinline__ float att_l2(float lse) { return lse == -__builtin_inff() ? __builtin_inff() : lse * ATT_LOG2E; }
 
 }  // namespace
 }  // namespace limn

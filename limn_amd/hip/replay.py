@@ -46,7 +46,7 @@ POINTER_ARGS = {
     STEP_XENT_BWD: frozenset(range(7)) | {11},
 }
 
-LAUNCHES = {STEP_SDPA_BWD: 2, STEP_ATTEND_BWD: 2, STEP_XENT_FWD: 3, STEP_XENT_BWD: 5}
+LAUNCHES = {STEP_SDPA_BWD: 2, STEP_ATTEND_FWD: 3, STEP_ATTEND_BWD: 5, STEP_XENT_FWD: 3, STEP_XENT_BWD: 5}
 
 ARG = np.dtype([("value", np.int64), ("slot", np.int32), ("reserved", np.int32)])
 STEP = np.dtype([("kind", np.int32), ("nargs", np.int32), ("first", np.int64), ("function", np.uint64),
@@ -92,8 +92,8 @@ class Program:
     @functools.cached_property
     def launches(self) -> int:
         """Kernel launches of the list, at most: a contraction given a workspace may fold k slices, one of
-        half widths copy its operands as well; attention given a workspace may join parts; LAUNCHES has the
-        kinds of several (a cross entropy's for one piece of the vocabulary)."""
+        half widths copy its operands as well; LAUNCHES has the other kinds of
+        several (a cross entropy's for one piece of the vocabulary)."""
         total = 0
         for kind, first in zip(self.steps["kind"].tolist(), self.steps["first"].tolist()):
             value = lambda k: int(self.args["value"][first + k])
@@ -101,8 +101,6 @@ class Program:
                 total += 1 + (value(19 if kind == STEP_MATMUL else 26) > 0)
             elif kind == STEP_CONTRACT:
                 total += 1 + (value(26) > 0) * (1 if value(3) == 1 else 2)
-            elif kind == STEP_ATTEND_FWD:
-                total += 1 + (value(20) > 0)
             else:
                 total += LAUNCHES.get(kind, 1)
         return total

@@ -14,6 +14,9 @@ step of the storage type (torch.finfo(t).eps / 2) and f that of float32, 2^-24:
   - delta = rowsum(dout * out) takes out as stored: off by u rowsum|dout||out|, and out's own error;
   - a probability below the least normal float32 number, 2^-126, may be 0 (the exponential gives no subnormal
     numbers): it is off by up to that number, which no relative bound covers;
+  - a float16 operand below 2^-14, the least normal one, is off by up to 2^-25 absolutely: the kernels multiply
+    the forward's weights by 2^7 and the dV product's by 2^14 first, so 2^-32 and 2^-39 of a weight; the
+    score gradients are taken as they are, scale apart, so 2^-25;
   - every stored result rounds once more: u times its value, and up to the least number of its type where the
     value is below it (float32 and bfloat16 sums and stores may take subnormal numbers as 0).
 """
@@ -57,6 +60,7 @@ def attend(q, k, v, *, causal=False, softcap=0.0, slopes=None, documents=None, p
     scale = hd**-0.5 if scale is None else scale
     u, least = HALF_STEP[dtype], LEAST[dtype]
     operand = 0.0 if dtype == "float32" else u
+    small = 1.0 if dtype == "float16" else 0.0
     q, k, v = (np.asarray(x, dtype=np.float64) for x in (q, k, v))
     shapes = dict(out=q.shape[:-1] + (hd_v,), lse=q.shape[:-1], dq=q.shape, dk=k.shape, dv=v.shape)
     got = {n: np.zeros(s) for n, s in shapes.items()}
@@ -89,7 +93,7 @@ def attend(q, k, v, *, causal=False, softcap=0.0, slopes=None, documents=None, p
                 n = seen.sum(1, keepdims=True)
                 rel = 2 * np.max(np.where(seen, e, 0.0), axis=1, keepdims=True) + (n + 16) * F
                 got["out"][b, h] = _product(p, V)
-                off["out"][b, h] = (rel + operand) * (p @ fine(V)) + TINY * (seen @ fine(V)) + u * fine(got["out"][b, h]) + least
+                off["out"][b, h] = (rel + operand) * (p @ fine(V)) + (TINY + small * 2.0**-32) * (seen @ fine(V)) + u * fine(got["out"][b, h]) + least
                 got["lse"][b, h] = np.where(total == 0, -np.inf, base + np.log(total))[:, 0]
                 off["lse"][b, h] = rel[:, 0] + 4 * F * fine(got["lse"][b, h])
                 if dout is None:
@@ -102,7 +106,7 @@ def attend(q, k, v, *, causal=False, softcap=0.0, slopes=None, documents=None, p
                 ddp = (hd_v + 8) * F * (fine(G) @ fine(V).T)
                 ds = np.where(seen, p * (dp - delta) * scale * bent, 0.0)
                 size = np.where(seen, p * abs(scale) * bent, 0.0)
-                dds = np.abs(ds) * (rel + 8 * F + operand) + size * (ddelta + ddp) + np.where(seen, TINY * (1 + fine(dp - delta) * abs(scale)), 0.0)
+                dds = np.abs(ds) * (rel + 8 * F + operand) + size * (ddelta + ddp) + np.where(seen, TINY * (1 + fine(dp - delta) * abs(scale)) + small * 2.0**-25 * abs(scale), 0.0)
                 if softcap:  # 1 - tanh^2, off by twice the tanh's own 4 f and by the score's
                     dds = dds + np.where(seen, np.abs(p * (dp - delta)) * abs(scale), 0.0) * (16 * F + 2 * e / softcap)
                 kv = h // group
@@ -112,7 +116,7 @@ def attend(q, k, v, *, causal=False, softcap=0.0, slopes=None, documents=None, p
                 got["dk"][b, kv] += _product(ds.T, Q)
                 off["dk"][b, kv] += dds.T @ fine(Q) + (m + 8) * F * (np.abs(ds).T @ fine(Q))
                 got["dv"][b, kv] += _product(p.T, G)
-                off["dv"][b, kv] += (p * (rel + operand) + TINY * seen).T @ fine(G) + (m + 8) * F * (p.T @ fine(G))
+                off["dv"][b, kv] += (p * (rel + operand) + (TINY + small * 2.0**-39) * seen).T @ fine(G) + (m + 8) * F * (p.T @ fine(G))
     for name in ("dk", "dv"):
         off[name] += u * fine(got[name]) + least
     names = ("out", "lse") if dout is None else ("out", "lse", "dq", "dk", "dv")
