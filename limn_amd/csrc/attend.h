@@ -37,9 +37,14 @@ int64_t attend_general_workspace(const AttendArgs& a, bool backward);
 int launch_attend_general_fwd(const AttendArgs& a);
 int launch_attend_general_bwd(const AttendArgs& a);
 
-// Joins `splits` partial results of `rows` packed rows: totals (splits, rows, hd_v) float, then stats
-// (splits, rows, 2) float (reference point of the exponentials in log2, sum), into out and lse.
-int launch_attend_join(const AttendArgs& a, const float* totals, const float* stats, int64_t splits);
+// Joins `splits` partial results of `rows` packed rows: totals (splits, rows, hd_v) float, and stats
+// (splits, rows, 2) float (reference point of the exponentials in log2, sum), into out and lse; sums and totals
+// are 2^up times the weights'. A split that has seen nothing is not read.
+int launch_attend_join(const AttendArgs& a, const float* totals, const float* stats, int64_t splits, float up);
+
+// Few queries against a cache, half widths (attend_token.hip).
+int64_t attend_token_workspace(const AttendArgs& a);
+int launch_attend_token(const AttendArgs& a);
 
 // bytes rounded up to where the next part of a workspace may start
 constexpr int64_t attend_align(int64_t bytes) { return (bytes + 255) / 256 * 256; }

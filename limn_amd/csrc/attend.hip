@@ -17,11 +17,12 @@ int attend_general_bwd_bf16(const AttendArgs& a);
 namespace {
 
 // One wave per packed row: the splits' reference points brought to the largest, their sums and totals added
-// in split order, so that the result does not depend on which workgroup ended first.
+// in split order, so that the result does not depend on which workgroup ended first. A split that saw nothing
+// (no reference point, and a sum of 0 that is added all the same: it is NaN where a score was) is not read.
 template <typename T>
 __global__ __launch_bounds__(64) void attend_join(const float* __restrict__ totals, const float* __restrict__ stats,
                                                   typename T::Storage* __restrict__ out, float* __restrict__ lse, int64_t rows_all,
-                                                  int splits, int group, int kv_heads, int t_q, int hd_v) {
+                                                  int splits, int group, int t_q, int hd_v, float up) {
   const int64_t row = blockIdx.x;
   const int64_t per = (int64_t)group * t_q, bk = row / per, r = row % per;
   float top = -__builtin_inff(), total = 0.f;
@@ -37,20 +38,21 @@ __global__ __launch_bounds__(64) void attend_join(const float* __restrict__ tota
   for (int d = threadIdx.x; d < hd_v; d += 64) {
     float x = 0.f;
     for (int s = 0; s < splits; s++) {
-      const float m = stats[(s * rows_all + row) * 2];
-      x += totals[(s * rows_all + row) * hd_v + d] * (m == -__builtin_inff() ? 1.f : fast_exp2(m - base));
+      const float* st = stats + (s * rows_all + row) * 2;
+      if (st[0] == -__builtin_inff() && st[1] == 0.f) continue;
+      x += totals[(s * rows_all + row) * hd_v + d] * (st[0] == -__builtin_inff() ? 1.f : fast_exp2(st[0] - base));
     }
     T::store(out + at * hd_v, d, total == 0.f ? 0.f : x * inv);
   }
-  if (threadIdx.x == 0) lse[at] = total == 0.f ? -__builtin_inff() : base * ATT_LN2 + logf(total);
+  if (threadIdx.x == 0) lse[at] = total == 0.f ? -__builtin_inff() : (base - up) * ATT_LN2 + logf(total);
 }
 
 template <typename T>
-int join(const AttendArgs& a, const float* totals, const float* stats, int64_t splits) {
+int join(const AttendArgs& a, const float* totals, const float* stats, int64_t splits, float up) {
   const int64_t rows_all = a.batch * a.heads * a.t_q;
   if (rows_all > 0x7fffffff) return fail(LIMN_HIP_EUNSUPPORTED, "attend: %lld rows exceed one launch", (long long)rows_all);
   hipLaunchKernelGGL((attend_join<T>), dim3((unsigned)rows_all), dim3(64), 0, a.stream, totals, stats, (typename T::Storage*)a.o0, (float*)a.o1,
-                     rows_all, (int)splits, (int)a.group(), (int)a.kv_heads, (int)a.t_q, (int)a.hd_v);
+                     rows_all, (int)splits, (int)a.group(), (int)a.t_q, (int)a.hd_v, up);
   return check_hip(hipGetLastError(), "joining attention's splits");
 }
 
@@ -108,18 +110,23 @@ int64_t granules_of(const AttendArgs& a) { return (a.t_k + 31) / 32; }
 int64_t row_blocks(const AttendArgs& a) { return a.batch * a.heads * ((a.t_q + ATT_ROWS - 1) / ATT_ROWS); }
 int64_t key_blocks(const AttendArgs& a) { return a.batch * a.kv_heads * ((a.t_k + ATT_ROWS - 1) / ATT_ROWS); }
 
-// Sizes the half-width kernels serve: 16-byte rows, a head's rows within 32-bit byte offsets, few enough
-// streamed tiles for a block's list of them.
-bool fast_sizes(const AttendArgs& a) {
-  return a.dtype != LIMN_HIP_FLOAT32 && a.hd == a.hd_v && a.hd % 8 == 0 && a.hd <= 128 && a.t_q <= (1 << 17) && a.t_k <= (1 << 17);
+// Sizes the half-width kernels serve: 16-byte rows; the tiled ones also need a head's rows within 32-bit byte
+// offsets and few enough streamed tiles for a block's list of them.
+bool half_sizes(const AttendArgs& a) { return a.dtype != LIMN_HIP_FLOAT32 && a.hd == a.hd_v && a.hd % 8 == 0 && a.hd <= 128; }
+bool fast_sizes(const AttendArgs& a) { return half_sizes(a) && a.t_q <= (1 << 17) && a.t_k <= (1 << 17); }
+
+bool aligned16(const AttendArgs& a, bool backward) {
+  const uintptr_t at = (uintptr_t)a.q | (uintptr_t)a.k | (uintptr_t)a.v | (uintptr_t)a.o0 | (backward ? (uintptr_t)a.o1 | (uintptr_t)a.o2 | (uintptr_t)a.out | (uintptr_t)a.dout : 0);
+  return at % 16 == 0;
 }
+
+// Forward calls of fewer queries than half a tiled block's 128 rows share their keys' bytes between the heads of a group
+// and split long caches (attend_token.hip).
+bool token_sizes(const AttendArgs& a) { return half_sizes(a) && a.t_q < 64; }
 
 // A call of such sizes goes to them where every buffer is 16-byte aligned and the scale positive (the forward's
 // reference point is taken over unscaled scores).
-bool fast_call(const AttendArgs& a, bool backward) {
-  const uintptr_t at = (uintptr_t)a.q | (uintptr_t)a.k | (uintptr_t)a.v | (uintptr_t)a.o0 | (backward ? (uintptr_t)a.o1 | (uintptr_t)a.o2 | (uintptr_t)a.out | (uintptr_t)a.dout : 0);
-  return fast_sizes(a) && a.scale > 0 && at % 16 == 0;
-}
+bool fast_call(const AttendArgs& a, bool backward) { return fast_sizes(a) && a.scale > 0 && aligned16(a, backward); }
 
 // flags of the blocks, the documents' ranges, and for the backward delta
 int64_t fast_workspace(const AttendArgs& a, bool backward) {
@@ -165,14 +172,16 @@ int launch_fast(const AttendArgs& a, bool backward) {
   return rc != LIMN_HIP_OK || !mend ? rc : launch_attend_mend_bwd(g, kv, ra, a.dtype, a.stream);
 }
 
-// Enough for whichever kernels the call's buffers and scale allow.
+// Enough for whichever kernels the call's buffers, rules and scale allow.
 int64_t workspace_of(const AttendArgs& a, bool backward) {
-  const int64_t general = attend_general_workspace(a, backward), fast = fast_workspace(a, backward);
-  return general > fast ? general : fast;
+  int64_t need = attend_general_workspace(a, backward);
+  const int64_t fast = fast_workspace(a, backward), token = !backward && token_sizes(a) ? attend_token_workspace(a) : 0;
+  if (fast > need) need = fast;
+  return token > need ? token : need;
 }
 
-// Few rows take the general kernels, which pack a key head's rows into one tile and split its keys.
 int launch(const AttendArgs& a, bool backward) {
+  if (!backward && token_sizes(a) && a.documents == nullptr && aligned16(a, false)) return launch_attend_token(a);
   if (fast_call(a, backward) && (backward || a.t_q >= 64)) return launch_fast(a, backward);
   return backward ? launch_attend_general_bwd(a) : launch_attend_general_fwd(a);
 }
@@ -186,9 +195,9 @@ int check_workspace(const char* name, const AttendArgs& a, bool backward) {
 
 }  // namespace
 
-int launch_attend_join(const AttendArgs& a, const float* totals, const float* stats, int64_t splits) {
-  if (a.dtype == LIMN_HIP_FLOAT32) return join<F32>(a, totals, stats, splits);
-  return a.dtype == LIMN_HIP_FLOAT16 ? join<F16>(a, totals, stats, splits) : join<BF16>(a, totals, stats, splits);
+int launch_attend_join(const AttendArgs& a, const float* totals, const float* stats, int64_t splits, float up) {
+  if (a.dtype == LIMN_HIP_FLOAT32) return join<F32>(a, totals, stats, splits, up);
+  return a.dtype == LIMN_HIP_FLOAT16 ? join<F16>(a, totals, stats, splits, up) : join<BF16>(a, totals, stats, splits, up);
 }
 
 int64_t attend_general_workspace(const AttendArgs& a, bool backward) {

@@ -30,6 +30,8 @@ int launch_attend_ranges(const RuleArgs& ra, int2* ranges, int64_t batch, int gr
 int launch_attend_mend_fwd(const FastArgs& g, const RuleArgs& ra, int dtype, hipStream_t stream);
 // blocks of the dQ pass (g.odd) and of the dK/dV pass (kv.odd) that are to be computed again
 int launch_attend_mend_bwd(const FastArgs& g, const FastArgs& kv, const RuleArgs& ra, int dtype, hipStream_t stream);
+// the packed rows of a forward call whose results are not all finite
+int launch_attend_mend_rows(const AttendArgs& a);
 
 #define LIMN_ATTEND_PASSES(D)                                                                              \
   int launch_attend_fwd_##D(const FastArgs& g, const RuleArgs& ra, int dtype, hipStream_t stream);         \

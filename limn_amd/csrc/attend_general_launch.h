@@ -64,7 +64,7 @@ int launch_gen_fwd(const AttendArgs& a, int64_t splits) {
   GenFwd g = {a.q, a.k, a.v, a.o0, (float*)a.o1, totals, stats, a.batch, (int)a.heads, (int)a.kv_heads, (int)a.hd, (int)a.hd_v, vec, (int)splits};
   hipLaunchKernelGGL((attend_general_fwd<T, DT>), dim3((unsigned)blocks), dim3(GEN_THREADS), 0, a.stream, g, rule_args(a));
   const int rc = check_hip(hipGetLastError(), "launching attention");
-  return rc != LIMN_HIP_OK || splits == 1 ? rc : launch_attend_join(a, totals, stats, splits);
+  return rc != LIMN_HIP_OK || splits == 1 ? rc : launch_attend_join(a, totals, stats, splits, 0.f);
 }
 
 template <typename T, int DT>

@@ -81,6 +81,24 @@ __global__ __launch_bounds__(GEN_THREADS, 1) void attend_mend_dkv(FastArgs g, Ru
   });
 }
 
+// The forward's tiles of 32 packed rows, each computed again if one of its results is not finite.
+template <typename T, int DT>
+__global__ __launch_bounds__(GEN_THREADS, 1) void attend_mend_rows(GenFwd g, RuleArgs ra, int64_t tiles, int row_tiles) {
+  __shared__ float lds[GEN_LDS];
+  const int group = g.heads / g.kv_heads, rows = group * ra.t_q;
+  for (int64_t id = blockIdx.x; id < tiles; id += gridDim.x) {
+    const int64_t bk = id / row_tiles, b = bk / g.kv_heads;
+    const int kvh = (int)(bk - b * g.kv_heads), row0 = (int)(id - bk * row_tiles) * 32;
+    const RowMap map = {group, kvh * group, rows};
+    bool odd = false;
+    for (int i = threadIdx.x; i < 32 * g.hd_v; i += GEN_THREADS) {
+      const int row = row0 + i / g.hd_v;
+      if (row < rows) odd |= !gen_finite(T::load((const u16*)g.out + b * g.heads * (int64_t)ra.t_q * g.hd_v + map.at(row, ra.t_q, g.hd_v), i % g.hd_v));
+    }
+    if (__syncthreads_or(odd)) gen_fwd_block<T, DT>(g, ra, map, b, kvh, row0, 0, lds);
+  }
+}
+
 constexpr int64_t MEND_GROUPS = 256;
 
 unsigned mend_grid(int64_t blocks) { return (unsigned)(blocks < MEND_GROUPS ? blocks : MEND_GROUPS); }
@@ -102,7 +120,20 @@ int mend_bwd(const FastArgs& g, const FastArgs& kv, const RuleArgs& ra, hipStrea
   return check_hip(hipGetLastError(), "launching attention's mending");
 }
 
+template <typename T, int DT>
+int mend_rows(const AttendArgs& a) {
+  const int64_t row_tiles = (a.group() * a.t_q + 31) / 32, tiles = a.batch * a.kv_heads * row_tiles;
+  const GenFwd g = {a.q, a.k, a.v, a.o0, (float*)a.o1, nullptr, nullptr, a.batch, (int)a.heads, (int)a.kv_heads, (int)a.hd, (int)a.hd_v, 1, 1};
+  hipLaunchKernelGGL((attend_mend_rows<T, DT>), dim3((unsigned)(tiles < 1024 ? tiles : 1024)), dim3(GEN_THREADS), 0, a.stream, g, rule_args(a), tiles, (int)row_tiles);
+  return check_hip(hipGetLastError(), "launching attention's mending");
+}
+
 }  // namespace
+
+int launch_attend_mend_rows(const AttendArgs& a) {
+  if (a.dtype == LIMN_HIP_BFLOAT16) return a.hd <= 64 ? mend_rows<BF16, 2>(a) : mend_rows<BF16, 4>(a);
+  return a.hd <= 64 ? mend_rows<F16, 2>(a) : mend_rows<F16, 4>(a);
+}
 
 int launch_attend_ranges(const RuleArgs& ra, int2* ranges, int64_t batch, int granules, hipStream_t stream) {
   const int64_t blocks = (batch * granules + 7) / 8;

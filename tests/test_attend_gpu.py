@@ -191,6 +191,20 @@ def test_tokens_against_a_cache(hipdev, dtype, heads, kv_heads, t_q, t_k, dim, l
         within(lse, *want["lse"], "lse")
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("bad", [np.nan, np.inf])
+def test_a_key_some_queries_do_not_see(hipdev, dtype, bad):
+    """The newest keys of several queries hold `bad`: the queries before them stay as they are, in a short cache and a long one."""
+    for t_k, length in ((90, 80), (3000, 2999)):
+        rng, (q, k, v, _) = draw(t_k, dtype, 1, 4, 2, 5, t_k, 64, 64)
+        v[0, 0, length - 2, 3] = bad  # seen by the last two queries
+        v[0, 1, length - 1, 60] = -bad  # by the last
+        out, lse = served(hipdev, q, k, v, dtype, dict(lengths=np.array([length], np.int32)), causal=True)
+        want = definition(q, k, v, dtype=dtype, causal=True, lengths=np.array([length], np.int32))
+        within(out, *want["out"], "out")
+        within(lse, *want["lse"], "lse")
+
+
 def test_a_call_gives_the_same_bits_again(hipdev):
     rng, (q, k, v, do) = draw(3, "bfloat16", 2, 8, 2, 333, 333, 128, 128)
     rules = dict(documents=packed(rng, 2, 333, 80))
