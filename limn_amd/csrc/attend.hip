@@ -16,42 +16,74 @@ int attend_general_bwd_bf16(const AttendArgs& a);
 
 namespace {
 
-// One wave per packed row: the splits' reference points brought to the largest, their sums and totals added
-// in split order, so that the result does not depend on which workgroup ended first. A split that saw nothing
-// (no reference point, and a sum of 0 that is added all the same: it is NaN where a score was) is not read.
+constexpr int JOIN_MOST = 1024;  // splits of a call: both planners stay at or below
+
+// A workgroup per packed row: the splits' reference points brought to the largest, their sums and totals added
+// in a fixed order (each wave a run of splits, then the waves), so that the result does not depend on which
+// workgroup ended first. A split that saw nothing (no reference point, and a sum of 0: it is NaN where a score
+// was) is not read. The factors are found first, a split a thread, so that the loads of the totals do not
+// wait for one another: 60 splits of 64 rows took 60 us with one wave that walked them in turn, 5 so.
 template <typename T>
-__global__ __launch_bounds__(64) void attend_join(const float* __restrict__ totals, const float* __restrict__ stats,
-                                                  typename T::Storage* __restrict__ out, float* __restrict__ lse, int64_t rows_all,
-                                                  int splits, int group, int t_q, int hd_v, float up) {
+__global__ __launch_bounds__(256) void attend_join(const float* __restrict__ totals, const float* __restrict__ stats,
+                                                   typename T::Storage* __restrict__ out, float* __restrict__ lse, int64_t rows_all,
+                                                   int splits, int group, int t_q, int hd_v, float up) {
+  __shared__ float factor[JOIN_MOST], part[4][256], sums[256];
   const int64_t row = blockIdx.x;
   const int64_t per = (int64_t)group * t_q, bk = row / per, r = row % per;
-  float top = -__builtin_inff(), total = 0.f;
-  for (int s = 0; s < splits; s++) top = fmaxf(top, stats[(s * rows_all + row) * 2]);
-  const float base = top == -__builtin_inff() ? 0.f : top;
-  for (int s = 0; s < splits; s++) {
-    const float* st = stats + (s * rows_all + row) * 2;
-    total += st[0] == -__builtin_inff() ? st[1] : st[1] * fast_exp2(st[0] - base);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  float top = -__builtin_inff();
+  for (int s = threadIdx.x; s < splits; s += 256) top = fmaxf(top, stats[(s * rows_all + row) * 2]);
+  sums[threadIdx.x] = top;
+  __syncthreads();
+  for (int h = 128; h > 0; h >>= 1) {
+    if (threadIdx.x < h) sums[threadIdx.x] = fmaxf(sums[threadIdx.x], sums[threadIdx.x + h]);
+    __syncthreads();
   }
+  top = sums[0];
+  __syncthreads();
+  const float base = top == -__builtin_inff() ? 0.f : top;
+  float total = 0.f;
+  for (int s = threadIdx.x; s < splits; s += 256) {
+    const float m = stats[(s * rows_all + row) * 2], l = stats[(s * rows_all + row) * 2 + 1];
+    const float f = m == -__builtin_inff() ? (l == 0.f ? 0.f : 1.f) : fast_exp2(m - base);
+    factor[s] = m == -__builtin_inff() && l == 0.f ? -1.f : f;  // -1: not read
+    total += l * f;
+  }
+  sums[threadIdx.x] = total;
+  __syncthreads();
+  for (int h = 128; h > 0; h >>= 1) {
+    if (threadIdx.x < h) sums[threadIdx.x] += sums[threadIdx.x + h];
+    __syncthreads();
+  }
+  total = sums[0];
+  const int run = (splits + 3) / 4, s1 = min(splits, (wave + 1) * run);
+#pragma unroll
+  for (int c = 0; c < 4; c++) {
+    const int d = c * 64 + lane;
+    float x = 0.f;
+    if (d < hd_v) {
+#pragma unroll 8
+      for (int s = wave * run; s < s1; s++) {
+        const float f = factor[s];
+        x += f < 0.f ? 0.f : f * totals[(s * rows_all + row) * hd_v + d];
+      }
+    }
+    part[wave][d] = x;
+  }
+  __syncthreads();
   // bk = b * kv_heads + kvh; head kvh * group + r % group of sequence b
   const int64_t at = (bk * group + r % group) * t_q + r / group;
   const float inv = total == 0.f ? 0.f : 1.f / total;
-  for (int d = threadIdx.x; d < hd_v; d += 64) {
-    float x = 0.f;
-    for (int s = 0; s < splits; s++) {
-      const float* st = stats + (s * rows_all + row) * 2;
-      if (st[0] == -__builtin_inff() && st[1] == 0.f) continue;
-      x += totals[(s * rows_all + row) * hd_v + d] * (st[0] == -__builtin_inff() ? 1.f : fast_exp2(st[0] - base));
-    }
-    T::store(out + at * hd_v, d, total == 0.f ? 0.f : x * inv);
-  }
+  const int d = threadIdx.x;
+  if (d < hd_v) T::store(out + at * hd_v, d, total == 0.f ? 0.f : ((part[0][d] + part[1][d]) + (part[2][d] + part[3][d])) * inv);
   if (threadIdx.x == 0) lse[at] = total == 0.f ? -__builtin_inff() : (base - up) * ATT_LN2 + logf(total);
 }
 
 template <typename T>
 int join(const AttendArgs& a, const float* totals, const float* stats, int64_t splits, float up) {
   const int64_t rows_all = a.batch * a.heads * a.t_q;
-  if (rows_all > 0x7fffffff) return fail(LIMN_HIP_EUNSUPPORTED, "attend: %lld rows exceed one launch", (long long)rows_all);
-  hipLaunchKernelGGL((attend_join<T>), dim3((unsigned)rows_all), dim3(64), 0, a.stream, totals, stats, (typename T::Storage*)a.o0, (float*)a.o1,
+  if (rows_all > 0x7fffffff || splits > JOIN_MOST) return fail(LIMN_HIP_EUNSUPPORTED, "attend: %lld rows exceed one launch", (long long)rows_all);
+  hipLaunchKernelGGL((attend_join<T>), dim3((unsigned)rows_all), dim3(256), 0, a.stream, totals, stats, (typename T::Storage*)a.o0, (float*)a.o1,
                      rows_all, (int)splits, (int)a.group(), (int)a.t_q, (int)a.hd_v, up);
   return check_hip(hipGetLastError(), "joining attention's splits");
 }
