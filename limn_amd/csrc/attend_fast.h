@@ -23,6 +23,7 @@ struct FastArgs {
   int* odd;            // one flag a block of resident rows: its totals were not all finite
   int64_t batch;
   int heads, kv_heads, hd, granules;
+  int head_group;      // see att_head_and_block
   float scale;
 };
 

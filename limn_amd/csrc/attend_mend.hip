@@ -8,7 +8,7 @@ namespace limn {
 namespace {
 
 // The least and greatest document of each 32 positions, padding and positions past the live keys left out
-// (an empty range if there is nothing else); the sign bit of y: some were left out.
+// (0x7fffffff and 0, an empty range, if there is nothing else).
 __global__ __launch_bounds__(256) void attend_ranges(RuleArgs ra, int2* __restrict__ ranges, int64_t batch, int granules) {
   const int64_t id = blockIdx.x * (int64_t)8 + (threadIdx.x >> 5), b = id / granules;
   if (b >= batch) return;  // a half wave at a time: the shuffles below stay inside it
@@ -16,15 +16,13 @@ __global__ __launch_bounds__(256) void attend_ranges(RuleArgs ra, int2* __restri
   const int len = ra.lengths ? ra.lengths[b] : ra.t_k;
   int doc = -1;
   if (p < ra.t_k && p < len) doc = ra.documents[b * ra.t_k + p];
-  int lo = doc < 0 ? 0x7fffffff : doc, hi = doc < 0 ? -1 : doc, none = doc < 0;
+  int lo = doc < 0 ? 0x7fffffff : doc, hi = doc < 0 ? 0 : doc;
 #pragma unroll
   for (int m = 1; m < 32; m <<= 1) {
     lo = min(lo, __shfl_xor(lo, m));
     hi = max(hi, __shfl_xor(hi, m));
-    none |= __shfl_xor(none, m);
   }
-  // an empty range has hi = 0 and lo above it
-  if (n == 0) ranges[id] = make_int2(lo, (hi < 0 ? 0 : hi) | (none ? (int)0x80000000 : 0));
+  if (n == 0) ranges[id] = make_int2(lo, hi);
 }
 
 // The flagged blocks among those of this workgroup (every gridDim.x-th), found 256 flags at a time.

@@ -29,47 +29,92 @@ namespace limn {
 namespace {
 
 constexpr int ATT_WORDS = 32;      // 64-tile words of the visit list: 131072 streamed rows
-constexpr int ATT_MOST_DOC_KEYS = ATT_WORDS * 64 * TILE;
+
+// ---- which head and block a workgroup takes ----------------------------------------------------------------
+
+// Workgroup id runs on XCD id % 8. Heads go to XCDs in groups of `group` (so that what a group's blocks stream
+// stays in one L2, see head_and_block in sdpa_mfma.h), group j to XCD j % 8: where documents or lengths differ, so
+// does the work of sequences, and an XCD that had all heads of one sequence (8 sequences, 8 XCDs) left the
+// others waiting: packed documents, forward, 8 x 16 heads x 4096 rows: 600 us so, 444 spread. The grid is
+// padded to whole groups; workgroups past the heads have nothing (false). group 0: heads in turn.
+__device__ __forceinline__ bool att_head_and_block(int64_t heads, int64_t nblocks, int group, int64_t& b, int64_t& blk) {
+  if (group == 0) {
+    b = blockIdx.x % heads;
+    blk = blockIdx.x / heads;
+    return true;
+  }
+  const int64_t slot = blockIdx.x / 8, per = group * nblocks, j = slot / per * 8 + blockIdx.x % 8, r = slot % per;
+  b = j * group + r % group;
+  blk = r / group;
+  return b < heads;
+}
+
+inline int64_t att_grid(int64_t heads, int64_t nblocks, int group) {
+  return group == 0 ? heads * nblocks : (heads + 8 * group - 1) / (8 * group) * 8 * group * nblocks;
+}
 
 // ---- documents: ranges, visit lists ---------------------------------------------------------------------
 
 struct DocRange {
   int lo, hi;
-  bool part;  // some positions have no document
   __device__ __forceinline__ bool meets(const DocRange& o) const { return lo <= hi && o.lo <= o.hi && lo <= o.hi && o.lo <= hi; }
-  __device__ __forceinline__ bool is(int doc) const { return !part && lo == doc && hi == doc; }
 };
 
 // positions [p0, p1], which may reach outside [0, 32 granules)
 __device__ __forceinline__ DocRange doc_range(const int2* ranges, int granules, int p0, int p1) {
-  DocRange r = {0x7fffffff, 0, p0 < 0 || p1 >= granules * 32};
+  DocRange r = {0x7fffffff, 0};
   const int g0 = max(p0, 0) >> 5, g1 = min(p1 >> 5, granules - 1);
   for (int g = g0; g <= g1; g++) {
     const int2 e = ranges[g];
     r.lo = min(r.lo, e.x);
-    r.hi = max(r.hi, e.y & 0x7fffffff);
-    r.part |= e.y < 0;
+    r.hi = max(r.hi, e.y);
   }
   return r;
 }
 
-// The streamed tiles a block visits, in order: [from, to), or those with a bit set.
+// The streamed tiles a block visits, in order from a first one on: every tile before `to`, or those with a bit
+// set in LDS, 64 tiles a word. The word at hand stays in scalar registers: the next tile is a count of its
+// trailing zeros, and LDS is read once in 64 tiles.
 struct Visit {
-  int to;
-  const uint64_t* bits;  // LDS, or nullptr: every tile
-  __device__ __forceinline__ int next(int t) const {
-    if (bits == nullptr || t >= to) return t;
-    int w = t >> 6;
-    uint64_t m = bits[w] >> (t & 63);
-    while (m == 0) {
-      if (++w * 64 >= to) return to;
-      t = w * 64;
-      m = bits[w];
+  int to, at;            // at: the next tile to look at (without bits), or its word's first tile
+  const uint64_t* bits;  // or nullptr
+  uint64_t word;
+  __device__ __forceinline__ void start(int first) {
+    at = first;
+    if (bits != nullptr) {
+      at = first & ~63;
+      word = at < to ? fetch() & (~0ull << (first & 63)) : 0;
     }
-    t += __builtin_ctzll(m);
-    return __builtin_amdgcn_readfirstlane(t < to ? t : to);
+  }
+  __device__ __forceinline__ uint64_t fetch() const {
+    const uint64_t w = bits[at >> 6];
+    return ((uint64_t)(unsigned)__builtin_amdgcn_readfirstlane((int)(w >> 32)) << 32) | (unsigned)__builtin_amdgcn_readfirstlane((int)w);
+  }
+  // the next tile, or `to` behind the last
+  __device__ __forceinline__ int next() {
+    if (bits == nullptr) return at < to ? at++ : to;
+    while (word == 0) {
+      if ((at += 64) >= to) {
+        at = to;  // stays there: a word past the end is never read
+        return to;
+      }
+      word = fetch();
+    }
+    const int t = at + __builtin_ctzll(word);
+    word &= word - 1;
+    return t;
   }
 };
+
+// A tile's documents go through LDS with its rows, and for each half of 32 the document of all of them, or
+// -2 where they differ. Lane l of one wave holds position l's.
+__device__ __forceinline__ void store_docs(int doc, int* docs, int* same) {
+  const int lane = threadIdx.x & 63;
+  docs[lane] = doc;
+  const int lo = __builtin_amdgcn_readlane(doc, 0), hi = __builtin_amdgcn_readlane(doc, 32);
+  const uint64_t eq = __ballot(doc == (lane < 32 ? lo : hi));
+  if (lane < 2) same[lane] = lane == 0 ? ((unsigned)eq == ~0u ? lo : -2) : ((unsigned)(eq >> 32) == ~0u ? hi : -2);
+}
 
 // ---- rows of hd elements in tiles of D ------------------------------------------------------------------
 
@@ -188,12 +233,13 @@ __global__ __launch_bounds__(THREADS, 2) void attend_fwd_mfma(FastArgs g, RuleAr
   constexpr float UP = shift_of<T>(7.f);
   __shared__ __attribute__((aligned(16))) u16 tiles[4 * TE];
   __shared__ __attribute__((aligned(16))) int kdocs[2][TILE];
+  __shared__ int same[2][2];
   __shared__ uint64_t bits[ATT_WORDS];
 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5, n = lane & 31;
   const int64_t nqb = (ra.t_q + ATT_ROWS - 1) / ATT_ROWS;
   int64_t bh, blk;
-  head_and_block(g.batch * g.heads, nqb, bh, blk);
+  if (!att_head_and_block(g.batch * g.heads, nqb, g.head_group, bh, blk)) return;
   const int64_t b = bh / g.heads;
   const int head = (int)(bh - b * g.heads), kvh = head / (g.heads / g.kv_heads);
   const int q0 = (int)(nqb - 1 - blk) * ATT_ROWS, wq0 = q0 + wave * 32, row = wq0 + n;  // causal: the longest rows go first
@@ -218,7 +264,7 @@ __global__ __launch_bounds__(THREADS, 2) void attend_fwd_mfma(FastArgs g, RuleAr
   const int last = min(q0 + ATT_ROWS, r.t_q) - 1;  // the block's last query
   int kend = r.len;
   if (r.causal) kend = min(kend, max(r.off + last + 1, r.pre));
-  Visit visit = {kend > 0 ? (kend + TILE - 1) / TILE : 0, nullptr};
+  Visit visit = {kend > 0 ? (kend + TILE - 1) / TILE : 0, 0, nullptr, 0};
   const int2* ranges = g.ranges ? g.ranges + b * g.granules : nullptr;
   int wave_doc = 0;  // the document of every row of the wave, or -1
   if (ranges != nullptr) {
@@ -237,13 +283,14 @@ __global__ __launch_bounds__(THREADS, 2) void attend_fwd_mfma(FastArgs g, RuleAr
 
   HeadStage<D> st;
   int dnext = 0;
-  int cur = visit.next(0), nxt = cur < visit.to ? visit.next(cur + 1) : visit.to;
+  visit.start(0);
+  int cur = visit.next(), nxt = visit.next();
   auto docs_load = [&](int t) { return ranges != nullptr && threadIdx.x < TILE && t * TILE + (int)threadIdx.x < r.len ? r.docs[t * TILE + threadIdx.x] : -1; };
   if (cur < visit.to) {
     st.load(krows, vrows, cur * TILE);
     dnext = docs_load(cur);
     st.store(tiles, tiles + TE);
-    if (threadIdx.x < TILE) kdocs[0][threadIdx.x] = dnext;
+    if (ranges != nullptr && wave == 0) store_docs(dnext, kdocs[0], same[0]);
     if (nxt < visit.to) {
       st.load(krows, vrows, nxt * TILE);
       dnext = docs_load(nxt);
@@ -272,10 +319,7 @@ __global__ __launch_bounds__(THREADS, 2) void attend_fwd_mfma(FastArgs g, RuleAr
         }
       }
       bool edge = s0 + 32 > r.len || (r.causal && s0 + 31 > r.off + wq0 && s0 + 31 >= r.pre);
-      if (ranges != nullptr && !edge) {
-        const int2 e = ranges[s0 >> 5];
-        edge = wave_doc < 0 || e.x != wave_doc || e.y != wave_doc;
-      }
+      if (ranges != nullptr) edge |= wave_doc < 0 || __builtin_amdgcn_readfirstlane(same[buf][sub]) != wave_doc;
       if (edge) {
         if (ranges != nullptr) {
 #pragma unroll
@@ -324,8 +368,8 @@ __global__ __launch_bounds__(THREADS, 2) void attend_fwd_mfma(FastArgs g, RuleAr
     if (cur < visit.to) {
       u16* Kn = tiles + 2 * (buf ^ 1) * TE;
       st.store(Kn, Kn + TE);
-      if (threadIdx.x < TILE) kdocs[buf ^ 1][threadIdx.x] = dnext;
-      nxt = visit.next(cur + 1);
+      if (ranges != nullptr && wave == 0) store_docs(dnext, kdocs[buf ^ 1], same[buf ^ 1]);
+      nxt = visit.next();
       if (nxt < visit.to) {
         st.load(krows, vrows, nxt * TILE);
         dnext = docs_load(nxt);
@@ -349,12 +393,13 @@ __global__ __launch_bounds__(THREADS, 2) void attend_dq_mfma(FastArgs g, RuleArg
   constexpr bool RAW = !CAP && !BIAS;
   __shared__ __attribute__((aligned(16))) u16 tiles[4 * TE];
   __shared__ __attribute__((aligned(16))) int kdocs[2][TILE];
+  __shared__ int same[2][2];
   __shared__ uint64_t bits[ATT_WORDS];
 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5, n = lane & 31;
   const int64_t nqb = (ra.t_q + ATT_ROWS - 1) / ATT_ROWS;
   int64_t bh, blk;
-  head_and_block(g.batch * g.heads, nqb, bh, blk);
+  if (!att_head_and_block(g.batch * g.heads, nqb, g.head_group, bh, blk)) return;
   const int64_t b = bh / g.heads;
   const int head = (int)(bh - b * g.heads), kvh = head / (g.heads / g.kv_heads);
   const int q0 = (int)(nqb - 1 - blk) * ATT_ROWS, wq0 = q0 + wave * 32, row = wq0 + n;
@@ -388,7 +433,7 @@ __global__ __launch_bounds__(THREADS, 2) void attend_dq_mfma(FastArgs g, RuleArg
   const int last = min(q0 + ATT_ROWS, r.t_q) - 1;
   int kend = r.len;
   if (r.causal) kend = min(kend, max(r.off + last + 1, r.pre));
-  Visit visit = {kend > 0 ? (kend + TILE - 1) / TILE : 0, nullptr};
+  Visit visit = {kend > 0 ? (kend + TILE - 1) / TILE : 0, 0, nullptr, 0};
   const int2* ranges = g.ranges ? g.ranges + b * g.granules : nullptr;
   int wave_doc = 0;
   if (ranges != nullptr) {
@@ -407,13 +452,14 @@ __global__ __launch_bounds__(THREADS, 2) void attend_dq_mfma(FastArgs g, RuleArg
 
   HeadStage<D> st;
   int dnext = 0;
-  int cur = visit.next(0), nxt = cur < visit.to ? visit.next(cur + 1) : visit.to;
+  visit.start(0);
+  int cur = visit.next(), nxt = visit.next();
   auto docs_load = [&](int t) { return ranges != nullptr && threadIdx.x < TILE && t * TILE + (int)threadIdx.x < r.len ? r.docs[t * TILE + threadIdx.x] : -1; };
   if (cur < visit.to) {
     st.load(krows, vrows, cur * TILE);
     dnext = docs_load(cur);
     st.store(tiles, tiles + TE);
-    if (threadIdx.x < TILE) kdocs[0][threadIdx.x] = dnext;
+    if (ranges != nullptr && wave == 0) store_docs(dnext, kdocs[0], same[0]);
     if (nxt < visit.to) {
       st.load(krows, vrows, nxt * TILE);
       dnext = docs_load(nxt);
@@ -442,10 +488,7 @@ __global__ __launch_bounds__(THREADS, 2) void attend_dq_mfma(FastArgs g, RuleArg
         s[i] = e * (dp[i] - delta) * (CAP ? bent : 1.f);  // times scale once, at the store
       }
       bool edge = s0 + 32 > r.len || (r.causal && s0 + 31 > r.off + wq0 && s0 + 31 >= r.pre);
-      if (ranges != nullptr && !edge) {
-        const int2 e = ranges[s0 >> 5];
-        edge = wave_doc < 0 || e.x != wave_doc || e.y != wave_doc;
-      }
+      if (ranges != nullptr) edge |= wave_doc < 0 || __builtin_amdgcn_readfirstlane(same[buf][sub]) != wave_doc;
       if (edge) {
         if (ranges != nullptr) {
 #pragma unroll
@@ -470,8 +513,8 @@ __global__ __launch_bounds__(THREADS, 2) void attend_dq_mfma(FastArgs g, RuleArg
     if (cur < visit.to) {
       u16* Kn = tiles + 2 * (buf ^ 1) * TE;
       st.store(Kn, Kn + TE);
-      if (threadIdx.x < TILE) kdocs[buf ^ 1][threadIdx.x] = dnext;
-      nxt = visit.next(cur + 1);
+      if (ranges != nullptr && wave == 0) store_docs(dnext, kdocs[buf ^ 1], same[buf ^ 1]);
+      nxt = visit.next();
       if (nxt < visit.to) {
         st.load(krows, vrows, nxt * TILE);
         dnext = docs_load(nxt);
@@ -484,10 +527,10 @@ __global__ __launch_bounds__(THREADS, 2) void attend_dq_mfma(FastArgs g, RuleArg
   store_rows<T, D>(g.o0 + rows0 * g.hd, acc, wq0, r.t_q, g.hd, g.scale, tiles + wave * TE);
 }
 
-// ---- dK/dV pass -----------------------------------------------------------------------------------------
+// ---- dK/dV pass up to 64 dims -----------------------------------------------------------------------------
 
 template <typename T, int D, bool CAP, bool BIAS>
-__global__ __launch_bounds__(THREADS, D <= 64 ? 2 : 1) void attend_dkv_mfma(FastArgs g, RuleArgs ra) {
+__global__ __launch_bounds__(THREADS, 2) void attend_dkv_mfma(FastArgs g, RuleArgs ra) {
   constexpr int TE = TILE * tile_stride<D>();
   constexpr bool RAW = !CAP && !BIAS;
   constexpr float UP = shift_of<T>(14.f), DOWN = std::is_same<T, F16>::value ? 1.f / 16384.f : 1.f;
@@ -495,12 +538,13 @@ __global__ __launch_bounds__(THREADS, D <= 64 ? 2 : 1) void attend_dkv_mfma(Fast
   __shared__ __attribute__((aligned(16))) float Ls[2][TILE];
   __shared__ __attribute__((aligned(16))) float Ds[2][TILE];
   __shared__ __attribute__((aligned(16))) int qdocs[2][TILE];
+  __shared__ int same[2][2];
   __shared__ uint64_t bits[ATT_WORDS];
 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5, n = lane & 31;
   const int64_t nkb = (ra.t_k + ATT_ROWS - 1) / ATT_ROWS;
   int64_t bk, blk;
-  head_and_block(g.batch * g.kv_heads, nkb, bk, blk);  // causal: the first keys are seen by the most queries
+  if (!att_head_and_block(g.batch * g.kv_heads, nkb, g.head_group, bk, blk)) return;  // causal: the first keys are seen by the most queries
   const int64_t b = bk / g.kv_heads;
   const int kvh = (int)(bk - b * g.kv_heads), group = g.heads / g.kv_heads;
   const int k0 = (int)blk * ATT_ROWS, wk0 = k0 + wave * 32, key = wk0 + n;
@@ -521,7 +565,7 @@ __global__ __launch_bounds__(THREADS, D <= 64 ? 2 : 1) void attend_dkv_mfma(Fast
 
   // query tiles: from the first that can see the block's first key on, unless a prefix opens it to all
   const int first_q = r.causal && k0 >= r.pre ? max(0, k0 - r.off) / TILE : 0;
-  Visit visit = {k0 < r.len ? (r.t_q + TILE - 1) / TILE : 0, nullptr};
+  Visit visit = {k0 < r.len ? (r.t_q + TILE - 1) / TILE : 0, 0, nullptr, 0};
   const int2* ranges = g.ranges ? g.ranges + b * g.granules : nullptr;
   int wave_doc = 0;
   if (ranges != nullptr) {
@@ -562,17 +606,19 @@ __global__ __launch_bounds__(THREADS, D <= 64 ? 2 : 1) void attend_dkv_mfma(Fast
     if (threadIdx.x < TILE) {
       Ls[buf][threadIdx.x] = lnext;
       Ds[buf][threadIdx.x] = dnext;
-      qdocs[buf][threadIdx.x] = qnext;
+      if (ranges != nullptr) store_docs(qnext, qdocs[buf], same[buf]);
     }
   };
-  const int begin = visit.next(first_q);
+  visit.start(first_q);
+  const int begin = visit.next();
   int gh = 0, cur = begin, ngh = 0, nxt = begin;
   // the tile after (ngh, nxt): the head's next, or the next head's first
   auto advance = [&]() __attribute__((always_inline)) {
-    nxt = visit.next(nxt + 1);
+    nxt = visit.next();
     if (nxt >= visit.to) {
       ngh++;
-      nxt = begin;
+      visit.start(first_q);
+      nxt = visit.next();
     }
   };
   const bool any = begin < visit.to;
@@ -619,7 +665,7 @@ __global__ __launch_bounds__(THREADS, D <= 64 ? 2 : 1) void attend_dkv_mfma(Fast
         dp[i] = s[i] * fmaf(dp[i], DOWN, -d4[i >> 2][i & 3]) * (CAP ? bent : 1.f);  // times scale once, at the store
       }
       bool edge = s0 + 32 > r.t_q || wk0 + 32 > r.len || (r.causal && r.off + s0 < wk0 + 31 && wk0 + 31 >= r.pre);
-      if (ranges != nullptr && !edge) edge = wave_doc < 0 || !doc_range(ranges, g.granules, r.off + s0, r.off + s0 + 31).is(wave_doc);
+      if (ranges != nullptr) edge |= wave_doc < 0 || __builtin_amdgcn_readfirstlane(same[buf][sub]) != wave_doc;
       if (edge) {
         if (ranges != nullptr) {
 #pragma unroll
@@ -667,22 +713,321 @@ __global__ __launch_bounds__(THREADS, D <= 64 ? 2 : 1) void attend_dkv_mfma(Fast
   store_rows<T, D>(g.o1 + bk * (int64_t)r.t_k * g.hd, gv, wk0, r.t_k, g.hd, DOWN, tiles + wave * TE);
 }
 
+// ---- dK/dV pass past 64 dims: two waves per SIMD --------------------------------------------------------------
+// The 8-wave workgroup of sdpa_bwd_kv_dual (which says what each wave does, and why K and V sit in LDS): wave w
+// takes keys 32 (w % 4) .. + 31 and queries 32 (w / 4) .. + 31 of every tile, tiles of 64 rows x 128 dims come by
+// LDS DMA (dims past hd as zeros) into one of two buffers while the other is computed. One wave a SIMD with K
+// and V in registers (as attend_dkv_mfma, 400 registers) took 1317 us where this takes 797 (4 x 16 heads over 4 key
+// heads, 4096 rows, capped).
+
+// rows [row0, row0 + 64) of hd elements into a swizzled 64 x 128 tile, this wave's eighth
+struct HeadDma8 {
+  static constexpr int RB = 256, PASSES = TILE * RB / 1024 / KV_WAVES;
+  int voff[PASSES], hd;
+  __device__ __forceinline__ HeadDma8(int hd_, int wave, int lane) : hd(hd_) {
+#pragma unroll
+    for (int p = 0; p < PASSES; p++) {
+      const int r = (p * KV_WAVES + wave) * (1024 / RB) + lane / (RB / 16), c = (lane % (RB / 16)) ^ swz128(r);
+      voff[p] = c * 8 < hd ? (r * hd + c * 8) * 2 : 0x7ffffff0;
+    }
+  }
+  // rows past `rows` read as zeros
+  __device__ __forceinline__ void copy(u16* tile, const u16* m, int row0, int rows, int wave) const {
+    const int left = (rows - row0) * hd * 2;
+    const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc((void*)(m + (int64_t)row0 * hd), (short)0, left > 0 ? left : 0, 0x00020000);
+#pragma unroll
+    for (int p = 0; p < PASSES; p++)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_void*)((char*)tile + (p * KV_WAVES + wave) * 1024), 16, voff[p], 0, 0, 0);
+  }
+};
+
+template <typename T, int D, bool CAP, bool BIAS>
+__global__ __launch_bounds__(64 * KV_WAVES, 1) void attend_dkv_wide(FastArgs g, RuleArgs ra) {
+#if defined(__HIP_DEVICE_COMPILE__)  // the host pass needs the stub alone
+  constexpr bool RAW = !CAP && !BIAS;
+  constexpr int KS = D / 16, DT = D / 32;
+  constexpr float UP = shift_of<T>(14.f), DOWN = std::is_same<T, F16>::value ? 1.f / 16384.f : 1.f;
+  __shared__ __attribute__((aligned(1024))) u16 Q0[TILE * 128];
+  __shared__ __attribute__((aligned(1024))) u16 Q1[TILE * 128];
+  __shared__ __attribute__((aligned(1024))) u16 O0[TILE * 128];
+  __shared__ __attribute__((aligned(1024))) u16 O1[TILE * 128];
+  __shared__ __attribute__((aligned(1024))) u16 Ks[ATT_ROWS * 128];
+  __shared__ __attribute__((aligned(1024))) u16 Vs[ATT_ROWS * 128];
+  __shared__ __attribute__((aligned(16))) float Ls[2][TILE];
+  __shared__ __attribute__((aligned(16))) float Ds[2][TILE];
+  __shared__ __attribute__((aligned(16))) int qdocs[2][TILE];
+  __shared__ int same[2][2];
+  __shared__ uint64_t bits[ATT_WORDS];
+
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5, n = lane & 31;
+  const int kg = wave & 3, hq = wave >> 2;  // key group, query half
+  const int64_t nkb = (ra.t_k + ATT_ROWS - 1) / ATT_ROWS;
+  int64_t bk, blk;
+  if (!att_head_and_block(g.batch * g.kv_heads, nkb, g.head_group, bk, blk)) return;
+  const int64_t b = bk / g.kv_heads;
+  const int kvh = (int)(bk - b * g.kv_heads), group = g.heads / g.kv_heads;
+  const int k0 = (int)blk * ATT_ROWS, wk0 = k0 + kg * 32, key = wk0 + n;
+  const Rules r = rules_of(ra, b);
+  const bool there = key < r.len;
+  const int doc = r.docs != nullptr ? (there ? r.docs[key] : -1) : 0;
+  const u16* kbase = g.k + bk * (int64_t)r.t_k * g.hd;
+  const u16* vbase = g.v + bk * (int64_t)r.t_k * g.hd;
+  const HeadDma8 dma(g.hd, wave, lane);
+  // byte offsets of this lane's LDS reads, see sdpa_bwd_kv_dual. A row's 16-deep step ds is 32 ds exclusive-or'ed
+  // into its first: the K and V rows' offsets are made so as they are read, which leaves their registers free
+  int rk0, rq[KS], rt[DT][2];
+  {
+    const SwzReads128 ad(lane);
+#pragma unroll
+    for (int ds = 0; ds < KS; ds++) {
+      rq[ds] = ad.row[ds] + hq * 32 * 256;
+    }
+    rk0 = ad.row[0] + kg * 32 * 256;
+#pragma unroll
+    for (int dt = 0; dt < DT; dt++)
+#pragma unroll
+      for (int jj = 0; jj < 2; jj++) rt[dt][jj] = ad.tr[dt][jj] + hq * 32 * 256;
+  }
+  auto rows_at = [](const u16* base, int off) __attribute__((always_inline)) { return *(const u16x8*)((const char*)base + off); };
+  auto transposed_at = [&](const u16* tile, int c, int dt) __attribute__((always_inline)) {
+    const char* p = (const char*)tile + c * 16 * 256;
+    const v4i16 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16*)(p + rt[dt][0]));
+    const v4i16 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16*)(p + rt[dt][1]));
+    return __builtin_bit_cast(u16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+  };
+
+  f32x16 gk[DT], gv[DT];
+#pragma unroll
+  for (int dt = 0; dt < DT; dt++) gk[dt] = gv[dt] = zero16();
+
+  // query tiles: from the first that can see the block's first key on, unless a prefix opens it to all
+  const int first_q = r.causal && k0 >= r.pre ? max(0, k0 - r.off) / TILE : 0;
+  Visit visit = {k0 < r.len ? (r.t_q + TILE - 1) / TILE : 0, 0, nullptr, 0};
+  const int2* ranges = g.ranges ? g.ranges + b * g.granules : nullptr;
+  int wave_doc = 0;
+  if (ranges != nullptr) {
+    const DocRange mine = doc_range(ranges, g.granules, k0, min(k0 + ATT_ROWS, r.t_k) - 1);
+    for (int w = wave; w * 64 < visit.to; w += KV_WAVES) {
+      const int t = w * 64 + lane;
+      const bool meets = t < visit.to && mine.meets(doc_range(ranges, g.granules, r.off + t * TILE, r.off + min(t * TILE + TILE, r.t_q) - 1));
+      const uint64_t word = __ballot(meets);
+      if (lane == 0) bits[w] = word;
+    }
+    visit.bits = bits;
+    const int first = __builtin_amdgcn_readfirstlane(doc);
+    wave_doc = __all(doc == first) ? first : -1;
+    __syncthreads();
+  }
+
+  const int64_t base_row = (b * g.heads + kvh * (int64_t)group) * r.t_q;
+  // tile `t` of query head `gh` of the group: its rows by DMA, its statistics through registers (the first wave)
+  // and its documents (the second), stored only when the tile before it is done: loads retire in order
+  float lnext = 0.f, dnext = 0.f;
+  int qnext = -1;
+  auto load = [&](int gh, int t, u16* Q, u16* O) __attribute__((always_inline)) {
+    const int64_t rows0 = base_row + (int64_t)gh * r.t_q;
+    dma.copy(Q, g.q + rows0 * g.hd, t * TILE, r.t_q, wave);
+    dma.copy(O, g.dout + rows0 * g.hd, t * TILE, r.t_q, wave);
+    const int qq = t * TILE + lane;
+    const bool ok = qq < r.t_q;
+    if (wave == 0) {
+      lnext = ok ? g.lse_in[rows0 + qq] : neg_inf();
+      dnext = ok ? g.delta[rows0 + qq] : 0.f;
+    }
+    if (wave == 1 && ranges != nullptr) qnext = ok ? query_doc(r, r.off + qq) : -1;
+  };
+  auto stats_store = [&](int buf) __attribute__((always_inline)) {
+    if (wave == 0) {
+      Ls[buf][lane] = att_l2(lnext) - UP;
+      Ds[buf][lane] = dnext * DOWN;
+    }
+    if (wave == 1 && ranges != nullptr) store_docs(qnext, qdocs[buf], same[buf]);
+  };
+
+  visit.start(first_q);
+  const int begin = visit.next();
+  int gh = 0, cur = begin, ngh = 0, nxt = begin;
+  auto advance = [&]() __attribute__((always_inline)) {
+    nxt = visit.next();
+    if (nxt >= visit.to) {
+      ngh++;
+      visit.start(first_q);
+      nxt = visit.next();
+    }
+  };
+
+  // this wave's 32 queries of the tile against its 32 keys
+  auto tile = [&](int buf, const u16* Qc, const u16* Oc) __attribute__((always_inline)) {
+    const int s0 = cur * TILE + hq * 32;
+    const float slope2 = BIAS ? ra.slopes[kvh * group + gh] * LOG2E : 0.f;
+    int rk = rk0;
+    asm volatile("" : "+v"(rk)::"memory");  // keeps the K and V reads and their offsets in the loop: hoisted, they would fill the registers
+    f32x16 s = zero16(), dp = zero16();
+    u16x8 xa[2][4];
+    auto xread = [&](int ds, u16x8* o) __attribute__((always_inline)) {
+      const int rkd = rk ^ (32 * ds);
+      o[0] = rows_at(Qc, rq[ds]); o[1] = rows_at(Ks, rkd); o[2] = rows_at(Oc, rq[ds]); o[3] = rows_at(Vs, rkd);
+    };
+    xread(0, xa[0]);
+#pragma unroll
+    for (int ds = 0; ds < KS; ds++) {
+      if (ds + 1 < KS) xread(ds + 1, xa[(ds + 1) & 1]);
+      s = T::mfma32(xa[ds & 1][0], xa[ds & 1][1], s);
+      dp = T::mfma32(xa[ds & 1][2], xa[ds & 1][3], dp);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    bool edge = s0 + 32 > r.t_q || wk0 + 32 > r.len || (r.causal && r.off + s0 < wk0 + 31 && wk0 + 31 >= r.pre);
+    if (ranges != nullptr) edge |= wave_doc < 0 || __builtin_amdgcn_readfirstlane(same[buf][hq]) != wave_doc;
+    const float near = (float)(r.off + s0 + 4 * h - key);
+    // the scores straight into packed operands, in two instances: with element tests and without
+    unsigned pk[8], gp[8];
+    auto soft = [&](auto tests) __attribute__((always_inline)) {
+      f32x4 l4, d4;
+      int4 q4 = {0, 0, 0, 0};
+      float pv = 0.f, gv2 = 0.f;
+#pragma unroll
+      for (int i = 0; i < 16; i++) {
+        if ((i & 3) == 0) {
+          l4 = *(const f32x4*)&Ls[buf][hq * 32 + 8 * (i >> 2) + 4 * h];
+          d4 = *(const f32x4*)&Ds[buf][hq * 32 + 8 * (i >> 2) + 4 * h];
+          if (decltype(tests)::value && ranges != nullptr) q4 = *(const int4*)&qdocs[buf][hq * 32 + 8 * (i >> 2) + 4 * h];
+        }
+        float bent = 1.f;
+        const float y = bend<CAP, BIAS, true>(s[i], r, slope2, near + (float)(8 * (i >> 2) + (i & 3)), bent);
+        float e = fast_exp2(RAW ? fmaf(y, r.c2, -l4[i & 3]) : y - l4[i & 3]);
+        float d = e * fmaf(dp[i], DOWN, -d4[i & 3]) * (CAP ? bent : 1.f);  // times scale once, at the store
+        if (decltype(tests)::value) {
+          const int qq = s0 + 8 * (i >> 2) + 4 * h + (i & 3), qd = (i & 3) == 0 ? q4.x : (i & 3) == 1 ? q4.y : (i & 3) == 2 ? q4.z : q4.w;
+          const bool see = (qq < r.t_q) & (doc >= 0) & (qd == doc) & sees(r, r.off + qq, key);
+          e = see ? e : 0.f;
+          d = see ? d : 0.f;
+        }
+        if (i & 1) {
+          pk[i >> 1] = T::pack2(pv, e);
+          gp[i >> 1] = T::pack2(gv2, d);
+        } else {
+          pv = e;
+          gv2 = d;
+        }
+      }
+    };
+    if (edge)
+      soft(std::true_type{});
+    else
+      soft(std::false_type{});
+    u16x8 pb[2], gb[2];
+#pragma unroll
+    for (int c = 0; c < 2; c++) {
+      const u32x4 wp = {pk[4 * c], pk[4 * c + 1], pk[4 * c + 2], pk[4 * c + 3]}, wg = {gp[4 * c], gp[4 * c + 1], gp[4 * c + 2], gp[4 * c + 3]};
+      pb[c] = __builtin_bit_cast(u16x8, wp);
+      gb[c] = __builtin_bit_cast(u16x8, wg);
+    }
+    u16x8 ya[2][2];
+    auto yread = [&](int j, u16x8* o) __attribute__((always_inline)) {
+      o[0] = transposed_at(Oc, j / DT, j % DT); o[1] = transposed_at(Qc, j / DT, j % DT);
+    };
+    yread(0, ya[0]);
+#pragma unroll
+    for (int j = 0; j < 2 * DT; j++) {
+      if (j + 1 < 2 * DT) yread(j + 1, ya[(j + 1) & 1]);
+      gv[j % DT] = T::mfma32(ya[j & 1][0], pb[j / DT], gv[j % DT]);
+      gk[j % DT] = T::mfma32(ya[j & 1][1], gb[j / DT], gk[j % DT]);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+  // one tile while the next is copied; behind the last one the last head's is copied again, for nothing
+  auto step = [&](int buf, const u16* Qc, const u16* Oc, u16* Qn, u16* On) __attribute__((always_inline)) {
+    load(min(ngh, group - 1), nxt, Qn, On);
+    __builtin_amdgcn_sched_barrier(0);
+    tile(buf, Qc, Oc);
+    __builtin_amdgcn_s_waitcnt(WAIT_VMEM);
+    stats_store(buf ^ 1);
+    __syncthreads();
+    gh = ngh;
+    cur = nxt;
+    advance();
+  };
+  if (begin < visit.to) {
+    int total = visit.to - begin;  // tiles of a head
+    if (ranges != nullptr) {
+      total = 0;
+      for (int w = begin >> 6; w * 64 < visit.to; w++) {
+        const uint64_t word = bits[w];
+        total += __builtin_popcountll(w == begin >> 6 ? word & (~0ull << (begin & 63)) : word);
+      }
+      total = __builtin_amdgcn_readfirstlane(total);
+    }
+    total *= group;
+    dma.copy(Ks, kbase, k0, r.len, wave);
+    dma.copy(Ks + TILE * 128, kbase, k0 + TILE, r.len, wave);
+    dma.copy(Vs, vbase, k0, r.len, wave);
+    dma.copy(Vs + TILE * 128, vbase, k0 + TILE, r.len, wave);
+    load(0, begin, Q0, O0);
+    __builtin_amdgcn_s_waitcnt(WAIT_VMEM);
+    stats_store(0);
+    __syncthreads();
+    advance();
+    int t = 0;
+    for (; t + 1 < total; t += 2) {
+      step(0, Q0, O0, Q1, O1);
+      step(1, Q1, O1, Q0, O0);
+    }
+    if (t < total) step(0, Q0, O0, Q1, O1);
+  }
+  __syncthreads();  // every wave is done with every buffer
+  const bool odd_k = any_odd(gk), odd_v = any_odd(gv);
+  if (threadIdx.x == 0) g.odd[bk * nkb + blk] = odd_k | odd_v;
+  // the second query half's partial sums to LDS, added to the first's: always in that order
+  char* const part_k = kg == 0 ? (char*)Ks : kg == 1 ? (char*)Vs : kg == 2 ? (char*)Q0 : (char*)O0;
+  char* const part_v = kg == 0 ? (char*)Ks + 16384 : kg == 1 ? (char*)Vs + 16384 : kg == 2 ? (char*)Q1 : (char*)O1;
+  if (hq == 1) {
+#pragma unroll
+    for (int dt = 0; dt < DT; dt++)
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        *(f32x4*)(part_k + ((dt * 4 + e) * 64 + lane) * 16) = f32x4{gk[dt][4 * e], gk[dt][4 * e + 1], gk[dt][4 * e + 2], gk[dt][4 * e + 3]};
+        *(f32x4*)(part_v + ((dt * 4 + e) * 64 + lane) * 16) = f32x4{gv[dt][4 * e], gv[dt][4 * e + 1], gv[dt][4 * e + 2], gv[dt][4 * e + 3]};
+      }
+  }
+  __syncthreads();
+  if (hq == 0) {
+#pragma unroll
+    for (int dt = 0; dt < DT; dt++)
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        const f32x4 pk4 = *(const f32x4*)(part_k + ((dt * 4 + e) * 64 + lane) * 16);
+        const f32x4 pv4 = *(const f32x4*)(part_v + ((dt * 4 + e) * 64 + lane) * 16);
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+          gk[dt][4 * e + j] += pk4[j];
+          gv[dt][4 * e + j] += pv4[j];
+        }
+      }
+    u16* stage = (u16*)part_k;  // which only this wave reads from now on
+    store_rows<T, D>(g.o0 + bk * (int64_t)r.t_k * g.hd, gk, wk0, r.t_k, g.hd, g.scale, stage);
+    store_rows<T, D>(g.o1 + bk * (int64_t)r.t_k * g.hd, gv, wk0, r.t_k, g.hd, DOWN, stage);
+  }
+#endif
+}
+
 // ---- launches -------------------------------------------------------------------------------------------
 
 enum AttendPass { ATTEND_PASS_FWD, ATTEND_PASS_DQ, ATTEND_PASS_DKV };
 
 template <AttendPass PASS, typename T, int D, bool CAP, bool BIAS>
 int launch_fast_as(const FastArgs& g, const RuleArgs& ra, hipStream_t stream) {
-  const int64_t blocks = PASS == ATTEND_PASS_DKV ? g.batch * g.kv_heads * ((ra.t_k + ATT_ROWS - 1) / ATT_ROWS)
-                                                 : g.batch * g.heads * ((ra.t_q + ATT_ROWS - 1) / ATT_ROWS);
+  const int64_t blocks = PASS == ATTEND_PASS_DKV ? att_grid(g.batch * g.kv_heads, (ra.t_k + ATT_ROWS - 1) / ATT_ROWS, g.head_group)
+                                                 : att_grid(g.batch * g.heads, (ra.t_q + ATT_ROWS - 1) / ATT_ROWS, g.head_group);
   if (blocks > 0x7fffffff) return fail(LIMN_HIP_EUNSUPPORTED, "attend: %lld workgroups exceed one launch", (long long)blocks);
   const dim3 grid((unsigned)blocks), block(THREADS);
   if constexpr (PASS == ATTEND_PASS_FWD)
     hipLaunchKernelGGL((attend_fwd_mfma<T, D, CAP, BIAS>), grid, block, 0, stream, g, ra);
   else if constexpr (PASS == ATTEND_PASS_DQ)
     hipLaunchKernelGGL((attend_dq_mfma<T, D, CAP, BIAS>), grid, block, 0, stream, g, ra);
-  else
+  else if constexpr (D <= 64)
     hipLaunchKernelGGL((attend_dkv_mfma<T, D, CAP, BIAS>), grid, block, 0, stream, g, ra);
+  else
+    hipLaunchKernelGGL((attend_dkv_wide<T, D, CAP, BIAS>), grid, dim3(64 * KV_WAVES), 0, stream, g, ra);
   return check_hip(hipGetLastError(), "launching attention");
 }
 
