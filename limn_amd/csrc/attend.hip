@@ -163,7 +163,7 @@ bool fast_call(const AttendArgs& a, bool backward) { return fast_sizes(a) && a.s
 // flags of the blocks, the documents' ranges, and for the backward delta
 int64_t fast_workspace(const AttendArgs& a, bool backward) {
   if (!fast_sizes(a)) return 0;
-  int64_t need = attend_align(row_blocks(a) * 4) + attend_align(a.batch * granules_of(a) * 8);
+  int64_t need = attend_align(row_blocks(a) * 4) + attend_align(a.batch * granules_of(a) * 16);
   if (backward) need += attend_align(key_blocks(a) * 4) + attend_align(a.batch * a.heads * a.t_q * 4);
   return need;
 }
@@ -189,7 +189,7 @@ int launch_fast(const AttendArgs& a, bool backward) {
     return p;
   };
   int* odd = (int*)take(row_blocks(a) * 4);
-  int2* ranges = (int2*)take(a.batch * granules_of(a) * 8);
+  int4* ranges = (int4*)take(a.batch * granules_of(a) * 16);
   FastArgs g = {};
   g.q = (const u16*)a.q, g.k = (const u16*)a.k, g.v = (const u16*)a.v, g.out = (const u16*)a.out, g.dout = (const u16*)a.dout;
   g.lse_in = a.lse, g.o0 = (u16*)a.o0, g.odd = odd, g.ranges = a.documents != nullptr ? ranges : nullptr;

@@ -16,7 +16,7 @@ struct FastArgs {
   const u16* dout;
   const float* lse_in;
   float* delta;
-  const int2* ranges;  // (batch, granules): documents of 32 positions, see attend_ranges; nullptr without
+  const int4* ranges;  // (batch, granules): documents of 32 positions, see attend_ranges; nullptr without
   u16* o0;             // out / dq / dk
   u16* o1;             // dv
   float* lse;
@@ -27,7 +27,7 @@ struct FastArgs {
   float scale;
 };
 
-int launch_attend_ranges(const RuleArgs& ra, int2* ranges, int64_t batch, int granules, hipStream_t stream);
+int launch_attend_ranges(const RuleArgs& ra, int4* ranges, int64_t batch, int granules, hipStream_t stream);
 int launch_attend_mend_fwd(const FastArgs& g, const RuleArgs& ra, int dtype, hipStream_t stream);
 // blocks of the dQ pass (g.odd) and of the dK/dV pass (kv.odd) that are to be computed again
 int launch_attend_mend_bwd(const FastArgs& g, const FastArgs& kv, const RuleArgs& ra, int dtype, hipStream_t stream);

@@ -8,21 +8,22 @@ namespace limn {
 namespace {
 
 // The least and greatest document of each 32 positions, padding and positions past the live keys left out
-// (0x7fffffff and 0, an empty range, if there is nothing else).
-__global__ __launch_bounds__(256) void attend_ranges(RuleArgs ra, int2* __restrict__ ranges, int64_t batch, int granules) {
+// (0x7fffffff and 0, an empty range, if there is nothing else), and the document of all 32, or -2.
+__global__ __launch_bounds__(256) void attend_ranges(RuleArgs ra, int4* __restrict__ ranges, int64_t batch, int granules) {
   const int64_t id = blockIdx.x * (int64_t)8 + (threadIdx.x >> 5), b = id / granules;
   if (b >= batch) return;  // a half wave at a time: the shuffles below stay inside it
   const int g = (int)(id - b * granules), n = threadIdx.x & 31, p = g * 32 + n;
   const int len = ra.lengths ? ra.lengths[b] : ra.t_k;
   int doc = -1;
   if (p < ra.t_k && p < len) doc = ra.documents[b * ra.t_k + p];
-  int lo = doc < 0 ? 0x7fffffff : doc, hi = doc < 0 ? 0 : doc;
+  int lo = doc < 0 ? 0x7fffffff : doc, hi = doc < 0 ? 0 : doc, none = doc < 0;
 #pragma unroll
   for (int m = 1; m < 32; m <<= 1) {
     lo = min(lo, __shfl_xor(lo, m));
     hi = max(hi, __shfl_xor(hi, m));
+    none |= __shfl_xor(none, m);
   }
-  if (n == 0) ranges[id] = make_int2(lo, hi);
+  if (n == 0) ranges[id] = make_int4(lo, hi, lo == hi && !none ? lo : -2, 0);
 }
 
 // The flagged blocks among those of this workgroup (every gridDim.x-th), found 256 flags at a time.
@@ -133,7 +134,7 @@ int launch_attend_mend_rows(const AttendArgs& a) {
   return a.hd <= 64 ? mend_rows<F16, 2>(a) : mend_rows<F16, 4>(a);
 }
 
-int launch_attend_ranges(const RuleArgs& ra, int2* ranges, int64_t batch, int granules, hipStream_t stream) {
+int launch_attend_ranges(const RuleArgs& ra, int4* ranges, int64_t batch, int granules, hipStream_t stream) {
   const int64_t blocks = (batch * granules + 7) / 8;
   if (blocks > 0x7fffffff) return fail(LIMN_HIP_EUNSUPPORTED, "attend: %lld workgroups exceed one launch", (long long)blocks);
   hipLaunchKernelGGL(attend_ranges, dim3((unsigned)blocks), dim3(256), 0, stream, ra, ranges, batch, granules);

@@ -28,7 +28,7 @@
 namespace limn {
 namespace {
 
-constexpr int ATT_WORDS = 32;      // 64-tile words of the visit list: 131072 streamed rows
+constexpr int ATT_WORDS = 32;     // 64-tile words of the visit list: 131072 streamed rows
 
 // ---- which head and block a workgroup takes ----------------------------------------------------------------
 
@@ -61,11 +61,11 @@ struct DocRange {
 };
 
 // positions [p0, p1], which may reach outside [0, 32 granules)
-__device__ __forceinline__ DocRange doc_range(const int2* ranges, int granules, int p0, int p1) {
+__device__ __forceinline__ DocRange doc_range(const int4* ranges, int granules, int p0, int p1) {
   DocRange r = {0x7fffffff, 0};
   const int g0 = max(p0, 0) >> 5, g1 = min(p1 >> 5, granules - 1);
   for (int g = g0; g <= g1; g++) {
-    const int2 e = ranges[g];
+    const int4 e = ranges[g];
     r.lo = min(r.lo, e.x);
     r.hi = max(r.hi, e.y);
   }
@@ -78,17 +78,28 @@ __device__ __forceinline__ DocRange doc_range(const int2* ranges, int granules, 
 struct Visit {
   int to, at;            // at: the next tile to look at (without bits), or its word's first tile
   const uint64_t* bits;  // or nullptr
-  uint64_t word;
+  const uint64_t* half;  // this wave's words of its halves (see alike_words): first halves, then ATT_WORDS on the second
+  uint64_t word, half0, half1;
+  int alike;             // of the tile that next() returned: bit 0 / 1, its first / second half has the wave's document alone
   __device__ __forceinline__ void start(int first) {
     at = first;
+    alike = 3;
     if (bits != nullptr) {
       at = first & ~63;
-      word = at < to ? fetch() & (~0ull << (first & 63)) : 0;
+      word = 0;
+      if (at < to) {
+        fetch();
+        word &= ~0ull << (first & 63);
+      }
     }
   }
-  __device__ __forceinline__ uint64_t fetch() const {
-    const uint64_t w = bits[at >> 6];
+  static __device__ __forceinline__ uint64_t scalar(uint64_t w) {
     return ((uint64_t)(unsigned)__builtin_amdgcn_readfirstlane((int)(w >> 32)) << 32) | (unsigned)__builtin_amdgcn_readfirstlane((int)w);
+  }
+  __device__ __forceinline__ void fetch() {
+    word = scalar(bits[at >> 6]);
+    half0 = scalar(half[at >> 6]);
+    half1 = scalar(half[ATT_WORDS + (at >> 6)]);
   }
   // the next tile, or `to` behind the last
   __device__ __forceinline__ int next() {
@@ -98,22 +109,45 @@ struct Visit {
         at = to;  // stays there: a word past the end is never read
         return to;
       }
-      word = fetch();
+      fetch();
     }
-    const int t = at + __builtin_ctzll(word);
+    const int bit = __builtin_ctzll(word);
     word &= word - 1;
-    return t;
+    alike = (int)((half0 >> bit) & 1) | ((int)((half1 >> bit) & 1) << 1);
+    return at + bit;
   }
 };
 
-// A tile's documents go through LDS with its rows, and for each half of 32 the document of all of them, or
-// -2 where they differ. Lane l of one wave holds position l's.
-__device__ __forceinline__ void store_docs(int doc, int* docs, int* same) {
+// The document that all 32 positions from p on have, or -2: granules hold it for whole granules (attend_ranges), and
+// positions that begin inside one are alike where both it and the next say so.
+__device__ __forceinline__ int same_doc(const int4* granules, int count, int p) {
+  const int g = p >> 5;
+  if (p < 0 || g >= count) return -2;
+  const int one = granules[g].z;
+  if ((p & 31) == 0) return one;
+  return g + 1 < count && granules[g + 1].z == one ? one : -2;
+}
+
+// The lists of one block: bits, a bit for each streamed tile (64 positions from p0 + 64 t on, of `rows` in all) whose
+// documents meet the block's, 64 tiles a word, the words shared by the waves; half, for this wave's document doc
+// (-1: its rows differ), a bit for each half tile that has it alone, which then needs no test of documents.
+__device__ __forceinline__ void list_tiles(uint64_t* bits, uint64_t* half, const int4* granules, int count, const DocRange& mine, int doc, int p0, int rows,
+                                           int tiles, int wave, int waves) {
   const int lane = threadIdx.x & 63;
-  docs[lane] = doc;
-  const int lo = __builtin_amdgcn_readlane(doc, 0), hi = __builtin_amdgcn_readlane(doc, 32);
-  const uint64_t eq = __ballot(doc == (lane < 32 ? lo : hi));
-  if (lane < 2) same[lane] = lane == 0 ? ((unsigned)eq == ~0u ? lo : -2) : ((unsigned)(eq >> 32) == ~0u ? hi : -2);
+  for (int w = 0; w * 64 < tiles; w++) {
+    const int t = w * 64 + lane;
+    if (w % waves == wave) {
+      const bool meets = t < tiles && mine.meets(doc_range(granules, count, p0 + t * TILE, p0 + min(t * TILE + TILE, rows) - 1));
+      const uint64_t word = __ballot(meets);
+      if (lane == 0) bits[w] = word;
+    }
+    const bool in = t < tiles && doc >= 0;
+    const uint64_t h0 = __ballot(in && same_doc(granules, count, p0 + t * TILE) == doc), h1 = __ballot(in && same_doc(granules, count, p0 + t * TILE + 32) == doc);
+    if (lane == 0) {
+      half[w] = h0;
+      half[ATT_WORDS + w] = h1;
+    }
+  }
 }
 
 // ---- rows of hd elements in tiles of D ------------------------------------------------------------------
@@ -233,8 +267,8 @@ __global__ __launch_bounds__(THREADS, 2) void attend_fwd_mfma(FastArgs g, RuleAr
   constexpr float UP = shift_of<T>(7.f);
   __shared__ __attribute__((aligned(16))) u16 tiles[4 * TE];
   __shared__ __attribute__((aligned(16))) int kdocs[2][TILE];
-  __shared__ int same[2][2];
   __shared__ uint64_t bits[ATT_WORDS];
+  __shared__ uint64_t halves[WAVES][2 * ATT_WORDS];
 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5, n = lane & 31;
   const int64_t nqb = (ra.t_q + ATT_ROWS - 1) / ATT_ROWS;
@@ -264,33 +298,27 @@ __global__ __launch_bounds__(THREADS, 2) void attend_fwd_mfma(FastArgs g, RuleAr
   const int last = min(q0 + ATT_ROWS, r.t_q) - 1;  // the block's last query
   int kend = r.len;
   if (r.causal) kend = min(kend, max(r.off + last + 1, r.pre));
-  Visit visit = {kend > 0 ? (kend + TILE - 1) / TILE : 0, 0, nullptr, 0};
-  const int2* ranges = g.ranges ? g.ranges + b * g.granules : nullptr;
-  int wave_doc = 0;  // the document of every row of the wave, or -1
+  Visit visit = {kend > 0 ? (kend + TILE - 1) / TILE : 0};
+  const int4* ranges = g.ranges ? g.ranges + b * g.granules : nullptr;
   if (ranges != nullptr) {
-    const DocRange mine = doc_range(ranges, g.granules, r.off + q0, r.off + last);
-    for (int w = wave; w * 64 < visit.to; w += WAVES) {
-      const int t = w * 64 + lane;
-      const bool meets = t < visit.to && mine.meets(doc_range(ranges, g.granules, t * TILE, min(t * TILE + TILE, g.granules * 32) - 1));
-      const uint64_t word = __ballot(meets);
-      if (lane == 0) bits[w] = word;
-    }
-    visit.bits = bits;
     const int first = __builtin_amdgcn_readfirstlane(doc);
-    wave_doc = __all(doc == first) ? first : -1;
+    list_tiles(bits, halves[wave], ranges, g.granules, doc_range(ranges, g.granules, r.off + q0, r.off + last), __all(doc == first) ? first : -1, 0,
+               g.granules * 32, visit.to, wave, WAVES);
+    visit.bits = bits;
+    visit.half = halves[wave];
     __syncthreads();
   }
 
   HeadStage<D> st;
   int dnext = 0;
   visit.start(0);
-  int cur = visit.next(), nxt = visit.next();
+  int cur = visit.next(), alike = visit.alike, nxt = visit.next();
   auto docs_load = [&](int t) { return ranges != nullptr && threadIdx.x < TILE && t * TILE + (int)threadIdx.x < r.len ? r.docs[t * TILE + threadIdx.x] : -1; };
   if (cur < visit.to) {
     st.load(krows, vrows, cur * TILE);
     dnext = docs_load(cur);
     st.store(tiles, tiles + TE);
-    if (ranges != nullptr && wave == 0) store_docs(dnext, kdocs[0], same[0]);
+    if (ranges != nullptr && wave == 0) kdocs[0][lane] = dnext;
     if (nxt < visit.to) {
       st.load(krows, vrows, nxt * TILE);
       dnext = docs_load(nxt);
@@ -319,7 +347,7 @@ __global__ __launch_bounds__(THREADS, 2) void attend_fwd_mfma(FastArgs g, RuleAr
         }
       }
       bool edge = s0 + 32 > r.len || (r.causal && s0 + 31 > r.off + wq0 && s0 + 31 >= r.pre);
-      if (ranges != nullptr) edge |= wave_doc < 0 || __builtin_amdgcn_readfirstlane(same[buf][sub]) != wave_doc;
+      edge |= ((alike >> sub) & 1) == 0;
       if (edge) {
         if (ranges != nullptr) {
 #pragma unroll
@@ -365,10 +393,11 @@ __global__ __launch_bounds__(THREADS, 2) void attend_fwd_mfma(FastArgs g, RuleAr
       }
     }
     cur = nxt;
+    alike = visit.alike;
     if (cur < visit.to) {
       u16* Kn = tiles + 2 * (buf ^ 1) * TE;
       st.store(Kn, Kn + TE);
-      if (ranges != nullptr && wave == 0) store_docs(dnext, kdocs[buf ^ 1], same[buf ^ 1]);
+      if (ranges != nullptr && wave == 0) kdocs[buf ^ 1][lane] = dnext;
       nxt = visit.next();
       if (nxt < visit.to) {
         st.load(krows, vrows, nxt * TILE);
@@ -393,8 +422,8 @@ __global__ __launch_bounds__(THREADS, 2) void attend_dq_mfma(FastArgs g, RuleArg
   constexpr bool RAW = !CAP && !BIAS;
   __shared__ __attribute__((aligned(16))) u16 tiles[4 * TE];
   __shared__ __attribute__((aligned(16))) int kdocs[2][TILE];
-  __shared__ int same[2][2];
   __shared__ uint64_t bits[ATT_WORDS];
+  __shared__ uint64_t halves[WAVES][2 * ATT_WORDS];
 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5, n = lane & 31;
   const int64_t nqb = (ra.t_q + ATT_ROWS - 1) / ATT_ROWS;
@@ -433,33 +462,27 @@ __global__ __launch_bounds__(THREADS, 2) void attend_dq_mfma(FastArgs g, RuleArg
   const int last = min(q0 + ATT_ROWS, r.t_q) - 1;
   int kend = r.len;
   if (r.causal) kend = min(kend, max(r.off + last + 1, r.pre));
-  Visit visit = {kend > 0 ? (kend + TILE - 1) / TILE : 0, 0, nullptr, 0};
-  const int2* ranges = g.ranges ? g.ranges + b * g.granules : nullptr;
-  int wave_doc = 0;
+  Visit visit = {kend > 0 ? (kend + TILE - 1) / TILE : 0};
+  const int4* ranges = g.ranges ? g.ranges + b * g.granules : nullptr;
   if (ranges != nullptr) {
-    const DocRange mine = doc_range(ranges, g.granules, r.off + q0, r.off + last);
-    for (int w = wave; w * 64 < visit.to; w += WAVES) {
-      const int t = w * 64 + lane;
-      const bool meets = t < visit.to && mine.meets(doc_range(ranges, g.granules, t * TILE, min(t * TILE + TILE, g.granules * 32) - 1));
-      const uint64_t word = __ballot(meets);
-      if (lane == 0) bits[w] = word;
-    }
-    visit.bits = bits;
     const int first = __builtin_amdgcn_readfirstlane(doc);
-    wave_doc = __all(doc == first) ? first : -1;
+    list_tiles(bits, halves[wave], ranges, g.granules, doc_range(ranges, g.granules, r.off + q0, r.off + last), __all(doc == first) ? first : -1, 0,
+               g.granules * 32, visit.to, wave, WAVES);
+    visit.bits = bits;
+    visit.half = halves[wave];
     __syncthreads();
   }
 
   HeadStage<D> st;
   int dnext = 0;
   visit.start(0);
-  int cur = visit.next(), nxt = visit.next();
+  int cur = visit.next(), alike = visit.alike, nxt = visit.next();
   auto docs_load = [&](int t) { return ranges != nullptr && threadIdx.x < TILE && t * TILE + (int)threadIdx.x < r.len ? r.docs[t * TILE + threadIdx.x] : -1; };
   if (cur < visit.to) {
     st.load(krows, vrows, cur * TILE);
     dnext = docs_load(cur);
     st.store(tiles, tiles + TE);
-    if (ranges != nullptr && wave == 0) store_docs(dnext, kdocs[0], same[0]);
+    if (ranges != nullptr && wave == 0) kdocs[0][lane] = dnext;
     if (nxt < visit.to) {
       st.load(krows, vrows, nxt * TILE);
       dnext = docs_load(nxt);
@@ -488,7 +511,7 @@ __global__ __launch_bounds__(THREADS, 2) void attend_dq_mfma(FastArgs g, RuleArg
         s[i] = e * (dp[i] - delta) * (CAP ? bent : 1.f);  // times scale once, at the store
       }
       bool edge = s0 + 32 > r.len || (r.causal && s0 + 31 > r.off + wq0 && s0 + 31 >= r.pre);
-      if (ranges != nullptr) edge |= wave_doc < 0 || __builtin_amdgcn_readfirstlane(same[buf][sub]) != wave_doc;
+      edge |= ((alike >> sub) & 1) == 0;
       if (edge) {
         if (ranges != nullptr) {
 #pragma unroll
@@ -510,10 +533,11 @@ __global__ __launch_bounds__(THREADS, 2) void attend_dq_mfma(FastArgs g, RuleArg
       }
     }
     cur = nxt;
+    alike = visit.alike;
     if (cur < visit.to) {
       u16* Kn = tiles + 2 * (buf ^ 1) * TE;
       st.store(Kn, Kn + TE);
-      if (ranges != nullptr && wave == 0) store_docs(dnext, kdocs[buf ^ 1], same[buf ^ 1]);
+      if (ranges != nullptr && wave == 0) kdocs[buf ^ 1][lane] = dnext;
       nxt = visit.next();
       if (nxt < visit.to) {
         st.load(krows, vrows, nxt * TILE);
@@ -538,8 +562,8 @@ __global__ __launch_bounds__(THREADS, 2) void attend_dkv_mfma(FastArgs g, RuleAr
   __shared__ __attribute__((aligned(16))) float Ls[2][TILE];
   __shared__ __attribute__((aligned(16))) float Ds[2][TILE];
   __shared__ __attribute__((aligned(16))) int qdocs[2][TILE];
-  __shared__ int same[2][2];
   __shared__ uint64_t bits[ATT_WORDS];
+  __shared__ uint64_t halves[WAVES][2 * ATT_WORDS];
 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5, n = lane & 31;
   const int64_t nkb = (ra.t_k + ATT_ROWS - 1) / ATT_ROWS;
@@ -565,20 +589,14 @@ __global__ __launch_bounds__(THREADS, 2) void attend_dkv_mfma(FastArgs g, RuleAr
 
   // query tiles: from the first that can see the block's first key on, unless a prefix opens it to all
   const int first_q = r.causal && k0 >= r.pre ? max(0, k0 - r.off) / TILE : 0;
-  Visit visit = {k0 < r.len ? (r.t_q + TILE - 1) / TILE : 0, 0, nullptr, 0};
-  const int2* ranges = g.ranges ? g.ranges + b * g.granules : nullptr;
-  int wave_doc = 0;
+  Visit visit = {k0 < r.len ? (r.t_q + TILE - 1) / TILE : 0};
+  const int4* ranges = g.ranges ? g.ranges + b * g.granules : nullptr;
   if (ranges != nullptr) {
-    const DocRange mine = doc_range(ranges, g.granules, k0, min(k0 + ATT_ROWS, r.t_k) - 1);
-    for (int w = wave; w * 64 < visit.to; w += WAVES) {
-      const int t = w * 64 + lane;
-      const bool meets = t < visit.to && mine.meets(doc_range(ranges, g.granules, r.off + t * TILE, r.off + min(t * TILE + TILE, r.t_q) - 1));
-      const uint64_t word = __ballot(meets);
-      if (lane == 0) bits[w] = word;
-    }
-    visit.bits = bits;
     const int first = __builtin_amdgcn_readfirstlane(doc);
-    wave_doc = __all(doc == first) ? first : -1;
+    list_tiles(bits, halves[wave], ranges, g.granules, doc_range(ranges, g.granules, k0, min(k0 + ATT_ROWS, r.t_k) - 1), __all(doc == first) ? first : -1,
+               r.off, r.t_q, visit.to, wave, WAVES);
+    visit.bits = bits;
+    visit.half = halves[wave];
     __syncthreads();
   }
 
@@ -606,12 +624,12 @@ __global__ __launch_bounds__(THREADS, 2) void attend_dkv_mfma(FastArgs g, RuleAr
     if (threadIdx.x < TILE) {
       Ls[buf][threadIdx.x] = lnext;
       Ds[buf][threadIdx.x] = dnext;
-      if (ranges != nullptr) store_docs(qnext, qdocs[buf], same[buf]);
+      if (ranges != nullptr) qdocs[buf][threadIdx.x] = qnext;
     }
   };
   visit.start(first_q);
   const int begin = visit.next();
-  int gh = 0, cur = begin, ngh = 0, nxt = begin;
+  int gh = 0, cur = begin, ngh = 0, nxt = begin, alike = visit.alike;
   // the tile after (ngh, nxt): the head's next, or the next head's first
   auto advance = [&]() __attribute__((always_inline)) {
     nxt = visit.next();
@@ -665,7 +683,7 @@ __global__ __launch_bounds__(THREADS, 2) void attend_dkv_mfma(FastArgs g, RuleAr
         dp[i] = s[i] * fmaf(dp[i], DOWN, -d4[i >> 2][i & 3]) * (CAP ? bent : 1.f);  // times scale once, at the store
       }
       bool edge = s0 + 32 > r.t_q || wk0 + 32 > r.len || (r.causal && r.off + s0 < wk0 + 31 && wk0 + 31 >= r.pre);
-      if (ranges != nullptr) edge |= wave_doc < 0 || __builtin_amdgcn_readfirstlane(same[buf][sub]) != wave_doc;
+      edge |= ((alike >> sub) & 1) == 0;
       if (edge) {
         if (ranges != nullptr) {
 #pragma unroll
@@ -700,6 +718,7 @@ __global__ __launch_bounds__(THREADS, 2) void attend_dkv_mfma(FastArgs g, RuleAr
     }
     gh = ngh;
     cur = nxt;
+    alike = visit.alike;
     if (gh < group) {
       store(buf ^ 1);
       advance();
@@ -756,8 +775,8 @@ __global__ __launch_bounds__(64 * KV_WAVES, 1) void attend_dkv_wide(FastArgs g, 
   __shared__ __attribute__((aligned(16))) float Ls[2][TILE];
   __shared__ __attribute__((aligned(16))) float Ds[2][TILE];
   __shared__ __attribute__((aligned(16))) int qdocs[2][TILE];
-  __shared__ int same[2][2];
   __shared__ uint64_t bits[ATT_WORDS];
+  __shared__ uint64_t halves[KV_WAVES][2 * ATT_WORDS];
 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5, n = lane & 31;
   const int kg = wave & 3, hq = wave >> 2;  // key group, query half
@@ -802,20 +821,14 @@ __global__ __launch_bounds__(64 * KV_WAVES, 1) void attend_dkv_wide(FastArgs g, 
 
   // query tiles: from the first that can see the block's first key on, unless a prefix opens it to all
   const int first_q = r.causal && k0 >= r.pre ? max(0, k0 - r.off) / TILE : 0;
-  Visit visit = {k0 < r.len ? (r.t_q + TILE - 1) / TILE : 0, 0, nullptr, 0};
-  const int2* ranges = g.ranges ? g.ranges + b * g.granules : nullptr;
-  int wave_doc = 0;
+  Visit visit = {k0 < r.len ? (r.t_q + TILE - 1) / TILE : 0};
+  const int4* ranges = g.ranges ? g.ranges + b * g.granules : nullptr;
   if (ranges != nullptr) {
-    const DocRange mine = doc_range(ranges, g.granules, k0, min(k0 + ATT_ROWS, r.t_k) - 1);
-    for (int w = wave; w * 64 < visit.to; w += KV_WAVES) {
-      const int t = w * 64 + lane;
-      const bool meets = t < visit.to && mine.meets(doc_range(ranges, g.granules, r.off + t * TILE, r.off + min(t * TILE + TILE, r.t_q) - 1));
-      const uint64_t word = __ballot(meets);
-      if (lane == 0) bits[w] = word;
-    }
-    visit.bits = bits;
     const int first = __builtin_amdgcn_readfirstlane(doc);
-    wave_doc = __all(doc == first) ? first : -1;
+    list_tiles(bits, halves[wave], ranges, g.granules, doc_range(ranges, g.granules, k0, min(k0 + ATT_ROWS, r.t_k) - 1), __all(doc == first) ? first : -1,
+               r.off, r.t_q, visit.to, wave, KV_WAVES);
+    visit.bits = bits;
+    visit.half = halves[wave];
     __syncthreads();
   }
 
@@ -841,12 +854,12 @@ __global__ __launch_bounds__(64 * KV_WAVES, 1) void attend_dkv_wide(FastArgs g, 
       Ls[buf][lane] = att_l2(lnext) - UP;
       Ds[buf][lane] = dnext * DOWN;
     }
-    if (wave == 1 && ranges != nullptr) store_docs(qnext, qdocs[buf], same[buf]);
+    if (wave == 1 && ranges != nullptr) qdocs[buf][lane] = qnext;
   };
 
   visit.start(first_q);
   const int begin = visit.next();
-  int gh = 0, cur = begin, ngh = 0, nxt = begin;
+  int gh = 0, cur = begin, ngh = 0, nxt = begin, alike = visit.alike;
   auto advance = [&]() __attribute__((always_inline)) {
     nxt = visit.next();
     if (nxt >= visit.to) {
@@ -877,7 +890,7 @@ __global__ __launch_bounds__(64 * KV_WAVES, 1) void attend_dkv_wide(FastArgs g, 
       __builtin_amdgcn_sched_barrier(0);
     }
     bool edge = s0 + 32 > r.t_q || wk0 + 32 > r.len || (r.causal && r.off + s0 < wk0 + 31 && wk0 + 31 >= r.pre);
-    if (ranges != nullptr) edge |= wave_doc < 0 || __builtin_amdgcn_readfirstlane(same[buf][hq]) != wave_doc;
+    edge |= ((alike >> hq) & 1) == 0;
     const float near = (float)(r.off + s0 + 4 * h - key);
     // the scores straight into packed operands, in two instances: with element tests and without
     unsigned pk[8], gp[8];
@@ -945,6 +958,7 @@ __global__ __launch_bounds__(64 * KV_WAVES, 1) void attend_dkv_wide(FastArgs g, 
     __syncthreads();
     gh = ngh;
     cur = nxt;
+    alike = visit.alike;
     advance();
   };
   if (begin < visit.to) {
@@ -1010,6 +1024,399 @@ __global__ __launch_bounds__(64 * KV_WAVES, 1) void attend_dkv_wide(FastArgs g, 
 #endif
 }
 
+// ---- forward and dQ pass past 64 dims: tiles by LDS DMA ---------------------------------------------------------
+// As attend_fwd_mfma and attend_dq_mfma, with the streamed tiles copied straight into swizzled LDS tiles of 64 x 128
+// (dims past hd as zeros), and the forward pipelined as sdpa_fwd_dma is: a tile's exponentials and its V product
+// are issued beside the next tile's scores. Staged through registers the forward took 753 us and the dQ pass 881
+// (8 x 16 heads x 4096 rows, causal).
+
+// rows [row0, row0 + 64) of hd elements into a swizzled 64 x 128 tile, this wave's quarter
+struct HeadDma4 {
+  static constexpr int RB = 256, PASSES = TILE * RB / 1024 / WAVES;
+  int voff[PASSES], hd;
+  __device__ __forceinline__ HeadDma4(int hd_, int wave, int lane) : hd(hd_) {
+#pragma unroll
+    for (int p = 0; p < PASSES; p++) {
+      const int r = (p * WAVES + wave) * (1024 / RB) + lane / (RB / 16), c = (lane % (RB / 16)) ^ swz128(r);
+      voff[p] = c * 8 < hd ? (r * hd + c * 8) * 2 : 0x7ffffff0;
+    }
+  }
+  // rows past `rows` read as zeros
+  __device__ __forceinline__ void copy(u16* tile, const u16* m, int row0, int rows, int wave) const {
+    const int left = (rows - row0) * hd * 2;
+    const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc((void*)(m + (int64_t)row0 * hd), (short)0, left > 0 ? left : 0, 0x00020000);
+#pragma unroll
+    for (int p = 0; p < PASSES; p++)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_void*)((char*)tile + (p * WAVES + wave) * 1024), 16, voff[p], 0, 0, 0);
+  }
+};
+
+// What a block of 128 query rows of one head is, for both passes.
+struct QueryBlock {
+  int64_t b, bh, nqb;
+  int head, kvh, q0, wq0, row, p, doc;
+};
+
+// The key tiles such a block visits: lists in LDS where there are documents.
+__device__ __forceinline__ Visit key_visit(const FastArgs& g, const Rules& r, const QueryBlock& qb, const int4* ranges, uint64_t* bits, uint64_t* half, int wave) {
+  const int last = min(qb.q0 + ATT_ROWS, r.t_q) - 1;
+  int kend = r.len;
+  if (r.causal) kend = min(kend, max(r.off + last + 1, r.pre));
+  Visit visit = {kend > 0 ? (kend + TILE - 1) / TILE : 0};
+  if (ranges != nullptr) {
+    const int first = __builtin_amdgcn_readfirstlane(qb.doc);
+    list_tiles(bits, half, ranges, g.granules, doc_range(ranges, g.granules, r.off + qb.q0, r.off + last), __all(qb.doc == first) ? first : -1, 0,
+               g.granules * 32, visit.to, wave, WAVES);
+    visit.bits = bits;
+    visit.half = half;
+    __syncthreads();
+  }
+  return visit;
+}
+
+// tiles of a visit that starts at 0
+__device__ __forceinline__ int visit_count(const Visit& v) {
+  if (v.bits == nullptr) return v.to;
+  int n = 0;
+  for (int w = 0; w * 64 < v.to; w++) n += __builtin_popcountll(v.bits[w]);
+  return __builtin_amdgcn_readfirstlane(n);
+}
+
+__device__ __forceinline__ bool query_block(const FastArgs& g, const RuleArgs& ra, QueryBlock& qb, int wave, int n) {
+  qb.nqb = (ra.t_q + ATT_ROWS - 1) / ATT_ROWS;
+  int64_t blk;
+  if (!att_head_and_block(g.batch * g.heads, qb.nqb, g.head_group, qb.bh, blk)) return false;
+  qb.b = qb.bh / g.heads;
+  qb.head = (int)(qb.bh - qb.b * g.heads);
+  qb.kvh = qb.head / (g.heads / g.kv_heads);
+  qb.q0 = (int)(qb.nqb - 1 - blk) * ATT_ROWS;  // causal: the longest rows go first
+  qb.wq0 = qb.q0 + wave * 32;
+  qb.row = qb.wq0 + n;
+  return true;
+}
+
+// Whether a half tile of 32 keys needs element tests for the wave's rows; alike: its bit of Visit::alike.
+__device__ __forceinline__ bool half_edge(const Rules& r, const QueryBlock& qb, int alike, int s0) {
+  return alike == 0 || s0 + 32 > r.len || (r.causal && s0 + 31 > r.off + qb.wq0 && s0 + 31 >= r.pre);
+}
+
+template <typename T, int D, bool CAP, bool BIAS>
+__global__ __launch_bounds__(THREADS, 2) void attend_fwd_wide(FastArgs g, RuleArgs ra) {
+#if defined(__HIP_DEVICE_COMPILE__)  // the host pass needs the stub alone
+  constexpr bool RAW = !CAP && !BIAS;
+  constexpr int KS = D / 16, DT = D / 32;
+  constexpr float UP = shift_of<T>(7.f);
+  __shared__ __attribute__((aligned(1024))) u16 K0[TILE * 128];
+  __shared__ __attribute__((aligned(1024))) u16 K1[TILE * 128];
+  __shared__ __attribute__((aligned(1024))) u16 V0[TILE * 128];
+  __shared__ __attribute__((aligned(1024))) u16 V1[TILE * 128];
+  __shared__ __attribute__((aligned(16))) int kdocs[2][TILE];
+  __shared__ uint64_t bits[ATT_WORDS];
+  __shared__ uint64_t halves[WAVES][2 * ATT_WORDS];
+
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5, n = lane & 31;
+  QueryBlock qb;
+  if (!query_block(g, ra, qb, wave, n)) return;
+  const Rules r = rules_of(ra, qb.b);
+  const bool there = qb.row < r.t_q;
+  const HeadRows qrows(g.q + qb.bh * (int64_t)r.t_q * g.hd, r.t_q, g.hd);
+  u16x8 qf[KS];
+#pragma unroll
+  for (int ds = 0; ds < KS; ds++) qf[ds] = qrows.load8(qb.row, ds * 16 + 8 * h);
+  qb.p = r.off + qb.row;
+  qb.doc = there ? query_doc(r, qb.p) : -1;
+  const int4* ranges = g.ranges ? g.ranges + qb.b * g.granules : nullptr;
+  const bool docs = ranges != nullptr;
+  const float slope2 = BIAS ? ra.slopes[qb.head] * LOG2E : 0.f;
+  const int64_t kv = (qb.b * g.kv_heads + qb.kvh) * (int64_t)r.t_k * g.hd;
+  const u16* kbase = g.k + kv;
+  const u16* vbase = g.v + kv;
+  const HeadDma4 dma(g.hd, wave, lane);
+  const SwzReads128 ad(lane);
+  const float unit = RAW ? r.c2 : 1.f, lift = RESCALE_LOG2 / unit;
+
+  f32x16 acc[DT], s[2];
+  float m = neg_inf(), l = 0.f;
+#pragma unroll
+  for (int dt = 0; dt < DT; dt++) acc[dt] = zero16();
+
+  Visit visit = key_visit(g, r, qb, ranges, bits, halves[wave], wave);
+  const int count = visit_count(visit);
+  visit.start(0);
+  int dnext = -1;
+  auto docs_load = [&](int t) __attribute__((always_inline)) {
+    if (docs && wave == 0) dnext = t * TILE + lane < r.len ? r.docs[t * TILE + lane] : -1;
+  };
+  auto docs_store = [&](int buf) __attribute__((always_inline)) {
+    if (docs && wave == 0) kdocs[buf][lane] = dnext;
+  };
+  auto scores = [&](const u16* Kt, f32x16 (&o)[2]) __attribute__((always_inline)) {
+    o[0] = zero16();
+    o[1] = zero16();
+#pragma unroll
+    for (int ds = 0; ds < KS; ds++)
+#pragma unroll
+      for (int sub = 0; sub < 2; sub++) o[sub] = T::mfma32(ad.rows(Kt, sub, ds), qf[ds], o[sub]);
+  };
+  // a tile's scores bent and masked, and the reference point moved where they pass it by more than 2^8
+  auto look = [&](f32x16 (&o)[2], int t, int buf, int alike) __attribute__((always_inline)) {
+    const float near = (float)(qb.p - t * TILE - 4 * h);
+#pragma unroll
+    for (int sub = 0; sub < 2; sub++) {
+      const int s0 = t * TILE + sub * 32;
+      if (!RAW) {
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+          float unused;
+          o[sub][i] = bend<CAP, BIAS, false>(o[sub][i], r, slope2, near - (float)(sub * 32 + 8 * (i >> 2) + (i & 3)), unused);
+        }
+      }
+      if (half_edge(r, qb, (alike >> sub) & 1, s0)) {
+        if (docs) {
+#pragma unroll
+          for (int q = 0; q < 4; q++) {
+            const int4 d4 = *(const int4*)&kdocs[buf][sub * 32 + 8 * q + 4 * h];
+            const int dd[4] = {d4.x, d4.y, d4.z, d4.w};
+#pragma unroll
+            for (int e = 0; e < 4; e++) o[sub][4 * q + e] = (qb.doc >= 0) & (dd[e] == qb.doc) ? o[sub][4 * q + e] : neg_inf();
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < 16; i++) o[sub][i] = sees(r, qb.p, s0 + 8 * (i >> 2) + 4 * h + (i & 3)) ? o[sub][i] : neg_inf();
+      }
+    }
+    float mx = neg_inf();
+#pragma unroll
+    for (int sub = 0; sub < 2; sub++)
+#pragma unroll
+      for (int i = 0; i < 16; i++) mx = fmaxf(mx, o[sub][i]);
+    mx = pair_max(mx);
+    if (__any(mx > m + lift)) {
+      const float mnew = fmaxf(m, mx);
+      const float alpha = mnew == neg_inf() ? 1.f : fast_exp2((m - mnew) * unit);
+      l *= alpha;
+#pragma unroll
+      for (int dt = 0; dt < DT; dt++) acc[dt] *= alpha;
+      m = mnew;
+    }
+  };
+  // a tile's probabilities (its scores in s) and V product, beside the next tile's scores
+  auto pipe = [&](auto has_next, const u16* Kn, const u16* Vc, int tn, int bufn, int alike) __attribute__((always_inline)) {
+    f32x16 sn[2];
+    if (decltype(has_next)::value) scores(Kn, sn);
+    const float base = (m == neg_inf() ? 0.f : m * unit) - UP;
+    float rs = 0.f;
+#pragma unroll
+    for (int sub = 0; sub < 2; sub++)
+#pragma unroll
+      for (int i = 0; i < 16; i++) {
+        const float e = RAW ? fast_exp2(fmaf(s[sub][i], unit, -base)) : fast_exp2(s[sub][i] - base);
+        s[sub][i] = e;
+        rs += e;
+      }
+    l += rs;
+#pragma unroll
+    for (int sub = 0; sub < 2; sub++)
+#pragma unroll
+      for (int c = 0; c < 2; c++) {
+        const u16x8 pb = pack8<T>(s[sub], 8 * c);
+#pragma unroll
+        for (int dt = 0; dt < DT; dt++) acc[dt] = T::mfma32(ad.transposed(Vc, sub * 32 + 16 * c, dt), pb, acc[dt]);
+      }
+    if (decltype(has_next)::value) {
+      look(sn, tn, bufn, alike);
+      s[0] = sn[0];
+      s[1] = sn[1];
+    }
+  };
+  if (count > 0) {
+    // tile it's K is in buffer it % 2 and its documents too, its V in buffer it % 2; K goes two tiles ahead, V one
+    const int t0 = visit.next(), alike0 = visit.alike;
+    int t1 = visit.next(), alike1 = visit.alike, t2 = visit.next();
+    dma.copy(K0, kbase, t0 * TILE, r.len, wave);
+    dma.copy(V0, vbase, t0 * TILE, r.len, wave);
+    dma.copy(K1, kbase, t1 * TILE, r.len, wave);
+    docs_load(t0);
+    docs_store(0);
+    docs_load(t1);
+    __builtin_amdgcn_s_waitcnt(WAIT_VMEM);
+    docs_store(1);
+    __syncthreads();
+    scores(K0, s);
+    look(s, t0, 0, alike0);
+    __syncthreads();  // every wave's reads of K buffer 0 are done before the third tile is copied there
+    // step: probabilities and V product of the tile in buffer `cur`, scores of the next
+    auto step = [&](int nextbuf, const u16* Kn, const u16* Vc, u16* Kf, u16* Vf) __attribute__((always_inline)) {
+      dma.copy(Kf, kbase, t2 * TILE, r.len, wave);
+      dma.copy(Vf, vbase, t1 * TILE, r.len, wave);
+      docs_load(t2);
+      pipe(std::true_type{}, Kn, Vc, t1, nextbuf, alike1);
+      __builtin_amdgcn_s_waitcnt(WAIT_VMEM);
+      docs_store(nextbuf ^ 1);
+      __syncthreads();
+      t1 = t2;
+      alike1 = visit.alike;
+      t2 = visit.next();
+    };
+    int it = 0;
+    for (; it + 2 < count; it += 2) {
+      step(1, K1, V0, K0, V1);
+      step(0, K0, V1, K1, V0);
+    }
+    if (it + 1 < count) {
+      step(1, K1, V0, K0, V1);
+      pipe(std::false_type{}, K0, V1, 0, 0, 0);
+    } else {
+      pipe(std::false_type{}, K0, V0, 0, 0, 0);
+    }
+  }
+  const float total = pair_sum(l);
+  const bool odd = any_odd(acc);  // a barrier: the tile buffers become staging below
+  if (threadIdx.x == 0) g.odd[qb.bh * qb.nqb + qb.q0 / ATT_ROWS] = odd;
+  const float inv = total == 0.f ? 0.f : 1.f / total;  // a row that sees nothing is a row of zeros
+  u16* stage = wave == 0 ? K0 : wave == 1 ? K1 : wave == 2 ? V0 : V1;
+  store_rows<T, D>(g.o0 + qb.bh * (int64_t)r.t_q * g.hd, acc, qb.wq0, r.t_q, g.hd, inv, stage);
+  if (h == 0 && there) g.lse[qb.bh * (int64_t)r.t_q + qb.row] = total == 0.f ? neg_inf() : (m * unit - UP) * ATT_LN2 + logf(total);
+#endif
+}
+
+template <typename T, int D, bool CAP, bool BIAS>
+__global__ __launch_bounds__(THREADS, 2) void attend_dq_wide(FastArgs g, RuleArgs ra) {
+#if defined(__HIP_DEVICE_COMPILE__)  // the host pass needs the stub alone
+  constexpr bool RAW = !CAP && !BIAS;
+  constexpr int KS = D / 16, DT = D / 32;
+  __shared__ __attribute__((aligned(1024))) u16 K0[TILE * 128];
+  __shared__ __attribute__((aligned(1024))) u16 K1[TILE * 128];
+  __shared__ __attribute__((aligned(1024))) u16 V0[TILE * 128];
+  __shared__ __attribute__((aligned(1024))) u16 V1[TILE * 128];
+  __shared__ __attribute__((aligned(16))) int kdocs[2][TILE];
+  __shared__ uint64_t bits[ATT_WORDS];
+  __shared__ uint64_t halves[WAVES][2 * ATT_WORDS];
+
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5, n = lane & 31;
+  QueryBlock qb;
+  if (!query_block(g, ra, qb, wave, n)) return;
+  const Rules r = rules_of(ra, qb.b);
+  const bool there = qb.row < r.t_q;
+  const int64_t rows0 = qb.bh * (int64_t)r.t_q;
+  const HeadRows qrows(g.q + rows0 * g.hd, r.t_q, g.hd), grows(g.dout + rows0 * g.hd, r.t_q, g.hd), orows(g.out + rows0 * g.hd, r.t_q, g.hd);
+  u16x8 qf[KS], of[KS];
+  float delta = 0.f;
+#pragma unroll
+  for (int ds = 0; ds < KS; ds++) {
+    qf[ds] = qrows.load8(qb.row, ds * 16 + 8 * h);
+    of[ds] = grows.load8(qb.row, ds * 16 + 8 * h);
+    const u16x8 o = orows.load8(qb.row, ds * 16 + 8 * h);
+#pragma unroll
+    for (int e = 0; e < 8; e++) delta = fmaf(T::unpack(of[ds][e]), T::unpack(o[e]), delta);
+  }
+  delta = pair_sum(delta);
+  if (h == 0 && there) g.delta[rows0 + qb.row] = delta;
+  const float l2 = there ? att_l2(g.lse_in[rows0 + qb.row]) : __builtin_inff();
+  qb.p = r.off + qb.row;
+  qb.doc = there ? query_doc(r, qb.p) : -1;
+  const int4* ranges = g.ranges ? g.ranges + qb.b * g.granules : nullptr;
+  const bool docs = ranges != nullptr;
+  const float slope2 = BIAS ? ra.slopes[qb.head] * LOG2E : 0.f;
+  const int64_t kv = (qb.b * g.kv_heads + qb.kvh) * (int64_t)r.t_k * g.hd;
+  const u16* kbase = g.k + kv;
+  const u16* vbase = g.v + kv;
+  const HeadDma4 dma(g.hd, wave, lane);
+  const SwzReads128 ad(lane);
+
+  f32x16 acc[DT];
+#pragma unroll
+  for (int dt = 0; dt < DT; dt++) acc[dt] = zero16();
+
+  Visit visit = key_visit(g, r, qb, ranges, bits, halves[wave], wave);
+  const int count = visit_count(visit);
+  visit.start(0);
+  int dnext = -1;
+  auto docs_load = [&](int t) __attribute__((always_inline)) {
+    if (docs && wave == 0) dnext = t * TILE + lane < r.len ? r.docs[t * TILE + lane] : -1;
+  };
+  auto docs_store = [&](int buf) __attribute__((always_inline)) {
+    if (docs && wave == 0) kdocs[buf][lane] = dnext;
+  };
+  int cur = visit.next(), alike = visit.alike, nxt = visit.next();
+  auto tile = [&](int buf, const u16* Kt, const u16* Vt) __attribute__((always_inline)) {
+#pragma unroll
+    for (int sub = 0; sub < 2; sub++) {
+      const int s0 = cur * TILE + sub * 32;
+      f32x16 s = zero16(), dp = zero16();
+#pragma unroll
+      for (int ds = 0; ds < KS; ds++) {
+        s = T::mfma32(ad.rows(Kt, sub, ds), qf[ds], s);
+        dp = T::mfma32(ad.rows(Vt, sub, ds), of[ds], dp);
+      }
+      const float near = (float)(qb.p - s0 - 4 * h);
+      unsigned gp[8];  // packed operands, in two instances: with element tests and without
+      auto soft = [&](auto tests) __attribute__((always_inline)) {
+        int4 d4 = {0, 0, 0, 0};
+        float first = 0.f;
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+          if (decltype(tests)::value && docs && (i & 3) == 0) d4 = *(const int4*)&kdocs[buf][sub * 32 + 8 * (i >> 2) + 4 * h];
+          float bent = 1.f;
+          const float y = bend<CAP, BIAS, true>(s[i], r, slope2, near - (float)(8 * (i >> 2) + (i & 3)), bent);
+          const float e = fast_exp2(RAW ? fmaf(y, r.c2, -l2) : y - l2);
+          float d = e * (dp[i] - delta) * (CAP ? bent : 1.f);  // times scale once, at the store
+          if (decltype(tests)::value) {
+            const int kd = (i & 3) == 0 ? d4.x : (i & 3) == 1 ? d4.y : (i & 3) == 2 ? d4.z : d4.w;
+            d = (qb.doc >= 0) & (kd == qb.doc) & sees(r, qb.p, s0 + 8 * (i >> 2) + 4 * h + (i & 3)) ? d : 0.f;
+          }
+          if (i & 1)
+            gp[i >> 1] = T::pack2(first, d);
+          else
+            first = d;
+        }
+      };
+      if (half_edge(r, qb, (alike >> sub) & 1, s0))
+        soft(std::true_type{});
+      else
+        soft(std::false_type{});
+#pragma unroll
+      for (int c = 0; c < 2; c++) {
+        const u32x4 w = {gp[4 * c], gp[4 * c + 1], gp[4 * c + 2], gp[4 * c + 3]};
+        const u16x8 gb = __builtin_bit_cast(u16x8, w);
+#pragma unroll
+        for (int dt = 0; dt < DT; dt++) acc[dt] = T::mfma32(ad.transposed(Kt, sub * 32 + 16 * c, dt), gb, acc[dt]);
+      }
+    }
+  };
+  auto step = [&](int buf, const u16* Kc, const u16* Vc, u16* Kn, u16* Vn) __attribute__((always_inline)) {
+    dma.copy(Kn, kbase, nxt * TILE, r.len, wave);
+    dma.copy(Vn, vbase, nxt * TILE, r.len, wave);
+    docs_load(nxt);
+    tile(buf, Kc, Vc);
+    __builtin_amdgcn_s_waitcnt(WAIT_VMEM);
+    docs_store(buf ^ 1);
+    __syncthreads();
+    cur = nxt;
+    alike = visit.alike;
+    nxt = visit.next();
+  };
+  if (count > 0) {
+    dma.copy(K0, kbase, cur * TILE, r.len, wave);
+    dma.copy(V0, vbase, cur * TILE, r.len, wave);
+    docs_load(cur);
+    __builtin_amdgcn_s_waitcnt(WAIT_VMEM);
+    docs_store(0);
+    __syncthreads();
+    int it = 0;
+    for (; it + 1 < count; it += 2) {
+      step(0, K0, V0, K1, V1);
+      step(1, K1, V1, K0, V0);
+    }
+    if (it < count) step(0, K0, V0, K1, V1);
+  }
+  const bool odd = any_odd(acc);  // a barrier: the tile buffers become staging below
+  if (threadIdx.x == 0) g.odd[qb.bh * qb.nqb + qb.q0 / ATT_ROWS] = odd;
+  u16* stage = wave == 0 ? K0 : wave == 1 ? K1 : wave == 2 ? V0 : V1;
+  store_rows<T, D>(g.o0 + rows0 * g.hd, acc, qb.wq0, r.t_q, g.hd, g.scale, stage);
+#endif
+}
+
 // ---- launches -------------------------------------------------------------------------------------------
 
 enum AttendPass { ATTEND_PASS_FWD, ATTEND_PASS_DQ, ATTEND_PASS_DKV };
@@ -1020,7 +1427,11 @@ int launch_fast_as(const FastArgs& g, const RuleArgs& ra, hipStream_t stream) {
                                                  : att_grid(g.batch * g.heads, (ra.t_q + ATT_ROWS - 1) / ATT_ROWS, g.head_group);
   if (blocks > 0x7fffffff) return fail(LIMN_HIP_EUNSUPPORTED, "attend: %lld workgroups exceed one launch", (long long)blocks);
   const dim3 grid((unsigned)blocks), block(THREADS);
-  if constexpr (PASS == ATTEND_PASS_FWD)
+  if constexpr (PASS == ATTEND_PASS_FWD && D > 64)
+    hipLaunchKernelGGL((attend_fwd_wide<T, D, CAP, BIAS>), grid, block, 0, stream, g, ra);
+  else if constexpr (PASS == ATTEND_PASS_DQ && D > 64)
+    hipLaunchKernelGGL((attend_dq_wide<T, D, CAP, BIAS>), grid, block, 0, stream, g, ra);
+  else if constexpr (PASS == ATTEND_PASS_FWD)
     hipLaunchKernelGGL((attend_fwd_mfma<T, D, CAP, BIAS>), grid, block, 0, stream, g, ra);
   else if constexpr (PASS == ATTEND_PASS_DQ)
     hipLaunchKernelGGL((attend_dq_mfma<T, D, CAP, BIAS>), grid, block, 0, stream, g, ra);
