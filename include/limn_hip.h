@@ -243,7 +243,9 @@ int64_t limn_hip_attend_workspace(int dtype, int64_t batch, int64_t heads, int64
  * The logits are never kept: the vocabulary goes by in pieces. A target outside [0, vocab) leaves its row
  * out: loss 0, no gradient, and what the row holds reaches nothing.
  *   x (rows, width) and w (vocab, width) of float32, float16 or bfloat16, targets (rows) int32; loss and lse
- *   (rows) float32. Sums and statistics are float32.
+ *   (rows) float32. Sums and statistics are float32. float32 operands are multiplied as sums of three bfloat16
+ *   numbers each: a product x w is exact to some 2^-24 |x w| + 2^-134 (|x| + |w|), and an infinity among the
+ *   operands of a row that has a target makes it NaN.
  * Workspace as for limn_hip_attend_fwd, of limn_hip_xent_workspace(...) bytes. No counterpart in the reference,
  * whose training example takes log_softmax of the logits (examples/train_stories.py:61-64).
  */

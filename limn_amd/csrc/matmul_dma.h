@@ -1,5 +1,5 @@
 // Operands of the contraction kernels that go from memory straight into LDS (buffer_load ... lds), in the
-// swizzled tiles that matmul.hip describes. Shared by matmul.hip and the cross entropy's products (xent_half.hip).
+// swizzled tiles that matmul.hip describes. Shared by matmul.hip and the cross entropy's products (xent_tiles.hip).
 #pragma once
 
 #include "matmul.h"

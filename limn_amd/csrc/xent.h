@@ -1,5 +1,4 @@
-// Internal launch interface of the head's cross entropy: float32 arithmetic for every case (xent_wide.hip) and half
-// widths on 16-bit matrix cores (xent_half.hip).
+// Internal launch interface of the head's cross entropy (xent_tiles.hip).
 #pragma once
 
 #include "matmul.h"
@@ -36,14 +35,9 @@ struct XentSpace {
   }
 };
 
-bool xent_wide_ok(const XentArgs& a);  // whether the sizes fit the kernels' 32-bit offsets
-int64_t xent_wide_workspace(const XentArgs& a, bool backward);
-int launch_xent_wide_fwd(const XentArgs& a);
-int launch_xent_wide_bwd(const XentArgs& a);
-
-bool xent_half_sizes(const XentArgs& a);
-int64_t xent_half_workspace(const XentArgs& a, bool backward);
-int launch_xent_half_fwd(const XentArgs& a);
-int launch_xent_half_bwd(const XentArgs& a);
+bool xent_sizes_ok(const XentArgs& a);  // whether the sizes fit the kernels' 32-bit offsets
+int64_t xent_workspace(const XentArgs& a, bool backward);
+int launch_xent_fwd(const XentArgs& a);
+int launch_xent_bwd(const XentArgs& a);
 
 }  // namespace limn

@@ -1,4 +1,4 @@
-// The C ABI of the head's cross entropy (include/limn_hip.h): argument checks and choice of kernels.
+// The C ABI of the head's cross entropy (include/limn_hip.h): argument checks.
 
 #include "xent.h"
 
@@ -11,21 +11,9 @@ int check_xent(const char* name, const XentArgs& a) {
   if (a.rows < 1 || a.width < 1 || a.vocab < 1)
     return fail(LIMN_HIP_EINVAL, "%s: sizes must be positive (rows %lld, width %lld, vocab %lld)", name, (long long)a.rows, (long long)a.width,
                 (long long)a.vocab);
-  if (a.vocab > 0x7fffffff || a.rows > ((int64_t)1 << 40) / a.width || a.vocab > ((int64_t)1 << 40) / a.width || !xent_wide_ok(a))
+  if (a.vocab > 0x7fffffff || a.rows > ((int64_t)1 << 40) / a.width || a.vocab > ((int64_t)1 << 40) / a.width || !xent_sizes_ok(a))
     return fail(LIMN_HIP_EUNSUPPORTED, "%s: sizes out of range (operands reach past 2 GiB)", name);
   return LIMN_HIP_OK;
-}
-
-// A call of sizes the half-width kernels serve goes to them where its operands are 16-byte aligned.
-bool half_call(const XentArgs& a, bool backward) {
-  const uintptr_t at = (uintptr_t)a.x | (uintptr_t)a.w | (backward ? (uintptr_t)a.o0 | (uintptr_t)a.o1 : 0);
-  return xent_half_sizes(a) && at % 16 == 0;
-}
-
-// Enough for whichever kernels the call's buffers allow.
-int64_t workspace_of(const XentArgs& a, bool backward) {
-  const int64_t wide = xent_wide_workspace(a, backward), half = xent_half_sizes(a) ? xent_half_workspace(a, backward) : 0;
-  return wide > half ? wide : half;
 }
 
 int check_call(const char* name, const XentArgs& a, bool backward) {
@@ -36,7 +24,7 @@ int check_call(const char* name, const XentArgs& a, bool backward) {
   const uintptr_t size = a.dtype == LIMN_HIP_FLOAT32 ? 4 : 2, outs = (uintptr_t)a.o0 | (uintptr_t)a.o1;
   if (((uintptr_t)a.x | (uintptr_t)a.w) % size != 0 || outs % (backward ? size : 4) != 0 || ((uintptr_t)a.targets | (uintptr_t)a.lse_in | (uintptr_t)a.g) % 4 != 0)
     return fail(LIMN_HIP_EINVAL, "%s: buffers must be aligned to their element size", name);
-  const int64_t need = workspace_of(a, backward);
+  const int64_t need = xent_workspace(a, backward);
   if (a.workspace == nullptr || a.workspace_bytes < need || (uintptr_t)a.workspace % 16 != 0)
     return fail(LIMN_HIP_EINVAL, "%s: needs a workspace of %lld bytes, 16-byte aligned", name, (long long)need);
   return LIMN_HIP_OK;
@@ -52,15 +40,14 @@ extern "C" {
 int64_t limn_hip_xent_workspace(int dtype, int64_t rows, int64_t width, int64_t vocab, int backward) {
   XentArgs a = {};
   a.dtype = dtype, a.rows = rows, a.width = width, a.vocab = vocab;
-  return check_xent("xent_workspace", a) == LIMN_HIP_OK ? workspace_of(a, backward != 0) : 0;
+  return check_xent("xent_workspace", a) == LIMN_HIP_OK ? xent_workspace(a, backward != 0) : 0;
 }
 
 int limn_hip_xent_fwd(const void* x, const void* w, const void* targets, void* loss, void* lse, int dtype, int64_t rows, int64_t width,
                       int64_t vocab, void* workspace, int64_t workspace_bytes, void* stream) {
   const XentArgs a = {x, w, (const int*)targets, nullptr, nullptr, loss, lse, dtype, rows, width, vocab, workspace, workspace_bytes, (hipStream_t)stream};
   const int rc = check_call("xent_fwd", a, false);
-  if (rc != LIMN_HIP_OK) return rc;
-  return half_call(a, false) ? launch_xent_half_fwd(a) : launch_xent_wide_fwd(a);
+  return rc != LIMN_HIP_OK ? rc : launch_xent_fwd(a);
 }
 
 int limn_hip_xent_bwd(const void* x, const void* w, const void* targets, const void* lse, const void* g, void* dx, void* dw, int dtype,
@@ -68,8 +55,7 @@ int limn_hip_xent_bwd(const void* x, const void* w, const void* targets, const v
   const XentArgs a = {x, w, (const int*)targets, (const float*)lse, (const float*)g, dx, dw, dtype, rows, width, vocab, workspace, workspace_bytes,
                       (hipStream_t)stream};
   const int rc = check_call("xent_bwd", a, true);
-  if (rc != LIMN_HIP_OK) return rc;
-  return half_call(a, true) ? launch_xent_half_bwd(a) : launch_xent_wide_bwd(a);
+  return rc != LIMN_HIP_OK ? rc : launch_xent_bwd(a);
 }
 
 }  // extern "C"

@@ -1,4 +1,13 @@
-// The head's cross entropy on 16-bit matrix cores: bf16/f16, width a multiple of 8, 16-byte aligned operands.
+// The head's cross entropy on 16-bit matrix cores.
+//
+// bf16 and f16 operands go as they are, or, where their rows are not 16-byte aligned or the width is no multiple of
+// 8, from copies padded with zeros. float32 operands go as three bf16 parts each, x = h + m + l with h the
+// nearest bf16 to x, m to x - h, l to the rest (8 + 8 + 8 bits and the parts' signs: x to 2^-24 or better, down to
+// half of bf16's least step, 2^-134), and a
+// product of two numbers as the six products of parts that are not below 2^-24 of it: h h, h m, m h, m m, h l, l h,
+// the smallest first (the splitting published as BF16x6: Henry, Tang, Heinecke, Leveraging the bfloat16
+// artificial intelligence datatype for higher-precision computations, 2019). 6 products at the 16-bit rate are
+// 2.6 times as fast as one at the float32 matrix rate (157 TFLOP/s); the sums are float32 either way.
 //
 // Four products, each on the tiles and the LDS pipeline of matmul.hip (256 x 256 tiles by 8 waves, or 128 x 128 by
 // 4 where the larger would leave compute units idle; operands from memory straight into swizzled LDS, the
@@ -13,6 +22,8 @@
 //    The piece (at most PIECE_BYTES of dz) is small enough that both products find most of it in the 256 MiB
 //    last-level cache.
 // Keeping the logits would save the second x w^T, a quarter of the matrix work, for rows * vocab * 4 bytes.
+//
+// Every operand is PARTS matrices of one shape, one part_a or part_b elements behind another (1 or 3).
 //
 // A row without a target has dz = 0; what its x holds reaches nothing (see Products and the flags of xent_dz).
 
@@ -52,12 +63,20 @@ struct Tile {
 
 #if defined(__HIP_DEVICE_COMPILE__)  // what the host pass, which only needs the kernels' stubs, cannot instantiate
 
-// The last stage of a k-contiguous operand whose depth is no multiple of 64: chunks past it read as zeros
-// (elsewhere they are the next row's elements).
+// The operand copy of DmaOperand from `shift` bytes on; last: the stage at which a k-contiguous operand's depth
+// ends, whose chunks past it read as zeros (elsewhere they are the next row's elements).
 template <int WAVES, typename D>
-__device__ __forceinline__ void copy_last(const D& d, char* tile, int st, int depth, int wave, int lane) {
+__device__ __forceinline__ void copy_from(const D& d, int64_t shift, char* tile, int st, int wave) {
   const int64_t off = (d.first + st) * d.step, left = d.extent - off;
-  const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc((void*)(d.base + off), (short)0, (int)(left > 0 ? left : 0), 0x00020000);
+  const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc((void*)(d.base + shift + off), (short)0, (int)(left > 0 ? left : 0), 0x00020000);
+#pragma unroll
+  for (int q = 0; q < D::PASSES; q++)
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_void*)(tile + (q * WAVES + wave) * 1024), 16, d.voff[q], 0, 0, 0);
+}
+template <int WAVES, typename D>
+__device__ __forceinline__ void copy_last(const D& d, int64_t shift, char* tile, int st, int depth, int wave, int lane) {
+  const int64_t off = (d.first + st) * d.step, left = d.extent - off;
+  const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc((void*)(d.base + shift + off), (short)0, (int)(left > 0 ? left : 0), 0x00020000);
   const int live = depth - (int)(d.first + st) * BK;  // elements of this stage that are there
 #pragma unroll
   for (int q = 0; q < D::PASSES; q++) {
@@ -66,11 +85,12 @@ __device__ __forceinline__ void copy_last(const D& d, char* tile, int st, int de
   }
 }
 
-// acc = sum over `stages` stages of k; `depth`: the depth at which k-contiguous operands end (TAIL). fix(tile of
-// b, stage) runs between a stage's arrival and its first read, with a barrier before it and, if it returns true, behind it.
-template <typename T, int BM, bool A_K, bool B_K, bool TAIL, typename DA, typename DB, typename FIX>
-__device__ __forceinline__ void tile_product(const DA& da, const DB& db, char* A0, char* A1, char* B0, char* B1, int stages, int depth, int wave, int lane,
-                                             f32x16 (*acc)[Tile<BM>::TN], FIX fix) {
+// acc = sum over `depth_stages` stages of k, for every pair of parts in turn, the smallest products first; `depth`:
+// where k-contiguous operands end (TAIL). fix(tile of b, stage) runs between a stage's arrival and its first
+// read, with a barrier before it and, if it returns true, behind it.
+template <typename T, int BM, int PARTS, bool A_K, bool B_K, bool TAIL, typename DA, typename DB, typename FIX>
+__device__ __forceinline__ void tile_product(const DA& da, const DB& db, int64_t part_a, int64_t part_b, char* A0, char* A1, char* B0, char* B1,
+                                             int depth_stages, int depth, int wave, int lane, f32x16 (*acc)[Tile<BM>::TN], FIX fix) {
   using L = Tile<BM>;
   constexpr int TM = L::TM, TN = L::TN, KS = L::KS;
   const int wm = wave / L::WN, wn = wave % L::WN;
@@ -84,23 +104,34 @@ __device__ __forceinline__ void tile_product(const DA& da, const DB& db, char* A
 #pragma unroll
     for (int j = 0; j < TN; j++) bo[j] = db.operand(bt, rdb, j, kk);
   };
-  auto copy = [&](char* at, char* bt, int st) __attribute__((always_inline)) {
+  // stages are copied in order: `at` is the next one's place in its pair of parts, `pair` the pair
+  int at = 0, pair = 0;
+  const int stages = PARTS == 3 ? 6 * depth_stages : depth_stages;
+  auto copy = [&](char* an, char* bn) __attribute__((always_inline)) {
+    // l h, h l, m m, m h, h m, h h: four bits a pair, the first lowest
+    const int64_t sa = PARTS == 3 ? ((0x001102 >> (4 * pair)) & 15) * part_a * 2 : 0, sb = PARTS == 3 ? ((0x010120 >> (4 * pair)) & 15) * part_b * 2 : 0;
+    bool done = false;
     if constexpr (TAIL) {
-      if (st == stages - 1) {
-        copy_last<L::WAVES>(da, at, st, depth, wave, lane);
-        copy_last<L::WAVES>(db, bt, st, depth, wave, lane);
-        return;
+      if (at == depth_stages - 1) {
+        copy_last<L::WAVES>(da, sa, an, at, depth, wave, lane);
+        copy_last<L::WAVES>(db, sb, bn, at, depth, wave, lane);
+        done = true;
       }
     }
-    da.copy(at, st, wave);
-    db.copy(bt, st, wave);
+    if (!done) {
+      copy_from<L::WAVES>(da, sa, an, at, wave);
+      copy_from<L::WAVES>(db, sb, bn, at, wave);
+    }
+    at++;
+    if (PARTS == 3 && at == depth_stages && pair < 5) at = 0, pair++;
   };
-  auto stage = [&](const char* at, const char* bt, char* an, char* bn, int st) __attribute__((always_inline)) {
-    copy(an, bn, st + 1);
+  auto stage = [&](const char* at_, const char* bt, char* an, char* bn, int st) __attribute__((always_inline)) {
+    const int coming = at;
+    copy(an, bn);
 #pragma unroll
     for (int kk = 0; kk < KS; kk++) {
       const int p = kk & 1;
-      if (kk + 1 < KS) read(at, bt, kk + 1, av[p ^ 1], bv[p ^ 1]);
+      if (kk + 1 < KS) read(at_, bt, kk + 1, av[p ^ 1], bv[p ^ 1]);
 #pragma unroll
       for (int i = 0; i < TM; i++)
 #pragma unroll
@@ -122,14 +153,14 @@ __device__ __forceinline__ void tile_product(const DA& da, const DB& db, char* A
     }
     __builtin_amdgcn_s_waitcnt(WAIT_VMEM);
     __syncthreads();
-    if (st + 1 < stages && fix(bn, st + 1)) __syncthreads();
+    if (st + 1 < stages && fix(bn, coming)) __syncthreads();
     read(an, bn, 0, av[0], bv[0]);
   };
 #pragma unroll
   for (int i = 0; i < TM; i++)
 #pragma unroll
     for (int j = 0; j < TN; j++) acc[i][j] = zero16();
-  copy(A0, B0, 0);
+  copy(A0, B0);
   __builtin_amdgcn_s_waitcnt(WAIT_VMEM);
   __syncthreads();
   if (fix(B0, 0)) __syncthreads();
@@ -163,6 +194,7 @@ struct Logits {
   const u16* w;         // the piece's rows
   const int* targets;
   int64_t rows, width, piece, vocab, v0;
+  int64_t part_x, part_w;  // elements between the parts
   // forward
   float2* stats;        // (tiles of columns, rows): largest logit, sum of exponentials against it
   float* picked;        // (rows): the target's logit
@@ -170,8 +202,8 @@ struct Logits {
   // backward
   const float* lse;
   const float* g;
-  u16* dz;              // (padded rows, ldz)
-  int64_t ldz;
+  u16* dz;              // (PARTS, padded rows, ldz)
+  int64_t ldz, part_dz;
   int* flags;           // one a 64 rows: a row without a target has logits that are not finite
 };
 
@@ -187,7 +219,7 @@ struct Logits {
 
 // ---- forward: a tile of logits into its rows' statistics ------------------------------------------------------
 
-template <typename T, int BM, bool TAIL>
+template <typename T, int BM, int PARTS, bool TAIL>
 __global__ __launch_bounds__(64 * Tile<BM>::WAVES, 2) void xent_stats(Logits a) {
 #if defined(__HIP_DEVICE_COMPILE__)
   LIMN_XENT_LDS(BM)
@@ -197,7 +229,7 @@ __global__ __launch_bounds__(64 * Tile<BM>::WAVES, 2) void xent_stats(Logits a) 
   const int64_t m0 = tm * BM, n0 = tn * BM;
   const DmaOperand<BM, true, L::WAVES> da(a.x, a.rows, a.width, a.width, m0, 0, wave, lane), db(a.w, a.piece, a.width, a.width, n0, 0, wave, lane);
   f32x16 acc[L::TM][L::TN];
-  tile_product<T, BM, true, true, TAIL>(da, db, A0, A1, B0, B1, (int)((a.width + BK - 1) / BK), (int)a.width, wave, lane, acc, no_fix);
+  tile_product<T, BM, PARTS, true, true, TAIL>(da, db, a.part_x, a.part_w, A0, A1, B0, B1, (int)((a.width + BK - 1) / BK), (int)a.width, wave, lane, acc, no_fix);
 
   // lane: rows 32 i + n32 of the wave, columns 32 j + 8 q + 4 h + e in items 4 q + e
   const int64_t col0 = n0 + wn * 64;
@@ -293,7 +325,7 @@ __global__ __launch_bounds__(256) void xent_rows(const float2* __restrict__ stat
 
 // ---- backward: a tile of logits into dz -------------------------------------------------------------------
 
-template <typename T, int BM, bool TAIL>
+template <typename T, int BM, int PARTS, bool TAIL>
 __global__ __launch_bounds__(64 * Tile<BM>::WAVES, 2) void xent_dz(Logits a) {
 #if defined(__HIP_DEVICE_COMPILE__)
   LIMN_XENT_LDS(BM)
@@ -303,7 +335,7 @@ __global__ __launch_bounds__(64 * Tile<BM>::WAVES, 2) void xent_dz(Logits a) {
   const int64_t m0 = tm * BM, n0 = tn * BM;
   const DmaOperand<BM, true, L::WAVES> da(a.x, a.rows, a.width, a.width, m0, 0, wave, lane), db(a.w, a.piece, a.width, a.width, n0, 0, wave, lane);
   f32x16 acc[L::TM][L::TN];
-  tile_product<T, BM, true, true, TAIL>(da, db, A0, A1, B0, B1, (int)((a.width + BK - 1) / BK), (int)a.width, wave, lane, acc, no_fix);
+  tile_product<T, BM, PARTS, true, true, TAIL>(da, db, a.part_x, a.part_w, A0, A1, B0, B1, (int)((a.width + BK - 1) / BK), (int)a.width, wave, lane, acc, no_fix);
 
   const int64_t col0 = n0 + wn * 64;
   __syncthreads();
@@ -315,39 +347,54 @@ __global__ __launch_bounds__(64 * Tile<BM>::WAVES, 2) void xent_dz(Logits a) {
   char* const region = (wave < 4 ? A0 : A1) + (wave & 3) * (BM == 256 ? 8192 : 4096);
   constexpr int PASS = BM == 256 ? 2 : 1;  // 32-row blocks a pass
 #pragma unroll
-  for (int p = 0; p < L::TM / PASS; p++) {
+  for (int i = 0; i < L::TM; i++) {
+    const int64_t row = m0 + wm * L::WTM + 32 * i + n32;
+    const int t32 = row < a.rows ? a.targets[row] : -1;
+    const bool live = t32 >= 0 && t32 < a.vocab;
+    const int64_t t = (int64_t)t32 - a.v0 - col0;
+    const float l2 = live ? a.lse[row] * LOG2E : 0.f, g = live ? a.g[row] : 0.f;
+    bool bad = false;
 #pragma unroll
-    for (int ii = 0; ii < PASS; ii++) {
-      const int i = p * PASS + ii;
-      const int64_t row = m0 + wm * L::WTM + 32 * i + n32;
-      const int t32 = row < a.rows ? a.targets[row] : -1;
-      const bool live = t32 >= 0 && t32 < a.vocab;
-      const int64_t t = (int64_t)t32 - a.v0 - col0;
-      const float l2 = live ? a.lse[row] * LOG2E : 0.f, g = live ? a.g[row] : 0.f;
-      bool bad = false;
+    for (int j = 0; j < L::TN; j++)
 #pragma unroll
-      for (int j = 0; j < L::TN; j++)
+      for (int e = 0; e < 16; e++) {
+        const int c = 32 * j + 8 * (e >> 2) + 4 * h + (e & 3);
+        const float z = acc[i][j][e];
+        bad |= !(fabsf(z) <= 3.402823466e38f);
+        const float d = g * (fast_exp2(fmaf(z, LOG2E, -l2)) - (c == t ? 1.f : 0.f));
+        acc[i][j][e] = live && col0 + c < a.piece ? d : 0.f;
+      }
+    if (bad && !live && row < a.rows) odd[(row - m0) / 64] = 1;  // every writer writes 1
+  }
 #pragma unroll
-        for (int q = 0; q < 4; q++) {
-          float v[4];
+  for (int part = 0; part < PARTS; part++) {
 #pragma unroll
-          for (int e = 0; e < 4; e++) {
-            const int c = 32 * j + 8 * q + 4 * h + e;
-            const float z = acc[i][j][4 * q + e];
-            bad |= !(fabsf(z) <= 3.402823466e38f);
-            const float d = g * (fast_exp2(fmaf(z, LOG2E, -l2)) - (c == t ? 1.f : 0.f));
-            v[e] = live && col0 + c < a.piece ? d : 0.f;
+    for (int p = 0; p < L::TM / PASS; p++) {
+#pragma unroll
+      for (int ii = 0; ii < PASS; ii++) {
+        const int i = p * PASS + ii, r = ii * 32 + n32;
+#pragma unroll
+        for (int j = 0; j < L::TN; j++)
+#pragma unroll
+          for (int q = 0; q < 4; q++) {
+            uint2 w;
+            w.x = T::pack2(acc[i][j][4 * q], acc[i][j][4 * q + 1]);
+            w.y = T::pack2(acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]);
+            if (part + 1 < PARTS) {  // what is left for the next part
+              acc[i][j][4 * q] -= T::unpack((u16)w.x);
+              acc[i][j][4 * q + 1] -= T::unpack((u16)(w.x >> 16));
+              acc[i][j][4 * q + 2] -= T::unpack((u16)w.y);
+              acc[i][j][4 * q + 3] -= T::unpack((u16)(w.y >> 16));
+            }
+            *(uint2*)(region + r * 128 + ((4 * j + q) ^ ((r >> 1) & 7)) * 16 + 8 * h) = w;
           }
-          const int r = ii * 32 + n32;
-          *(uint2*)(region + r * 128 + ((4 * j + q) ^ ((r >> 1) & 7)) * 16 + 8 * h) = make_uint2(T::pack2(v[0], v[1]), T::pack2(v[2], v[3]));
-        }
-      if (bad && !live && row < a.rows) odd[(row - m0) / 64] = 1;  // every writer writes 1
-    }
+      }
 #pragma unroll
-    for (int it = 0; it < PASS * 4; it++) {
-      const int r = it * 8 + lane / 8, cc = lane & 7;
-      const u32x4 s = *(const u32x4*)(region + r * 128 + (cc ^ ((r >> 1) & 7)) * 16);
-      *(u32x4*)(a.dz + (m0 + wm * L::WTM + p * PASS * 32 + r) * a.ldz + col0 + cc * 8) = s;
+      for (int it = 0; it < PASS * 4; it++) {
+        const int r = it * 8 + lane / 8, cc = lane & 7;
+        const u32x4 s = *(const u32x4*)(region + r * 128 + (cc ^ ((r >> 1) & 7)) * 16);
+        *(u32x4*)(a.dz + part * a.part_dz + (m0 + wm * L::WTM + p * PASS * 32 + r) * a.ldz + col0 + cc * 8) = s;
+      }
     }
   }
   if (tn == 0) {
@@ -367,9 +414,12 @@ struct Products {
   const u16* b;
   int64_t m, n, k;       // of the result and of the padded contraction
   int64_t a_rows, a_depth, a_stride;
-  int64_t b_depth, b_stride;
+  int64_t b_depth, b_stride, b_cols;
+  int64_t part_a, part_b;
   int64_t chunk;
-  u16* out;              // of half width, row stride n; or nullptr:
+  int64_t width;         // columns of the result that there are: n rounds them up to a multiple of 8
+  void* out;             // (m, width) of the result's type; or nullptr:
+  int out_f32, vec;      // its type; whether its rows take vector stores
   float* wide;           // (slices, m, n) float32
   const float* add;      // (m, n) float32 added to an unsplit result, or nullptr
   const int* flags;      // dw: see xent_dz; a flagged stage's rows of x without a target are taken as zeros
@@ -377,7 +427,32 @@ struct Products {
   int64_t rows, vocab;
 };
 
-template <typename T, int BM, bool A_K>
+// 4 columns of a result's row; columns past the width are padding and not stored
+template <typename T>
+__device__ __forceinline__ void store4(const Products& s, int64_t row, int64_t col, f32x4 v) {
+  if (col >= s.width) return;
+  if (s.out_f32) {
+    float* o = (float*)s.out + row * s.width + col;
+    if (s.vec) {
+      *(f32x4*)o = v;
+      return;
+    }
+#pragma unroll
+    for (int e = 0; e < 4; e++)
+      if (col + e < s.width) o[e] = v[e];
+    return;
+  }
+  u16* o = (u16*)s.out + row * s.width + col;
+  if (s.vec) {
+    *(uint2*)o = make_uint2(T::pack2(v[0], v[1]), T::pack2(v[2], v[3]));
+    return;
+  }
+#pragma unroll
+  for (int e = 0; e < 4; e++)
+    if (col + e < s.width) o[e] = T::pack(v[e]);
+}
+
+template <typename T, int BM, int PARTS, bool A_K>
 __global__ __launch_bounds__(64 * Tile<BM>::WAVES, 2) void xent_product(Products s) {
 #if defined(__HIP_DEVICE_COMPILE__)
   LIMN_XENT_LDS(BM)
@@ -386,7 +461,7 @@ __global__ __launch_bounds__(64 * Tile<BM>::WAVES, 2) void xent_product(Products
   tile_of(tiles_m, tiles_n, tm, tn, slice);
   const int64_t m0 = tm * BM, n0 = tn * BM, k_lo = slice * s.chunk, k_hi = k_lo + s.chunk < s.k ? k_lo + s.chunk : s.k;
   const DmaOperand<BM, A_K, L::WAVES> da(s.a, s.a_rows, s.a_depth, s.a_stride, m0, k_lo, wave, lane);
-  const DmaOperand<BM, false, L::WAVES> db(s.b, s.n, s.b_depth, s.b_stride, n0, k_lo, wave, lane);
+  const DmaOperand<BM, false, L::WAVES> db(s.b, s.b_cols, s.b_depth, s.b_stride, n0, k_lo, wave, lane);
   f32x16 acc[L::TM][L::TN];
   // an infinity or a NaN in a row of x without a target meets a dz of 0, which would be NaN: such rows of the
   // tile are overwritten with zeros (only where xent_dz saw one; a scalar load a stage otherwise)
@@ -401,7 +476,7 @@ __global__ __launch_bounds__(64 * Tile<BM>::WAVES, 2) void xent_product(Products
       for (int c = threadIdx.x % PER; c < RB / 16; c += PER) *(u32x4*)(tile + r * RB + c * 16) = u32x4{0, 0, 0, 0};
     return true;
   };
-  tile_product<T, BM, A_K, false, false>(da, db, A0, A1, B0, B1, (int)((k_hi - k_lo + BK - 1) / BK), 0, wave, lane, acc, fix);
+  tile_product<T, BM, PARTS, A_K, false, false>(da, db, s.part_a, s.part_b, A0, A1, B0, B1, (int)((k_hi - k_lo + BK - 1) / BK), 0, wave, lane, acc, fix);
 
   __syncthreads();
   // 32 rows x 64 columns of float32 a wave through LDS (8 KB), then whole row segments
@@ -432,7 +507,7 @@ __global__ __launch_bounds__(64 * Tile<BM>::WAVES, 2) void xent_product(Products
         if (row >= s.m || col >= s.n) continue;  // n is a multiple of 8
         if (s.add != nullptr) v += *(const f32x4*)(s.add + row * s.n + col);
         if (s.out != nullptr)
-          *(uint2*)(s.out + row * s.n + col) = make_uint2(T::pack2(v[0], v[1]), T::pack2(v[2], v[3]));
+          store4<T>(s, row, col, v);
         else
           *(f32x4*)(s.wide + (slice * s.m + row) * s.n + col) = v;
       }
@@ -441,17 +516,52 @@ __global__ __launch_bounds__(64 * Tile<BM>::WAVES, 2) void xent_product(Products
 #endif
 }
 
-// out = round(add + slices in order), or the same kept in float32
+// out = round(add + slices in order), or the same kept in float32 (s.wide)
 template <typename T>
-__global__ __launch_bounds__(256) void xent_fold(const float* __restrict__ slices, const float* add, int64_t count, int64_t total, u16* out, float* wide) {
+__global__ __launch_bounds__(256) void xent_fold(Products s, const float* __restrict__ slices, int64_t count) {
+  const int64_t total = s.m * s.n;
   for (int64_t i = (blockIdx.x * (int64_t)256 + threadIdx.x) * 4; i < total; i += (int64_t)gridDim.x * 1024) {
     f32x4 v = *(const f32x4*)(slices + i);
+#pragma unroll 4
     for (int64_t k = 1; k < count; k++) v += *(const f32x4*)(slices + k * total + i);
-    if (add != nullptr) v += *(const f32x4*)(add + i);
-    if (out != nullptr)
-      *(uint2*)(out + i) = make_uint2(T::pack2(v[0], v[1]), T::pack2(v[2], v[3]));
-    else
-      *(f32x4*)(wide + i) = v;
+    if (s.add != nullptr) v += *(const f32x4*)(s.add + i);
+    if (s.out != nullptr) {
+      const int64_t row = i / s.n;
+      store4<T>(s, row, i - row * s.n, v);
+    } else {
+      *(f32x4*)(s.wide + i) = v;
+    }
+  }
+}
+
+// A matrix of `rows` rows of `width` elements as PARTS matrices of rows of `padded` elements, zeros past the width:
+// 8 consecutive elements a thread.
+template <typename S, typename T, int PARTS>
+__global__ __launch_bounds__(256) void xent_parts(const typename S::Storage* __restrict__ src, u16* __restrict__ dst, int64_t rows, int width, int padded, int64_t part) {
+  const int chunks = padded / 8;
+  const int64_t total = rows * chunks;
+  for (int64_t i = blockIdx.x * (int64_t)256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+    const int64_t row = i / chunks;
+    const int c = (int)(i - row * chunks) * 8;
+    float v[8];
+#pragma unroll
+    for (int e = 0; e < 8; e++) v[e] = c + e < width ? S::load(src, row * width + c + e) : 0.f;
+#pragma unroll
+    for (int p = 0; p < PARTS; p++) {
+      u16x8 w;
+#pragma unroll
+      for (int e = 0; e < 8; e++) {
+        u16 h = T::pack(v[e]);
+        if (PARTS > 1) {
+          const bool huge = !(fabsf(T::unpack(h)) <= 3.402823466e38f);
+          // the largest numbers round past bfloat16's: cut off instead; an infinity or a NaN is its first part alone
+          if (huge && fabsf(v[e]) <= 3.402823466e38f) h = (u16)(__float_as_uint(v[e]) >> 16);
+          v[e] = fabsf(v[e]) <= 3.402823466e38f ? v[e] - T::unpack(h) : 0.f;
+        }
+        w[e] = h;
+      }
+      *(u16x8*)(dst + p * part + row * padded + c) = w;
+    }
   }
 }
 
@@ -463,10 +573,23 @@ constexpr int64_t FILL = 256;  // workgroups that give every CU one
 
 int tile_for(int64_t m, int64_t n) { return ((m + 255) / 256) * ((n + 255) / 256) >= FILL ? 256 : 128; }
 
-// vocabulary entries whose dz goes by at a time, a multiple of 256
-int64_t piece_of(const XentArgs& a) {
-  const int64_t whole = up(a.vocab, 256), most = PIECE_BYTES / 2 / up(a.rows, 256) / 256 * 256;
-  return most >= whole ? whole : most < 1024 ? 1024 : most;
+bool f32(const XentArgs& a) { return a.dtype == LIMN_HIP_FLOAT32; }
+int parts_of(const XentArgs& a) { return f32(a) ? 3 : 1; }
+int64_t padded_width(const XentArgs& a) { return up(a.width, 8); }
+
+// Whether x and w go as they are: half widths in 16-byte rows.
+bool rows16(const XentArgs& a) { return !f32(a) && a.width % 8 == 0; }
+bool as_is(const XentArgs& a) { return rows16(a) && ((uintptr_t)a.x | (uintptr_t)a.w) % 16 == 0; }
+
+// Vocabulary entries that go by at a time, a multiple of 256 and 1024 at least: what 32-bit offsets reach, dz
+// within PIECE_BYTES, and the copies of the weight's rows, where there are any, too.
+int64_t piece_of(const XentArgs& a, bool backward, bool copies) {
+  const int64_t whole = up(a.vocab, 256), half = PIECE_BYTES / 2 / parts_of(a);
+  int64_t most = (int64_t)0x70000000 / 2 / padded_width(a);
+  if (backward && half / up(a.rows, 256) < most) most = half / up(a.rows, 256);
+  if (copies && half / padded_width(a) < most) most = half / padded_width(a);
+  most = most < 1024 ? 1024 : most / 256 * 256;
+  return most < whole ? most : whole;
 }
 
 struct Cut {
@@ -478,97 +601,120 @@ Cut cut(int64_t m, int64_t n, int64_t k) {
   return {p.tile, p.split, p.chunk};
 }
 
-struct BwdPlan {
-  int64_t piece, pieces, rows_pad, slices;  // slices: float32 (slices x result) bytes the products need at most
-};
-
 int64_t product_bytes(int64_t m, int64_t n, int64_t k) {
   const Cut c = cut(m, n, k);
   return c.split > 1 ? c.split * m * n * 4 : 0;
 }
 
-BwdPlan bwd_plan(const XentArgs& a) {
+struct BwdPlan {
+  int64_t piece, pieces, rows_pad, slices;  // slices: float32 (slices x result) bytes the products need at most
+};
+
+BwdPlan bwd_plan(const XentArgs& a, bool copies) {
   BwdPlan p;
-  p.piece = piece_of(a);
+  const int64_t width = padded_width(a);
+  p.piece = piece_of(a, true, copies);
   p.pieces = (a.vocab + p.piece - 1) / p.piece;
   p.rows_pad = up(a.rows, 256);
   p.slices = 0;
   for (const int64_t n : {p.piece < a.vocab ? p.piece : a.vocab, a.vocab - (p.pieces - 1) * p.piece}) {
-    const int64_t dx = product_bytes(a.rows, a.width, up(n, 64)), dw = product_bytes(n, a.width, up(a.rows, 64));
+    const int64_t dx = product_bytes(a.rows, width, up(n, 64)), dw = product_bytes(n, width, up(a.rows, 64));
     if (dx > p.slices) p.slices = dx;
     if (dw > p.slices) p.slices = dw;
   }
   return p;
 }
 
-// rows of a w piece whose byte offsets stay in 32 bits
-int64_t stats_piece(const XentArgs& a) {
-  const int64_t most = ((int64_t)0x70000000 / 2 / a.width) / 256 * 256;
-  return most < a.vocab ? most : up(a.vocab, 256);
-}
-
-template <typename T, int BM>
+template <typename T, int BM, int PARTS>
 int launch_stats(const Logits& l, hipStream_t stream) {
   const int64_t blocks = ((l.rows + BM - 1) / BM) * ((l.piece + BM - 1) / BM);
   if (blocks > 0x7fffffff) return fail(LIMN_HIP_EUNSUPPORTED, "xent: %lld workgroups exceed one launch", (long long)blocks);
   const dim3 grid((unsigned)blocks), block(64 * Tile<BM>::WAVES);
   if (l.width % BK == 0)
-    hipLaunchKernelGGL((xent_stats<T, BM, false>), grid, block, 0, stream, l);
+    hipLaunchKernelGGL((xent_stats<T, BM, PARTS, false>), grid, block, 0, stream, l);
   else
-    hipLaunchKernelGGL((xent_stats<T, BM, true>), grid, block, 0, stream, l);
+    hipLaunchKernelGGL((xent_stats<T, BM, PARTS, true>), grid, block, 0, stream, l);
   return check_hip(hipGetLastError(), "launching the cross entropy's logits");
 }
 
-template <typename T, int BM>
+template <typename T, int BM, int PARTS>
 int launch_dz(const Logits& l, hipStream_t stream) {
   const int64_t blocks = ((l.rows + BM - 1) / BM) * (l.ldz / BM);
   if (blocks > 0x7fffffff) return fail(LIMN_HIP_EUNSUPPORTED, "xent: %lld workgroups exceed one launch", (long long)blocks);
   const dim3 grid((unsigned)blocks), block(64 * Tile<BM>::WAVES);
   if (l.width % BK == 0)
-    hipLaunchKernelGGL((xent_dz<T, BM, false>), grid, block, 0, stream, l);
+    hipLaunchKernelGGL((xent_dz<T, BM, PARTS, false>), grid, block, 0, stream, l);
   else
-    hipLaunchKernelGGL((xent_dz<T, BM, true>), grid, block, 0, stream, l);
+    hipLaunchKernelGGL((xent_dz<T, BM, PARTS, true>), grid, block, 0, stream, l);
   return check_hip(hipGetLastError(), "launching the cross entropy's gradient");
 }
 
-template <typename T, bool A_K>
-int launch_product(Products s, const Cut& c, float* slices, float* acc, bool first, u16* out, hipStream_t stream) {
+template <typename T, int PARTS, bool A_K>
+int launch_product(Products s, const Cut& c, float* slices, float* acc, bool first, void* out, hipStream_t stream) {
   // unsplit: straight to out (the last piece of dx, or dw), or into the float32 totals; split: slices, then a fold
   const bool split = c.split > 1;
+  const float* add = first ? nullptr : acc;
   s.chunk = c.chunk;
   s.out = split ? nullptr : out;
   s.wide = split ? slices : acc;
-  s.add = split || first ? nullptr : acc;
+  s.add = split ? nullptr : add;
   const int64_t blocks = c.split * ((s.m + c.tile - 1) / c.tile) * ((s.n + c.tile - 1) / c.tile);
   if (blocks > 0x7fffffff) return fail(LIMN_HIP_EUNSUPPORTED, "xent: %lld workgroups exceed one launch", (long long)blocks);
   if (c.tile == 256)
-    hipLaunchKernelGGL((xent_product<T, 256, A_K>), dim3((unsigned)blocks), dim3(512), 0, stream, s);
+    hipLaunchKernelGGL((xent_product<T, 256, PARTS, A_K>), dim3((unsigned)blocks), dim3(512), 0, stream, s);
   else
-    hipLaunchKernelGGL((xent_product<T, 128, A_K>), dim3((unsigned)blocks), dim3(256), 0, stream, s);
+    hipLaunchKernelGGL((xent_product<T, 128, PARTS, A_K>), dim3((unsigned)blocks), dim3(256), 0, stream, s);
   const int rc = check_hip(hipGetLastError(), "launching a product of the cross entropy's gradient");
   if (rc != LIMN_HIP_OK || !split) return rc;
-  const int64_t total = s.m * s.n, groups = (total / 4 + 255) / 256;
-  hipLaunchKernelGGL((xent_fold<T>), dim3((unsigned)(groups < 4096 ? groups : 4096)), dim3(256), 0, stream, slices, first ? nullptr : acc, c.split, total, out, acc);
+  s.out = out;
+  s.wide = acc;
+  s.add = add;
+  const int64_t groups = (s.m * s.n / 4 + 255) / 256;
+  hipLaunchKernelGGL((xent_fold<T>), dim3((unsigned)(groups < 4096 ? groups : 4096)), dim3(256), 0, stream, s, slices, c.split);
   return check_hip(hipGetLastError(), "launching the fold of a product's slices");
 }
 
-template <typename T>
+template <typename S, typename T, int PARTS>
+int launch_parts(const void* src, u16* dst, int64_t rows, const XentArgs& a, int64_t part) {
+  const int64_t padded = padded_width(a), groups = (rows * (padded / 8) + 255) / 256;
+  hipLaunchKernelGGL((xent_parts<S, T, PARTS>), dim3((unsigned)(groups < 16384 ? groups : 16384)), dim3(256), 0, a.stream, (const typename S::Storage*)src, dst, rows,
+                     (int)a.width, (int)padded, part);
+  return check_hip(hipGetLastError(), "launching an operand's parts");
+}
+
+// S: the operands' type, T: the type the products take, in PARTS parts.
+template <typename S, typename T, int PARTS>
 int fwd(const XentArgs& a) {
-  const int64_t piece = stats_piece(a);
+  const bool copies = !as_is(a);
+  const int64_t piece = piece_of(a, false, copies), width = padded_width(a);
   const int bm = tile_for(a.rows, a.vocab);
   XentSpace space(a.workspace);
   const int64_t tiles = (a.vocab + bm - 1) / bm;
   Logits l = {};
-  l.x = (const u16*)a.x, l.targets = a.targets, l.rows = a.rows, l.width = a.width, l.vocab = a.vocab;
+  l.x = (const u16*)a.x, l.targets = a.targets, l.rows = a.rows, l.width = width, l.vocab = a.vocab;
   l.stats = (float2*)space.take(tiles * a.rows * 8);
   l.picked = (float*)space.take(a.rows * 4);
+  u16* wp = nullptr;
   int rc = LIMN_HIP_OK;
+  if (copies) {
+    u16* xp = (u16*)space.take(PARTS * a.rows * width * 2);
+    wp = (u16*)space.take(PARTS * piece * width * 2);
+    l.x = xp;
+    l.part_x = a.rows * width;
+    rc = launch_parts<S, T, PARTS>(a.x, xp, a.rows, a, l.part_x);
+  }
   for (int64_t v0 = 0; v0 < a.vocab && rc == LIMN_HIP_OK; v0 += piece) {
-    l.w = (const u16*)a.w + v0 * a.width;
+    const typename S::Storage* w = (const typename S::Storage*)a.w + v0 * a.width;
     l.v0 = v0;
     l.piece = a.vocab - v0 < piece ? a.vocab - v0 : piece;
     l.tile0 = v0 / bm;
-    rc = bm == 256 ? launch_stats<T, 256>(l, a.stream) : launch_stats<T, 128>(l, a.stream);
+    l.w = (const u16*)w;
+    if (copies) {
+      l.w = wp;
+      l.part_w = l.piece * width;
+      if ((rc = launch_parts<S, T, PARTS>(w, wp, l.piece, a, l.part_w)) != LIMN_HIP_OK) return rc;
+    }
+    rc = bm == 256 ? launch_stats<T, 256, PARTS>(l, a.stream) : launch_stats<T, 128, PARTS>(l, a.stream);
   }
   if (rc != LIMN_HIP_OK) return rc;
   hipLaunchKernelGGL(xent_rows, dim3((unsigned)((a.rows + 31) / 32)), dim3(256), 0, a.stream, l.stats, l.picked, a.targets, (float*)a.o0, (float*)a.o1, a.rows, tiles,
@@ -576,33 +722,55 @@ int fwd(const XentArgs& a) {
   return check_hip(hipGetLastError(), "launching the cross entropy's rows");
 }
 
-template <typename T>
+template <typename S, typename T, int PARTS>
 int bwd(const XentArgs& a) {
-  const BwdPlan p = bwd_plan(a);
+  const bool copies = !as_is(a);
+  const BwdPlan p = bwd_plan(a, copies);
+  const int64_t width = padded_width(a);
   XentSpace space(a.workspace);
   Logits l = {};
-  l.x = (const u16*)a.x, l.targets = a.targets, l.rows = a.rows, l.width = a.width, l.vocab = a.vocab, l.lse = a.lse_in, l.g = a.g;
-  l.dz = (u16*)space.take(p.rows_pad * p.piece * 2);
+  l.x = (const u16*)a.x, l.targets = a.targets, l.rows = a.rows, l.width = width, l.vocab = a.vocab, l.lse = a.lse_in, l.g = a.g;
+  l.dz = (u16*)space.take(PARTS * p.rows_pad * p.piece * 2);
   l.flags = (int*)space.take(p.rows_pad / 64 * 4);
   float* slices = (float*)space.take(p.slices);
-  float* acc = p.pieces > 1 ? (float*)space.take(a.rows * a.width * 4) : nullptr;
+  float* acc = p.pieces > 1 ? (float*)space.take(a.rows * width * 4) : nullptr;
+  u16* wp = nullptr;
+  int rc = LIMN_HIP_OK;
+  if (copies) {
+    u16* xp = (u16*)space.take(PARTS * a.rows * width * 2);
+    wp = (u16*)space.take(PARTS * p.piece * width * 2);
+    l.x = xp;
+    l.part_x = a.rows * width;
+    if ((rc = launch_parts<S, T, PARTS>(a.x, xp, a.rows, a, l.part_x)) != LIMN_HIP_OK) return rc;
+  }
   for (int64_t v0 = 0; v0 < a.vocab; v0 += p.piece) {
     const bool first = v0 == 0, last = v0 + p.piece >= a.vocab;
-    l.w = (const u16*)a.w + v0 * a.width;
+    const typename S::Storage* w = (const typename S::Storage*)a.w + v0 * a.width;
     l.v0 = v0;
     l.piece = last ? a.vocab - v0 : p.piece;
     l.ldz = up(l.piece, 256);
-    int rc = tile_for(a.rows, l.ldz) == 256 ? launch_dz<T, 256>(l, a.stream) : launch_dz<T, 128>(l, a.stream);
+    l.part_dz = p.rows_pad * l.ldz;
+    l.w = (const u16*)w;
+    if (copies) {
+      l.w = wp;
+      l.part_w = l.piece * width;
+      if ((rc = launch_parts<S, T, PARTS>(w, wp, l.piece, a, l.part_w)) != LIMN_HIP_OK) return rc;
+    }
+    rc = tile_for(a.rows, l.ldz) == 256 ? launch_dz<T, 256, PARTS>(l, a.stream) : launch_dz<T, 128, PARTS>(l, a.stream);
     if (rc != LIMN_HIP_OK) return rc;
     Products s = {};
     s.rows = a.rows, s.vocab = a.vocab, s.targets = a.targets, s.flags = l.flags;
-    s.a = l.dz, s.b = l.w, s.m = a.rows, s.n = a.width, s.k = up(l.piece, 64);
-    s.a_rows = p.rows_pad, s.a_depth = l.ldz, s.a_stride = l.ldz, s.b_depth = l.piece, s.b_stride = a.width;
-    rc = launch_product<T, true>(s, cut(s.m, s.n, s.k), slices, acc, first, last ? (u16*)a.o0 : nullptr, a.stream);
+    s.out_f32 = f32(a), s.width = a.width, s.n = width;
+    s.a = l.dz, s.part_a = l.part_dz, s.b = l.w, s.part_b = l.part_w, s.m = a.rows, s.k = up(l.piece, 64);
+    s.a_rows = p.rows_pad, s.a_depth = l.ldz, s.a_stride = l.ldz, s.b_depth = l.piece, s.b_stride = width, s.b_cols = width;
+    s.vec = a.width % 4 == 0 && (uintptr_t)a.o0 % (f32(a) ? 16 : 8) == 0;
+    rc = launch_product<T, PARTS, true>(s, cut(s.m, s.n, s.k), slices, acc, first, last ? a.o0 : nullptr, a.stream);
     if (rc != LIMN_HIP_OK) return rc;
-    s.b = (const u16*)a.x, s.m = l.piece, s.k = up(a.rows, 64);
+    s.b = l.x, s.part_b = l.part_x, s.m = l.piece, s.k = up(a.rows, 64);
     s.a_rows = l.ldz, s.a_depth = p.rows_pad, s.b_depth = a.rows;
-    rc = launch_product<T, false>(s, cut(s.m, s.n, s.k), slices, nullptr, true, (u16*)a.o1 + v0 * a.width, a.stream);
+    void* dw = (typename S::Storage*)a.o1 + v0 * a.width;
+    s.vec = a.width % 4 == 0 && (uintptr_t)dw % (f32(a) ? 16 : 8) == 0;
+    rc = launch_product<T, PARTS, false>(s, cut(s.m, s.n, s.k), slices, nullptr, true, dw, a.stream);
     if (rc != LIMN_HIP_OK) return rc;
   }
   return LIMN_HIP_OK;
@@ -610,21 +778,38 @@ int bwd(const XentArgs& a) {
 
 }  // namespace
 
-// 16-byte rows, every operand's bytes within 32-bit offsets of a base (a tile may reach 256 rows past its end)
-bool xent_half_sizes(const XentArgs& a) {
-  if (a.dtype == LIMN_HIP_FLOAT32 || a.width % 8 != 0) return false;
-  const int64_t most = (int64_t)0x7f000000 / 2, piece = piece_of(a);
-  if ((a.rows + 512) * a.width >= most || (stats_piece(a) + 512) * a.width >= most || stats_piece(a) < 256) return false;
-  return (up(a.rows, 256) + 512) * piece < most && (piece + 512) * a.width < most;
+// every operand's bytes within 32-bit offsets of a base (a tile may reach 256 rows past its end)
+bool xent_sizes_ok(const XentArgs& a) {
+  const int64_t most = (int64_t)0x7f000000 / 2, width = padded_width(a), piece = piece_of(a, true, false), ahead = piece_of(a, false, false);
+  return (a.rows + 512) * width < most && (ahead + 512) * width < most && (up(a.rows, 256) + 512) * piece < most && (piece + 512) * width < most;
 }
 
-int64_t xent_half_workspace(const XentArgs& a, bool backward) {
-  if (!backward) return xent_align(((a.vocab + 127) / 128) * a.rows * 8) + xent_align(a.rows * 4);
-  const BwdPlan p = bwd_plan(a);
-  return xent_align(p.rows_pad * p.piece * 2) + xent_align(p.rows_pad / 64 * 4) + xent_align(p.slices) + (p.pieces > 1 ? xent_align(a.rows * a.width * 4) : 0);
+namespace {
+
+int64_t workspace_of(const XentArgs& a, bool backward, bool copies) {
+  const int64_t width = padded_width(a), parts = parts_of(a), row = parts * 2 * width;
+  int64_t need = copies ? xent_align(a.rows * row) + xent_align(piece_of(a, backward, copies) * row) : 0;
+  if (!backward) return need + xent_align(((a.vocab + 127) / 128) * a.rows * 8) + xent_align(a.rows * 4);
+  const BwdPlan p = bwd_plan(a, copies);
+  need += xent_align(parts * p.rows_pad * p.piece * 2) + xent_align(p.rows_pad / 64 * 4) + xent_align(p.slices);
+  return need + (p.pieces > 1 ? xent_align(a.rows * width * 4) : 0);
 }
 
-int launch_xent_half_fwd(const XentArgs& a) { return a.dtype == LIMN_HIP_BFLOAT16 ? fwd<BF16>(a) : fwd<F16>(a); }
-int launch_xent_half_bwd(const XentArgs& a) { return a.dtype == LIMN_HIP_BFLOAT16 ? bwd<BF16>(a) : bwd<F16>(a); }
+}  // namespace
+
+// Enough whether or not the call's buffers are aligned as their sizes allow.
+int64_t xent_workspace(const XentArgs& a, bool backward) {
+  const int64_t copied = workspace_of(a, backward, true), plain = rows16(a) ? workspace_of(a, backward, false) : 0;
+  return copied > plain ? copied : plain;
+}
+
+int launch_xent_fwd(const XentArgs& a) {
+  if (f32(a)) return fwd<F32, BF16, 3>(a);
+  return a.dtype == LIMN_HIP_BFLOAT16 ? fwd<BF16, BF16, 1>(a) : fwd<F16, F16, 1>(a);
+}
+int launch_xent_bwd(const XentArgs& a) {
+  if (f32(a)) return bwd<F32, BF16, 3>(a);
+  return a.dtype == LIMN_HIP_BFLOAT16 ? bwd<BF16, BF16, 1>(a) : bwd<F16, F16, 1>(a);
+}
 
 }  // namespace limn

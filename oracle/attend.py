@@ -138,7 +138,12 @@ def xent(x, w, targets, g=None, dtype="float32"):
         z = x @ w.T
         top = z.max(1, keepdims=True)
         lse = (top + np.log(np.exp(z - top).sum(1, keepdims=True)))[:, 0]
-        e = ((width + 8) * F * (np.abs(x) @ np.abs(w).T)).max(1) + 4 * F * np.abs(z).max(1)
+        # a float32 operand is the sum of three bfloat16 numbers, each rounded from what the ones before leave: 24 bits,
+        # or as many as there are above bfloat16's least step, 2^-133, so the operand is off by up to half of that and a
+        # product by 2^-134 times the other operand
+        lost = 2.0**-134 if dtype == "float32" else 0.0
+        lost_z = lost * (np.abs(x).sum(1) + np.abs(w).sum(1).max())
+        e = ((width + 8) * F * (np.abs(x) @ np.abs(w).T)).max(1) + 4 * F * np.abs(z).max(1) + lost_z
         rel = 2 * e + (vocab**0.5 + 32) * F  # the sum of positive terms runs in many short chains
         loss = np.where(live, lse - z[np.arange(rows), at], 0.0)
     out = dict(loss=(loss, np.where(live, rel + e + 8 * F * np.abs(lse), 0.0)), lse=(lse, rel + 8 * F * np.abs(lse)))
@@ -155,10 +160,10 @@ def xent(x, w, targets, g=None, dtype="float32"):
     dx, dw = dz @ w, dz.T @ xs
     dxo = ddz @ np.abs(w) + (vocab + 8) * F * (np.abs(dz) @ np.abs(w)) + u * np.abs(dx) + least
     dwo = ddz.T @ np.abs(xs) + (rows + 8) * F * (np.abs(dz).T @ np.abs(xs)) + u * np.abs(dw) + least
-    if operand:  # a dz below the type's least normal number is off by a part of that number
-        tiny = 2.0**-24 if dtype == "float16" else 0.0
-        dxo = dxo + tiny * np.abs(w).sum(0)
-        dwo = dwo + tiny * np.abs(xs).sum(0)
+    # a dz, or a float32 one's last part, below its type's least normal number is off by a part of that number
+    tiny = 2.0**-24 if dtype == "float16" else TINY
+    dxo = dxo + tiny * np.abs(w).sum(0) + lost * np.abs(dz).sum(1, keepdims=True)
+    dwo = dwo + tiny * np.abs(xs).sum(0) + lost * np.abs(dz).sum(0)[:, None]
     out.update(dx=(dx, dxo), dw=(dw, dwo))
     return out
 

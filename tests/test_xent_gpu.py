@@ -83,6 +83,23 @@ def test_several_pieces_of_the_vocabulary(hipdev, dtype):
     check(hipdev, x, w, targets, (rng.random(rows) / rows).astype(np.float32), dtype)
 
 
+def test_float32_numbers_of_every_size(hipdev):
+    """Rows scaled from 2^-120 to 2^120 and back by the weight's columns: a float32 goes to its products in parts, each of which must hold its bits."""
+    rng, x, w, targets = draw(9, "float32", 100, 64, 300)
+    scale = np.exp2(rng.integers(-60, 61, 64)).astype(np.float32)
+    x, w = x * scale, w / scale
+    check(hipdev, x, w, targets, rng.standard_normal(100).astype(np.float32), "float32")
+    big = np.zeros((4, 8), np.float32)
+    big[0, 0] = np.finfo(np.float32).max  # past bfloat16's largest
+    w = np.zeros((5, 8), np.float32)
+    w[0, 0] = 1e-38
+    w[1, 1] = 1.0
+    got = check(hipdev, big, w, np.array([0, 1, 2, 4], np.int32), np.ones(4, np.float32), "float32")
+    # float32's largest goes whole; 1e-38 (subnormal) goes to bfloat16's least step 2^-133, so their product 3.4028235
+    # is off by up to 2^128 2^-134 = 2^-6, and lse, whose slope by a score is below 1, by no more (8 steps beside that)
+    assert abs(got["lse"][0] - np.log(np.exp(3.4028235) + 4)) < 2.0**-6 + 2.0**-20
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 def test_no_row_has_a_target(hipdev, dtype):
     rng, x, w, targets = draw(2, dtype, 70, 64, 130)
