@@ -290,12 +290,15 @@ __global__ __launch_bounds__(64 * Tile<BM>::WAVES, 2) void xent_stats(Logits a) 
 #endif
 }
 
-// 32 rows a workgroup, 8 threads a row, each a run of the row's tiles; joined in order.
+// R rows a workgroup, 256 / R threads a row, each a run of the row's tiles; joined in order. Bound by the latency of a
+// thread's chain of loads: 32 rows where that gives every CU a workgroup, else 4 (48 rows, 250 tiles: 13 -> 5.5 us).
+template <int R>
 __global__ __launch_bounds__(256) void xent_rows(const float2* __restrict__ stats, const float* __restrict__ picked, const int* __restrict__ targets,
                                                  float* __restrict__ loss, float* __restrict__ lse, int64_t rows, int64_t tiles, int64_t vocab) {
-  __shared__ float2 part[8][32];
-  const int r = threadIdx.x & 31, g = threadIdx.x >> 5;
-  const int64_t row = blockIdx.x * (int64_t)32 + r, run = (tiles + 7) / 8, t1 = (g + 1) * run < tiles ? (g + 1) * run : tiles;
+  constexpr int RUNS = 256 / R;
+  __shared__ float2 part[RUNS][R];
+  const int r = threadIdx.x % R, g = threadIdx.x / R;
+  const int64_t row = blockIdx.x * (int64_t)R + r, run = (tiles + RUNS - 1) / RUNS, t1 = (g + 1) * run < tiles ? (g + 1) * run : tiles;
   float m = -__builtin_inff(), l = 0.f;
   if (row < rows) {
 #pragma unroll 4
@@ -314,8 +317,8 @@ __global__ __launch_bounds__(256) void xent_rows(const float2* __restrict__ stat
   __syncthreads();
   if (g == 0 && row < rows) {
     float top = -__builtin_inff(), total = 0.f;
-    for (int k = 0; k < 8; k++) top = fmaxf(top, part[k][r].x);
-    for (int k = 0; k < 8; k++) total += part[k][r].x == -__builtin_inff() ? part[k][r].y : part[k][r].y * fast_exp2((part[k][r].x - top) * LOG2E);
+    for (int k = 0; k < RUNS; k++) top = fmaxf(top, part[k][r].x);
+    for (int k = 0; k < RUNS; k++) total += part[k][r].x == -__builtin_inff() ? part[k][r].y : part[k][r].y * fast_exp2((part[k][r].x - top) * LOG2E);
     const float z = top + logf(total);
     const int t = targets[row];
     lse[row] = z;
@@ -516,21 +519,29 @@ __global__ __launch_bounds__(64 * Tile<BM>::WAVES, 2) void xent_product(Products
 #endif
 }
 
-// out = round(add + slices in order), or the same kept in float32 (s.wide)
+// out = round(add + slices), or the same kept in float32 (s.wide). A workgroup is 64 threads of 4 elements by G runs
+// of the slices, which are joined in order in LDS.
 template <typename T>
-__global__ __launch_bounds__(256) void xent_fold(Products s, const float* __restrict__ slices, int64_t count) {
-  const int64_t total = s.m * s.n;
-  for (int64_t i = (blockIdx.x * (int64_t)256 + threadIdx.x) * 4; i < total; i += (int64_t)gridDim.x * 1024) {
-    f32x4 v = *(const f32x4*)(slices + i);
+__global__ __launch_bounds__(1024) void xent_fold(Products s, const float* __restrict__ slices, int64_t count) {
+  __shared__ f32x4 part[16][64];
+  const int x = threadIdx.x, y = threadIdx.y, runs = blockDim.y;
+  const int64_t total = s.m * s.n, i = (blockIdx.x * (int64_t)64 + x) * 4, run = (count + runs - 1) / runs;
+  const int64_t k1 = (y + 1) * run < count ? (y + 1) * run : count;
+  f32x4 v = {0.f, 0.f, 0.f, 0.f};
+  if (i < total) {
 #pragma unroll 4
-    for (int64_t k = 1; k < count; k++) v += *(const f32x4*)(slices + k * total + i);
-    if (s.add != nullptr) v += *(const f32x4*)(s.add + i);
-    if (s.out != nullptr) {
-      const int64_t row = i / s.n;
-      store4<T>(s, row, i - row * s.n, v);
-    } else {
-      *(f32x4*)(s.wide + i) = v;
-    }
+    for (int64_t k = y * run; k < k1; k++) v += *(const f32x4*)(slices + k * total + i);
+  }
+  part[y][x] = v;
+  __syncthreads();
+  if (y != 0 || i >= total) return;
+  for (int g = 1; g < runs; g++) v += part[g][x];
+  if (s.add != nullptr) v += *(const f32x4*)(s.add + i);
+  if (s.out != nullptr) {
+    const int64_t row = i / s.n;
+    store4<T>(s, row, i - row * s.n, v);
+  } else {
+    *(f32x4*)(s.wide + i) = v;
   }
 }
 
@@ -596,13 +607,21 @@ struct Cut {
   int tile;
   int64_t split, chunk;
 };
-Cut cut(int64_t m, int64_t n, int64_t k) {
+// As matmul.hip cuts its products. In three parts a slice of k is six times the work for the same partial result, so
+// tiles of 128 that would give a CU one workgroup are cut too (float32, 8191 x 512 of 2048 rows: 175 -> 114 us
+// and 13 for the sum of the halves).
+Cut cut(int64_t m, int64_t n, int64_t k, int parts) {
+  const int64_t tiles = ((m + 127) / 128) * ((n + 127) / 128);
+  if (parts == 3 && tile_for(m, n) == 128 && tiles >= FILL && 2 * tiles <= 3 * FILL && k >= 256) {
+    const int64_t chunk = up((k + 1) / 2, BK);
+    return {128, 2, chunk};
+  }
   const MatmulPlan p = plan_matmul(MatmulShape{1, m, n, k});
   return {p.tile, p.split, p.chunk};
 }
 
-int64_t product_bytes(int64_t m, int64_t n, int64_t k) {
-  const Cut c = cut(m, n, k);
+int64_t product_bytes(int64_t m, int64_t n, int64_t k, int parts) {
+  const Cut c = cut(m, n, k, parts);
   return c.split > 1 ? c.split * m * n * 4 : 0;
 }
 
@@ -618,7 +637,7 @@ BwdPlan bwd_plan(const XentArgs& a, bool copies) {
   p.rows_pad = up(a.rows, 256);
   p.slices = 0;
   for (const int64_t n : {p.piece < a.vocab ? p.piece : a.vocab, a.vocab - (p.pieces - 1) * p.piece}) {
-    const int64_t dx = product_bytes(a.rows, width, up(n, 64)), dw = product_bytes(n, width, up(a.rows, 64));
+    const int64_t dx = product_bytes(a.rows, width, up(n, 64), parts_of(a)), dw = product_bytes(n, width, up(a.rows, 64), parts_of(a));
     if (dx > p.slices) p.slices = dx;
     if (dw > p.slices) p.slices = dw;
   }
@@ -669,8 +688,11 @@ int launch_product(Products s, const Cut& c, float* slices, float* acc, bool fir
   s.out = out;
   s.wide = acc;
   s.add = add;
-  const int64_t groups = (s.m * s.n / 4 + 255) / 256;
-  hipLaunchKernelGGL((xent_fold<T>), dim3((unsigned)(groups < 4096 ? groups : 4096)), dim3(256), 0, stream, s, slices, c.split);
+  // two loads a thread or more: a run's chain is what a small result waits for (48 x 512 of 62 slices: 18 -> 5 us)
+  const int64_t groups = (s.m * s.n / 4 + 63) / 64;
+  if (groups > 0x7fffffff) return fail(LIMN_HIP_EUNSUPPORTED, "xent: %lld workgroups exceed one launch", (long long)groups);
+  const int runs = c.split < 8 ? 4 : c.split < 32 ? 8 : 16;
+  hipLaunchKernelGGL((xent_fold<T>), dim3((unsigned)groups), dim3(64, runs), 0, stream, s, slices, c.split);
   return check_hip(hipGetLastError(), "launching the fold of a product's slices");
 }
 
@@ -717,8 +739,12 @@ int fwd(const XentArgs& a) {
     rc = bm == 256 ? launch_stats<T, 256, PARTS>(l, a.stream) : launch_stats<T, 128, PARTS>(l, a.stream);
   }
   if (rc != LIMN_HIP_OK) return rc;
-  hipLaunchKernelGGL(xent_rows, dim3((unsigned)((a.rows + 31) / 32)), dim3(256), 0, a.stream, l.stats, l.picked, a.targets, (float*)a.o0, (float*)a.o1, a.rows, tiles,
-                     a.vocab);
+  if (a.rows >= 32 * FILL)
+    hipLaunchKernelGGL((xent_rows<32>), dim3((unsigned)((a.rows + 31) / 32)), dim3(256), 0, a.stream, l.stats, l.picked, a.targets, (float*)a.o0, (float*)a.o1, a.rows,
+                       tiles, a.vocab);
+  else
+    hipLaunchKernelGGL((xent_rows<4>), dim3((unsigned)((a.rows + 3) / 4)), dim3(256), 0, a.stream, l.stats, l.picked, a.targets, (float*)a.o0, (float*)a.o1, a.rows,
+                       tiles, a.vocab);
   return check_hip(hipGetLastError(), "launching the cross entropy's rows");
 }
 
@@ -764,13 +790,13 @@ int bwd(const XentArgs& a) {
     s.a = l.dz, s.part_a = l.part_dz, s.b = l.w, s.part_b = l.part_w, s.m = a.rows, s.k = up(l.piece, 64);
     s.a_rows = p.rows_pad, s.a_depth = l.ldz, s.a_stride = l.ldz, s.b_depth = l.piece, s.b_stride = width, s.b_cols = width;
     s.vec = a.width % 4 == 0 && (uintptr_t)a.o0 % (f32(a) ? 16 : 8) == 0;
-    rc = launch_product<T, PARTS, true>(s, cut(s.m, s.n, s.k), slices, acc, first, last ? a.o0 : nullptr, a.stream);
+    rc = launch_product<T, PARTS, true>(s, cut(s.m, s.n, s.k, PARTS), slices, acc, first, last ? a.o0 : nullptr, a.stream);
     if (rc != LIMN_HIP_OK) return rc;
     s.b = l.x, s.part_b = l.part_x, s.m = l.piece, s.k = up(a.rows, 64);
     s.a_rows = l.ldz, s.a_depth = p.rows_pad, s.b_depth = a.rows;
     void* dw = (typename S::Storage*)a.o1 + v0 * a.width;
     s.vec = a.width % 4 == 0 && (uintptr_t)dw % (f32(a) ? 16 : 8) == 0;
-    rc = launch_product<T, PARTS, false>(s, cut(s.m, s.n, s.k), slices, nullptr, true, dw, a.stream);
+    rc = launch_product<T, PARTS, false>(s, cut(s.m, s.n, s.k, PARTS), slices, nullptr, true, dw, a.stream);
     if (rc != LIMN_HIP_OK) return rc;
   }
   return LIMN_HIP_OK;

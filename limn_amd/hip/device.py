@@ -602,9 +602,9 @@ class HipDevice(CompiledDevice):
         x, w, targets = node.srcs[:3]
         if x.dtype not in ABI_CODE or x.dtype not in FLOATS or w.dtype != x.dtype:
             raise NotImplementedError(f"{name}: no kernel for dtypes {x.dtype} and {w.dtype}")
-        if len(x.shape) != 2 or len(w.shape) != 2 or x.shape[1] != w.shape[1] or any(math.prod(s.shape) != x.shape[0] for s in (targets, *node.srcs[3:])):
+        if not x.shape or len(w.shape) != 2 or x.shape[-1] != w.shape[1] or any(s.shape != x.shape[:-1] for s in (targets, *node.srcs[3:])):
             raise ValueError(f"{name} shape mismatch: {[s.shape for s in node.srcs]}")
-        code, sizes = ABI_CODE[x.dtype], (x.shape[0], x.shape[1], w.shape[0])
+        code, sizes = ABI_CODE[x.dtype], (math.prod(x.shape[:-1]), *reversed(w.shape))
         workspace = self._held(int(self.lib.limn_hip_xent_workspace(code, *sizes, int(backward))))
         entry = self.lib.limn_hip_xent_bwd if backward else self.lib.limn_hip_xent_fwd
         kind = replay.STEP_XENT_BWD if backward else replay.STEP_XENT_FWD

@@ -35,25 +35,24 @@ def linear_cross_entropy(x: Tensor, weight: Tensor, targets: Tensor, reduction: 
         raise ValueError(f"linear_cross_entropy: targets must be {x.shape[:-1]} int32, got {targets.shape} {targets.dtype}")
     if reduction not in ("mean", "sum", "none"):
         raise ValueError(f"linear_cross_entropy: reduction is mean, sum or none, not {reduction!r}")
-    common = promote(x.dtype, weight.dtype)
-    rows, vocab = math.prod(x.shape[:-1]), weight.shape[0]
-    flat, head, at = x.cast(common).reshape(rows, x.shape[-1]), weight.cast(common), targets.reshape(rows)
-    loss = _rows(flat, head, at)
+    common, vocab = promote(x.dtype, weight.dtype), weight.shape[0]
+    loss = _rows(x.cast(common), weight.cast(common), targets)
     if reduction == "none":
-        return loss.reshape(*targets.shape)
+        return loss
     total = loss.sum()
     if reduction == "sum":
         return total
-    live = ((at >= 0) * (at < vocab)).cast(loss.dtype).sum()
+    live = ((targets >= 0) * (targets < vocab)).cast(loss.dtype).sum()
     return total * live.maximum(1.0).reciprocal()
 
 
 def _rows(x: Tensor, w: Tensor, targets: Tensor) -> Tensor:
+    """The rows' losses, shaped as targets. The kernels take the leading dims as one (row-major bytes)."""
     dev = active_device()
     if x.dtype == float64 or not dev.has_custom(XENT_FWD):
         return _composed(x, w, targets)
     x, w, targets = contiguous(x), contiguous(w), contiguous(targets)
-    rows = (x.shape[0],)
+    rows = targets.shape
     loss, lse = custom(XENT_FWD, (x.node, w.node, targets.node), (), ((float32, rows), (float32, rows)))
 
     def backward(g: Tensor):
@@ -66,7 +65,7 @@ def _rows(x: Tensor, w: Tensor, targets: Tensor) -> Tensor:
 
 
 def _composed(x: Tensor, w: Tensor, targets: Tensor) -> Tensor:
-    wide, vocab = accumulate_in(x.dtype), w.shape[0]
-    logp = (x.cast(wide) @ w.cast(wide).transpose()).log_softmax(-1)
-    picked = Tensor.arange(vocab).reshape(1, vocab).eq(targets.reshape(-1, 1))
-    return -(picked.where(logp, 0.0)).sum(axis=-1)
+    wide, vocab, rows = accumulate_in(x.dtype), w.shape[0], math.prod(targets.shape)
+    logp = (x.cast(wide).reshape(rows, x.shape[-1]) @ w.cast(wide).transpose()).log_softmax(-1)
+    picked = Tensor.arange(vocab).reshape(1, vocab).eq(targets.reshape(rows, 1))
+    return -(picked.where(logp, 0.0)).sum(axis=-1).reshape(*targets.shape)
