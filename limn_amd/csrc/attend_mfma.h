@@ -232,10 +232,18 @@ __device__ __forceinline__ bool any_odd(const f32x16 (&acc)[N]) {
 
 // float16 has no normal numbers below 2^-14: probabilities go into its products multiplied by a power of two, 2^7
 // in the forward (where the reference point lets them reach 2^8) and 2^14 in the dV product (where none
-// passes 1), taken off again at the store. bfloat16 has float32's range.
+// passes 1), taken off again at the store. dS = p (dp - delta) goes multiplied by 2^8: an element is then off by 2^-33
+// at most where it is below the normal numbers, and a sum of 2^16 such of random sign by 2^-25, which the
+// result's own rounding costs it too; past 2^8 it overflows, and the block is recomputed in float. bfloat16 has
+// float32's range.
 template <typename T>
 constexpr float shift_of(float bits) {
   return std::is_same<T, F16>::value ? bits : 0.f;
+}
+constexpr float DS_BITS = 8.f;
+template <typename T>
+constexpr float ds_down() {
+  return std::is_same<T, F16>::value ? 1.f / 256.f : 1.f;
 }
 
 // ---- scores ---------------------------------------------------------------------------------------------
@@ -457,7 +465,7 @@ __global__ __launch_bounds__(THREADS, 2) void attend_dq_mfma(FastArgs g, RuleArg
   for (int dt = 0; dt < D / 32; dt++) acc[dt] = zero16();
   delta = pair_sum(delta);
   if (h == 0 && there) g.delta[rows0 + row] = delta;
-  const float l2 = there ? att_l2(g.lse_in[rows0 + row]) : __builtin_inff();
+  const float l2 = there ? att_l2(g.lse_in[rows0 + row]) - shift_of<T>(DS_BITS) : __builtin_inff();
 
   const int last = min(q0 + ATT_ROWS, r.t_q) - 1;
   int kend = r.len;
@@ -548,7 +556,7 @@ __global__ __launch_bounds__(THREADS, 2) void attend_dq_mfma(FastArgs g, RuleArg
   }
   const bool odd = any_odd(acc);
   if (threadIdx.x == 0) g.odd[bh * nqb + q0 / ATT_ROWS] = odd;
-  store_rows<T, D>(g.o0 + rows0 * g.hd, acc, wq0, r.t_q, g.hd, g.scale, tiles + wave * TE);
+  store_rows<T, D>(g.o0 + rows0 * g.hd, acc, wq0, r.t_q, g.hd, g.scale * ds_down<T>(), tiles + wave * TE);
 }
 
 // ---- dK/dV pass up to 64 dims -----------------------------------------------------------------------------
@@ -558,6 +566,7 @@ __global__ __launch_bounds__(THREADS, 2) void attend_dkv_mfma(FastArgs g, RuleAr
   constexpr int TE = TILE * tile_stride<D>();
   constexpr bool RAW = !CAP && !BIAS;
   constexpr float UP = shift_of<T>(14.f), DOWN = std::is_same<T, F16>::value ? 1.f / 16384.f : 1.f;
+  constexpr float DS = DOWN / ds_down<T>();  // turns p 2^14 (dp - delta) into dS 2^8
   __shared__ __attribute__((aligned(16))) u16 tiles[4 * TE];
   __shared__ __attribute__((aligned(16))) float Ls[2][TILE];
   __shared__ __attribute__((aligned(16))) float Ds[2][TILE];
@@ -614,7 +623,7 @@ __global__ __launch_bounds__(THREADS, 2) void attend_dkv_mfma(FastArgs g, RuleAr
       const int qq = t * TILE + (int)threadIdx.x;
       const bool ok = qq < r.t_q;
       lnext = ok ? att_l2(g.lse_in[rows0 + qq]) - UP : __builtin_inff();
-      dnext = ok ? g.delta[rows0 + qq] * DOWN : 0.f;
+      dnext = ok ? g.delta[rows0 + qq] * DS : 0.f;
       qnext = ok ? query_doc(r, r.off + qq) : -1;
     }
   };
@@ -680,7 +689,7 @@ __global__ __launch_bounds__(THREADS, 2) void attend_dkv_mfma(FastArgs g, RuleAr
         const float y = bend<CAP, BIAS, true>(s[i], r, slope2, near + (float)(8 * (i >> 2) + (i & 3)), bent);
         const float l2 = l4[i >> 2][i & 3];
         s[i] = fast_exp2(RAW ? fmaf(y, r.c2, -l2) : y - l2);
-        dp[i] = s[i] * fmaf(dp[i], DOWN, -d4[i >> 2][i & 3]) * (CAP ? bent : 1.f);  // times scale once, at the store
+        dp[i] = s[i] * fmaf(dp[i], DS, -d4[i >> 2][i & 3]) * (CAP ? bent : 1.f);  // times scale once, at the store
       }
       bool edge = s0 + 32 > r.t_q || wk0 + 32 > r.len || (r.causal && r.off + s0 < wk0 + 31 && wk0 + 31 >= r.pre);
       edge |= ((alike >> sub) & 1) == 0;
@@ -728,7 +737,7 @@ __global__ __launch_bounds__(THREADS, 2) void attend_dkv_mfma(FastArgs g, RuleAr
   }
   const bool odd_k = any_odd(gk), odd_v = any_odd(gv);
   if (threadIdx.x == 0) g.odd[bk * nkb + blk] = odd_k | odd_v;
-  store_rows<T, D>(g.o0 + bk * (int64_t)r.t_k * g.hd, gk, wk0, r.t_k, g.hd, g.scale, tiles + wave * TE);
+  store_rows<T, D>(g.o0 + bk * (int64_t)r.t_k * g.hd, gk, wk0, r.t_k, g.hd, g.scale * ds_down<T>(), tiles + wave * TE);
   store_rows<T, D>(g.o1 + bk * (int64_t)r.t_k * g.hd, gv, wk0, r.t_k, g.hd, DOWN, tiles + wave * TE);
 }
 
@@ -766,6 +775,7 @@ __global__ __launch_bounds__(64 * KV_WAVES, 1) void attend_dkv_wide(FastArgs g, 
   constexpr bool RAW = !CAP && !BIAS;
   constexpr int KS = D / 16, DT = D / 32;
   constexpr float UP = shift_of<T>(14.f), DOWN = std::is_same<T, F16>::value ? 1.f / 16384.f : 1.f;
+  constexpr float DS = DOWN / ds_down<T>();  // turns p 2^14 (dp - delta) into dS 2^8
   __shared__ __attribute__((aligned(1024))) u16 Q0[TILE * 128];
   __shared__ __attribute__((aligned(1024))) u16 Q1[TILE * 128];
   __shared__ __attribute__((aligned(1024))) u16 O0[TILE * 128];
@@ -852,7 +862,7 @@ __global__ __launch_bounds__(64 * KV_WAVES, 1) void attend_dkv_wide(FastArgs g, 
   auto stats_store = [&](int buf) __attribute__((always_inline)) {
     if (wave == 0) {
       Ls[buf][lane] = att_l2(lnext) - UP;
-      Ds[buf][lane] = dnext * DOWN;
+      Ds[buf][lane] = dnext * DS;
     }
     if (wave == 1 && ranges != nullptr) qdocs[buf][lane] = qnext;
   };
@@ -908,7 +918,7 @@ __global__ __launch_bounds__(64 * KV_WAVES, 1) void attend_dkv_wide(FastArgs g, 
         float bent = 1.f;
         const float y = bend<CAP, BIAS, true>(s[i], r, slope2, near + (float)(8 * (i >> 2) + (i & 3)), bent);
         float e = fast_exp2(RAW ? fmaf(y, r.c2, -l4[i & 3]) : y - l4[i & 3]);
-        float d = e * fmaf(dp[i], DOWN, -d4[i & 3]) * (CAP ? bent : 1.f);  // times scale once, at the store
+        float d = e * fmaf(dp[i], DS, -d4[i & 3]) * (CAP ? bent : 1.f);  // times scale once, at the store
         if (decltype(tests)::value) {
           const int qq = s0 + 8 * (i >> 2) + 4 * h + (i & 3), qd = (i & 3) == 0 ? q4.x : (i & 3) == 1 ? q4.y : (i & 3) == 2 ? q4.z : q4.w;
           const bool see = (qq < r.t_q) & (doc >= 0) & (qd == doc) & sees(r, r.off + qq, key);
@@ -1018,7 +1028,7 @@ __global__ __launch_bounds__(64 * KV_WAVES, 1) void attend_dkv_wide(FastArgs g, 
         }
       }
     u16* stage = (u16*)part_k;  // which only this wave reads from now on
-    store_rows<T, D>(g.o0 + bk * (int64_t)r.t_k * g.hd, gk, wk0, r.t_k, g.hd, g.scale, stage);
+    store_rows<T, D>(g.o0 + bk * (int64_t)r.t_k * g.hd, gk, wk0, r.t_k, g.hd, g.scale * ds_down<T>(), stage);
     store_rows<T, D>(g.o1 + bk * (int64_t)r.t_k * g.hd, gv, wk0, r.t_k, g.hd, DOWN, stage);
   }
 #endif
@@ -1312,7 +1322,7 @@ __global__ __launch_bounds__(THREADS, 2) void attend_dq_wide(FastArgs g, RuleArg
   }
   delta = pair_sum(delta);
   if (h == 0 && there) g.delta[rows0 + qb.row] = delta;
-  const float l2 = there ? att_l2(g.lse_in[rows0 + qb.row]) : __builtin_inff();
+  const float l2 = there ? att_l2(g.lse_in[rows0 + qb.row]) - shift_of<T>(DS_BITS) : __builtin_inff();
   qb.p = r.off + qb.row;
   qb.doc = there ? query_doc(r, qb.p) : -1;
   const int4* ranges = g.ranges ? g.ranges + qb.b * g.granules : nullptr;
@@ -1413,7 +1423,7 @@ __global__ __launch_bounds__(THREADS, 2) void attend_dq_wide(FastArgs g, RuleArg
   const bool odd = any_odd(acc);  // a barrier: the tile buffers become staging below
   if (threadIdx.x == 0) g.odd[qb.bh * qb.nqb + qb.q0 / ATT_ROWS] = odd;
   u16* stage = wave == 0 ? K0 : wave == 1 ? K1 : wave == 2 ? V0 : V1;
-  store_rows<T, D>(g.o0 + rows0 * g.hd, acc, qb.wq0, r.t_q, g.hd, g.scale, stage);
+  store_rows<T, D>(g.o0 + rows0 * g.hd, acc, qb.wq0, r.t_q, g.hd, g.scale * ds_down<T>(), stage);
 #endif
 }
 

@@ -36,6 +36,9 @@ namespace {
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 constexpr int64_t PIECE_BYTES = (int64_t)128 << 20;
 
+template <typename T>
+constexpr bool IS_F16 = std::is_same<T, F16>::value;
+
 __device__ __forceinline__ f32x16 zero16() {
   f32x16 z;
 #pragma unroll
@@ -205,6 +208,7 @@ struct Logits {
   u16* dz;              // (PARTS, padded rows, ldz)
   int64_t ldz, part_dz;
   int* flags;           // one a 64 rows: a row without a target has logits that are not finite
+  const float* scale;   // float16: what dz is multiplied by, and its inverse
 };
 
 #define LIMN_XENT_LDS(BM)                                                          \
@@ -326,6 +330,30 @@ __global__ __launch_bounds__(256) void xent_rows(const float2* __restrict__ stat
   }
 }
 
+// dz = g (p - [v = target]) can lie far below float16's numbers where g is a mean's 1 / rows and p one of many: it goes
+// multiplied by the power of two that brings the largest |g| (of the finite ones with a target) to [2^14, 2^15), which
+// the products' stores take off again. One workgroup; {power, inverse}.
+__global__ __launch_bounds__(1024) void xent_scale(const float* __restrict__ g, const int* __restrict__ targets, int64_t rows, int64_t vocab, float* __restrict__ scale) {
+  __shared__ float most[16];
+  float m = 0.f;
+#pragma unroll 4
+  for (int64_t r = threadIdx.x; r < rows; r += 1024) {
+    const float v = fabsf(g[r]);
+    const int t = targets[r];
+    if (t >= 0 && t < vocab && v <= 3.402823466e38f) m = fmaxf(m, v);
+  }
+#pragma unroll
+  for (int d = 32; d > 0; d /= 2) m = fmaxf(m, __shfl_xor(m, d));
+  if ((threadIdx.x & 63) == 0) most[threadIdx.x >> 6] = m;
+  __syncthreads();
+  if (threadIdx.x != 0) return;
+  for (int i = 1; i < 16; i++) m = fmaxf(m, most[i]);
+  const int bits = m == 0.f ? 0 : 14 - ilogbf(m);
+  const int e = bits < 120 ? bits : 120;  // the inverse stays a normal number
+  scale[0] = ldexpf(1.f, e);
+  scale[1] = ldexpf(1.f, -e);
+}
+
 // ---- backward: a tile of logits into dz -------------------------------------------------------------------
 
 template <typename T, int BM, int PARTS, bool TAIL>
@@ -341,6 +369,7 @@ __global__ __launch_bounds__(64 * Tile<BM>::WAVES, 2) void xent_dz(Logits a) {
   tile_product<T, BM, PARTS, true, true, TAIL>(da, db, a.part_x, a.part_w, A0, A1, B0, B1, (int)((a.width + BK - 1) / BK), (int)a.width, wave, lane, acc, no_fix);
 
   const int64_t col0 = n0 + wn * 64;
+  const float up = IS_F16<T> ? a.scale[0] : 1.f;
   __syncthreads();
   // each wave writes its rows' halves through 8 KB of LDS, 64 rows at a time, and stores whole 128-byte
   // segments; rows past the end and columns past the piece are zeros, which both products count on
@@ -355,7 +384,7 @@ __global__ __launch_bounds__(64 * Tile<BM>::WAVES, 2) void xent_dz(Logits a) {
     const int t32 = row < a.rows ? a.targets[row] : -1;
     const bool live = t32 >= 0 && t32 < a.vocab;
     const int64_t t = (int64_t)t32 - a.v0 - col0;
-    const float l2 = live ? a.lse[row] * LOG2E : 0.f, g = live ? a.g[row] : 0.f;
+    const float l2 = live ? a.lse[row] * LOG2E : 0.f, g = live ? a.g[row] * up : 0.f;
     bool bad = false;
 #pragma unroll
     for (int j = 0; j < L::TN; j++)
@@ -427,6 +456,7 @@ struct Products {
   const float* add;      // (m, n) float32 added to an unsplit result, or nullptr
   const int* flags;      // dw: see xent_dz; a flagged stage's rows of x without a target are taken as zeros
   const int* targets;
+  const float* scale;    // float16: see xent_scale
   int64_t rows, vocab;
 };
 
@@ -434,6 +464,7 @@ struct Products {
 template <typename T>
 __device__ __forceinline__ void store4(const Products& s, int64_t row, int64_t col, f32x4 v) {
   if (col >= s.width) return;
+  if (IS_F16<T>) v *= s.scale[1];
   if (s.out_f32) {
     float* o = (float*)s.out + row * s.width + col;
     if (s.vec) {
@@ -758,6 +789,12 @@ int bwd(const XentArgs& a) {
   l.x = (const u16*)a.x, l.targets = a.targets, l.rows = a.rows, l.width = width, l.vocab = a.vocab, l.lse = a.lse_in, l.g = a.g;
   l.dz = (u16*)space.take(PARTS * p.rows_pad * p.piece * 2);
   l.flags = (int*)space.take(p.rows_pad / 64 * 4);
+  if (IS_F16<T>) {
+    float* scale = (float*)space.take(8);
+    hipLaunchKernelGGL(xent_scale, dim3(1), dim3(1024), 0, a.stream, a.g, a.targets, a.rows, a.vocab, scale);
+    if (const int bad = check_hip(hipGetLastError(), "launching the gradient's scale"); bad != LIMN_HIP_OK) return bad;
+    l.scale = scale;
+  }
   float* slices = (float*)space.take(p.slices);
   float* acc = p.pieces > 1 ? (float*)space.take(a.rows * width * 4) : nullptr;
   u16* wp = nullptr;
@@ -785,7 +822,7 @@ int bwd(const XentArgs& a) {
     rc = tile_for(a.rows, l.ldz) == 256 ? launch_dz<T, 256, PARTS>(l, a.stream) : launch_dz<T, 128, PARTS>(l, a.stream);
     if (rc != LIMN_HIP_OK) return rc;
     Products s = {};
-    s.rows = a.rows, s.vocab = a.vocab, s.targets = a.targets, s.flags = l.flags;
+    s.rows = a.rows, s.vocab = a.vocab, s.targets = a.targets, s.flags = l.flags, s.scale = l.scale;
     s.out_f32 = f32(a), s.width = a.width, s.n = width;
     s.a = l.dz, s.part_a = l.part_dz, s.b = l.w, s.part_b = l.part_w, s.m = a.rows, s.k = up(l.piece, 64);
     s.a_rows = p.rows_pad, s.a_depth = l.ldz, s.a_stride = l.ldz, s.b_depth = l.piece, s.b_stride = width, s.b_cols = width;
@@ -817,7 +854,7 @@ int64_t workspace_of(const XentArgs& a, bool backward, bool copies) {
   int64_t need = copies ? xent_align(a.rows * row) + xent_align(piece_of(a, backward, copies) * row) : 0;
   if (!backward) return need + xent_align(((a.vocab + 127) / 128) * a.rows * 8) + xent_align(a.rows * 4);
   const BwdPlan p = bwd_plan(a, copies);
-  need += xent_align(parts * p.rows_pad * p.piece * 2) + xent_align(p.rows_pad / 64 * 4) + xent_align(p.slices);
+  need += xent_align(parts * p.rows_pad * p.piece * 2) + xent_align(p.rows_pad / 64 * 4) + xent_align(8) + xent_align(p.slices);
   return need + (p.pieces > 1 ? xent_align(a.rows * width * 4) : 0);
 }
 

@@ -16,7 +16,7 @@ step of the storage type (torch.finfo(t).eps / 2) and f that of float32, 2^-24:
     numbers): it is off by up to that number, which no relative bound covers;
   - a float16 operand below 2^-14, the least normal one, is off by up to 2^-25 absolutely: the kernels multiply
     the forward's weights by 2^7 and the dV product's by 2^14 first, so 2^-32 and 2^-39 of a weight; the
-    score gradients are taken as they are, scale apart, so 2^-25;
+    score gradients, scale apart, by 2^8, so 2^-33;
   - every stored result rounds once more: u times its value, and up to the least number of its type where the
     value is below it (float32 and bfloat16 sums and stores may take subnormal numbers as 0).
 """
@@ -106,7 +106,7 @@ def attend(q, k, v, *, causal=False, softcap=0.0, slopes=None, documents=None, p
                 ddp = (hd_v + 8) * F * (fine(G) @ fine(V).T)
                 ds = np.where(seen, p * (dp - delta) * scale * bent, 0.0)
                 size = np.where(seen, p * abs(scale) * bent, 0.0)
-                dds = np.abs(ds) * (rel + 8 * F + operand) + size * (ddelta + ddp) + np.where(seen, TINY * (1 + fine(dp - delta) * abs(scale)) + small * 2.0**-25 * abs(scale), 0.0)
+                dds = np.abs(ds) * (rel + 8 * F + operand) + size * (ddelta + ddp) + np.where(seen, TINY * (1 + fine(dp - delta) * abs(scale)) + small * 2.0**-33 * abs(scale), 0.0)
                 if softcap:  # 1 - tanh^2, off by twice the tanh's own 4 f and by the score's
                     dds = dds + np.where(seen, np.abs(p * (dp - delta)) * abs(scale), 0.0) * (16 * F + 2 * e / softcap)
                 kv = h // group
@@ -160,8 +160,9 @@ def xent(x, w, targets, g=None, dtype="float32"):
     dx, dw = dz @ w, dz.T @ xs
     dxo = ddz @ np.abs(w) + (vocab + 8) * F * (np.abs(dz) @ np.abs(w)) + u * np.abs(dx) + least
     dwo = ddz.T @ np.abs(xs) + (rows + 8) * F * (np.abs(dz).T @ np.abs(xs)) + u * np.abs(dw) + least
-    # a dz, or a float32 one's last part, below its type's least normal number is off by a part of that number
-    tiny = 2.0**-24 if dtype == "float16" else TINY
+    # a dz, or a float32 one's last part, below its type's least normal number is off by a part of that number; float16's
+    # are multiplied by a power of two that brings the largest |g| to 2^14 or more, so 2^-25 2^-14 of that is left
+    tiny = 2.0**-39 * np.abs(g).max(initial=0.0) + TINY if dtype == "float16" else TINY
     dxo = dxo + tiny * np.abs(w).sum(0) + lost * np.abs(dz).sum(1, keepdims=True)
     dwo = dwo + tiny * np.abs(xs).sum(0) + lost * np.abs(dz).sum(0)[:, None]
     out.update(dx=(dx, dxo), dw=(dw, dwo))

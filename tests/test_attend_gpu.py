@@ -65,6 +65,18 @@ def test_lengths(hipdev, dtype, t_q, t_k):
     check(hipdev, q, k, v, do, dtype, {}, dict())
 
 
+@pytest.mark.parametrize("dtype", HALVES)
+@pytest.mark.parametrize("hd", [64, 80, 128])
+@pytest.mark.parametrize("bits", [-12, 10])
+def test_cotangents_of_every_size(hipdev, dtype, hd, bits):
+    """A mean's cotangents, and a loss multiplied up: float16's numbers reach neither products of small ones nor,
+    past 2^16, of large ones."""
+    rng, (q, k, v, do) = draw(hd + bits, dtype, 1, 2, 1, 190, 190, hd, hd)
+    do = storage_values(do * np.float32(2.0**bits), DTYPES[dtype])
+    check(hipdev, q, k, v, do, dtype, {}, dict(causal=True))
+    check(hipdev, q, k, v, do, dtype, dict(slopes=np.array([0.25, 0.0625], np.float32)), dict(causal=True, softcap=5.0))
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("hd,hd_v", [(1, 1), (8, 8), (16, 16), (32, 32), (33, 33), (40, 40), (64, 64), (64, 80), (72, 72), (80, 80), (96, 96), (100, 100), (128, 128), (128, 64), (160, 200), (256, 256)])
 def test_head_dims(hipdev, dtype, hd, hd_v):

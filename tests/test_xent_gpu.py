@@ -83,6 +83,27 @@ def test_several_pieces_of_the_vocabulary(hipdev, dtype):
     check(hipdev, x, w, targets, (rng.random(rows) / rows).astype(np.float32), dtype)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("bits", [-130, -20, -12, 8, (-20, 4)])
+def test_cotangents_of_every_size(hipdev, dtype, bits):
+    """A mean over many rows, a loss multiplied up, and rows of very unlike weight."""
+    rng, x, w, targets = draw(11, dtype, 150, 72, 1111, left_out=0.2)
+    g = rng.standard_normal(150) * (2.0**bits if isinstance(bits, int) else np.exp2(rng.integers(*bits, 150)))
+    check(hipdev, x, w, targets, g.astype(np.float32), dtype)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_cotangents_of_rows_left_out(hipdev, dtype):
+    """Whatever a row without a target gets as its cotangent, the others' gradients hold their bits."""
+    rng, x, w, targets = draw(12, dtype, 70, 64, 300, left_out=0.3)
+    g = rng.standard_normal(70).astype(np.float32) * np.float32(2.0**-14)
+    want = check(hipdev, x, w, targets, g, dtype)
+    g[targets < 0] = np.resize(np.float32([np.inf, np.nan, 1e38]), (targets < 0).sum())
+    got = check(hipdev, x, w, targets, g, dtype)
+    for name in want:
+        np.testing.assert_array_equal(got[name], want[name])
+
+
 def test_float32_numbers_of_every_size(hipdev):
     """Rows scaled from 2^-120 to 2^120 and back by the weight's columns: a float32 goes to its products in parts, each of which must hold its bits."""
     rng, x, w, targets = draw(9, "float32", 100, 64, 300)
