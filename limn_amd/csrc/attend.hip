@@ -136,16 +136,22 @@ int check_pointers(const char* name, const AttendArgs& a, bool backward) {
   return LIMN_HIP_OK;
 }
 
-// ---- the half-width kernels ----
+// ---- the tiled kernels ----
 
 int64_t granules_of(const AttendArgs& a) { return (a.t_k + 31) / 32; }
 int64_t row_blocks(const AttendArgs& a) { return a.batch * a.heads * ((a.t_q + ATT_ROWS - 1) / ATT_ROWS); }
 int64_t key_blocks(const AttendArgs& a) { return a.batch * a.kv_heads * ((a.t_k + ATT_ROWS - 1) / ATT_ROWS); }
 
-// Sizes the half-width kernels serve: 16-byte rows; the tiled ones also need a head's rows within 32-bit byte
+// float32 calls go to the tiles of 128 rows where the general kernels, with a workgroup for every 32, have more than
+// one for a CU. Causal at 64 dims, forward and backward, tiled against general: 8 heads x 256 rows 24 + 67 against
+// 18 + 57 us, 8 x 1024 64 + 196 against 77 + 181, 16 x 1024 65 + 197 against 107 + 355, 64 x 1024 94 + 260 against 423 + 1393.
+bool f32_rows(const AttendArgs& a) { return a.batch * a.heads * ((a.t_q + 31) / 32) > 256; }
+
+// Sizes these kernels serve: 16-byte rows; the tiled ones also need a head's rows within 32-bit byte
 // offsets and few enough streamed tiles for a block's list of them.
-bool half_sizes(const AttendArgs& a) { return a.dtype != LIMN_HIP_FLOAT32 && a.hd == a.hd_v && a.hd % 8 == 0 && a.hd <= 128; }
-bool fast_sizes(const AttendArgs& a) { return half_sizes(a) && a.t_q <= (1 << 17) && a.t_k <= (1 << 17); }
+bool row_sizes(const AttendArgs& a) { return a.hd == a.hd_v && a.hd % (a.dtype == LIMN_HIP_FLOAT32 ? 4 : 8) == 0 && a.hd <= 128; }
+bool half_sizes(const AttendArgs& a) { return a.dtype != LIMN_HIP_FLOAT32 && row_sizes(a); }
+bool fast_sizes(const AttendArgs& a) { return row_sizes(a) && a.t_q <= (1 << 17) && a.t_k <= (1 << 17) && (a.dtype != LIMN_HIP_FLOAT32 || f32_rows(a)); }
 
 bool aligned16(const AttendArgs& a, bool backward) {
   const uintptr_t at = (uintptr_t)a.q | (uintptr_t)a.k | (uintptr_t)a.v | (uintptr_t)a.o0 | (backward ? (uintptr_t)a.o1 | (uintptr_t)a.o2 | (uintptr_t)a.out | (uintptr_t)a.dout : 0);
@@ -177,8 +183,9 @@ int head_group(const AttendArgs& a, int64_t heads) {
   return heads < 8 || (heads < 64 && heads % (8 * group) != 0) ? 0 : group;
 }
 
-#define LIMN_ATTEND_WIDTH(PASS) \
-  (a.hd <= 64 ? launch_attend_##PASS##_64 : a.hd <= 96 ? launch_attend_##PASS##_96 : launch_attend_##PASS##_128)
+#define LIMN_ATTEND_PASS(PASS, G)                                       \
+  (a.dtype == LIMN_HIP_FLOAT32 ? launch_attend_##PASS##_parts(G, ra, a.stream) \
+                               : (a.hd <= 64 ? launch_attend_##PASS##_64 : a.hd <= 96 ? launch_attend_##PASS##_96 : launch_attend_##PASS##_128)(G, ra, a.dtype, a.stream))
 
 int launch_fast(const AttendArgs& a, bool backward) {
   const RuleArgs ra = rule_args(a);
@@ -197,11 +204,12 @@ int launch_fast(const AttendArgs& a, bool backward) {
   g.head_group = head_group(a, a.batch * a.heads);
   int rc = LIMN_HIP_OK;
   if (a.documents != nullptr && (rc = launch_attend_ranges(ra, ranges, a.batch, g.granules, a.stream)) != LIMN_HIP_OK) return rc;
-  // without causality and documents a hidden key is one past the live ones, which reads as zeros
-  const bool mend = a.causal || a.documents != nullptr;
+  // without causality and documents a hidden key is one past the live ones, which reads as zeros; float32's parts do
+  // not hold infinities
+  const bool mend = a.causal || a.documents != nullptr || a.dtype == LIMN_HIP_FLOAT32;
   if (!backward) {
     g.lse = (float*)a.o1;
-    rc = LIMN_ATTEND_WIDTH(fwd)(g, ra, a.dtype, a.stream);
+    rc = LIMN_ATTEND_PASS(fwd, g);
     return rc != LIMN_HIP_OK || !mend ? rc : launch_attend_mend_fwd(g, ra, a.dtype, a.stream);
   }
   FastArgs kv = g;
@@ -210,8 +218,8 @@ int launch_fast(const AttendArgs& a, bool backward) {
   kv.o0 = (u16*)a.o1;
   kv.o1 = (u16*)a.o2;
   kv.head_group = head_group(a, a.batch * a.kv_heads);
-  if ((rc = LIMN_ATTEND_WIDTH(dq)(g, ra, a.dtype, a.stream)) != LIMN_HIP_OK) return rc;
-  rc = LIMN_ATTEND_WIDTH(dkv)(kv, ra, a.dtype, a.stream);
+  if ((rc = LIMN_ATTEND_PASS(dq, g)) != LIMN_HIP_OK) return rc;
+  rc = LIMN_ATTEND_PASS(dkv, kv);
   return rc != LIMN_HIP_OK || !mend ? rc : launch_attend_mend_bwd(g, kv, ra, a.dtype, a.stream);
 }
 

@@ -1,4 +1,5 @@
-// Arguments of the half-width kernels of attention with score rules (attend_mfma.h), of the kernel that finds
+// Arguments of the tiled kernels of attention with score rules (attend_mfma.h for half widths, attend_parts.h for
+// float32, whose buffers are float), of the kernel that finds
 // documents' ranges and of the one that mends blocks with non-finite totals (attend_mend.hip).
 #pragma once
 
@@ -41,6 +42,9 @@ int launch_attend_mend_rows(const AttendArgs& a);
 LIMN_ATTEND_PASSES(64)
 LIMN_ATTEND_PASSES(96)
 LIMN_ATTEND_PASSES(128)
+int launch_attend_fwd_parts(const FastArgs& g, const RuleArgs& ra, hipStream_t stream);
+int launch_attend_dq_parts(const FastArgs& g, const RuleArgs& ra, hipStream_t stream);
+int launch_attend_dkv_parts(const FastArgs& g, const RuleArgs& ra, hipStream_t stream);
 #undef LIMN_ATTEND_PASSES
 
 }  // namespace limn

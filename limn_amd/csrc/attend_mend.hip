@@ -1,4 +1,4 @@
-// Beside the half-width kernels of attention with score rules (attend_mfma.h): the ranges of documents that
+// Beside the tiled kernels of attention with score rules (attend_mfma.h, attend_parts.h): the ranges of documents that
 // let them skip tiles, and the blocks that hidden infinities or NaN spoiled, computed again in float.
 
 #include "attend_fast.h"
@@ -142,11 +142,13 @@ int launch_attend_ranges(const RuleArgs& ra, int4* ranges, int64_t batch, int gr
 }
 
 int launch_attend_mend_fwd(const FastArgs& g, const RuleArgs& ra, int dtype, hipStream_t stream) {
+  if (dtype == LIMN_HIP_FLOAT32) return g.hd <= 64 ? mend_fwd<F32, 2>(g, ra, stream) : mend_fwd<F32, 4>(g, ra, stream);
   if (dtype == LIMN_HIP_BFLOAT16) return g.hd <= 64 ? mend_fwd<BF16, 2>(g, ra, stream) : mend_fwd<BF16, 4>(g, ra, stream);
   return g.hd <= 64 ? mend_fwd<F16, 2>(g, ra, stream) : mend_fwd<F16, 4>(g, ra, stream);
 }
 
 int launch_attend_mend_bwd(const FastArgs& g, const FastArgs& kv, const RuleArgs& ra, int dtype, hipStream_t stream) {
+  if (dtype == LIMN_HIP_FLOAT32) return g.hd <= 64 ? mend_bwd<F32, 2>(g, kv, ra, stream) : mend_bwd<F32, 4>(g, kv, ra, stream);
   if (dtype == LIMN_HIP_BFLOAT16) return g.hd <= 64 ? mend_bwd<BF16, 2>(g, kv, ra, stream) : mend_bwd<BF16, 4>(g, kv, ra, stream);
   return g.hd <= 64 ? mend_bwd<F16, 2>(g, kv, ra, stream) : mend_bwd<F16, 4>(g, kv, ra, stream);
 }

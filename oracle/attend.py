@@ -17,6 +17,9 @@ step of the storage type (torch.finfo(t).eps / 2) and f that of float32, 2^-24:
   - a float16 operand below 2^-14, the least normal one, is off by up to 2^-25 absolutely: the kernels multiply
     the forward's weights by 2^7 and the dV product's by 2^14 first, so 2^-32 and 2^-39 of a weight; the
     score gradients, scale apart, by 2^8, so 2^-33;
+  - a float32 operand goes as three bfloat16 numbers, each rounded from what the ones before leave: 24 bits, or as
+    many as there are above bfloat16's least step, 2^-133, so it is off by up to 2^-134 and a product by that
+    times the other operand (a weight by less than 2^-126, which it already is);
   - every stored result rounds once more: u times its value, and up to the least number of its type where the
     value is below it (float32 and bfloat16 sums and stores may take subnormal numbers as 0).
 """
@@ -61,6 +64,7 @@ def attend(q, k, v, *, causal=False, softcap=0.0, slopes=None, documents=None, p
     u, least = HALF_STEP[dtype], LEAST[dtype]
     operand = 0.0 if dtype == "float32" else u
     small = 1.0 if dtype == "float16" else 0.0
+    lost = 2.0**-134 if dtype == "float32" else 0.0
     q, k, v = (np.asarray(x, dtype=np.float64) for x in (q, k, v))
     shapes = dict(out=q.shape[:-1] + (hd_v,), lse=q.shape[:-1], dq=q.shape, dk=k.shape, dv=v.shape)
     got = {n: np.zeros(s) for n, s in shapes.items()}
@@ -74,7 +78,7 @@ def attend(q, k, v, *, causal=False, softcap=0.0, slopes=None, documents=None, p
             for h in range(heads):
                 Q, K, V = q[b, h], k[b, h // group], v[b, h // group]
                 x = np.where(seen, Q @ K.T, 0.0) * scale
-                e = (hd + 8) * F * abs(scale) * (fine(Q) @ fine(K).T) + 4 * F * np.abs(x)
+                e = (hd + 8) * F * abs(scale) * (fine(Q) @ fine(K).T) + 4 * F * np.abs(x) + lost * abs(scale) * (fine(Q).sum(1)[:, None] + fine(K).sum(1)[None, :])
                 bent = 1.0
                 s = x
                 if softcap:
@@ -103,7 +107,7 @@ def attend(q, k, v, *, causal=False, softcap=0.0, slopes=None, documents=None, p
                 dp = np.where(seen, G @ V.T, 0.0)
                 delta = (np.where(n > 0, G, 0.0) * O).sum(1, keepdims=True)
                 ddelta = (fine(G) * (off["out"][b, h] + hd_v * F * fine(O))).sum(1, keepdims=True)
-                ddp = (hd_v + 8) * F * (fine(G) @ fine(V).T)
+                ddp = (hd_v + 8) * F * (fine(G) @ fine(V).T) + lost * (fine(G).sum(1)[:, None] + fine(V).sum(1)[None, :])
                 ds = np.where(seen, p * (dp - delta) * scale * bent, 0.0)
                 size = np.where(seen, p * abs(scale) * bent, 0.0)
                 dds = np.abs(ds) * (rel + 8 * F + operand) + size * (ddelta + ddp) + np.where(seen, TINY * (1 + fine(dp - delta) * abs(scale)) + small * 2.0**-33 * abs(scale), 0.0)
@@ -111,10 +115,10 @@ def attend(q, k, v, *, causal=False, softcap=0.0, slopes=None, documents=None, p
                     dds = dds + np.where(seen, np.abs(p * (dp - delta)) * abs(scale), 0.0) * (16 * F + 2 * e / softcap)
                 kv = h // group
                 got["dq"][b, h] = _product(ds, K)
-                off["dq"][b, h] = dds @ fine(K) + (n + 8) * F * (np.abs(ds) @ fine(K)) + u * fine(got["dq"][b, h]) + least
+                off["dq"][b, h] = dds @ fine(K) + lost * np.abs(ds).sum(1, keepdims=True) + (n + 8) * F * (np.abs(ds) @ fine(K)) + u * fine(got["dq"][b, h]) + least
                 m = seen.sum(0)[:, None] * group
                 got["dk"][b, kv] += _product(ds.T, Q)
-                off["dk"][b, kv] += dds.T @ fine(Q) + (m + 8) * F * (np.abs(ds).T @ fine(Q))
+                off["dk"][b, kv] += dds.T @ fine(Q) + lost * np.abs(ds).sum(0)[:, None] + (m + 8) * F * (np.abs(ds).T @ fine(Q))
                 got["dv"][b, kv] += _product(p.T, G)
                 off["dv"][b, kv] += (p * (rel + operand) + (TINY + small * 2.0**-39) * seen).T @ fine(G) + (m + 8) * F * (p.T @ fine(G))
     for name in ("dk", "dv"):
