@@ -88,6 +88,35 @@ int join(const AttendArgs& a, const float* totals, const float* stats, int64_t s
   return check_hip(hipGetLastError(), "joining attention's splits");
 }
 
+// dk and dv of the key rows: the parts' totals added in order and rounded (4 elements a thread), blocks with one that is
+// not finite flagged.
+template <typename T>
+__global__ __launch_bounds__(256) void attend_join_keys(const float* __restrict__ partial, int parts, typename T::Storage* __restrict__ dk,
+                                                        typename T::Storage* __restrict__ dv, int* __restrict__ odd, int64_t elements, int hd, int t_k) {
+  const int64_t i = (blockIdx.x * (int64_t)256 + threadIdx.x) * 4;
+  if (i >= elements) return;
+  const float* at = partial + blockIdx.y * elements + i;
+  f32x4 v = *(const f32x4*)at;
+#pragma unroll 4
+  for (int k = 1; k < parts; k++) v += *(const f32x4*)(at + 2 * k * elements);
+  typename T::Storage* o = blockIdx.y ? dv : dk;
+#pragma unroll
+  for (int e = 0; e < 4; e++) T::store(o, i + e, v[e]);
+  const f32x4 zero = v * 0.f;
+  if (zero[0] + zero[1] + zero[2] + zero[3] != 0.f) {
+    const int64_t row = i / hd, bk = row / t_k;
+    atomicOr(odd + bk * ((t_k + ATT_ROWS - 1) / ATT_ROWS) + (row - bk * t_k) / ATT_ROWS, 1);
+  }
+}
+
+template <typename T>
+int join_keys(const AttendArgs& a, const FastArgs& kv) {
+  const int64_t elements = a.batch * a.kv_heads * a.t_k * a.hd, groups = (elements / 4 + 255) / 256;
+  hipLaunchKernelGGL((attend_join_keys<T>), dim3((unsigned)groups, 2), dim3(256), 0, a.stream, kv.partial, kv.head_parts * kv.tile_parts,
+                     (typename T::Storage*)a.o1, (typename T::Storage*)a.o2, kv.odd, elements, (int)a.hd, (int)a.t_k);
+  return check_hip(hipGetLastError(), "joining attention's key parts");
+}
+
 constexpr int64_t FILL = 512;  // workgroups that give every CU two
 
 // Parts of the keys a general forward is cut into: rows in too few tiles to fill the GPU walk long
@@ -166,11 +195,31 @@ bool token_sizes(const AttendArgs& a) { return half_sizes(a) && a.t_q < 64; }
 // reference point is taken over unscaled scores).
 bool fast_call(const AttendArgs& a, bool backward) { return fast_sizes(a) && a.scale > 0 && aligned16(a, backward); }
 
+// Parts of the queries that a call with fewer key blocks than fill the GPU (two workgroups a CU up to 64 half-width
+// dims, one else) cuts its dK/dV pass into, the heads of a group first: at least 4 tiles each. The backward of 16 heads
+// over 2 key heads, 2048 x 128 bf16 causal, 505 -> 154 us; 12 over 3, 901 x 80 float32, 862 -> 235; 16 over 16,
+// 512 x 64 bf16, whose parts are short, 41.0 -> 41.8.
+struct KeyParts {
+  int heads, tiles;
+};
+KeyParts key_parts(const AttendArgs& a) {
+  const int64_t fill = a.dtype != LIMN_HIP_FLOAT32 && a.hd <= 64 ? 512 : 256, tiles = (a.t_q + 63) / 64;
+  int64_t want = fill / key_blocks(a);
+  if (want > a.group() * tiles / 4) want = a.group() * tiles / 4;
+  if (want < 2) return {1, 1};
+  const int64_t heads = want < a.group() ? want : a.group();
+  return {(int)heads, (int)(want / heads)};
+}
+int64_t key_parts_bytes(const AttendArgs& a) {
+  const KeyParts p = key_parts(a);
+  return p.heads * p.tiles > 1 ? p.heads * p.tiles * 2 * a.batch * a.kv_heads * a.t_k * a.hd * 4 : 0;
+}
+
 // flags of the blocks, the documents' ranges, and for the backward delta
 int64_t fast_workspace(const AttendArgs& a, bool backward) {
   if (!fast_sizes(a)) return 0;
   int64_t need = attend_align(row_blocks(a) * 4) + attend_align(a.batch * granules_of(a) * 16);
-  if (backward) need += attend_align(key_blocks(a) * 4) + attend_align(a.batch * a.heads * a.t_q * 4);
+  if (backward) need += attend_align(key_blocks(a) * 4) + attend_align(a.batch * a.heads * a.t_q * 4) + attend_align(key_parts_bytes(a));
   return need;
 }
 
@@ -218,8 +267,13 @@ int launch_fast(const AttendArgs& a, bool backward) {
   kv.o0 = (u16*)a.o1;
   kv.o1 = (u16*)a.o2;
   kv.head_group = head_group(a, a.batch * a.kv_heads);
+  const KeyParts parts = key_parts(a);
+  kv.head_parts = parts.heads, kv.tile_parts = parts.tiles;
+  kv.partial = parts.heads * parts.tiles > 1 ? (float*)take(key_parts_bytes(a)) : nullptr;
   if ((rc = LIMN_ATTEND_PASS(dq, g)) != LIMN_HIP_OK) return rc;
   rc = LIMN_ATTEND_PASS(dkv, kv);
+  if (rc == LIMN_HIP_OK && kv.partial != nullptr)
+    rc = a.dtype == LIMN_HIP_FLOAT32 ? join_keys<F32>(a, kv) : a.dtype == LIMN_HIP_FLOAT16 ? join_keys<F16>(a, kv) : join_keys<BF16>(a, kv);
   return rc != LIMN_HIP_OK || !mend ? rc : launch_attend_mend_bwd(g, kv, ra, a.dtype, a.stream);
 }
 

@@ -26,6 +26,10 @@ struct FastArgs {
   int heads, kv_heads, hd, granules;
   int head_group;      // see att_head_and_block
   float scale;
+  // dK/dV pass of a call with too few key blocks for the GPU: blockIdx.y is a part of the query heads times one of the
+  // query tiles, whose float totals go to partial (part, dk and dv, key rows, hd) for attend_join_keys to add
+  int head_parts, tile_parts;
+  float* partial;
 };
 
 int launch_attend_ranges(const RuleArgs& ra, int4* ranges, int64_t batch, int granules, hipStream_t stream);

@@ -219,6 +219,50 @@ __device__ __forceinline__ void store_rows(u16* base, const f32x16* acc, int row
   }
 }
 
+// 32 rows of float results: a lane holds row n's 4 consecutive elements
+template <int D>
+__device__ __forceinline__ void store_floats(float* base, int64_t first, const f32x16* acc, int row0, int rows, int hd, float mul) {
+  const int lane = threadIdx.x & 63, h = lane >> 5, row = row0 + (lane & 31);
+  if (row >= rows) return;
+  float* o = base + (first + row) * hd;
+#pragma unroll
+  for (int dt = 0; dt < D / 32; dt++)
+#pragma unroll
+    for (int q = 0; q < 4; q++) {
+      const int d = dt * 32 + 8 * q + 4 * h;
+      if (d < hd) *(f32x4*)(o + d) = f32x4{acc[dt][4 * q], acc[dt][4 * q + 1], acc[dt][4 * q + 2], acc[dt][4 * q + 3]} * mul;
+    }
+}
+
+// What of a key block's queries a workgroup of the dK/dV pass takes: heads [g0, g1) of the group and tiles [first, to).
+struct KeyPart {
+  int g0, g1, first, to;
+  __device__ __forceinline__ KeyPart(const FastArgs& g, const Rules& r, int k0, int group) {
+    const int y = blockIdx.y, hp = y / g.tile_parts, tp = y - hp * g.tile_parts;
+    g0 = group * hp / g.head_parts;
+    g1 = group * (hp + 1) / g.head_parts;
+    // from the first tile that can see the block's first key on, unless a prefix opens it to all
+    first = r.causal && k0 >= r.pre ? max(0, k0 - r.off) / TILE : 0;
+    to = k0 < r.len ? (r.t_q + TILE - 1) / TILE : 0;
+    const int tiles = max(0, to - first);
+    to = min(to, first + (int)((int64_t)tiles * (tp + 1) / g.tile_parts));
+    first += (int)((int64_t)tiles * tp / g.tile_parts);
+  }
+};
+
+// The dK and dV totals of a key block, or of a part of it.
+template <int D, typename STORE>
+__device__ __forceinline__ void store_keys(const FastArgs& g, int64_t bk, int t_k, int wk0, const f32x16* gk, const f32x16* gv, float mul_k, float mul_v, STORE store) {
+  if (g.partial == nullptr) {
+    store(gk, g.o0, mul_k);
+    store(gv, g.o1, mul_v);
+    return;
+  }
+  const int64_t keys = g.batch * g.kv_heads * (int64_t)t_k;
+  store_floats<D>(g.partial, (2 * blockIdx.y) * keys + bk * t_k, gk, wk0, t_k, g.hd, mul_k);
+  store_floats<D>(g.partial, (2 * blockIdx.y + 1) * keys + bk * t_k, gv, wk0, t_k, g.hd, mul_v);
+}
+
 // Whether any of the workgroup's totals is not finite.
 template <int N>
 __device__ __forceinline__ bool any_odd(const f32x16 (&acc)[N]) {
@@ -596,9 +640,9 @@ __global__ __launch_bounds__(THREADS, 2) void attend_dkv_mfma(FastArgs g, RuleAr
 #pragma unroll
   for (int dt = 0; dt < D / 32; dt++) gk[dt] = gv[dt] = zero16();
 
-  // query tiles: from the first that can see the block's first key on, unless a prefix opens it to all
-  const int first_q = r.causal && k0 >= r.pre ? max(0, k0 - r.off) / TILE : 0;
-  Visit visit = {k0 < r.len ? (r.t_q + TILE - 1) / TILE : 0};
+  const KeyPart part(g, r, k0, group);
+  const int first_q = part.first;
+  Visit visit = {part.to};
   const int4* ranges = g.ranges ? g.ranges + b * g.granules : nullptr;
   if (ranges != nullptr) {
     const int first = __builtin_amdgcn_readfirstlane(doc);
@@ -638,7 +682,7 @@ __global__ __launch_bounds__(THREADS, 2) void attend_dkv_mfma(FastArgs g, RuleAr
   };
   visit.start(first_q);
   const int begin = visit.next();
-  int gh = 0, cur = begin, ngh = 0, nxt = begin, alike = visit.alike;
+  int gh = part.g0, cur = begin, ngh = gh, nxt = begin, alike = visit.alike;
   // the tile after (ngh, nxt): the head's next, or the next head's first
   auto advance = [&]() __attribute__((always_inline)) {
     nxt = visit.next();
@@ -653,10 +697,10 @@ __global__ __launch_bounds__(THREADS, 2) void attend_dkv_mfma(FastArgs g, RuleAr
     load(gh, cur);
     store(0);
     advance();
-    if (ngh < group) load(ngh, nxt);
+    if (ngh < part.g1) load(ngh, nxt);
   }
   __syncthreads();
-  for (int buf = 0; any && gh < group; buf ^= 1) {
+  for (int buf = 0; any && gh < part.g1; buf ^= 1) {
     const int r0 = cur * TILE;
     const float slope2 = BIAS ? ra.slopes[kvh * group + gh] * LOG2E : 0.f;
     const u16* Qt = tiles + 2 * buf * TE;
@@ -728,17 +772,17 @@ __global__ __launch_bounds__(THREADS, 2) void attend_dkv_mfma(FastArgs g, RuleAr
     gh = ngh;
     cur = nxt;
     alike = visit.alike;
-    if (gh < group) {
+    if (gh < part.g1) {
       store(buf ^ 1);
       advance();
-      if (ngh < group) load(ngh, nxt);
+      if (ngh < part.g1) load(ngh, nxt);
     }
     __syncthreads();
   }
   const bool odd_k = any_odd(gk), odd_v = any_odd(gv);
-  if (threadIdx.x == 0) g.odd[bk * nkb + blk] = odd_k | odd_v;
-  store_rows<T, D>(g.o0 + bk * (int64_t)r.t_k * g.hd, gk, wk0, r.t_k, g.hd, g.scale * ds_down<T>(), tiles + wave * TE);
-  store_rows<T, D>(g.o1 + bk * (int64_t)r.t_k * g.hd, gv, wk0, r.t_k, g.hd, DOWN, tiles + wave * TE);
+  if (threadIdx.x == 0 && blockIdx.y == 0) g.odd[bk * nkb + blk] = g.partial == nullptr && (odd_k | odd_v);
+  store_keys<D>(g, bk, r.t_k, wk0, gk, gv, g.scale * ds_down<T>(), DOWN,
+                [&](const f32x16* acc, u16* o, float mul) __attribute__((always_inline)) { store_rows<T, D>(o + bk * (int64_t)r.t_k * g.hd, acc, wk0, r.t_k, g.hd, mul, tiles + wave * TE); });
 }
 
 // ---- dK/dV pass past 64 dims: two waves per SIMD --------------------------------------------------------------
@@ -829,9 +873,9 @@ __global__ __launch_bounds__(64 * KV_WAVES, 1) void attend_dkv_wide(FastArgs g, 
 #pragma unroll
   for (int dt = 0; dt < DT; dt++) gk[dt] = gv[dt] = zero16();
 
-  // query tiles: from the first that can see the block's first key on, unless a prefix opens it to all
-  const int first_q = r.causal && k0 >= r.pre ? max(0, k0 - r.off) / TILE : 0;
-  Visit visit = {k0 < r.len ? (r.t_q + TILE - 1) / TILE : 0};
+  const KeyPart part(g, r, k0, group);
+  const int first_q = part.first;
+  Visit visit = {part.to};
   const int4* ranges = g.ranges ? g.ranges + b * g.granules : nullptr;
   if (ranges != nullptr) {
     const int first = __builtin_amdgcn_readfirstlane(doc);
@@ -869,7 +913,7 @@ __global__ __launch_bounds__(64 * KV_WAVES, 1) void attend_dkv_wide(FastArgs g, 
 
   visit.start(first_q);
   const int begin = visit.next();
-  int gh = 0, cur = begin, ngh = 0, nxt = begin, alike = visit.alike;
+  int gh = part.g0, cur = begin, ngh = gh, nxt = begin, alike = visit.alike;
   auto advance = [&]() __attribute__((always_inline)) {
     nxt = visit.next();
     if (nxt >= visit.to) {
@@ -960,7 +1004,7 @@ __global__ __launch_bounds__(64 * KV_WAVES, 1) void attend_dkv_wide(FastArgs g, 
   };
   // one tile while the next is copied; behind the last one the last head's is copied again, for nothing
   auto step = [&](int buf, const u16* Qc, const u16* Oc, u16* Qn, u16* On) __attribute__((always_inline)) {
-    load(min(ngh, group - 1), nxt, Qn, On);
+    load(min(ngh, part.g1 - 1), nxt, Qn, On);
     __builtin_amdgcn_sched_barrier(0);
     tile(buf, Qc, Oc);
     __builtin_amdgcn_s_waitcnt(WAIT_VMEM);
@@ -981,12 +1025,12 @@ __global__ __launch_bounds__(64 * KV_WAVES, 1) void attend_dkv_wide(FastArgs g, 
       }
       total = __builtin_amdgcn_readfirstlane(total);
     }
-    total *= group;
+    total *= part.g1 - part.g0;
     dma.copy(Ks, kbase, k0, r.len, wave);
     dma.copy(Ks + TILE * 128, kbase, k0 + TILE, r.len, wave);
     dma.copy(Vs, vbase, k0, r.len, wave);
     dma.copy(Vs + TILE * 128, vbase, k0 + TILE, r.len, wave);
-    load(0, begin, Q0, O0);
+    load(gh, begin, Q0, O0);
     __builtin_amdgcn_s_waitcnt(WAIT_VMEM);
     stats_store(0);
     __syncthreads();
@@ -1000,7 +1044,7 @@ __global__ __launch_bounds__(64 * KV_WAVES, 1) void attend_dkv_wide(FastArgs g, 
   }
   __syncthreads();  // every wave is done with every buffer
   const bool odd_k = any_odd(gk), odd_v = any_odd(gv);
-  if (threadIdx.x == 0) g.odd[bk * nkb + blk] = odd_k | odd_v;
+  if (threadIdx.x == 0 && blockIdx.y == 0) g.odd[bk * nkb + blk] = g.partial == nullptr && (odd_k | odd_v);
   // the second query half's partial sums to LDS, added to the first's: always in that order
   char* const part_k = kg == 0 ? (char*)Ks : kg == 1 ? (char*)Vs : kg == 2 ? (char*)Q0 : (char*)O0;
   char* const part_v = kg == 0 ? (char*)Ks + 16384 : kg == 1 ? (char*)Vs + 16384 : kg == 2 ? (char*)Q1 : (char*)O1;
@@ -1028,8 +1072,8 @@ __global__ __launch_bounds__(64 * KV_WAVES, 1) void attend_dkv_wide(FastArgs g, 
         }
       }
     u16* stage = (u16*)part_k;  // which only this wave reads from now on
-    store_rows<T, D>(g.o0 + bk * (int64_t)r.t_k * g.hd, gk, wk0, r.t_k, g.hd, g.scale * ds_down<T>(), stage);
-    store_rows<T, D>(g.o1 + bk * (int64_t)r.t_k * g.hd, gv, wk0, r.t_k, g.hd, DOWN, stage);
+    store_keys<D>(g, bk, r.t_k, wk0, gk, gv, g.scale * ds_down<T>(), DOWN,
+                  [&](const f32x16* acc, u16* o, float mul) __attribute__((always_inline)) { store_rows<T, D>(o + bk * (int64_t)r.t_k * g.hd, acc, wk0, r.t_k, g.hd, mul, stage); });
   }
 #endif
 }
@@ -1436,7 +1480,7 @@ int launch_fast_as(const FastArgs& g, const RuleArgs& ra, hipStream_t stream) {
   const int64_t blocks = PASS == ATTEND_PASS_DKV ? att_grid(g.batch * g.kv_heads, (ra.t_k + ATT_ROWS - 1) / ATT_ROWS, g.head_group)
                                                  : att_grid(g.batch * g.heads, (ra.t_q + ATT_ROWS - 1) / ATT_ROWS, g.head_group);
   if (blocks > 0x7fffffff) return fail(LIMN_HIP_EUNSUPPORTED, "attend: %lld workgroups exceed one launch", (long long)blocks);
-  const dim3 grid((unsigned)blocks), block(THREADS);
+  const dim3 grid((unsigned)blocks, PASS == ATTEND_PASS_DKV ? (unsigned)(g.head_parts * g.tile_parts) : 1), block(THREADS);
   if constexpr (PASS == ATTEND_PASS_FWD && D > 64)
     hipLaunchKernelGGL((attend_fwd_wide<T, D, CAP, BIAS>), grid, block, 0, stream, g, ra);
   else if constexpr (PASS == ATTEND_PASS_DQ && D > 64)

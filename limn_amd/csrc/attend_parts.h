@@ -155,21 +155,6 @@ __device__ __forceinline__ void gather(const u16* tile, int r0, const f32x16& s,
   }
 }
 
-// 32 rows of float results: a lane holds row n's 4 consecutive elements
-template <int D>
-__device__ __forceinline__ void store_floats(u16* base, int64_t first, const f32x16* acc, int row0, int rows, int hd, float mul) {
-  const int lane = threadIdx.x & 63, h = lane >> 5, row = row0 + (lane & 31);
-  if (row >= rows) return;
-  float* o = (float*)base + (first + row) * hd;
-#pragma unroll
-  for (int dt = 0; dt < D / 32; dt++)
-#pragma unroll
-    for (int q = 0; q < 4; q++) {
-      const int d = dt * 32 + 8 * q + 4 * h;
-      if (d < hd) *(f32x4*)(o + d) = f32x4{acc[dt][4 * q], acc[dt][4 * q + 1], acc[dt][4 * q + 2], acc[dt][4 * q + 3]} * mul;
-    }
-}
-
 // The streamed rows a block visits, PartTile rows at a time: the visit's tiles of 64, in halves where a tile is 32.
 template <int D>
 struct PartWalk {
@@ -297,7 +282,7 @@ __global__ __launch_bounds__(THREADS, D <= 64 ? 2 : 1) void attend_fwd_parts(Fas
   const float total = pair_sum(l);
   const bool odd = any_odd(acc);
   if (threadIdx.x == 0) g.odd[qb.bh * qb.nqb + qb.q0 / ATT_ROWS] = odd;
-  store_floats<D>(g.o0, qb.bh * r.t_q, acc, qb.wq0, r.t_q, g.hd, total == 0.f ? 0.f : 1.f / total);
+  store_floats<D>((float*)g.o0, qb.bh * r.t_q, acc, qb.wq0, r.t_q, g.hd, total == 0.f ? 0.f : 1.f / total);
   if (h == 0 && there) g.lse[qb.bh * (int64_t)r.t_q + qb.row] = total == 0.f ? neg_inf() : m * unit * ATT_LN2 + logf(total);
 }
 
@@ -394,7 +379,7 @@ __global__ __launch_bounds__(THREADS, 1) void attend_dq_parts(FastArgs g, RuleAr
   }
   const bool odd = any_odd(acc);
   if (threadIdx.x == 0) g.odd[qb.bh * qb.nqb + qb.q0 / ATT_ROWS] = odd;
-  store_floats<D>(g.o0, rows0, acc, qb.wq0, r.t_q, g.hd, g.scale);
+  store_floats<D>((float*)g.o0, rows0, acc, qb.wq0, r.t_q, g.hd, g.scale);
 }
 
 // ---- dK/dV pass -------------------------------------------------------------------------------------------
@@ -432,9 +417,9 @@ __global__ __launch_bounds__(THREADS, 1) void attend_dkv_parts(FastArgs g, RuleA
 #pragma unroll
   for (int dt = 0; dt < D / 32; dt++) gk[dt] = gv[dt] = zero16();
 
-  // query tiles: from the first that can see the block's first key on, unless a prefix opens it to all
-  const int first_q = r.causal && k0 >= r.pre ? max(0, k0 - r.off) / TILE : 0;
-  Visit visit = {k0 < r.len ? (r.t_q + TILE - 1) / TILE : 0};
+  const KeyPart part(g, r, k0, group);
+  const int first_q = part.first;
+  Visit visit = {part.to};
   const int4* ranges = g.ranges ? g.ranges + b * g.granules : nullptr;
   if (ranges != nullptr) {
     const int first = __builtin_amdgcn_readfirstlane(doc);
@@ -462,9 +447,9 @@ __global__ __launch_bounds__(THREADS, 1) void attend_dkv_parts(FastArgs g, RuleA
   };
   PartWalk<D> walk(visit);
   walk.start(first_q);
-  int gh = walk.more() ? 0 : group;
-  if (gh < group) load(gh, walk.row());
-  while (gh < group) {
+  int gh = walk.more() ? part.g0 : part.g1;
+  if (gh < part.g1) load(gh, walk.row());
+  while (gh < part.g1) {
     const int r0 = walk.row(), alike = walk.alike();
     const float slope2 = BIAS ? ra.slopes[kvh * group + gh] * LOG2E : 0.f;
     __syncthreads();
@@ -479,7 +464,7 @@ __global__ __launch_bounds__(THREADS, 1) void attend_dkv_parts(FastArgs g, RuleA
       gh++;
       walk.start(first_q);
     }
-    if (gh < group) load(gh, walk.row());
+    if (gh < part.g1) load(gh, walk.row());
     __syncthreads();
 #pragma unroll 1
     for (int sub = 0; sub < P::SUBS; sub++) {
@@ -520,9 +505,9 @@ __global__ __launch_bounds__(THREADS, 1) void attend_dkv_parts(FastArgs g, RuleA
     }
   }
   const bool odd_k = any_odd(gk), odd_v = any_odd(gv);
-  if (threadIdx.x == 0) g.odd[bk * nkb + blk] = odd_k | odd_v;
-  store_floats<D>(g.o0, bk * r.t_k, gk, wk0, r.t_k, g.hd, g.scale);
-  store_floats<D>(g.o1, bk * r.t_k, gv, wk0, r.t_k, g.hd, 1.f);
+  if (threadIdx.x == 0 && blockIdx.y == 0) g.odd[bk * nkb + blk] = g.partial == nullptr && (odd_k | odd_v);
+  store_keys<D>(g, bk, r.t_k, wk0, gk, gv, g.scale, 1.f,
+                [&](const f32x16* acc, u16* o, float mul) __attribute__((always_inline)) { store_floats<D>((float*)o, bk * r.t_k, acc, wk0, r.t_k, g.hd, mul); });
 }
 
 // ---- launches -----------------------------------------------------------------------------------------------
@@ -532,7 +517,7 @@ int launch_parts_as(const FastArgs& g, const RuleArgs& ra, hipStream_t stream) {
   const int64_t blocks = PASS == ATTEND_PASS_DKV ? att_grid(g.batch * g.kv_heads, (ra.t_k + ATT_ROWS - 1) / ATT_ROWS, g.head_group)
                                                  : att_grid(g.batch * g.heads, (ra.t_q + ATT_ROWS - 1) / ATT_ROWS, g.head_group);
   if (blocks > 0x7fffffff) return fail(LIMN_HIP_EUNSUPPORTED, "attend: %lld workgroups exceed one launch", (long long)blocks);
-  const dim3 grid((unsigned)blocks), block(THREADS);
+  const dim3 grid((unsigned)blocks, PASS == ATTEND_PASS_DKV ? (unsigned)(g.head_parts * g.tile_parts) : 1), block(THREADS);
   if constexpr (PASS == ATTEND_PASS_FWD)
     hipLaunchKernelGGL((attend_fwd_parts<D, CAP, BIAS>), grid, block, 0, stream, g, ra);
   else if constexpr (PASS == ATTEND_PASS_DQ)

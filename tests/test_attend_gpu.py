@@ -114,6 +114,19 @@ def test_rules(hipdev, dtype, dim, causal, softcap, alibi, documents, prefix, ra
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("heads,kv_heads,t_q,t_k", [(2, 2, 600, 600), (6, 2, 700, 700), (5, 1, 1000, 1000), (4, 1, 65, 700)])
+def test_few_key_heads_cut_into_parts(hipdev, dtype, hd, heads, kv_heads, t_q, t_k):
+    """Too few key blocks for the GPU: the queries' heads, then their tiles, are spread over workgroups."""
+    rng, (q, k, v, do) = draw(heads + t_q + hd, dtype, 1, heads, kv_heads, t_q, t_k, hd, hd)
+    check(hipdev, q, k, v, do, dtype, {}, dict(causal=True))
+    check(hipdev, q, k, v, do, dtype, dict(documents=packed(rng, 1, t_k, 150), prefix=np.array([130], np.int32)), dict(causal=True, softcap=5.0))
+    check(hipdev, q, k, v, do, dtype, dict(lengths=np.array([t_k - 90], np.int32)), dict())
+    v[0, 0, t_k - 5] = np.inf  # the last rows alone see it
+    check(hipdev, q, k, v, do, dtype, {}, dict(causal=True))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 def test_documents_in_any_order_and_rows_that_see_nothing(hipdev, dtype):
     rng, (q, k, v, do) = draw(5, dtype, 3, 2, 2, 200, 200, 64, 64)
     docs = rng.integers(-1, 4, (3, 200)).astype(np.int32)
