@@ -223,11 +223,12 @@ int64_t fast_workspace(const AttendArgs& a, bool backward) {
   return need;
 }
 
-// Heads in a group of one XCD (att_head_and_block): 4 where every sequence has the same work, 2 where documents or
-// lengths make it differ, so that each XCD has some of every sequence; fewer heads than give each XCD two
-// groups go alone, and fewer than 8, or a few that 8 does not divide, in turn.
-int head_group(const AttendArgs& a, int64_t heads) {
-  int group = a.documents != nullptr || a.lengths != nullptr ? 2 : 4;
+// Heads in a group of one XCD (att_head_and_block): 4, or 2 in a backward whose sequences differ in work by documents or
+// lengths, so that each XCD has some of every sequence (8 x 16 heads x 4096 x 128, documents of 1024: backward 1124
+// with 4 and 1096 with 2 us, forward 394 and 400); fewer heads than give each XCD two groups go alone, and fewer
+// than 8, or a few that 8 does not divide, in turn.
+int head_group(const AttendArgs& a, int64_t heads, bool backward) {
+  int group = backward && (a.documents != nullptr || a.lengths != nullptr) ? 2 : 4;
   while (group > 1 && heads < 16 * group) group /= 2;
   return heads < 8 || (heads < 64 && heads % (8 * group) != 0) ? 0 : group;
 }
@@ -250,7 +251,7 @@ int launch_fast(const AttendArgs& a, bool backward) {
   g.q = (const u16*)a.q, g.k = (const u16*)a.k, g.v = (const u16*)a.v, g.out = (const u16*)a.out, g.dout = (const u16*)a.dout;
   g.lse_in = a.lse, g.o0 = (u16*)a.o0, g.odd = odd, g.ranges = a.documents != nullptr ? ranges : nullptr;
   g.batch = a.batch, g.heads = (int)a.heads, g.kv_heads = (int)a.kv_heads, g.hd = (int)a.hd, g.granules = (int)granules_of(a), g.scale = (float)a.scale;
-  g.head_group = head_group(a, a.batch * a.heads);
+  g.head_group = head_group(a, a.batch * a.heads, backward);
   int rc = LIMN_HIP_OK;
   if (a.documents != nullptr && (rc = launch_attend_ranges(ra, ranges, a.batch, g.granules, a.stream)) != LIMN_HIP_OK) return rc;
   // without causality and documents a hidden key is one past the live ones, which reads as zeros; float32's parts do
@@ -266,7 +267,7 @@ int launch_fast(const AttendArgs& a, bool backward) {
   g.delta = kv.delta = (float*)take(a.batch * a.heads * a.t_q * 4);
   kv.o0 = (u16*)a.o1;
   kv.o1 = (u16*)a.o2;
-  kv.head_group = head_group(a, a.batch * a.kv_heads);
+  kv.head_group = head_group(a, a.batch * a.kv_heads, backward);
   const KeyParts parts = key_parts(a);
   kv.head_parts = parts.heads, kv.tile_parts = parts.tiles;
   kv.partial = parts.heads * parts.tiles > 1 ? (float*)take(key_parts_bytes(a)) : nullptr;

@@ -60,16 +60,11 @@ struct DocRange {
   __device__ __forceinline__ bool meets(const DocRange& o) const { return lo <= hi && o.lo <= o.hi && lo <= o.hi && o.lo <= hi; }
 };
 
-// positions [p0, p1], which may reach outside [0, 32 granules)
-__device__ __forceinline__ DocRange doc_range(const int4* ranges, int granules, int p0, int p1) {
-  DocRange r = {0x7fffffff, 0};
-  const int g0 = max(p0, 0) >> 5, g1 = min(p1 >> 5, granules - 1);
-  for (int g = g0; g <= g1; g++) {
-    const int4 e = ranges[g];
-    r.lo = min(r.lo, e.x);
-    r.hi = max(r.hi, e.y);
-  }
-  return r;
+// A granule's entry (attend_ranges); an empty one outside [0, count). The load is unconditional: a block's loads of
+// entries all go out at once, and one wait is all that a block's start has for them.
+__device__ __forceinline__ int4 granule_at(const int4* granules, int count, int g) {
+  const int4 e = granules[min(max(g, 0), count - 1)];
+  return g < 0 || g >= count ? int4{0x7fffffff, 0, -2, 0} : e;
 }
 
 // The streamed tiles a block visits, in order from a first one on: every tile before `to`, or those with a bit
@@ -118,31 +113,31 @@ struct Visit {
   }
 };
 
-// The document that all 32 positions from p on have, or -2: granules hold it for whole granules (attend_ranges), and
-// positions that begin inside one are alike where both it and the next say so.
-__device__ __forceinline__ int same_doc(const int4* granules, int count, int p) {
-  const int g = p >> 5;
-  if (p < 0 || g >= count) return -2;
-  const int one = granules[g].z;
-  if ((p & 31) == 0) return one;
-  return g + 1 < count && granules[g + 1].z == one ? one : -2;
-}
-
-// The lists of one block: bits, a bit for each streamed tile (64 positions from p0 + 64 t on, of `rows` in all) whose
-// documents meet the block's, 64 tiles a word, the words shared by the waves; half, for this wave's document doc
-// (-1: its rows differ), a bit for each half tile that has it alone, which then needs no test of documents.
-__device__ __forceinline__ void list_tiles(uint64_t* bits, uint64_t* half, const int4* granules, int count, const DocRange& mine, int doc, int p0, int rows,
-                                           int tiles, int wave, int waves) {
+// The lists of one block of ATT_ROWS positions from p on: bits, a bit for each streamed tile (64 positions from p0 + 64 t
+// on) whose documents meet the block's, 64 tiles a word, the words shared by the waves; half, for this wave's
+// document doc (-1: its rows differ), a bit for each half tile that has it alone, which then needs no test of
+// documents. Entries hold granules of 32 positions: where p0 is inside one, a half tile has one document if both
+// entries that it reaches into say so.
+__device__ __forceinline__ void list_tiles(uint64_t* bits, uint64_t* half, const int4* granules, int count, int p, int doc, int p0, int tiles, int wave, int waves) {
   const int lane = threadIdx.x & 63;
+  const bool inside = (p0 & 31) != 0;
+  constexpr int OWN = ATT_ROWS / 32 + 1;
+  int4 own[OWN];
+#pragma unroll
+  for (int j = 0; j < OWN; j++) own[j] = granule_at(granules, count, (p >> 5) + j);
+  if ((p & 31) == 0) own[OWN - 1] = int4{0x7fffffff, 0, -2, 0};
   for (int w = 0; w * 64 < tiles; w++) {
-    const int t = w * 64 + lane;
+    const int t = w * 64 + lane, g = (p0 >> 5) + 2 * t;
+    const int4 e0 = granule_at(granules, count, g), e1 = granule_at(granules, count, g + 1), e2 = granule_at(granules, count, inside ? g + 2 : -1);
     if (w % waves == wave) {
-      const bool meets = t < tiles && mine.meets(doc_range(granules, count, p0 + t * TILE, p0 + min(t * TILE + TILE, rows) - 1));
-      const uint64_t word = __ballot(meets);
+      DocRange mine = {0x7fffffff, 0};
+#pragma unroll
+      for (int j = 0; j < OWN; j++) mine = {min(mine.lo, own[j].x), max(mine.hi, own[j].y)};
+      const uint64_t word = __ballot(t < tiles && mine.meets(DocRange{min(min(e0.x, e1.x), e2.x), max(max(e0.y, e1.y), e2.y)}));
       if (lane == 0) bits[w] = word;
     }
     const bool in = t < tiles && doc >= 0;
-    const uint64_t h0 = __ballot(in && same_doc(granules, count, p0 + t * TILE) == doc), h1 = __ballot(in && same_doc(granules, count, p0 + t * TILE + 32) == doc);
+    const uint64_t h0 = __ballot(in && e0.z == doc && (!inside || e1.z == doc)), h1 = __ballot(in && e1.z == doc && (!inside || e2.z == doc));
     if (lane == 0) {
       half[w] = h0;
       half[ATT_WORDS + w] = h1;
@@ -354,8 +349,7 @@ __global__ __launch_bounds__(THREADS, 2) void attend_fwd_mfma(FastArgs g, RuleAr
   const int4* ranges = g.ranges ? g.ranges + b * g.granules : nullptr;
   if (ranges != nullptr) {
     const int first = __builtin_amdgcn_readfirstlane(doc);
-    list_tiles(bits, halves[wave], ranges, g.granules, doc_range(ranges, g.granules, r.off + q0, r.off + last), __all(doc == first) ? first : -1, 0,
-               g.granules * 32, visit.to, wave, WAVES);
+    list_tiles(bits, halves[wave], ranges, g.granules, r.off + q0, __all(doc == first) ? first : -1, 0, visit.to, wave, WAVES);
     visit.bits = bits;
     visit.half = halves[wave];
     __syncthreads();
@@ -398,10 +392,10 @@ __global__ __launch_bounds__(THREADS, 2) void attend_fwd_mfma(FastArgs g, RuleAr
           s[i] = bend<CAP, BIAS, false>(s[i], r, slope2, near - (float)(8 * (i >> 2) + (i & 3)), unused);
         }
       }
-      bool edge = s0 + 32 > r.len || (r.causal && s0 + 31 > r.off + wq0 && s0 + 31 >= r.pre);
-      edge |= ((alike >> sub) & 1) == 0;
-      if (edge) {
-        if (ranges != nullptr) {
+      const bool edge = s0 + 32 > r.len || (r.causal && s0 + 31 > r.off + wq0 && s0 + 31 >= r.pre);
+      const bool alone = (alike >> sub) & 1;
+      if (edge | !alone) {
+        if (!alone) {
 #pragma unroll
           for (int q = 0; q < 4; q++) {
             const int4 d4 = *(const int4*)&kdocs[buf][sub * 32 + 8 * q + 4 * h];
@@ -518,8 +512,7 @@ __global__ __launch_bounds__(THREADS, 2) void attend_dq_mfma(FastArgs g, RuleArg
   const int4* ranges = g.ranges ? g.ranges + b * g.granules : nullptr;
   if (ranges != nullptr) {
     const int first = __builtin_amdgcn_readfirstlane(doc);
-    list_tiles(bits, halves[wave], ranges, g.granules, doc_range(ranges, g.granules, r.off + q0, r.off + last), __all(doc == first) ? first : -1, 0,
-               g.granules * 32, visit.to, wave, WAVES);
+    list_tiles(bits, halves[wave], ranges, g.granules, r.off + q0, __all(doc == first) ? first : -1, 0, visit.to, wave, WAVES);
     visit.bits = bits;
     visit.half = halves[wave];
     __syncthreads();
@@ -562,10 +555,10 @@ __global__ __launch_bounds__(THREADS, 2) void attend_dq_mfma(FastArgs g, RuleArg
         const float e = fast_exp2(RAW ? fmaf(y, r.c2, -l2) : y - l2);
         s[i] = e * (dp[i] - delta) * (CAP ? bent : 1.f);  // times scale once, at the store
       }
-      bool edge = s0 + 32 > r.len || (r.causal && s0 + 31 > r.off + wq0 && s0 + 31 >= r.pre);
-      edge |= ((alike >> sub) & 1) == 0;
-      if (edge) {
-        if (ranges != nullptr) {
+      const bool edge = s0 + 32 > r.len || (r.causal && s0 + 31 > r.off + wq0 && s0 + 31 >= r.pre);
+      const bool alone = (alike >> sub) & 1;
+      if (edge | !alone) {
+        if (!alone) {
 #pragma unroll
           for (int q = 0; q < 4; q++) {
             const int4 d4 = *(const int4*)&kdocs[buf][sub * 32 + 8 * q + 4 * h];
@@ -646,8 +639,7 @@ __global__ __launch_bounds__(THREADS, 2) void attend_dkv_mfma(FastArgs g, RuleAr
   const int4* ranges = g.ranges ? g.ranges + b * g.granules : nullptr;
   if (ranges != nullptr) {
     const int first = __builtin_amdgcn_readfirstlane(doc);
-    list_tiles(bits, halves[wave], ranges, g.granules, doc_range(ranges, g.granules, k0, min(k0 + ATT_ROWS, r.t_k) - 1), __all(doc == first) ? first : -1,
-               r.off, r.t_q, visit.to, wave, WAVES);
+    list_tiles(bits, halves[wave], ranges, g.granules, k0, __all(doc == first) ? first : -1, r.off, visit.to, wave, WAVES);
     visit.bits = bits;
     visit.half = halves[wave];
     __syncthreads();
@@ -735,10 +727,10 @@ __global__ __launch_bounds__(THREADS, 2) void attend_dkv_mfma(FastArgs g, RuleAr
         s[i] = fast_exp2(RAW ? fmaf(y, r.c2, -l2) : y - l2);
         dp[i] = s[i] * fmaf(dp[i], DS, -d4[i >> 2][i & 3]) * (CAP ? bent : 1.f);  // times scale once, at the store
       }
-      bool edge = s0 + 32 > r.t_q || wk0 + 32 > r.len || (r.causal && r.off + s0 < wk0 + 31 && wk0 + 31 >= r.pre);
-      edge |= ((alike >> sub) & 1) == 0;
-      if (edge) {
-        if (ranges != nullptr) {
+      const bool edge = s0 + 32 > r.t_q || wk0 + 32 > r.len || (r.causal && r.off + s0 < wk0 + 31 && wk0 + 31 >= r.pre);
+      const bool alone = (alike >> sub) & 1;
+      if (edge | !alone) {
+        if (!alone) {
 #pragma unroll
           for (int q = 0; q < 4; q++) {
             const int4 q4 = *(const int4*)&qdocs[buf][sub * 32 + 8 * q + 4 * h];
@@ -879,8 +871,7 @@ __global__ __launch_bounds__(64 * KV_WAVES, 1) void attend_dkv_wide(FastArgs g, 
   const int4* ranges = g.ranges ? g.ranges + b * g.granules : nullptr;
   if (ranges != nullptr) {
     const int first = __builtin_amdgcn_readfirstlane(doc);
-    list_tiles(bits, halves[wave], ranges, g.granules, doc_range(ranges, g.granules, k0, min(k0 + ATT_ROWS, r.t_k) - 1), __all(doc == first) ? first : -1,
-               r.off, r.t_q, visit.to, wave, KV_WAVES);
+    list_tiles(bits, halves[wave], ranges, g.granules, k0, __all(doc == first) ? first : -1, r.off, visit.to, wave, KV_WAVES);
     visit.bits = bits;
     visit.half = halves[wave];
     __syncthreads();
@@ -1119,8 +1110,7 @@ __device__ __forceinline__ Visit key_visit(const FastArgs& g, const Rules& r, co
   Visit visit = {kend > 0 ? (kend + TILE - 1) / TILE : 0};
   if (ranges != nullptr) {
     const int first = __builtin_amdgcn_readfirstlane(qb.doc);
-    list_tiles(bits, half, ranges, g.granules, doc_range(ranges, g.granules, r.off + qb.q0, r.off + last), __all(qb.doc == first) ? first : -1, 0,
-               g.granules * 32, visit.to, wave, WAVES);
+    list_tiles(bits, half, ranges, g.granules, r.off + qb.q0, __all(qb.doc == first) ? first : -1, 0, visit.to, wave, WAVES);
     visit.bits = bits;
     visit.half = half;
     __syncthreads();
@@ -1226,7 +1216,7 @@ __global__ __launch_bounds__(THREADS, 2) void attend_fwd_wide(FastArgs g, RuleAr
         }
       }
       if (half_edge(r, qb, (alike >> sub) & 1, s0)) {
-        if (docs) {
+        if (docs && !((alike >> sub) & 1)) {
 #pragma unroll
           for (int q = 0; q < 4; q++) {
             const int4 d4 = *(const int4*)&kdocs[buf][sub * 32 + 8 * q + 4 * h];

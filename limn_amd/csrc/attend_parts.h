@@ -423,8 +423,7 @@ __global__ __launch_bounds__(THREADS, 1) void attend_dkv_parts(FastArgs g, RuleA
   const int4* ranges = g.ranges ? g.ranges + b * g.granules : nullptr;
   if (ranges != nullptr) {
     const int first = __builtin_amdgcn_readfirstlane(doc);
-    list_tiles(bits, halves[wave], ranges, g.granules, doc_range(ranges, g.granules, k0, min(k0 + ATT_ROWS, r.t_k) - 1), __all(doc == first) ? first : -1,
-               r.off, r.t_q, visit.to, wave, WAVES);
+    list_tiles(bits, halves[wave], ranges, g.granules, k0, __all(doc == first) ? first : -1, r.off, visit.to, wave, WAVES);
     visit.bits = bits;
     visit.half = halves[wave];
     __syncthreads();
