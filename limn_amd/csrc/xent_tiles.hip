@@ -623,29 +623,51 @@ int64_t padded_width(const XentArgs& a) { return up(a.width, 8); }
 bool rows16(const XentArgs& a) { return !f32(a) && a.width % 8 == 0; }
 bool as_is(const XentArgs& a) { return rows16(a) && ((uintptr_t)a.x | (uintptr_t)a.w) % 16 == 0; }
 
+// Rounds of tiles that keep the GPU: whole ones, or the part of one that smaller tiles or slices make of a few.
+double rounds(int64_t tiles) { return tiles * 4 >= 3 * FILL ? (double)((tiles + FILL - 1) / FILL) : 1.3 * (double)tiles / FILL; }
+
 // Vocabulary entries that go by at a time, a multiple of 256 and 1024 at least: what 32-bit offsets reach, dz
-// within PIECE_BYTES, and the copies of the weight's rows, where there are any, too.
+// within PIECE_BYTES or half as much again, and the copies of the weight's rows, where there are any, too. Of such sizes
+// a backward takes the one whose dz and dw tiles leave the fewest CUs idle over all pieces, in units of one tile's stage of
+// 64 deep; 16 of them are what a piece's launches and its tiles' beginnings and ends cost (4001 rows, width 760,
+// vocabulary 50257: 3 pieces of 16384 and one of 1105, forward and backward, 1679 us; 2 of 20480 and one of 9297 1640).
 int64_t piece_of(const XentArgs& a, bool backward, bool copies) {
-  const int64_t whole = up(a.vocab, 256), half = PIECE_BYTES / 2 / parts_of(a);
-  int64_t most = (int64_t)0x70000000 / 2 / padded_width(a);
-  if (backward && half / up(a.rows, 256) < most) most = half / up(a.rows, 256);
+  const int64_t whole = up(a.vocab, 256), half = PIECE_BYTES / 2 / parts_of(a), rows = (a.rows + 255) / 256, cols = (padded_width(a) + 255) / 256;
+  const int64_t reach = (int64_t)0x70000000 / 2 / padded_width(a);
+  int64_t most = reach;
   if (copies && half / padded_width(a) < most) most = half / padded_width(a);
-  most = most < 1024 ? 1024 : most / 256 * 256;
-  return most < whole ? most : whole;
+  const int64_t fit = backward && half / (256 * rows) < most ? half / (256 * rows) : most;
+  int64_t best = fit < 1024 ? 1024 : fit / 256 * 256;
+  if (best >= whole) return whole;
+  if (!backward) return best;
+  double least = 0;
+  const int64_t end = best + best / 2 < most ? best + best / 2 : most;
+  for (int64_t p = up(best / 2 < 1024 ? 1024 : best / 2, 256), at = 0; p <= end; p += 256) {
+    const int64_t pieces = (a.vocab + p - 1) / p, rest = a.vocab - (pieces - 1) * p;
+    auto cost = [&](int64_t n) {
+      const int64_t tiles = (n + 255) / 256;
+      return rounds(rows * tiles) * (double)(a.width + 63) / 64 + rounds(tiles * cols) * (double)(a.rows + 63) / 64 + 16;
+    };
+    const double c = (double)(pieces - 1) * cost(p) + cost(rest);
+    if (at++ == 0 || c < least) {
+      least = c;
+      best = p;
+    }
+  }
+  return best < whole ? best : whole;
 }
 
 struct Cut {
   int tile;
   int64_t split, chunk;
 };
-// As matmul.hip cuts its products. In three parts a slice of k is six times the work for the same partial result, so
-// tiles of 128 that would give a CU one workgroup are cut too (float32, 8191 x 512 of 2048 rows: 175 -> 114 us
-// and 13 for the sum of the halves).
+// Tiles of 256 in as many slices of k as leave no more than a quarter of the CUs idle, where slices are long enough for
+// their partial results (in three parts a slice is six times the work); else as matmul.hip cuts its products.
 Cut cut(int64_t m, int64_t n, int64_t k, int parts) {
-  const int64_t tiles = ((m + 127) / 128) * ((n + 127) / 128);
-  if (parts == 3 && tile_for(m, n) == 128 && tiles >= FILL && 2 * tiles <= 3 * FILL && k >= 256) {
-    const int64_t chunk = up((k + 1) / 2, BK);
-    return {128, 2, chunk};
+  const int64_t tiles = ((m + 255) / 256) * ((n + 255) / 256);
+  if (tiles < FILL) {
+    const int64_t split = FILL / tiles, chunk = up((k + split - 1) / split, BK);
+    if (split * tiles * 4 >= 3 * FILL && (split == 1 || chunk * (parts == 3 ? 6 : 1) >= 1024)) return {256, (k + chunk - 1) / chunk, chunk};
   }
   const MatmulPlan p = plan_matmul(MatmulShape{1, m, n, k});
   return {p.tile, p.split, p.chunk};
