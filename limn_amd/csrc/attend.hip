@@ -215,11 +215,22 @@ int64_t key_parts_bytes(const AttendArgs& a) {
   return p.heads * p.tiles > 1 ? p.heads * p.tiles * 2 * a.batch * a.kv_heads * a.t_k * a.hd * 4 : 0;
 }
 
+// Bytes of dS between the backward's passes past 64 half-width dims, 0 for none: 2 a pair of positions, whether it is seen
+// or not, up to HANDED_MOST, a hundredth of the memory; longer calls compute the scores a second time instead. Backward of
+// 4 x 16 heads over 4 key heads x 4096 x 128, capped: 1163 us so, 1237 computed twice; 8 x 12 over 6 x 1021 x 80: 144
+// and 149; 16 x 16 x 300 x 128: 96 and 101; 8 x 16 x 4096 x 128 with documents of 1024 (4 GiB, past the limit): 1081 and 1104.
+constexpr int64_t HANDED_MOST = (int64_t)5 << 29;
+int64_t key_tiles(const AttendArgs& a) { return (a.t_k + ATT_ROWS - 1) / ATT_ROWS * 2; }  // whole key blocks
+int64_t handed_bytes(const AttendArgs& a) {
+  if (!half_sizes(a) || a.hd <= 64 || row_blocks(a) > HANDED_MOST / (64 * ATT_ROWS * 2) / key_tiles(a)) return 0;
+  return row_blocks(a) * key_tiles(a) * 64 * ATT_ROWS * 2;
+}
+
 // flags of the blocks, the documents' ranges, and for the backward delta
 int64_t fast_workspace(const AttendArgs& a, bool backward) {
   if (!fast_sizes(a)) return 0;
   int64_t need = attend_align(row_blocks(a) * 4) + attend_align(a.batch * granules_of(a) * 16);
-  if (backward) need += attend_align(key_blocks(a) * 4) + attend_align(a.batch * a.heads * a.t_q * 4) + attend_align(key_parts_bytes(a));
+  if (backward) need += attend_align(key_blocks(a) * 4) + attend_align(a.batch * a.heads * a.t_q * 4) + attend_align(key_parts_bytes(a)) + attend_align(handed_bytes(a));
   return need;
 }
 
@@ -271,8 +282,13 @@ int launch_fast(const AttendArgs& a, bool backward) {
   const KeyParts parts = key_parts(a);
   kv.head_parts = parts.heads, kv.tile_parts = parts.tiles;
   kv.partial = parts.heads * parts.tiles > 1 ? (float*)take(key_parts_bytes(a)) : nullptr;
-  if ((rc = LIMN_ATTEND_PASS(dq, g)) != LIMN_HIP_OK) return rc;
+  g.row_blocks = kv.row_blocks = (int)((a.t_q + ATT_ROWS - 1) / ATT_ROWS);
+  g.key_tiles = kv.key_tiles = (int)key_tiles(a);
+  g.ds = kv.ds = handed_bytes(a) > 0 ? (u16*)take(handed_bytes(a)) : nullptr;
+  rc = g.ds != nullptr ? launch_attend_delta(g, a.batch * a.heads * a.t_q, a.dtype, a.stream) : LIMN_ATTEND_PASS(dq, g);
+  if (rc != LIMN_HIP_OK) return rc;
   rc = LIMN_ATTEND_PASS(dkv, kv);
+  if (rc == LIMN_HIP_OK && g.ds != nullptr) rc = LIMN_ATTEND_PASS(dq, g);
   if (rc == LIMN_HIP_OK && kv.partial != nullptr)
     rc = a.dtype == LIMN_HIP_FLOAT32 ? join_keys<F32>(a, kv) : a.dtype == LIMN_HIP_FLOAT16 ? join_keys<F16>(a, kv) : join_keys<BF16>(a, kv);
   return rc != LIMN_HIP_OK || !mend ? rc : launch_attend_mend_bwd(g, kv, ra, a.dtype, a.stream);

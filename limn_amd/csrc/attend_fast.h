@@ -30,9 +30,14 @@ struct FastArgs {
   // query tiles, whose float totals go to partial (part, dk and dv, key rows, hd) for attend_join_keys to add
   int head_parts, tile_parts;
   float* partial;
+  // backward past 64 half-width dims: the score gradients on their way from the dK/dV pass to the dQ pass, or nullptr:
+  // (heads of all sequences, row_blocks, key_tiles, 64 keys, 128 queries)
+  u16* ds;
+  int row_blocks, key_tiles;
 };
 
 int launch_attend_ranges(const RuleArgs& ra, int4* ranges, int64_t batch, int granules, hipStream_t stream);
+int launch_attend_delta(const FastArgs& g, int64_t rows, int dtype, hipStream_t stream);
 int launch_attend_mend_fwd(const FastArgs& g, const RuleArgs& ra, int dtype, hipStream_t stream);
 // blocks of the dQ pass (g.odd) and of the dK/dV pass (kv.odd) that are to be computed again
 int launch_attend_mend_bwd(const FastArgs& g, const FastArgs& kv, const RuleArgs& ra, int dtype, hipStream_t stream);

@@ -26,6 +26,23 @@ __global__ __launch_bounds__(256) void attend_ranges(RuleArgs ra, int4* __restri
   if (n == 0) ranges[id] = make_int4(lo, hi, lo == hi && !none ? lo : -2, 0);
 }
 
+// delta = rowsum(dout * out), 16 lanes a row
+template <typename T>
+__global__ __launch_bounds__(256) void attend_delta(FastArgs g, int64_t rows) {
+  const int64_t row = blockIdx.x * (int64_t)16 + (threadIdx.x >> 4);
+  if (row >= rows) return;  // 16 lanes at a time: the shuffles below stay inside them
+  const int d = (threadIdx.x & 15) * 8;
+  float x = 0.f;
+  if (d < g.hd) {
+    const u16x8 a = *(const u16x8*)(g.dout + row * g.hd + d), b = *(const u16x8*)(g.out + row * g.hd + d);
+#pragma unroll
+    for (int e = 0; e < 8; e++) x = fmaf(T::unpack(a[e]), T::unpack(b[e]), x);
+  }
+#pragma unroll
+  for (int m = 1; m < 16; m <<= 1) x += __shfl_xor(x, m);
+  if (d == 0) g.delta[row] = x;
+}
+
 // The flagged blocks among those of this workgroup (every gridDim.x-th), found 256 flags at a time.
 template <typename F>
 __device__ __forceinline__ void each_odd(const int* odd, int64_t blocks, F f) {
@@ -139,6 +156,16 @@ int launch_attend_ranges(const RuleArgs& ra, int4* ranges, int64_t batch, int gr
   if (blocks > 0x7fffffff) return fail(LIMN_HIP_EUNSUPPORTED, "attend: %lld workgroups exceed one launch", (long long)blocks);
   hipLaunchKernelGGL(attend_ranges, dim3((unsigned)blocks), dim3(256), 0, stream, ra, ranges, batch, granules);
   return check_hip(hipGetLastError(), "launching the documents' ranges");
+}
+
+int launch_attend_delta(const FastArgs& g, int64_t rows, int dtype, hipStream_t stream) {
+  const int64_t blocks = (rows + 15) / 16;
+  if (blocks > 0x7fffffff) return fail(LIMN_HIP_EUNSUPPORTED, "attend: %lld workgroups exceed one launch", (long long)blocks);
+  if (dtype == LIMN_HIP_BFLOAT16)
+    hipLaunchKernelGGL((attend_delta<BF16>), dim3((unsigned)blocks), dim3(256), 0, stream, g, rows);
+  else
+    hipLaunchKernelGGL((attend_delta<F16>), dim3((unsigned)blocks), dim3(256), 0, stream, g, rows);
+  return check_hip(hipGetLastError(), "launching attention's row sums");
 }
 
 int launch_attend_mend_fwd(const FastArgs& g, const RuleArgs& ra, int dtype, hipStream_t stream) {

@@ -160,6 +160,17 @@ struct HeadRows {
   }
 };
 
+// Words beside a streamed tile (documents, statistics), loaded a tile ahead by every wave though one stores them: a load
+// that only some waves take leaves a copy of the register to make, which waits for every load of the wave, those of the
+// next tile too (backward of 8 x 16 heads x 4096 x 64 with documents of 1000: 680 us so, 659 now). A word outside
+// [0, count) is 0; what it stands for is masked by its position.
+struct Words {
+  __amdgpu_buffer_rsrc_t rsrc;
+  __device__ __forceinline__ Words(const void* base, int count) { rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)base, (short)0, base == nullptr ? 0 : count * 4, 0x00020000); }
+  __device__ __forceinline__ int whole(int i) const { return (int)__builtin_amdgcn_raw_buffer_load_b32(rsrc, i * 4, 0, 0); }
+  __device__ __forceinline__ float real(int i) const { return __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(rsrc, i * 4, 0, 0)); }
+};
+
 // Global -> registers -> LDS staging of two 64-row tiles, as Stage<D> of sdpa_mfma.h does it.
 template <int D>
 struct HeadStage {
@@ -359,7 +370,8 @@ __global__ __launch_bounds__(THREADS, 2) void attend_fwd_mfma(FastArgs g, RuleAr
   int dnext = 0;
   visit.start(0);
   int cur = visit.next(), alike = visit.alike, nxt = visit.next();
-  auto docs_load = [&](int t) { return ranges != nullptr && threadIdx.x < TILE && t * TILE + (int)threadIdx.x < r.len ? r.docs[t * TILE + threadIdx.x] : -1; };
+  const Words dwords(r.docs, r.len);
+  auto docs_load = [&](int t) { return dwords.whole(t * TILE + lane); };
   if (cur < visit.to) {
     st.load(krows, vrows, cur * TILE);
     dnext = docs_load(cur);
@@ -522,7 +534,8 @@ __global__ __launch_bounds__(THREADS, 2) void attend_dq_mfma(FastArgs g, RuleArg
   int dnext = 0;
   visit.start(0);
   int cur = visit.next(), alike = visit.alike, nxt = visit.next();
-  auto docs_load = [&](int t) { return ranges != nullptr && threadIdx.x < TILE && t * TILE + (int)threadIdx.x < r.len ? r.docs[t * TILE + threadIdx.x] : -1; };
+  const Words dwords(r.docs, r.len);
+  auto docs_load = [&](int t) { return dwords.whole(t * TILE + lane); };
   if (cur < visit.to) {
     st.load(krows, vrows, cur * TILE);
     dnext = docs_load(cur);
@@ -646,8 +659,9 @@ __global__ __launch_bounds__(THREADS, 2) void attend_dkv_mfma(FastArgs g, RuleAr
   }
 
   HeadStage<D> st;
+  const Words dwords(r.docs, r.t_k);
   float lnext = 0.f, dnext = 0.f;
-  int qnext = -1;
+  int qnext = -1, tnext = 0;
   const int64_t head_rows = r.t_q;
   const int64_t base_row = (b * g.heads + kvh * (int64_t)group) * head_rows;
   // tile `t` of query head `gh` of the group
@@ -655,21 +669,19 @@ __global__ __launch_bounds__(THREADS, 2) void attend_dkv_mfma(FastArgs g, RuleAr
     const int64_t rows0 = base_row + gh * head_rows;
     const HeadRows qrows(g.q + rows0 * g.hd, r.t_q, g.hd), grows(g.dout + rows0 * g.hd, r.t_q, g.hd);
     st.load(qrows, grows, t * TILE);
-    if (threadIdx.x < TILE) {
-      const int qq = t * TILE + (int)threadIdx.x;
-      const bool ok = qq < r.t_q;
-      lnext = ok ? att_l2(g.lse_in[rows0 + qq]) - UP : __builtin_inff();
-      dnext = ok ? g.delta[rows0 + qq] * DS : 0.f;
-      qnext = ok ? query_doc(r, r.off + qq) : -1;
-    }
+    const int qq = t * TILE + lane;
+    lnext = Words(g.lse_in + rows0, r.t_q).real(qq);
+    dnext = Words(g.delta + rows0, r.t_q).real(qq);
+    qnext = dwords.whole(r.off + qq);
+    tnext = t;
   };
   auto store = [&](int buf) __attribute__((always_inline)) {
     u16* Qn = tiles + 2 * buf * TE;
     st.store(Qn, Qn + TE);
-    if (threadIdx.x < TILE) {
-      Ls[buf][threadIdx.x] = lnext;
-      Ds[buf][threadIdx.x] = dnext;
-      if (ranges != nullptr) qdocs[buf][threadIdx.x] = qnext;
+    if (wave == 0) {
+      Ls[buf][lane] = att_l2(lnext) - UP;
+      Ds[buf][lane] = dnext * DS;
+      if (ranges != nullptr) qdocs[buf][lane] = r.off + tnext * TILE + lane < 0 ? -1 : qnext;
     }
   };
   visit.start(first_q);
@@ -805,7 +817,9 @@ struct HeadDma8 {
   }
 };
 
-template <typename T, int D, bool CAP, bool BIAS>
+constexpr int HAND_STORES = 2;  // vector stores of dS a wave and tile, see below
+
+template <typename T, int D, bool CAP, bool BIAS, bool HAND>
 __global__ __launch_bounds__(64 * KV_WAVES, 1) void attend_dkv_wide(FastArgs g, RuleArgs ra) {
 #if defined(__HIP_DEVICE_COMPILE__)  // the host pass needs the stub alone
   constexpr bool RAW = !CAP && !BIAS;
@@ -880,26 +894,25 @@ __global__ __launch_bounds__(64 * KV_WAVES, 1) void attend_dkv_wide(FastArgs g, 
   const int64_t base_row = (b * g.heads + kvh * (int64_t)group) * r.t_q;
   // tile `t` of query head `gh` of the group: its rows by DMA, its statistics through registers (the first wave)
   // and its documents (the second), stored only when the tile before it is done: loads retire in order
+  const Words dwords(r.docs, r.t_k);
   float lnext = 0.f, dnext = 0.f;
-  int qnext = -1;
+  int qnext = -1, tnext = 0;
   auto load = [&](int gh, int t, u16* Q, u16* O) __attribute__((always_inline)) {
     const int64_t rows0 = base_row + (int64_t)gh * r.t_q;
     dma.copy(Q, g.q + rows0 * g.hd, t * TILE, r.t_q, wave);
     dma.copy(O, g.dout + rows0 * g.hd, t * TILE, r.t_q, wave);
     const int qq = t * TILE + lane;
-    const bool ok = qq < r.t_q;
-    if (wave == 0) {
-      lnext = ok ? g.lse_in[rows0 + qq] : neg_inf();
-      dnext = ok ? g.delta[rows0 + qq] : 0.f;
-    }
-    if (wave == 1 && ranges != nullptr) qnext = ok ? query_doc(r, r.off + qq) : -1;
+    lnext = Words(g.lse_in + rows0, r.t_q).real(qq);
+    dnext = Words(g.delta + rows0, r.t_q).real(qq);
+    qnext = dwords.whole(r.off + qq);
+    tnext = t;
   };
   auto stats_store = [&](int buf) __attribute__((always_inline)) {
     if (wave == 0) {
       Ls[buf][lane] = att_l2(lnext) - UP;
       Ds[buf][lane] = dnext * DS;
     }
-    if (wave == 1 && ranges != nullptr) qdocs[buf][lane] = qnext;
+    if (wave == 1 && ranges != nullptr) qdocs[buf][lane] = r.off + tnext * TILE + lane < 0 ? -1 : qnext;
   };
 
   visit.start(first_q);
@@ -973,6 +986,18 @@ __global__ __launch_bounds__(64 * KV_WAVES, 1) void attend_dkv_wide(FastArgs g, 
       soft(std::true_type{});
     else
       soft(std::false_type{});
+    if (HAND) {
+      // the wave's 32 keys x 32 queries for attend_dq_handed: the halves of a wave trade, so that a lane stores 8 queries
+      // of its key, even eights the first half and odd ones the second, 1 KB a store
+      const int64_t at = ((b * g.heads + kvh * (int64_t)group + gh) * g.row_blocks + (cur >> 1)) * g.key_tiles + blk * 2 + (kg >> 1);
+      u16* o = g.ds + at * (TILE * ATT_ROWS) + (((cur & 1) * 2 + hq) * 4 + (kg & 1) * 2) * 512 + lane * 8;
+#pragma unroll
+      for (int q = 0; q < 2; q++) {
+        const auto x = __builtin_amdgcn_permlane32_swap(gp[4 * q], gp[4 * q + 2], false, false);
+        const auto y = __builtin_amdgcn_permlane32_swap(gp[4 * q + 1], gp[4 * q + 3], false, false);
+        *(u32x4*)(o + 512 * q) = u32x4{x[0], y[0], x[1], y[1]};
+      }
+    }
     u16x8 pb[2], gb[2];
 #pragma unroll
     for (int c = 0; c < 2; c++) {
@@ -998,7 +1023,7 @@ __global__ __launch_bounds__(64 * KV_WAVES, 1) void attend_dkv_wide(FastArgs g, 
     load(min(ngh, part.g1 - 1), nxt, Qn, On);
     __builtin_amdgcn_sched_barrier(0);
     tile(buf, Qc, Oc);
-    __builtin_amdgcn_s_waitcnt(WAIT_VMEM);
+    __builtin_amdgcn_s_waitcnt(HAND ? WAIT_VMEM + HAND_STORES : WAIT_VMEM);  // the tile's stores, issued behind the copies, stay under way
     stats_store(buf ^ 1);
     __syncthreads();
     gh = ngh;
@@ -1188,8 +1213,9 @@ __global__ __launch_bounds__(THREADS, 2) void attend_fwd_wide(FastArgs g, RuleAr
   const int count = visit_count(visit);
   visit.start(0);
   int dnext = -1;
+  const Words dwords(r.docs, r.len);
   auto docs_load = [&](int t) __attribute__((always_inline)) {
-    if (docs && wave == 0) dnext = t * TILE + lane < r.len ? r.docs[t * TILE + lane] : -1;
+    dnext = dwords.whole(t * TILE + lane);
   };
   auto docs_store = [&](int buf) __attribute__((always_inline)) {
     if (docs && wave == 0) kdocs[buf][lane] = dnext;
@@ -1376,8 +1402,9 @@ __global__ __launch_bounds__(THREADS, 2) void attend_dq_wide(FastArgs g, RuleArg
   const int count = visit_count(visit);
   visit.start(0);
   int dnext = -1;
+  const Words dwords(r.docs, r.len);
   auto docs_load = [&](int t) __attribute__((always_inline)) {
-    if (docs && wave == 0) dnext = t * TILE + lane < r.len ? r.docs[t * TILE + lane] : -1;
+    dnext = dwords.whole(t * TILE + lane);
   };
   auto docs_store = [&](int buf) __attribute__((always_inline)) {
     if (docs && wave == 0) kdocs[buf][lane] = dnext;
@@ -1461,6 +1488,135 @@ __global__ __launch_bounds__(THREADS, 2) void attend_dq_wide(FastArgs g, RuleArg
 #endif
 }
 
+// ---- dQ pass past 64 dims from the dS that the dK/dV pass left ------------------------------------------------------
+// dS comes in matrices of 64 keys x 128 queries (16 KB; a head's query blocks by its key tiles): 4 KB for every 32 queries,
+// a wave's, of 1 KB for 32 keys and every second 16 bytes of theirs, each in the order in which a wave of the dK/dV pass
+// stores it (chunks of 8 queries: of the first eight of 16, key by key, then of the second). A wave copies its own 4 KB
+// into LDS, chunks of a KB exchanged so that the four 64-byte pieces which a half wave reads transposed lie in
+// different banks. One product where attend_dq_wide has three, bound by the reads of dS. The dK/dV pass wrote those
+// matrices' halves of 64 queries that its own lists and causality name; the others are not read.
+
+template <typename T, int D>
+__global__ __launch_bounds__(THREADS, 2) void attend_dq_handed(FastArgs g, RuleArgs ra) {
+#if defined(__HIP_DEVICE_COMPILE__)  // the host pass needs the stub alone
+  constexpr int DT = D / 32;
+  __shared__ __attribute__((aligned(1024))) u16 K0[TILE * 128];
+  __shared__ __attribute__((aligned(1024))) u16 K1[TILE * 128];
+  __shared__ __attribute__((aligned(1024))) u16 S0[TILE * 128];
+  __shared__ __attribute__((aligned(1024))) u16 S1[TILE * 128];
+  __shared__ uint64_t bits[ATT_WORDS];
+  __shared__ uint64_t halves[WAVES][2 * ATT_WORDS];
+
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 31;
+  QueryBlock qb;
+  if (!query_block(g, ra, qb, wave, n)) return;
+  const Rules r = rules_of(ra, qb.b);
+  const u16* kbase = g.k + (qb.b * g.kv_heads + qb.kvh) * (int64_t)r.t_k * g.hd;
+  const u16* sbase = g.ds + (qb.bh * g.row_blocks + qb.q0 / ATT_ROWS) * g.key_tiles * (int64_t)(TILE * ATT_ROWS);
+  const HeadDma4 dma(g.hd, wave, lane);
+  const SwzReads128 ad(lane);
+  int rs[2], sv[2];  // byte offsets of the transposing reads of dS, and of its copy's chunks by the parity of the KB
+#pragma unroll
+  for (int jj = 0; jj < 2; jj++) {
+    const int i = lane & 15, q = (lane >> 4) & 1, e = (i >> 1) & 1, key = 4 * (lane >> 5) + 8 * jj + (i >> 2);
+    rs[jj] = wave * 4096 + q * 1024 + (e * 32 + (key ^ (4 * (e + 2 * q)))) * 16 + (i & 1) * 8;
+    sv[jj] = (lane ^ (4 * ((lane >> 5) + 2 * jj))) * 16;
+  }
+  auto columns = [&](const u16* tile, int c) __attribute__((always_inline)) {  // keys 16 c .. + 15
+    const char* p = (const char*)tile + (c >> 1) * 2048 + (c & 1) * 256;
+    const v4i16 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16*)(p + rs[0]));
+    const v4i16 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16*)(p + rs[1]));
+    return __builtin_bit_cast(u16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+  };
+  f32x16 acc[DT];
+#pragma unroll
+  for (int dt = 0; dt < DT; dt++) acc[dt] = zero16();
+
+  const int last = min(qb.q0 + ATT_ROWS, r.t_q) - 1, tile = qb.wq0 / TILE;  // tile: the wave's queries'
+  int kend = r.len;
+  if (r.causal) kend = min(kend, max(r.off + last + 1, r.pre));
+  Visit visit = {kend > 0 ? (kend + TILE - 1) / TILE : 0};
+  const int4* ranges = g.ranges ? g.ranges + qb.b * g.granules : nullptr;
+  if (ranges != nullptr) {
+    const int p = r.off + qb.q0, pt = r.off + tile * TILE;
+    const bool inside = (p & 31) != 0;
+    DocRange block = {0x7fffffff, 0}, own = block;
+#pragma unroll
+    for (int j = 0; j < ATT_ROWS / 32 + 1; j++) {
+      const int4 e = granule_at(ranges, g.granules, j < ATT_ROWS / 32 || inside ? (p >> 5) + j : -1);
+      block = {min(block.lo, e.x), max(block.hi, e.y)};
+    }
+#pragma unroll
+    for (int j = 0; j < 3; j++) {
+      const int4 e = granule_at(ranges, g.granules, j < 2 || inside ? (pt >> 5) + j : -1);
+      own = {min(own.lo, e.x), max(own.hi, e.y)};
+    }
+    for (int w = 0; w * 64 < visit.to; w++) {
+      const int t = w * 64 + lane;
+      DocRange keys = {0x7fffffff, 0}, all = keys;  // of the tile, and of its key block of ATT_ROWS
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        const int4 e = granule_at(ranges, g.granules, (t >> 1) * 4 + j);
+        all = {min(all.lo, e.x), max(all.hi, e.y)};
+        if ((j >> 1) == (t & 1)) keys = {min(keys.lo, e.x), max(keys.hi, e.y)};
+      }
+      const uint64_t word = __ballot(t < visit.to && block.meets(keys)), wrote = __ballot(t < visit.to && own.meets(all));
+      if (lane == 0) {
+        if (w % WAVES == wave) bits[w] = word;
+        halves[wave][w] = halves[wave][ATT_WORDS + w] = wrote;
+      }
+    }
+    visit.bits = bits;
+    visit.half = halves[wave];
+    __syncthreads();
+  }
+  const int count = visit_count(visit);
+  visit.start(0);
+  int cur = visit.next(), alike = visit.alike, nxt = visit.next();
+  auto copy = [&](int t, u16* K, u16* S) __attribute__((always_inline)) {
+    dma.copy(K, kbase, t * TILE, r.len, wave);
+    const u16* m = sbase + (int64_t)min(t, g.key_tiles - 1) * (TILE * ATT_ROWS) + wave * 2048;
+    const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void*)m, (short)0, 4096, 0x00020000);
+#pragma unroll
+    for (int p = 0; p < 4; p++)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_void*)((char*)S + wave * 4096 + p * 1024), 16, p * 1024 + sv[p & 1], 0, 0, 0);
+  };
+  auto step = [&](const u16* Kc, const u16* Sc, u16* Kn, u16* Sn) __attribute__((always_inline)) {
+    copy(nxt, Kn, Sn);
+    const int k0 = (cur >> 1) * ATT_ROWS;
+    const int first = r.causal && k0 >= r.pre ? max(0, k0 - r.off) / TILE : 0;
+    if ((alike & 1) && tile >= first && tile * TILE < r.t_q) {
+#pragma unroll
+      for (int c = 0; c < 4; c++) {
+        const u16x8 b = columns(Sc, c);
+#pragma unroll
+        for (int dt = 0; dt < DT; dt++) acc[dt] = T::mfma32(ad.transposed(Kc, 16 * c, dt), b, acc[dt]);
+      }
+    }
+    __builtin_amdgcn_s_waitcnt(WAIT_VMEM);
+    __syncthreads();
+    cur = nxt;
+    alike = visit.alike;
+    nxt = visit.next();
+  };
+  if (count > 0) {
+    copy(cur, K0, S0);
+    __builtin_amdgcn_s_waitcnt(WAIT_VMEM);
+    __syncthreads();
+    int it = 0;
+    for (; it + 1 < count; it += 2) {
+      step(K0, S0, K1, S1);
+      step(K1, S1, K0, S0);
+    }
+    if (it < count) step(K0, S0, K1, S1);
+  }
+  const bool odd = any_odd(acc);  // a barrier: the tile buffers become staging below
+  if (threadIdx.x == 0) g.odd[qb.bh * qb.nqb + qb.q0 / ATT_ROWS] = odd;
+  u16* stage = wave == 0 ? K0 : wave == 1 ? K1 : wave == 2 ? S0 : S1;
+  store_rows<T, D>(g.o0 + qb.bh * (int64_t)r.t_q * g.hd, acc, qb.wq0, r.t_q, g.hd, g.scale * ds_down<T>(), stage);
+#endif
+}
+
 // ---- launches -------------------------------------------------------------------------------------------
 
 enum AttendPass { ATTEND_PASS_FWD, ATTEND_PASS_DQ, ATTEND_PASS_DKV };
@@ -1471,6 +1627,12 @@ int launch_fast_as(const FastArgs& g, const RuleArgs& ra, hipStream_t stream) {
                                                  : att_grid(g.batch * g.heads, (ra.t_q + ATT_ROWS - 1) / ATT_ROWS, g.head_group);
   if (blocks > 0x7fffffff) return fail(LIMN_HIP_EUNSUPPORTED, "attend: %lld workgroups exceed one launch", (long long)blocks);
   const dim3 grid((unsigned)blocks, PASS == ATTEND_PASS_DKV ? (unsigned)(g.head_parts * g.tile_parts) : 1), block(THREADS);
+  if constexpr (PASS == ATTEND_PASS_DQ && D > 64) {
+    if (g.ds != nullptr) {
+      hipLaunchKernelGGL((attend_dq_handed<T, D>), grid, block, 0, stream, g, ra);
+      return check_hip(hipGetLastError(), "launching attention");
+    }
+  }
   if constexpr (PASS == ATTEND_PASS_FWD && D > 64)
     hipLaunchKernelGGL((attend_fwd_wide<T, D, CAP, BIAS>), grid, block, 0, stream, g, ra);
   else if constexpr (PASS == ATTEND_PASS_DQ && D > 64)
@@ -1481,8 +1643,10 @@ int launch_fast_as(const FastArgs& g, const RuleArgs& ra, hipStream_t stream) {
     hipLaunchKernelGGL((attend_dq_mfma<T, D, CAP, BIAS>), grid, block, 0, stream, g, ra);
   else if constexpr (D <= 64)
     hipLaunchKernelGGL((attend_dkv_mfma<T, D, CAP, BIAS>), grid, block, 0, stream, g, ra);
+  else if (g.ds != nullptr)
+    hipLaunchKernelGGL((attend_dkv_wide<T, D, CAP, BIAS, true>), grid, dim3(64 * KV_WAVES), 0, stream, g, ra);
   else
-    hipLaunchKernelGGL((attend_dkv_wide<T, D, CAP, BIAS>), grid, dim3(64 * KV_WAVES), 0, stream, g, ra);
+    hipLaunchKernelGGL((attend_dkv_wide<T, D, CAP, BIAS, false>), grid, dim3(64 * KV_WAVES), 0, stream, g, ra);
   return check_hip(hipGetLastError(), "launching attention");
 }
 

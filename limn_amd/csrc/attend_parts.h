@@ -216,11 +216,12 @@ __global__ __launch_bounds__(THREADS, D <= 64 ? 2 : 1) void attend_fwd_parts(Fas
   const int4* ranges = g.ranges ? g.ranges + qb.b * g.granules : nullptr;
   PartWalk<D> walk(key_visit(g, r, qb, ranges, bits, halves[wave], wave));
   PartStage<D> st;
+  const Words dwords(r.docs, r.len);
   int dnext = 0;
   walk.start(0);
   auto load = [&](int k0) __attribute__((always_inline)) {
     st.load(krows, vrows, k0);
-    if (ranges != nullptr && threadIdx.x < R) dnext = k0 + (int)threadIdx.x < r.len ? r.docs[k0 + threadIdx.x] : -1;
+    dnext = dwords.whole(k0 + lane);
   };
   if (walk.more()) load(walk.row());
   while (walk.more()) {
@@ -333,11 +334,12 @@ __global__ __launch_bounds__(THREADS, 1) void attend_dq_parts(FastArgs g, RuleAr
   const int4* ranges = g.ranges ? g.ranges + qb.b * g.granules : nullptr;
   PartWalk<D> walk(key_visit(g, r, qb, ranges, bits, halves[wave], wave));
   PartStage<D> st;
+  const Words dwords(r.docs, r.len);
   int dnext = 0;
   walk.start(0);
   auto load = [&](int k0) __attribute__((always_inline)) {
     st.load(krows, vrows, k0);
-    if (ranges != nullptr && threadIdx.x < R) dnext = k0 + (int)threadIdx.x < r.len ? r.docs[k0 + threadIdx.x] : -1;
+    dnext = dwords.whole(k0 + lane);
   };
   if (walk.more()) load(walk.row());
   while (walk.more()) {
@@ -430,19 +432,17 @@ __global__ __launch_bounds__(THREADS, 1) void attend_dkv_parts(FastArgs g, RuleA
   }
 
   PartStage<D> st;
+  const Words dwords(r.docs, r.t_k);
   float lnext = 0.f, dnext = 0.f;
-  int qnext = -1;
+  int qnext = -1, qpos = 0;
   const int64_t base_row = (b * g.heads + kvh * (int64_t)group) * r.t_q;
   auto load = [&](int gh, int q0) __attribute__((always_inline)) {
     const int64_t rows0 = base_row + gh * (int64_t)r.t_q;
     st.load(FloatRows(g.q, rows0, r.t_q, g.hd), FloatRows(g.dout, rows0, r.t_q, g.hd), q0);
-    if (threadIdx.x < R) {
-      const int qq = q0 + (int)threadIdx.x;
-      const bool ok = qq < r.t_q;
-      lnext = ok ? att_l2(g.lse_in[rows0 + qq]) : __builtin_inff();
-      dnext = ok ? g.delta[rows0 + qq] : 0.f;
-      qnext = ok ? query_doc(r, r.off + qq) : -1;
-    }
+    lnext = Words(g.lse_in + rows0, r.t_q).real(q0 + lane);
+    dnext = Words(g.delta + rows0, r.t_q).real(q0 + lane);
+    qnext = dwords.whole(r.off + q0 + lane);
+    qpos = r.off + q0 + lane;
   };
   PartWalk<D> walk(visit);
   walk.start(first_q);
@@ -454,9 +454,9 @@ __global__ __launch_bounds__(THREADS, 1) void attend_dkv_parts(FastArgs g, RuleA
     __syncthreads();
     st.store(tiles);
     if (threadIdx.x < R) {
-      Ls[threadIdx.x] = lnext;
+      Ls[threadIdx.x] = att_l2(lnext);
       Ds[threadIdx.x] = dnext;
-      qdocs[threadIdx.x] = qnext;
+      qdocs[threadIdx.x] = qpos < 0 ? -1 : qnext;
     }
     walk.next();
     if (!walk.more()) {  // the next head's first

@@ -126,6 +126,23 @@ def test_few_key_heads_cut_into_parts(hipdev, dtype, hd, heads, kv_heads, t_q, t
     check(hipdev, q, k, v, do, dtype, {}, dict(causal=True))
 
 
+@pytest.mark.parametrize("dtype,hd,softcap", [("bfloat16", 128, 0.0), ("float16", 72, 4.0)])
+def test_score_gradients_past_the_workspace_limit(hipdev, dtype, hd, softcap):
+    """Calls whose score gradients would take more than 2.5 GiB compute the scores again in the dQ pass: two heads, repeated
+    until they do, each repeat bit for bit the first."""
+    rng, (q, k, v, do) = draw(hd, dtype, 1, 2, 2, 2048, 2048, hd, hd)
+    reps = (5 << 29) // (2 * 16 * 32 * 16384) + 1
+    docs = packed(rng, 1, 2048, 400)
+    rules = dict(documents=docs, prefix=np.array([300], np.int32)) if softcap else {}
+    flags = dict(causal=True, softcap=softcap)
+    many = lambda x: np.tile(x, (reps, *[1] * (x.ndim - 1)))  # noqa: E731
+    got = trained(hipdev, *(many(x) for x in (q, k, v, do)), dtype, {n: many(x) for n, x in rules.items()}, flags)
+    want = definition(q, k, v, dout=do, dtype=dtype, **flags, **rules)
+    for name, x in got.items():
+        within(x[:1], *want[name], f"{name} {dtype}")
+        assert all(np.array_equal(x[r], x[0]) for r in range(1, reps)), name
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 def test_documents_in_any_order_and_rows_that_see_nothing(hipdev, dtype):
     rng, (q, k, v, do) = draw(5, dtype, 3, 2, 2, 200, 200, 64, 64)
