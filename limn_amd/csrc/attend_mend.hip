@@ -70,30 +70,22 @@ __global__ __launch_bounds__(GEN_THREADS, 1) void attend_mend_fwd(FastArgs g, Ru
   });
 }
 
+// Both of the backward's passes: two kernels were 2 us more where there is nothing to mend.
 template <typename T, int DT>
-__global__ __launch_bounds__(GEN_THREADS, 1) void attend_mend_dq(FastArgs g, RuleArgs ra, int64_t blocks) {
+__global__ __launch_bounds__(GEN_THREADS, 1) void attend_mend_bwd(FastArgs g, FastArgs kv, RuleArgs ra, int64_t blocks, int64_t kv_blocks) {
   __shared__ float lds[GEN_LDS];
-  const int64_t nqb = (ra.t_q + ATT_ROWS - 1) / ATT_ROWS;
+  const int64_t nqb = (ra.t_q + ATT_ROWS - 1) / ATT_ROWS, nkb = (ra.t_k + ATT_ROWS - 1) / ATT_ROWS;
+  const int group = g.heads / g.kv_heads;
+  const GenBwd gen = {g.q, g.k, g.v, g.out, g.dout, g.lse_in, g.delta, g.o0, kv.o0, kv.o1, g.heads, g.kv_heads, g.hd, g.hd, 1, g.scale};
   each_odd(g.odd, blocks, [&](int64_t id) {
     const int64_t bh = id / nqb, b = bh / g.heads;
     const int head = (int)(bh - b * g.heads), q0 = (int)(id - bh * nqb) * ATT_ROWS;
-    const GenBwd gen = {g.q, g.k, g.v, g.out, g.dout, g.lse_in, g.delta, g.o0, nullptr, nullptr, g.heads, g.kv_heads, g.hd, g.hd, 1, g.scale};
-    for (int j = 0; j < ATT_ROWS && q0 + j < ra.t_q; j += 32)
-      gen_dq_block<T, DT>(gen, ra, RowMap{1, head, ra.t_q}, b, head / (g.heads / g.kv_heads), q0 + j, false, lds);
+    for (int j = 0; j < ATT_ROWS && q0 + j < ra.t_q; j += 32) gen_dq_block<T, DT>(gen, ra, RowMap{1, head, ra.t_q}, b, head / group, q0 + j, false, lds);
   });
-}
-
-template <typename T, int DT>
-__global__ __launch_bounds__(GEN_THREADS, 1) void attend_mend_dkv(FastArgs g, RuleArgs ra, int64_t blocks) {
-  __shared__ float lds[GEN_LDS];
-  const int64_t nkb = (ra.t_k + ATT_ROWS - 1) / ATT_ROWS;
-  const int group = g.heads / g.kv_heads;
-  each_odd(g.odd, blocks, [&](int64_t id) {
+  each_odd(kv.odd, kv_blocks, [&](int64_t id) {
     const int64_t bk = id / nkb, b = bk / g.kv_heads;
     const int kvh = (int)(bk - b * g.kv_heads), k0 = (int)(id - bk * nkb) * ATT_ROWS;
-    const GenBwd gen = {g.q, g.k, g.v, g.out, g.dout, g.lse_in, g.delta, nullptr, g.o0, g.o1, g.heads, g.kv_heads, g.hd, g.hd, 1, g.scale};
-    for (int j = 0; j < ATT_ROWS && k0 + j < ra.t_k; j += 32)
-      gen_dkv_block<T, DT>(gen, ra, RowMap{group, kvh * group, group * ra.t_q}, b, kvh, k0 + j, lds);
+    for (int j = 0; j < ATT_ROWS && k0 + j < ra.t_k; j += 32) gen_dkv_block<T, DT>(gen, ra, RowMap{group, kvh * group, group * ra.t_q}, b, kvh, k0 + j, lds);
   });
 }
 
@@ -129,10 +121,7 @@ int mend_fwd(const FastArgs& g, const RuleArgs& ra, hipStream_t stream) {
 template <typename T, int DT>
 int mend_bwd(const FastArgs& g, const FastArgs& kv, const RuleArgs& ra, hipStream_t stream) {
   const int64_t blocks = g.batch * g.heads * ((ra.t_q + ATT_ROWS - 1) / ATT_ROWS), kv_blocks = g.batch * g.kv_heads * ((ra.t_k + ATT_ROWS - 1) / ATT_ROWS);
-  hipLaunchKernelGGL((attend_mend_dq<T, DT>), dim3(mend_grid(blocks)), dim3(GEN_THREADS), 0, stream, g, ra, blocks);
-  const int rc = check_hip(hipGetLastError(), "launching attention's mending");
-  if (rc != LIMN_HIP_OK) return rc;
-  hipLaunchKernelGGL((attend_mend_dkv<T, DT>), dim3(mend_grid(kv_blocks)), dim3(GEN_THREADS), 0, stream, kv, ra, kv_blocks);
+  hipLaunchKernelGGL((attend_mend_bwd<T, DT>), dim3(mend_grid(blocks > kv_blocks ? blocks : kv_blocks)), dim3(GEN_THREADS), 0, stream, g, kv, ra, blocks, kv_blocks);
   return check_hip(hipGetLastError(), "launching attention's mending");
 }
 

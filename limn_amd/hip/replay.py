@@ -46,7 +46,7 @@ POINTER_ARGS = {
     STEP_XENT_BWD: frozenset(range(7)) | {11},
 }
 
-LAUNCHES = {STEP_SDPA_BWD: 2, STEP_ATTEND_FWD: 3, STEP_ATTEND_BWD: 7, STEP_XENT_FWD: 4, STEP_XENT_BWD: 8}
+LAUNCHES = {STEP_SDPA_BWD: 2, STEP_ATTEND_FWD: 3, STEP_ATTEND_BWD: 6, STEP_XENT_FWD: 4, STEP_XENT_BWD: 8}
 
 ARG = np.dtype([("value", np.int64), ("slot", np.int32), ("reserved", np.int32)])
 STEP = np.dtype([("kind", np.int32), ("nargs", np.int32), ("first", np.int64), ("function", np.uint64),
