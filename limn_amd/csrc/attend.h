@@ -1,4 +1,4 @@
-// Internal launch interface between the C ABI (attend_capi.hip) and the kernels of attention with score rules.
+// Internal launch interface between the C ABI (attend.hip) and the kernels of attention with score rules.
 #pragma once
 
 #include "common.h"
@@ -32,7 +32,7 @@ struct AttendArgs {
   int64_t group() const { return heads / kv_heads; }
 };
 
-// Kernels in float arithmetic for every type and head dim up to 256 (attend_general.hip).
+// Kernels in float arithmetic for every type and head dim up to 256 (attend_general.h).
 int64_t attend_general_workspace(const AttendArgs& a, bool backward);
 int launch_attend_general_fwd(const AttendArgs& a);
 int launch_attend_general_bwd(const AttendArgs& a);

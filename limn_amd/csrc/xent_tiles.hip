@@ -576,15 +576,26 @@ __global__ __launch_bounds__(1024) void xent_fold(Products s, const float* __res
   }
 }
 
-// A matrix of `rows` rows of `width` elements as PARTS matrices of rows of `padded` elements, zeros past the width:
-// 8 consecutive elements a thread.
+// A matrix of `rows` rows of `width` elements and where its PARTS matrices of rows of `padded` elements go, `part` elements
+// behind one another.
+struct Copied {
+  const void* src;
+  u16* dst;
+  int64_t rows, part;
+};
+
+// Two such matrices in one launch, zeros past the width: 8 consecutive elements a thread.
 template <typename S, typename T, int PARTS>
-__global__ __launch_bounds__(256) void xent_parts(const typename S::Storage* __restrict__ src, u16* __restrict__ dst, int64_t rows, int width, int padded, int64_t part) {
+__global__ __launch_bounds__(256) void xent_parts(Copied m0, Copied m1, int width, int padded) {
   const int chunks = padded / 8;
-  const int64_t total = rows * chunks;
+  const int64_t total = (m0.rows + m1.rows) * chunks;
   for (int64_t i = blockIdx.x * (int64_t)256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
-    const int64_t row = i / chunks;
-    const int c = (int)(i - row * chunks) * 8;
+    const int64_t both = i / chunks;
+    const int c = (int)(i - both * chunks) * 8;
+    const bool second = both >= m0.rows;
+    const int64_t row = second ? both - m0.rows : both, part = second ? m1.part : m0.part;
+    const typename S::Storage* src = (const typename S::Storage*)(second ? m1.src : m0.src);
+    u16* dst = second ? m1.dst : m0.dst;
     float v[8];
 #pragma unroll
     for (int e = 0; e < 8; e++) v[e] = c + e < width ? S::load(src, row * width + c + e) : 0.f;
@@ -662,15 +673,16 @@ struct Cut {
   int64_t split, chunk;
 };
 // Tiles of 256 in as many slices of k as leave no more than a quarter of the CUs idle, where slices are long enough for
-// their partial results (in three parts a slice is six times the work); else as matmul.hip cuts its products.
+// their partial results; else as matmul.hip cuts its products. In three parts a slice is six times the work.
 Cut cut(int64_t m, int64_t n, int64_t k, int parts) {
-  const int64_t tiles = ((m + 255) / 256) * ((n + 255) / 256);
-  if (tiles < FILL) {
+  const int64_t tiles = ((m + 255) / 256) * ((n + 255) / 256), work = parts == 3 ? 6 : 1;
+  if (tiles < FILL && m > 128) {
     const int64_t split = FILL / tiles, chunk = up((k + split - 1) / split, BK);
-    if (split * tiles * 4 >= 3 * FILL && (split == 1 || chunk * (parts == 3 ? 6 : 1) >= 1024)) return {256, (k + chunk - 1) / chunk, chunk};
+    if (split * tiles * 4 >= 3 * FILL && (split == 1 || chunk * work >= 1024)) return {256, (k + chunk - 1) / chunk, chunk};
   }
-  const MatmulPlan p = plan_matmul(MatmulShape{1, m, n, k});
-  return {p.tile, p.split, p.chunk};
+  const MatmulPlan p = plan_matmul(MatmulShape{1, m, n, k * work});
+  const int64_t chunk = up((k + p.split - 1) / p.split, BK);
+  return {p.tile, (k + chunk - 1) / chunk, chunk};
 }
 
 int64_t product_bytes(int64_t m, int64_t n, int64_t k, int parts) {
@@ -750,10 +762,9 @@ int launch_product(Products s, const Cut& c, float* slices, float* acc, bool fir
 }
 
 template <typename S, typename T, int PARTS>
-int launch_parts(const void* src, u16* dst, int64_t rows, const XentArgs& a, int64_t part) {
-  const int64_t padded = padded_width(a), groups = (rows * (padded / 8) + 255) / 256;
-  hipLaunchKernelGGL((xent_parts<S, T, PARTS>), dim3((unsigned)(groups < 16384 ? groups : 16384)), dim3(256), 0, a.stream, (const typename S::Storage*)src, dst, rows,
-                     (int)a.width, (int)padded, part);
+int launch_parts(const Copied& m0, const Copied& m1, const XentArgs& a) {
+  const int64_t padded = padded_width(a), groups = ((m0.rows + m1.rows) * (padded / 8) + 255) / 256;
+  hipLaunchKernelGGL((xent_parts<S, T, PARTS>), dim3((unsigned)(groups < 16384 ? groups : 16384)), dim3(256), 0, a.stream, m0, m1, (int)a.width, (int)padded);
   return check_hip(hipGetLastError(), "launching an operand's parts");
 }
 
@@ -776,7 +787,6 @@ int fwd(const XentArgs& a) {
     wp = (u16*)space.take(PARTS * piece * width * 2);
     l.x = xp;
     l.part_x = a.rows * width;
-    rc = launch_parts<S, T, PARTS>(a.x, xp, a.rows, a, l.part_x);
   }
   for (int64_t v0 = 0; v0 < a.vocab && rc == LIMN_HIP_OK; v0 += piece) {
     const typename S::Storage* w = (const typename S::Storage*)a.w + v0 * a.width;
@@ -787,7 +797,8 @@ int fwd(const XentArgs& a) {
     if (copies) {
       l.w = wp;
       l.part_w = l.piece * width;
-      if ((rc = launch_parts<S, T, PARTS>(w, wp, l.piece, a, l.part_w)) != LIMN_HIP_OK) return rc;
+      const Copied rows = {a.x, (u16*)l.x, v0 == 0 ? a.rows : 0, l.part_x};
+      if ((rc = launch_parts<S, T, PARTS>(rows, Copied{w, wp, l.piece, l.part_w}, a)) != LIMN_HIP_OK) return rc;
     }
     rc = bm == 256 ? launch_stats<T, 256, PARTS>(l, a.stream) : launch_stats<T, 128, PARTS>(l, a.stream);
   }
@@ -826,7 +837,6 @@ int bwd(const XentArgs& a) {
     wp = (u16*)space.take(PARTS * p.piece * width * 2);
     l.x = xp;
     l.part_x = a.rows * width;
-    if ((rc = launch_parts<S, T, PARTS>(a.x, xp, a.rows, a, l.part_x)) != LIMN_HIP_OK) return rc;
   }
   for (int64_t v0 = 0; v0 < a.vocab; v0 += p.piece) {
     const bool first = v0 == 0, last = v0 + p.piece >= a.vocab;
@@ -839,7 +849,8 @@ int bwd(const XentArgs& a) {
     if (copies) {
       l.w = wp;
       l.part_w = l.piece * width;
-      if ((rc = launch_parts<S, T, PARTS>(w, wp, l.piece, a, l.part_w)) != LIMN_HIP_OK) return rc;
+      const Copied rows = {a.x, (u16*)l.x, v0 == 0 ? a.rows : 0, l.part_x};
+      if ((rc = launch_parts<S, T, PARTS>(rows, Copied{w, wp, l.piece, l.part_w}, a)) != LIMN_HIP_OK) return rc;
     }
     rc = tile_for(a.rows, l.ldz) == 256 ? launch_dz<T, 256, PARTS>(l, a.stream) : launch_dz<T, 128, PARTS>(l, a.stream);
     if (rc != LIMN_HIP_OK) return rc;
