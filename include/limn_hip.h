@@ -214,8 +214,10 @@ int limn_hip_contract_pays(int dtype, int64_t batch, int64_t M, int64_t N, int64
  *   outside [0, t_k] is taken as the nearest end. t_q <= t_k where the call is causal or has documents or
  *   lengths. hd and hd_v at most 256.
  * `workspace` must hold limn_hip_attend_workspace(...) bytes, 16-byte aligned, for this call alone: calls
- * that may overlap, and captured graphs that may run at once, need one each. Every result is deterministic.
- * No counterpart in the reference (its attention has a causal and a key mask, limn/tensor.py:509-575);
+ * that may overlap, and captured graphs that may run at once, need one each. A backward's holds up to 2.5 GiB of
+ * score gradients between its passes. Every result is deterministic. Sums and statistics are float32; float32
+ * operands are multiplied as sums of three bfloat16 numbers each (to some 2^-24 |x y| + 2^-134 (|x| + |y|)) where
+ * the call has more than 256 tiles of 32 query rows. No counterpart in the reference (its attention has a causal and a key mask, limn/tensor.py:509-575);
  * composed there, the scores are a tensor in memory.
  */
 int limn_hip_attend_fwd(const void* q, const void* k, const void* v, const void* slopes, const void* documents,
@@ -254,7 +256,7 @@ int limn_hip_xent_fwd(const void* x, const void* w, const void* targets, void* l
 
 /* Its gradients for the cotangents g (rows, float32) of loss: dx = dz w and dw = dz^T x, with
  * dz[n, v] = g[n] (exp(z[n, v] - lse[n]) - [v = targets[n]]); a half width rounds dz to its own type, as the
- * operand of both products. */
+ * operand of both products, float16 multiplied by the power of two that fits the largest |g|. */
 int limn_hip_xent_bwd(const void* x, const void* w, const void* targets, const void* lse, const void* g, void* dx, void* dw,
                       int dtype, int64_t rows, int64_t width, int64_t vocab, void* workspace, int64_t workspace_bytes,
                       void* stream);

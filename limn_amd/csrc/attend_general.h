@@ -11,8 +11,10 @@
 //   accumulator item i then holds streamed row 8 (i / 4) + 4 h + i % 4, which is exactly the pair of
 //     rows (h = 0, 1) that step i of the next product contracts: its B operand is item i as it stands,
 //     and its A operand one element X[streamed row][32 dt + n] a lane, 128 consecutive bytes a half-wave.
-// Nothing is staged, so there is no barrier in the loop; what bounds it is the float matrix rate
-// (64 cycles an instruction).
+// Nothing is staged, so there is no barrier in the loop, and 64 workgroups already spread 8 heads x 256 rows over the GPU
+// (float32 x 64, every rule: forward 22 us, backward 27 + 37, chains of loads and products). Where there are many, what
+// bounds it is the reads: a wave's streamed tile serves 32 resident rows alone (64 heads x 2048 x 64 causal: forward 1248
+// us, 27 of the 157 TFLOP/s that float32 products reach).
 //
 // A hidden pair contributes nothing, whatever stands in the hidden row: its probability is selected to 0,
 // and where the streamed row of a product holds an infinity or a NaN (0 times which is NaN), the row's

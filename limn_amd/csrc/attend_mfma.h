@@ -15,6 +15,11 @@
 //    so capped attention is bound by the vector ALU.
 //  - the query heads of a key head are one loop of the dK/dV pass: their gradients are one sum in head order.
 //
+// Measured (causal, bf16; of the rate of the products it must do): 4 x 16 heads over 4 key heads x 4096 x 128, capped:
+// forward 366 us (750 TFLOP/s), backward 1090 (630); 8 x 16 heads x 4096 x 128 with documents of 1024: 385 and 1080 us
+// (540 and 480 TFLOP/s: of some 10 us that a workgroup takes to begin and end, 12 tiles hide less than 33);
+// 32 x 8 heads x 512 x 64 with distance and documents of 200: 47 and 104 us, bound by those beginnings.
+//
 // Hidden pairs have exact zeros in the second products, but a zero times an infinity or a NaN is NaN. Such a
 // result stays NaN to the end of the block, so a block whose totals are not all finite says so (odd), and a
 // launch behind the pass computes those blocks again in float arithmetic (attend_mend.hip, by attend_general.h's
@@ -793,8 +798,8 @@ __global__ __launch_bounds__(THREADS, 2) void attend_dkv_mfma(FastArgs g, RuleAr
 // The 8-wave workgroup of sdpa_bwd_kv_dual (which says what each wave does, and why K and V sit in LDS): wave w
 // takes keys 32 (w % 4) .. + 31 and queries 32 (w / 4) .. + 31 of every tile, tiles of 64 rows x 128 dims come by
 // LDS DMA (dims past hd as zeros) into one of two buffers while the other is computed. One wave a SIMD with K
-// and V in registers (as attend_dkv_mfma, 400 registers) took 1317 us where this takes 797 (4 x 16 heads over 4 key
-// heads, 4096 rows, capped).
+// and V in registers (as attend_dkv_mfma, 400 registers) took 1317 us where this takes 700, 850 with dS stored for the
+// dQ pass (4 x 16 heads over 4 key heads, 4096 rows, capped).
 
 // rows [row0, row0 + 64) of hd elements into a swizzled 64 x 128 tile, this wave's eighth
 struct HeadDma8 {
@@ -1097,8 +1102,8 @@ __global__ __launch_bounds__(64 * KV_WAVES, 1) void attend_dkv_wide(FastArgs g, 
 // ---- forward and dQ pass past 64 dims: tiles by LDS DMA ---------------------------------------------------------
 // As attend_fwd_mfma and attend_dq_mfma, with the streamed tiles copied straight into swizzled LDS tiles of 64 x 128
 // (dims past hd as zeros), and the forward pipelined as sdpa_fwd_dma is: a tile's exponentials and its V product
-// are issued beside the next tile's scores. Staged through registers the forward took 753 us and the dQ pass 881
-// (8 x 16 heads x 4096 rows, causal).
+// are issued beside the next tile's scores. Staged through registers the forward took 753 us and the dQ pass 881,
+// so 577 and 773 (8 x 16 heads x 4096 rows, causal).
 
 // rows [row0, row0 + 64) of hd elements into a swizzled 64 x 128 tile, this wave's quarter
 struct HeadDma4 {
@@ -1493,7 +1498,7 @@ __global__ __launch_bounds__(THREADS, 2) void attend_dq_wide(FastArgs g, RuleArg
 // a wave's, of 1 KB for 32 keys and every second 16 bytes of theirs, each in the order in which a wave of the dK/dV pass
 // stores it (chunks of 8 queries: of the first eight of 16, key by key, then of the second). A wave copies its own 4 KB
 // into LDS, chunks of a KB exchanged so that the four 64-byte pieces which a half wave reads transposed lie in
-// different banks. One product where attend_dq_wide has three, bound by the reads of dS. The dK/dV pass wrote those
+// different banks. One product where attend_dq_wide has three, bound by the reads of dS (1.1 GB in 278 us, 4 TB/s, at 4 x 16 heads x 4096). The dK/dV pass wrote those
 // matrices' halves of 64 queries that its own lists and causality name; the others are not read.
 
 template <typename T, int D>
