@@ -265,9 +265,9 @@ int launch_fast(const AttendArgs& a, bool backward) {
   g.head_group = head_group(a, a.batch * a.heads, backward);
   int rc = LIMN_HIP_OK;
   if (a.documents != nullptr && (rc = launch_attend_ranges(ra, ranges, a.batch, g.granules, a.stream)) != LIMN_HIP_OK) return rc;
-  // without causality and documents a hidden key is one past the live ones, which reads as zeros; float32's parts do
-  // not hold infinities
-  const bool mend = a.causal || a.documents != nullptr || a.dtype == LIMN_HIP_FLOAT32;
+  // without causality and documents a hidden key is one past the live ones, which reads as zeros; but float32's parts do
+  // not hold infinities, and float16's score gradients may overflow where the result does not
+  const bool mend = a.causal || a.documents != nullptr || a.dtype == LIMN_HIP_FLOAT32 || (backward && a.dtype == LIMN_HIP_FLOAT16);
   if (!backward) {
     g.lse = (float*)a.o1;
     rc = LIMN_ATTEND_PASS(fwd, g);

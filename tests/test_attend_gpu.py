@@ -77,6 +77,14 @@ def test_cotangents_of_every_size(hipdev, dtype, hd, bits):
     check(hipdev, q, k, v, do, dtype, dict(slopes=np.array([0.25, 0.0625], np.float32)), dict(causal=True, softcap=5.0))
 
 
+@pytest.mark.parametrize("hd", [64, 80, 128])
+def test_large_cotangents_of_a_call_that_sees_everything(hipdev, hd):
+    """Score gradients past float16's range (they go multiplied by 2^8) in a call without masks, whose gradients are finite."""
+    _, (q, k, v, do) = draw(hd, "float16", 1, 2, 1, 130, 130, hd, hd)
+    got = check(hipdev, q, k, v, storage_values(do * np.float32(2.0**11), DTYPES["float16"]), "float16", {}, dict(scale=0.25))
+    assert np.abs(got["dq"]).max() > 256
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("hd,hd_v", [(1, 1), (8, 8), (16, 16), (32, 32), (33, 33), (40, 40), (64, 64), (64, 80), (72, 72), (80, 80), (96, 96), (100, 100), (128, 128), (128, 64), (160, 200), (256, 256)])
 def test_head_dims(hipdev, dtype, hd, hd_v):
