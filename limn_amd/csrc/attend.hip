@@ -187,9 +187,11 @@ bool aligned16(const AttendArgs& a, bool backward) {
   return at % 16 == 0;
 }
 
-// Forward calls of fewer queries than half a tiled block's 128 rows share their keys' bytes between the heads of a group
-// and split long caches (attend_token.hip).
-bool token_sizes(const AttendArgs& a) { return half_sizes(a) && a.t_q < 64; }
+// Forward calls that share their keys' bytes between the heads of a group and split long caches (attend_token.hip): of fewer
+// queries than half a tiled block's 128 rows, and of a part of a sequence against a long cache in so few blocks that the
+// tiled kernel would leave CUs idle. 32768 keys x 128, tiled against these: 128 queries of 8 heads 642 and 90 us, of 32
+// over 8 key heads 646 and 186, 512 of 32 (128 blocks) 646 and 637; 1024 keys, 128 of 8: 30 and 31 (64 dims 26 and 20).
+bool token_sizes(const AttendArgs& a) { return half_sizes(a) && (a.t_q < 64 || (row_blocks(a) < 128 && a.t_k >= 1024 && a.t_q <= a.t_k / 4)); }
 
 // A call of such sizes goes to them where every buffer is 16-byte aligned and the scale positive (the forward's
 // reference point is taken over unscaled scores).

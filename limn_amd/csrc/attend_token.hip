@@ -1,5 +1,5 @@
-// Attention with score rules for few queries against a cache (the single-token form): half widths,
-// hd == hd_v up to 128 in multiples of 8, no documents.
+// Attention with score rules for few queries against a cache (the single-token form, and parts of a sequence against
+// what came before): half widths, hd == hd_v up to 128 in multiples of 8, no documents.
 //
 // What bounds it is reading k and v once (2 hd bytes each a key): everything is laid out for that.
 //  - The queries of every head that shares a key head are rows of one tile (16 NR packed rows), so k and v are

@@ -242,6 +242,24 @@ def test_tokens_against_a_cache(hipdev, dtype, heads, kv_heads, t_q, t_k, dim, l
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("heads,kv_heads,t_q,t_k,dim,lengths", [
+    (2, 2, 64, 1024, 64, [1024]), (4, 2, 200, 1500, 128, [1500, 333]), (3, 1, 256, 1024, 80, [1000]), (2, 1, 333, 4097, 64, [4097]), (6, 3, 65, 2000, 40, [64, 0, 1999])])
+def test_part_of_a_sequence_against_its_cache(hipdev, dtype, heads, kv_heads, t_q, t_k, dim, lengths):
+    rng, (q, k, v, _) = draw(t_k + dim, dtype, len(lengths), heads, kv_heads, t_q, t_k, dim, dim, std=2.0)
+    for b, n in enumerate(lengths):
+        k[b, :, n:] = np.nan
+        v[b, :, n:] = np.nan
+    rules = dict(lengths=np.array(lengths, np.int32), slopes=(0.9 ** np.arange(1, heads + 1) * 0.05).astype(np.float32), prefix=np.full(len(lengths), 300, np.int32))
+    if min(lengths) > 100:
+        v[0, 0, min(lengths) - 50, 3] = np.inf  # seen by the last rows alone
+    for softcap, given in ((0.0, dict(lengths=rules["lengths"])), (20.0, rules)):
+        out, lse = served(hipdev, q, k, v, dtype, given, causal=True, softcap=softcap)
+        want = definition(q, k, v, dtype=dtype, causal=True, softcap=softcap, **given)
+        within(out, *want["out"], "out")
+        within(lse, *want["lse"], "lse")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("bad", [np.nan, np.inf])
 def test_a_key_some_queries_do_not_see(hipdev, dtype, bad):
     """The newest keys of several queries hold `bad`: the queries before them stay as they are, in a short cache and a long one."""
