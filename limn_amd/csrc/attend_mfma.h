@@ -11,8 +11,9 @@
 //  - a half tile that every row of the wave sees whole takes no element tests (a wave-uniform branch);
 //  - the cap and the distance are float arithmetic on the score tile. Per 32 x 32 tile at D = 128 the matrix
 //    cores take 512 cycles a wave for the forward's two products; the softmax takes 16 exponentials of 16
-//    cycles and about 6 other operations of 4 an element, the cap an exponential and a reciprocal more,
-//    so capped attention is bound by the vector ALU.
+//    cycles and about 6 other operations of 4 an element, the cap an exponential and a reciprocal more.
+//    At two waves a SIMD it is the length of that chain which counts, not its issue: a polynomial tanh of near
+//    scores, 20 cycles an element less, took as long (385 and 375 us forward, 1096 and 1110 backward, of the case below).
 //  - the query heads of a key head are one loop of the dK/dV pass: their gradients are one sum in head order.
 //
 // Measured (causal, bf16; of the rate of the products it must do): 4 x 16 heads over 4 key heads x 4096 x 128, capped:
