@@ -46,7 +46,7 @@ POINTER_ARGS = {
     STEP_XENT_BWD: frozenset(range(7)) | {11},
 }
 
-LAUNCHES = {STEP_SDPA_BWD: 2, STEP_ATTEND_FWD: 3, STEP_ATTEND_BWD: 6, STEP_XENT_FWD: 4, STEP_XENT_BWD: 8}
+LAUNCHES = {STEP_SDPA_BWD: 2, STEP_ATTEND_FWD: 2, STEP_ATTEND_BWD: 4, STEP_XENT_FWD: 4, STEP_XENT_BWD: 8}
 
 ARG = np.dtype([("value", np.int64), ("slot", np.int32), ("reserved", np.int32)])
 STEP = np.dtype([("kind", np.int32), ("nargs", np.int32), ("first", np.int64), ("function", np.uint64),
@@ -93,7 +93,8 @@ class Program:
     def launches(self) -> int:
         """Kernel launches of the list, at most: a contraction given a workspace may fold k slices, one of
         half widths copy its operands as well; LAUNCHES has the other kinds of
-        several (a cross entropy's for one piece of the vocabulary)."""
+        several (a cross entropy's for one piece of the vocabulary, attention's without documents or parts: one
+        attention and its gradients are faster launch by launch, 230 us against 241 at 8 x 12 heads x 1021 x 80)."""
         total = 0
         for kind, first in zip(self.steps["kind"].tolist(), self.steps["first"].tolist()):
             value = lambda k: int(self.args["value"][first + k])
