@@ -470,14 +470,13 @@ __device__ __forceinline__ void gen_dq_block(const GenBwd& g, const RuleArgs& ra
 }
 
 // dk and dv of keys [key0, key0 + 32): a hidden key, one past the live ones too, gets zeros.
-template <typename T, int DT>
+// KEEP: the resident fragments stay in registers; past 128 dims they would not fit beside the totals, and are read
+// again for every tile (from L1).
+template <typename T, int DT, bool KEEP = (DT <= 4)>
 __device__ __forceinline__ void gen_dkv_block(const GenBwd& g, const RuleArgs& ra, const RowMap& map, int64_t b, int kvh, int key0,
                                               float* lds) {
   typedef typename T::Storage S;
   constexpr int CH = DT * 4;
-  // head dims past 128: the resident fragments would not fit the registers beside the totals, and are
-  // read again for every tile (from L1)
-  constexpr bool KEEP = DT <= 4;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 31, h = lane >> 5;
   const Rules r = rules_of(ra, b);
   const int key = key0 + n;

@@ -85,7 +85,7 @@ __global__ __launch_bounds__(GEN_THREADS, 1) void attend_mend_bwd(FastArgs g, Fa
   each_odd(kv.odd, kv_blocks, [&](int64_t id) {
     const int64_t bk = id / nkb, b = bk / g.kv_heads;
     const int kvh = (int)(bk - b * g.kv_heads), k0 = (int)(id - bk * nkb) * ATT_ROWS;
-    for (int j = 0; j < ATT_ROWS && k0 + j < ra.t_k; j += 32) gen_dkv_block<T, DT>(gen, ra, RowMap{group, kvh * group, group * ra.t_q}, b, kvh, k0 + j, lds);
+    for (int j = 0; j < ATT_ROWS && k0 + j < ra.t_k; j += 32) gen_dkv_block<T, DT, (DT <= 2)>(gen, ra, RowMap{group, kvh * group, group * ra.t_q}, b, kvh, k0 + j, lds);
   });
 }
 
