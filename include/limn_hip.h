@@ -217,7 +217,7 @@ int limn_hip_contract_pays(int dtype, int64_t batch, int64_t M, int64_t N, int64
  * that may overlap, and captured graphs that may run at once, need one each. A backward's holds up to 2.5 GiB of
  * score gradients between its passes. Every result is deterministic. Sums and statistics are float32; float32
  * operands are multiplied as sums of three bfloat16 numbers each (to some 2^-24 |x y| + 2^-134 (|x| + |y|)) where
- * the call has more than 256 tiles of 32 query rows. No counterpart in the reference (its attention has a causal and a key mask, limn/tensor.py:509-575);
+ * the call has more than 256 tiles of 32 query rows (128 in a backward). No counterpart in the reference (its attention has a causal and a key mask, limn/tensor.py:509-575);
  * composed there, the scores are a tensor in memory.
  */
 int limn_hip_attend_fwd(const void* q, const void* k, const void* v, const void* slopes, const void* documents,

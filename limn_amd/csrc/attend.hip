@@ -172,15 +172,22 @@ int64_t row_blocks(const AttendArgs& a) { return a.batch * a.heads * ((a.t_q + A
 int64_t key_blocks(const AttendArgs& a) { return a.batch * a.kv_heads * ((a.t_k + ATT_ROWS - 1) / ATT_ROWS); }
 
 // float32 calls go to the tiles of 128 rows where the general kernels, with a workgroup for every 32, have more than
-// one for a CU. Causal at 64 dims, forward and backward, tiled against general: 8 heads x 256 rows 24 + 67 against
-// 18 + 57 us, 8 x 1024 64 + 196 against 77 + 181, 16 x 1024 65 + 197 against 107 + 355, 64 x 1024 94 + 260 against 423 + 1393.
-bool f32_rows(const AttendArgs& a) { return a.batch * a.heads * ((a.t_q + 31) / 32) > 256; }
+// one for a CU; a backward, whose few key blocks are cut into parts, from half as many on. Causal, forward + backward, tiled
+// against general at 64 dims: 8 heads x 256 rows 23 + 65 against 18 + 56 us, 8 x 512 37 + 88 against 27 + 98, 2 x 4096 223 +
+// 413 against 134 + 655, 16 x 1024 65 + 154 against 107 + 356, 64 x 1024 94 + 256 against 424 + 1393; at 128 dims 8 x 256
+// 38 + 107 against 29 + 104, 8 x 512 63 + 142 against 43 + 177, 16 x 1024 117 + 253 against 184 + 646.
+bool f32_rows(const AttendArgs& a, bool backward) {
+  const int64_t tiles = a.batch * a.heads * ((a.t_q + 31) / 32);
+  return backward ? tiles >= 128 : tiles > 256;
+}
 
 // Sizes these kernels serve: 16-byte rows; the tiled ones also need a head's rows within 32-bit byte
 // offsets and few enough streamed tiles for a block's list of them.
 bool row_sizes(const AttendArgs& a) { return a.hd == a.hd_v && a.hd % (a.dtype == LIMN_HIP_FLOAT32 ? 4 : 8) == 0 && a.hd <= 128; }
 bool half_sizes(const AttendArgs& a) { return a.dtype != LIMN_HIP_FLOAT32 && row_sizes(a); }
-bool fast_sizes(const AttendArgs& a) { return row_sizes(a) && a.t_q <= (1 << 17) && a.t_k <= (1 << 17) && (a.dtype != LIMN_HIP_FLOAT32 || f32_rows(a)); }
+bool fast_sizes(const AttendArgs& a, bool backward) {
+  return row_sizes(a) && a.t_q <= (1 << 17) && a.t_k <= (1 << 17) && (a.dtype != LIMN_HIP_FLOAT32 || f32_rows(a, backward));
+}
 
 bool aligned16(const AttendArgs& a, bool backward) {
   const uintptr_t at = (uintptr_t)a.q | (uintptr_t)a.k | (uintptr_t)a.v | (uintptr_t)a.o0 | (backward ? (uintptr_t)a.o1 | (uintptr_t)a.o2 | (uintptr_t)a.out | (uintptr_t)a.dout : 0);
@@ -195,7 +202,7 @@ bool token_sizes(const AttendArgs& a) { return half_sizes(a) && (a.t_q < 64 || (
 
 // A call of such sizes goes to them where every buffer is 16-byte aligned and the scale positive (the forward's
 // reference point is taken over unscaled scores).
-bool fast_call(const AttendArgs& a, bool backward) { return fast_sizes(a) && a.scale > 0 && aligned16(a, backward); }
+bool fast_call(const AttendArgs& a, bool backward) { return fast_sizes(a, backward) && a.scale > 0 && aligned16(a, backward); }
 
 // Parts of the queries that a call with fewer key blocks than fill the GPU (two workgroups a CU up to 64 half-width
 // dims, one else) cuts its dK/dV pass into, the heads of a group first: at least 4 tiles each. The backward of 16 heads
@@ -230,7 +237,7 @@ int64_t handed_bytes(const AttendArgs& a) {
 
 // flags of the blocks, the documents' ranges, and for the backward delta
 int64_t fast_workspace(const AttendArgs& a, bool backward) {
-  if (!fast_sizes(a)) return 0;
+  if (!fast_sizes(a, backward)) return 0;
   int64_t need = attend_align(row_blocks(a) * 4) + attend_align(a.batch * granules_of(a) * 16);
   if (backward) need += attend_align(key_blocks(a) * 4) + attend_align(a.batch * a.heads * a.t_q * 4) + attend_align(key_parts_bytes(a)) + attend_align(handed_bytes(a));
   return need;
