@@ -21,8 +21,8 @@
 //    dx += dz w (float32 totals over the pieces, rounded once behind the last) and dw = dz^T x.
 //    The piece (at most PIECE_BYTES of dz) is small enough that both products find most of it in the 256 MiB
 //    last-level cache.
-// 8192 rows x 2048 x 65536 bf16: 7.5 ms, the four products at 1180 TFLOP/s (a library product reaches 1230); 2048 x 512 x
-// 8191 float32: 473 us, 145 TFLOP/s in float32 terms (a library product 153); 48 rows x 512 x 32000 bf16: 68 us of kernels
+// 8192 rows x 2048 x 65536 bf16: 7.5-7.8 ms, the four products at 1130-1180 TFLOP/s (a library product reaches 1230); 2048 x
+// 512 x 8191 float32: 473-500 us, 140 TFLOP/s in float32 terms (a library product 153); 48 rows x 512 x 32000 bf16: 68 us of kernels
 // whose chains of stages few rows do not hide.
 // Keeping the logits would save the second x w^T, a quarter of the matrix work, for rows * vocab * 4 bytes.
 //
