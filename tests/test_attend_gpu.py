@@ -260,6 +260,20 @@ def test_part_of_a_sequence_against_its_cache(hipdev, dtype, heads, kv_heads, t_
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("heads,kv_heads,t_q,t_k,dim", [(4, 2, 130, 1111, 64), (2, 2, 256, 1024, 128)])
+def test_other_keys_than_the_queries_own(hipdev, dtype, heads, kv_heads, t_q, t_k, dim):
+    """Queries that see every live key, the distance taken from the end of them."""
+    rng, (q, k, v, _) = draw(t_k + dim, dtype, 2, heads, kv_heads, t_q, t_k, dim, dim)
+    k[1, :, 700:] = np.nan
+    v[1, :, 700:] = np.inf
+    given = dict(lengths=np.array([t_k, 700], np.int32), slopes=(0.02 * 0.9 ** np.arange(heads)).astype(np.float32))
+    out, lse = served(hipdev, q, k, v, dtype, given, softcap=10.0)
+    want = definition(q, k, v, dtype=dtype, softcap=10.0, **given)
+    within(out, *want["out"], "out")
+    within(lse, *want["lse"], "lse")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("bad", [np.nan, np.inf])
 def test_a_key_some_queries_do_not_see(hipdev, dtype, bad):
     """The newest keys of several queries hold `bad`: the queries before them stay as they are, in a short cache and a long one."""
