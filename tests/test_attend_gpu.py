@@ -331,3 +331,35 @@ def test_captured_and_replayed(hipdev, dtype, graphs):
         hipdev.replay_graphs = saved
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+def test_two_captured_programs_in_turn(hipdev, dtype):
+    """Two programs of the same sizes, whose workspaces (parts, score gradients between the passes) are one, replayed in turn."""
+    use_device(hipdev)
+    t = DTYPES[dtype]
+
+    def program(softcap):
+        def step(q, k, v, do, docs):
+            out = attend(q, k, v, causal=True, documents=docs, softcap=softcap)
+            out = attend(out, k, v, causal=True, softcap=softcap)
+            got = [out, *grad((out * do).sum(), [q, k, v])]
+            realize(*got)
+            return got
+
+        return step, capture(step)
+
+    def args(seed):
+        rng, (q, k, v, do) = draw(seed, dtype, 4, 4, 1, 300, 300, 128, 128)
+        return [*(Tensor(x, dtype=t, requires_grad=True) for x in (q, k, v)), Tensor(do, dtype=t), Tensor(packed(rng, 4, 300, 90), dtype=int32)]
+
+    programs, sets = [program(0.0), program(6.0)], [args(s) for s in range(2)]
+    for _, captured in programs:
+        for a in sets:
+            captured(*a)
+    for _ in range(3):
+        for a in sets:
+            results = [(step, captured(*a)) for step, captured in programs]
+            for step, got in results:
+                got = [x.numpy() for x in got]
+                fresh = [Tensor(x.numpy(), dtype=x.dtype, requires_grad=i < 3) for i, x in enumerate(a)]
+                for x, y in zip(got, step(*fresh)):
+                    np.testing.assert_array_equal(x, y.numpy())
