@@ -500,10 +500,11 @@ __device__ __forceinline__ void gen_dkv_block(const GenBwd& g, const RuleArgs& r
 #pragma unroll
   for (int dt = 0; dt < DT; dt++) gk[dt] = gv[dt] = gen_zero();
 
-  // the first row that can see one of the keys: query key0 - off, unless a prefix opens them to all
-  int from = 0;
-  if (r.causal && key0 >= r.pre) from = max(0, key0 - r.off) * map.group;
+  // the first row that can see one of the keys: query key0 - off, unless a prefix opens them to all. Of keys past the live
+  // ones no row does, and key0 - off may be past t_q there, whose rows 32 bits do not count.
   const int tiles = key0 < r.len ? (map.rows + 31) / 32 : 0;
+  int from = 0;
+  if (tiles > 0 && r.causal && key0 >= r.pre) from = max(0, key0 - r.off) * map.group;
   for (int rt = from / 32 + wave; rt < tiles; rt += GEN_WAVES) {
     const int row0 = rt * 32, row = row0 + n;
     const bool row_there = row < map.rows;
