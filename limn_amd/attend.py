@@ -107,6 +107,31 @@ def through(out: Tensor, inputs: tuple[Tensor, ...], g: Tensor) -> tuple[Tensor 
     return tuple(next(found) if t.requires_grad else None for t in inputs)
 
 
+def _tanh_terms(count: int) -> list[float]:
+    """The first coefficients of tanh(z) / z in powers of z^2, from tanh' = 1 - tanh^2."""
+    terms = [1.0]
+    while len(terms) < count:
+        n = len(terms)
+        terms.append(-sum(terms[i] * terms[n - 1 - i] for i in range(n)) / (2 * n + 1))
+    return terms
+
+
+def _capped(s: Tensor, softcap: float, wide) -> Tensor:
+    """softcap tanh(s / softcap), to a few half steps of itself: 1 - 2 / (1 + e^2z) is off by half steps of 1, however
+    small z is, so up to |z| = 1/2 the series takes its place (its first term left out is past the last bit)."""
+    inverse = 1.0 / softcap
+    z = s * inverse
+    near = s.minimum(0.625 * softcap).maximum(-0.625 * softcap)  # no more than the series is good for, where it is not taken
+    square = (near * inverse) * (near * inverse)
+    terms = _tanh_terms(16 if wide == float64 else 7)
+    ratio = square * terms[-1] + terms[-2]
+    for c in reversed(terms[:-2]):
+        ratio = ratio * square + c
+    # past +-40 tanh is +-1 in any float width, and the exponential finite
+    far = (1.0 - 2.0 * ((z * 2.0).minimum(80.0).maximum(-80.0).exp() + 1.0).reciprocal()) * softcap
+    return ((z * z) <= 0.25).where(near * ratio, far)
+
+
 def _composed(q: Tensor, k: Tensor, v: Tensor, slopes, documents, prefix, lengths, causal: bool, scale: float, softcap: float) -> Tensor:
     """The same from limn's primitives, the scores and weights at the accumulation width. (A weight of 0
     times a hidden key's infinity or NaN is NaN here; the kernels leave hidden keys out altogether.)"""
@@ -118,9 +143,7 @@ def _composed(q: Tensor, k: Tensor, v: Tensor, slopes, documents, prefix, length
     values = v.cast(wide).reshape(*lead, kv_heads, 1, t_k, v.shape[-1])
     s = (rows @ keys.transpose(-2, -1)) * scale
     if softcap:
-        # tanh(x) = 1 - 2 / (1 + exp(2x)); past +-40 it is +-1 in any float width, and the exponential finite
-        e = (s * (2.0 / softcap)).minimum(80.0).maximum(-80.0).exp()
-        s = (1.0 - 2.0 * (e + 1.0).reciprocal()) * softcap
+        s = _capped(s, softcap, wide)
     key = Tensor.arange(t_k).reshape(*ones, 1, 1, 1, t_k)
     at = Tensor.arange(t_q).reshape(*ones, 1, 1, t_q, 1)
     length = None if lengths is None else lengths.minimum(t_k).maximum(0).reshape(*lead, 1, 1, 1, 1)

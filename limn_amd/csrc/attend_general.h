@@ -92,9 +92,9 @@ __device__ __forceinline__ float gen_score(const Rules& r, float x, float slope2
   float y = x * r.c2;
   bent = 1.f;
   if (r.cap_out > 0.f) {
-    const float t = tanhf(y / r.cap_out);
-    y = t * r.cap_out;
-    bent = 1.f - t * t;
+    const float z = y * r.cap_un, t = tanhf(z);
+    if (fabsf(z) > 0x1p-13f) y = t * r.cap_out;  // below, the score itself: z may be under float's normal numbers
+    bent = fmaf(-t, t, 1.f);
   }
   return y - slope2 * far;
 }

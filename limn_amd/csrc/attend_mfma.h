@@ -304,14 +304,23 @@ constexpr float ds_down() {
 
 // ---- scores ---------------------------------------------------------------------------------------------
 
+// How scores are capped. CAP_SHORT, half widths under caps up to CAP_SHORT_MOST: 1 - 2 / (1 + e^2z), whose error is one of the
+// cap, 8 2^-24 of it, wherever z is: 2^-15 of a score at most here, a sixteenth of float16's half step on a weight.
+// CAP_EXACT, everything else: cap_scores. (Forward and backward of 4 x 16 heads over 4 key heads x 4096 x 128, cap 50: 369 + 1135
+// us short, 383 + 1150 exact; of 8 x 16 x 2048 x 64 161 + 459 and 177 + 454; where many scores are past half the cap
+// 355 + 1106 and 513 + 1264, as the exact form computes both of its halves there.)
+enum Cap { CAP_NONE, CAP_SHORT, CAP_EXACT };
+constexpr float CAP_SHORT_MOST = 64.f;
+
 // A score tile item into log2 units (as it is, if there is neither cap nor distance: then c2 comes in with
-// the exponential), and for the backward the cap's derivative.
-template <bool CAP, bool BIAS, bool GRAD>
+// the exponential; under CAP_EXACT cap_scores has been over the tile), and for the backward the cap's derivative.
+template <Cap CAP, bool BIAS, bool GRAD>
 __device__ __forceinline__ float bend(float x, const Rules& r, float slope2, float far, float& bent) {
   float y = x;
-  if (CAP) {
-    // tanh(z) = 1 - 2 / (1 + e^2z): off by some 2^-23 absolutely, a part of a half width's step after the
-    // softmax; the derivative 1 - tanh^2 = 4 w (1 - w) with w = 1 / (1 + e^2z)
+  if (CAP == CAP_EXACT) {
+    if (GRAD) bent = cap_slope(r, x);
+  } else if (CAP == CAP_SHORT) {
+    // the derivative 1 - tanh^2 = 4 w (1 - w) with w = 1 / (1 + e^2z)
     const float w = __builtin_amdgcn_rcpf(1.f + fast_exp2(x * r.cap_in));
     y = fmaf(-2.f * r.cap_out, w, r.cap_out);
     if (GRAD) bent = 4.f * w * (1.f - w);
@@ -322,12 +331,19 @@ __device__ __forceinline__ float bend(float x, const Rules& r, float slope2, flo
   return y;
 }
 
+// a head's distance penalty in log2 units
+template <Cap CAP, bool BIAS>
+__device__ __forceinline__ float head_slope(const RuleArgs& ra, int head) {
+  if (!BIAS || (CAP == CAP_EXACT && ra.slopes == nullptr)) return 0.f;
+  return ra.slopes[head] * LOG2E;
+}
+
 // ---- forward --------------------------------------------------------------------------------------------
 
-template <typename T, int D, bool CAP, bool BIAS>
+template <typename T, int D, Cap CAP, bool BIAS>
 __global__ __launch_bounds__(THREADS, 2) void attend_fwd_mfma(FastArgs g, RuleArgs ra) {
   constexpr int TE = TILE * tile_stride<D>();
-  constexpr bool RAW = !CAP && !BIAS;
+  constexpr bool RAW = CAP == CAP_NONE && !BIAS;
   constexpr float UP = shift_of<T>(7.f);
   __shared__ __attribute__((aligned(16))) u16 tiles[4 * TE];
   __shared__ __attribute__((aligned(16))) int kdocs[2][TILE];
@@ -345,7 +361,7 @@ __global__ __launch_bounds__(THREADS, 2) void attend_fwd_mfma(FastArgs g, RuleAr
   const int p = r.off + row;
   const bool there = row < r.t_q;
   const int doc = there ? query_doc(r, p) : -1;
-  const float slope2 = BIAS ? ra.slopes[head] * LOG2E : 0.f;
+  const float slope2 = head_slope<CAP, BIAS>(ra, head);
   const HeadRows qrows(g.q + bh * (int64_t)r.t_q * g.hd, r.t_q, g.hd);
   const int64_t kv = (b * g.kv_heads + kvh) * (int64_t)r.t_k * g.hd;
   const HeadRows krows(g.k + kv, r.len, g.hd), vrows(g.v + kv, r.len, g.hd);  // keys past the live ones read as zeros
@@ -403,6 +419,7 @@ __global__ __launch_bounds__(THREADS, 2) void attend_fwd_mfma(FastArgs g, RuleAr
 #pragma unroll
       for (int ds = 0; ds < D / 16; ds++) s = T::mfma32(kfr[ds], qf[ds], s);
       const float near = (float)(p - s0 - 4 * h);
+      if (CAP == CAP_EXACT) cap_scores<16>(s, r);
       if (!RAW) {
 #pragma unroll
         for (int i = 0; i < 16; i++) {
@@ -480,10 +497,10 @@ __global__ __launch_bounds__(THREADS, 2) void attend_fwd_mfma(FastArgs g, RuleAr
 
 // ---- dQ pass: also delta = rowsum(dout * out), which the dK/dV pass reads ---------------------------------
 
-template <typename T, int D, bool CAP, bool BIAS>
+template <typename T, int D, Cap CAP, bool BIAS>
 __global__ __launch_bounds__(THREADS, 2) void attend_dq_mfma(FastArgs g, RuleArgs ra) {
   constexpr int TE = TILE * tile_stride<D>();
-  constexpr bool RAW = !CAP && !BIAS;
+  constexpr bool RAW = CAP == CAP_NONE && !BIAS;
   __shared__ __attribute__((aligned(16))) u16 tiles[4 * TE];
   __shared__ __attribute__((aligned(16))) int kdocs[2][TILE];
   __shared__ uint64_t bits[ATT_WORDS];
@@ -500,7 +517,7 @@ __global__ __launch_bounds__(THREADS, 2) void attend_dq_mfma(FastArgs g, RuleArg
   const int p = r.off + row;
   const bool there = row < r.t_q;
   const int doc = there ? query_doc(r, p) : -1;
-  const float slope2 = BIAS ? ra.slopes[head] * LOG2E : 0.f;
+  const float slope2 = head_slope<CAP, BIAS>(ra, head);
   const int64_t rows0 = bh * (int64_t)r.t_q;
   const HeadRows qrows(g.q + rows0 * g.hd, r.t_q, g.hd), grows(g.dout + rows0 * g.hd, r.t_q, g.hd), orows(g.out + rows0 * g.hd, r.t_q, g.hd);
   const int64_t kv = (b * g.kv_heads + kvh) * (int64_t)r.t_k * g.hd;
@@ -567,12 +584,13 @@ __global__ __launch_bounds__(THREADS, 2) void attend_dq_mfma(FastArgs g, RuleArg
         dp = T::mfma32(read_row<D>(Vt, sub * 32 + n, 2 * ds + h), of[ds], dp);
       }
       const float near = (float)(p - s0 - 4 * h);
+      if (CAP == CAP_EXACT) cap_scores<16>(s, r);
 #pragma unroll
       for (int i = 0; i < 16; i++) {
         float bent = 1.f;
         const float y = bend<CAP, BIAS, true>(s[i], r, slope2, near - (float)(8 * (i >> 2) + (i & 3)), bent);
         const float e = fast_exp2(RAW ? fmaf(y, r.c2, -l2) : y - l2);
-        s[i] = e * (dp[i] - delta) * (CAP ? bent : 1.f);  // times scale once, at the store
+        s[i] = e * (dp[i] - delta) * (CAP != CAP_NONE ? bent : 1.f);  // times scale once, at the store
       }
       const bool edge = s0 + 32 > r.len || (r.causal && s0 + 31 > r.off + wq0 && s0 + 31 >= r.pre);
       const bool alone = (alike >> sub) & 1;
@@ -617,10 +635,10 @@ __global__ __launch_bounds__(THREADS, 2) void attend_dq_mfma(FastArgs g, RuleArg
 
 // ---- dK/dV pass up to 64 dims -----------------------------------------------------------------------------
 
-template <typename T, int D, bool CAP, bool BIAS>
+template <typename T, int D, Cap CAP, bool BIAS>
 __global__ __launch_bounds__(THREADS, 2) void attend_dkv_mfma(FastArgs g, RuleArgs ra) {
   constexpr int TE = TILE * tile_stride<D>();
-  constexpr bool RAW = !CAP && !BIAS;
+  constexpr bool RAW = CAP == CAP_NONE && !BIAS;
   constexpr float UP = shift_of<T>(14.f), DOWN = std::is_same<T, F16>::value ? 1.f / 16384.f : 1.f;
   constexpr float DS = DOWN / ds_down<T>();  // turns p 2^14 (dp - delta) into dS 2^8
   __shared__ __attribute__((aligned(16))) u16 tiles[4 * TE];
@@ -712,7 +730,7 @@ __global__ __launch_bounds__(THREADS, 2) void attend_dkv_mfma(FastArgs g, RuleAr
   __syncthreads();
   for (int buf = 0; any && gh < part.g1; buf ^= 1) {
     const int r0 = cur * TILE;
-    const float slope2 = BIAS ? ra.slopes[kvh * group + gh] * LOG2E : 0.f;
+    const float slope2 = head_slope<CAP, BIAS>(ra, kvh * group + gh);
     const u16* Qt = tiles + 2 * buf * TE;
     const u16* Gt = Qt + TE;
 #pragma unroll
@@ -737,13 +755,14 @@ __global__ __launch_bounds__(THREADS, 2) void attend_dkv_mfma(FastArgs g, RuleAr
         d4[q] = *(const f32x4*)&Ds[buf][sub * 32 + 8 * q + 4 * h];
       }
       const float near = (float)(r.off + s0 + 4 * h - key);
+      if (CAP == CAP_EXACT) cap_scores<16>(s, r);
 #pragma unroll
       for (int i = 0; i < 16; i++) {
         float bent = 1.f;
         const float y = bend<CAP, BIAS, true>(s[i], r, slope2, near + (float)(8 * (i >> 2) + (i & 3)), bent);
         const float l2 = l4[i >> 2][i & 3];
         s[i] = fast_exp2(RAW ? fmaf(y, r.c2, -l2) : y - l2);
-        dp[i] = s[i] * fmaf(dp[i], DS, -d4[i >> 2][i & 3]) * (CAP ? bent : 1.f);  // times scale once, at the store
+        dp[i] = s[i] * fmaf(dp[i], DS, -d4[i >> 2][i & 3]) * (CAP != CAP_NONE ? bent : 1.f);  // times scale once, at the store
       }
       const bool edge = s0 + 32 > r.t_q || wk0 + 32 > r.len || (r.causal && r.off + s0 < wk0 + 31 && wk0 + 31 >= r.pre);
       const bool alone = (alike >> sub) & 1;
@@ -825,10 +844,10 @@ struct HeadDma8 {
 
 constexpr int HAND_STORES = 2;  // vector stores of dS a wave and tile, see below
 
-template <typename T, int D, bool CAP, bool BIAS, bool HAND>
+template <typename T, int D, Cap CAP, bool BIAS, bool HAND>
 __global__ __launch_bounds__(64 * KV_WAVES, 1) void attend_dkv_wide(FastArgs g, RuleArgs ra) {
 #if defined(__HIP_DEVICE_COMPILE__)  // the host pass needs the stub alone
-  constexpr bool RAW = !CAP && !BIAS;
+  constexpr bool RAW = CAP == CAP_NONE && !BIAS;
   constexpr int KS = D / 16, DT = D / 32;
   constexpr float UP = shift_of<T>(14.f), DOWN = std::is_same<T, F16>::value ? 1.f / 16384.f : 1.f;
   constexpr float DS = DOWN / ds_down<T>();  // turns p 2^14 (dp - delta) into dS 2^8
@@ -936,7 +955,7 @@ __global__ __launch_bounds__(64 * KV_WAVES, 1) void attend_dkv_wide(FastArgs g, 
   // this wave's 32 queries of the tile against its 32 keys
   auto tile = [&](int buf, const u16* Qc, const u16* Oc) __attribute__((always_inline)) {
     const int s0 = cur * TILE + hq * 32;
-    const float slope2 = BIAS ? ra.slopes[kvh * group + gh] * LOG2E : 0.f;
+    const float slope2 = head_slope<CAP, BIAS>(ra, kvh * group + gh);
     int rk = rk0;
     asm volatile("" : "+v"(rk)::"memory");  // keeps the K and V reads and their offsets in the loop: hoisted, they would fill the registers
     f32x16 s = zero16(), dp = zero16();
@@ -956,6 +975,7 @@ __global__ __launch_bounds__(64 * KV_WAVES, 1) void attend_dkv_wide(FastArgs g, 
     bool edge = s0 + 32 > r.t_q || wk0 + 32 > r.len || (r.causal && r.off + s0 < wk0 + 31 && wk0 + 31 >= r.pre);
     edge |= ((alike >> hq) & 1) == 0;
     const float near = (float)(r.off + s0 + 4 * h - key);
+    if (CAP == CAP_EXACT) cap_scores<16>(s, r);
     // the scores straight into packed operands, in two instances: with element tests and without
     unsigned pk[8], gp[8];
     auto soft = [&](auto tests) __attribute__((always_inline)) {
@@ -972,7 +992,7 @@ __global__ __launch_bounds__(64 * KV_WAVES, 1) void attend_dkv_wide(FastArgs g, 
         float bent = 1.f;
         const float y = bend<CAP, BIAS, true>(s[i], r, slope2, near + (float)(8 * (i >> 2) + (i & 3)), bent);
         float e = fast_exp2(RAW ? fmaf(y, r.c2, -l4[i & 3]) : y - l4[i & 3]);
-        float d = e * fmaf(dp[i], DS, -d4[i & 3]) * (CAP ? bent : 1.f);  // times scale once, at the store
+        float d = e * fmaf(dp[i], DS, -d4[i & 3]) * (CAP != CAP_NONE ? bent : 1.f);  // times scale once, at the store
         if (decltype(tests)::value) {
           const int qq = s0 + 8 * (i >> 2) + 4 * h + (i & 3), qd = (i & 3) == 0 ? q4.x : (i & 3) == 1 ? q4.y : (i & 3) == 2 ? q4.z : q4.w;
           const bool see = (qq < r.t_q) & (doc >= 0) & (qd == doc) & sees(r, r.off + qq, key);
@@ -1175,10 +1195,10 @@ __device__ __forceinline__ bool half_edge(const Rules& r, const QueryBlock& qb, 
   return alike == 0 || s0 + 32 > r.len || (r.causal && s0 + 31 > r.off + qb.wq0 && s0 + 31 >= r.pre);
 }
 
-template <typename T, int D, bool CAP, bool BIAS>
+template <typename T, int D, Cap CAP, bool BIAS>
 __global__ __launch_bounds__(THREADS, 2) void attend_fwd_wide(FastArgs g, RuleArgs ra) {
 #if defined(__HIP_DEVICE_COMPILE__)  // the host pass needs the stub alone
-  constexpr bool RAW = !CAP && !BIAS;
+  constexpr bool RAW = CAP == CAP_NONE && !BIAS;
   constexpr int KS = D / 16, DT = D / 32;
   constexpr float UP = shift_of<T>(7.f);
   __shared__ __attribute__((aligned(1024))) u16 K0[TILE * 128];
@@ -1202,7 +1222,7 @@ __global__ __launch_bounds__(THREADS, 2) void attend_fwd_wide(FastArgs g, RuleAr
   qb.doc = there ? query_doc(r, qb.p) : -1;
   const int4* ranges = g.ranges ? g.ranges + qb.b * g.granules : nullptr;
   const bool docs = ranges != nullptr;
-  const float slope2 = BIAS ? ra.slopes[qb.head] * LOG2E : 0.f;
+  const float slope2 = head_slope<CAP, BIAS>(ra, qb.head);
   const int64_t kv = (qb.b * g.kv_heads + qb.kvh) * (int64_t)r.t_k * g.hd;
   const u16* kbase = g.k + kv;
   const u16* vbase = g.v + kv;
@@ -1240,6 +1260,7 @@ __global__ __launch_bounds__(THREADS, 2) void attend_fwd_wide(FastArgs g, RuleAr
 #pragma unroll
     for (int sub = 0; sub < 2; sub++) {
       const int s0 = t * TILE + sub * 32;
+      if (CAP == CAP_EXACT) cap_scores<16>(o[sub], r);
       if (!RAW) {
 #pragma unroll
         for (int i = 0; i < 16; i++) {
@@ -1356,10 +1377,10 @@ __global__ __launch_bounds__(THREADS, 2) void attend_fwd_wide(FastArgs g, RuleAr
 #endif
 }
 
-template <typename T, int D, bool CAP, bool BIAS>
+template <typename T, int D, Cap CAP, bool BIAS>
 __global__ __launch_bounds__(THREADS, 2) void attend_dq_wide(FastArgs g, RuleArgs ra) {
 #if defined(__HIP_DEVICE_COMPILE__)  // the host pass needs the stub alone
-  constexpr bool RAW = !CAP && !BIAS;
+  constexpr bool RAW = CAP == CAP_NONE && !BIAS;
   constexpr int KS = D / 16, DT = D / 32;
   __shared__ __attribute__((aligned(1024))) u16 K0[TILE * 128];
   __shared__ __attribute__((aligned(1024))) u16 K1[TILE * 128];
@@ -1393,7 +1414,7 @@ __global__ __launch_bounds__(THREADS, 2) void attend_dq_wide(FastArgs g, RuleArg
   qb.doc = there ? query_doc(r, qb.p) : -1;
   const int4* ranges = g.ranges ? g.ranges + qb.b * g.granules : nullptr;
   const bool docs = ranges != nullptr;
-  const float slope2 = BIAS ? ra.slopes[qb.head] * LOG2E : 0.f;
+  const float slope2 = head_slope<CAP, BIAS>(ra, qb.head);
   const int64_t kv = (qb.b * g.kv_heads + qb.kvh) * (int64_t)r.t_k * g.hd;
   const u16* kbase = g.k + kv;
   const u16* vbase = g.v + kv;
@@ -1427,6 +1448,7 @@ __global__ __launch_bounds__(THREADS, 2) void attend_dq_wide(FastArgs g, RuleArg
         dp = T::mfma32(ad.rows(Vt, sub, ds), of[ds], dp);
       }
       const float near = (float)(qb.p - s0 - 4 * h);
+      if (CAP == CAP_EXACT) cap_scores<16>(s, r);
       unsigned gp[8];  // packed operands, in two instances: with element tests and without
       auto soft = [&](auto tests) __attribute__((always_inline)) {
         int4 d4 = {0, 0, 0, 0};
@@ -1437,7 +1459,7 @@ __global__ __launch_bounds__(THREADS, 2) void attend_dq_wide(FastArgs g, RuleArg
           float bent = 1.f;
           const float y = bend<CAP, BIAS, true>(s[i], r, slope2, near - (float)(8 * (i >> 2) + (i & 3)), bent);
           const float e = fast_exp2(RAW ? fmaf(y, r.c2, -l2) : y - l2);
-          float d = e * (dp[i] - delta) * (CAP ? bent : 1.f);  // times scale once, at the store
+          float d = e * (dp[i] - delta) * (CAP != CAP_NONE ? bent : 1.f);  // times scale once, at the store
           if (decltype(tests)::value) {
             const int kd = (i & 3) == 0 ? d4.x : (i & 3) == 1 ? d4.y : (i & 3) == 2 ? d4.z : d4.w;
             d = (qb.doc >= 0) & (kd == qb.doc) & sees(r, qb.p, s0 + 8 * (i >> 2) + 4 * h + (i & 3)) ? d : 0.f;
@@ -1627,7 +1649,7 @@ __global__ __launch_bounds__(THREADS, 2) void attend_dq_handed(FastArgs g, RuleA
 
 enum AttendPass { ATTEND_PASS_FWD, ATTEND_PASS_DQ, ATTEND_PASS_DKV };
 
-template <AttendPass PASS, typename T, int D, bool CAP, bool BIAS>
+template <AttendPass PASS, typename T, int D, Cap CAP, bool BIAS>
 int launch_fast_as(const FastArgs& g, const RuleArgs& ra, hipStream_t stream) {
   const int64_t blocks = PASS == ATTEND_PASS_DKV ? att_grid(g.batch * g.kv_heads, (ra.t_k + ATT_ROWS - 1) / ATT_ROWS, g.head_group)
                                                  : att_grid(g.batch * g.heads, (ra.t_q + ATT_ROWS - 1) / ATT_ROWS, g.head_group);
@@ -1658,9 +1680,10 @@ int launch_fast_as(const FastArgs& g, const RuleArgs& ra, hipStream_t stream) {
 
 template <AttendPass PASS, typename T, int D>
 int launch_fast_rules(const FastArgs& g, const RuleArgs& ra, hipStream_t stream) {
-  const bool cap = ra.softcap > 0.f, bias = ra.slopes != nullptr;
-  if (cap) return bias ? launch_fast_as<PASS, T, D, true, true>(g, ra, stream) : launch_fast_as<PASS, T, D, true, false>(g, ra, stream);
-  return bias ? launch_fast_as<PASS, T, D, false, true>(g, ra, stream) : launch_fast_as<PASS, T, D, false, false>(g, ra, stream);
+  const bool bias = ra.slopes != nullptr;
+  if (ra.softcap > CAP_SHORT_MOST) return launch_fast_as<PASS, T, D, CAP_EXACT, true>(g, ra, stream);  // slopes of 0 without any
+  if (ra.softcap > 0.f) return bias ? launch_fast_as<PASS, T, D, CAP_SHORT, true>(g, ra, stream) : launch_fast_as<PASS, T, D, CAP_SHORT, false>(g, ra, stream);
+  return bias ? launch_fast_as<PASS, T, D, CAP_NONE, true>(g, ra, stream) : launch_fast_as<PASS, T, D, CAP_NONE, false>(g, ra, stream);
 }
 
 }  // namespace

@@ -181,11 +181,11 @@ struct PartWalk {
 
 // ---- forward ----------------------------------------------------------------------------------------------
 
-template <int D, bool CAP, bool BIAS>
+template <int D, Cap CAP, bool BIAS>
 __global__ __launch_bounds__(THREADS, D <= 64 ? 2 : 1) void attend_fwd_parts(FastArgs g, RuleArgs ra) {
   using P = PartTile<D>;
   constexpr int R = P::ROWS;
-  constexpr bool RAW = !CAP && !BIAS;
+  constexpr bool RAW = CAP == CAP_NONE && !BIAS;
   __shared__ __attribute__((aligned(16))) u16 tiles[6 * P::MATRIX];
   __shared__ __attribute__((aligned(16))) int kdocs[R];
   __shared__ uint64_t bits[ATT_WORDS];
@@ -199,7 +199,7 @@ __global__ __launch_bounds__(THREADS, D <= 64 ? 2 : 1) void attend_fwd_parts(Fas
   const bool there = qb.row < r.t_q;
   qb.p = p;
   qb.doc = there ? query_doc(r, p) : -1;
-  const float slope2 = BIAS ? ra.slopes[qb.head] * LOG2E : 0.f;
+  const float slope2 = head_slope<CAP, BIAS>(ra, qb.head);
   const FloatRows qrows(g.q, qb.bh * r.t_q, r.t_q, g.hd);
   const int64_t kv = (qb.b * g.kv_heads + qb.kvh) * (int64_t)r.t_k;
   const FloatRows krows(g.k, kv, r.len, g.hd), vrows(g.v, kv, r.len, g.hd);  // keys past the live ones read as zeros
@@ -237,6 +237,7 @@ __global__ __launch_bounds__(THREADS, D <= 64 ? 2 : 1) void attend_fwd_parts(Fas
       const int s0 = k0 + sub * 32;
       f32x16 s = scores<D>(tiles, sub * 32 + n, qf, h);
       const float near = (float)(p - s0 - 4 * h);
+      if (CAP == CAP_EXACT) cap_scores<16>(s, r);
       if (!RAW) {
 #pragma unroll
         for (int i = 0; i < 16; i++) {
@@ -289,11 +290,11 @@ __global__ __launch_bounds__(THREADS, D <= 64 ? 2 : 1) void attend_fwd_parts(Fas
 
 // ---- dQ pass: also delta = rowsum(dout * out) ---------------------------------------------------------------
 
-template <int D, bool CAP, bool BIAS>
+template <int D, Cap CAP, bool BIAS>
 __global__ __launch_bounds__(THREADS, 1) void attend_dq_parts(FastArgs g, RuleArgs ra) {
   using P = PartTile<D>;
   constexpr int R = P::ROWS;
-  constexpr bool RAW = !CAP && !BIAS;
+  constexpr bool RAW = CAP == CAP_NONE && !BIAS;
   __shared__ __attribute__((aligned(16))) u16 tiles[6 * P::MATRIX];
   __shared__ __attribute__((aligned(16))) int kdocs[R];
   __shared__ uint64_t bits[ATT_WORDS];
@@ -307,7 +308,7 @@ __global__ __launch_bounds__(THREADS, 1) void attend_dq_parts(FastArgs g, RuleAr
   const bool there = qb.row < r.t_q;
   qb.p = p;
   qb.doc = there ? query_doc(r, p) : -1;
-  const float slope2 = BIAS ? ra.slopes[qb.head] * LOG2E : 0.f;
+  const float slope2 = head_slope<CAP, BIAS>(ra, qb.head);
   const int64_t rows0 = qb.bh * r.t_q, kv = (qb.b * g.kv_heads + qb.kvh) * (int64_t)r.t_k;
   const FloatRows qrows(g.q, rows0, r.t_q, g.hd), grows(g.dout, rows0, r.t_q, g.hd), orows(g.out, rows0, r.t_q, g.hd);
   const FloatRows krows(g.k, kv, r.len, g.hd), vrows(g.v, kv, r.len, g.hd);
@@ -356,12 +357,13 @@ __global__ __launch_bounds__(THREADS, 1) void attend_dq_parts(FastArgs g, RuleAr
       f32x16 s = scores<D>(tiles, sub * 32 + n, qf, h);
       const f32x16 dp = scores<D>(tiles + 3 * P::MATRIX, sub * 32 + n, of, h);
       const float near = (float)(p - s0 - 4 * h);
+      if (CAP == CAP_EXACT) cap_scores<16>(s, r);
 #pragma unroll
       for (int i = 0; i < 16; i++) {
         float bent = 1.f;
         const float y = bend<CAP, BIAS, true>(s[i], r, slope2, near - (float)(8 * (i >> 2) + (i & 3)), bent);
         const float e = fast_exp2(RAW ? fmaf(y, r.c2, -l2) : y - l2);
-        s[i] = e * (dp[i] - delta) * (CAP ? bent : 1.f);  // times scale once, at the store
+        s[i] = e * (dp[i] - delta) * (CAP != CAP_NONE ? bent : 1.f);  // times scale once, at the store
       }
       if (half_edge(r, qb, (alike >> sub) & 1, s0)) {
         if (ranges != nullptr) {
@@ -386,11 +388,11 @@ __global__ __launch_bounds__(THREADS, 1) void attend_dq_parts(FastArgs g, RuleAr
 
 // ---- dK/dV pass -------------------------------------------------------------------------------------------
 
-template <int D, bool CAP, bool BIAS>
+template <int D, Cap CAP, bool BIAS>
 __global__ __launch_bounds__(THREADS, 1) void attend_dkv_parts(FastArgs g, RuleArgs ra) {
   using P = PartTile<D>;
   constexpr int R = P::ROWS;
-  constexpr bool RAW = !CAP && !BIAS;
+  constexpr bool RAW = CAP == CAP_NONE && !BIAS;
   __shared__ __attribute__((aligned(16))) u16 tiles[6 * P::MATRIX];
   __shared__ __attribute__((aligned(16))) float Ls[R];
   __shared__ __attribute__((aligned(16))) float Ds[R];
@@ -450,7 +452,7 @@ __global__ __launch_bounds__(THREADS, 1) void attend_dkv_parts(FastArgs g, RuleA
   if (gh < part.g1) load(gh, walk.row());
   while (gh < part.g1) {
     const int r0 = walk.row(), alike = walk.alike();
-    const float slope2 = BIAS ? ra.slopes[kvh * group + gh] * LOG2E : 0.f;
+    const float slope2 = head_slope<CAP, BIAS>(ra, kvh * group + gh);
     __syncthreads();
     st.store(tiles);
     if (threadIdx.x < R) {
@@ -471,6 +473,7 @@ __global__ __launch_bounds__(THREADS, 1) void attend_dkv_parts(FastArgs g, RuleA
       f32x16 s = scores<D>(tiles, sub * 32 + n, kf, h);
       f32x16 dp = scores<D>(tiles + 3 * P::MATRIX, sub * 32 + n, vf, h);
       const float near = (float)(r.off + s0 + 4 * h - key);
+      if (CAP == CAP_EXACT) cap_scores<16>(s, r);
 #pragma unroll
       for (int q = 0; q < 4; q++) {
         const f32x4 l4 = *(const f32x4*)&Ls[sub * 32 + 8 * q + 4 * h], d4 = *(const f32x4*)&Ds[sub * 32 + 8 * q + 4 * h];
@@ -480,7 +483,7 @@ __global__ __launch_bounds__(THREADS, 1) void attend_dkv_parts(FastArgs g, RuleA
           float bent = 1.f;
           const float y = bend<CAP, BIAS, true>(s[i], r, slope2, near + (float)(8 * q + e), bent);
           s[i] = fast_exp2(RAW ? fmaf(y, r.c2, -l4[e]) : y - l4[e]);
-          dp[i] = s[i] * (dp[i] - d4[e]) * (CAP ? bent : 1.f);  // times scale once, at the store
+          dp[i] = s[i] * (dp[i] - d4[e]) * (CAP != CAP_NONE ? bent : 1.f);  // times scale once, at the store
         }
       }
       bool edge = s0 + 32 > r.t_q || wk0 + 32 > r.len || (r.causal && r.off + s0 < wk0 + 31 && wk0 + 31 >= r.pre);
@@ -511,7 +514,7 @@ __global__ __launch_bounds__(THREADS, 1) void attend_dkv_parts(FastArgs g, RuleA
 
 // ---- launches -----------------------------------------------------------------------------------------------
 
-template <AttendPass PASS, int D, bool CAP, bool BIAS>
+template <AttendPass PASS, int D, Cap CAP, bool BIAS>
 int launch_parts_as(const FastArgs& g, const RuleArgs& ra, hipStream_t stream) {
   const int64_t blocks = PASS == ATTEND_PASS_DKV ? att_grid(g.batch * g.kv_heads, (ra.t_k + ATT_ROWS - 1) / ATT_ROWS, g.head_group)
                                                  : att_grid(g.batch * g.heads, (ra.t_q + ATT_ROWS - 1) / ATT_ROWS, g.head_group);
@@ -529,8 +532,8 @@ int launch_parts_as(const FastArgs& g, const RuleArgs& ra, hipStream_t stream) {
 template <AttendPass PASS, int D>
 int launch_parts_rules(const FastArgs& g, const RuleArgs& ra, hipStream_t stream) {
   const bool cap = ra.softcap > 0.f, bias = ra.slopes != nullptr;
-  if (cap) return bias ? launch_parts_as<PASS, D, true, true>(g, ra, stream) : launch_parts_as<PASS, D, true, false>(g, ra, stream);
-  return bias ? launch_parts_as<PASS, D, false, true>(g, ra, stream) : launch_parts_as<PASS, D, false, false>(g, ra, stream);
+  if (cap) return bias ? launch_parts_as<PASS, D, CAP_EXACT, true>(g, ra, stream) : launch_parts_as<PASS, D, CAP_EXACT, false>(g, ra, stream);
+  return bias ? launch_parts_as<PASS, D, CAP_NONE, true>(g, ra, stream) : launch_parts_as<PASS, D, CAP_NONE, false>(g, ra, stream);
 }
 
 template <AttendPass PASS>

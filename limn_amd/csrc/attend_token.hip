@@ -183,14 +183,17 @@ __global__ __launch_bounds__(64 * waves, waves == 4 ? 2 : 1) void attend_token(T
     for (int t = 0; t < NR; t++) {
       float y[8], mx = -__builtin_inff();
 #pragma unroll
+      for (int j = 0; j < 8; j++) y[j] = s[t][j >> 2][j & 3];
+      if (r.cap_out > 0.f) {
+        cap_scores<8>(y, r);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; j++) y[j] *= r.c2;
+      }
+#pragma unroll
       for (int j = 0; j < 8; j++) {
         const int key = k0 + 16 * (j >> 2) + 4 * g + (j & 3);
-        float x = s[t][j >> 2][j & 3];
-        if (r.cap_out > 0.f)
-          x = fmaf(-2.f * r.cap_out, __builtin_amdgcn_rcpf(1.f + fast_exp2(x * r.cap_in)), r.cap_out);  // as bend in attend_mfma.h
-        else
-          x *= r.c2;
-        x = fmaf(-slope2[t], fabsf((float)(p[t] - key)), x);
+        float x = fmaf(-slope2[t], fabsf((float)(p[t] - key)), y[j]);
         if (edge) x = sees(r, p[t], key) ? x : -__builtin_inff();
         y[j] = x;
         mx = fmaxf(mx, x);

@@ -7,7 +7,11 @@ hidden pairs left out of every sum (a hidden row's infinities and NaN are never 
 The bounds are first-order bounds on the kernels' roundings, with u the half
 step of the storage type (torch.finfo(t).eps / 2) and f that of float32, 2^-24:
   - a score is a float32 sum of hd products: off by at most e = (hd + 8) f scale sum|q||k|, plus f times the
-    distance term, plus 4 f times the cap (whose tanh is off by at most 4 f absolutely) and 4 f |s|;
+    distance term, plus 4 f |s|, and where it is capped 16 f |cap tanh(x / cap)| more: near 0 a polynomial of relative
+    error 2^-25.9 and two products (with their constants, 7 f); past |x / cap| = 1/2, where tanh is .46, 1 - 2 w with
+    w = 1 / (1 + e) off by 3.5 f absolutely (an exponential and a reciprocal of 2 f each, w <= .27), the exponent's two
+    constants and products by 4 f relatively (times 2z / sinh 2z <= .85), the product with the cap by 3 f. Half
+    widths under caps up to 64 take the latter alone, w up to 1: 8 f of the cap;
   - a probability is then off by a factor of at most 1 + 2 max_j e + 8 f (its own and the sum's scores, one
     exponential, the sum), and by u more where it is rounded to be an operand (half widths);
   - a sum of n terms in float32 adds (n + 8) f times the sum of its terms' magnitudes;
@@ -84,7 +88,7 @@ def attend(q, k, v, *, causal=False, softcap=0.0, slopes=None, documents=None, p
                 if softcap:
                     t = np.tanh(x / softcap)
                     s, bent = softcap * t, 1 - t * t
-                    e = e + 8 * F * softcap
+                    e = e + (8 * F * softcap if dtype != "float32" and softcap <= 64 else 16 * F * np.abs(s))
                 if slopes is not None:
                     s = s - slopes[h] * far
                     e = e + 4 * F * slopes[h] * far + 4 * F * np.abs(s)

@@ -1,0 +1,56 @@
+"""Caps far above the scores they are for, and scores about a cap, in the form composed from limn's primitives."""
+
+from __future__ import annotations
+
+import numpy as np
+import pytest
+
+from limn_amd.attend import attend
+from limn_amd.seam import Tensor, float32, float64, grad, set_device
+from oracle.attend import attend as definition
+from oracle.attend import within
+
+
+@pytest.fixture(autouse=True)
+def _numpy():
+    set_device("numpy")
+
+
+def drawn(spread, seed=0):
+    rng = np.random.default_rng(seed)
+    q, k, v, do = (rng.standard_normal(s).astype(np.float32) for s in ((1, 2, 9, 16), (1, 1, 9, 16), (1, 1, 9, 8), (1, 2, 9, 8)))
+    return q * np.float32(spread), k, v, do
+
+
+@pytest.mark.parametrize("spread", [0.01, 1.0, 4.0])
+@pytest.mark.parametrize("softcap", [1.0, 50.0, 1e3, 1e5, 1e8, 1e30])
+def test_a_cap_is_as_exact_as_the_scores_under_it(softcap, spread):
+    """float32: a score is off by a part of itself, not of the cap, so out and the gradients are what an uncapped call's are."""
+    q, k, v, do = drawn(spread)
+    tq, tk, tv = (Tensor(x, dtype=float32, requires_grad=True) for x in (q, k, v))
+    out = attend(tq, tk, tv, causal=True, softcap=softcap)
+    got = [out, *grad((out * Tensor(do, dtype=float32)).sum(), [tq, tk, tv])]
+    want = definition(q, k, v, dout=do, causal=True, softcap=softcap, dtype="float32")
+    for name, t in zip(("out", "dq", "dk", "dv"), got):
+        within(t.numpy(), *want[name], name)
+
+
+@pytest.mark.parametrize("softcap", [0.5, 1.0, 4.0, 1e6])
+def test_scores_on_both_sides_of_half_the_cap_in_float64(softcap):
+    q, k, v, do = (x.astype(np.float64) for x in drawn(2.0, seed=1))
+    q[0, 0, 3] = 0.0
+    tq, tk, tv = (Tensor(x, dtype=float64, requires_grad=True) for x in (q, k, v))
+    out = attend(tq, tk, tv, softcap=softcap)
+    got = [out, *grad((out * Tensor(do, dtype=float64)).sum(), [tq, tk, tv])]
+    want = definition(q, k, v, dout=do, softcap=softcap)
+    for name, t in zip(("out", "dq", "dk", "dv"), got):
+        within(t.numpy(), want[name][0], 1e-12, name)
+
+
+def test_an_infinite_score_is_the_cap():
+    q, k, v, _ = drawn(1.0, seed=2)
+    q[0, 0, 0, 0] = np.inf  # every score of this row is an infinity of its key's sign
+    out = attend(*(Tensor(x, dtype=float32) for x in (q, k, v)), softcap=5.0)
+    p = np.exp(np.where(k[0, 0, :, 0] > 0, 5.0, -5.0) - 5.0)
+    row, want = out.numpy()[0, 0, 0], p @ v[0, 0] / p.sum()
+    within(row, want, 64 * 2.0**-24 * (p @ np.abs(v[0, 0])) / p.sum())  # an exponential, two sums of 9, a quotient: under 64 half steps
