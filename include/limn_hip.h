@@ -212,7 +212,7 @@ int limn_hip_contract_pays(int dtype, int64_t batch, int64_t M, int64_t N, int64
  *   heads, t_q, hd_v) of float32, float16 or bfloat16, lse (batch, heads, t_q) float32; slopes (heads)
  *   float32, documents (batch, t_k), prefix (batch) and lengths (batch) int32, each NULL for none. A length
  *   outside [0, t_k] is taken as the nearest end. t_q <= t_k where the call is causal or has documents or
- *   lengths. hd and hd_v at most 256.
+ *   lengths. hd and hd_v at most 256. scale between -2^120 and 2^120; softcap 0 for none, else from 2^-120 to 2^120.
  * `workspace` must hold limn_hip_attend_workspace(...) bytes, 16-byte aligned, for this call alone: calls
  * that may overlap, and captured graphs that may run at once, need one each. A backward's holds up to 2.5 GiB of
  * score gradients between its passes. Every result is deterministic. Sums and statistics are float32; float32

@@ -20,6 +20,7 @@ import math
 from limn_amd.seam import CUT_OPS, FLOATS, Node, Op, Tensor, accumulate_in, active_device, custom, float32, float64, grad, int32, promote
 
 ATTEND_FWD, ATTEND_BWD = "attend_fwd", "attend_bwd"
+MOST = 2.0**120  # of a scale or a cap: its float32 form, with the constants of the exponential, stays a normal number
 
 
 def attend(q: Tensor, k: Tensor, v: Tensor, *, causal: bool = False, softcap: float = 0.0, slopes: Tensor | None = None,
@@ -33,8 +34,9 @@ def attend(q: Tensor, k: Tensor, v: Tensor, *, causal: bool = False, softcap: fl
     - `lengths` (..., int32): only the first lengths keys are live, and the queries are the last of them (a
       cache with room for more);
     - `slopes` (heads,) float32: each head takes slopes[h] |p(i) - j| off its scores; it gets no gradient;
-    - `softcap`: scores capped at +-softcap by a tanh, before the distance is taken off; 0 for none;
-    - `scale`: of the scores, 1 / sqrt(hd) if not given.
+    - `softcap`: scores capped at +-softcap by a tanh, before the distance is taken off; 0 for none, else from 2^-120 to
+      2^120;
+    - `scale`: of the scores, 1 / sqrt(hd) if not given; up to 2^120 either way.
 
     A query that sees no key gives zeros and passes no gradient. The leading dims of q, k and v are equal, as
     are those of documents, prefix and lengths.
@@ -54,11 +56,11 @@ def attend(q: Tensor, k: Tensor, v: Tensor, *, causal: bool = False, softcap: fl
     if prefix is not None and not causal:
         raise ValueError("attend: a prefix opens keys that causality hides; the call is not causal")
     softcap = float(softcap)
-    if not (math.isfinite(softcap) and softcap >= 0):
-        raise ValueError(f"attend: softcap must be finite, and positive or 0 for none, got {softcap}")
+    if softcap != 0 and not 1 / MOST <= softcap <= MOST:
+        raise ValueError(f"attend: softcap must be positive, between 2^-120 and 2^120, or 0 for none, got {softcap}")
     scale = hd**-0.5 if scale is None else float(scale)
-    if not math.isfinite(scale):
-        raise ValueError(f"attend: scale must be finite, got {scale}")
+    if not abs(scale) <= MOST:
+        raise ValueError(f"attend: scale must be finite, between -2^120 and 2^120, got {scale}")
     if slopes is not None and (slopes.shape != (heads,) or slopes.dtype != float32):
         raise ValueError(f"attend: slopes must be ({heads},) float32, got {slopes.shape} {slopes.dtype}")
     for name, t, shape in (("documents", documents, lead + (t_k,)), ("prefix", prefix, lead), ("lengths", lengths, lead)):

@@ -143,13 +143,16 @@ int check_attend(const char* name, const AttendArgs& a) {
     return fail(LIMN_HIP_EINVAL, "%s: %lld query heads do not share %lld key heads evenly", name, (long long)a.heads, (long long)a.kv_heads);
   if (a.t_q > a.t_k && (a.causal || a.documents != nullptr || a.lengths != nullptr))
     return fail(LIMN_HIP_EINVAL, "%s: the queries are the last of the keys' positions: %lld queries and %lld keys", name, (long long)a.t_q, (long long)a.t_k);
-  if (!isfinite(a.scale)) return fail(LIMN_HIP_EINVAL, "%s: scale must be finite", name);
-  if (!isfinite(a.softcap) || a.softcap < 0) return fail(LIMN_HIP_EINVAL, "%s: softcap must be finite, and positive or 0 for none", name);
+  // the kernels' constants are floats: a scale or a cap past this, or a cap below its inverse, would be an infinity or a 0 there
+  const double most = 0x1p120;
+  if (!(fabs(a.scale) <= most)) return fail(LIMN_HIP_EINVAL, "%s: scale must be finite, between -2^120 and 2^120", name);
+  if (a.softcap != 0 && !(a.softcap >= 1 / most && a.softcap <= most))
+    return fail(LIMN_HIP_EINVAL, "%s: softcap must be positive, between 2^-120 and 2^120, or 0 for none", name);
   if (a.prefix != nullptr && !a.causal) return fail(LIMN_HIP_EINVAL, "%s: a prefix opens keys that causality hides; the call is not causal", name);
   if (a.hd > 256 || a.hd_v > 256) return fail(LIMN_HIP_EUNSUPPORTED, "%s: no kernel for head dims %lld and %lld (at most 256)", name, (long long)a.hd, (long long)a.hd_v);
   // positions and packed rows are 32-bit in the kernels; element offsets are 64-bit
-  const int64_t most = (int64_t)1 << 30;
-  if (a.t_k > most || a.t_q > most / a.group() || a.heads > most || a.batch > ((int64_t)1 << 40) / a.heads / (a.t_q > a.t_k ? a.t_q : a.t_k))
+  const int64_t size = (int64_t)1 << 30;
+  if (a.t_k > size || a.t_q > size / a.group() || a.heads > size || a.batch > ((int64_t)1 << 40) / a.heads / (a.t_q > a.t_k ? a.t_q : a.t_k))
     return fail(LIMN_HIP_EUNSUPPORTED, "%s: sizes out of range", name);
   return LIMN_HIP_OK;
 }
@@ -200,9 +203,9 @@ bool aligned16(const AttendArgs& a, bool backward) {
 // over 8 key heads 646 and 186, 512 of 32 (128 blocks) 646 and 637; 1024 keys, 128 of 8: 30 and 31 (64 dims 26 and 20).
 bool token_sizes(const AttendArgs& a) { return half_sizes(a) && (a.t_q < 64 || (row_blocks(a) < 128 && a.t_k >= 1024 && a.t_q <= a.t_k / 4)); }
 
-// A call of such sizes goes to them where every buffer is 16-byte aligned and the scale positive (the forward's
-// reference point is taken over unscaled scores).
-bool fast_call(const AttendArgs& a, bool backward) { return fast_sizes(a, backward) && a.scale > 0 && aligned16(a, backward); }
+// A call of such sizes goes to them where every buffer is 16-byte aligned and the scale positive: the forward's
+// reference point is taken over unscaled scores, and moves when one passes it by 8 / (scale log2 e), which must be a number.
+bool fast_call(const AttendArgs& a, bool backward) { return fast_sizes(a, backward) && a.scale >= 0x1p-100 && aligned16(a, backward); }
 
 // Parts of the queries that a call with fewer key blocks than fill the GPU (two workgroups a CU up to 64 half-width
 // dims, one else) cuts its dK/dV pass into, the heads of a group first: at least 4 tiles each. The backward of 16 heads

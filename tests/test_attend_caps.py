@@ -2,10 +2,13 @@
 
 from __future__ import annotations
 
+import ctypes
+
 import numpy as np
 import pytest
 
 from limn_amd.attend import attend
+from limn_amd.hip import runtime
 from limn_amd.seam import Tensor, float32, float64, grad, set_device
 from oracle.attend import attend as definition
 from oracle.attend import within
@@ -54,3 +57,28 @@ def test_an_infinite_score_is_the_cap():
     p = np.exp(np.where(k[0, 0, :, 0] > 0, 5.0, -5.0) - 5.0)
     row, want = out.numpy()[0, 0, 0], p @ v[0, 0] / p.sum()
     within(row, want, 64 * 2.0**-24 * (p @ np.abs(v[0, 0])) / p.sum())  # an exponential, two sums of 9, a quotient: under 64 half steps
+
+
+@pytest.mark.parametrize("kw,message", [
+    (dict(softcap=1e39), "softcap"), (dict(softcap=1e-39), "softcap"), (dict(softcap=float("inf")), "softcap"), (dict(softcap=-1e-3), "softcap"),
+    (dict(scale=1e39), "scale"), (dict(scale=-1e39), "scale"), (dict(scale=float("nan")), "scale")])
+def test_numbers_that_float32_does_not_hold_are_refused(kw, message):
+    """By the function, and by the C ABI before anything is launched (the pointers are never read)."""
+    with pytest.raises(ValueError, match=message):
+        attend(*(Tensor(x, dtype=float32) for x in drawn(1.0)[:3]), **kw)
+    lib, fake = runtime.kernels(), ctypes.c_void_p(0x1000)
+    rules = (dict(scale=0.25, softcap=0.0) | kw)
+    tail = (1, 1, 2, 1, 9, 9, 16, 16, 0, rules["scale"], rules["softcap"], fake, 1 << 40, None)
+    for status in (lib.limn_hip_attend_fwd(*[fake] * 3, *[None] * 4, *[fake] * 2, *tail), lib.limn_hip_attend_bwd(*[fake] * 3, *[None] * 4, *[fake] * 6, *tail)):
+        assert status == 1 and message in lib.limn_hip_last_error().decode()
+
+
+@pytest.mark.parametrize("scale", [0.0, 1e-39, -1e-39, 1e-30])
+def test_scales_of_nothing(scale):
+    q, k, v, do = drawn(1.0, seed=3)
+    tq, tk, tv = (Tensor(x, dtype=float32, requires_grad=True) for x in (q, k, v))
+    out = attend(tq, tk, tv, causal=True, scale=scale)
+    got = [out, *grad((out * Tensor(do, dtype=float32)).sum(), [tq, tk, tv])]
+    want = definition(q, k, v, dout=do, causal=True, scale=scale, dtype="float32")
+    for name, t in zip(("out", "dq", "dk", "dv"), got):
+        within(t.numpy(), *want[name], name)

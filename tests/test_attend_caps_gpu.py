@@ -58,3 +58,17 @@ def test_an_infinite_score_is_the_cap(hipdev, dtype, hd):
     # weights and result rounded to the type, and sums of 130 terms of one exponential each
     bound = (2 * half + 200 * 2.0**-24) * (p @ np.abs(v[0, 0])) / p.sum()
     within(out[0, 0, 77], p @ v[0, 0] / p.sum(), bound)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("hd", [33, 64, 128])
+@pytest.mark.parametrize("scale", [1e-20, 1e-29, 1e-31, 1e-39, 1e-50, -1e-39])
+def test_scales_of_nothing(hipdev, dtype, hd, scale):
+    """Equal weights: out, the logsumexp, and the values' gradient of a mean. The tiles take the score units of a scale's inverse."""
+    _, (q, k, v, do) = draw(hd, dtype, 1, 2, 1, 150, 150, hd, hd)
+    check(hipdev, q, k, v, do, dtype, {}, dict(causal=True, scale=scale))
+    out, lse = served(hipdev, q, k, v, dtype, {}, causal=True, scale=scale)
+    want = definition(q, k, v, dtype=dtype, causal=True, scale=scale)
+    within(lse, *want["lse"], "lse")
+    if dtype == "float32" and hd % 4 == 0:
+        check_tiles(hipdev, q, k, v, do, {}, dict(causal=True, scale=scale))
