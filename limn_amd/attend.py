@@ -16,6 +16,7 @@ positions), query head h reads key head h // (heads / kv_heads), and
 from __future__ import annotations
 
 import math
+from collections.abc import Callable
 
 from limn_amd.seam import CUT_OPS, FLOATS, Node, Op, Tensor, accumulate_in, active_device, custom, float32, float64, grad, int32, promote
 
@@ -81,7 +82,7 @@ def attend(q: Tensor, k: Tensor, v: Tensor, *, causal: bool = False, softcap: fl
 
     def backward(g: Tensor):
         if records(q, k, v) or not dev.has_custom(ATTEND_BWD):
-            return through(_composed(q, k, v, *rules, causal, scale, softcap), (q, k, v), g)
+            return through(lambda *qkv: _composed(*qkv, *rules, causal, scale, softcap), (q, k, v), g)
         do = contiguous(g)
         srcs = tuple(t.node for t in (q, k, v, *given)) + (out, lse, do.node)
         return tuple(Tensor.from_node(n) for n in custom(ATTEND_BWD, srcs, params, tuple((t.dtype, t.shape) for t in (q, k, v))))
@@ -102,11 +103,13 @@ def records(*tensors: Tensor) -> bool:
     return Tensor.from_node(tensors[0].node, tensors, lambda g: (g,) * len(tensors)).requires_grad
 
 
-def through(out: Tensor, inputs: tuple[Tensor, ...], g: Tensor) -> tuple[Tensor | None, ...]:
-    """The cotangents that g on `out` gives each input, by limn's own rules for out's graph."""
-    wanted = [t for t in inputs if t.requires_grad]
-    found = iter(grad((out * g).sum(), wanted, create_graph=True))
-    return tuple(next(found) if t.requires_grad else None for t in inputs)
+def through(build: Callable[..., Tensor], inputs: tuple[Tensor, ...], g: Tensor) -> tuple[Tensor | None, ...]:
+    """The cotangents that g on build(*inputs) gives each input, by limn's own rules for its graph. It is built of a tensor of
+    its own for each input: g comes from the inputs too, one input may be another's, or made from it, and none of those paths
+    is the input's share here."""
+    own = [Tensor.from_node(t.node, (t,), lambda c: (c,)) for t in inputs]
+    found = iter(grad((build(*own) * g).sum(), [t for t in own if t.requires_grad], create_graph=True))
+    return tuple(next(found) if t.requires_grad else None for t in own)
 
 
 def _tanh_terms(count: int) -> list[float]:

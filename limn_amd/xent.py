@@ -57,7 +57,7 @@ def _rows(x: Tensor, w: Tensor, targets: Tensor) -> Tensor:
 
     def backward(g: Tensor):
         if records(x, w) or not dev.has_custom(XENT_BWD):
-            return through(_composed(x, w, targets), (x, w), g)
+            return through(lambda x, w: _composed(x, w, targets), (x, w), g)
         srcs = (x.node, w.node, targets.node, lse, contiguous(g).node)
         return tuple(Tensor.from_node(n) for n in custom(XENT_BWD, srcs, (), ((x.dtype, x.shape), (w.dtype, w.shape))))
 
