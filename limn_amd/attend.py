@@ -2,7 +2,7 @@
 with query heads that share key heads and the live length of a cache.
 
 `attend` is to these what `Tensor.attention` (reference `limn/tensor.py:509-575`) is to causal and key
-masks: it emits the CUSTOM kernels "attend_fwd" and "attend_bwd" where the active device registers them
+masks: it emits the CUSTOM kernels "attend_fwd" and "attend_bwd" where the active device registers both
 (the hip device does, `limn_hip_attend_fwd` and `limn_hip_attend_bwd` of include/limn_hip.h), and the form composed
 from limn's primitives elsewhere, for float64, and where the gradient must itself be differentiable.
 
@@ -71,7 +71,7 @@ def attend(q: Tensor, k: Tensor, v: Tensor, *, causal: bool = False, softcap: fl
     q, k, v = (t.cast(width) for t in (q, k, v))
     rules = (slopes, documents, prefix, lengths)
     dev = active_device()
-    if width == float64 or max(hd, v.shape[-1]) > 256 or not dev.has_custom(ATTEND_FWD):
+    if width == float64 or max(hd, v.shape[-1]) > 256 or not (dev.has_custom(ATTEND_FWD) and dev.has_custom(ATTEND_BWD)):
         return _composed(q, k, v, *rules, causal, scale, softcap)
     q, k, v = contiguous(q), contiguous(k), contiguous(v)
     given = tuple(contiguous(t) for t in rules if t is not None)
@@ -81,7 +81,7 @@ def attend(q: Tensor, k: Tensor, v: Tensor, *, causal: bool = False, softcap: fl
     out, lse = custom(ATTEND_FWD, tuple(t.node for t in (q, k, v, *given)), params, outs)
 
     def backward(g: Tensor):
-        if records(q, k, v) or not dev.has_custom(ATTEND_BWD):
+        if records(q, k, v):
             return through(lambda *qkv: _composed(*qkv, *rules, causal, scale, softcap), (q, k, v), g)
         do = contiguous(g)
         srcs = tuple(t.node for t in (q, k, v, *given)) + (out, lse, do.node)

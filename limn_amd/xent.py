@@ -49,14 +49,14 @@ def linear_cross_entropy(x: Tensor, weight: Tensor, targets: Tensor, reduction: 
 def _rows(x: Tensor, w: Tensor, targets: Tensor) -> Tensor:
     """The rows' losses, shaped as targets. The kernels take the leading dims as one (row-major bytes)."""
     dev = active_device()
-    if x.dtype == float64 or not dev.has_custom(XENT_FWD):
+    if x.dtype == float64 or not (dev.has_custom(XENT_FWD) and dev.has_custom(XENT_BWD)):
         return _composed(x, w, targets)
     x, w, targets = contiguous(x), contiguous(w), contiguous(targets)
     rows = targets.shape
     loss, lse = custom(XENT_FWD, (x.node, w.node, targets.node), (), ((float32, rows), (float32, rows)))
 
     def backward(g: Tensor):
-        if records(x, w) or not dev.has_custom(XENT_BWD):
+        if records(x, w):
             return through(lambda x, w: _composed(x, w, targets), (x, w), g)
         srcs = (x.node, w.node, targets.node, lse, contiguous(g).node)
         return tuple(Tensor.from_node(n) for n in custom(XENT_BWD, srcs, (), ((x.dtype, x.shape), (w.dtype, w.shape))))

@@ -67,3 +67,14 @@ def test_inputs_that_share_tensors(name):
     for i, (a, b) in enumerate(zip(got, want)):
         # chains of some hundred float32 roundings: a thousand half steps of the largest; a share counted twice is its own size
         assert np.abs(a - b).max() <= 2.0**-14 * np.abs(b).max(), (i, np.abs(a - b).max(), np.abs(b).max())
+
+
+@pytest.mark.parametrize("name", ["keys from both", "a head from its rows"])
+def test_a_device_with_the_forward_kernels_alone(name):
+    set_device("numpy")
+    rng = np.random.default_rng(7)
+    x, w = (rng.standard_normal((1, 2, 5, 4)).astype(np.float32) for _ in range(2))
+    want = orders(CALLS[name], x, w, float64)
+    active_device().custom.update({n: f for n, f in KERNELS.items() if n.endswith("fwd")})
+    for a, b in zip(orders(CALLS[name], x, w, float32), want):
+        assert np.abs(a - b).max() <= 2.0**-14 * np.abs(b).max()
