@@ -5,8 +5,8 @@ limn's training example computes as log_softmax of the head's output (reference
 `examples/train_stories.py:61-64`). There the logits are a (rows, vocab) tensor, and their log_softmax and its
 gradient two more; here the CUSTOM kernels "xent_fwd" and "xent_bwd" (`limn_hip_xent_fwd` and
 `limn_hip_xent_bwd` of include/limn_hip.h) walk the vocabulary in pieces and keep two numbers a row. Where the active
-device registers none, for float64, and where the gradient must itself be differentiable, it is composed
-from limn's primitives.
+device does not register both, for float64, and where the gradient must itself be differentiable, it is
+composed from limn's primitives.
 """
 
 from __future__ import annotations
@@ -66,6 +66,9 @@ def _rows(x: Tensor, w: Tensor, targets: Tensor) -> Tensor:
 
 def _composed(x: Tensor, w: Tensor, targets: Tensor) -> Tensor:
     wide, vocab, rows = accumulate_in(x.dtype), w.shape[0], math.prod(targets.shape)
-    logp = (x.cast(wide).reshape(rows, x.shape[-1]) @ w.cast(wide).transpose()).log_softmax(-1)
+    # a row left out goes as zeros, and its logits too: what it or the weight holds is multiplied by no gradient of 0
+    live = ((targets >= 0) * (targets < vocab)).reshape(rows, 1)
+    kept = live.where(x.cast(wide).reshape(rows, x.shape[-1]), 0.0)
+    logp = live.where(kept @ w.cast(wide).transpose(), 0.0).log_softmax(-1)
     picked = Tensor.arange(vocab).reshape(1, vocab).eq(targets.reshape(rows, 1))
     return -(picked.where(logp, 0.0)).sum(axis=-1).reshape(*targets.shape)
