@@ -28,7 +28,8 @@
 //
 // Every operand is PARTS matrices of one shape, one part_a or part_b elements behind another (1 or 3).
 //
-// A row without a target has dz = 0; what its x holds reaches nothing (see Products and the flags of xent_dz).
+// A row without a target has dz = 0; what its x holds reaches nothing (see Products and the flags of xent_dz), and its dx is
+// stored as zeros, as a dz of 0 times a weight that is not finite would be NaN.
 
 #include "matmul_dma.h"
 #include "xent.h"
@@ -463,11 +464,19 @@ struct Products {
   int64_t rows, vocab;
 };
 
-// 4 columns of a result's row; columns past the width are padding and not stored
-template <typename T>
+// 4 columns of a result's row; columns past the width are padding and not stored. DX: zeros for a row without a target, which
+// is asked for only where a total is not finite.
+template <typename T, bool DX>
 __device__ __forceinline__ void store4(const Products& s, int64_t row, int64_t col, f32x4 v) {
   if (col >= s.width) return;
   if (IS_F16<T>) v *= s.scale[1];
+  if (DX) {
+    const f32x4 odd = v * 0.f;
+    if (odd[0] + odd[1] + odd[2] + odd[3] != 0.f) {
+      const int t = s.targets[row];
+      if (t < 0 || t >= s.vocab) v = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+  }
   if (s.out_f32) {
     float* o = (float*)s.out + row * s.width + col;
     if (s.vec) {
@@ -544,7 +553,7 @@ __global__ __launch_bounds__(64 * Tile<BM>::WAVES, 2) void xent_product(Products
         if (row >= s.m || col >= s.n) continue;  // n is a multiple of 8
         if (s.add != nullptr) v += *(const f32x4*)(s.add + row * s.n + col);
         if (s.out != nullptr)
-          store4<T>(s, row, col, v);
+          store4<T, A_K>(s, row, col, v);
         else
           *(f32x4*)(s.wide + (slice * s.m + row) * s.n + col) = v;
       }
@@ -555,7 +564,7 @@ __global__ __launch_bounds__(64 * Tile<BM>::WAVES, 2) void xent_product(Products
 
 // out = round(add + slices), or the same kept in float32 (s.wide). A workgroup is 64 threads of 4 elements by G runs
 // of the slices, which are joined in order in LDS.
-template <typename T>
+template <typename T, bool DX>
 __global__ __launch_bounds__(1024) void xent_fold(Products s, const float* __restrict__ slices, int64_t count) {
   __shared__ f32x4 part[16][64];
   const int x = threadIdx.x, y = threadIdx.y, runs = blockDim.y;
@@ -573,7 +582,7 @@ __global__ __launch_bounds__(1024) void xent_fold(Products s, const float* __res
   if (s.add != nullptr) v += *(const f32x4*)(s.add + i);
   if (s.out != nullptr) {
     const int64_t row = i / s.n;
-    store4<T>(s, row, i - row * s.n, v);
+    store4<T, DX>(s, row, i - row * s.n, v);
   } else {
     *(f32x4*)(s.wide + i) = v;
   }
@@ -760,7 +769,7 @@ int launch_product(Products s, const Cut& c, float* slices, float* acc, bool fir
   const int64_t groups = (s.m * s.n / 4 + 63) / 64;
   if (groups > 0x7fffffff) return fail(LIMN_HIP_EUNSUPPORTED, "xent: %lld workgroups exceed one launch", (long long)groups);
   const int runs = c.split < 8 ? 4 : c.split < 32 ? 8 : 16;
-  hipLaunchKernelGGL((xent_fold<T>), dim3((unsigned)groups), dim3(64, runs), 0, stream, s, slices, c.split);
+  hipLaunchKernelGGL((xent_fold<T, A_K>), dim3((unsigned)groups), dim3(64, runs), 0, stream, s, slices, c.split);
   return check_hip(hipGetLastError(), "launching the fold of a product's slices");
 }
 
