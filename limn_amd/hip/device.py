@@ -22,8 +22,6 @@ import ctypes
 import dataclasses
 import math
 import time
-import weakref
-from collections.abc import Callable
 from typing import Any
 
 import numpy as np
@@ -73,7 +71,7 @@ def plan_context(order: list[Node], sinks: list[Node]) -> tuple[set, set]:
 class HipBuffer:
     """Device bytes; the pointer returns to its device's pool when the last reference drops."""
 
-    __slots__ = ("ptr", "nbytes", "pool", "__weakref__")
+    __slots__ = ("ptr", "nbytes", "pool")
 
     def __init__(self, ptr: int, nbytes: int, pool: dict[int, list[int]]):
         self.ptr = ptr
@@ -117,6 +115,10 @@ class ArenaBuffer:
 class HipDevice(CompiledDevice):
     """Construct through set_device("hip"), which checks the runtime and the GPU first."""
 
+    _workspace: HipBuffer | None = None  # see _scratch
+    _taped: list[HipBuffer] = []  # the workspaces that the run which records a launch list has been given
+    _running: int | None = None  # id of the plan whose launch list is being replayed
+
     def __init__(self) -> None:
         self.plan_kept: set | None = None  # set by plan_of for runners(), see there
         self.plan_custom_inputs: set | None = None
@@ -142,7 +144,6 @@ class HipDevice(CompiledDevice):
         self._committed: list[tuple[Buffer, Buffer]] = []  # launched, kept alive until the barrier
         self._commit_table: tuple[int, int, Buffer] | None = None  # (pinned host ptr, rows, device copy)
         self._commit_kernel: int | None = None
-        self._workspaces: weakref.WeakValueDictionary[int, HipBuffer] = weakref.WeakValueDictionary()  # by bytes, see _held
         self.custom[SDPA] = self._sdpa_runner
         self.custom[SDPA_BWD_Q] = self._sdpa_runner
         self.custom[SDPA_BWD_KV] = self._sdpa_runner
@@ -167,15 +168,21 @@ class HipDevice(CompiledDevice):
         if status != 0 and self.pool:
             self.trim()
             status = self.api.hipMalloc(ctypes.byref(ptr), max(nb, 1))
+        if status != 0 and self._release_workspace():
+            self.trim()
+            status = self.api.hipMalloc(ctypes.byref(ptr), max(nb, 1))
         check(status, f"allocating {nb} bytes")
         return HipBuffer(ptr.value, nb, self.pool)
 
     def trim(self) -> None:
-        """Give every pooled buffer, and every launch list's idle arenas, back to the runtime."""
+        """Give every pooled buffer, every launch list's idle arenas, and a workspace that no list
+        names, back to the runtime."""
         self.finish()
         for entry in self.replays.values():
             if entry[1] is not None:
                 entry[1].arenas = [a for a in entry[1].arenas if a.live]
+        if not self._naming(self._workspace):
+            self._workspace = None
         for ptrs in self.pool.values():
             for ptr in ptrs:
                 self.api.hipFree(ctypes.c_void_p(ptr))
@@ -255,6 +262,7 @@ class HipDevice(CompiledDevice):
         out_positions: list[tuple[int, int]] = []
         assigns: list[tuple[int, int]] = []
         self.tape = tape = []
+        self._taped = []
         try:
             for call in plan.calls:
                 outs = [self.out_alloc(nb, call.zero_fill) for nb in call.out_nbytes]
@@ -269,6 +277,7 @@ class HipDevice(CompiledDevice):
                     assigns.append((call.assign_target, base))
         finally:
             self.tape = None
+            workspaces, self._taped = tuple(self._taped), []
         for p, i in assigns:
             self.commit(sources[p], outs_all[i])
             bufs[p] = outs_all[i]
@@ -281,10 +290,17 @@ class HipDevice(CompiledDevice):
             nbytes = tuple(o.nbytes for o in outs_all)
             offsets, total = replay.arena_layout(nbytes)
             entry[1] = replay.Program(bound[0], bound[1], nbytes, tuple(out_positions), tuple(assigns), plan.positions,
-                                      offsets, total)
+                                      offsets, total, workspaces)
         return [bufs[p] for p in plan.sinks]
 
     def _replay(self, plan, prog: "replay.Program", sources):
+        self._running = id(plan)
+        try:
+            return self._replayed(plan, prog, sources)
+        finally:
+            self._running = None
+
+    def _replayed(self, plan, prog: "replay.Program", sources):
         start = time.perf_counter()
         bufs: list = [None] * plan.positions
         slots = np.zeros(prog.nslots, dtype=np.int64)
@@ -504,45 +520,59 @@ class HipDevice(CompiledDevice):
 
     def _fused_backward(self, code: int, ints: tuple, scale: float, masked: bool) -> Runner | None:
         """The runner of a paired backward call (outputs dq, dk, dv) through limn_hip_sdpa_bwd, or
-        None when the call has no dS hand-off route or its workspace would pass SDPA_HANDOFF_CAP.
-        The workspace is allocated on the first run and kept with the runner, so a replayed or
-        graph-captured list sees the same pointer every time."""
+        None when the call has no dS hand-off route or its workspace would pass SDPA_HANDOFF_CAP."""
         lib = self.lib
         need = int(lib.limn_hip_sdpa_bwd_workspace(code, *ints, int(masked)))
         if need <= 0 or need > self.SDPA_HANDOFF_CAP:
             return None
-        held: list = []
 
         def run(inputs: list[Buffer], outs: list[Buffer]) -> None:
-            if not held:
-                held.append(self._alloc(need))
-            ws = held[0]
+            ws, room = self._scratch(need)
             mask = inputs[6].ptr if masked else None
             args = (*[b.ptr for b in inputs[:6]], mask, outs[0].ptr, outs[1].ptr, outs[2].ptr, code, *ints)
-            check_limn(lib.limn_hip_sdpa_bwd(*args, scale, BWD_BOTH, ws.ptr, ws.nbytes, None))
+            check_limn(lib.limn_hip_sdpa_bwd(*args, scale, BWD_BOTH, ws, room, None))
             if self.tape is not None:
-                self.tape.append(replay.Launch(replay.STEP_SDPA_BWD, (*args, BWD_BOTH, ws.ptr, ws.nbytes), scale=scale))
+                self.tape.append(replay.Launch(replay.STEP_SDPA_BWD, (*args, BWD_BOTH, ws, room), scale=scale))
 
         return run
 
-    def _held(self, need: int) -> Callable[[], tuple[int | None, int]]:
-        """A runner's workspace as (pointer, bytes): taken on its first run and kept with it, so a replayed
-        or graph-captured list sees the same pointer every time. Runners that need as many bytes share one
-        (the layers of a model, say): every launch of the device is on the null stream, one runner's after
-        another's."""
-        held: list = []
+    # ---- the operators' workspace ----
 
-        def workspace() -> tuple[int | None, int]:
-            if need <= 0:
-                return None, 0
-            if not held:
-                shared = self._workspaces.get(need)
-                if shared is None:
-                    shared = self._workspaces[need] = self._alloc(need)
-                held.append(shared)
-            return held[0].ptr, held[0].nbytes
+    def _scratch(self, need: int) -> tuple[int | None, int]:
+        """A workspace for one operator call, as (pointer, bytes). The device keeps one, as large as the
+        largest call since it was let go: every launch is on the null stream, one behind another, and
+        none keeps anything there. A launch list names the one that it was recorded with and keeps it; when a
+        larger one takes its place, the lists that name it are dropped, and recorded again as their plans
+        run on, so what is held for calls of many sizes is what the largest needs and an eighth."""
+        if need <= 0:
+            return None, 0
+        if self._workspace is None or self._workspace.nbytes < need:
+            self._release_workspace()
+            step = max(1 << 20, 1 << max(0, need.bit_length() - 4))  # in steps of an eighth, so that sizes that creep up grow it rarely
+            self._workspace = self._alloc(-(-need // step) * step)
+        if self.tape is not None and self._workspace not in self._taped:
+            self._taped.append(self._workspace)
+        return self._workspace.ptr, need
 
-        return workspace
+    def _naming(self, workspace: HipBuffer | None) -> list[int]:
+        """The plans whose launch lists name this workspace."""
+        return [key for key, entry in self.replays.items() if entry[1] is not None and workspace in entry[1].workspaces]
+
+    def _release_workspace(self) -> bool:
+        """Let the workspace go, and the launch lists that name it (but one that is being replayed, which keeps
+        it): back to the runtime at once, as no call asks for its size again. False if there is none."""
+        if self._workspace is None:
+            return False
+        for key in self._naming(self._workspace):
+            if key != self._running:
+                self._drop_replay(key)
+        self.finish()
+        ptr, nbytes = self._workspace.ptr, self._workspace.nbytes
+        self._workspace = None  # into the pool, unless a list or a recording still holds it
+        if ptr in self.pool.get(nbytes, ()):
+            self.pool[nbytes].remove(ptr)
+            self.api.hipFree(ctypes.c_void_p(ptr))
+        return True
 
     # ---- attention with score rules, the head's cross entropy ----
 
@@ -576,7 +606,7 @@ class HipDevice(CompiledDevice):
                 raise ValueError(f"{name} shape mismatch: out {out.shape}, dout {do.shape} {do.dtype}, lse {lse.shape}")
         code, sizes = ABI_CODE[q.dtype], (batch, heads, kv_heads, t_q, t_k, hd, hd_v)
         flags, scale, softcap = int(bool(causal)), float(scale), float(softcap)
-        workspace = self._held(int(self.lib.limn_hip_attend_workspace(code, *sizes, int(backward))))
+        need = int(self.lib.limn_hip_attend_workspace(code, *sizes, int(backward)))
         entry = self.lib.limn_hip_attend_bwd if backward else self.lib.limn_hip_attend_fwd
         kind = replay.STEP_ATTEND_BWD if backward else replay.STEP_ATTEND_FWD
         cap_bits = ctypes.c_int64.from_buffer_copy(ctypes.c_double(softcap)).value
@@ -585,7 +615,7 @@ class HipDevice(CompiledDevice):
             ptrs = [b.ptr for b in inputs]
             rules = iter(ptrs[3:count])
             args = (*ptrs[:3], *(next(rules) if on else None for on in given), *ptrs[count:], *(b.ptr for b in outs), code, *sizes, flags)
-            ws, room = workspace()
+            ws, room = self._scratch(need)
             check_limn(entry(*args, scale, softcap, ws, room, None))
             if self.tape is not None:
                 self.tape.append(replay.Launch(kind, (*args, cap_bits, ws, room), scale=scale))
@@ -605,13 +635,13 @@ class HipDevice(CompiledDevice):
         if not x.shape or len(w.shape) != 2 or x.shape[-1] != w.shape[1] or any(s.shape != x.shape[:-1] for s in (targets, *node.srcs[3:])):
             raise ValueError(f"{name} shape mismatch: {[s.shape for s in node.srcs]}")
         code, sizes = ABI_CODE[x.dtype], (math.prod(x.shape[:-1]), *reversed(w.shape))
-        workspace = self._held(int(self.lib.limn_hip_xent_workspace(code, *sizes, int(backward))))
+        need = int(self.lib.limn_hip_xent_workspace(code, *sizes, int(backward)))
         entry = self.lib.limn_hip_xent_bwd if backward else self.lib.limn_hip_xent_fwd
         kind = replay.STEP_XENT_BWD if backward else replay.STEP_XENT_FWD
 
         def run(inputs: list[Buffer], outs: list[Buffer]) -> None:
             args = (*(b.ptr for b in inputs), *(b.ptr for b in outs), code, *sizes)
-            ws, room = workspace()
+            ws, room = self._scratch(need)
             check_limn(entry(*args, ws, room, None))
             if self.tape is not None:
                 self.tape.append(replay.Launch(kind, (*args, ws, room)))

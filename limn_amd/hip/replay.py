@@ -77,6 +77,7 @@ class Program:
     positions: int  # slots [0, positions) are the plan's buffer positions, then the outputs
     arena_offsets: tuple[int, ...] = ()  # each output's byte offset in the replay's one allocation
     arena_bytes: int = 0
+    workspaces: tuple = ()  # the buffers the steps name as workspaces, held so that they stay theirs
     # captured graphs by binding (slot values), the most recently used last; a training loop that
     # keeps the previous step's result alive while it runs the next alternates two bindings
     graphs: dict[bytes, ctypes.c_void_p] = field(default_factory=dict)
