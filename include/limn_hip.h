@@ -215,10 +215,15 @@ int limn_hip_contract_pays(int dtype, int64_t batch, int64_t M, int64_t N, int64
  *   lengths. hd and hd_v at most 256. scale between -2^120 and 2^120; softcap 0 for none, else from 2^-120 to 2^120.
  * `workspace` must hold limn_hip_attend_workspace(...) bytes, 16-byte aligned, for this call alone: calls
  * that may overlap, and captured graphs that may run at once, need one each. A backward's holds up to 2.5 GiB of
- * score gradients between its passes. Every result is deterministic. Sums and statistics are float32; float32
- * operands are multiplied as sums of three bfloat16 numbers each (to some 2^-24 |x y| + 2^-134 (|x| + |y|)) where
- * the call has more than 256 tiles of 32 query rows (128 in a backward). No counterpart in the reference (its attention has a causal and a key mask, limn/tensor.py:509-575);
- * composed there, the scores are a tensor in memory.
+ * score gradients between its passes. Every result is deterministic. Sums and statistics are float32. Where the
+ * 16-bit matrix cores take a half width's second products, their operands are rounded to that width: the
+ * probabilities (of out and dv) and the score gradients (of dq and dk); delta, the row sum of dout out, takes
+ * out as it is stored. A capped score is off by some 16 half steps of float32 of itself; in half widths under
+ * caps up to 64 by 8 of the cap. float32 operands are multiplied as sums of three bfloat16 numbers each (to some
+ * 2^-24 |x y| + 2^-134 (|x| + |y|)) in a forward of more than 256 tiles of 32 query rows, a backward of 128 or
+ * more, where hd == hd_v is a multiple of 4 up to 128, t_q and t_k are at most 2^17, the scale is 2^-100 or more and
+ * every buffer 16-byte aligned. No counterpart in the reference (its attention has a causal and a key mask,
+ * limn/tensor.py:509-575); composed there, the scores are a tensor in memory.
  */
 int limn_hip_attend_fwd(const void* q, const void* k, const void* v, const void* slopes, const void* documents,
                         const void* prefix, const void* lengths, void* out, void* lse, int dtype, int64_t batch,
@@ -243,11 +248,13 @@ int64_t limn_hip_attend_workspace(int dtype, int64_t batch, int64_t heads, int64
  * z[n, v] = x[n] . w[v],
  *   loss[n] = lse[n] - z[n, targets[n]], lse[n] = logsumexp_v z[n, v]
  * The logits are never kept: the vocabulary goes by in pieces. A target outside [0, vocab) leaves its row
- * out: loss 0, no gradient, and what the row holds reaches nothing.
+ * out: loss 0, no gradient (zeros, whatever the weight holds), and what the row holds reaches nothing.
  *   x (rows, width) and w (vocab, width) of float32, float16 or bfloat16, targets (rows) int32; loss and lse
  *   (rows) float32. Sums and statistics are float32. float32 operands are multiplied as sums of three bfloat16
  *   numbers each: a product x w is exact to some 2^-24 |x w| + 2^-134 (|x| + |w|), and an infinity among the
  *   operands of a row that has a target makes it NaN.
+ * 32-bit offsets reach (rows + 512) * width below some 2^30, at least 690000 rows and widths up to 260000 (the
+ * workspace's entry says: 0 past them); larger calls are LIMN_HIP_EUNSUPPORTED, and a caller takes the rows in parts.
  * Workspace as for limn_hip_attend_fwd, of limn_hip_xent_workspace(...) bytes. No counterpart in the reference,
  * whose training example takes log_softmax of the logits (examples/train_stories.py:61-64).
  */

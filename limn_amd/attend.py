@@ -39,7 +39,9 @@ def attend(q: Tensor, k: Tensor, v: Tensor, *, causal: bool = False, softcap: fl
       2^120;
     - `scale`: of the scores, 1 / sqrt(hd) if not given; up to 2^120 either way.
 
-    A query that sees no key gives zeros and passes no gradient. The leading dims of q, k and v are equal, as
+    A query that sees no key gives zeros and passes no gradient. What hidden keys hold changes nothing where the device's
+    kernels run (head dims up to 256, not float64); composed of primitives, an infinity or a NaN there
+    spoils the rows that do not see it too. The leading dims of q, k and v are equal, as
     are those of documents, prefix and lengths.
     """
     if min(q.ndim, k.ndim, v.ndim) < 3:

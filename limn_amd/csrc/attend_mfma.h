@@ -12,8 +12,8 @@
 //  - the cap and the distance are float arithmetic on the score tile. Per 32 x 32 tile at D = 128 the matrix
 //    cores take 512 cycles a wave for the forward's two products; the softmax takes 16 exponentials of 16
 //    cycles and about 6 other operations of 4 an element, the cap an exponential and a reciprocal more.
-//    At two waves a SIMD it is the length of that chain which counts, not its issue: a polynomial tanh of near
-//    scores, 20 cycles an element less, took as long (385 and 375 us forward, 1096 and 1110 backward, of the case below).
+//    At two waves a SIMD it is the length of that chain which counts, not its issue: the exact cap of near scores, a
+//    polynomial of some 10 cycles an element less, takes no less (see Cap).
 //  - the query heads of a key head are one loop of the dK/dV pass: their gradients are one sum in head order.
 //
 // Measured (causal, bf16; of the rate of the products it must do): 4 x 16 heads over 4 key heads x 4096 x 128, capped:

@@ -92,10 +92,12 @@ class Program:
 
     @functools.cached_property
     def launches(self) -> int:
-        """Kernel launches of the list, at most: a contraction given a workspace may fold k slices, one of
-        half widths copy its operands as well; LAUNCHES has the other kinds of
-        several (a cross entropy's for one piece of the vocabulary, attention's without documents or parts: one
-        attention and its gradients are faster launch by launch, 230 us against 241 at 8 x 12 heads x 1021 x 80)."""
+        """Kernel launches of the list, as they count for the choice between a graph and its steps: a contraction
+        given a workspace may fold k slices, one of half widths copy its operands as well; LAUNCHES has the other
+        kinds of several. It is an estimate for those: a cross entropy's for one piece of the vocabulary, attention's
+        without documents (one more a pass) and parts (one more in the backward), so that one attention and its
+        gradients go launch by launch, which is faster with documents too (8 x 12 heads x 1021 x 80, a prefix: 230 us
+        against 241 as a graph; 2 x 4 x 256 x 64 float32, documents and every other rule: 133 against 147)."""
         total = 0
         for kind, first in zip(self.steps["kind"].tolist(), self.steps["first"].tolist()):
             value = lambda k: int(self.args["value"][first + k])

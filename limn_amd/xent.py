@@ -24,6 +24,8 @@ def linear_cross_entropy(x: Tensor, weight: Tensor, targets: Tensor, reduction: 
 
     A target outside [0, vocab) leaves its row out. `reduction`: "mean" over the other rows (0 where there is
     none), "sum", or "none" for the rows' own losses, shaped as targets; float32 for every width but float64.
+    The kernels take up to some 2^30 elements and 690000 rows of x; more raise NotImplementedError when the loss is
+    realized, and go in parts whose sums are added.
     """
     if x.ndim < 1 or weight.ndim != 2:
         raise ValueError(f"linear_cross_entropy needs rows (..., width) and a (vocab, width) weight, got {x.shape} and {weight.shape}")
