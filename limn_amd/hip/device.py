@@ -22,6 +22,7 @@ import ctypes
 import dataclasses
 import math
 import time
+from collections.abc import Callable
 from typing import Any
 
 import numpy as np
@@ -66,6 +67,28 @@ def plan_context(order: list[Node], sinks: list[Node]) -> tuple[set, set]:
     values (every sink, every CUSTOM src), and the CUSTOM srcs alone."""
     custom_inputs = {realized(src) for n in order if n.op is Op.CUSTOM for src in n.srcs}
     return {realized(s) for s in sinks} | custom_inputs, custom_inputs
+
+
+def by_source(build: Callable[[Node], Runner]) -> Callable[[Node], Runner]:
+    """A CUSTOM builder whose runners take one buffer a src. A plan's call has each distinct src once (keys that are
+    the values too, say), so a node that names one twice gets its buffer twice here."""
+
+    def built(node: Node) -> Runner:
+        run, places = build(node), {}
+        which = [places.setdefault(src, len(places)) for src in node.srcs]
+        if len(places) == len(which):
+            return run
+
+        def spread(fn: Runner | None) -> Runner | None:
+            return None if fn is None else lambda inputs, outs: fn([inputs[p] for p in which], outs)
+
+        each, pair = spread(run), getattr(run, "sdpa_pair", None)
+        if pair is not None:  # see HipDevice._pair_backward: only calls that repeat alike pair
+            name, key, fused = pair
+            each.sdpa_pair = (name, (key, tuple(which)), lambda: spread(fused()))
+        return each
+
+    return built
 
 
 class HipBuffer:
@@ -144,11 +167,9 @@ class HipDevice(CompiledDevice):
         self._committed: list[tuple[Buffer, Buffer]] = []  # launched, kept alive until the barrier
         self._commit_table: tuple[int, int, Buffer] | None = None  # (pinned host ptr, rows, device copy)
         self._commit_kernel: int | None = None
-        self.custom[SDPA] = self._sdpa_runner
-        self.custom[SDPA_BWD_Q] = self._sdpa_runner
-        self.custom[SDPA_BWD_KV] = self._sdpa_runner
-        self.custom[ATTEND_FWD] = self.custom[ATTEND_BWD] = self._attend_runner
-        self.custom[XENT_FWD] = self.custom[XENT_BWD] = self._xent_runner
+        self.custom[SDPA] = self.custom[SDPA_BWD_Q] = self.custom[SDPA_BWD_KV] = by_source(self._sdpa_runner)
+        self.custom[ATTEND_FWD] = self.custom[ATTEND_BWD] = by_source(self._attend_runner)
+        self.custom[XENT_FWD] = self.custom[XENT_BWD] = by_source(self._xent_runner)
         # pre-bound launch lists: id(plan) -> [plan, Program or None, refused], least recently
         # run first, at most replay.PLANS_KEPT; `tape` collects the launches of the run that
         # records one (every launch site appends while it is set)
