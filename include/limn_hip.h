@@ -5,7 +5,8 @@
  * limn reaches its GPU kernels through ctypes (reference limn/backend_cuda.py:54-151 binds the
  * CUDA driver and NVRTC the same way). The generated loop-nest kernels go through hipRTC and
  * hipModuleLaunchKernel directly; the three fused-attention CUSTOM kernels, the dense
- * contraction, attention with score rules and the head's cross entropy are hand-written and exported here.
+ * contraction, attention with score rules, the head's cross entropy, and what answering with a language model takes
+ * (attention over a paged cache, sampling, 8-bit linear layers) are hand-written and exported here.
  *
  * Conventions for every entry point:
  *  - pointers are device pointers (hipMalloc'd), row-major and contiguous;
@@ -271,6 +272,77 @@ int limn_hip_xent_bwd(const void* x, const void* w, const void* targets, const v
 int64_t limn_hip_xent_workspace(int dtype, int64_t rows, int64_t width, int64_t vocab, int backward);
 
 /*
+ * Attention of packed new tokens over a paged cache, which takes up their keys and values: a layer of a server's step.
+ * Sequence s has the rows starts[s] .. starts[s + 1] of q, k and v, n of them, which are the last of its L = lengths[s]
+ * positions: row i of them sits at p(i) = L - n + i. Key j of the sequence lies in place j % page of page
+ * table[s][j / page]. The keys and values of the new tokens go to their places, and with query head h reading key head
+ * h / (heads / kv_heads),
+ *   s[i, j] = cap(scale q_i . k_j) - slopes[h] (p(i) - j),  cap(x) = softcap tanh(x / softcap), or x at 0
+ *   out_i = sum_j softmax_j(s[i, j]) v_j over the keys j <= p(i).
+ *   q (tokens, heads, hd), k and v (tokens, kv_heads, hd), tokens q_row, k_row and v_row elements apart (so that they may lie
+ *   side by side in the rows of one projection); key_pages and value_pages (pages, kv_heads, page, hd), out (tokens,
+ *   heads, hd), all of float32, float16 or bfloat16; starts (sequences + 1, ascending), lengths (sequences), table (sequences,
+ *   table_pages) int32; slopes (heads) float32 or NULL. k and v NULL: the cache holds the new tokens already.
+ * Rows of no sequence give zeros and write nothing. Positions below 0 (more rows than L) see nothing and give zeros. Of a
+ * page number outside [0, pages) the keys are not there: nothing is written, and no query sees them. L is taken as
+ * within [0, table_pages * page], starts as within [0, tokens]; a table's entries behind the last position are not read. What
+ * a key that a query does not see holds, infinities and NaN among them, changes nothing in its row. Pages that this
+ * call writes to belong to one sequence; others may be shared. q, k, v and out do not overlap the pages.
+ * hd at most 256; scale between -2^120 and 2^120; softcap 0 for none, else from 2^-120 to 2^120.
+ * `workspace` must hold limn_hip_attend_paged_workspace(...) bytes, 16-byte aligned, for this call alone, as for
+ * limn_hip_attend_fwd. Results are deterministic; sums and statistics are float32. Half widths multiply on 16-bit matrix cores
+ * where hd is a multiple of 8 up to 128 and every buffer and row 16-byte aligned: the weights are rounded to the half width
+ * there. No counterpart in the reference.
+ */
+int limn_hip_attend_paged(const void* q, const void* k, const void* v, void* key_pages, void* value_pages, const void* starts,
+                          const void* lengths, const void* table, const void* slopes, void* out, int dtype, int64_t tokens,
+                          int64_t sequences, int64_t heads, int64_t kv_heads, int64_t hd, int64_t pages, int64_t page,
+                          int64_t table_pages, int64_t q_row, int64_t k_row, int64_t v_row, double scale, double softcap,
+                          void* workspace, int64_t workspace_bytes, void* stream);
+
+int64_t limn_hip_attend_paged_workspace(int dtype, int64_t tokens, int64_t sequences, int64_t heads, int64_t kv_heads, int64_t hd,
+                                        int64_t pages, int64_t page, int64_t table_pages);
+
+/*
+ * A token for each row of logits from a given uniform number u. With w_j = exp((x_j - max x) / temperature) and the order of
+ * x descending, equal ones by index: the first top_k are kept; of those the ones before which less than top_p of their mass
+ * lies; of those the ones with w_j >= min_p; the first always. The token is the first one whose mass with all before it
+ * passes u times the kept mass; its logprob the logarithm of its share of that mass.
+ *   logits (rows, vocab), rows row_stride elements apart, of float32, float16 or bfloat16; uniforms, temperature, top_p and
+ *   min_p (rows) float32, top_k (rows) int32, the last four NULL for none; tokens (rows) int32, logprobs (rows) float32 or NULL.
+ * A temperature of 0 or below, or NaN, takes the first of the order with a logprob of 0. top_k outside [1, vocab), top_p of 1
+ * or more or NaN, and min_p of 0 or below or NaN keep everything. A u outside [0, 1) is taken as the nearest end (NaN: the
+ * last one kept). NaN among the logits counts as minus infinity; a row without anything above that gives -1 and minus
+ * infinity; an infinite logit has all of the mass. vocab up to 2^24.
+ * Weights and masses are computed in 64 bits; results are deterministic. Workspace as above, of limn_hip_sample_workspace(...)
+ * bytes. No counterpart in the reference (its training example draws from a softmax on the host, examples/train_stories.py).
+ */
+int limn_hip_sample(const void* logits, const void* uniforms, const void* temperature, const void* top_k, const void* top_p,
+                    const void* min_p, void* tokens, void* logprobs, int dtype, int64_t rows, int64_t vocab, int64_t row_stride,
+                    void* workspace, int64_t workspace_bytes, void* stream);
+
+int64_t limn_hip_sample_workspace(int dtype, int64_t rows, int64_t vocab);
+
+/*
+ * Rows x (rows, width) of float32, float16 or bfloat16 brought to 8 bits: scales[r] = max(max |x[r]| / 127, 2^-126) and
+ * values[r][i] = round(x[r][i] / scales[r]), ties to even, in float32 arithmetic. A row with an infinity or a NaN gets the scale NaN
+ * and zeros. No counterpart in the reference.
+ */
+int limn_hip_quantize_rows(const void* x, void* values, void* scales, int dtype, int64_t rows, int64_t width, void* stream);
+
+/*
+ * A linear layer in 8-bit integers: x (rows, width) brought to 8 bits as limn_hip_quantize_rows does, x8 with scales s, then
+ *   out[r][n] = (sum_i x8[r][i] weight[n][i]) s[r] weight_scales[n] + bias[n]
+ * with weight (outputs, width) int8, weight_scales (outputs) float32, bias (outputs) of x's type or NULL, out (rows, outputs) of x's
+ * type. The sums are exact; their products with the scales and the sum with the bias are float32, rounded once to out's type.
+ * width up to 2^17. Workspace as above, of limn_hip_int8_linear_workspace(...) bytes. No counterpart in the reference.
+ */
+int limn_hip_int8_linear(const void* x, const void* weight, const void* weight_scales, const void* bias, void* out, int dtype,
+                         int64_t rows, int64_t width, int64_t outputs, void* workspace, int64_t workspace_bytes, void* stream);
+
+int64_t limn_hip_int8_linear_workspace(int dtype, int64_t rows, int64_t width, int64_t outputs);
+
+/*
  * A pre-bound launch list: the kernels of one recorded execution of a plan, replayed against new
  * buffers. Each step is one launch: a hipRTC module kernel (`function`, `grid` x `block`
  * threads, its arguments the kernel's parameters in order), a zero fill (pointer, bytes), or one
@@ -278,8 +350,9 @@ int64_t limn_hip_xent_workspace(int dtype, int64_t rows, int64_t width, int64_t 
  * limn_hip_contract (27), limn_hip_sdpa_fwd (13 before `scale`), limn_hip_sdpa_bwd_q (15),
  * limn_hip_sdpa_bwd_kv (16) or limn_hip_sdpa_bwd (17 before `scale`, then passes, workspace and
  * its size: 20), limn_hip_attend_fwd (18 before `scale`, then softcap as the bits of a double, workspace and
- * its size: 21), limn_hip_attend_bwd (22, then the same: 25), with `scale` in the step, limn_hip_xent_fwd (11)
- * or limn_hip_xent_bwd (13). An
+ * its size: 21), limn_hip_attend_bwd (22, then the same: 25), with `scale` in the step, limn_hip_xent_fwd (11),
+ * limn_hip_xent_bwd (13), limn_hip_attend_paged (22 before `scale`, then softcap's bits, workspace and its size: 25, with
+ * `scale` in the step), limn_hip_sample (14), limn_hip_quantize_rows (6) or limn_hip_int8_linear (11). An
  * argument is `value` when `slot` < 0, else slots[slot] + value: a byte offset into the buffer
  * this replay binds to that slot. Steps run in order on `stream`; the first failing one stops the
  * list and its status is returned. No counterpart in the reference: its capture replays a plan
@@ -299,6 +372,10 @@ enum {
   LIMN_HIP_STEP_ATTEND_BWD = 10,
   LIMN_HIP_STEP_XENT_FWD = 11,
   LIMN_HIP_STEP_XENT_BWD = 12,
+  LIMN_HIP_STEP_ATTEND_PAGED = 13,
+  LIMN_HIP_STEP_SAMPLE = 14,
+  LIMN_HIP_STEP_QUANTIZE_ROWS = 15,
+  LIMN_HIP_STEP_INT8_LINEAR = 16,
 };
 
 typedef struct {

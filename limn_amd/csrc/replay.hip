@@ -177,6 +177,39 @@ int run_step(const limn_hip_replay_step& s, int64_t i, const limn_hip_replay_arg
       auto at = [&](int k) { return (void*)(intptr_t)v[k]; };
       return limn_hip_xent_bwd(at(0), at(1), at(2), at(3), at(4), at(5), at(6), (int)v[7], v[8], v[9], v[10], at(11), v[12], stream);
     }
+    case LIMN_HIP_STEP_ATTEND_PAGED: {
+      int rc = expect(s, i, 25, "attend_paged");
+      if (rc != LIMN_HIP_OK) return rc;
+      int64_t v[25];
+      for (int k = 0; k < 25; k++) v[k] = bound(a[k], slots);
+      auto at = [&](int k) { return (void*)(intptr_t)v[k]; };
+      double softcap;
+      memcpy(&softcap, &v[22], sizeof softcap);
+      return limn_hip_attend_paged(at(0), at(1), at(2), at(3), at(4), at(5), at(6), at(7), at(8), at(9), (int)v[10], v[11], v[12], v[13], v[14], v[15],
+                                   v[16], v[17], v[18], v[19], v[20], v[21], s.scale, softcap, at(23), v[24], stream);
+    }
+    case LIMN_HIP_STEP_SAMPLE: {
+      int rc = expect(s, i, 14, "sample");
+      if (rc != LIMN_HIP_OK) return rc;
+      int64_t v[14];
+      for (int k = 0; k < 14; k++) v[k] = bound(a[k], slots);
+      auto at = [&](int k) { return (void*)(intptr_t)v[k]; };
+      return limn_hip_sample(at(0), at(1), at(2), at(3), at(4), at(5), at(6), at(7), (int)v[8], v[9], v[10], v[11], at(12), v[13], stream);
+    }
+    case LIMN_HIP_STEP_QUANTIZE_ROWS: {
+      int rc = expect(s, i, 6, "quantize_rows");
+      if (rc != LIMN_HIP_OK) return rc;
+      return limn_hip_quantize_rows(ptr(a[0], slots), (void*)ptr(a[1], slots), (void*)ptr(a[2], slots), (int)bound(a[3], slots), bound(a[4], slots),
+                                    bound(a[5], slots), stream);
+    }
+    case LIMN_HIP_STEP_INT8_LINEAR: {
+      int rc = expect(s, i, 11, "int8_linear");
+      if (rc != LIMN_HIP_OK) return rc;
+      int64_t v[11];
+      for (int k = 0; k < 11; k++) v[k] = bound(a[k], slots);
+      auto at = [&](int k) { return (void*)(intptr_t)v[k]; };
+      return limn_hip_int8_linear(at(0), at(1), at(2), at(3), at(4), (int)v[5], v[6], v[7], v[8], at(9), v[10], stream);
+    }
     default:
       return fail(LIMN_HIP_EINVAL, "replay step %lld: unknown kind %d", (long long)i, s.kind);
   }

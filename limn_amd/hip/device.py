@@ -9,7 +9,8 @@ this GPU rather than translated:
   hipRTC once per program and launched with hipModuleLaunchKernel on the null stream;
 - the CUSTOM attention kernels `sdpa`, `sdpa_bwd_q` and `sdpa_bwd_kv` are the hand-written
   MFMA/LDS kernels of liblimn_hip.so, reached through its C ABI (include/limn_hip.h), and so are
-  `attend_fwd`/`attend_bwd` (limn_amd/attend.py) and `xent_fwd`/`xent_bwd` (limn_amd/xent.py);
+  `attend_fwd`/`attend_bwd` (limn_amd/attend.py), `xent_fwd`/`xent_bwd` (limn_amd/xent.py), `attend_paged`
+  (limn_amd/paged.py), `sample` (limn_amd/sampling.py), `quantize_rows` and `int8_linear` (limn_amd/int8.py);
 - host arrays handed in are uploaded per batch (`prepare`), and an ASSIGN whose target is a host
   array is written back (`commit`), as the reference device does;
 - `finish()` synchronizes once per batch, which pins an asynchronous failure to its batch.
@@ -30,12 +31,13 @@ import numpy as np
 from limn_amd.dtypes import ABI_CODE
 from limn_amd.hip import replay, runtime
 from limn_amd.hip.runtime import DEVICE_TO_DEVICE, DEVICE_TO_HOST, HOST_TO_DEVICE, check, check_limn
-from limn_amd.seam import FLOATS, CompiledDevice, LoopNest, Node, Op, Runner, accumulate_in, float32, int32, realized
+from limn_amd.seam import FLOATS, CompiledDevice, LoopNest, Node, Op, Runner, accumulate_in, float32, int8, int32, realized
 
 Buffer = Any
 
 SDPA, SDPA_BWD_Q, SDPA_BWD_KV = "sdpa", "sdpa_bwd_q", "sdpa_bwd_kv"
 ATTEND_FWD, ATTEND_BWD, XENT_FWD, XENT_BWD = "attend_fwd", "attend_bwd", "xent_fwd", "xent_bwd"  # limn_amd/attend.py, limn_amd/xent.py
+ATTEND_PAGED, SAMPLE, QUANTIZE_ROWS, INT8_LINEAR = "attend_paged", "sample", "quantize_rows", "int8_linear"  # limn_amd/paged.py, sampling.py, int8.py
 BWD_BOTH = 3  # LIMN_HIP_BWD_BOTH: limn_hip_sdpa_bwd runs both passes
 
 
@@ -170,6 +172,8 @@ class HipDevice(CompiledDevice):
         self.custom[SDPA] = self.custom[SDPA_BWD_Q] = self.custom[SDPA_BWD_KV] = by_source(self._sdpa_runner)
         self.custom[ATTEND_FWD] = self.custom[ATTEND_BWD] = by_source(self._attend_runner)
         self.custom[XENT_FWD] = self.custom[XENT_BWD] = by_source(self._xent_runner)
+        self.custom[ATTEND_PAGED], self.custom[SAMPLE] = by_source(self._paged_runner), by_source(self._sample_runner)
+        self.custom[QUANTIZE_ROWS], self.custom[INT8_LINEAR] = by_source(self._quantize_runner), by_source(self._int8_runner)
         # pre-bound launch lists: id(plan) -> [plan, Program or None, refused], least recently
         # run first, at most replay.PLANS_KEPT; `tape` collects the launches of the run that
         # records one (every launch site appends while it is set)
@@ -666,5 +670,102 @@ class HipDevice(CompiledDevice):
             check_limn(entry(*args, ws, room, None))
             if self.tape is not None:
                 self.tape.append(replay.Launch(kind, (*args, ws, room)))
+
+        return run
+
+    # ---- answering with a language model ----
+
+    def _paged_runner(self, node: Node) -> Runner:
+        """CUSTOM attend_paged (srcs q, the new k and v if given, both pools of pages, starts, lengths, table, slopes if given),
+        bound to limn_hip_attend_paged. It writes the pools, which are sources, in place. params: (scale, softcap, whether k
+        and v are given, whether slopes are)."""
+        name, (scale, softcap, fresh, sloped) = node.arg.name, node.arg.params
+        if len(node.srcs) != 6 + 2 * fresh + sloped:
+            raise ValueError(f"{name}: expected {6 + 2 * fresh + sloped} srcs, got {len(node.srcs)}")
+        q, news, (keys, values, starts, lengths, table), slopes = node.srcs[0], node.srcs[1 : 1 + 2 * fresh], node.srcs[1 + 2 * fresh : 6 + 2 * fresh], node.srcs[6 + 2 * fresh :]
+        if q.dtype not in ABI_CODE or q.dtype not in FLOATS or any(s.dtype != q.dtype for s in (*news, keys, values)):
+            raise NotImplementedError(f"{name}: no kernel for dtypes {[s.dtype for s in (q, *news, keys, values)]}")
+        if len(q.shape) != 3 or len(keys.shape) != 4 or len(table.shape) != 2:
+            raise ValueError(f"{name} shape mismatch: {[s.shape for s in node.srcs]}")
+        (tokens, heads, hd), (pages, kv_heads, page, _), (sequences, table_pages) = q.shape, keys.shape, table.shape
+        if (keys.shape[-1] != hd or values.shape != keys.shape or any(s.shape != (tokens, kv_heads, hd) for s in news) or starts.shape != (sequences + 1,)
+                or lengths.shape != (sequences,) or any(s.shape != (heads,) or s.dtype != float32 for s in slopes) or any(s.dtype != int32 for s in (starts, lengths, table))):
+            raise ValueError(f"{name} shape mismatch: {[(s.shape, s.dtype) for s in node.srcs]}")
+        code, sizes = ABI_CODE[q.dtype], (tokens, sequences, heads, kv_heads, hd, pages, page, table_pages)
+        rows, scale, softcap = (heads * hd, kv_heads * hd, kv_heads * hd), float(scale), float(softcap)
+        need = int(self.lib.limn_hip_attend_paged_workspace(code, *sizes))
+        cap_bits = ctypes.c_int64.from_buffer_copy(ctypes.c_double(softcap)).value
+
+        def run(inputs: list[Buffer], outs: list[Buffer]) -> None:
+            ptrs = [b.ptr for b in inputs]
+            args = (ptrs[0], *(ptrs[1:3] if fresh else (None, None)), *ptrs[1 + 2 * fresh : 6 + 2 * fresh], ptrs[-1] if sloped else None, outs[0].ptr, code, *sizes, *rows)
+            ws, room = self._scratch(need)
+            check_limn(self.lib.limn_hip_attend_paged(*args, scale, softcap, ws, room, None))
+            if self.tape is not None:
+                self.tape.append(replay.Launch(replay.STEP_ATTEND_PAGED, (*args, cap_bits, ws, room), scale=scale))
+
+        return run
+
+    def _sample_runner(self, node: Node) -> Runner:
+        """CUSTOM sample (srcs logits, uniforms, the settings given), bound to limn_hip_sample. params: which of temperature,
+        top_k, top_p, min_p are given."""
+        name, given = node.arg.name, node.arg.params
+        if len(node.srcs) != 2 + sum(given):
+            raise ValueError(f"{name}: expected {2 + sum(given)} srcs, got {len(node.srcs)}")
+        logits = node.srcs[0]
+        if logits.dtype not in ABI_CODE or logits.dtype not in FLOATS:
+            raise NotImplementedError(f"{name}: no kernel for dtype {logits.dtype}")
+        kinds = (float32, *(kind for on, kind in zip(given, (float32, int32, float32, float32)) if on))
+        if not logits.shape or any(s.shape != logits.shape[:-1] or s.dtype != kind for s, kind in zip(node.srcs[1:], kinds)):
+            raise ValueError(f"{name} shape mismatch: {[(s.shape, s.dtype) for s in node.srcs]}")
+        code, rows, vocab = ABI_CODE[logits.dtype], math.prod(logits.shape[:-1]), logits.shape[-1]
+        need = int(self.lib.limn_hip_sample_workspace(code, rows, vocab))
+
+        def run(inputs: list[Buffer], outs: list[Buffer]) -> None:
+            rules = iter(b.ptr for b in inputs[2:])
+            args = (inputs[0].ptr, inputs[1].ptr, *(next(rules) if on else None for on in given), outs[0].ptr, outs[1].ptr, code, rows, vocab, vocab)
+            ws, room = self._scratch(need)
+            check_limn(self.lib.limn_hip_sample(*args, ws, room, None))
+            if self.tape is not None:
+                self.tape.append(replay.Launch(replay.STEP_SAMPLE, (*args, ws, room)))
+
+        return run
+
+    def _quantize_runner(self, node: Node) -> Runner:
+        """CUSTOM quantize_rows (src x), bound to limn_hip_quantize_rows."""
+        (x,) = node.srcs
+        if x.dtype not in ABI_CODE or x.dtype not in FLOATS or not x.shape:
+            raise NotImplementedError(f"{node.arg.name}: no kernel for {x.shape} {x.dtype}")
+        sizes = (ABI_CODE[x.dtype], math.prod(x.shape[:-1]), x.shape[-1])
+
+        def run(inputs: list[Buffer], outs: list[Buffer]) -> None:
+            args = (inputs[0].ptr, outs[0].ptr, outs[1].ptr, *sizes)
+            check_limn(self.lib.limn_hip_quantize_rows(*args, None))
+            if self.tape is not None:
+                self.tape.append(replay.Launch(replay.STEP_QUANTIZE_ROWS, args))
+
+        return run
+
+    def _int8_runner(self, node: Node) -> Runner:
+        """CUSTOM int8_linear (srcs x, weight, scales, bias if given), bound to limn_hip_int8_linear. params: (whether a bias is
+        given,)."""
+        name, (biased,) = node.arg.name, node.arg.params
+        if len(node.srcs) != 3 + biased:
+            raise ValueError(f"{name}: expected {3 + biased} srcs, got {len(node.srcs)}")
+        x, w, scales, bias = node.srcs[0], node.srcs[1], node.srcs[2], node.srcs[3:]
+        if x.dtype not in ABI_CODE or x.dtype not in FLOATS or w.dtype != int8 or scales.dtype != float32 or any(s.dtype != x.dtype for s in bias):
+            raise NotImplementedError(f"{name}: no kernel for dtypes {[s.dtype for s in node.srcs]}")
+        if not x.shape or len(w.shape) != 2 or x.shape[-1] != w.shape[1] or any(s.shape != w.shape[:1] for s in (scales, *bias)):
+            raise ValueError(f"{name} shape mismatch: {[s.shape for s in node.srcs]}")
+        code, sizes = ABI_CODE[x.dtype], (math.prod(x.shape[:-1]), w.shape[1], w.shape[0])
+        need = int(self.lib.limn_hip_int8_linear_workspace(code, *sizes))
+
+        def run(inputs: list[Buffer], outs: list[Buffer]) -> None:
+            ptrs = [b.ptr for b in inputs]
+            args = (*ptrs[:3], ptrs[3] if biased else None, outs[0].ptr, code, *sizes)
+            ws, room = self._scratch(need)
+            check_limn(self.lib.limn_hip_int8_linear(*args, ws, room, None))
+            if self.tape is not None:
+                self.tape.append(replay.Launch(replay.STEP_INT8_LINEAR, (*args, ws, room)))
 
         return run

@@ -28,7 +28,8 @@ from dataclasses import dataclass, field
 import numpy as np
 
 (STEP_KERNEL, STEP_ZERO, STEP_MATMUL, STEP_SDPA_FWD, STEP_SDPA_BWD_Q, STEP_SDPA_BWD_KV, STEP_MATMUL_ADD,
- STEP_SDPA_BWD, STEP_CONTRACT, STEP_ATTEND_FWD, STEP_ATTEND_BWD, STEP_XENT_FWD, STEP_XENT_BWD) = range(13)
+ STEP_SDPA_BWD, STEP_CONTRACT, STEP_ATTEND_FWD, STEP_ATTEND_BWD, STEP_XENT_FWD, STEP_XENT_BWD, STEP_ATTEND_PAGED, STEP_SAMPLE,
+ STEP_QUANTIZE_ROWS, STEP_INT8_LINEAR) = range(17)
 
 # which arguments of each step kind are device pointers (the rest are sizes, codes and flags)
 POINTER_ARGS = {
@@ -44,9 +45,14 @@ POINTER_ARGS = {
     STEP_ATTEND_BWD: frozenset(range(13)) | {23},
     STEP_XENT_FWD: frozenset(range(5)) | {9},
     STEP_XENT_BWD: frozenset(range(7)) | {11},
+    STEP_ATTEND_PAGED: frozenset(range(10)) | {23},
+    STEP_SAMPLE: frozenset(range(8)) | {12},
+    STEP_QUANTIZE_ROWS: frozenset(range(3)),
+    STEP_INT8_LINEAR: frozenset(range(5)) | {9},
 }
 
-LAUNCHES = {STEP_SDPA_BWD: 2, STEP_ATTEND_FWD: 2, STEP_ATTEND_BWD: 4, STEP_XENT_FWD: 4, STEP_XENT_BWD: 8}
+LAUNCHES = {STEP_SDPA_BWD: 2, STEP_ATTEND_FWD: 2, STEP_ATTEND_BWD: 4, STEP_XENT_FWD: 4, STEP_XENT_BWD: 8,
+            STEP_ATTEND_PAGED: 2, STEP_INT8_LINEAR: 2}
 
 ARG = np.dtype([("value", np.int64), ("slot", np.int32), ("reserved", np.int32)])
 STEP = np.dtype([("kind", np.int32), ("nargs", np.int32), ("first", np.int64), ("function", np.uint64),

@@ -119,6 +119,13 @@ _LIMN = {
     "limn_hip_xent_fwd": (c_int, [c_void_p] * 5 + [c_int, _I64, _I64, _I64, c_void_p, _I64, c_void_p]),
     "limn_hip_xent_bwd": (c_int, [c_void_p] * 7 + [c_int, _I64, _I64, _I64, c_void_p, _I64, c_void_p]),
     "limn_hip_xent_workspace": (_I64, [c_int, _I64, _I64, _I64, c_int]),
+    "limn_hip_attend_paged": (c_int, [c_void_p] * 10 + [c_int] + [_I64] * 11 + [ctypes.c_double, ctypes.c_double, c_void_p, _I64, c_void_p]),
+    "limn_hip_attend_paged_workspace": (_I64, [c_int] + [_I64] * 8),
+    "limn_hip_sample": (c_int, [c_void_p] * 8 + [c_int, _I64, _I64, _I64, c_void_p, _I64, c_void_p]),
+    "limn_hip_sample_workspace": (_I64, [c_int, _I64, _I64]),
+    "limn_hip_quantize_rows": (c_int, [c_void_p] * 3 + [c_int, _I64, _I64, c_void_p]),
+    "limn_hip_int8_linear": (c_int, [c_void_p] * 5 + [c_int, _I64, _I64, _I64, c_void_p, _I64, c_void_p]),
+    "limn_hip_int8_linear_workspace": (_I64, [c_int, _I64, _I64, _I64]),
 }
 
 # The C ABI's status codes (include/limn_hip.h) and the Python exception each maps to.
