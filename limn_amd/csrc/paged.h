@@ -73,14 +73,26 @@ __device__ __forceinline__ Sequence sequence_at(const PagedView& v, int s) {
   return Sequence{b, e - b, len, len - (e - b)};
 }
 
-// The sequence of a row, or -1: the last one that starts at or before it, if it reaches the row.
-__device__ __forceinline__ int sequence_of(const PagedView& v, int row) {
-  int lo = 0, hi = v.sequences;  // starts[lo] <= row < starts[hi], if any starts at or before it
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (v.starts[mid] <= row) lo = mid; else hi = mid;
+// The last sequence whose place(s), which does not fall along the sequences, is at most `at`; the first if there is none. For
+// a whole wave at a time: 64 sequences are looked at with one load.
+template <typename F>
+__device__ __forceinline__ int last_sequence(const PagedView& v, int at, F place) {
+  const int lane = threadIdx.x & 63;
+  int lo = 0, span = v.sequences;
+  while (span > 1) {
+    const int step = (span + 63) / 64;
+    const uint64_t before = __ballot(lane * step < span && place(min(lo + lane * step, v.sequences - 1)) <= at);
+    const int k = before == 0 ? 0 : 63 - __builtin_clzll(before);
+    lo += k * step;
+    span = min(step, span - k * step);
   }
-  return v.starts[lo] <= row && row < v.starts[lo + 1] ? lo : -1;
+  return __builtin_amdgcn_readfirstlane(lo);
+}
+
+// The sequence of a row, or -1: the last one that starts at or before it, if it reaches the row. For a whole wave.
+__device__ __forceinline__ int sequence_of(const PagedView& v, int row) {
+  const int s = last_sequence(v, row, [&](int i) { return v.starts[i]; });
+  return v.starts[s] <= row && row < v.starts[s + 1] ? s : -1;
 }
 
 // The elements before key j of sequence s and key head h in the pages, or -1 where its page is not one of the cache's.

@@ -1,7 +1,7 @@
 // The C ABI of attention over a paged cache: argument checks, choice of kernels; the write of the new tokens' keys and
 // values into their pages; and the kernel that serves every type, head dim and alignment.
 
-#include "paged.h"
+#include "paged_fast.h"
 
 #include <math.h>
 
@@ -105,6 +105,41 @@ int write_of(const PagedArgs& a) {
   return check_hip(hipGetLastError(), "launching the write of a paged cache");
 }
 
+// ---- the tiled kernels ----
+
+// Joins the parts of a sequence: a wave a token and head, the parts' totals brought to the largest reference point and added
+// in their order. A part that saw nothing (no reference point and a sum of 0: it is NaN where a score was) counts nothing.
+template <typename T>
+__global__ __launch_bounds__(256) void paged_join(PagedFast f, PagedView v) {
+  const int lane = threadIdx.x & 63;
+  const int64_t id = blockIdx.x * (int64_t)4 + (threadIdx.x >> 6), rows_all = (int64_t)v.tokens * v.heads;
+  if (id >= rows_all) return;  // whole waves, and there is no barrier
+  const int row = (int)(id / v.heads), s = sequence_of(v, row);
+  if (s < 0) return;
+  const Sequence q = sequence_at(v, s);
+  const int tile = ((row - q.row0) * v.group + (int)(id - (int64_t)row * v.heads) % v.group) / f.rows;
+  const int parts = (span_of(v, q, tile, f.rows, f.k != nullptr, f.keys).tiles + f.part_tiles - 1) / f.part_tiles;
+  if (parts <= 1 || q.n * v.group < f.few_rows || q.n * v.group >= f.many_rows) return;
+  float top = -__builtin_inff();
+  for (int p = 0; p < parts; p++) top = fmaxf(top, f.stats[(p * rows_all + id) * 2]);
+  const float base = top == -__builtin_inff() ? 0.f : top;
+  float total = 0.f, x[2] = {0.f, 0.f};
+#pragma unroll 4
+  for (int p = 0; p < parts; p++) {
+    const float m = f.stats[(p * rows_all + id) * 2], l = f.stats[(p * rows_all + id) * 2 + 1];
+    if (m == -__builtin_inff() && l == 0.f) continue;
+    const float w = m == -__builtin_inff() ? 1.f : fast_exp2(m - base);
+    total += l * w;
+#pragma unroll
+    for (int c = 0; c < 2; c++)
+      if (c * 64 + lane < v.hd) x[c] += w * f.totals[(p * rows_all + id) * v.hd + c * 64 + lane];
+  }
+  const float inv = total == 0.f ? 0.f : 1.f / total;
+#pragma unroll
+  for (int c = 0; c < 2; c++)
+    if (c * 64 + lane < v.hd) T::store((typename T::Storage*)f.out + id * v.hd, c * 64 + lane, x[c] * inv);
+}
+
 int check_paged(const PagedArgs& a) {
   const char* name = "attend_paged";
   if (a.dtype != LIMN_HIP_FLOAT32 && a.dtype != LIMN_HIP_FLOAT16 && a.dtype != LIMN_HIP_BFLOAT16)
@@ -144,6 +179,63 @@ int check_buffers(const PagedArgs& a) {
   return LIMN_HIP_OK;
 }
 
+template <typename T>
+int join_of(const PagedArgs& a, const PagedFast& f) {
+  hipLaunchKernelGGL((paged_join<T>), dim3((unsigned)((a.tokens * a.heads + 3) / 4)), dim3(256), 0, a.stream, f, paged_view(a));
+  return check_hip(hipGetLastError(), "joining the parts of attention over a paged cache");
+}
+
+int join(const PagedArgs& a, const PagedFast& f) {
+  return a.dtype == LIMN_HIP_FLOAT32 ? join_of<F32>(a, f) : a.dtype == LIMN_HIP_FLOAT16 ? join_of<F16>(a, f) : join_of<BF16>(a, f);
+}
+
+// Sizes that the tiled kernels serve: rows of whole 16-byte chunks; places counted in 32 bits.
+bool fast_sizes(const PagedArgs& a) {
+  return a.hd <= 128 && a.hd % (a.dtype == LIMN_HIP_FLOAT32 ? 4 : 8) == 0 && a.pages < (int64_t)0xffffffff / a.kv_heads / a.page;
+}
+// A call of such sizes goes to them where every buffer and row is 16-byte aligned, and its constants stay normal numbers.
+bool fast_call(const PagedArgs& a) {
+  const uintptr_t at = (uintptr_t)a.q | (uintptr_t)a.k | (uintptr_t)a.v | (uintptr_t)a.key_pages | (uintptr_t)a.value_pages | (uintptr_t)a.out;
+  const int64_t per = a.dtype == LIMN_HIP_FLOAT32 ? 4 : 8;
+  return fast_sizes(a) && at % 16 == 0 && a.q_row % per == 0 && (a.k == nullptr || (a.k_row % per == 0 && a.v_row % per == 0));
+}
+
+// Row tiles of 16 where one holds a sequence's packed rows, else of 32. Up to 64 key tiles go to one workgroup of many waves a
+// row tile while such workgroups leave waves free; longer caches to workgroups of 4 waves, in as many parts as give every
+// CU four of them, each at least 8 key tiles.
+PagedPlan token_plan(const PagedArgs& a) {
+  PagedPlan p;
+  const int64_t rows = (a.tokens + a.sequences - 1) / a.sequences * a.group(), tiles = (a.table_pages * a.page + 31) / 32 + 1;
+  p.nr = rows <= 16 ? 1 : 2;
+  const int64_t units = a.sequences * a.kv_heads * ((rows + 16 * p.nr - 1) / (16 * p.nr));
+  p.lone = tiles <= 65 && units <= 256;
+  int64_t parts = p.lone ? 1 : 1024 / units;
+  if (parts > tiles / 8) parts = tiles / 8;
+  if (parts < 1) parts = 1;
+  p.part_tiles = (int)((tiles + parts - 1) / parts);
+  p.parts = (int)((tiles + p.part_tiles - 1) / p.part_tiles);
+  return p;
+}
+
+constexpr int64_t align256(int64_t bytes) { return (bytes + 255) / 256 * 256; }
+
+int64_t parts_bytes(const PagedArgs& a, const PagedPlan& p) {
+  return p.parts > 1 ? align256(p.parts * a.tokens * a.heads * a.hd * 4) + align256(p.parts * a.tokens * a.heads * 8) : 0;
+}
+
+int64_t workspace_of(const PagedArgs& a) { return fast_sizes(a) ? parts_bytes(a, token_plan(a)) : 0; }
+
+int launch_fast(const PagedArgs& a) {
+  const PagedPlan p = token_plan(a);
+  PagedFast f = {a.q, a.k, a.v, a.key_pages, a.value_pages, a.out, nullptr, nullptr, p.parts, p.part_tiles, 0, 0x7fffffff, 16 * p.nr, 32};
+  if (p.parts > 1) {
+    f.totals = (float*)a.workspace;
+    f.stats = (float*)((char*)a.workspace + align256(p.parts * a.tokens * a.heads * a.hd * 4));
+  }
+  const int rc = launch_paged_token(a, f, p);
+  return rc == LIMN_HIP_OK && p.parts > 1 ? join(a, f) : rc;
+}
+
 }  // namespace
 }  // namespace limn
 
@@ -151,7 +243,9 @@ using namespace limn;
 
 extern "C" int64_t limn_hip_attend_paged_workspace(int dtype, int64_t tokens, int64_t sequences, int64_t heads, int64_t kv_heads, int64_t hd, int64_t pages,
                                                    int64_t page, int64_t table_pages) {
-  return 0;
+  const PagedArgs a = {nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, dtype, tokens, sequences, heads, kv_heads, hd, pages,
+                       page, table_pages, heads * hd, 0, 0, 1.0, 0.0, nullptr, 0, nullptr};
+  return check_paged(a) == LIMN_HIP_OK ? workspace_of(a) : 0;
 }
 
 extern "C" int limn_hip_attend_paged(const void* q, const void* k, const void* v, void* key_pages, void* value_pages, const void* starts, const void* lengths,
@@ -163,6 +257,10 @@ extern "C" int limn_hip_attend_paged(const void* q, const void* k, const void* v
   int rc = check_paged(a);
   if (rc == LIMN_HIP_OK) rc = check_buffers(a);
   if (rc != LIMN_HIP_OK) return rc;
+  const int64_t need = workspace_of(a);
+  if (need > 0 && (workspace == nullptr || (uintptr_t)workspace % 16 != 0 || workspace_bytes < need))
+    return fail(LIMN_HIP_EINVAL, "attend_paged: needs a workspace of %lld bytes, 16-byte aligned", (long long)need);
+  if (fast_call(a)) return launch_fast(a);
   rc = dtype == LIMN_HIP_FLOAT32 ? write_of<float>(a) : write_of<u16>(a);
   if (rc != LIMN_HIP_OK) return rc;
   return dtype == LIMN_HIP_FLOAT32 ? rows_of<F32>(a) : dtype == LIMN_HIP_FLOAT16 ? rows_of<F16>(a) : rows_of<BF16>(a);
