@@ -80,7 +80,10 @@ __global__ __launch_bounds__(256) void paged_rows(PagedView v, const typename T:
       const int64_t at = ((int64_t)__shfl((int)(place >> 32), i) << 32) | (unsigned)__shfl((int)place, i);
 #pragma unroll
       for (int c = 0; c < 4; c++)
-        if (c * 64 + lane < v.hd) acc[c] = fmaf(wi, T::load(value_pages, at + c * 64 + lane), acc[c]);
+        if (c * 64 + lane < v.hd) {
+          const float x = T::load(value_pages, at + c * 64 + lane);
+          acc[c] = x - x == 0.f ? fmaf(wi, x, acc[c]) : acc[c] + x;  // (an infinity stays one under a weight that has come to 0)
+        }
     }
   }
   const float inv = l == 0.f ? 0.f : 1.f / l;
@@ -110,16 +113,17 @@ int write_of(const PagedArgs& a) {
 // Joins the parts of a sequence: a wave a token and head, the parts' totals brought to the largest reference point and added
 // in their order. A part that saw nothing (no reference point and a sum of 0: it is NaN where a score was) counts nothing.
 template <typename T>
-__global__ __launch_bounds__(256) void paged_join(PagedFast f, PagedView v) {
+__global__ __launch_bounds__(256) void paged_join(PagedFast few, PagedFast many, PagedView v) {
   const int lane = threadIdx.x & 63;
   const int64_t id = blockIdx.x * (int64_t)4 + (threadIdx.x >> 6), rows_all = (int64_t)v.tokens * v.heads;
   if (id >= rows_all) return;  // whole waves, and there is no barrier
   const int row = (int)(id / v.heads), s = sequence_of(v, row);
   if (s < 0) return;
   const Sequence q = sequence_at(v, s);
+  const PagedFast& f = q.n * v.group < few.many_rows ? few : many;
   const int tile = ((row - q.row0) * v.group + (int)(id - (int64_t)row * v.heads) % v.group) / f.rows;
   const int parts = (span_of(v, q, tile, f.rows, f.k != nullptr, f.keys).tiles + f.part_tiles - 1) / f.part_tiles;
-  if (parts <= 1 || q.n * v.group < f.few_rows || q.n * v.group >= f.many_rows) return;
+  if (parts <= 1) return;
   float top = -__builtin_inff();
   for (int p = 0; p < parts; p++) top = fmaxf(top, f.stats[(p * rows_all + id) * 2]);
   const float base = top == -__builtin_inff() ? 0.f : top;
@@ -132,7 +136,10 @@ __global__ __launch_bounds__(256) void paged_join(PagedFast f, PagedView v) {
     total += l * w;
 #pragma unroll
     for (int c = 0; c < 2; c++)
-      if (c * 64 + lane < v.hd) x[c] += w * f.totals[(p * rows_all + id) * v.hd + c * 64 + lane];
+      if (c * 64 + lane < v.hd) {
+        const float y = f.totals[(p * rows_all + id) * v.hd + c * 64 + lane];
+        x[c] += y - y == 0.f ? w * y : y;  // (an infinity stays one under a weight that has come to 0)
+      }
   }
   const float inv = total == 0.f ? 0.f : 1.f / total;
 #pragma unroll
@@ -180,13 +187,13 @@ int check_buffers(const PagedArgs& a) {
 }
 
 template <typename T>
-int join_of(const PagedArgs& a, const PagedFast& f) {
-  hipLaunchKernelGGL((paged_join<T>), dim3((unsigned)((a.tokens * a.heads + 3) / 4)), dim3(256), 0, a.stream, f, paged_view(a));
+int join_of(const PagedArgs& a, const PagedFast& few, const PagedFast& many) {
+  hipLaunchKernelGGL((paged_join<T>), dim3((unsigned)((a.tokens * a.heads + 3) / 4)), dim3(256), 0, a.stream, few, many, paged_view(a));
   return check_hip(hipGetLastError(), "joining the parts of attention over a paged cache");
 }
 
-int join(const PagedArgs& a, const PagedFast& f) {
-  return a.dtype == LIMN_HIP_FLOAT32 ? join_of<F32>(a, f) : a.dtype == LIMN_HIP_FLOAT16 ? join_of<F16>(a, f) : join_of<BF16>(a, f);
+int join(const PagedArgs& a, const PagedFast& few, const PagedFast& many) {
+  return a.dtype == LIMN_HIP_FLOAT32 ? join_of<F32>(a, few, many) : a.dtype == LIMN_HIP_FLOAT16 ? join_of<F16>(a, few, many) : join_of<BF16>(a, few, many);
 }
 
 // Sizes that the tiled kernels serve: rows of whole 16-byte chunks; places counted in 32 bits.
@@ -200,40 +207,77 @@ bool fast_call(const PagedArgs& a) {
   return fast_sizes(a) && at % 16 == 0 && a.q_row % per == 0 && (a.k == nullptr || (a.k_row % per == 0 && a.v_row % per == 0));
 }
 
-// Row tiles of 16 where one holds a sequence's packed rows, else of 32. Up to 64 key tiles go to one workgroup of many waves a
-// row tile while such workgroups leave waves free; longer caches to workgroups of 4 waves, in as many parts as give every
-// CU four of them, each at least 8 key tiles.
-PagedPlan token_plan(const PagedArgs& a) {
-  PagedPlan p;
-  const int64_t rows = (a.tokens + a.sequences - 1) / a.sequences * a.group(), tiles = (a.table_pages * a.page + 31) / 32 + 1;
-  p.nr = rows <= 16 ? 1 : 2;
-  const int64_t units = a.sequences * a.kv_heads * ((rows + 16 * p.nr - 1) / (16 * p.nr));
-  p.lone = tiles <= 65 && units <= 256;
-  int64_t parts = p.lone ? 1 : 1024 / units;
-  if (parts > tiles / 8) parts = tiles / 8;
-  if (parts < 1) parts = 1;
-  p.part_tiles = (int)((tiles + parts - 1) / parts);
-  p.parts = (int)((tiles + p.part_tiles - 1) / p.part_tiles);
+// Sequences of up to FEW_ROWS packed rows go to paged_token, those of more to paged_tiles (half widths).
+constexpr int FEW_ROWS = 64;
+
+// What a call launches: how many sequences have how many rows is known on the device alone, so a call that may have both kinds
+// launches both kernels, each for its own.
+struct Plan {
+  bool few, many;
+  PagedPlan token;
+  int tile_parts, tile_part;  // paged_tiles: parts at most, key tiles of a part
+  int parts() const { return few && token.parts > tile_parts ? token.parts : many ? tile_parts : token.parts; }
+};
+
+// parts of `tiles` key tiles that bring `units` workgroups to `fill`, each at least 8 tiles
+void cut(int64_t tiles, int64_t units, int64_t fill, int& parts, int& part) {
+  int64_t p = fill / (units > 1 ? units : 1);
+  if (p > tiles / 8) p = tiles / 8;
+  if (p < 1) p = 1;
+  part = (int)((tiles + p - 1) / p);
+  parts = (int)((tiles + part - 1) / part);
+}
+
+// Whether the scale fits paged_tiles: it multiplies a tile's maximum behind the products, and must be a normal number above 0.
+bool tile_scale(const PagedArgs& a) { return a.scale >= 0x1p-100; }
+
+Plan plan_of(const PagedArgs& a, bool tiled) {
+  Plan p;
+  const int64_t places = a.table_pages * a.page, all = a.tokens * a.group(), each = (a.tokens + a.sequences - 1) / a.sequences * a.group();
+  p.many = tiled && a.dtype != LIMN_HIP_FLOAT32 && all > FEW_ROWS;
+  p.few = !p.many || a.sequences > 1;
+  // paged_token: row tiles of 16 where one holds a sequence's packed rows, else of 32 (where most sequences go to the
+  // other kernel, these are taken to have one token). Up to 64 key tiles go to one workgroup of many waves a row tile while
+  // such workgroups leave waves free; longer caches to workgroups of 4 waves, in parts that give every CU four of them.
+  const int64_t rows = p.many && each > FEW_ROWS ? a.group() : each, tiles = (places + 31) / 32 + 1;
+  p.token.nr = rows <= 16 ? 1 : 2;
+  const int64_t units = a.sequences * a.kv_heads * ((rows + 16 * p.token.nr - 1) / (16 * p.token.nr));
+  p.token.lone = tiles <= 65 && units <= 256;
+  cut(tiles, units, p.token.lone ? 1 : 1024, p.token.parts, p.token.part_tiles);
+  if (p.token.lone) p.token.parts = 1, p.token.part_tiles = (int)tiles;
+  // paged_tiles: two workgroups a CU
+  cut((places + 63) / 64 + 1, (all + 127) / 128 * a.kv_heads, 512, p.tile_parts, p.tile_part);
   return p;
 }
 
 constexpr int64_t align256(int64_t bytes) { return (bytes + 255) / 256 * 256; }
 
-int64_t parts_bytes(const PagedArgs& a, const PagedPlan& p) {
-  return p.parts > 1 ? align256(p.parts * a.tokens * a.heads * a.hd * 4) + align256(p.parts * a.tokens * a.heads * 8) : 0;
+// Enough whatever the call's scale and alignment.
+int64_t workspace_of(const PagedArgs& a) {
+  if (!fast_sizes(a)) return 0;
+  const int64_t tiled = plan_of(a, true).parts(), other = plan_of(a, false).parts(), parts = tiled > other ? tiled : other, rows = a.tokens * a.heads;
+  return parts > 1 ? align256(parts * rows * a.hd * 4) + align256(parts * rows * 8) : 0;
 }
 
-int64_t workspace_of(const PagedArgs& a) { return fast_sizes(a) ? parts_bytes(a, token_plan(a)) : 0; }
-
 int launch_fast(const PagedArgs& a) {
-  const PagedPlan p = token_plan(a);
-  PagedFast f = {a.q, a.k, a.v, a.key_pages, a.value_pages, a.out, nullptr, nullptr, p.parts, p.part_tiles, 0, 0x7fffffff, 16 * p.nr, 32};
-  if (p.parts > 1) {
-    f.totals = (float*)a.workspace;
-    f.stats = (float*)((char*)a.workspace + align256(p.parts * a.tokens * a.heads * a.hd * 4));
+  const Plan p = plan_of(a, tile_scale(a));
+  PagedFast few = {a.q, a.k, a.v, a.key_pages, a.value_pages, a.out, nullptr, nullptr, p.token.parts, p.token.part_tiles, 0, p.many ? FEW_ROWS + 1 : 0x7fffffff, 16 * p.token.nr, 32};
+  if (p.parts() > 1) {  // a row has one kind's partial results: both kinds' share the room
+    few.totals = (float*)a.workspace;
+    few.stats = (float*)((char*)a.workspace + align256(p.parts() * a.tokens * a.heads * a.hd * 4));
   }
-  const int rc = launch_paged_token(a, f, p);
-  return rc == LIMN_HIP_OK && p.parts > 1 ? join(a, f) : rc;
+  PagedFast many = few;
+  many.parts = p.tile_parts;
+  many.part_tiles = p.tile_part;
+  many.few_rows = p.few ? FEW_ROWS + 1 : 0;
+  many.many_rows = 0x7fffffff;
+  many.rows = 128;
+  many.keys = 64;
+  if (!p.few) few.many_rows = 0;
+  int rc = LIMN_HIP_OK;
+  if (p.few) rc = launch_paged_token(a, few, p.token);
+  if (rc == LIMN_HIP_OK && p.many) rc = a.hd <= 64 ? launch_paged_tiles_64(a, many) : a.hd <= 96 ? launch_paged_tiles_96(a, many) : launch_paged_tiles_128(a, many);
+  return rc == LIMN_HIP_OK && p.parts() > 1 ? join(a, few, many) : rc;
 }
 
 }  // namespace

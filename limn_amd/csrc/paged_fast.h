@@ -30,6 +30,9 @@ struct PagedPlan {
 };
 
 int launch_paged_token(const PagedArgs& a, const PagedFast& f, const PagedPlan& p);
+int launch_paged_tiles_64(const PagedArgs& a, const PagedFast& f);
+int launch_paged_tiles_96(const PagedArgs& a, const PagedFast& f);
+int launch_paged_tiles_128(const PagedArgs& a, const PagedFast& f);
 
 // Slots for row tiles of `rows` packed rows: sequence s has those from starts[s] * group / rows + s on, one for every tile
 // that it has and up to one more, so that a slot finds its sequence without a sum over those before it.
@@ -99,6 +102,42 @@ __device__ __forceinline__ void put_rows(const PagedView& v, int s, const Sequen
     if (place < 0) continue;
     *(uint4*)(key_pages + place + d) = *(const uint4*)(k + (q.row0 + i) * v.k_row + d);
     *(uint4*)(value_pages + place + d) = *(const uint4*)(val + (q.row0 + i) * v.v_row + d);
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ bool is_odd(typename T::Storage x) {  // an infinity or a NaN
+  if constexpr (std::is_same<T, F32>::value)
+    return (__float_as_uint(x) & 0x7f800000u) == 0x7f800000u;
+  else
+    return (x & (std::is_same<T, BF16>::value ? 0x7f80 : 0x7c00)) == (std::is_same<T, BF16>::value ? 0x7f80 : 0x7c00);
+}
+
+// Values that are not finite times a weight that has come to 0 (of a key that a row does not see, or a weight below the
+// operand's least number) would be NaN. Where a workgroup finds such values, its products take them as 0, and this adds them
+// to the results as they are stored: an infinity or a NaN times any weight above 0 is itself, and the sum with it. One wave, for the keys
+// [j0, j1) of a sequence and its packed rows [r0, r1), whose stores are done; to partial totals if `totals` is not nullptr.
+template <typename T>
+__device__ __forceinline__ void give_back(const PagedView& v, int s, const Sequence& q, int kvh, int j0, int j1, int held, int r0, int r1, const typename T::Storage* fresh,
+                                          const typename T::Storage* pool, typename T::Storage* out, float* totals) {
+  __threadfence_block();
+  for (int j = j0; j < j1; j++) {
+    const int64_t place = key_place(v, s, kvh, j);
+    if (place < 0) continue;
+    const typename T::Storage* from = j < held ? pool + place : fresh + (q.row0 + j - q.off) * v.v_row;
+    for (int d = threadIdx.x & 63; d < v.hd; d += 64) {
+      const typename T::Storage x = from[d];
+      if (!is_odd<T>(x)) continue;
+      for (int r = r0; r < r1; r++) {
+        const int i = r / v.group;
+        if (q.off + i < j) continue;
+        const int64_t at = (((int64_t)(q.row0 + i) * v.heads + kvh * v.group + r - i * v.group)) * v.hd + d;
+        if (totals != nullptr)
+          totals[at] += T::load(&x, 0);
+        else
+          T::store(out, at, T::load(out, at) + T::load(&x, 0));
+      }
+    }
   }
 }
 

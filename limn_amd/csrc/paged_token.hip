@@ -14,9 +14,8 @@
 //    first part, so one launch does both. Only among them a query may not see a key;
 //  - long caches are cut into parts over workgroups, joined by a second kernel in the order of the parts.
 //
-// Hidden keys' values must not reach a row: a weight of 0 times an infinity or a NaN is NaN. Only the tiles
-// of the new tokens hold such keys; elements there that are not finite go into the product as 0, and to the rows that see
-// them by a loop.
+// Hidden keys' values must not reach a row: a weight of 0 times an infinity or a NaN is NaN. Tiles
+// with keys that some rows do not see are looked over, and all of them where a result is not finite (see give_back).
 
 #include "paged_fast.h"
 
@@ -53,10 +52,6 @@ struct Operands {
       return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
   }
   static __device__ __forceinline__ f32x4 scores(Chunk k, Chunk q, f32x4 c) { return mfma(k.x, q.x, c); }
-  static __device__ __forceinline__ bool odd(u16 x) {
-    constexpr u16 E = std::is_same<T, BF16>::value ? 0x7f80 : 0x7c00;
-    return (x & E) == E;
-  }
   // the weights of a lane's 8 keys as an operand, and the product with their values' element e
   struct Weights {
     u16x8 x;
@@ -87,7 +82,6 @@ struct Operands<F32, W> {
     for (int t = 0; t < 4; t++) c = __builtin_amdgcn_mfma_f32_16x16x4f32(k.x[t], q.x[t], c, 0, 0, 0);
     return c;
   }
-  static __device__ __forceinline__ bool odd(float x) { return (__float_as_uint(x) & 0x7f800000u) == 0x7f800000u; }
   struct Weights {
     float x[8];
   };
@@ -112,6 +106,7 @@ __global__ __launch_bounds__(64 * waves, waves == 4 ? 2 : 1) void paged_token(Pa
   typedef typename O::S S;
   constexpr int PER = O::PER, KS = D / (4 * PER), R = 16 * NR;
   __shared__ float lds[waves * 16 * 17 + waves * NR * 32];
+  __shared__ int found;  // values that are not finite were taken out
   constexpr float UP = std::is_same<T, F16>::value ? 7.f : 0.f;  // float16 weights times 2^7: see shift_of in attend_mfma.h
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15, g = lane >> 4;
   int id = blockIdx.x;
@@ -204,6 +199,10 @@ __global__ __launch_bounds__(64 * waves, waves == 4 ? 2 : 1) void paged_token(Pa
       vr[j] = *(const typename O::Values*)(row != 0xffffffffu && W * n < v.hd ? from + W * n : zeros);
     }
   };
+  if (threadIdx.x == 0) found = 0;
+  __syncthreads();
+  bool careful = false;
+again:
   int kt = first + wave;
   unsigned here = look_up(kt), next = look_up(kt + waves);
   if (kt < last) {
@@ -263,42 +262,15 @@ __global__ __launch_bounds__(64 * waves, waves == 4 ? 2 : 1) void paged_token(Pa
         l[t] += y[t][j];
       }
     }
-    if (partial && pmin != pmax) {
-      // elements that are not finite go into the product as 0, and here to the rows that see them
-      unsigned bad = 0;
+    if (careful || (partial && pmin != pmax)) {  // see give_back
 #pragma unroll
       for (int j = 0; j < 8; j++)
 #pragma unroll
         for (int e = 0; e < W; e++)
-          if (O::odd(vr[j].x[e])) {
-            bad |= 1u << (16 * (j >> 2) + 4 * g + (j & 3));
+          if (is_odd<T>(vr[j].x[e])) {
             vr[j].x[e] = 0;
+            found = 1;
           }
-#pragma unroll
-      for (int o = 1; o < 64; o <<= 1) bad |= __shfl_xor((int)bad, o);
-      while (bad != 0) {
-        const int key = __builtin_ctz(bad);
-        bad &= bad - 1;
-        const S* from = kt < old_tiles ? pool_v + (int64_t)(unsigned)__shfl((int)here, key) * v.hd : fresh_v + (q.row0 + (k0 + key - q.off)) * v.v_row;
-#pragma unroll
-        for (int t = 0; t < NR; t++) {
-          float w = 0.f;
-#pragma unroll
-          for (int j = 0; j < 8; j++) {
-            const float x = __shfl(y[t][j], 16 * ((key >> 2) & 3) + n);
-            if (j == 4 * (key >> 4) + (key & 3)) w = x;
-          }
-          const bool sees = k0 + key <= p[t];
-#pragma unroll
-          for (int i = 0; i < 4; i++)
-#pragma unroll
-            for (int e = 0; e < W; e++) {
-              const int d = W * (4 * g + i) + e;
-              const S x = d < v.hd ? from[d] : S(0);
-              if (sees && O::odd(x)) acc[t][e][i] += w * T::load(&x, 0);
-            }
-        }
-      }
     }
 #pragma unroll
     for (int t = 0; t < NR; t++) {
@@ -309,6 +281,26 @@ __global__ __launch_bounds__(64 * waves, waves == 4 ? 2 : 1) void paged_token(Pa
     if (more) load_v(kt + waves, next);
     here = next;
     next = after;
+  }
+  if (!careful) {
+    float spoiled = 0.f;  // a finite number times 0 stays 0
+#pragma unroll
+    for (int t = 0; t < NR; t++)
+#pragma unroll
+      for (int e = 0; e < W; e++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) spoiled = fmaf(acc[t][e][i], 0.f, spoiled);
+    if (__any(spoiled != 0.f)) {  // once more, every tile's values looked over
+      careful = true;
+#pragma unroll
+      for (int t = 0; t < NR; t++) {
+        m[t] = -__builtin_inff();
+        l[t] = 0.f;
+#pragma unroll
+        for (int e = 0; e < W; e++) acc[t][e] = f32x4{0.f, 0.f, 0.f, 0.f};
+      }
+      goto again;
+    }
   }
 
   // join the waves in order, one 16-dim slice of one row tile at a time
@@ -359,6 +351,9 @@ __global__ __launch_bounds__(64 * waves, waves == 4 ? 2 : 1) void paged_token(Pa
     }
     __syncthreads();
   }
+  if (found != 0 && wave == 0)
+    give_back<T>(v, it.s, q, kvh, begin_of(first), last == tiles ? end : begin_of(last), held, tile * R, min(tile * R + R, rows), fresh_v, pool_v,
+                 (S*)a.out, tiles <= a.part_tiles ? nullptr : a.totals + part * rows_all * v.hd);
 #endif
 }
 
