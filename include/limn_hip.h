@@ -286,7 +286,8 @@ int64_t limn_hip_xent_workspace(int dtype, int64_t rows, int64_t width, int64_t 
  * Rows of no sequence give zeros and write nothing. Positions below 0 (more rows than L) see nothing and give zeros. Of a
  * page number outside [0, pages) the keys are not there: nothing is written, and no query sees them. L is taken as
  * within [0, table_pages * page], starts as within [0, tokens]; a table's entries behind the last position are not read. What
- * a key that a query does not see holds, infinities and NaN among them, changes nothing in its row. Pages that this
+ * a key that a query does not see holds, infinities and NaN among them, changes nothing in its row; an infinite value that it
+ * sees gives an infinity, or NaN where its weight is below float32's least number (float16's, 2^-31). Pages that this
  * call writes to belong to one sequence; others may be shared. q, k, v and out do not overlap the pages.
  * hd at most 256; scale between -2^120 and 2^120; softcap 0 for none, else from 2^-120 to 2^120.
  * `workspace` must hold limn_hip_attend_paged_workspace(...) bytes, 16-byte aligned, for this call alone, as for

@@ -111,35 +111,44 @@ int write_of(const PagedArgs& a) {
 // ---- the tiled kernels ----
 
 // Joins the parts of a sequence: a wave a token and head, the parts' totals brought to the largest reference point and added
-// in their order. A part that saw nothing (no reference point and a sum of 0: it is NaN where a score was) counts nothing.
+// in their order. A part that saw nothing (no reference point and a sum of 0: it is NaN where a score was) counts nothing. A lane
+// has a part's statistics, so that the loads do not wait for one another.
 template <typename T>
-__global__ __launch_bounds__(256) void paged_join(PagedFast few, PagedFast many, PagedView v) {
+__global__ __launch_bounds__(256) void paged_join(PagedFast f, PagedView v) {
   const int lane = threadIdx.x & 63;
   const int64_t id = blockIdx.x * (int64_t)4 + (threadIdx.x >> 6), rows_all = (int64_t)v.tokens * v.heads;
   if (id >= rows_all) return;  // whole waves, and there is no barrier
   const int row = (int)(id / v.heads), s = sequence_of(v, row);
   if (s < 0) return;
   const Sequence q = sequence_at(v, s);
-  const PagedFast& f = q.n * v.group < few.many_rows ? few : many;
   const int tile = ((row - q.row0) * v.group + (int)(id - (int64_t)row * v.heads) % v.group) / f.rows;
   const int parts = (span_of(v, q, tile, f.rows, f.k != nullptr, f.keys).tiles + f.part_tiles - 1) / f.part_tiles;
   if (parts <= 1) return;
   float top = -__builtin_inff();
-  for (int p = 0; p < parts; p++) top = fmaxf(top, f.stats[(p * rows_all + id) * 2]);
+  for (int p = lane; p < parts; p += 64) top = fmaxf(top, f.stats[(p * rows_all + id) * 2]);
+  for (int o = 1; o < 64; o <<= 1) top = fmaxf(top, __shfl_xor(top, o));
   const float base = top == -__builtin_inff() ? 0.f : top;
   float total = 0.f, x[2] = {0.f, 0.f};
-#pragma unroll 4
-  for (int p = 0; p < parts; p++) {
-    const float m = f.stats[(p * rows_all + id) * 2], l = f.stats[(p * rows_all + id) * 2 + 1];
-    if (m == -__builtin_inff() && l == 0.f) continue;
-    const float w = m == -__builtin_inff() ? 1.f : fast_exp2(m - base);
-    total += l * w;
+  for (int p0 = 0; p0 < parts; p0 += 64) {
+    const int many = min(64, parts - p0);
+    float w = 0.f, sum = 0.f;
+    if (lane < many) {
+      const float2 st = *(const float2*)&f.stats[((p0 + lane) * rows_all + id) * 2];
+      w = st.x == -__builtin_inff() ? (st.y == 0.f ? 0.f : 1.f) : fast_exp2(st.x - base);
+      sum = st.x == -__builtin_inff() && st.y == 0.f ? 0.f : st.y * w;
+    }
+    for (int o = 1; o < 64; o <<= 1) sum += __shfl_xor(sum, o);
+    total += sum;
+#pragma unroll 8
+    for (int p = 0; p < many; p++) {
+      const float wp = __shfl(w, p);
 #pragma unroll
-    for (int c = 0; c < 2; c++)
-      if (c * 64 + lane < v.hd) {
-        const float y = f.totals[(p * rows_all + id) * v.hd + c * 64 + lane];
-        x[c] += y - y == 0.f ? w * y : y;  // (an infinity stays one under a weight that has come to 0)
-      }
+      for (int c = 0; c < 2; c++)
+        if (c * 64 + lane < v.hd) {
+          const float y = f.totals[((p0 + p) * rows_all + id) * v.hd + c * 64 + lane];
+          x[c] += y - y == 0.f ? wp * y : y;  // (an infinity stays one under a weight that has come to 0)
+        }
+    }
   }
   const float inv = total == 0.f ? 0.f : 1.f / total;
 #pragma unroll
@@ -187,13 +196,9 @@ int check_buffers(const PagedArgs& a) {
 }
 
 template <typename T>
-int join_of(const PagedArgs& a, const PagedFast& few, const PagedFast& many) {
-  hipLaunchKernelGGL((paged_join<T>), dim3((unsigned)((a.tokens * a.heads + 3) / 4)), dim3(256), 0, a.stream, few, many, paged_view(a));
+int join_of(const PagedArgs& a, const PagedFast& f) {
+  hipLaunchKernelGGL((paged_join<T>), dim3((unsigned)((a.tokens * a.heads + 3) / 4)), dim3(256), 0, a.stream, f, paged_view(a));
   return check_hip(hipGetLastError(), "joining the parts of attention over a paged cache");
-}
-
-int join(const PagedArgs& a, const PagedFast& few, const PagedFast& many) {
-  return a.dtype == LIMN_HIP_FLOAT32 ? join_of<F32>(a, few, many) : a.dtype == LIMN_HIP_FLOAT16 ? join_of<F16>(a, few, many) : join_of<BF16>(a, few, many);
 }
 
 // Sizes that the tiled kernels serve: rows of whole 16-byte chunks; places counted in 32 bits.
@@ -204,80 +209,76 @@ bool fast_sizes(const PagedArgs& a) {
 bool fast_call(const PagedArgs& a) {
   const uintptr_t at = (uintptr_t)a.q | (uintptr_t)a.k | (uintptr_t)a.v | (uintptr_t)a.key_pages | (uintptr_t)a.value_pages | (uintptr_t)a.out;
   const int64_t per = a.dtype == LIMN_HIP_FLOAT32 ? 4 : 8;
-  return fast_sizes(a) && at % 16 == 0 && a.q_row % per == 0 && (a.k == nullptr || (a.k_row % per == 0 && a.v_row % per == 0));
+  return fast_sizes(a) && at % 16 == 0 && a.q_row % per == 0 && (a.k == nullptr || (a.k_row % per == 0 && a.v_row % per == 0 && a.k_row < (1 << 29) && a.v_row < (1 << 29)));
 }
 
-// Sequences of up to FEW_ROWS packed rows go to paged_token, those of more to paged_tiles (half widths).
-constexpr int FEW_ROWS = 64;
-
-// What a call launches: how many sequences have how many rows is known on the device alone, so a call that may have both kinds
-// launches both kernels, each for its own.
+// How a call is run: by paged_tiles (half widths) or paged_token, and in how many parts.
 struct Plan {
-  bool few, many;
-  PagedPlan token;
-  int tile_parts, tile_part;  // paged_tiles: parts at most, key tiles of a part
-  int parts() const { return few && token.parts > tile_parts ? token.parts : many ? tile_parts : token.parts; }
+  bool tiled, lone;
+  int rows, parts, part_tiles;
 };
 
 // parts of `tiles` key tiles that bring `units` workgroups to `fill`, each at least 8 tiles
-void cut(int64_t tiles, int64_t units, int64_t fill, int& parts, int& part) {
-  int64_t p = fill / (units > 1 ? units : 1);
-  if (p > tiles / 8) p = tiles / 8;
-  if (p < 1) p = 1;
-  part = (int)((tiles + p - 1) / p);
-  parts = (int)((tiles + part - 1) / part);
+void cut(Plan& p, int64_t tiles, int64_t units, int64_t fill) {
+  int64_t n = fill / (units > 1 ? units : 1);
+  if (n > tiles / 8) n = tiles / 8;
+  if (n < 1) n = 1;
+  p.part_tiles = (int)((tiles + n - 1) / n);
+  p.parts = (int)((tiles + p.part_tiles - 1) / p.part_tiles);
 }
 
-// Whether the scale fits paged_tiles: it multiplies a tile's maximum behind the products, and must be a normal number above 0.
-bool tile_scale(const PagedArgs& a) { return a.scale >= 0x1p-100; }
+// paged_token takes the calls that have a token a sequence or fewer, or few rows in all; paged_tiles the others, in which
+// any sequence may have many (how many each has is known on the device alone). 24 single tokens beside two parts of 500:
+// 58 us by paged_tiles alone, 73 with a launch of each kernel for its own sequences; 32 single tokens 180 us by paged_tiles, 156 by
+// paged_token.
+constexpr int FEW_ROWS = 64;
 
 Plan plan_of(const PagedArgs& a, bool tiled) {
   Plan p;
   const int64_t places = a.table_pages * a.page, all = a.tokens * a.group(), each = (a.tokens + a.sequences - 1) / a.sequences * a.group();
-  p.many = tiled && a.dtype != LIMN_HIP_FLOAT32 && all > FEW_ROWS;
-  p.few = !p.many || a.sequences > 1;
-  // paged_token: row tiles of 16 where one holds a sequence's packed rows, else of 32 (where most sequences go to the
-  // other kernel, these are taken to have one token). Up to 64 key tiles go to one workgroup of many waves a row tile while
-  // such workgroups leave waves free; longer caches to workgroups of 4 waves, in parts that give every CU four of them.
-  const int64_t rows = p.many && each > FEW_ROWS ? a.group() : each, tiles = (places + 31) / 32 + 1;
-  p.token.nr = rows <= 16 ? 1 : 2;
-  const int64_t units = a.sequences * a.kv_heads * ((rows + 16 * p.token.nr - 1) / (16 * p.token.nr));
-  p.token.lone = tiles <= 65 && units <= 256;
-  cut(tiles, units, p.token.lone ? 1 : 1024, p.token.parts, p.token.part_tiles);
-  if (p.token.lone) p.token.parts = 1, p.token.part_tiles = (int)tiles;
-  // paged_tiles: two workgroups a CU
-  cut((places + 63) / 64 + 1, (all + 127) / 128 * a.kv_heads, 512, p.tile_parts, p.tile_part);
+  p.tiled = tiled && a.dtype != LIMN_HIP_FLOAT32 && a.tokens > a.sequences && all > FEW_ROWS;
+  p.lone = false;
+  if (p.tiled) {  // (24 single tokens beside two parts of 500, in parts for 256, 512, 768 and 1024 workgroups: 96, 70, 53 and 63 us)
+    p.rows = 128;
+    cut(p, (places + 63) / 64 + 1, (a.sequences + all / 128) * a.kv_heads, 768);
+    return p;
+  }
+  // Row tiles of 16 where one holds a sequence's packed rows, else of 32. Up to 64 key tiles go to one workgroup of many waves a
+  // row tile while such workgroups leave waves free; longer caches to workgroups of 4 waves, two a CU. (32 tokens over up to 8192
+  // positions, 8 key heads, in parts for 512, 768, 1024 and 2048 workgroups: 156, 172, 167 and 185 us.)
+  const int64_t tiles = (places + 31) / 32 + 1;
+  p.rows = each <= 16 ? 16 : 32;
+  const int64_t units = a.sequences * a.kv_heads * ((each + p.rows - 1) / p.rows);
+  p.lone = tiles <= 65 && units <= 256;
+  cut(p, tiles, units, p.lone ? 1 : 512);
   return p;
 }
 
 constexpr int64_t align256(int64_t bytes) { return (bytes + 255) / 256 * 256; }
 
+// Whether the scale fits paged_tiles: it multiplies a tile's maximum behind the products, and must be a normal number above 0.
+bool tile_scale(const PagedArgs& a) { return a.scale >= 0x1p-100; }
+
 // Enough whatever the call's scale and alignment.
 int64_t workspace_of(const PagedArgs& a) {
   if (!fast_sizes(a)) return 0;
-  const int64_t tiled = plan_of(a, true).parts(), other = plan_of(a, false).parts(), parts = tiled > other ? tiled : other, rows = a.tokens * a.heads;
+  const int64_t tiled = plan_of(a, true).parts, other = plan_of(a, false).parts, parts = tiled > other ? tiled : other, rows = a.tokens * a.heads;
   return parts > 1 ? align256(parts * rows * a.hd * 4) + align256(parts * rows * 8) : 0;
 }
 
 int launch_fast(const PagedArgs& a) {
   const Plan p = plan_of(a, tile_scale(a));
-  PagedFast few = {a.q, a.k, a.v, a.key_pages, a.value_pages, a.out, nullptr, nullptr, p.token.parts, p.token.part_tiles, 0, p.many ? FEW_ROWS + 1 : 0x7fffffff, 16 * p.token.nr, 32};
-  if (p.parts() > 1) {  // a row has one kind's partial results: both kinds' share the room
-    few.totals = (float*)a.workspace;
-    few.stats = (float*)((char*)a.workspace + align256(p.parts() * a.tokens * a.heads * a.hd * 4));
+  PagedFast f = {a.q, a.k, a.v, a.key_pages, a.value_pages, a.out, nullptr, nullptr, p.parts, p.part_tiles, p.rows, p.tiled ? 64 : 32};
+  if (p.parts > 1) {
+    f.totals = (float*)a.workspace;
+    f.stats = (float*)((char*)a.workspace + align256(p.parts * a.tokens * a.heads * a.hd * 4));
   }
-  PagedFast many = few;
-  many.parts = p.tile_parts;
-  many.part_tiles = p.tile_part;
-  many.few_rows = p.few ? FEW_ROWS + 1 : 0;
-  many.many_rows = 0x7fffffff;
-  many.rows = 128;
-  many.keys = 64;
-  if (!p.few) few.many_rows = 0;
-  int rc = LIMN_HIP_OK;
-  if (p.few) rc = launch_paged_token(a, few, p.token);
-  if (rc == LIMN_HIP_OK && p.many) rc = a.hd <= 64 ? launch_paged_tiles_64(a, many) : a.hd <= 96 ? launch_paged_tiles_96(a, many) : launch_paged_tiles_128(a, many);
-  return rc == LIMN_HIP_OK && p.parts() > 1 ? join(a, few, many) : rc;
+  const int rc = !p.tiled        ? launch_paged_token(a, f, p.lone)
+                 : a.hd <= 64 ? launch_paged_tiles_64(a, f)
+                 : a.hd <= 96 ? launch_paged_tiles_96(a, f)
+                              : launch_paged_tiles_128(a, f);
+  if (rc != LIMN_HIP_OK || p.parts == 1) return rc;
+  return a.dtype == LIMN_HIP_FLOAT32 ? join_of<F32>(a, f) : a.dtype == LIMN_HIP_FLOAT16 ? join_of<F16>(a, f) : join_of<BF16>(a, f);
 }
 
 }  // namespace

@@ -18,18 +18,11 @@ struct PagedFast {
   void* out;
   float* totals;  // of sequences with more than one part: (parts, tokens * heads, hd)
   float* stats;   // (parts, tokens * heads, 2): the reference point of the exponentials in log2, and their sum
-  int parts, part_tiles;    // parts at most; key tiles of a part
-  int few_rows, many_rows;  // the sequences of this launch: those with few_rows <= packed rows of a key head < many_rows
-  int rows, keys;           // a row tile's packed rows, a key tile's keys
+  int parts, part_tiles;  // parts at most; key tiles of a part
+  int rows, keys;         // a row tile's packed rows, a key tile's keys
 };
 
-struct PagedPlan {
-  int nr;     // paged_token: row tiles of 16 nr
-  bool lone;  // paged_token: one workgroup of many waves a row tile
-  int parts, part_tiles;
-};
-
-int launch_paged_token(const PagedArgs& a, const PagedFast& f, const PagedPlan& p);
+int launch_paged_token(const PagedArgs& a, const PagedFast& f, bool lone);  // lone: one workgroup of many waves a row tile
 int launch_paged_tiles_64(const PagedArgs& a, const PagedFast& f);
 int launch_paged_tiles_96(const PagedArgs& a, const PagedFast& f);
 int launch_paged_tiles_128(const PagedArgs& a, const PagedFast& f);
@@ -43,6 +36,12 @@ namespace {
 constexpr float PAGED_LOG2E = ATT_LOG2E;
 __device__ __attribute__((aligned(16))) const float paged_zeros[128] = {};  // what a lane reads of a key that is not there
 
+// An address, or that of zeros where there is nothing. By masks: a choice of pointers becomes a branch for every load.
+__device__ __forceinline__ uint64_t or_zeros(bool there, uint64_t at) {
+  const uint64_t mask = (uint64_t)0 - (uint64_t)there;
+  return (at & mask) | ((uint64_t)paged_zeros & ~mask);
+}
+
 // A tile of packed rows of one sequence.
 struct Item {
   bool live;
@@ -55,13 +54,12 @@ __device__ __forceinline__ int slot_of(const PagedView& v, int s, int rows) {
 }
 
 // The tile of a slot: the last sequence whose slots begin at or before it.
-__device__ __forceinline__ Item item_at(const PagedView& v, int slot, int rows, int few, int many) {
+__device__ __forceinline__ Item item_at(const PagedView& v, int slot, int rows) {
   Item it;
   it.s = last_sequence(v, slot, [&](int i) { return slot_of(v, i, rows); });
   it.tile = slot - slot_of(v, it.s, rows);
   it.seq = sequence_at(v, it.s);
-  const int all = it.seq.n * v.group;
-  it.live = it.tile >= 0 && (int64_t)it.tile * rows < all && all >= few && all < many;
+  it.live = it.tile >= 0 && (int64_t)it.tile * rows < it.seq.n * v.group;
   return it;
 }
 
@@ -113,10 +111,11 @@ __device__ __forceinline__ bool is_odd(typename T::Storage x) {  // an infinity 
     return (x & (std::is_same<T, BF16>::value ? 0x7f80 : 0x7c00)) == (std::is_same<T, BF16>::value ? 0x7f80 : 0x7c00);
 }
 
-// Values that are not finite times a weight that has come to 0 (of a key that a row does not see, or a weight below the
-// operand's least number) would be NaN. Where a workgroup finds such values, its products take them as 0, and this adds them
-// to the results as they are stored: an infinity or a NaN times any weight above 0 is itself, and the sum with it. One wave, for the keys
-// [j0, j1) of a sequence and its packed rows [r0, r1), whose stores are done; to partial totals if `totals` is not nullptr.
+// A weight of 0 of a key that a row does not see, times a value that is not finite, would be NaN. So tiles of keys that some
+// rows do not see have their values looked over; what is not finite there goes into the products as 0, and this adds it to
+// the results as they are stored, for the rows that see it: an infinity or a NaN times any weight above 0 is itself, and the sum with it.
+// One wave, for the keys [j0, j1) of a sequence and its packed rows [r0, r1), whose stores are done; to partial totals if
+// `totals` is not nullptr.
 template <typename T>
 __device__ __forceinline__ void give_back(const PagedView& v, int s, const Sequence& q, int kvh, int j0, int j1, int held, int r0, int r1, const typename T::Storage* fresh,
                                           const typename T::Storage* pool, typename T::Storage* out, float* totals) {

@@ -79,7 +79,7 @@ __global__ __launch_bounds__(THREADS, 2) void paged_tiles(PagedFast a, PagedView
   id /= v.kv_heads;
   const int part = id % a.parts, slot = slots - 1 - id / a.parts;  // the last rows of a sequence see the most keys: they go first
   zero_idle(v, (u16*)a.out, THREADS);
-  const Item it = item_at(v, slot, ATT_ROWS, a.few_rows, a.many_rows);
+  const Item it = item_at(v, slot, ATT_ROWS);
   if (!it.live) return;
   const Sequence& q = it.seq;
   const Rules r = paged_rules(v);
@@ -94,7 +94,7 @@ __global__ __launch_bounds__(THREADS, 2) void paged_tiles(PagedFast a, PagedView
   if (part > 0 && first >= span.tiles) return;
 
   const int w0 = tile * ATT_ROWS + wave * 32, row = w0 + n;  // packed rows of the sequence and key head
-  const bool there = row < rows;
+  const bool there = row < rows, idle = w0 >= rows;  // a wave without rows copies and looks over its part of the tiles alone
   const int i = (there ? row : 0) / group, head = kvh * group + (there ? row - i * group : 0), p = q.off + i;
   const int64_t at = (int64_t)(q.row0 + i) * v.heads + head;
   const int p_wave = q.off + min(w0, rows - 1) / group, p_block = q.off + tile * ATT_ROWS / group;  // the first rows' positions
@@ -123,21 +123,21 @@ __global__ __launch_bounds__(THREADS, 2) void paged_tiles(PagedFast a, PagedView
   };
   auto copy = [&](u16* to, const u16* pool, const u16* fresh, int64_t fresh_row, int t, unsigned places) __attribute__((always_inline)) {
     const bool old = t < span.old_tiles;
-    const u16* base = old ? pool : fresh + (q.row0 + begin_of(t) - q.off) * fresh_row;
-    const int64_t stride = old ? hd : fresh_row;
+    const uint64_t base = (uint64_t)(old ? pool : fresh + (q.row0 + begin_of(t) - q.off) * fresh_row);
+    const unsigned stride = (unsigned)(old ? hd : fresh_row) * 2u;
+    unsigned place[PASSES];
+#pragma unroll
+    for (int x = 0; x < PASSES; x++) place[x] = (unsigned)__shfl((int)places, (x * WAVES + wave) * RPI + lane / CPR);
 #pragma unroll
     for (int x = 0; x < PASSES; x++) {
       const int kr = (x * WAVES + wave) * RPI + lane / CPR, c = (lane % CPR) ^ Reads::swizzle(kr);
-      const unsigned place = (unsigned)__shfl((int)places, kr);
-      const u16* from = place != 0xffffffffu && c * 8 < hd ? base + (old ? place : (unsigned)kr) * stride + c * 8 : (const u16*)paged_zeros;
+      const uint64_t from = or_zeros(place[x] != 0xffffffffu && c * 8 < hd, base + (uint64_t)(old ? place[x] : (unsigned)kr) * stride + c * 16);
       __builtin_amdgcn_global_load_lds((global_void*)from, (lds_void*)((char*)to + (x * WAVES + wave) * 1024), 16, 0, 0);
     }
   };
-  // this wave's rows of a tile of values, looked over (see give_back): of the tiles that some rows of the block do not see
-  // whole, and of every tile once the results are not finite
-  bool careful = false;
+  // this wave's rows of a tile of values that some rows of the block do not see whole, looked over (see give_back)
   auto look_over = [&](u16* tile_v, int t) __attribute__((always_inline)) {
-    if (!careful && begin_of(t) + TILE - 1 <= p_block) return;
+    if (begin_of(t) + TILE - 1 <= p_block) return;
 #pragma unroll
     for (int x = 0; x < PASSES; x++) {
       u16x8* mine = (u16x8*)((char*)tile_v + (x * WAVES + wave) * 1024) + lane;
@@ -205,6 +205,7 @@ __global__ __launch_bounds__(THREADS, 2) void paged_tiles(PagedFast a, PagedView
   };
   // a tile's probabilities (its scores in s) and V product, beside the next tile's scores
   auto pipe = [&](auto has_next, const u16* Kn, const u16* Vc, int t, uint64_t good) __attribute__((always_inline)) {
+    if (idle) return;
     f32x16 sn[2];
     if (decltype(has_next)::value) scores(Kn, sn);
     const float base = (m == neg_inf() ? 0.f : m * unit) - UP;
@@ -235,8 +236,7 @@ __global__ __launch_bounds__(THREADS, 2) void paged_tiles(PagedFast a, PagedView
   const int count = last - first;
   if (threadIdx.x == 0) found = 0;
   __syncthreads();
-  for (;;) {
-    if (count <= 0) break;
+  if (count > 0) {
     // tile it's K and V are in buffers it % 2; K goes two tiles ahead, V one, the table three
     int t = first;
     const unsigned place0 = look_up(t);
@@ -247,8 +247,11 @@ __global__ __launch_bounds__(THREADS, 2) void paged_tiles(PagedFast a, PagedView
     __builtin_amdgcn_s_waitcnt(WAIT_VMEM);
     look_over(V0, t);
     __syncthreads();
-    scores(K0, s);
-    look(s, begin_of(t), __ballot(place0 != 0xffffffffu));
+    const uint64_t good0 = __ballot(place0 != 0xffffffffu);
+    if (!idle) {
+      scores(K0, s);
+      look(s, begin_of(t), good0);
+    }
     __syncthreads();  // every wave's reads of K buffer 0 are done before the third tile is copied there
     auto step = [&](const u16* Kn, const u16* Vc, u16* Kf, u16* Vf) __attribute__((always_inline)) {
       copy(Kf, pool_k, fresh_k, v.k_row, t + 2, place2);
@@ -273,15 +276,9 @@ __global__ __launch_bounds__(THREADS, 2) void paged_tiles(PagedFast a, PagedView
     } else {
       pipe(std::false_type{}, K0, V0, t, 0);
     }
-    const bool spoiled = any_odd(acc);  // a barrier: the tile buffers are free
-    if (careful || !spoiled) break;
-    careful = true;
-    m = neg_inf();
-    l = 0.f;
-#pragma unroll
-    for (int dt = 0; dt < DT; dt++) acc[dt] = zero16();
   }
   const float total = pair_sum(l);
+  __syncthreads();  // the tile buffers become staging below
   __syncthreads();  // the tile buffers become staging below
   // the keys of this part, for what was taken out of their values
   const int j0 = begin_of(first), j1 = last == span.tiles ? span.end : begin_of(last);

@@ -15,7 +15,7 @@
 //  - long caches are cut into parts over workgroups, joined by a second kernel in the order of the parts.
 //
 // Hidden keys' values must not reach a row: a weight of 0 times an infinity or a NaN is NaN. Tiles
-// with keys that some rows do not see are looked over, and all of them where a result is not finite (see give_back).
+// with keys that some rows do not see are looked over (see give_back).
 
 #include "paged_fast.h"
 
@@ -114,7 +114,7 @@ __global__ __launch_bounds__(64 * waves, waves == 4 ? 2 : 1) void paged_token(Pa
   id /= v.kv_heads;
   const int part = id % a.parts, slot = id / a.parts;
   zero_idle(v, (S*)a.out, 64 * waves);
-  const Item it = item_at(v, slot, R, a.few_rows, a.many_rows);
+  const Item it = item_at(v, slot, R);
   if (!it.live) return;
   const Sequence& q = it.seq;
   const PagedRules r = paged_rules(v);
@@ -159,7 +159,6 @@ __global__ __launch_bounds__(64 * waves, waves == 4 ? 2 : 1) void paged_token(Pa
 
   const S* pool_k = (const S*)a.key_pages;
   const S* pool_v = (const S*)a.value_pages;
-  const S* zeros = (const S*)paged_zeros;
   typename O::Chunk kr[2][KS];
   typename O::Values vr[8];
   // a tile: its keys from k0 on, up to k1; from the pages if it is an old one
@@ -176,33 +175,29 @@ __global__ __launch_bounds__(64 * waves, waves == 4 ? 2 : 1) void paged_token(Pa
   };
   auto load_k = [&](int kt, unsigned rows_) __attribute__((always_inline)) {
     const bool old = kt < old_tiles;
-    const int k0 = begin_of(kt);
+    const uint64_t base = (uint64_t)(old ? pool_k : fresh_k + (q.row0 + begin_of(kt) - q.off) * v.k_row) + 16 * g;
+    const unsigned stride = (unsigned)(old ? v.hd : v.k_row) * (unsigned)sizeof(S);
 #pragma unroll
     for (int t = 0; t < 2; t++) {
       const unsigned row = __shfl((int)rows_, 16 * t + n);
-      const S* from = old ? pool_k + (int64_t)row * v.hd : fresh_k + (q.row0 + (k0 + 16 * t + n - q.off)) * v.k_row;
+      const uint64_t from = base + (uint64_t)(old ? row : (unsigned)(16 * t + n)) * stride;
 #pragma unroll
-      for (int s = 0; s < KS; s++) {
-        const int d = PER * (4 * s + g);
-        kr[t][s] = *(const typename O::Chunk*)(row != 0xffffffffu && d < v.hd ? from + d : zeros);
-      }
+      for (int s = 0; s < KS; s++) kr[t][s] = *(const typename O::Chunk*)or_zeros(row != 0xffffffffu && PER * (4 * s + g) < v.hd, from + 64 * s);
     }
   };
   auto load_v = [&](int kt, unsigned rows_) __attribute__((always_inline)) {
     const bool old = kt < old_tiles;
-    const int k0 = begin_of(kt);
+    const uint64_t base = (uint64_t)(old ? pool_v : fresh_v + (q.row0 + begin_of(kt) - q.off) * v.v_row) + sizeof(typename O::Values) * n;
+    const unsigned stride = (unsigned)(old ? v.hd : v.v_row) * (unsigned)sizeof(S);
 #pragma unroll
     for (int j = 0; j < 8; j++) {
       const int key = 16 * (j >> 2) + 4 * g + (j & 3);
       const unsigned row = __shfl((int)rows_, key);
-      const S* from = old ? pool_v + (int64_t)row * v.hd : fresh_v + (q.row0 + (k0 + key - q.off)) * v.v_row;
-      vr[j] = *(const typename O::Values*)(row != 0xffffffffu && W * n < v.hd ? from + W * n : zeros);
+      vr[j] = *(const typename O::Values*)or_zeros(row != 0xffffffffu && W * n < v.hd, base + (uint64_t)(old ? row : (unsigned)key) * stride);
     }
   };
   if (threadIdx.x == 0) found = 0;
   __syncthreads();
-  bool careful = false;
-again:
   int kt = first + wave;
   unsigned here = look_up(kt), next = look_up(kt + waves);
   if (kt < last) {
@@ -262,7 +257,7 @@ again:
         l[t] += y[t][j];
       }
     }
-    if (careful || (partial && pmin != pmax)) {  // see give_back
+    if (partial && pmin != pmax) {  // see give_back
 #pragma unroll
       for (int j = 0; j < 8; j++)
 #pragma unroll
@@ -282,27 +277,6 @@ again:
     here = next;
     next = after;
   }
-  if (!careful) {
-    float spoiled = 0.f;  // a finite number times 0 stays 0
-#pragma unroll
-    for (int t = 0; t < NR; t++)
-#pragma unroll
-      for (int e = 0; e < W; e++)
-#pragma unroll
-        for (int i = 0; i < 4; i++) spoiled = fmaf(acc[t][e][i], 0.f, spoiled);
-    if (__any(spoiled != 0.f)) {  // once more, every tile's values looked over
-      careful = true;
-#pragma unroll
-      for (int t = 0; t < NR; t++) {
-        m[t] = -__builtin_inff();
-        l[t] = 0.f;
-#pragma unroll
-        for (int e = 0; e < W; e++) acc[t][e] = f32x4{0.f, 0.f, 0.f, 0.f};
-      }
-      goto again;
-    }
-  }
-
   // join the waves in order, one 16-dim slice of one row tile at a time
   float* sm = lds + waves * 16 * 17;
 #pragma unroll
@@ -375,15 +349,15 @@ int launch_token(const PagedArgs& a, const PagedFast& f, bool lone) {
 }
 
 template <typename T>
-int launch_token_type(const PagedArgs& a, const PagedFast& f, const PagedPlan& p) {
-  if (a.hd <= 64) return p.nr == 1 ? launch_token<T, 64, 1>(a, f, p.lone) : launch_token<T, 64, 2>(a, f, p.lone);
-  return p.nr == 1 ? launch_token<T, 128, 1>(a, f, p.lone) : launch_token<T, 128, 2>(a, f, p.lone);
+int launch_token_type(const PagedArgs& a, const PagedFast& f, bool lone) {
+  if (a.hd <= 64) return f.rows == 16 ? launch_token<T, 64, 1>(a, f, lone) : launch_token<T, 64, 2>(a, f, lone);
+  return f.rows == 16 ? launch_token<T, 128, 1>(a, f, lone) : launch_token<T, 128, 2>(a, f, lone);
 }
 
 }  // namespace
 
-int launch_paged_token(const PagedArgs& a, const PagedFast& f, const PagedPlan& p) {
-  return a.dtype == LIMN_HIP_FLOAT32 ? launch_token_type<F32>(a, f, p) : a.dtype == LIMN_HIP_FLOAT16 ? launch_token_type<F16>(a, f, p) : launch_token_type<BF16>(a, f, p);
+int launch_paged_token(const PagedArgs& a, const PagedFast& f, bool lone) {
+  return a.dtype == LIMN_HIP_FLOAT32 ? launch_token_type<F32>(a, f, lone) : a.dtype == LIMN_HIP_FLOAT16 ? launch_token_type<F16>(a, f, lone) : launch_token_type<BF16>(a, f, lone);
 }
 
 }  // namespace limn

@@ -21,11 +21,20 @@ import numpy as np
 from oracle.attend import F, HALF_STEP, LEAST, TINY, _product
 
 
+def same_kind(got, want):
+    """got with NaN where want says NaN and got has an infinity: what an infinite value gives under a weight that may be 0."""
+    return np.where(np.isnan(want) & np.isinf(got), np.nan, got)
+
+
 PAST = {"float32": 2.0**128, "bfloat16": 2.0**128 * (1 - 2.0**-9), "float16": 65520.0}  # from here on a number rounds to infinity
 
 
 def paged(q, k, v, key_pages, value_pages, starts, lengths, table, *, softcap=0.0, slopes=None, scale=None, dtype="float32"):
-    """out (tokens, heads, hd) with its bound, and the pages as the call leaves them: (out, bound), key_pages, value_pages."""
+    """out (tokens, heads, hd) with its bound, and the pages as the call leaves them: (out, bound), key_pages, value_pages. An infinity
+    in out is given as NaN where one of the infinite values that make it has a weight which may come to 0 as an operand or beside a
+    larger score of another part, below 2^-31 for float16 (2^-25, half its least number, and 2^7 that weights are multiplied by, and
+    one bit for the weight's error), 2^-124 else (float32's least normal number and two bits): 0 times an infinity is NaN, so a kernel may
+    give either there (see `same_kind`)."""
     tokens, heads, hd = q.shape
     pages, kv_heads, page, _ = key_pages.shape
     scale = hd**-0.5 if scale is None else scale
@@ -74,6 +83,8 @@ def paged(q, k, v, key_pages, value_pages, starts, lengths, table, *, softcap=0.
                 p = np.where(total == 0, 0.0, w / np.where(total == 0, 1.0, total))
                 rel = 2 * np.max(np.where(seen, err, 0.0), axis=1, keepdims=True, initial=0.0) + (n + 16) * F
                 out[b:e, h] = _product(p, Vh)
+                faint = seen & (w < (2.0**-31 if dtype == "float16" else 2.0**-124) * np.maximum(total, 1.0))
+                out[b:e, h] = np.where(np.isinf(out[b:e, h]) & (faint.astype(float) @ (~np.isfinite(Vh)) > 0), np.nan, out[b:e, h])
                 off[b:e, h] = (rel + operand) * (p @ fine(Vh)) + (TINY + small * 2.0**-32) * (seen @ fine(Vh)) + u * fine(out[b:e, h]) + least
     return (out, off), keys, values
 

@@ -12,7 +12,7 @@ from limn_amd.hip import runtime
 from limn_amd.paged import attend_paged
 from limn_amd.seam import Tensor, capture, float32, int32, realize, use_device
 from oracle.attend import within
-from oracle.serving import paged
+from oracle.serving import paged, same_kind
 from serving import paged_inputs
 
 pytestmark = pytest.mark.gpu
@@ -65,7 +65,7 @@ def called(dev, x, dtype, softcap=0.0, scale=None, apart=0, shift=0):
 def check(dev, x, dtype, softcap=0.0, scale=None, **kw):
     got = called(dev, x, dtype, softcap, scale, **kw)
     (want, bound), keys, values = paged(**x, softcap=softcap, scale=scale, dtype=dtype)
-    within(got["out"], want, bound, f"out {dtype}")
+    within(same_kind(got["out"], want), want, bound, f"out {dtype}")
     np.testing.assert_array_equal(got["keys"], keys)
     np.testing.assert_array_equal(got["values"], values)
     return got
