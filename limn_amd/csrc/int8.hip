@@ -3,15 +3,25 @@
 //
 //   s = max(max |x| / 127, 2^-126),  x8 = round(x / s) (ties to even),  y = (x8 . w8) s scale + bias.
 //
-// Sums of products are whole numbers in 32 bits, exact up to 2^17 terms of 127 * 128. The product runs on
-// v_mfma_i32_32x32x32_i8 in the tiles of matmul.hip's DMA kernel, with bytes where that has 16-bit elements: rows of 128
-// bytes a stage, 16-byte chunk c of LDS row r at position c ^ ((r >> 1) & 7), copied straight to LDS, the next stage in
-// flight while one is multiplied. Rows of x8 are padded with zeros to whole stages, so what a stage holds of a weight's next
-// row is multiplied by 0; rows past an operand's end read as zeros.
+// Sums of products are whole numbers in 32 bits, exact up to 2^17 terms of 127 * 128, so any order of adding gives the same.
+// Rows of x8 are padded with zeros to whole multiples of 256 bytes: what a stage holds of a weight's next row is multiplied by 0, and
+// rows past an operand's end read as zeros, so the loops have no tests of bounds.
+//
+// int8_tiles (many rows; bound by the matrix cores): output tiles of 256 x 256, 128 x 128 or 64 x 64 on 4 waves, one a SIMD, each
+// with a quarter as accumulators of v_mfma_i32_32x32x32_i8. A wave's 128 x 128 takes 8 reads of LDS for 16 products, half
+// of what 8 waves of 128 x 64 do, whose LDS was busy all the time. Stages of 64 bytes a row go straight to LDS
+// (buffer_load ... lds) into one of four buffers, three stages ahead; chunk c of LDS row r lies at c ^ ((r >> 3) & 3), so that the 16
+// rows a read serves in a cycle (those of one parity of r >> 2 in 32) are in 16 places of the 64 banks. Operands are read a k
+// step ahead, the last one's of a stage in the next stage, which has landed by then.
+//
+// int8_few (up to 64 rows; bound by reading the weight once): a wave has 16 outputs and a part of the width, its bytes read from
+// memory straight into operands of v_mfma_i32_16x16x64_i8; the waves of a workgroup add their sums in LDS.
 
 #include "common.h"
 
 #include <math.h>
+
+#include <type_traits>
 
 namespace limn {
 namespace {
@@ -20,8 +30,11 @@ typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef int i32x16 __attribute__((ext_vector_type(16)));
 typedef __attribute__((address_space(3))) void lds_void;
 
-constexpr int STAGE = 128;          // bytes of a row that a stage holds
-constexpr int WAIT_VMEM = 0x0F70;   // s_waitcnt: every vector memory operation done, the other counters free
+constexpr int PAD = 256;     // rows of x8 are padded to whole multiples of this: four stages
+constexpr int STAGE = 64;    // bytes of a row that a stage of int8_tiles holds
+
+// the s_waitcnt immediate that leaves the newest n vector memory operations in flight, and the other counters free
+constexpr int wait_vm(int n) { return 0x0F70 | (n & 15) | ((n >> 4) << 14); }
 
 struct Int8Args {
   const void* x;
@@ -33,7 +46,7 @@ struct Int8Args {
   int64_t rows, width, outputs;
   void* workspace;
   hipStream_t stream;
-  int64_t padded() const { return (width + STAGE - 1) / STAGE * STAGE; }
+  int64_t padded() const { return (width + PAD - 1) / PAD * PAD; }
 };
 
 constexpr int64_t align256(int64_t bytes) { return (bytes + 255) / 256 * 256; }
@@ -41,40 +54,86 @@ constexpr int64_t align256(int64_t bytes) { return (bytes + 255) / 256 * 256; }
 // The copy of the weight with aligned rows that a call needs where its rows are not.
 bool needs_copy(const void* w, int64_t width) { return width % 16 != 0 || (uintptr_t)w % 16 != 0; }
 
-// A workgroup a row: its largest magnitude, then its numbers, `stride` bytes a row, zeros behind the width. A row with an
-// infinity or a NaN gets the scale NaN and zeros.
+// 8 consecutive elements
 template <typename T>
-__global__ __launch_bounds__(256) void quantize_rows(const typename T::Storage* __restrict__ x, signed char* __restrict__ out, float* __restrict__ scales,
-                                                     int64_t width, int64_t stride) {
+struct Eight {
+  u16x8 x;
+  __device__ __forceinline__ void load(const u16* p) { x = *(const u16x8*)p; }
+  __device__ __forceinline__ float at(int i) const { return T::unpack(x[i]); }
+};
+template <>
+struct Eight<F32> {
+  f32x4 lo, hi;
+  __device__ __forceinline__ void load(const float* p) {
+    lo = *(const f32x4*)p;
+    hi = *(const f32x4*)(p + 4);
+  }
+  __device__ __forceinline__ float at(int i) const { return i < 4 ? lo[i & 3] : hi[i & 3]; }
+};
+
+constexpr int HELD = 4;  // eights a thread of quantize_rows holds between its two uses: 8192 elements a row
+
+// A workgroup a row: its largest magnitude, then its numbers, `stride` bytes a row, zeros behind the width. A row with an
+// infinity or a NaN gets the scale NaN and zeros. With `vec` (rows of whole aligned eights) the row's first 8192 elements are read
+// once. Workgroups past the rows copy a weight's rows, `w_width` bytes, to w_out with zeros behind.
+template <typename T>
+__global__ __launch_bounds__(256) void quantize_rows(const typename T::Storage* __restrict__ x, signed char* __restrict__ out, float* __restrict__ scales, int64_t rows, int64_t width,
+                                                     int64_t stride, int vec, const signed char* __restrict__ w, signed char* __restrict__ w_out, int64_t outputs) {
   __shared__ float tops[4];
+  if (blockIdx.x >= rows) {
+    for (int64_t r = blockIdx.x - rows; r < outputs; r += gridDim.x - rows)
+      for (int64_t i = threadIdx.x; i < stride; i += 256) w_out[r * stride + i] = i < width ? w[r * width + i] : 0;
+    return;
+  }
   const typename T::Storage* row = x + blockIdx.x * width;
+  signed char* o = out + blockIdx.x * stride;
   float top = 0.f, odd = 0.f;
-  for (int64_t i = threadIdx.x; i < width; i += 256) {
-    const float v = T::load(row, i);
+  Eight<T> held[HELD];
+  auto look = [&](float v) __attribute__((always_inline)) {
     top = fmaxf(top, fabsf(v));
     odd = fmaf(v, 0.f, odd);  // NaN once an infinity or a NaN was there
-  }
+  };
+  const int64_t eights = vec ? width / 8 : 0;
+#pragma unroll
+  for (int h = 0; h < HELD; h++)
+    if (h * 256 + threadIdx.x < eights) held[h].load(row + (h * 256 + threadIdx.x) * 8);
+#pragma unroll
+  for (int h = 0; h < HELD; h++)
+    if (h * 256 + threadIdx.x < eights) {
+#pragma unroll
+      for (int i = 0; i < 8; i++) look(held[h].at(i));
+    }
+  for (int64_t i = (vec ? HELD * 2048 : 0) + threadIdx.x; i < width; i += 256) look(T::load(row, i));
   if (odd != odd) top = __builtin_inff();
-  for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
+#pragma unroll
+  for (int m = 1; m < 64; m <<= 1) top = fmaxf(top, __shfl_xor(top, m));
   if ((threadIdx.x & 63) == 0) tops[threadIdx.x >> 6] = top;
   __syncthreads();
   top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
   const bool fine = top < __builtin_inff();
   const float s = fmaxf(top / 127.f, 0x1p-126f);
   if (threadIdx.x == 0) scales[blockIdx.x] = fine ? s : __builtin_nanf("");
-  signed char* o = out + blockIdx.x * stride;
-  for (int64_t i = threadIdx.x; i < stride; i += 256) o[i] = fine && i < width ? (signed char)(int)rintf(T::load(row, i) / s) : 0;
-}
-
-__global__ __launch_bounds__(256) void pad_rows(const signed char* __restrict__ w, signed char* __restrict__ out, int64_t width, int64_t stride) {
-  for (int64_t i = threadIdx.x; i < stride; i += 256) out[blockIdx.x * stride + i] = i < width ? w[blockIdx.x * width + i] : 0;
+  auto round8 = [&](float v) __attribute__((always_inline)) { return fine ? (int)rintf(v / s) : 0; };
+#pragma unroll
+  for (int h = 0; h < HELD; h++)
+    if (h * 256 + threadIdx.x < eights) {
+      unsigned lo = 0, hi = 0;
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        lo |= ((unsigned)round8(held[h].at(i)) & 255u) << (8 * i);
+        hi |= ((unsigned)round8(held[h].at(4 + i)) & 255u) << (8 * i);
+      }
+      *(uint2*)(o + (h * 256 + threadIdx.x) * 8) = make_uint2(lo, hi);
+    }
+  for (int64_t i = (vec ? HELD * 2048 : 0) + threadIdx.x; i < width; i += 256) o[i] = (signed char)round8(T::load(row, i));
+  for (int64_t i = width + threadIdx.x; i < stride; i += 256) o[i] = 0;
 }
 
 // One operand's tile of ROWS rows from row0 on: the copy of a stage to LDS, and the matrix instruction's operands.
-template <int ROWS, int WAVES>
+template <int ROWS>
 struct Tile {
-  static constexpr int BYTES = ROWS * STAGE, PASSES = BYTES / (1024 * WAVES);
-  static __device__ __forceinline__ int swizzle(int r) { return (r >> 1) & 7; }
+  static constexpr int BYTES = ROWS * STAGE, PASSES = BYTES / (1024 * 4);
+  static __device__ __forceinline__ int swizzle(int r) { return (r >> 3) & 3; }
   const char* base;
   int64_t extent;  // bytes from base to the operand's end
   int voff[PASSES];
@@ -83,8 +142,8 @@ struct Tile {
     extent = (rows - row0) * stride;
 #pragma unroll
     for (int q = 0; q < PASSES; q++) {
-      const int r = (q * WAVES + wave) * 8 + lane / 8;
-      voff[q] = (int)(r * stride) + ((lane % 8) ^ swizzle(r)) * 16;
+      const int r = (q * 4 + wave) * 16 + lane / 4;
+      voff[q] = (int)(r * stride) + ((lane % 4) ^ swizzle(r)) * 16;
     }
   }
   __device__ __forceinline__ void copy(char* tile, int stage, int wave) const {
@@ -92,94 +151,216 @@ struct Tile {
     const __amdgpu_buffer_rsrc_t r =
         __builtin_amdgcn_make_buffer_rsrc((void*)(base + off), (short)0, (int)(left < 0 ? 0 : left < 0x7fffffff ? left : 0x7fffffff), 0x00020000);
 #pragma unroll
-    for (int q = 0; q < PASSES; q++)
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_void*)(tile + (q * WAVES + wave) * 1024), 16, voff[q], 0, 0, 0);
+    for (int q = 0; q < PASSES; q++) __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_void*)(tile + (q * 4 + wave) * 1024), 16, voff[q], 0, 0, 0);
   }
   // lane l: bytes 32 kk + 16 (l / 32) .. + 15 of row row0 + l % 32; kk a place in rd
   static __device__ __forceinline__ void offsets(int row0, int lane, int* rd) {
     const int r = lane & 31, h = lane >> 5;
 #pragma unroll
-    for (int kk = 0; kk < 4; kk++) rd[kk] = (row0 + r) * STAGE + (((2 * kk + h) ^ swizzle(r)) & 7) * 16;
+    for (int kk = 0; kk < 2; kk++) rd[kk] = (row0 + r) * STAGE + ((2 * kk + h) ^ swizzle(r)) * 16;
   }
-  static __device__ __forceinline__ i32x4 operand(const char* tile, const int* rd, int t, int kk) { return *(const i32x4*)(tile + rd[kk] + t * 32 * STAGE); }
+  static __device__ __forceinline__ i32x4 operand(const char* tile, int at, int t) { return *(const i32x4*)(tile + at + t * 32 * STAGE); }
 };
 
-// out[m, n] = (x8[m] . w8[n]) s[m] scale[n] + bias[n], one rounding a step in float, rounded to the type at the end.
+// A sum times the weight's scale, then times the scale of x, which may be as large as x.
+__device__ __forceinline__ float scaled(int sum, float w_scale, float x_scale) {
+  return (float)sum * w_scale * x_scale;
+}
+
 template <typename T, int BM>
-__global__ __launch_bounds__(BM == 256 ? 512 : 256, 2) void int8_tiles(const signed char* __restrict__ x8, const float* __restrict__ scales, const signed char* __restrict__ w8,
-                                                                       int64_t w_stride, Int8Args a) {
+__global__ __launch_bounds__(256, BM == 256 ? 1 : 2) void int8_tiles(const signed char* __restrict__ x8, const float* __restrict__ scales, const signed char* __restrict__ w8,
+                                                                    int64_t w_stride, Int8Args a) {
 #if defined(__HIP_DEVICE_COMPILE__)  // the host pass needs the stub alone
-  constexpr int WAVES = BM == 256 ? 8 : 4, WN = WAVES / 2, WTM = BM / 2, WTN = BM / WN, TM = WTM / 32, TN = WTN / 32;
-  typedef Tile<BM, WAVES> O;
-  __shared__ __attribute__((aligned(1024))) char A0[O::BYTES];
-  __shared__ __attribute__((aligned(1024))) char A1[O::BYTES];
-  __shared__ __attribute__((aligned(1024))) char B0[O::BYTES];
-  __shared__ __attribute__((aligned(1024))) char B1[O::BYTES];
+  constexpr int WT = BM / 2, TM = WT / 32;  // a wave's tile, WT x WT
+  typedef Tile<BM> O;
+  constexpr int FLIGHT = 2 * O::PASSES;  // copies of a stage and wave
+  __shared__ __attribute__((aligned(1024))) char A0[O::BYTES], A1[O::BYTES], A2[O::BYTES], A3[O::BYTES];
+  __shared__ __attribute__((aligned(1024))) char B0[O::BYTES], B1[O::BYTES], B2[O::BYTES], B3[O::BYTES];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5, n32 = lane & 31;
-  const int wm = wave / WN, wn = wave % WN;
+  const int wm = wave >> 1, wn = wave & 1;
   const int64_t tiles_n = (a.outputs + BM - 1) / BM, tiles_m = (a.rows + BM - 1) / BM;
   int64_t id = blockIdx.x;
   if (gridDim.x % 8 == 0) id = (id % 8) * (gridDim.x / 8) + id / 8;  // an XCD's workgroups: a run of tiles, 4 tile rows at a time
   constexpr int64_t GROUP = 4;
   const int64_t group = id / (GROUP * tiles_n), first = group * GROUP, live = tiles_m - first < GROUP ? tiles_m - first : GROUP;
   const int64_t m0 = (first + (id - group * GROUP * tiles_n) % live) * BM, n0 = (id - group * GROUP * tiles_n) / live * BM;
-  const int64_t padded = (a.width + STAGE - 1) / STAGE * STAGE;
-  const int stages = (int)(padded / STAGE);
+  const int64_t padded = (a.width + PAD - 1) / PAD * PAD;
+  const int stages = (int)(padded / STAGE);  // a multiple of 4
 
-  i32x16 acc[TM][TN];
+  i32x16 acc[TM][TM];
 #pragma unroll
   for (int i = 0; i < TM; i++)
 #pragma unroll
-    for (int j = 0; j < TN; j++)
+    for (int j = 0; j < TM; j++)
 #pragma unroll
       for (int e = 0; e < 16; e++) acc[i][j][e] = 0;
   const O da(x8, a.rows, padded, m0, wave, lane), db(w8, a.outputs, w_stride, n0, wave, lane);
-  int rda[4], rdb[4];
-  O::offsets(wm * WTM, lane, rda);
-  O::offsets(wn * WTN, lane, rdb);
-  auto stage = [&](const char* at, const char* bt, char* an, char* bn, int st) __attribute__((always_inline)) {
-    da.copy(an, st + 1, wave);
-    db.copy(bn, st + 1, wave);
+  int rda[2], rdb[2];
+  O::offsets(wm * WT, lane, rda);
+  O::offsets(wn * WT, lane, rdb);
+  i32x4 av[2][TM], bv[2][TM];
+  auto read = [&](const char* at, const char* bt, int kk, i32x4* ao, i32x4* bo) __attribute__((always_inline)) {
 #pragma unroll
-    for (int kk = 0; kk < 4; kk++) {
-      i32x4 av[TM], bv[TN];
+    for (int i = 0; i < TM; i++) ao[i] = O::operand(at, rda[kk], i);
 #pragma unroll
-      for (int i = 0; i < TM; i++) av[i] = O::operand(at, rda, i, kk);
+    for (int j = 0; j < TM; j++) bo[j] = O::operand(bt, rdb[kk], j);
+  };
+  auto multiply = [&](const i32x4* ao, const i32x4* bo) __attribute__((always_inline)) {
+    // the weight's operand first: a lane then holds 4 consecutive outputs of a row
 #pragma unroll
-      for (int j = 0; j < TN; j++) bv[j] = O::operand(bt, rdb, j, kk);
-      // the weight's operand first: a lane then holds 4 consecutive outputs of a row
+    for (int i = 0; i < TM; i++)
 #pragma unroll
-      for (int i = 0; i < TM; i++)
-#pragma unroll
-        for (int j = 0; j < TN; j++) acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(bv[j], av[i], acc[i][j], 0, 0, 0);
-    }
-    __builtin_amdgcn_s_waitcnt(WAIT_VMEM);
+      for (int j = 0; j < TM; j++) acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(bo[j], ao[i], acc[i][j], 0, 0, 0);
+  };
+  // stage st from (at, bt), whose first operands are in registers; (an, bn) the next one's, (af, bf) where stage st + 3 goes:
+  // the buffer that every wave is done with at the barrier
+  auto stage = [&](const char* at, const char* bt, const char* an, const char* bn, char* af, char* bf, int st) __attribute__((always_inline)) {
+    __builtin_amdgcn_s_waitcnt(wait_vm(FLIGHT));  // this wave's part of stage st + 1 has landed, st + 2 is on its way
     __syncthreads();
+    da.copy(af, st + 3, wave);
+    db.copy(bf, st + 3, wave);
+    read(at, bt, 1, av[1], bv[1]);
+    multiply(av[0], bv[0]);
+    read(an, bn, 0, av[0], bv[0]);
+    multiply(av[1], bv[1]);
   };
   da.copy(A0, 0, wave);
   db.copy(B0, 0, wave);
-  __builtin_amdgcn_s_waitcnt(WAIT_VMEM);
+  da.copy(A1, 1, wave);
+  db.copy(B1, 1, wave);
+  da.copy(A2, 2, wave);
+  db.copy(B2, 2, wave);
+  __builtin_amdgcn_s_waitcnt(wait_vm(2 * FLIGHT));
   __syncthreads();
-  for (int st = 0; st < stages; st += 2) {
-    stage(A0, B0, A1, B1, st);
-    if (st + 1 < stages) stage(A1, B1, A0, B0, st + 1);
+  read(A0, B0, 0, av[0], bv[0]);
+  for (int st = 0; st < stages; st += 4) {
+    stage(A0, B0, A1, B1, A3, B3, st);
+    stage(A1, B1, A2, B2, A0, B0, st + 1);
+    stage(A2, B2, A3, B3, A1, B1, st + 2);
+    stage(A3, B3, A0, B0, A2, B2, st + 3);
   }
-  typename T::Storage* out = (typename T::Storage*)a.out;
-  const typename T::Storage* bias = (const typename T::Storage*)a.bias;
+  __builtin_amdgcn_s_waitcnt(wait_vm(0));  // no copy may land in what is staged below
+  __syncthreads();
+
+  // Through LDS, so that a store instruction writes whole row segments: 32 rows of a wave's sums at a time, 16-byte chunk c of row r
+  // at c ^ (r & 7). Coming back, a lane has 8 outputs of a row, the same ones for every row.
+  typedef typename T::Storage S;
+  constexpr int LPR = WT / 8, RPI = 64 / LPR;  // lanes a row, rows at a time
+  static_assert(32 * WT * 4 == O::BYTES, "a wave's rows fill a buffer");
+  char* const region = wave == 0 ? A0 : wave == 1 ? A1 : wave == 2 ? B0 : B1;
+  S* out = (S*)a.out;
+  const S* bias = (const S*)a.bias;
+  const int64_t col = n0 + wn * WT + (lane % LPR) * 8;
+  const bool wide = a.outputs % 8 == 0 && ((uintptr_t)out & 15) == 0;
+  float ws[8], bs[8];
+#pragma unroll
+  for (int e = 0; e < 8; e++) {
+    ws[e] = col + e < a.outputs ? a.w_scales[col + e] : 0.f;
+    bs[e] = bias != nullptr && col + e < a.outputs ? T::load(bias, col + e) : 0.f;
+  }
 #pragma unroll
   for (int i = 0; i < TM; i++) {
-    const int64_t row = m0 + wm * WTM + i * 32 + n32;
-    const float s = row < a.rows ? scales[row] : 0.f;
 #pragma unroll
-    for (int j = 0; j < TN; j++)
+    for (int j = 0; j < TM; j++)
 #pragma unroll
-      for (int e = 0; e < 16; e++) {
-        const int64_t col = n0 + wn * WTN + j * 32 + 8 * (e >> 2) + 4 * h + (e & 3);
-        if (row >= a.rows || col >= a.outputs) continue;
-        float y = (float)acc[i][j][e] * a.w_scales[col] * s;  // the scale of x last: it may be as large as x
-        if (bias != nullptr) y += T::load(bias, col);
-        T::store(out, row * a.outputs + col, y);
+      for (int q = 0; q < 4; q++)
+        *(i32x4*)(region + n32 * WT * 4 + ((8 * j + 2 * q + h) ^ (n32 & 7)) * 16) = i32x4{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int it = 0; it < 32 / RPI; it++) {
+      const int r = it * RPI + lane / LPR;
+      const int64_t row = m0 + wm * WT + i * 32 + r;
+      const float s = row < a.rows ? scales[row] : 0.f;
+      float y[8];
+#pragma unroll
+      for (int half = 0; half < 2; half++) {
+        const i32x4 c = *(const i32x4*)(region + r * WT * 4 + ((2 * (lane % LPR) + half) ^ (r & 7)) * 16);
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          const float v = scaled(c[e], ws[4 * half + e], s);
+          y[4 * half + e] = bias != nullptr ? v + bs[4 * half + e] : v;
+        }
       }
+      if (row >= a.rows || col >= a.outputs) continue;
+      S* o = out + row * a.outputs + col;
+      if (wide) {
+        if constexpr (std::is_same<T, F32>::value) {
+          *(f32x4*)o = f32x4{y[0], y[1], y[2], y[3]};
+          *(f32x4*)(o + 4) = f32x4{y[4], y[5], y[6], y[7]};
+        } else {
+          *(u32x4*)o = u32x4{T::pack2(y[0], y[1]), T::pack2(y[2], y[3]), T::pack2(y[4], y[5]), T::pack2(y[6], y[7])};
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; e++)
+          if (col + e < a.outputs) T::store(o, e, y[e]);
+      }
+    }
+    __builtin_amdgcn_wave_barrier();
+  }
+#endif
+}
+
+// 16 outputs of up to 16 NR rows; the width in pairs of 64 bytes, 4 of a wave's in flight while 4 are multiplied.
+template <typename T, int NR, int FEW_WAVES>
+__global__ __launch_bounds__(64 * FEW_WAVES) void int8_few(const signed char* __restrict__ x8, const float* __restrict__ scales, const signed char* __restrict__ w8, int64_t w_stride, Int8Args a) {
+#if defined(__HIP_DEVICE_COMPILE__)  // the host pass needs the stub alone
+  constexpr int U = NR == 4 ? 2 : 4;  // pairs in flight
+  __shared__ __attribute__((aligned(16))) int sums[FEW_WAVES * NR * 256];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15, g = lane >> 4;
+  const int64_t n0 = blockIdx.x * (int64_t)16, padded = (a.width + PAD - 1) / PAD * PAD;
+  const int pairs = (int)(padded / 128);
+  const int64_t left = (a.outputs - n0) * w_stride;
+  const __amdgpu_buffer_rsrc_t rw = __builtin_amdgcn_make_buffer_rsrc((void*)(w8 + n0 * w_stride), (short)0, (int)(left < 0x7fffffff ? left : 0x7fffffff), 0x00020000);
+  const __amdgpu_buffer_rsrc_t rx = __builtin_amdgcn_make_buffer_rsrc((void*)x8, (short)0, (int)(a.rows * padded), 0x00020000);
+  const int wv = (int)(n * w_stride) + 16 * g, xv = (int)(n * padded) + 16 * g;
+  i32x4 acc[NR];
+#pragma unroll
+  for (int t = 0; t < NR; t++) acc[t] = i32x4{0, 0, 0, 0};
+  struct Batch {
+    i32x4 w[2 * U], x[NR][2 * U];
+  };
+  auto load = [&](Batch& b, int p0) __attribute__((always_inline)) {
+#pragma unroll
+    for (int u = 0; u < U; u++)
+#pragma unroll
+      for (int k = 0; k < 2; k++) {
+        const int p = p0 + u * FEW_WAVES, off = p * 128 + k * 64;
+        b.w[2 * u + k] = __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(rw, wv + off, 0, 0));
+#pragma unroll
+        for (int t = 0; t < NR; t++)
+          b.x[t][2 * u + k] = __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(rx, p < pairs ? xv + (int)(16 * t * padded) + off : 0x7ffffff0, 0, 0));
+      }
+  };
+  auto multiply = [&](const Batch& b) __attribute__((always_inline)) {
+#pragma unroll
+    for (int u = 0; u < 2 * U; u++)
+#pragma unroll
+      for (int t = 0; t < NR; t++) acc[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(b.w[u], b.x[t][u], acc[t], 0, 0, 0);
+  };
+  constexpr int STEP = U * FEW_WAVES;
+  Batch b0, b1;
+  load(b0, wave);
+  for (int p = wave; p < pairs; p += 2 * STEP) {
+    load(b1, p + STEP);
+    multiply(b0);
+    load(b0, p + 2 * STEP);
+    multiply(b1);
+  }
+#pragma unroll
+  for (int t = 0; t < NR; t++) *(i32x4*)&sums[((wave * NR + t) * 16 + n) * 16 + 4 * g] = acc[t];  // row n, outputs 4 g .. + 3
+  __syncthreads();
+  typedef typename T::Storage S;
+  const S* bias = (const S*)a.bias;
+  for (int i = threadIdx.x; i < NR * 256; i += 64 * FEW_WAVES) {
+    int sum = 0;
+#pragma unroll
+    for (int w = 0; w < FEW_WAVES; w++) sum += sums[w * NR * 256 + i];
+    const int64_t row = i >> 4, col = n0 + (i & 15);
+    if (row >= a.rows || col >= a.outputs) continue;
+    float y = scaled(sum, a.w_scales[col], scales[row]);
+    if (bias != nullptr) y += T::load(bias, col);
+    T::store((S*)a.out, row * a.outputs + col, y);
   }
 #endif
 }
@@ -188,21 +369,40 @@ template <typename T, int BM>
 int tiles_of(const Int8Args& a, const signed char* x8, const float* scales, const signed char* w8, int64_t w_stride) {
   const int64_t blocks = ((a.rows + BM - 1) / BM) * ((a.outputs + BM - 1) / BM);
   if (blocks > 0x7fffffff) return fail(LIMN_HIP_EUNSUPPORTED, "int8_linear: %lld workgroups exceed one launch", (long long)blocks);
-  hipLaunchKernelGGL((int8_tiles<T, BM>), dim3((unsigned)blocks), dim3(BM == 256 ? 512 : 256), 0, a.stream, x8, scales, w8, w_stride, a);
+  hipLaunchKernelGGL((int8_tiles<T, BM>), dim3((unsigned)blocks), dim3(256), 0, a.stream, x8, scales, w8, w_stride, a);
   return check_hip(hipGetLastError(), "launching the 8-bit product");
 }
 
+template <typename T, int NR>
+int few_of(const Int8Args& a, const signed char* x8, const float* scales, const signed char* w8, int64_t w_stride) {
+  const int64_t blocks = (a.outputs + 15) / 16;
+  // few outputs: the width over 16 waves instead of 4
+  if (blocks < 256)
+    hipLaunchKernelGGL((int8_few<T, NR, 16>), dim3((unsigned)blocks), dim3(1024), 0, a.stream, x8, scales, w8, w_stride, a);
+  else
+    hipLaunchKernelGGL((int8_few<T, NR, 4>), dim3((unsigned)blocks), dim3(256), 0, a.stream, x8, scales, w8, w_stride, a);
+  return check_hip(hipGetLastError(), "launching the 8-bit product of few rows");
+}
+
+// x8, the scales, and the copy of a weight whose rows are not aligned, in one launch.
 template <typename T>
-int quantize_of(const void* x, void* values, float* scales, int64_t rows, int64_t width, int64_t stride, hipStream_t stream) {
-  hipLaunchKernelGGL((quantize_rows<T>), dim3((unsigned)rows), dim3(256), 0, stream, (const typename T::Storage*)x, (signed char*)values, scales, width, stride);
+int quantize_of(const void* x, void* values, float* scales, int64_t rows, int64_t width, int64_t stride, const void* w, void* w_out, int64_t outputs, hipStream_t stream) {
+  typedef typename T::Storage S;
+  const int vec = width % 8 == 0 && (uintptr_t)x % 16 == 0 && (uintptr_t)values % 8 == 0 && stride % 8 == 0;
+  const int64_t copies = w_out == nullptr ? 0 : outputs < 1024 ? outputs : 1024;
+  if (rows + copies > 0x7fffffff) return fail(LIMN_HIP_EUNSUPPORTED, "quantize_rows: %lld rows exceed one launch", (long long)rows);
+  hipLaunchKernelGGL((quantize_rows<T>), dim3((unsigned)(rows + copies)), dim3(256), 0, stream, (const S*)x, (signed char*)values, scales, rows, width, stride, vec,
+                     (const signed char*)w, (signed char*)w_out, outputs);
   return check_hip(hipGetLastError(), "launching the rounding of rows to 8 bits");
 }
 
-int quantize(int dtype, const void* x, void* values, float* scales, int64_t rows, int64_t width, int64_t stride, hipStream_t stream) {
-  return dtype == LIMN_HIP_FLOAT32   ? quantize_of<F32>(x, values, scales, rows, width, stride, stream)
-         : dtype == LIMN_HIP_FLOAT16 ? quantize_of<F16>(x, values, scales, rows, width, stride, stream)
-                                     : quantize_of<BF16>(x, values, scales, rows, width, stride, stream);
+int quantize(int dtype, const void* x, void* values, float* scales, int64_t rows, int64_t width, int64_t stride, const void* w, void* w_out, int64_t outputs, hipStream_t stream) {
+  return dtype == LIMN_HIP_FLOAT32   ? quantize_of<F32>(x, values, scales, rows, width, stride, w, w_out, outputs, stream)
+         : dtype == LIMN_HIP_FLOAT16 ? quantize_of<F16>(x, values, scales, rows, width, stride, w, w_out, outputs, stream)
+                                     : quantize_of<BF16>(x, values, scales, rows, width, stride, w, w_out, outputs, stream);
 }
+
+constexpr int64_t FEW = 64;  // rows up to which int8_few takes a call
 
 template <typename T>
 int linear(const Int8Args& a) {
@@ -211,18 +411,21 @@ int linear(const Int8Args& a) {
   float* scales = (float*)(x8 + align256(a.rows * padded));
   const signed char* w8 = (const signed char*)a.w;
   int64_t w_stride = a.width;
-  int rc = quantize(a.dtype, a.x, x8, scales, a.rows, a.width, padded, a.stream);
+  signed char* copy = needs_copy(a.w, a.width) ? (signed char*)scales + align256(a.rows * 4) : nullptr;
+  const int rc = quantize(a.dtype, a.x, x8, scales, a.rows, a.width, padded, a.w, copy, a.outputs, a.stream);
   if (rc != LIMN_HIP_OK) return rc;
-  if (needs_copy(a.w, a.width)) {
-    signed char* copy = (signed char*)scales + align256(a.rows * 4);
-    hipLaunchKernelGGL(pad_rows, dim3((unsigned)a.outputs), dim3(256), 0, a.stream, w8, copy, a.width, padded);
-    rc = check_hip(hipGetLastError(), "launching the copy of an 8-bit weight");
-    if (rc != LIMN_HIP_OK) return rc;
+  if (copy != nullptr) {
     w8 = copy;
     w_stride = padded;
   }
-  const int64_t t256 = ((a.rows + 255) / 256) * ((a.outputs + 255) / 256);
-  return t256 >= 256 ? tiles_of<T, 256>(a, x8, scales, w8, w_stride) : tiles_of<T, 128>(a, x8, scales, w8, w_stride);
+  if (a.rows <= 16) return few_of<T, 1>(a, x8, scales, w8, w_stride);
+  if (a.rows <= 32) return few_of<T, 2>(a, x8, scales, w8, w_stride);
+  if (a.rows <= FEW) return few_of<T, 4>(a, x8, scales, w8, w_stride);
+  // the largest tiles that give every CU a workgroup
+  const auto tiles = [&](int64_t m) { return ((a.rows + m - 1) / m) * ((a.outputs + m - 1) / m); };
+  if (tiles(256) >= 256) return tiles_of<T, 256>(a, x8, scales, w8, w_stride);
+  if (tiles(128) >= 256) return tiles_of<T, 128>(a, x8, scales, w8, w_stride);
+  return tiles_of<T, 64>(a, x8, scales, w8, w_stride);
 }
 
 int check_sizes(const char* name, int dtype, int64_t rows, int64_t width, int64_t outputs) {
@@ -248,12 +451,12 @@ extern "C" int limn_hip_quantize_rows(const void* x, void* values, void* scales,
   if ((uintptr_t)x % (dtype == LIMN_HIP_FLOAT32 ? 4 : 2) != 0 || (uintptr_t)scales % 4 != 0)
     return fail(LIMN_HIP_EINVAL, "%s: buffers must be aligned to their element size", name);
   if (rows > 0x7fffffff || width > ((int64_t)1 << 40) / rows) return fail(LIMN_HIP_EUNSUPPORTED, "%s: sizes out of range", name);
-  return quantize(dtype, x, values, (float*)scales, rows, width, width, (hipStream_t)stream);
+  return quantize(dtype, x, values, (float*)scales, rows, width, width, nullptr, nullptr, 0, (hipStream_t)stream);
 }
 
 extern "C" int64_t limn_hip_int8_linear_workspace(int dtype, int64_t rows, int64_t width, int64_t outputs) {
   if (rows < 1 || width < 1 || width > WIDEST || outputs < 1 || rows > 0x7fffffff || outputs > 0x7fffffff) return 0;
-  const int64_t padded = (width + STAGE - 1) / STAGE * STAGE;
+  const int64_t padded = (width + PAD - 1) / PAD * PAD;
   return align256(rows * padded) + align256(rows * 4) + outputs * padded;  // the copy too: a weight's rows may be aligned, its start not
 }
 
