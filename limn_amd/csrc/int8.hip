@@ -215,14 +215,23 @@ __global__ __launch_bounds__(256, BM == 256 ? 1 : 2) void int8_tiles(const signe
   // stage st from (at, bt), whose first operands are in registers; (an, bn) the next one's, (af, bf) where stage st + 3 goes:
   // the buffer that every wave is done with at the barrier
   auto stage = [&](const char* at, const char* bt, const char* an, const char* bn, char* af, char* bf, int st) __attribute__((always_inline)) {
-    __builtin_amdgcn_s_waitcnt(wait_vm(FLIGHT));  // this wave's part of stage st + 1 has landed, st + 2 is on its way
-    __syncthreads();
+    // this wave's part of stage st + 1 has landed, st + 2 is on its way; then every wave's has
+    asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(FLIGHT) : "memory");
     da.copy(af, st + 3, wave);
     db.copy(bf, st + 3, wave);
     read(at, bt, 1, av[1], bv[1]);
     multiply(av[0], bv[0]);
     read(an, bn, 0, av[0], bv[0]);
     multiply(av[1], bv[1]);
+    // the copies, then each k step's products with the reads for the next one among them
+    __builtin_amdgcn_sched_group_barrier(0x020, FLIGHT, 0);
+#pragma unroll
+    for (int k = 0; k < 2; k++)
+#pragma unroll
+      for (int r = 0; r < 2 * TM; r++) {
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x008, TM > 1 ? TM / 2 : 1, 0);
+      }
   };
   da.copy(A0, 0, wave);
   db.copy(B0, 0, wave);
