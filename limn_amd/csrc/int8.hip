@@ -223,13 +223,13 @@ __global__ __launch_bounds__(256, BM == 256 ? 1 : 2) void int8_tiles(const signe
     multiply(av[0], bv[0]);
     read(an, bn, 0, av[0], bv[0]);
     multiply(av[1], bv[1]);
-    // the copies, then each k step's products with the reads for the next one among them
-    __builtin_amdgcn_sched_group_barrier(0x020, FLIGHT, 0);
+    // the copies and the reads for the next k step among the products
 #pragma unroll
     for (int k = 0; k < 2; k++)
 #pragma unroll
       for (int r = 0; r < 2 * TM; r++) {
         __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        if ((k * 2 * TM + r) % 2 == 0) __builtin_amdgcn_sched_group_barrier(0x020, FLIGHT / (2 * TM), 0);
         __builtin_amdgcn_sched_group_barrier(0x008, TM > 1 ? TM / 2 : 1, 0);
       }
   };
