@@ -9,12 +9,11 @@
 //
 // int8_tiles (many rows; bound by the matrix cores): output tiles of 256 x 256, 128 x 128 or 64 x 64 on 4 waves, one a SIMD, each
 // with a quarter as accumulators of v_mfma_i32_32x32x32_i8. A wave's 128 x 128 takes 8 reads of LDS for 16 products, half
-// of what 8 waves of 128 x 64 do, whose LDS was busy all the time. Stages of 64 bytes a row go straight to LDS
-// (buffer_load ... lds) into one of four buffers, three stages ahead; chunk c of LDS row r lies at c ^ ((r >> 3) & 3), so that the 16
-// rows a read serves in a cycle (those of one parity of r >> 2 in 32) are in 16 places of the 64 banks. Operands are read a k
+// of what 8 waves of 128 x 64 do, whose LDS was busy all the time. Stages of 64 bytes a row (128 in the smaller tiles) go straight to LDS
+// (buffer_load ... lds) into one of four buffers, three stages ahead. Operands are read a k
 // step ahead, the last one's of a stage in the next stage, which has landed by then.
 //
-// int8_few (up to 64 rows; bound by reading the weight once): a wave has 16 outputs and a part of the width, its bytes read from
+// int8_few (up to 16 rows; bound by reading the weight once): a wave has 16 outputs and a part of the width, its bytes read from
 // memory straight into operands of v_mfma_i32_16x16x64_i8; the waves of a workgroup add their sums in LDS.
 
 #include "common.h"
@@ -31,7 +30,6 @@ typedef int i32x16 __attribute__((ext_vector_type(16)));
 typedef __attribute__((address_space(3))) void lds_void;
 
 constexpr int PAD = 256;     // rows of x8 are padded to whole multiples of this: four stages
-constexpr int STAGE = 64;    // bytes of a row that a stage of int8_tiles holds
 
 // the s_waitcnt immediate that leaves the newest n vector memory operations in flight, and the other counters free
 constexpr int wait_vm(int n) { return 0x0F70 | (n & 15) | ((n >> 4) << 14); }
@@ -130,10 +128,12 @@ __global__ __launch_bounds__(256) void quantize_rows(const typename T::Storage* 
 }
 
 // One operand's tile of ROWS rows from row0 on: the copy of a stage to LDS, and the matrix instruction's operands.
-template <int ROWS>
+// STAGE bytes a row; chunk c of LDS row r lies at c ^ swizzle(r), so that the 16 rows a read serves in a cycle (those of one parity
+// of r >> 2 in 32) are in 16 places of the 64 banks.
+template <int ROWS, int STAGE>
 struct Tile {
-  static constexpr int BYTES = ROWS * STAGE, PASSES = BYTES / (1024 * 4);
-  static __device__ __forceinline__ int swizzle(int r) { return (r >> 3) & 3; }
+  static constexpr int BYTES = ROWS * STAGE, PASSES = BYTES / (1024 * 4), CHUNKS = STAGE / 16, RPI = 64 / CHUNKS, KK = STAGE / 32;
+  static __device__ __forceinline__ int swizzle(int r) { return STAGE == 64 ? (r >> 3) & 3 : (r >> 1) & 7; }
   const char* base;
   int64_t extent;  // bytes from base to the operand's end
   int voff[PASSES];
@@ -142,8 +142,8 @@ struct Tile {
     extent = (rows - row0) * stride;
 #pragma unroll
     for (int q = 0; q < PASSES; q++) {
-      const int r = (q * 4 + wave) * 16 + lane / 4;
-      voff[q] = (int)(r * stride) + ((lane % 4) ^ swizzle(r)) * 16;
+      const int r = (q * 4 + wave) * RPI + lane / CHUNKS;
+      voff[q] = (int)(r * stride) + ((lane % CHUNKS) ^ swizzle(r)) * 16;
     }
   }
   __device__ __forceinline__ void copy(char* tile, int stage, int wave) const {
@@ -157,7 +157,7 @@ struct Tile {
   static __device__ __forceinline__ void offsets(int row0, int lane, int* rd) {
     const int r = lane & 31, h = lane >> 5;
 #pragma unroll
-    for (int kk = 0; kk < 2; kk++) rd[kk] = (row0 + r) * STAGE + ((2 * kk + h) ^ swizzle(r)) * 16;
+    for (int kk = 0; kk < KK; kk++) rd[kk] = (row0 + r) * STAGE + ((2 * kk + h) ^ swizzle(r)) * 16;
   }
   static __device__ __forceinline__ i32x4 operand(const char* tile, int at, int t) { return *(const i32x4*)(tile + at + t * 32 * STAGE); }
 };
@@ -167,13 +167,13 @@ __device__ __forceinline__ float scaled(int sum, float w_scale, float x_scale) {
   return (float)sum * w_scale * x_scale;
 }
 
-template <typename T, int BM>
-__global__ __launch_bounds__(256, BM == 256 ? 1 : 2) void int8_tiles(const signed char* __restrict__ x8, const float* __restrict__ scales, const signed char* __restrict__ w8,
+template <typename T, int BM, int STAGE>
+__global__ __launch_bounds__(256, BM * STAGE > 8192 ? 1 : 2) void int8_tiles(const signed char* __restrict__ x8, const float* __restrict__ scales, const signed char* __restrict__ w8,
                                                                     int64_t w_stride, Int8Args a) {
 #if defined(__HIP_DEVICE_COMPILE__)  // the host pass needs the stub alone
   constexpr int WT = BM / 2, TM = WT / 32;  // a wave's tile, WT x WT
-  typedef Tile<BM> O;
-  constexpr int FLIGHT = 2 * O::PASSES;  // copies of a stage and wave
+  typedef Tile<BM, STAGE> O;
+  constexpr int FLIGHT = 2 * O::PASSES, KK = O::KK;  // copies of a stage and wave; k steps of a stage
   __shared__ __attribute__((aligned(1024))) char A0[O::BYTES], A1[O::BYTES], A2[O::BYTES], A3[O::BYTES];
   __shared__ __attribute__((aligned(1024))) char B0[O::BYTES], B1[O::BYTES], B2[O::BYTES], B3[O::BYTES];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5, n32 = lane & 31;
@@ -185,7 +185,8 @@ __global__ __launch_bounds__(256, BM == 256 ? 1 : 2) void int8_tiles(const signe
   const int64_t group = id / (GROUP * tiles_n), first = group * GROUP, live = tiles_m - first < GROUP ? tiles_m - first : GROUP;
   const int64_t m0 = (first + (id - group * GROUP * tiles_n) % live) * BM, n0 = (id - group * GROUP * tiles_n) / live * BM;
   const int64_t padded = (a.width + PAD - 1) / PAD * PAD;
-  const int stages = (int)(padded / STAGE);  // a multiple of 4
+  // the largest tiles take whole fours of stages: a way out between them cost the accumulators' way through memory
+  const int stages = (int)(BM == 256 ? padded / STAGE : (a.width + STAGE - 1) / STAGE);
 
   i32x16 acc[TM][TM];
 #pragma unroll
@@ -195,7 +196,7 @@ __global__ __launch_bounds__(256, BM == 256 ? 1 : 2) void int8_tiles(const signe
 #pragma unroll
       for (int e = 0; e < 16; e++) acc[i][j][e] = 0;
   const O da(x8, a.rows, padded, m0, wave, lane), db(w8, a.outputs, w_stride, n0, wave, lane);
-  int rda[2], rdb[2];
+  int rda[KK], rdb[KK];
   O::offsets(wm * WT, lane, rda);
   O::offsets(wn * WT, lane, rdb);
   i32x4 av[2][TM], bv[2][TM];
@@ -219,17 +220,21 @@ __global__ __launch_bounds__(256, BM == 256 ? 1 : 2) void int8_tiles(const signe
     asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(FLIGHT) : "memory");
     da.copy(af, st + 3, wave);
     db.copy(bf, st + 3, wave);
-    read(at, bt, 1, av[1], bv[1]);
-    multiply(av[0], bv[0]);
-    read(an, bn, 0, av[0], bv[0]);
-    multiply(av[1], bv[1]);
+#pragma unroll
+    for (int kk = 0; kk < KK; kk++) {
+      if (kk + 1 < KK)
+        read(at, bt, kk + 1, av[(kk + 1) & 1], bv[(kk + 1) & 1]);
+      else
+        read(an, bn, 0, av[0], bv[0]);
+      multiply(av[kk & 1], bv[kk & 1]);
+    }
     // the copies and the reads for the next k step among the products
 #pragma unroll
-    for (int k = 0; k < 2; k++)
+    for (int k = 0; k < KK; k++)
 #pragma unroll
       for (int r = 0; r < 2 * TM; r++) {
         __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-        if ((k * 2 * TM + r) % 2 == 0) __builtin_amdgcn_sched_group_barrier(0x020, FLIGHT / (2 * TM), 0);
+        if ((k * 2 * TM + r) % 2 == 0) __builtin_amdgcn_sched_group_barrier(0x020, FLIGHT / (KK * TM), 0);
         __builtin_amdgcn_sched_group_barrier(0x008, TM > 1 ? TM / 2 : 1, 0);
       }
   };
@@ -244,18 +249,22 @@ __global__ __launch_bounds__(256, BM == 256 ? 1 : 2) void int8_tiles(const signe
   read(A0, B0, 0, av[0], bv[0]);
   for (int st = 0; st < stages; st += 4) {
     stage(A0, B0, A1, B1, A3, B3, st);
+    if (BM < 256 && st + 1 >= stages) break;
     stage(A1, B1, A2, B2, A0, B0, st + 1);
+    if (BM < 256 && st + 2 >= stages) break;
     stage(A2, B2, A3, B3, A1, B1, st + 2);
+    if (BM < 256 && st + 3 >= stages) break;
     stage(A3, B3, A0, B0, A2, B2, st + 3);
   }
   __builtin_amdgcn_s_waitcnt(wait_vm(0));  // no copy may land in what is staged below
   __syncthreads();
 
   // Through LDS, so that a store instruction writes whole row segments: 32 rows of a wave's sums at a time, 16-byte chunk c of row r
-  // at c ^ (r & 7). Coming back, a lane has 8 outputs of a row, the same ones for every row.
+  // at c ^ (r & 7). Coming back, a lane has 8 outputs of a row, the same ones for every row; where rows of the result are not aligned,
+  // one output of up to 64 in turn.
   typedef typename T::Storage S;
   constexpr int LPR = WT / 8, RPI = 64 / LPR;  // lanes a row, rows at a time
-  static_assert(32 * WT * 4 == O::BYTES, "a wave's rows fill a buffer");
+  static_assert(32 * WT * 4 <= O::BYTES, "a wave's rows fit a buffer");
   char* const region = wave == 0 ? A0 : wave == 1 ? A1 : wave == 2 ? B0 : B1;
   S* out = (S*)a.out;
   const S* bias = (const S*)a.bias;
@@ -267,6 +276,9 @@ __global__ __launch_bounds__(256, BM == 256 ? 1 : 2) void int8_tiles(const signe
     ws[e] = col + e < a.outputs ? a.w_scales[col + e] : 0.f;
     bs[e] = bias != nullptr && col + e < a.outputs ? T::load(bias, col + e) : 0.f;
   }
+  float xs[TM];  // the scales of the 32 rows, one a lane of each half
+#pragma unroll
+  for (int i = 0; i < TM; i++) xs[i] = scales[min(m0 + wm * WT + i * 32 + n32, a.rows - 1)];
 #pragma unroll
   for (int i = 0; i < TM; i++) {
 #pragma unroll
@@ -275,11 +287,29 @@ __global__ __launch_bounds__(256, BM == 256 ? 1 : 2) void int8_tiles(const signe
       for (int q = 0; q < 4; q++)
         *(i32x4*)(region + n32 * WT * 4 + ((8 * j + 2 * q + h) ^ (n32 & 7)) * 16) = i32x4{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
     __builtin_amdgcn_wave_barrier();
+    if (!wide) {
+      constexpr int SPAN = WT < 64 ? WT : 64;
+#pragma unroll 1
+      for (int cs = 0; cs < WT / SPAN; cs++) {
+        const int in = cs * 64 + lane % SPAN;
+        const int64_t c = n0 + wn * WT + in;
+        const float w = c < a.outputs ? a.w_scales[c] : 0.f, b = bias != nullptr && c < a.outputs ? T::load(bias, c) : 0.f;
+#pragma unroll 4  // run once a block: its own fetch is most of its time if it is unrolled
+        for (int r0 = 0; r0 < 32; r0 += 64 / SPAN) {
+          const int r = r0 + lane / SPAN;
+          const int64_t row = m0 + wm * WT + i * 32 + r;
+          const float v = scaled(*(const int*)(region + r * WT * 4 + ((in >> 2) ^ (r & 7)) * 16 + (in & 3) * 4), w, __shfl(xs[i], r));
+          if (row < a.rows && c < a.outputs) T::store(out, row * a.outputs + c, bias != nullptr ? v + b : v);
+        }
+      }
+      __builtin_amdgcn_wave_barrier();
+      continue;
+    }
 #pragma unroll
     for (int it = 0; it < 32 / RPI; it++) {
       const int r = it * RPI + lane / LPR;
       const int64_t row = m0 + wm * WT + i * 32 + r;
-      const float s = row < a.rows ? scales[row] : 0.f;
+      const float s = __shfl(xs[i], r);
       float y[8];
 #pragma unroll
       for (int half = 0; half < 2; half++) {
@@ -292,17 +322,11 @@ __global__ __launch_bounds__(256, BM == 256 ? 1 : 2) void int8_tiles(const signe
       }
       if (row >= a.rows || col >= a.outputs) continue;
       S* o = out + row * a.outputs + col;
-      if (wide) {
-        if constexpr (std::is_same<T, F32>::value) {
-          *(f32x4*)o = f32x4{y[0], y[1], y[2], y[3]};
-          *(f32x4*)(o + 4) = f32x4{y[4], y[5], y[6], y[7]};
-        } else {
-          *(u32x4*)o = u32x4{T::pack2(y[0], y[1]), T::pack2(y[2], y[3]), T::pack2(y[4], y[5]), T::pack2(y[6], y[7])};
-        }
+      if constexpr (std::is_same<T, F32>::value) {
+        *(f32x4*)o = f32x4{y[0], y[1], y[2], y[3]};
+        *(f32x4*)(o + 4) = f32x4{y[4], y[5], y[6], y[7]};
       } else {
-#pragma unroll
-        for (int e = 0; e < 8; e++)
-          if (col + e < a.outputs) T::store(o, e, y[e]);
+        *(u32x4*)o = u32x4{T::pack2(y[0], y[1]), T::pack2(y[2], y[3]), T::pack2(y[4], y[5]), T::pack2(y[6], y[7])};
       }
     }
     __builtin_amdgcn_wave_barrier();
@@ -310,86 +334,71 @@ __global__ __launch_bounds__(256, BM == 256 ? 1 : 2) void int8_tiles(const signe
 #endif
 }
 
-// 16 outputs of up to 16 NR rows; the width in pairs of 64 bytes, 4 of a wave's in flight while 4 are multiplied.
-template <typename T, int NR, int FEW_WAVES>
-__global__ __launch_bounds__(64 * FEW_WAVES) void int8_few(const signed char* __restrict__ x8, const float* __restrict__ scales, const signed char* __restrict__ w8, int64_t w_stride, Int8Args a) {
+// 16 outputs of up to 16 rows; the width in pairs of 64 bytes, 4 of a wave's in flight while 4 are multiplied.
+template <typename T>
+__global__ __launch_bounds__(256) void int8_few(const signed char* __restrict__ x8, const float* __restrict__ scales, const signed char* __restrict__ w8, int64_t w_stride, Int8Args a) {
 #if defined(__HIP_DEVICE_COMPILE__)  // the host pass needs the stub alone
-  constexpr int U = NR == 4 ? 2 : 4;  // pairs in flight
-  __shared__ __attribute__((aligned(16))) int sums[FEW_WAVES * NR * 256];
+  constexpr int U = 4, STEP = 4 * U;  // pairs of a wave, and of the workgroup, in a batch
+  __shared__ __attribute__((aligned(16))) int sums[4 * 256];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15, g = lane >> 4;
   const int64_t n0 = blockIdx.x * (int64_t)16, padded = (a.width + PAD - 1) / PAD * PAD;
-  const int pairs = (int)(padded / 128);
+  const int pairs = (int)((a.width + 127) / 128);
   const int64_t left = (a.outputs - n0) * w_stride;
   const __amdgpu_buffer_rsrc_t rw = __builtin_amdgcn_make_buffer_rsrc((void*)(w8 + n0 * w_stride), (short)0, (int)(left < 0x7fffffff ? left : 0x7fffffff), 0x00020000);
   const __amdgpu_buffer_rsrc_t rx = __builtin_amdgcn_make_buffer_rsrc((void*)x8, (short)0, (int)(a.rows * padded), 0x00020000);
   const int wv = (int)(n * w_stride) + 16 * g, xv = (int)(n * padded) + 16 * g;
-  i32x4 acc[NR];
-#pragma unroll
-  for (int t = 0; t < NR; t++) acc[t] = i32x4{0, 0, 0, 0};
+  i32x4 acc = {0, 0, 0, 0};
   struct Batch {
-    i32x4 w[2 * U], x[NR][2 * U];
+    i32x4 w[2 * U], x[2 * U];
   };
   auto load = [&](Batch& b, int p0) __attribute__((always_inline)) {
 #pragma unroll
     for (int u = 0; u < U; u++)
 #pragma unroll
       for (int k = 0; k < 2; k++) {
-        const int p = p0 + u * FEW_WAVES, off = p * 128 + k * 64;
-        b.w[2 * u + k] = __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(rw, wv + off, 0, 0));
-#pragma unroll
-        for (int t = 0; t < NR; t++)
-          b.x[t][2 * u + k] = __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(rx, p < pairs ? xv + (int)(16 * t * padded) + off : 0x7ffffff0, 0, 0));
+        const int p = p0 + 4 * u, off = p * 128 + k * 64;  // past the width: zeros, and nothing of the next row is read
+        b.w[2 * u + k] = __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(rw, p < pairs ? wv + off : 0x7ffffff0, 0, 0));
+        b.x[2 * u + k] = __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(rx, p < pairs ? xv + off : 0x7ffffff0, 0, 0));
       }
   };
   auto multiply = [&](const Batch& b) __attribute__((always_inline)) {
 #pragma unroll
-    for (int u = 0; u < 2 * U; u++)
-#pragma unroll
-      for (int t = 0; t < NR; t++) acc[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(b.w[u], b.x[t][u], acc[t], 0, 0, 0);
+    for (int u = 0; u < 2 * U; u++) acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(b.w[u], b.x[u], acc, 0, 0, 0);
   };
-  constexpr int STEP = U * FEW_WAVES;
   Batch b0, b1;
   load(b0, wave);
   for (int p = wave; p < pairs; p += 2 * STEP) {
-    load(b1, p + STEP);
+    if (p + STEP < pairs) load(b1, p + STEP);
     multiply(b0);
-    load(b0, p + 2 * STEP);
+    if (p + STEP >= pairs) break;
+    if (p + 2 * STEP < pairs) load(b0, p + 2 * STEP);
     multiply(b1);
   }
-#pragma unroll
-  for (int t = 0; t < NR; t++) *(i32x4*)&sums[((wave * NR + t) * 16 + n) * 16 + 4 * g] = acc[t];  // row n, outputs 4 g .. + 3
+  *(i32x4*)&sums[(wave * 16 + n) * 16 + 4 * g] = acc;  // row n, outputs 4 g .. + 3
   __syncthreads();
   typedef typename T::Storage S;
   const S* bias = (const S*)a.bias;
-  for (int i = threadIdx.x; i < NR * 256; i += 64 * FEW_WAVES) {
-    int sum = 0;
-#pragma unroll
-    for (int w = 0; w < FEW_WAVES; w++) sum += sums[w * NR * 256 + i];
-    const int64_t row = i >> 4, col = n0 + (i & 15);
-    if (row >= a.rows || col >= a.outputs) continue;
-    float y = scaled(sum, a.w_scales[col], scales[row]);
-    if (bias != nullptr) y += T::load(bias, col);
-    T::store((S*)a.out, row * a.outputs + col, y);
-  }
+  const int i = threadIdx.x;
+  const int sum = (sums[i] + sums[256 + i]) + (sums[512 + i] + sums[768 + i]);
+  const int64_t row = i >> 4, col = n0 + (i & 15);
+  if (row >= a.rows || col >= a.outputs) return;
+  float y = scaled(sum, a.w_scales[col], scales[row]);
+  if (bias != nullptr) y += T::load(bias, col);
+  T::store((S*)a.out, row * a.outputs + col, y);
 #endif
 }
 
-template <typename T, int BM>
+template <typename T, int BM, int STAGE>
 int tiles_of(const Int8Args& a, const signed char* x8, const float* scales, const signed char* w8, int64_t w_stride) {
   const int64_t blocks = ((a.rows + BM - 1) / BM) * ((a.outputs + BM - 1) / BM);
   if (blocks > 0x7fffffff) return fail(LIMN_HIP_EUNSUPPORTED, "int8_linear: %lld workgroups exceed one launch", (long long)blocks);
-  hipLaunchKernelGGL((int8_tiles<T, BM>), dim3((unsigned)blocks), dim3(256), 0, a.stream, x8, scales, w8, w_stride, a);
+  hipLaunchKernelGGL((int8_tiles<T, BM, STAGE>), dim3((unsigned)blocks), dim3(256), 0, a.stream, x8, scales, w8, w_stride, a);
   return check_hip(hipGetLastError(), "launching the 8-bit product");
 }
 
-template <typename T, int NR>
+template <typename T>
 int few_of(const Int8Args& a, const signed char* x8, const float* scales, const signed char* w8, int64_t w_stride) {
-  const int64_t blocks = (a.outputs + 15) / 16;
-  // few outputs: the width over 16 waves instead of 4
-  if (blocks < 256)
-    hipLaunchKernelGGL((int8_few<T, NR, 16>), dim3((unsigned)blocks), dim3(1024), 0, a.stream, x8, scales, w8, w_stride, a);
-  else
-    hipLaunchKernelGGL((int8_few<T, NR, 4>), dim3((unsigned)blocks), dim3(256), 0, a.stream, x8, scales, w8, w_stride, a);
+  hipLaunchKernelGGL((int8_few<T>), dim3((unsigned)((a.outputs + 15) / 16)), dim3(256), 0, a.stream, x8, scales, w8, w_stride, a);
   return check_hip(hipGetLastError(), "launching the 8-bit product of few rows");
 }
 
@@ -411,7 +420,9 @@ int quantize(int dtype, const void* x, void* values, float* scales, int64_t rows
                                      : quantize_of<BF16>(x, values, scales, rows, width, stride, w, w_out, outputs, stream);
 }
 
-constexpr int64_t FEW = 64;  // rows up to which int8_few takes a call
+// Rows up to which int8_few takes a call: those of one operand. (16 x 4096 x 8192, few and tiles, the rows' rounding with them: 13.4
+// and 14.3 us; 16 x 4096 x 2048 11.2 and 13.4; 32 x 4096 x 8192, two operands a wave, 17.3 and 14.9.)
+constexpr int64_t FEW = 16;
 
 template <typename T>
 int linear(const Int8Args& a) {
@@ -427,14 +438,13 @@ int linear(const Int8Args& a) {
     w8 = copy;
     w_stride = padded;
   }
-  if (a.rows <= 16) return few_of<T, 1>(a, x8, scales, w8, w_stride);
-  if (a.rows <= 32) return few_of<T, 2>(a, x8, scales, w8, w_stride);
-  if (a.rows <= FEW) return few_of<T, 4>(a, x8, scales, w8, w_stride);
-  // the largest tiles that give every CU a workgroup
+  if (a.rows <= FEW) return few_of<T>(a, x8, scales, w8, w_stride);
+  // The largest tiles where they give every CU a workgroup, the middle ones where they do more than half (1024 x 760 x 2288, 144 of
+  // them: 16.0 us, 16.9 in the small ones; 512 x 4096 x 4096, 128: 25.5 and 23.2).
   const auto tiles = [&](int64_t m) { return ((a.rows + m - 1) / m) * ((a.outputs + m - 1) / m); };
-  if (tiles(256) >= 256) return tiles_of<T, 256>(a, x8, scales, w8, w_stride);
-  if (tiles(128) >= 256) return tiles_of<T, 128>(a, x8, scales, w8, w_stride);
-  return tiles_of<T, 64>(a, x8, scales, w8, w_stride);
+  if (tiles(256) >= 256) return tiles_of<T, 256, 64>(a, x8, scales, w8, w_stride);
+  if (tiles(128) > 128) return tiles_of<T, 128, 128>(a, x8, scales, w8, w_stride);
+  return tiles_of<T, 64, 128>(a, x8, scales, w8, w_stride);
 }
 
 int check_sizes(const char* name, int dtype, int64_t rows, int64_t width, int64_t outputs) {
