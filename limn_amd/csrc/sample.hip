@@ -2,8 +2,13 @@
 //
 // With w_j = exp((x_j - max x) / temperature) and the order of x descending, equal ones by index, every filter keeps a
 // beginning of the order, and so does the draw end one: each is a search for the place where a running count (top-k) or a
-// running mass (top-p, the draw) passes a number. A row's workgroup finds such a place by histograms: 2048 bins of equal
-// width in (max - x) / temperature, then the key bits of x inside the bin that it lies in, 11, 11 and 10 at a time.
+// running mass (top-p, the draw) passes a number. A row has a workgroup, which reads it
+//  - for its largest logit;
+//  - into a histogram of 2048 bins of equal width in (max - x) / temperature (of counts alone, if there is a top-k);
+//  - for the members of the bins that matter, at most a thousand, which it sorts: with a top-k those of all bins up to the border's,
+//    and everything else is done on them; without, those of one bin for every border.
+// Rows of up to 1024 logits are sorted whole. A bin with more members (rows of equal logits) is taken apart by the bits of x
+// instead, 11, 11 and 10 at a time.
 //
 // Masses are whole numbers, w 2^F rounded with F such that a row's sum stays below 2^63: sums of them do not depend on
 // the order that atomics come in, and they are exact to V 2^-F of the largest weight (2^-28 of it for 2^17 tokens at
@@ -14,10 +19,12 @@
 
 #include <math.h>
 
+#include <type_traits>
+
 namespace limn {
 namespace {
 
-constexpr int THREADS = 1024, WAVES = THREADS / 64, BINS = 2048;
+constexpr int BINS = 2048;
 
 struct SampleArgs {
   const float* uniforms;
@@ -32,74 +39,127 @@ struct SampleArgs {
 };
 
 // x as an unsigned number of the same order: NaN as minus infinity, both zeros alike
+__device__ __forceinline__ float cleaned(float x) { return x != x ? -__builtin_inff() : x + 0.f; }
 __device__ __forceinline__ unsigned key_of(float x) {
-  const unsigned b = __float_as_uint(x != x ? -__builtin_inff() : x + 0.f);
+  const unsigned b = __float_as_uint(cleaned(x));
   return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 __device__ __forceinline__ float of_key(unsigned k) { return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k); }
 
-constexpr unsigned NOTHING = 0x007fffffu;  // the key of minus infinity
-
-// The first elements of the order: those with a larger key, and `taken` of those with this one.
+// The first elements of the order: those with a larger key, and `taken` of those with this one; and what they hold.
 struct Border {
   unsigned key, taken;
+  uint64_t mass;
+  int index;  // of the last of them; -1: not looked for
 };
-__device__ __forceinline__ bool shorter(Border a, Border b) { return a.key > b.key || (a.key == b.key && a.taken < b.taken); }
+__device__ __forceinline__ bool shorter(const Border& a, const Border& b) { return a.key > b.key || (a.key == b.key && a.taken < b.taken); }
 
+template <int TH>
 struct Shared {
-  uint64_t mass0[BINS], mass[BINS], sums[WAVES];
-  unsigned count0[BINS], count[BINS], counts[WAVES];
-  uint64_t found_mass;
-  unsigned found_bin, found_count, word;
+  uint64_t list[TH], sums[TH / 64];
+  unsigned counts[TH / 64];
+  uint64_t found_mass, found_element;
+  unsigned found_bin, found_count, listed, word;
+  double powers[64];  // 2^(i / 64)
 };
+template <int TH>
+struct Bins {
+  uint64_t mass0[BINS], mass[BINS];
+  unsigned count0[BINS], count[BINS];
+};
+struct Nothing {};
 
-template <typename T>
+// A row of logits, seen by a workgroup of TH threads.
+template <typename T, int TH>
 struct Row {
-  const typename T::Storage* x;
-  int vocab, bits;
-  float top, inv;  // the largest logit; 1 / temperature
-  double inv64;
-  Shared& sh;
+  typedef typename T::Storage S;
+  static constexpr int PER = 16 / (int)sizeof(S), WAVES = TH / 64;
+  const S* x;
+  int vocab, bits, head, chunks;  // elements before the first 16-byte boundary, and whole 16-byte chunks from there
+  float top, inv;                 // the largest logit; 1 / temperature
+  double scale;                   // log2(e) / temperature
+  Shared<TH>& sh;
 
-  __device__ __forceinline__ float at(int i) const { return T::load(x, i); }
-  __device__ __forceinline__ double weight(float v) const { return v == top ? 1.0 : exp(((double)v - (double)top) * inv64); }
-  __device__ __forceinline__ uint64_t whole(float v) const { return (uint64_t)rint(ldexp(weight(v), bits)); }
+  __device__ __forceinline__ Row(const S* x_, int vocab_, int bits_, Shared<TH>& sh_) : x(x_), vocab(vocab_), bits(bits_), top(0.f), inv(0.f), scale(0.0), sh(sh_) {
+    head = min(vocab, (int)((16 - ((uintptr_t)x & 15)) & 15) / (int)sizeof(S));
+    chunks = (vocab - head) / PER;
+  }
+
+  // f(logit, index) for every element, some of them by this thread
+  template <typename F>
+  __device__ __forceinline__ void each(F f) const {
+    const u32x4* body = (const u32x4*)(x + head);
+    int c = threadIdx.x;
+    constexpr int U = 4;
+    for (; c + (U - 1) * TH < chunks; c += U * TH) {
+      u32x4 w[U];
+#pragma unroll
+      for (int u = 0; u < U; u++) w[u] = body[c + u * TH];
+#pragma unroll
+      for (int u = 0; u < U; u++) eight(w[u], head + (c + u * TH) * PER, f);
+    }
+    for (; c < chunks; c += TH) eight(body[c], head + c * PER, f);
+    const int rest = vocab - chunks * PER;  // before and behind the chunks: fewer than 2 PER
+    if ((int)threadIdx.x < rest) {
+      const int i = (int)threadIdx.x < head ? (int)threadIdx.x : chunks * PER + (int)threadIdx.x;
+      f(cleaned(T::load(x, i)), i);
+    }
+  }
+  template <typename F>
+  __device__ __forceinline__ void eight(u32x4 w, int i, F f) const {
+#pragma unroll
+    for (int e = 0; e < PER; e++) {
+      if constexpr (PER == 4)
+        f(cleaned(__uint_as_float(w[e])), i + e);
+      else
+        f(cleaned(T::unpack((u16)(w[e >> 1] >> (16 * (e & 1))))), i + e);
+    }
+  }
+
+  // 2^F exp((v - top) / temperature) as a whole number: 2^t with t = k / 64 + r, |r| <= 2^-7, 2^(k / 64) from the table and 2^r by
+  // its series, whose first term left out is below 2^-54; the sum with 2^52 rounds it.
+  __device__ __forceinline__ double weight64(float v) const {
+    const double t = ((double)v - (double)top) * scale;
+    const double k = rint(t * 64.0), r = fma(k, -0.015625, t);
+    double p = fma(r, 1.3333558146428443e-3, 9.618129107628477e-3);
+    p = fma(p, r, 5.5504108664821576e-2);
+    p = fma(p, r, 2.402265069591007e-1);
+    p = fma(p, r, 6.931471805599453e-1);
+    p = fma(p, r, 1.0);
+    const int n = (int)k;
+    return ldexp(p * sh.powers[n & 63], n >> 6);
+  }
+  __device__ __forceinline__ double weight(float v) const {
+    if (v == top) return 1.0;
+    const double t = ((double)v - (double)top) * scale;
+    return t > -1000.0 ? weight64(v) : 0.0;
+  }
+  __device__ __forceinline__ uint64_t whole(float v) const {
+    const double w = ldexp(weight(v), bits);  // at most 2^52
+    return (uint64_t)__double_as_longlong(w + 4503599627370496.0) - 0x4330000000000000ull;
+  }
   // monotone in v: each step rounds, none turns the order round
   __device__ __forceinline__ int bin(float v) const { return v == top ? 0 : (int)fminf((top - v) * inv * 64.f, (float)(BINS - 1)); }
 
   __device__ uint64_t sum(uint64_t v) const {
+#pragma unroll
     for (int o = 32; o > 0; o >>= 1) v += __shfl_xor((unsigned long long)v, o);
     __syncthreads();
     if ((threadIdx.x & 63) == 0) sh.sums[threadIdx.x >> 6] = v;
     __syncthreads();
     v = 0;
+#pragma unroll
     for (int w = 0; w < WAVES; w++) v += sh.sums[w];
+    __syncthreads();
     return v;
   }
 
-  __device__ void clear(uint64_t* mass, unsigned* count) const {
-    __syncthreads();
-    for (int b = threadIdx.x; b < BINS; b += THREADS) {
-      mass[b] = 0;
-      count[b] = 0;
-    }
-    __syncthreads();
-  }
-
-  // The first bin at which reached(mass, count) of everything up to and with it is true; the mass and count before it
-  // are added to m and c. Every thread gets it; BINS if there is none.
-  template <typename F>
-  __device__ int first_bin(const uint64_t* mass, const unsigned* count, F reached, uint64_t& m, unsigned& c) const {
-    constexpr int PER = BINS / THREADS;
+  // m and c: of this thread's elements; what the threads before it have, and before all of them the given, comes back in bm and bc
+  __device__ __forceinline__ void before(uint64_t m, unsigned c, uint64_t& bm, unsigned& bc) const {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    uint64_t pm = 0;
-    unsigned pc = 0;
-    for (int i = 0; i < PER; i++) {
-      pm += mass[threadIdx.x * PER + i];
-      pc += count[threadIdx.x * PER + i];
-    }
-    uint64_t im = pm;
-    unsigned ic = pc;
+    uint64_t im = m;
+    unsigned ic = c;
+#pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
       const uint64_t um = __shfl_up((unsigned long long)im, o);
       const unsigned uc = __shfl_up(ic, o);
@@ -108,28 +168,46 @@ struct Row {
         ic += uc;
       }
     }
-    if (threadIdx.x == 0) sh.found_bin = BINS;
     if (lane == 63) {
       sh.sums[wave] = im;
       sh.counts[wave] = ic;
     }
     __syncthreads();
-    uint64_t bm = m + im - pm;
-    unsigned bc = c + ic - pc;
-    for (int w = 0; w < wave; w++) {
-      bm += sh.sums[w];
-      bc += sh.counts[w];
+    bm += im - m;
+    bc += ic - c;
+#pragma unroll
+    for (int w = 0; w < WAVES; w++)
+      if (w < wave) {
+        bm += sh.sums[w];
+        bc += sh.counts[w];
+      }
+    __syncthreads();
+  }
+
+  // The first bin at which reached(mass, count) of everything up to and with it is true; the mass and count before it
+  // are added to m and c. Every thread gets it; BINS if there is none.
+  template <typename F>
+  __device__ int first_bin(const uint64_t* mass, const unsigned* count, F reached, uint64_t& m, unsigned& c) const {
+    constexpr int PT = BINS / TH;
+    uint64_t pm = 0, bm = m;
+    unsigned pc = 0, bc = c;
+#pragma unroll
+    for (int i = 0; i < PT; i++) {
+      pm += mass[threadIdx.x * PT + i];
+      pc += count[threadIdx.x * PT + i];
     }
+    if (threadIdx.x == 0) sh.found_bin = BINS;
+    before(pm, pc, bm, bc);
     if (!reached(bm, bc) && reached(bm + pm, bc + pc)) {  // one thread at most: both grow along the bins
       int i = 0;
-      for (; i + 1 < PER; i++) {
-        const uint64_t nm = bm + mass[threadIdx.x * PER + i];
-        const unsigned nc = bc + count[threadIdx.x * PER + i];
+      for (; i + 1 < PT; i++) {
+        const uint64_t nm = bm + mass[threadIdx.x * PT + i];
+        const unsigned nc = bc + count[threadIdx.x * PT + i];
         if (reached(nm, nc)) break;
         bm = nm;
         bc = nc;
       }
-      sh.found_bin = threadIdx.x * PER + i;
+      sh.found_bin = threadIdx.x * PT + i;
       sh.found_mass = bm;
       sh.found_count = bc;
     }
@@ -143,68 +221,138 @@ struct Row {
     return b;
   }
 
-  // The shortest beginning of the order of which reached(mass, count) is true, or the whole of it: key 0.
+  __device__ void clear(uint64_t* mass, unsigned* count) const {
+    __syncthreads();
+    for (int b = threadIdx.x; b < BINS; b += TH) {
+      mass[b] = 0;
+      count[b] = 0;
+    }
+    __syncthreads();
+  }
+
+  // The elements that take(logit) is true of, TH of them at most, in the order: each thread gets one (a larger key first, as the
+  // complement of its key above its index), or ~0.
   template <typename F>
-  __device__ Border find(F reached) const {
+  __device__ uint64_t sorted(F take) const {
+    __syncthreads();
+    if (threadIdx.x == 0) sh.listed = 0;
+    __syncthreads();
+    each([&](float v, int i) __attribute__((always_inline)) {
+      if (take(v)) {
+        const unsigned at = atomicAdd(&sh.listed, 1u);
+        if (at < TH) sh.list[at] = ((uint64_t)~key_of(v) << 32) | (unsigned)i;
+      }
+    });
+    __syncthreads();
+    const int n = min((int)sh.listed, TH);
+    uint64_t e = (int)threadIdx.x < n ? sh.list[threadIdx.x] : ~0ull;
+    int size = 64;
+    while (size < n) size <<= 1;  // what lies behind is not touched
+    for (int k = 2; k <= size; k <<= 1)
+      for (int j = k >> 1; j > 0; j >>= 1) {
+        uint64_t o;
+        if (j >= 64) {
+          __syncthreads();
+          sh.list[threadIdx.x] = e;
+          __syncthreads();
+          o = sh.list[threadIdx.x ^ j];
+        } else {
+          o = __shfl_xor((unsigned long long)e, j);
+        }
+        const bool low = (threadIdx.x & j) == 0, up = (threadIdx.x & k) == 0;
+        if (low == up ? o < e : o > e) e = o;
+      }
+    __syncthreads();
+    return e;
+  }
+
+  // Of the sorted elements e, before which m and c lie: the first one with which reached(mass, count) is true. Every thread gets it.
+  template <typename F>
+  __device__ Border place(uint64_t e, F reached, uint64_t m, unsigned c) const {
+    const float v = of_key(~(unsigned)(e >> 32));
+    const uint64_t w = e == ~0ull ? 0 : whole(v);
+    if (threadIdx.x == 0) sh.found_element = ~0ull;
+    before(w, e == ~0ull ? 0u : 1u, m, c);
+    if (e != ~0ull && !reached(m, c) && reached(m + w, c + 1)) {
+      sh.found_element = e;
+      sh.found_mass = m + w;
+    }
+    __syncthreads();
+    Border b = {0u, 0xffffffffu, 0, -1};
+    const uint64_t f = sh.found_element;
+    if (f != ~0ull) {
+      b = Border{~(unsigned)(f >> 32), 0u, sh.found_mass, (int)(unsigned)f};
+      if (threadIdx.x == 0) sh.word = 0;
+      __syncthreads();  // how many with its key come up to it
+      if (e != ~0ull && (e >> 32) == (f >> 32) && e <= f) atomicAdd(&sh.word, 1u);
+      __syncthreads();
+      b.taken = sh.word;
+    }
+    __syncthreads();
+    return b;
+  }
+
+  // The shortest beginning of the order of which reached(mass, count) is true, from the histogram.
+  template <typename F>
+  __device__ Border find(Bins<TH>& bins, F reached) const {
     uint64_t m = 0;
     unsigned c = 0;
-    const int b0 = first_bin(sh.mass0, sh.count0, reached, m, c);
-    if (b0 == BINS) return Border{0u, 0xffffffffu};
+    const int b0 = first_bin(bins.mass0, bins.count0, reached, m, c);
+    if (b0 == BINS) return Border{0u, 0xffffffffu, 0, -1};
+    if (bins.count0[b0] <= TH) return place(sorted([&](float v) __attribute__((always_inline)) { return bin(v) == b0; }), reached, m, c);
     unsigned prefix = 0;
     for (int level = 0; level < 3; level++) {
       const int shift = level == 0 ? 21 : level == 1 ? 10 : 0, width = level == 2 ? 10 : 11;
-      clear(sh.mass, sh.count);
-      for (int i = threadIdx.x; i < vocab; i += THREADS) {
-        const float v = at(i);
+      clear(bins.mass, bins.count);
+      each([&](float v, int) __attribute__((always_inline)) {
         const unsigned k = key_of(v);
-        if (bin(of_key(k)) != b0 || (level > 0 && (k >> (shift + width)) != prefix)) continue;
+        if (bin(v) != b0 || (level > 0 && (k >> (shift + width)) != prefix)) return;
         const int b = (1 << width) - 1 - (int)((k >> shift) & ((1u << width) - 1));  // larger keys first
-        atomicAdd(&sh.count[b], 1u);
-        atomicAdd((unsigned long long*)&sh.mass[b], (unsigned long long)whole(of_key(k)));
-      }
+        atomicAdd(&bins.count[b], 1u);
+        atomicAdd((unsigned long long*)&bins.mass[b], (unsigned long long)whole(v));
+      });
       __syncthreads();
-      const int b = first_bin(sh.mass, sh.count, reached, m, c);
+      const int b = first_bin(bins.mass, bins.count, reached, m, c);
       prefix = (prefix << width) | (unsigned)((1 << width) - 1 - b);
     }
     // equal ones, each of the same mass
-    const uint64_t each = whole(of_key(prefix));
-    unsigned lo = 1, hi = sh.count[1023 - (prefix & 1023u)];
+    const uint64_t each_mass = whole(of_key(prefix));
+    unsigned lo = 1, hi = bins.count[1023 - (prefix & 1023u)];
     while (lo < hi) {
       const unsigned mid = lo + (hi - lo) / 2;
-      if (reached(m + mid * each, c + mid)) hi = mid; else lo = mid + 1;
+      if (reached(m + mid * each_mass, c + mid)) hi = mid; else lo = mid + 1;
     }
-    return Border{prefix, lo};
+    return Border{prefix, lo, m + lo * each_mass, -1};
   }
 
-  // the mass of a beginning of the order
-  __device__ uint64_t mass_of(Border e) const {
+  // the mass of the elements with this key or a larger one
+  __device__ uint64_t mass_from(unsigned key) const {
     uint64_t v = 0;
-    for (int i = threadIdx.x; i < vocab; i += THREADS) {
-      const unsigned k = key_of(at(i));
-      if (k > e.key) v += whole(of_key(k));
-    }
-    return sum(v) + (e.taken == 0xffffffffu ? 0 : e.taken * whole(of_key(e.key)));
+    each([&](float x, int) __attribute__((always_inline)) {
+      if (key_of(x) >= key) v += whole(x);
+    });
+    return sum(v);
   }
 
   // the index of the nth element with this key
   __device__ int index_of(unsigned key, unsigned nth) const {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    unsigned before = 0;
-    for (int i0 = 0; i0 < vocab; i0 += THREADS) {
+    unsigned seen = 0;
+    for (int i0 = 0; i0 < vocab; i0 += TH) {
       const int i = i0 + threadIdx.x;
-      const bool hit = i < vocab && key_of(at(i)) == key;
+      const bool hit = i < vocab && key_of(T::load(x, i)) == key;
       const uint64_t hits = __ballot(hit);
       __syncthreads();
       if (lane == 0) sh.counts[wave] = (unsigned)__popcll(hits);
       __syncthreads();
-      unsigned mine = before, all = before;
+      unsigned mine = seen, all = seen;
       for (int w = 0; w < WAVES; w++) {
         if (w < wave) mine += sh.counts[w];
         all += sh.counts[w];
       }
       if (hit && mine + (unsigned)__popcll(hits & ((1ull << lane) - 1)) + 1 == nth) sh.word = (unsigned)i;
       if (all >= nth) break;
-      before = all;
+      seen = all;
     }
     __syncthreads();
     return (int)sh.word;
@@ -213,7 +361,6 @@ struct Row {
   // the least key whose weight is p or more (the largest logit's at least)
   __device__ unsigned least_key(double p) const {
     unsigned lo = 0, hi = key_of(top);
-    if (p > 1.0) return hi;
     while (lo < hi) {
       const unsigned mid = lo + (hi - lo) / 2;
       if (weight(of_key(mid)) >= p) hi = mid; else lo = mid + 1;
@@ -222,88 +369,153 @@ struct Row {
   }
 };
 
-template <typename T>
-__global__ __launch_bounds__(THREADS) void sample_rows(const typename T::Storage* __restrict__ logits, SampleArgs a) {
-  __shared__ Shared sh;
+// The first mass of a beginning that reaches p of the whole: the last one kept is the first with which it does; the first element
+// always is kept.
+__device__ __forceinline__ uint64_t least_mass(float p, uint64_t total) {
+  const double want = ceil(fmax((double)p, 0.0) * (double)total);
+  return want > 1.0 ? (uint64_t)want : 1;
+}
+// The mass before the drawn token, at most: u of the kept mass, and below the whole of it.
+__device__ __forceinline__ uint64_t mass_before(float u, uint64_t total) {
+  const double share = u > 0.f ? (double)u * (double)total : u == u ? 0.0 : (double)total;
+  return share < (double)total ? min((uint64_t)share, total - 1) : total - 1;
+}
+
+// WHOLE: rows of up to TH logits.
+template <typename T, int TH, bool WHOLE>
+__global__ __launch_bounds__(TH) void sample_rows(const typename T::Storage* __restrict__ logits, SampleArgs a) {
+  __shared__ Shared<TH> sh;
+  __shared__ std::conditional_t<WHOLE, Nothing, Bins<TH>> bins;
   const int64_t n = blockIdx.x;
   const int vocab = (int)a.vocab;
-  const float t = a.temperature != nullptr ? a.temperature[n] : 1.f;
-  Row<T> row = {logits + n * a.row_stride, vocab, a.bits, 0.f, 0.f, 0.0, sh};
-  unsigned best = 0;
-  for (int i = threadIdx.x; i < vocab; i += THREADS) best = max(best, key_of(row.at(i)));
-  for (int o = 32; o > 0; o >>= 1) best = max(best, (unsigned)__shfl_xor((int)best, o));
-  if ((threadIdx.x & 63) == 0) sh.counts[threadIdx.x >> 6] = best;
+  const float t = a.temperature != nullptr ? a.temperature[n] : 1.f, p = a.top_p != nullptr ? a.top_p[n] : 1.f, q = a.min_p != nullptr ? a.min_p[n] : 0.f, u = a.uniforms[n];
+  const int k = a.top_k != nullptr ? a.top_k[n] : 0;
+  if (threadIdx.x < 64) sh.powers[threadIdx.x] = exp2(threadIdx.x * 0.015625);
+  Row<T, TH> row(logits + n * a.row_stride, vocab, a.bits, sh);
+  float best = -__builtin_inff();
+  row.each([&](float v, int) __attribute__((always_inline)) { best = fmaxf(best, v); });
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) best = fmaxf(best, __shfl_xor(best, o));
+  if ((threadIdx.x & 63) == 0) sh.counts[threadIdx.x >> 6] = __float_as_uint(best);
   __syncthreads();
-  for (int w = 0; w < WAVES; w++) best = max(best, sh.counts[w]);
+#pragma unroll
+  for (int w = 0; w < TH / 64; w++) best = fmaxf(best, __uint_as_float(sh.counts[w]));
   __syncthreads();
-  if (best <= NOTHING) {  // no number above minus infinity
-    if (threadIdx.x == 0) {
-      a.tokens[n] = -1;
-      if (a.logprobs != nullptr) a.logprobs[n] = -__builtin_inff();
-    }
+  auto give = [&](int token, float logprob) {
+    if (threadIdx.x != 0) return;
+    a.tokens[n] = token;
+    if (a.logprobs != nullptr) a.logprobs[n] = logprob;
+  };
+  if (best == -__builtin_inff()) {  // no number above minus infinity
+    give(-1, -__builtin_inff());
     return;
   }
   if (!(t > 0.f)) {
-    const int i = row.index_of(best, 1);
-    if (threadIdx.x == 0) {
-      a.tokens[n] = i;
-      if (a.logprobs != nullptr) a.logprobs[n] = 0.f;
-    }
+    if (threadIdx.x == 0) sh.word = 0xffffffffu;
+    __syncthreads();
+    unsigned first = 0xffffffffu;
+    row.each([&](float v, int i) __attribute__((always_inline)) {
+      if (v == best) first = min(first, (unsigned)i);
+    });
+    if (first != 0xffffffffu) atomicMin(&sh.word, first);
+    __syncthreads();
+    give((int)sh.word, 0.f);
     return;
   }
-  row.top = of_key(best);
+  row.top = best + 0.f;
   row.inv = 1.f / t;
-  row.inv64 = 1.0 / (double)t;
-  row.clear(sh.mass0, sh.count0);
-  uint64_t total = 0;
-  for (int i = threadIdx.x; i < vocab; i += THREADS) {
-    const float v = of_key(key_of(row.at(i)));
-    const uint64_t w = row.whole(v);
-    const int b = row.bin(v);
-    total += w;
-    atomicAdd(&sh.count0[b], 1u);
-    atomicAdd((unsigned long long*)&sh.mass0[b], (unsigned long long)w);
-  }
-  total = row.sum(total);
-  Border end = {0u, 0xffffffffu};
-  const int k = a.top_k != nullptr ? a.top_k[n] : 0;
-  if (k > 0 && k < vocab) {
-    end = row.find([=](uint64_t, unsigned c) { return c >= (unsigned)k; });
-    total = row.mass_of(end);
-  }
-  const float p = a.top_p != nullptr ? a.top_p[n] : 1.f;
-  if (p < 1.f) {
-    // the last one kept is the first with which the mass reaches p of the whole; the first element always is one
-    const double want = fmax((double)p, 0.0) * (double)total;
-    const uint64_t least = (uint64_t)ceil(want) > 1 ? (uint64_t)ceil(want) : 1;
-    const Border e = row.find([=](uint64_t m, unsigned) { return m >= least; });
-    if (shorter(e, end)) {
-      end = e;
-      total = row.mass_of(end);
+  row.scale = 1.4426950408889634 / (double)t;
+
+  const bool few = k > 0 && k < vocab;
+  Border end = {0u, 0xffffffffu, 0, -1};
+  // everything on the sorted beginning e of the order, which holds all that is kept
+  auto on_sorted = [&](uint64_t e) {
+    uint64_t total;
+    if (few) {
+      end = row.place(e, [=](uint64_t, unsigned c) { return c >= (unsigned)k; }, 0, 0);
+      total = end.mass;
+    } else {
+      total = row.sum(e == ~0ull ? 0 : row.whole(of_key(~(unsigned)(e >> 32))));
     }
-  }
-  const float q = a.min_p != nullptr ? a.min_p[n] : 0.f;
-  if (q > 0.f) {
-    const Border e = {row.least_key((double)q), q > 1.f ? 1u : 0xffffffffu};  // past 1: the first alone
-    if (shorter(e, end)) {
-      end = e;
-      total = q > 1.f ? row.mass_of(end) : row.mass_of(Border{end.key - 1, 0u});  // those of its key too
+    if (p < 1.f) {
+      const uint64_t least = least_mass(p, total);
+      const Border b = row.place(e, [=](uint64_t m, unsigned) { return m >= least; }, 0, 0);
+      if (shorter(b, end)) {
+        end = b;
+        total = end.mass;
+      }
     }
-  }
-  const float u = a.uniforms[n];
-  const double share = u > 0.f ? (double)u * (double)total : u == u ? 0.0 : (double)total;
-  const uint64_t before = share < (double)total ? min((uint64_t)share, total - 1) : total - 1;
-  const Border drawn = row.find([=](uint64_t m, unsigned) { return m > before; });
-  const int i = row.index_of(drawn.key, drawn.taken);
-  if (threadIdx.x == 0) {
-    a.tokens[n] = i;
-    if (a.logprobs != nullptr) a.logprobs[n] = (float)log(ldexp(row.weight(of_key(drawn.key)), a.bits) / (double)total);
+    if (q > 0.f) {  // a run of the order from its first element on
+      const float v = of_key(~(unsigned)(e >> 32));
+      const bool keep = e != ~0ull && (threadIdx.x == 0 || row.weight(v) >= (double)q);
+      const uint64_t kept = row.sum(keep ? row.whole(v) : 0);
+      total = min(total, kept);
+    }
+    const uint64_t before = mass_before(u, total);
+    const Border drawn = row.place(e, [=](uint64_t m, unsigned) { return m > before; }, 0, 0);
+    give(drawn.index, (float)log(ldexp(row.weight(of_key(drawn.key)), a.bits) / (double)total));
+  };
+  if constexpr (WHOLE) {
+    __syncthreads();  // the table
+    on_sorted(row.sorted([](float) { return true; }));
+  } else {
+    row.clear(bins.mass0, bins.count0);
+    if (few) {
+      row.each([&](float v, int) __attribute__((always_inline)) { atomicAdd(&bins.count0[row.bin(v)], 1u); });
+      __syncthreads();
+      uint64_t m = 0;
+      unsigned c = 0;
+      const int last = row.first_bin(bins.mass0, bins.count0, [=](uint64_t, unsigned n) { return n >= (unsigned)k; }, m, c);
+      if (c + bins.count0[last] <= TH) {
+        on_sorted(row.sorted([&](float v) __attribute__((always_inline)) { return row.bin(v) <= last; }));
+        return;
+      }
+      row.clear(bins.mass0, bins.count0);
+    }
+    uint64_t total = 0;
+    row.each([&](float v, int) __attribute__((always_inline)) {
+      const uint64_t w = row.whole(v);
+      const int b = row.bin(v);
+      total += w;
+      atomicAdd(&bins.count0[b], 1u);
+      atomicAdd((unsigned long long*)&bins.mass0[b], (unsigned long long)w);
+    });
+    total = row.sum(total);
+    if (few) {
+      end = row.find(bins, [=](uint64_t, unsigned c) { return c >= (unsigned)k; });
+      total = end.mass;
+    }
+    if (p < 1.f) {
+      const uint64_t least = least_mass(p, total);
+      const Border b = row.find(bins, [=](uint64_t m, unsigned) { return m >= least; });
+      if (shorter(b, end)) {
+        end = b;
+        total = end.mass;
+      }
+    }
+    if (q > 0.f && (end.taken == 0xffffffffu || row.weight(of_key(end.key)) < (double)q || q > 1.f)) {
+      if (q > 1.f)  // the first alone
+        total = row.whole(row.top);
+      else
+        total = min(total, row.mass_from(row.least_key((double)q)));
+    }
+    const uint64_t before = mass_before(u, total);
+    const Border drawn = row.find(bins, [=](uint64_t m, unsigned) { return m > before; });
+    const int i = drawn.index >= 0 ? drawn.index : row.index_of(drawn.key, drawn.taken);
+    give(i, (float)log(ldexp(row.weight(of_key(drawn.key)), a.bits) / (double)total));
   }
 }
 
 template <typename T>
 int sample_of(const void* logits, const SampleArgs& a, hipStream_t stream) {
-  hipLaunchKernelGGL((sample_rows<T>), dim3((unsigned)a.rows), dim3(THREADS), 0, stream, (const typename T::Storage*)logits, a);
+  typedef typename T::Storage S;
+  const dim3 grid((unsigned)a.rows);
+  if (a.vocab <= 256)
+    hipLaunchKernelGGL((sample_rows<T, 256, true>), grid, dim3(256), 0, stream, (const S*)logits, a);
+  else if (a.vocab <= 1024)
+    hipLaunchKernelGGL((sample_rows<T, 1024, true>), grid, dim3(1024), 0, stream, (const S*)logits, a);
+  else
+    hipLaunchKernelGGL((sample_rows<T, 1024, false>), grid, dim3(1024), 0, stream, (const S*)logits, a);
   return check_hip(hipGetLastError(), "launching sampling");
 }
 
