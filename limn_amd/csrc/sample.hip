@@ -60,14 +60,21 @@ struct Shared {
   unsigned counts[TH / 64];
   uint64_t found_mass, found_element;
   unsigned found_bin, found_count, listed, word;
-  double powers[64];  // 2^(i / 64)
+  double powers[64];  // 2^(F + i / 64)
 };
 template <int TH>
 struct Bins {
   uint64_t mass0[BINS], mass[BINS];
-  unsigned count0[BINS], count[BINS];
+  unsigned count0[BINS], count[BINS];  // count0: where a top-k asks for it
 };
 struct Nothing {};
+
+// What a search looks for: a number of elements, or a mass.
+struct Target {
+  bool counts;
+  uint64_t least;
+  __device__ __forceinline__ bool reached(uint64_t mass, unsigned count) const { return (counts ? (uint64_t)count : mass) >= least; }
+};
 
 // A row of logits, seen by a workgroup of TH threads.
 template <typename T, int TH>
@@ -76,14 +83,17 @@ struct Row {
   static constexpr int PER = 16 / (int)sizeof(S), WAVES = TH / 64;
   const S* x;
   int vocab, bits, head, chunks;  // elements before the first 16-byte boundary, and whole 16-byte chunks from there
-  float top, inv;                 // the largest logit; 1 / temperature
-  double scale;                   // log2(e) / temperature
+  bool infinite;                  // infinite logits have all of the mass: they go as 0, the others as minus infinity
+  float top, inv;                 // the largest logit; 64 / temperature
+  double top64, scale;            // 64 log2(e) / temperature
   Shared<TH>& sh;
 
-  __device__ __forceinline__ Row(const S* x_, int vocab_, int bits_, Shared<TH>& sh_) : x(x_), vocab(vocab_), bits(bits_), top(0.f), inv(0.f), scale(0.0), sh(sh_) {
+  __device__ __forceinline__ Row(const S* x_, int vocab_, int bits_, Shared<TH>& sh_) : x(x_), vocab(vocab_), bits(bits_), infinite(false), top(0.f), inv(0.f), top64(0.0), scale(0.0), sh(sh_) {
     head = min(vocab, (int)((16 - ((uintptr_t)x & 15)) & 15) / (int)sizeof(S));
     chunks = (vocab - head) / PER;
   }
+
+  __device__ __forceinline__ float seen(float v) const { return !infinite ? cleaned(v) : v == __builtin_inff() ? 0.f : -__builtin_inff(); }
 
   // f(logit, index) for every element, some of them by this thread
   template <typename F>
@@ -95,14 +105,15 @@ struct Row {
       u32x4 w[U];
 #pragma unroll
       for (int u = 0; u < U; u++) w[u] = body[c + u * TH];
-#pragma unroll
-      for (int u = 0; u < U; u++) eight(w[u], head + (c + u * TH) * PER, f);
+      // four chunks on their way, one after another worked on by one copy of f's code: four copies' registers spilled
+#pragma unroll 1
+      for (int u = 0; u < U; u++) eight(u < 2 ? u == 0 ? w[0] : w[1] : u == 2 ? w[2] : w[3], head + (c + u * TH) * PER, f);
     }
     for (; c < chunks; c += TH) eight(body[c], head + c * PER, f);
     const int rest = vocab - chunks * PER;  // before and behind the chunks: fewer than 2 PER
     if ((int)threadIdx.x < rest) {
       const int i = (int)threadIdx.x < head ? (int)threadIdx.x : chunks * PER + (int)threadIdx.x;
-      f(cleaned(T::load(x, i)), i);
+      f(seen(T::load(x, i)), i);
     }
   }
   template <typename F>
@@ -110,38 +121,34 @@ struct Row {
 #pragma unroll
     for (int e = 0; e < PER; e++) {
       if constexpr (PER == 4)
-        f(cleaned(__uint_as_float(w[e])), i + e);
+        f(seen(__uint_as_float(w[e])), i + e);
       else
-        f(cleaned(T::unpack((u16)(w[e >> 1] >> (16 * (e & 1))))), i + e);
+        f(seen(T::unpack((u16)(w[e >> 1] >> (16 * (e & 1))))), i + e);
     }
   }
 
-  // 2^F exp((v - top) / temperature) as a whole number: 2^t with t = k / 64 + r, |r| <= 2^-7, 2^(k / 64) from the table and 2^r by
-  // its series, whose first term left out is below 2^-54; the sum with 2^52 rounds it.
-  __device__ __forceinline__ double weight64(float v) const {
-    const double t = ((double)v - (double)top) * scale;
-    const double k = rint(t * 64.0), r = fma(k, -0.015625, t);
-    double p = fma(r, 1.3333558146428443e-3, 9.618129107628477e-3);
-    p = fma(p, r, 5.5504108664821576e-2);
-    p = fma(p, r, 2.402265069591007e-1);
-    p = fma(p, r, 6.931471805599453e-1);
+  // 64 log2 of v's weight, and no less than -70 * 64: such a weight rounds to 0
+  __device__ __forceinline__ double exponent(float v) const { return fmax(((double)v - top64) * scale, -4480.0); }
+  // 2^F exp((v - top) / temperature): 2^(x / 64) with x = k + r, |r| <= 1/2, is 2^(k / 64) from the table times the series of 2^(r / 64),
+  // whose first term left out is below 2^-54.
+  __device__ __forceinline__ double weight(double x) const {
+    const double k = rint(x), r = x - k;
+    double p = fma(r, 1.2417843701716923e-12, 5.732851688640402e-10);
+    p = fma(p, r, 2.1173137155464774e-7);
+    p = fma(p, r, 5.864904955056169e-5);
+    p = fma(p, r, 1.0830424696249145e-2);
     p = fma(p, r, 1.0);
     const int n = (int)k;
-    return ldexp(p * sh.powers[n & 63], n >> 6);
+    const uint64_t w = (uint64_t)__double_as_longlong(p * sh.powers[n & 63]);
+    return __longlong_as_double((long long)(w + ((uint64_t)(unsigned)((n & ~63) << 14) << 32)));  // 2^(n / 64)'s whole part onto the exponent
   }
-  __device__ __forceinline__ double weight(float v) const {
-    if (v == top) return 1.0;
-    const double t = ((double)v - (double)top) * scale;
-    return t > -1000.0 ? weight64(v) : 0.0;
-  }
-  __device__ __forceinline__ uint64_t whole(float v) const {
-    const double w = ldexp(weight(v), bits);  // at most 2^52
-    return (uint64_t)__double_as_longlong(w + 4503599627370496.0) - 0x4330000000000000ull;
-  }
-  // monotone in v: each step rounds, none turns the order round
-  __device__ __forceinline__ int bin(float v) const { return v == top ? 0 : (int)fminf((top - v) * inv * 64.f, (float)(BINS - 1)); }
+  // rounded: the sum with 2^52 has no bits below 1 (a weight is at most 2^52)
+  __device__ __forceinline__ uint64_t whole64(double w) const { return (uint64_t)__double_as_longlong(w + 4503599627370496.0) - 0x4330000000000000ull; }
+  __device__ __forceinline__ uint64_t whole(float v) const { return whole64(weight(exponent(v))); }
+  // 64 bins an e-fold of the weight; monotone in v: each step rounds, none turns the order round
+  __device__ __forceinline__ int bin(float v) const { return v == top ? 0 : (int)fminf((top - v) * inv, (float)(BINS - 1)); }
 
-  __device__ uint64_t sum(uint64_t v) const {
+  __device__ __forceinline__ uint64_t sum(uint64_t v) const {
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) v += __shfl_xor((unsigned long long)v, o);
     __syncthreads();
@@ -184,10 +191,9 @@ struct Row {
     __syncthreads();
   }
 
-  // The first bin at which reached(mass, count) of everything up to and with it is true; the mass and count before it
+  // The first bin at which everything up to and with it reaches the target; the mass and count before it
   // are added to m and c. Every thread gets it; BINS if there is none.
-  template <typename F>
-  __device__ int first_bin(const uint64_t* mass, const unsigned* count, F reached, uint64_t& m, unsigned& c) const {
+  __device__ __forceinline__ int first_bin(const uint64_t* mass, const unsigned* count, Target target, uint64_t& m, unsigned& c) const {
     constexpr int PT = BINS / TH;
     uint64_t pm = 0, bm = m;
     unsigned pc = 0, bc = c;
@@ -198,12 +204,12 @@ struct Row {
     }
     if (threadIdx.x == 0) sh.found_bin = BINS;
     before(pm, pc, bm, bc);
-    if (!reached(bm, bc) && reached(bm + pm, bc + pc)) {  // one thread at most: both grow along the bins
+    if (!target.reached(bm, bc) && target.reached(bm + pm, bc + pc)) {  // one thread at most: both grow along the bins
       int i = 0;
       for (; i + 1 < PT; i++) {
         const uint64_t nm = bm + mass[threadIdx.x * PT + i];
         const unsigned nc = bc + count[threadIdx.x * PT + i];
-        if (reached(nm, nc)) break;
+        if (target.reached(nm, nc)) break;
         bm = nm;
         bc = nc;
       }
@@ -221,7 +227,7 @@ struct Row {
     return b;
   }
 
-  __device__ void clear(uint64_t* mass, unsigned* count) const {
+  __device__ __forceinline__ void clear(uint64_t* mass, unsigned* count) const {
     __syncthreads();
     for (int b = threadIdx.x; b < BINS; b += TH) {
       mass[b] = 0;
@@ -230,10 +236,10 @@ struct Row {
     __syncthreads();
   }
 
-  // The elements that take(logit) is true of, TH of them at most, in the order: each thread gets one (a larger key first, as the
-  // complement of its key above its index), or ~0.
+  // The elements that take(logit) is true of, in the order: each thread gets one (a larger key first, as the complement of its key
+  // above its index), or ~0. More than TH of them: not all.
   template <typename F>
-  __device__ uint64_t sorted(F take) const {
+  __device__ __forceinline__ uint64_t sorted(F take, bool& all) const {
     __syncthreads();
     if (threadIdx.x == 0) sh.listed = 0;
     __syncthreads();
@@ -244,10 +250,13 @@ struct Row {
       }
     });
     __syncthreads();
-    const int n = min((int)sh.listed, TH);
+    all = sh.listed <= TH;
+    if (!all) return ~0ull;
+    const int n = (int)sh.listed;
     uint64_t e = (int)threadIdx.x < n ? sh.list[threadIdx.x] : ~0ull;
     int size = 64;
-    while (size < n) size <<= 1;  // what lies behind is not touched
+    while (size < n) size <<= 1;
+    const bool inside = (int)(threadIdx.x & ~63u) < size;  // waves of nothing but ~0 wait at the barriers
     for (int k = 2; k <= size; k <<= 1)
       for (int j = k >> 1; j > 0; j >>= 1) {
         uint64_t o;
@@ -257,6 +266,7 @@ struct Row {
           __syncthreads();
           o = sh.list[threadIdx.x ^ j];
         } else {
+          if (!inside) continue;
           o = __shfl_xor((unsigned long long)e, j);
         }
         const bool low = (threadIdx.x & j) == 0, up = (threadIdx.x & k) == 0;
@@ -266,14 +276,13 @@ struct Row {
     return e;
   }
 
-  // Of the sorted elements e, before which m and c lie: the first one with which reached(mass, count) is true. Every thread gets it.
-  template <typename F>
-  __device__ Border place(uint64_t e, F reached, uint64_t m, unsigned c) const {
+  // Of the sorted elements e, before which m and c lie: the first one that reaches the target. Every thread gets it.
+  __device__ __forceinline__ Border place(uint64_t e, Target target, uint64_t m, unsigned c) const {
     const float v = of_key(~(unsigned)(e >> 32));
     const uint64_t w = e == ~0ull ? 0 : whole(v);
     if (threadIdx.x == 0) sh.found_element = ~0ull;
     before(w, e == ~0ull ? 0u : 1u, m, c);
-    if (e != ~0ull && !reached(m, c) && reached(m + w, c + 1)) {
+    if (e != ~0ull && !target.reached(m, c) && target.reached(m + w, c + 1)) {
       sh.found_element = e;
       sh.found_mass = m + w;
     }
@@ -292,14 +301,15 @@ struct Row {
     return b;
   }
 
-  // The shortest beginning of the order of which reached(mass, count) is true, from the histogram.
-  template <typename F>
-  __device__ Border find(Bins<TH>& bins, F reached) const {
+  // The shortest beginning of the order that reaches the target, from the histogram.
+  __device__ __forceinline__ Border find(Bins<TH>& bins, Target target) const {
     uint64_t m = 0;
     unsigned c = 0;
-    const int b0 = first_bin(bins.mass0, bins.count0, reached, m, c);
+    const int b0 = first_bin(bins.mass0, bins.count0, target, m, c);
     if (b0 == BINS) return Border{0u, 0xffffffffu, 0, -1};
-    if (bins.count0[b0] <= TH) return place(sorted([&](float v) __attribute__((always_inline)) { return bin(v) == b0; }), reached, m, c);
+    bool all;
+    const uint64_t e = sorted([&](float v) __attribute__((always_inline)) { return bin(v) == b0; }, all);
+    if (all) return place(e, target, m, c);
     unsigned prefix = 0;
     for (int level = 0; level < 3; level++) {
       const int shift = level == 0 ? 21 : level == 1 ? 10 : 0, width = level == 2 ? 10 : 11;
@@ -312,7 +322,7 @@ struct Row {
         atomicAdd((unsigned long long*)&bins.mass[b], (unsigned long long)whole(v));
       });
       __syncthreads();
-      const int b = first_bin(bins.mass, bins.count, reached, m, c);
+      const int b = first_bin(bins.mass, bins.count, target, m, c);
       prefix = (prefix << width) | (unsigned)((1 << width) - 1 - b);
     }
     // equal ones, each of the same mass
@@ -320,52 +330,33 @@ struct Row {
     unsigned lo = 1, hi = bins.count[1023 - (prefix & 1023u)];
     while (lo < hi) {
       const unsigned mid = lo + (hi - lo) / 2;
-      if (reached(m + mid * each_mass, c + mid)) hi = mid; else lo = mid + 1;
+      if (target.reached(m + mid * each_mass, c + mid)) hi = mid; else lo = mid + 1;
     }
     return Border{prefix, lo, m + lo * each_mass, -1};
   }
 
-  // the mass of the elements with this key or a larger one
-  __device__ uint64_t mass_from(unsigned key) const {
-    uint64_t v = 0;
-    each([&](float x, int) __attribute__((always_inline)) {
-      if (key_of(x) >= key) v += whole(x);
-    });
-    return sum(v);
-  }
-
   // the index of the nth element with this key
-  __device__ int index_of(unsigned key, unsigned nth) const {
+  __device__ __forceinline__ int index_of(unsigned key, unsigned nth) const {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    unsigned seen = 0;
+    unsigned passed = 0;
     for (int i0 = 0; i0 < vocab; i0 += TH) {
       const int i = i0 + threadIdx.x;
-      const bool hit = i < vocab && key_of(T::load(x, i)) == key;
+      const bool hit = i < vocab && key_of(seen(T::load(x, i))) == key;
       const uint64_t hits = __ballot(hit);
       __syncthreads();
       if (lane == 0) sh.counts[wave] = (unsigned)__popcll(hits);
       __syncthreads();
-      unsigned mine = seen, all = seen;
+      unsigned mine = passed, all = passed;
       for (int w = 0; w < WAVES; w++) {
         if (w < wave) mine += sh.counts[w];
         all += sh.counts[w];
       }
       if (hit && mine + (unsigned)__popcll(hits & ((1ull << lane) - 1)) + 1 == nth) sh.word = (unsigned)i;
       if (all >= nth) break;
-      seen = all;
+      passed = all;
     }
     __syncthreads();
     return (int)sh.word;
-  }
-
-  // the least key whose weight is p or more (the largest logit's at least)
-  __device__ unsigned least_key(double p) const {
-    unsigned lo = 0, hi = key_of(top);
-    while (lo < hi) {
-      const unsigned mid = lo + (hi - lo) / 2;
-      if (weight(of_key(mid)) >= p) hi = mid; else lo = mid + 1;
-    }
-    return hi;
   }
 };
 
@@ -390,7 +381,7 @@ __global__ __launch_bounds__(TH) void sample_rows(const typename T::Storage* __r
   const int vocab = (int)a.vocab;
   const float t = a.temperature != nullptr ? a.temperature[n] : 1.f, p = a.top_p != nullptr ? a.top_p[n] : 1.f, q = a.min_p != nullptr ? a.min_p[n] : 0.f, u = a.uniforms[n];
   const int k = a.top_k != nullptr ? a.top_k[n] : 0;
-  if (threadIdx.x < 64) sh.powers[threadIdx.x] = exp2(threadIdx.x * 0.015625);
+  if (threadIdx.x < 64) sh.powers[threadIdx.x] = exp2(a.bits + threadIdx.x * 0.015625);
   Row<T, TH> row(logits + n * a.row_stride, vocab, a.bits, sh);
   float best = -__builtin_inff();
   row.each([&](float v, int) __attribute__((always_inline)) { best = fmaxf(best, v); });
@@ -422,42 +413,20 @@ __global__ __launch_bounds__(TH) void sample_rows(const typename T::Storage* __r
     give((int)sh.word, 0.f);
     return;
   }
-  row.top = best + 0.f;
-  row.inv = 1.f / t;
-  row.scale = 1.4426950408889634 / (double)t;
+  row.infinite = best == __builtin_inff();
+  row.top = row.infinite ? 0.f : best + 0.f;
+  row.top64 = (double)row.top;
+  row.inv = 64.f / t;
+  row.scale = 64.0 * 1.4426950408889634 / (double)t;
 
+  const double one = ldexp(1.0, a.bits);  // the largest weight
   const bool few = k > 0 && k < vocab;
-  Border end = {0u, 0xffffffffu, 0, -1};
-  // everything on the sorted beginning e of the order, which holds all that is kept
-  auto on_sorted = [&](uint64_t e) {
-    uint64_t total;
-    if (few) {
-      end = row.place(e, [=](uint64_t, unsigned c) { return c >= (unsigned)k; }, 0, 0);
-      total = end.mass;
-    } else {
-      total = row.sum(e == ~0ull ? 0 : row.whole(of_key(~(unsigned)(e >> 32))));
-    }
-    if (p < 1.f) {
-      const uint64_t least = least_mass(p, total);
-      const Border b = row.place(e, [=](uint64_t m, unsigned) { return m >= least; }, 0, 0);
-      if (shorter(b, end)) {
-        end = b;
-        total = end.mass;
-      }
-    }
-    if (q > 0.f) {  // a run of the order from its first element on
-      const float v = of_key(~(unsigned)(e >> 32));
-      const bool keep = e != ~0ull && (threadIdx.x == 0 || row.weight(v) >= (double)q);
-      const uint64_t kept = row.sum(keep ? row.whole(v) : 0);
-      total = min(total, kept);
-    }
-    const uint64_t before = mass_before(u, total);
-    const Border drawn = row.place(e, [=](uint64_t m, unsigned) { return m > before; }, 0, 0);
-    give(drawn.index, (float)log(ldexp(row.weight(of_key(drawn.key)), a.bits) / (double)total));
-  };
+  // either all that is kept, sorted, or a histogram
+  bool whole = WHOLE;
+  uint64_t e = ~0ull, total = 0, kept = 0;
+  const double least_weight = (double)q * one;
   if constexpr (WHOLE) {
-    __syncthreads();  // the table
-    on_sorted(row.sorted([](float) { return true; }));
+    e = row.sorted([](float) __attribute__((always_inline)) { return true; }, whole);
   } else {
     row.clear(bins.mass0, bins.count0);
     if (few) {
@@ -465,45 +434,51 @@ __global__ __launch_bounds__(TH) void sample_rows(const typename T::Storage* __r
       __syncthreads();
       uint64_t m = 0;
       unsigned c = 0;
-      const int last = row.first_bin(bins.mass0, bins.count0, [=](uint64_t, unsigned n) { return n >= (unsigned)k; }, m, c);
-      if (c + bins.count0[last] <= TH) {
-        on_sorted(row.sorted([&](float v) __attribute__((always_inline)) { return row.bin(v) <= last; }));
-        return;
-      }
-      row.clear(bins.mass0, bins.count0);
+      const int last = row.first_bin(bins.mass0, bins.count0, Target{true, (uint64_t)k}, m, c);
+      if (c + bins.count0[last] <= TH) e = row.sorted([&](float v) __attribute__((always_inline)) { return row.bin(v) <= last; }, whole);
     }
-    uint64_t total = 0;
-    row.each([&](float v, int) __attribute__((always_inline)) {
-      const uint64_t w = row.whole(v);
-      const int b = row.bin(v);
-      total += w;
-      atomicAdd(&bins.count0[b], 1u);
-      atomicAdd((unsigned long long*)&bins.mass0[b], (unsigned long long)w);
-    });
-    total = row.sum(total);
-    if (few) {
-      end = row.find(bins, [=](uint64_t, unsigned c) { return c >= (unsigned)k; });
-      total = end.mass;
+    if (!whole) {  // the masses; of the last bin, which may have most of the elements, in registers
+      uint64_t rest = 0;
+      row.each([&](float v, int) __attribute__((always_inline)) {
+        const double w = row.weight(row.exponent(v));
+        const uint64_t m = row.whole64(w);
+        const int b = row.bin(v);
+        total += m;
+        kept += w >= least_weight ? m : 0;
+        if (b < BINS - 1)
+          atomicAdd((unsigned long long*)&bins.mass0[b], (unsigned long long)m);
+        else
+          rest += m;
+      });
+      rest = row.sum(rest);
+      if (threadIdx.x == 0) bins.mass0[BINS - 1] = rest;
     }
-    if (p < 1.f) {
-      const uint64_t least = least_mass(p, total);
-      const Border b = row.find(bins, [=](uint64_t m, unsigned) { return m >= least; });
-      if (shorter(b, end)) {
-        end = b;
-        total = end.mass;
-      }
-    }
-    if (q > 0.f && (end.taken == 0xffffffffu || row.weight(of_key(end.key)) < (double)q || q > 1.f)) {
-      if (q > 1.f)  // the first alone
-        total = row.whole(row.top);
-      else
-        total = min(total, row.mass_from(row.least_key((double)q)));
-    }
-    const uint64_t before = mass_before(u, total);
-    const Border drawn = row.find(bins, [=](uint64_t m, unsigned) { return m > before; });
-    const int i = drawn.index >= 0 ? drawn.index : row.index_of(drawn.key, drawn.taken);
-    give(i, (float)log(ldexp(row.weight(of_key(drawn.key)), a.bits) / (double)total));
   }
+  if (whole) {
+    const double w = e == ~0ull ? 0.0 : row.weight(row.exponent(of_key(~(unsigned)(e >> 32))));
+    total = row.whole64(w);
+    kept = threadIdx.x == 0 || w >= least_weight ? total : 0;
+  }
+  total = row.sum(total);
+  if (q > 0.f) kept = row.sum(kept);
+  Border end = {0u, 0xffffffffu, 0, -1}, b;
+  // top-k, top-p, and with all that is kept known, the draw
+  for (int step = few ? 0 : p < 1.f ? 1 : 2; step < 3; step++) {
+    if (step == 1 && !(p < 1.f)) continue;
+    if (step == 2 && q > 0.f) total = min(total, q > 1.f ? row.whole(row.top) : kept);  // past 1: the first alone
+    const Target target = {step == 0, step == 0 ? (uint64_t)k : step == 1 ? least_mass(p, total) : mass_before(u, total) + 1};
+    if constexpr (WHOLE) {
+      b = row.place(e, target, 0, 0);
+    } else {
+      b = whole ? row.place(e, target, 0, 0) : row.find(bins, target);
+    }
+    if (step < 2 && shorter(b, end)) {
+      end = b;
+      total = b.mass;
+    }
+  }
+  const int i = b.index >= 0 ? b.index : row.index_of(b.key, b.taken);
+  give(i, (float)log(row.weight(row.exponent(of_key(b.key))) / (double)total));
 }
 
 template <typename T>
