@@ -46,13 +46,18 @@ __device__ __forceinline__ unsigned key_of(float x) {
 }
 __device__ __forceinline__ float of_key(unsigned k) { return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k); }
 
-// The first elements of the order: those with a larger key, and `taken` of those with this one; and what they hold.
+constexpr unsigned NOTHING = 0x007fffffu;  // the key of minus infinity
+
+// The first elements of the order: those with a larger key, and of those with this one the ones up to an index or, where it is not
+// known (-1), `taken` of them; and their mass. Borders with the same key are found the same way.
 struct Border {
   unsigned key, taken;
+  int index;
   uint64_t mass;
-  int index;  // of the last of them; -1: not looked for
 };
-__device__ __forceinline__ bool shorter(const Border& a, const Border& b) { return a.key > b.key || (a.key == b.key && a.taken < b.taken); }
+__device__ __forceinline__ bool shorter(const Border& a, const Border& b) {
+  return a.key > b.key || (a.key == b.key && (a.index >= 0 ? a.index < b.index : a.taken < b.taken));
+}
 
 template <int TH>
 struct Shared {
@@ -236,15 +241,30 @@ struct Row {
     __syncthreads();
   }
 
-  // The elements that take(logit) is true of, in the order: each thread gets one (a larger key first, as the complement of its key
-  // above its index), or ~0. More than TH of them: not all.
-  template <typename F>
-  __device__ __forceinline__ uint64_t sorted(F take, bool& all) const {
+  // The least logit of bin b or a bin before it: 64 keys between the ones that are known are looked at at a time, by every wave.
+  __device__ __forceinline__ float edge(int b) const {
+    unsigned lo = NOTHING, hi = key_of(top);  // bin(of_key(hi)) <= b
+    while (lo < hi) {
+      const unsigned step = (hi - lo) / 64 + 1, lane = threadIdx.x & 63;
+      auto probe = [&](unsigned l) __attribute__((always_inline)) { return hi - min(hi - lo, step * (l + 1)); };
+      const uint64_t bad = ~__ballot(bin(of_key(probe(lane))) <= b);  // lanes from some one on
+      const unsigned good = bad == 0 ? 64u : (unsigned)__builtin_ctzll(bad);
+      const unsigned least = good == 0 ? hi : probe(good - 1);
+      lo = bad == 0 ? least : probe(good) + 1;
+      hi = least;
+    }
+    return of_key(hi);
+  }
+
+  // The elements of the row from lo to hi (all of them, if ALL), in the order: each thread gets one (a larger key first, as the
+  // complement of its key above its index), or ~0. More than TH of them: not all.
+  template <bool ALL>
+  __device__ __forceinline__ uint64_t sorted(float lo, float hi, bool& all) const {
     __syncthreads();
     if (threadIdx.x == 0) sh.listed = 0;
     __syncthreads();
     each([&](float v, int i) __attribute__((always_inline)) {
-      if (take(v)) {
+      if (ALL || (v >= lo && v <= hi)) {
         const unsigned at = atomicAdd(&sh.listed, 1u);
         if (at < TH) sh.list[at] = ((uint64_t)~key_of(v) << 32) | (unsigned)i;
       }
@@ -254,49 +274,49 @@ struct Row {
     if (!all) return ~0ull;
     const int n = (int)sh.listed;
     uint64_t e = (int)threadIdx.x < n ? sh.list[threadIdx.x] : ~0ull;
-    int size = 64;
-    while (size < n) size <<= 1;
-    const bool inside = (int)(threadIdx.x & ~63u) < size;  // waves of nothing but ~0 wait at the barriers
-    for (int k = 2; k <= size; k <<= 1)
-      for (int j = k >> 1; j > 0; j >>= 1) {
-        uint64_t o;
-        if (j >= 64) {
-          __syncthreads();
-          sh.list[threadIdx.x] = e;
-          __syncthreads();
-          o = sh.list[threadIdx.x ^ j];
-        } else {
-          if (!inside) continue;
-          o = __shfl_xor((unsigned long long)e, j);
-        }
-        const bool low = (threadIdx.x & j) == 0, up = (threadIdx.x & k) == 0;
-        if (low == up ? o < e : o > e) e = o;
+    const int wave0 = (int)(threadIdx.x & ~63u);
+    if (n <= 512) {  // the place of each is the number of those before it: n reads that all lanes share; a sorting network of 36 steps took 6 us for 256
+      int rank = 0;
+      if (wave0 < n) {
+#pragma unroll 8
+        for (int j = 0; j < n; j++) rank += sh.list[j] < e;
       }
+      __syncthreads();
+      if ((int)threadIdx.x < n) sh.list[rank] = e;
+      __syncthreads();
+      e = (int)threadIdx.x < n ? sh.list[threadIdx.x] : ~0ull;
+    } else {
+      for (int k = 2; k <= TH; k <<= 1)
+        for (int j = k >> 1; j > 0; j >>= 1) {
+          uint64_t o;
+          if (j >= 64) {
+            __syncthreads();
+            sh.list[threadIdx.x] = e;
+            __syncthreads();
+            o = sh.list[threadIdx.x ^ j];
+          } else {
+            o = __shfl_xor((unsigned long long)e, j);
+          }
+          const bool low = (threadIdx.x & j) == 0, up = (threadIdx.x & k) == 0;
+          if (low == up ? o < e : o > e) e = o;
+        }
+    }
     __syncthreads();
     return e;
   }
 
-  // Of the sorted elements e, before which m and c lie: the first one that reaches the target. Every thread gets it.
-  __device__ __forceinline__ Border place(uint64_t e, Target target, uint64_t m, unsigned c) const {
-    const float v = of_key(~(unsigned)(e >> 32));
-    const uint64_t w = e == ~0ull ? 0 : whole(v);
+  // Of the sorted elements e, each with its mass w and the mass m and count c before it: the first one that reaches the target. Every
+  // thread gets it.
+  __device__ __forceinline__ Border place(uint64_t e, uint64_t w, Target target, uint64_t m, unsigned c) const {
     if (threadIdx.x == 0) sh.found_element = ~0ull;
-    before(w, e == ~0ull ? 0u : 1u, m, c);
+    __syncthreads();
     if (e != ~0ull && !target.reached(m, c) && target.reached(m + w, c + 1)) {
       sh.found_element = e;
       sh.found_mass = m + w;
     }
     __syncthreads();
-    Border b = {0u, 0xffffffffu, 0, -1};
     const uint64_t f = sh.found_element;
-    if (f != ~0ull) {
-      b = Border{~(unsigned)(f >> 32), 0u, sh.found_mass, (int)(unsigned)f};
-      if (threadIdx.x == 0) sh.word = 0;
-      __syncthreads();  // how many with its key come up to it
-      if (e != ~0ull && (e >> 32) == (f >> 32) && e <= f) atomicAdd(&sh.word, 1u);
-      __syncthreads();
-      b.taken = sh.word;
-    }
+    const Border b = f == ~0ull ? Border{0u, 0xffffffffu, 0x7fffffff, 0} : Border{~(unsigned)(f >> 32), 0u, (int)(unsigned)f, sh.found_mass};
     __syncthreads();
     return b;
   }
@@ -306,10 +326,14 @@ struct Row {
     uint64_t m = 0;
     unsigned c = 0;
     const int b0 = first_bin(bins.mass0, bins.count0, target, m, c);
-    if (b0 == BINS) return Border{0u, 0xffffffffu, 0, -1};
+    if (b0 == BINS) return Border{0u, 0xffffffffu, 0x7fffffff, 0};
     bool all;
-    const uint64_t e = sorted([&](float v) __attribute__((always_inline)) { return bin(v) == b0; }, all);
-    if (all) return place(e, target, m, c);
+    const uint64_t e = sorted<false>(edge(b0), b0 == 0 ? __builtin_inff() : of_key(key_of(edge(b0 - 1)) - 1), all);
+    if (all) {
+      const uint64_t w = e == ~0ull ? 0 : whole(of_key(~(unsigned)(e >> 32)));
+      before(w, e == ~0ull ? 0u : 1u, m, c);
+      return place(e, w, target, m, c);
+    }
     unsigned prefix = 0;
     for (int level = 0; level < 3; level++) {
       const int shift = level == 0 ? 21 : level == 1 ? 10 : 0, width = level == 2 ? 10 : 11;
@@ -332,7 +356,7 @@ struct Row {
       const unsigned mid = lo + (hi - lo) / 2;
       if (target.reached(m + mid * each_mass, c + mid)) hi = mid; else lo = mid + 1;
     }
-    return Border{prefix, lo, m + lo * each_mass, -1};
+    return Border{prefix, lo, -1, m + lo * each_mass};
   }
 
   // the index of the nth element with this key
@@ -426,7 +450,7 @@ __global__ __launch_bounds__(TH) void sample_rows(const typename T::Storage* __r
   uint64_t e = ~0ull, total = 0, kept = 0;
   const double least_weight = (double)q * one;
   if constexpr (WHOLE) {
-    e = row.sorted([](float) __attribute__((always_inline)) { return true; }, whole);
+    e = row.template sorted<true>(0.f, 0.f, whole);
   } else {
     row.clear(bins.mass0, bins.count0);
     if (few) {
@@ -435,7 +459,7 @@ __global__ __launch_bounds__(TH) void sample_rows(const typename T::Storage* __r
       uint64_t m = 0;
       unsigned c = 0;
       const int last = row.first_bin(bins.mass0, bins.count0, Target{true, (uint64_t)k}, m, c);
-      if (c + bins.count0[last] <= TH) e = row.sorted([&](float v) __attribute__((always_inline)) { return row.bin(v) <= last; }, whole);
+      if (c + bins.count0[last] <= TH) e = row.template sorted<false>(row.edge(last), __builtin_inff(), whole);
     }
     if (!whole) {  // the masses; of the last bin, which may have most of the elements, in registers
       uint64_t rest = 0;
@@ -454,23 +478,26 @@ __global__ __launch_bounds__(TH) void sample_rows(const typename T::Storage* __r
       if (threadIdx.x == 0) bins.mass0[BINS - 1] = rest;
     }
   }
+  uint64_t w = 0, m = 0;  // sorted: this thread's element's mass, and the mass before it
   if (whole) {
-    const double w = e == ~0ull ? 0.0 : row.weight(row.exponent(of_key(~(unsigned)(e >> 32))));
-    total = row.whole64(w);
-    kept = threadIdx.x == 0 || w >= least_weight ? total : 0;
+    const double x = e == ~0ull ? 0.0 : row.weight(row.exponent(of_key(~(unsigned)(e >> 32))));
+    total = w = row.whole64(x);
+    kept = threadIdx.x == 0 || x >= least_weight ? w : 0;
+    unsigned c = 0;
+    row.before(w, 0u, m, c);
   }
   total = row.sum(total);
   if (q > 0.f) kept = row.sum(kept);
-  Border end = {0u, 0xffffffffu, 0, -1}, b;
+  Border end = {0u, 0xffffffffu, 0x7fffffff, 0}, b;
   // top-k, top-p, and with all that is kept known, the draw
   for (int step = few ? 0 : p < 1.f ? 1 : 2; step < 3; step++) {
     if (step == 1 && !(p < 1.f)) continue;
     if (step == 2 && q > 0.f) total = min(total, q > 1.f ? row.whole(row.top) : kept);  // past 1: the first alone
     const Target target = {step == 0, step == 0 ? (uint64_t)k : step == 1 ? least_mass(p, total) : mass_before(u, total) + 1};
     if constexpr (WHOLE) {
-      b = row.place(e, target, 0, 0);
+      b = row.place(e, w, target, m, threadIdx.x);
     } else {
-      b = whole ? row.place(e, target, 0, 0) : row.find(bins, target);
+      b = whole ? row.place(e, w, target, m, threadIdx.x) : row.find(bins, target);
     }
     if (step < 2 && shorter(b, end)) {
       end = b;
