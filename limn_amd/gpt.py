@@ -23,6 +23,8 @@ attention are bf16. The backward of each cast hands float32 gradients to the mas
 Off by default and beside the C5 workload, the configuration has the variants that `attend` and
 `linear_cross_entropy` serve: fewer key heads than query heads, capped scores, a distance penalty in
 place of learned positions, several documents packed into each row, and the head's loss without logits.
+
+`GPT.extend` is the same model over new tokens and a paged cache of the ones before; `limn_amd.serve` answers with it.
 """
 
 from __future__ import annotations
@@ -33,6 +35,8 @@ from dataclasses import dataclass
 import numpy as np
 
 from limn_amd.attend import attend
+from limn_amd.int8 import int8_linear
+from limn_amd.paged import attend_paged
 from limn_amd.seam import DType, Node, Op, Tensor, bfloat16, float32, int32, nn, optim
 from limn_amd.xent import linear_cross_entropy
 
@@ -99,8 +103,19 @@ def materialized(x: Tensor) -> Tensor:
     return Tensor.from_node(Node(Op.CONTIGUOUS, (x.node,), x.dtype, x.shape), (x,), lambda g: (materialized(g),))
 
 
-def mixed(layer: Linear, x: Tensor) -> Tensor:
+@dataclass(frozen=True)
+class Held:
+    """A Linear's weight as answering reads it: cast once, or int8 with a scale for each output."""
+
+    weight: Tensor
+    bias: Tensor | None
+    scales: Tensor | None = None
+
+
+def mixed(layer: Linear | Held, x: Tensor) -> Tensor:
     """A Linear with its float32 weight and bias cast to x's dtype at use."""
+    if isinstance(layer, Held) and layer.scales is not None:
+        return int8_linear(x, layer.weight, layer.scales, layer.bias)
     y = x @ layer.weight.cast(x.dtype).transpose()
     return y if layer.bias is None else y + layer.bias.cast(x.dtype)
 
@@ -138,6 +153,17 @@ class Block:
             q, k, v = heads(qkv[:, :, :at]), heads(qkv[:, :, at : at + kv]), heads(qkv[:, :, at + kv :])
         return attend(q, k, v, causal=True, softcap=cfg.softcap, slopes=slopes, documents=documents)
 
+    def extend(self, x: Tensor, pages: tuple[Tensor, Tensor], where: tuple[Tensor, Tensor, Tensor], slopes: Tensor | None) -> Tensor:
+        """The rows x (tokens, dim) of new tokens through the block, over `pages` of the keys and values before them; `where`:
+        starts, lengths and table, as `attend_paged` takes them."""
+        n, c = x.shape
+        cfg, hd = self.cfg, self.cfg.dim // self.heads
+        qkv, kv = mixed(self.qkv, normed(self.ln1, x)), cfg.key_heads * hd
+        q, k, v = (part.reshape(n, -1, hd) for part in (qkv[:, :c], qkv[:, c : c + kv], qkv[:, c + kv :]))
+        att = attend_paged(q, k, v, *pages, *where, softcap=cfg.softcap, slopes=slopes)
+        x = materialized(x + mixed(self.proj, att.reshape(n, c)))
+        return materialized(x + mixed(self.down, gelu(mixed(self.up, normed(self.ln2, x)))))
+
 
 class GPT:
     def __init__(self, cfg: GPTConfig):
@@ -160,6 +186,17 @@ class GPT:
         x = materialized(x.cast(self.cfg.dtype))
         for block in self.blocks:
             x = block(x, self.slopes, documents)
+        return normed(self.ln, x)
+
+    def extend(self, tokens: Tensor, positions: Tensor, pages: list[tuple[Tensor, Tensor]], where: tuple[Tensor, Tensor, Tensor]) -> Tensor:
+        """The last rows (tokens, dim) of packed new tokens (tokens,) at their positions (tokens,), both int32, over each block's pages
+        of what came before; what `rows` gives for them in the whole of their sequences."""
+        x = self.tok(tokens)
+        if self.slopes is None:
+            x = x + self.pos(positions)
+        x = materialized(x.cast(self.cfg.dtype))
+        for block, own in zip(self.blocks, pages):
+            x = block.extend(x, own, where, self.slopes)
         return normed(self.ln, x)
 
     def __call__(self, tokens: Tensor, documents: Tensor | None = None) -> Tensor:

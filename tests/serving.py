@@ -6,6 +6,9 @@ import numpy as np
 
 from conftest import DTYPES, storage_values
 
+from limn_amd.gpt import mixed, normed
+from limn_amd.seam import Tensor, float32, int32
+
 
 def paged_inputs(seed, dtype="float32", counts=(1,), lengths=(5,), heads=2, kv_heads=None, hd=8, page=4, spare=0, table_pages=None, slopes=False, std=1.0, rows_before=0):
     """Packed tokens, pools whose pages are dealt at random, a table with -1 behind each sequence's pages."""
@@ -29,3 +32,17 @@ def paged_inputs(seed, dtype="float32", counts=(1,), lengths=(5,), heads=2, kv_h
 def logit_rows(seed, rows, vocab, dtype="float32", spread=2.5):
     rng = np.random.default_rng(seed)
     return storage_values((rng.standard_normal((rows, vocab)) * spread).astype(np.float32), DTYPES[dtype]), rng.random(rows).astype(np.float32), rng
+
+
+PROMPTS = [[1, 2, 3, 4, 5], [7], [9, 8, 7, 6, 5, 4, 3, 2, 1, 0, 11], [30, 31]]
+
+
+def whole_logits(model, tokens) -> np.ndarray:
+    """The logits (tokens, vocab) of a whole sequence through the model as training runs it."""
+    x = model.tok(Tensor(np.array([tokens], dtype=np.int32), dtype=int32))
+    if model.slopes is None:
+        x = x + model.pos(Tensor.arange(len(tokens)))
+    x = x.cast(model.cfg.dtype)
+    for block in model.blocks:
+        x = block(x, model.slopes, None)
+    return mixed(model.head, normed(model.ln, x)).cast(float32).numpy()[0]
