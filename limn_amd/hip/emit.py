@@ -1822,6 +1822,8 @@ def bias_cast(nests: list[LoopNest], bias: Node, reader: int, kept: set) -> int 
 
 INLINE_CELLS = 1 << 16  # the largest producer evaluated in its readers instead of launched
 INLINE_BODY = 24  # ... and the most instructions in its body
+INLINE_WHOLE = 48  # ... and with the producers evaluated in it: a float32 residual stream of few rows is a chain of small sums, and each read all before it again
+# (a training step of 4 float32 layers, 1 x 64 x 512: 8670 us without this bound, 3530 at 96, 2230 at 48; 5 other small steps, bfloat16, the same)
 
 
 class InlineSet:
@@ -1914,7 +1916,7 @@ def inline_producers(nests: list[LoopNest], plans: list[Planned], kept: set | No
     kernel (reference limn/schedule.py:46-141), a launch of a few microseconds for a few
     kilobytes. A producer qualifies when its output is not kept (a sink or a CUSTOM input;
     `kept` None inlines nothing), it has at most INLINE_CELLS cells and INLINE_BODY
-    instructions, and every reader is an emitted nest (not a contraction, not a relu epilogue)
+    instructions (INLINE_WHOLE with those of the producers evaluated in it), and every reader is an emitted nest (not a contraction, not a relu epilogue)
     that reads it by plain loads. Its inputs stay valid for the whole plan: the executor keeps
     every buffer of a transaction and commits assigns only at its end."""
     if kept is None:
@@ -1925,6 +1927,7 @@ def inline_producers(nests: list[LoopNest], plans: list[Planned], kept: set | No
         for node in nest.kernel.inputs:
             readers.setdefault(node, set()).add(c)
     chosen: set[int] = set()
+    whole: dict = {}  # a chosen producer's output -> the instructions of its body and of those evaluated in it
     for j, (nest, plan) in enumerate(zip(nests, plans)):
         target = nest.kernel.target
         if not plan.notes.get("elementwise") or j in fused or target in kept or target not in readers:
@@ -1933,7 +1936,8 @@ def inline_producers(nests: list[LoopNest], plans: list[Planned], kept: set | No
             continue
         if not _stores_its_cells(nest):
             continue
-        ok = True
+        size = len(read_nest(nest).body) + sum(whole.get(n, 0) for n in nest.kernel.inputs)
+        ok = size <= INLINE_WHOLE
         for c in readers[target]:
             if c in fused or plans[c].contraction is not None or c <= j:
                 ok = False
@@ -1944,6 +1948,7 @@ def inline_producers(nests: list[LoopNest], plans: list[Planned], kept: set | No
                 break
         if ok:
             chosen.add(j)
+            whole[target] = size
     return chosen
 
 
