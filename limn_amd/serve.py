@@ -15,6 +15,7 @@ from collections.abc import Sequence
 
 import numpy as np
 
+from limn_amd.attend import contiguous
 from limn_amd.gpt import GPT, Held, Linear, mixed
 from limn_amd.int8 import quantize_rows
 from limn_amd.sampling import sample
@@ -50,7 +51,9 @@ class Cache:
         shape = (pages, cfg.key_heads, page, cfg.dim // cfg.heads)
         self.page = page
         self.free = list(range(pages))[::-1]
-        self.layers = [(Tensor.zeros(shape, dtype=dtype or cfg.dtype), Tensor.zeros(shape, dtype=dtype or cfg.dtype)) for _ in model.blocks]
+        zero = Tensor.zeros((1, 1, 1, 1), dtype=dtype or cfg.dtype).expand(*shape)
+        self.layers = [(contiguous(zero), contiguous(zero)) for _ in model.blocks]  # filled on the device
+        realize(*(pool for pools in self.layers for pool in pools))
         self.tables: dict[int, list[int]] = {}
 
     def reserve(self, sequence: int, length: int) -> None:
