@@ -5,10 +5,15 @@
 // running mass (top-p, the draw) passes a number. A row has a workgroup, which reads it
 //  - for its largest logit;
 //  - into a histogram of 2048 bins of equal width in (max - x) / temperature (of counts alone, if there is a top-k);
-//  - for the members of the bins that matter, at most a thousand, which it sorts: with a top-k those of all bins up to the border's,
-//    and everything else is done on them; without, those of one bin for every border.
-// Rows of up to 1024 logits are sorted whole. A bin with more members (rows of equal logits) is taken apart by the bits of x
-// instead, 11, 11 and 10 at a time.
+//  - for the members of the bins that matter, which it sorts: with a top-k those of all bins up to the border's, and everything
+//    else is done on them; with a top-p that of its border and the ones that the draw can end in; or the draw's alone.
+// Rows of up to 1024 logits are sorted whole. A bin with more than 1024 members (rows of equal logits) is taken apart by the bits
+// of x instead, 11, 11 and 10 at a time.
+//
+// What bounds it: 256 rows of 131072 bfloat16 logits, a workgroup a CU, take 130 us: 19 for the largest (the 67 MB come once from
+// memory and then from the last cache), 48 for the masses, which is the rate of 64-bit atomics on shared memory (48 cycles for 64
+// of them), 24 for the members, 20 for sorting and placing. 64 rows of 32000 with a top-k take 29 us, one row of 131072 40, chains of
+// small steps; up to 256 logits 10.
 //
 // Masses are whole numbers, w 2^F rounded with F such that a row's sum stays below 2^63: sums of them do not depend on
 // the order that atomics come in, and they are exact to V 2^-F of the largest weight (2^-28 of it for 2^17 tokens at
@@ -61,7 +66,7 @@ __device__ __forceinline__ bool shorter(const Border& a, const Border& b) {
 
 template <int TH>
 struct Shared {
-  uint64_t list[TH], sums[TH / 64];
+  uint64_t list[TH], sums[TH / 64];  // list: of elements, see Row::append
   unsigned counts[TH / 64];
   uint64_t found_mass, found_element;
   unsigned found_bin, found_count, listed, word;
@@ -71,6 +76,9 @@ template <int TH>
 struct Bins {
   uint64_t mass0[BINS], mass[BINS];
   unsigned count0[BINS], count[BINS];  // count0: where a top-k asks for it
+  uint64_t list[2][TH];
+  unsigned listed[2];
+  float least[3], most[3];  // the logits of three bins
 };
 struct Nothing {};
 
@@ -88,17 +96,17 @@ struct Row {
   static constexpr int PER = 16 / (int)sizeof(S), WAVES = TH / 64;
   const S* x;
   int vocab, bits, head, chunks;  // elements before the first 16-byte boundary, and whole 16-byte chunks from there
-  bool infinite;                  // infinite logits have all of the mass: they go as 0, the others as minus infinity
+  float least, most;              // infinite logits have all of the mass: they go as the largest number, all others as minus infinity
   float top, inv;                 // the largest logit; 64 / temperature
   double top64, scale;            // 64 log2(e) / temperature
   Shared<TH>& sh;
 
-  __device__ __forceinline__ Row(const S* x_, int vocab_, int bits_, Shared<TH>& sh_) : x(x_), vocab(vocab_), bits(bits_), infinite(false), top(0.f), inv(0.f), top64(0.0), scale(0.0), sh(sh_) {
+  __device__ __forceinline__ Row(const S* x_, int vocab_, int bits_, Shared<TH>& sh_) : x(x_), vocab(vocab_), bits(bits_), least(-__builtin_inff()), most(__builtin_inff()), top(0.f), inv(0.f), top64(0.0), scale(0.0), sh(sh_) {
     head = min(vocab, (int)((16 - ((uintptr_t)x & 15)) & 15) / (int)sizeof(S));
     chunks = (vocab - head) / PER;
   }
 
-  __device__ __forceinline__ float seen(float v) const { return !infinite ? cleaned(v) : v == __builtin_inff() ? 0.f : -__builtin_inff(); }
+  __device__ __forceinline__ float seen(float v) const { return v >= least ? fminf(v, most) : -__builtin_inff(); }
 
   // f(logit, index) for every element, some of them by this thread
   template <typename F>
@@ -232,6 +240,20 @@ struct Row {
     return b;
   }
 
+  // The same for a mass alone, where the sums along the bins are at hand: bm before this thread's two, m0 in the first of them.
+  __device__ __forceinline__ int bin_at(uint64_t bm, uint64_t m0, uint64_t m1, uint64_t least, uint64_t& m) const {
+    if (bm < least && least <= bm + m0 + m1) {  // one thread
+      const bool second = bm + m0 < least;
+      sh.found_bin = threadIdx.x * 2 + second;
+      sh.found_mass = second ? bm + m0 : bm;
+    }
+    __syncthreads();
+    const int b = sh.found_bin;
+    m = sh.found_mass;
+    __syncthreads();
+    return b;
+  }
+
   __device__ __forceinline__ void clear(uint64_t* mass, unsigned* count) const {
     __syncthreads();
     for (int b = threadIdx.x; b < BINS; b += TH) {
@@ -256,44 +278,53 @@ struct Row {
     return of_key(hi);
   }
 
-  // The elements of the row from lo to hi (all of them, if ALL), in the order: each thread gets one (a larger key first, as the
-  // complement of its key above its index), or ~0. More than TH of them: not all.
-  template <bool ALL>
-  __device__ __forceinline__ uint64_t sorted(float lo, float hi, bool& all) const {
+  // ... and the largest of bin b
+  __device__ __forceinline__ float largest(int b) const { return b == 0 ? __builtin_inff() : of_key(key_of(edge(b - 1)) - 1); }
+
+  // list takes an element (a larger key first, as the complement of its key above its index)
+  __device__ __forceinline__ void append(uint64_t* list, unsigned& listed, float v, int i) const {
+    const unsigned at = atomicAdd(&listed, 1u);
+    if (at < TH) list[at] = ((uint64_t)~key_of(v) << 32) | (unsigned)i;
+  }
+
+  // The elements of the row that in(logit) is true of, in the order: each thread gets one as it is listed, or ~0. More than TH of
+  // them: not all.
+  template <typename F>
+  __device__ __forceinline__ uint64_t sorted(F in, bool& all) const {
     __syncthreads();
     if (threadIdx.x == 0) sh.listed = 0;
     __syncthreads();
     each([&](float v, int i) __attribute__((always_inline)) {
-      if (ALL || (v >= lo && v <= hi)) {
-        const unsigned at = atomicAdd(&sh.listed, 1u);
-        if (at < TH) sh.list[at] = ((uint64_t)~key_of(v) << 32) | (unsigned)i;
-      }
+      if (in(v)) append(sh.list, sh.listed, v, i);
     });
     __syncthreads();
     all = sh.listed <= TH;
-    if (!all) return ~0ull;
-    const int n = (int)sh.listed;
-    uint64_t e = (int)threadIdx.x < n ? sh.list[threadIdx.x] : ~0ull;
+    return all ? arranged(sh.list, (int)sh.listed) : ~0ull;
+  }
+
+  // a list of n elements: each thread gets the one of its place, or ~0
+  __device__ __forceinline__ uint64_t arranged(uint64_t* list, int n) const {
+    uint64_t e = (int)threadIdx.x < n ? list[threadIdx.x] : ~0ull;
     const int wave0 = (int)(threadIdx.x & ~63u);
     if (n <= 512) {  // the place of each is the number of those before it: n reads that all lanes share; a sorting network of 36 steps took 6 us for 256
       int rank = 0;
       if (wave0 < n) {
 #pragma unroll 8
-        for (int j = 0; j < n; j++) rank += sh.list[j] < e;
+        for (int j = 0; j < n; j++) rank += list[j] < e;
       }
       __syncthreads();
-      if ((int)threadIdx.x < n) sh.list[rank] = e;
+      if ((int)threadIdx.x < n) list[rank] = e;
       __syncthreads();
-      e = (int)threadIdx.x < n ? sh.list[threadIdx.x] : ~0ull;
+      e = (int)threadIdx.x < n ? list[threadIdx.x] : ~0ull;
     } else {
       for (int k = 2; k <= TH; k <<= 1)
         for (int j = k >> 1; j > 0; j >>= 1) {
           uint64_t o;
           if (j >= 64) {
             __syncthreads();
-            sh.list[threadIdx.x] = e;
+            list[threadIdx.x] = e;
             __syncthreads();
-            o = sh.list[threadIdx.x ^ j];
+            o = list[threadIdx.x ^ j];
           } else {
             o = __shfl_xor((unsigned long long)e, j);
           }
@@ -321,6 +352,13 @@ struct Row {
     return b;
   }
 
+  // ... of a bin's, sorted, with the mass m and count c before it
+  __device__ __forceinline__ Border reaches(uint64_t e, Target target, uint64_t m, unsigned c) const {
+    const uint64_t w = e == ~0ull ? 0 : whole(of_key(~(unsigned)(e >> 32)));
+    before(w, e == ~0ull ? 0u : 1u, m, c);
+    return place(e, w, target, m, c);
+  }
+
   // The shortest beginning of the order that reaches the target, from the histogram.
   __device__ __forceinline__ Border find(Bins<TH>& bins, Target target) const {
     uint64_t m = 0;
@@ -328,12 +366,9 @@ struct Row {
     const int b0 = first_bin(bins.mass0, bins.count0, target, m, c);
     if (b0 == BINS) return Border{0u, 0xffffffffu, 0x7fffffff, 0};
     bool all;
-    const uint64_t e = sorted<false>(edge(b0), b0 == 0 ? __builtin_inff() : of_key(key_of(edge(b0 - 1)) - 1), all);
-    if (all) {
-      const uint64_t w = e == ~0ull ? 0 : whole(of_key(~(unsigned)(e >> 32)));
-      before(w, e == ~0ull ? 0u : 1u, m, c);
-      return place(e, w, target, m, c);
-    }
+    const float least = edge(b0), most = largest(b0);
+    const uint64_t e = sorted([=](float v) __attribute__((always_inline)) { return v >= least && v <= most; }, all);
+    if (all) return reaches(e, target, m, c);
     unsigned prefix = 0;
     for (int level = 0; level < 3; level++) {
       const int shift = level == 0 ? 21 : level == 1 ? 10 : 0, width = level == 2 ? 10 : 11;
@@ -437,8 +472,11 @@ __global__ __launch_bounds__(TH) void sample_rows(const typename T::Storage* __r
     give((int)sh.word, 0.f);
     return;
   }
-  row.infinite = best == __builtin_inff();
-  row.top = row.infinite ? 0.f : best + 0.f;
+  if (best == __builtin_inff()) {
+    row.least = best;
+    row.most = best = __FLT_MAX__;
+  }
+  row.top = best;
   row.top64 = (double)row.top;
   row.inv = 64.f / t;
   row.scale = 64.0 * 1.4426950408889634 / (double)t;
@@ -450,7 +488,7 @@ __global__ __launch_bounds__(TH) void sample_rows(const typename T::Storage* __r
   uint64_t e = ~0ull, total = 0, kept = 0;
   const double least_weight = (double)q * one;
   if constexpr (WHOLE) {
-    e = row.template sorted<true>(0.f, 0.f, whole);
+    e = row.sorted([](float) __attribute__((always_inline)) { return true; }, whole);
   } else {
     row.clear(bins.mass0, bins.count0);
     if (few) {
@@ -459,16 +497,19 @@ __global__ __launch_bounds__(TH) void sample_rows(const typename T::Storage* __r
       uint64_t m = 0;
       unsigned c = 0;
       const int last = row.first_bin(bins.mass0, bins.count0, Target{true, (uint64_t)k}, m, c);
-      if (c + bins.count0[last] <= TH) e = row.template sorted<false>(row.edge(last), __builtin_inff(), whole);
+      if (c + bins.count0[last] <= TH) {
+        const float lo = row.edge(last);
+        e = row.sorted([=](float v) __attribute__((always_inline)) { return v >= lo; }, whole);
+      }
     }
     if (!whole) {  // the masses; of the last bin, which may have most of the elements, in registers
       uint64_t rest = 0;
+      const bool least = q > 0.f;
       row.each([&](float v, int) __attribute__((always_inline)) {
         const double w = row.weight(row.exponent(v));
         const uint64_t m = row.whole64(w);
         const int b = row.bin(v);
-        total += m;
-        kept += w >= least_weight ? m : 0;
+        if (least) kept += w >= least_weight ? m : 0;
         if (b < BINS - 1)
           atomicAdd((unsigned long long*)&bins.mass0[b], (unsigned long long)m);
         else
@@ -476,6 +517,8 @@ __global__ __launch_bounds__(TH) void sample_rows(const typename T::Storage* __r
       });
       rest = row.sum(rest);
       if (threadIdx.x == 0) bins.mass0[BINS - 1] = rest;
+      __syncthreads();
+      for (int b = threadIdx.x; b < BINS; b += TH) total += bins.mass0[b];
     }
   }
   uint64_t w = 0, m = 0;  // sorted: this thread's element's mass, and the mass before it
@@ -487,12 +530,68 @@ __global__ __launch_bounds__(TH) void sample_rows(const typename T::Storage* __r
     row.before(w, 0u, m, c);
   }
   total = row.sum(total);
-  if (q > 0.f) kept = row.sum(kept);
+  kept = q > 1.f ? row.whole(row.top) : q > 0.f ? row.sum(kept) : total;  // past 1: the first alone
   Border end = {0u, 0xffffffffu, 0x7fffffff, 0}, b;
+  bool drawn = false;
+  if constexpr (!WHOLE) {
+    // The border of a top-p lies in one bin, and the draw, whatever the border's place in it, in one or in two others most often:
+    // one reading for the members of all three, where one for each border took 16 us more for 256 rows of 131072.
+    if (!whole && !few && p < 1.f) {
+      uint64_t mp = 0, m1 = 0, m2 = 0;  // the masses before the border's bin and the draw's two
+      const Target border = {false, least_mass(p, total)};
+      const uint64_t two[2] = {bins.mass0[2 * threadIdx.x], bins.mass0[2 * threadIdx.x + 1]};
+      static_assert(BINS == 2 * TH, "two bins for a thread");
+      uint64_t bm = 0;
+      unsigned c = 0;
+      row.before(two[0] + two[1], 0u, bm, c);
+      const int bp = row.bin_at(bm, two[0], two[1], border.least, mp);
+      const int b1 = row.bin_at(bm, two[0], two[1], mass_before(u, min(mp + 1, kept)) + 1, m1);
+      const int b2 = row.bin_at(bm, two[0], two[1], mass_before(u, min(mp + bins.mass0[bp], kept)) + 1, m2);
+      if (b1 == b2 || m1 + bins.mass0[b1] == m2) {  // nothing between the two
+        const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+        if (wave < 3) {  // each edge by a wave of its own
+          const int b = wave == 0 ? bp : wave == 1 ? b1 : b2;
+          const float l = row.edge(b), h = row.largest(b);
+          if ((threadIdx.x & 63) == 0) {
+            bins.least[wave] = l;
+            bins.most[wave] = wave == 2 && b1 == b2 ? -__builtin_inff() : h;
+          }
+        }
+        if (threadIdx.x == 0) sh.listed = bins.listed[0] = bins.listed[1] = 0;
+        __syncthreads();
+        const float lop = bins.least[0], hip = bins.most[0], lo1 = bins.least[1], hi1 = bins.most[1], lo2 = bins.least[2], hi2 = bins.most[2];
+        row.each([&](float v, int i) __attribute__((always_inline)) {
+          const bool in = v >= lop && v <= hip, in1 = v >= lo1 && v <= hi1, in2 = v >= lo2 && v <= hi2;
+          if (in | in1 | in2) {
+            if (in) row.append(sh.list, sh.listed, v, i);
+            if (in1 | in2) row.append(bins.list[in2], bins.listed[in2], v, i);
+          }
+        });
+        __syncthreads();
+        drawn = max(sh.listed, max(bins.listed[0], bins.listed[1])) <= TH;
+      }
+      if (drawn) {
+        Target target = border;
+        uint64_t* list = sh.list;
+        unsigned listed = sh.listed;
+#pragma unroll 1
+        for (int step = 0; step < 2; step++) {
+          b = row.reaches(row.arranged(list, (int)listed), target, mp, 0);
+          if (step == 1) break;
+          total = min(b.mass, kept);
+          target.least = mass_before(u, total) + 1;
+          const int other = b1 != b2 && target.least > m2;
+          list = bins.list[other];
+          listed = bins.listed[other];
+          mp = other ? m2 : m1;
+        }
+      }
+    }
+  }
   // top-k, top-p, and with all that is kept known, the draw
-  for (int step = few ? 0 : p < 1.f ? 1 : 2; step < 3; step++) {
+  for (int step = drawn ? 3 : few ? 0 : p < 1.f ? 1 : 2; step < 3; step++) {
     if (step == 1 && !(p < 1.f)) continue;
-    if (step == 2 && q > 0.f) total = min(total, q > 1.f ? row.whole(row.top) : kept);  // past 1: the first alone
+    if (step == 2) total = min(total, kept);
     const Target target = {step == 0, step == 0 ? (uint64_t)k : step == 1 ? least_mass(p, total) : mass_before(u, total) + 1};
     if constexpr (WHOLE) {
       b = row.place(e, w, target, m, threadIdx.x);
