@@ -10,10 +10,11 @@
 // Rows of up to 1024 logits are sorted whole. A bin with more than 1024 members (rows of equal logits) is taken apart by the bits
 // of x instead, 11, 11 and 10 at a time.
 //
-// What bounds it: 256 rows of 131072 bfloat16 logits, a workgroup a CU, take 130 us: 19 for the largest (the 67 MB come once from
+// What bounds it: 256 rows of 131072 float32 logits, a workgroup a CU, take 130 us: 19 for the largest (the 134 MB come once from
 // memory and then from the last cache), 48 for the masses, which is the rate of 64-bit atomics on shared memory (48 cycles for 64
-// of them), 24 for the members, 20 for sorting and placing. 64 rows of 32000 with a top-k take 29 us, one row of 131072 40, chains of
-// small steps; up to 256 logits 10.
+// of them), 24 for the members, 20 for sorting and placing. 64 rows of 65536 bfloat16 with a top-k take 29 us, one row of 50257 40,
+// chains of small steps; 32 rows of 256 10. (Tried for a top-k and no faster: the kth of every four threads' largest as a bound
+// in place of the counts, 28 us.)
 //
 // Masses are whole numbers, w 2^F rounded with F such that a row's sum stays below 2^63: sums of them do not depend on
 // the order that atomics come in, and they are exact to V 2^-F of the largest weight (2^-28 of it for 2^17 tokens at
