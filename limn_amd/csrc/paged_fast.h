@@ -1,5 +1,5 @@
 // Shared by the kernels of attention over a paged cache that take the tokens of a sequence in tiles (paged_token.hip,
-// paged_tiles.hip): which tile a workgroup has, the score rules, the write of the new tokens, partial results.
+// paged_tiles.h): which tile a workgroup has, the score rules, the write of the new tokens, partial results.
 #pragma once
 
 #include "attend_rules.h"
@@ -145,7 +145,6 @@ __device__ __forceinline__ Rules paged_rules(const PagedView& v) {
   const RuleArgs a = {nullptr, nullptr, nullptr, nullptr, 0, 0, 1, v.scale, v.softcap};
   return rules_of(a, 0);
 }
-typedef Rules PagedRules;
 
 }  // namespace
 }  // namespace limn

@@ -279,7 +279,6 @@ __global__ __launch_bounds__(THREADS, 2) void paged_tiles(PagedFast a, PagedView
   }
   const float total = pair_sum(l);
   __syncthreads();  // the tile buffers become staging below
-  __syncthreads();  // the tile buffers become staging below
   // the keys of this part, for what was taken out of their values
   const int j0 = begin_of(first), j1 = last == span.tiles ? span.end : begin_of(last);
   const bool odd = found != 0;

@@ -117,7 +117,7 @@ __global__ __launch_bounds__(64 * waves, waves == 4 ? 2 : 1) void paged_token(Pa
   const Item it = item_at(v, slot, R);
   if (!it.live) return;
   const Sequence& q = it.seq;
-  const PagedRules r = paged_rules(v);
+  const Rules r = paged_rules(v);
   const int group = v.group, rows = q.n * group, tile = it.tile;
   const S* fresh_k = a.k != nullptr ? (const S*)a.k + kvh * (int64_t)v.hd : nullptr;
   const S* fresh_v = a.k != nullptr ? (const S*)a.v + kvh * (int64_t)v.hd : nullptr;

@@ -35,7 +35,7 @@ def attend_paged(q: Tensor, k: Tensor | None, v: Tensor | None, key_pages: Tenso
       new tokens leaves the first of them without a position: they see nothing and give zeros.
     - `table` (sequences, table_pages) int32: the pages of each one's positions. Behind the last position it may hold
       anything. Keys of a page number that is not in the cache are not there: nothing is written, and no query sees them.
-      Sequences may share pages that none of them writes to in this call.
+      Sequences may share pages that none of them writes to in this call; a page that is written stands in the table once.
     - `slopes` (heads,) float32, `softcap`, `scale`: as in `attend`.
 
     There is no gradient: the call is for answering (under `no_grad`, or on tensors that need none).
