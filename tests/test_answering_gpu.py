@@ -1,0 +1,145 @@
+"""attend_paged, int8_linear and sample one behind another by their C ABI: on a stream of the caller's, and captured into
+graphs that are replayed in turn with other work between, every replay against the same calls made eagerly. And sample where a top-p's
+border and the draw meet many equal logits."""
+
+from __future__ import annotations
+
+import ctypes
+
+import numpy as np
+import pytest
+import torch
+
+from conftest import DTYPES, storage_values
+from limn_amd.dtypes import ABI_CODE
+from limn_amd.hip import runtime
+from limn_amd.seam import bfloat16
+from test_sample_gpu import TYPES, called, check
+
+pytestmark = pytest.mark.gpu
+BF16 = ABI_CODE[bfloat16]
+
+
+class Step:
+    """A layer's end and a draw: attention of `counts` new tokens over a cache, a head in 8 bits, a token for each row."""
+
+    def __init__(self, lib, seed, counts, most, heads=4, kv_heads=2, hd=64, page=16, vocab=1500):
+        self.lib, rng = lib, np.random.default_rng(seed)
+        tokens, seqs, table_pages = sum(counts), len(counts), -(-most // page)
+        pages = seqs * table_pages + 1
+        on = lambda *shape, kind=torch.bfloat16: torch.tensor(rng.standard_normal(shape), dtype=torch.float32).to(kind).cuda()  # noqa: E731
+        self.q, self.k, self.v = on(tokens, heads, hd), on(tokens, kv_heads, hd), on(tokens, kv_heads, hd)
+        self.pools = [on(pages, kv_heads, page, hd) for _ in range(2)]
+        self.starts = torch.tensor(np.concatenate([[0], np.cumsum(counts)]), dtype=torch.int32).cuda()
+        self.lengths = torch.tensor(rng.integers(max(counts), most + 1, seqs), dtype=torch.int32).cuda()
+        self.table = torch.tensor(rng.permutation(pages)[: seqs * table_pages].reshape(seqs, -1), dtype=torch.int32).cuda()
+        self.w8 = torch.tensor(rng.integers(-127, 128, (vocab, heads * hd)), dtype=torch.int8).cuda()
+        self.scales = torch.full((vocab,), 0.004).cuda()
+        self.u, self.top_p = torch.tensor(rng.random(tokens), dtype=torch.float32).cuda(), torch.full((tokens,), 0.9).cuda()
+        self.sizes = (tokens, seqs, heads, kv_heads, hd, pages, page, table_pages)
+        self.wide, self.vocab = heads * hd, vocab
+        self.out, self.logits = torch.empty_like(self.q), torch.empty(tokens, vocab, dtype=torch.bfloat16, device="cuda")
+        self.drawn, self.logs = torch.empty(tokens, dtype=torch.int32, device="cuda"), torch.empty(tokens, device="cuda")
+        need = (lib.limn_hip_attend_paged_workspace(BF16, *self.sizes), lib.limn_hip_int8_linear_workspace(BF16, tokens, self.wide, vocab), lib.limn_hip_sample_workspace(BF16, tokens, vocab))
+        self.rooms = [torch.empty(max(n, 16), dtype=torch.uint8, device="cuda") for n in need]
+        self.need = need
+
+    def run(self, stream):
+        p = lambda *ts: [t.data_ptr() for t in ts]  # noqa: E731
+        (tokens, _, heads, kv_heads, hd, *_), lib, hds = self.sizes, self.lib, self.sizes[4]
+        check_ = runtime.check_limn
+        check_(lib.limn_hip_attend_paged(*p(self.q, self.k, self.v, *self.pools, self.starts, self.lengths, self.table), None, self.out.data_ptr(), BF16, *self.sizes,
+                                         heads * hds, kv_heads * hds, kv_heads * hds, hd**-0.5, 0.0, self.rooms[0].data_ptr(), self.need[0], stream))
+        check_(lib.limn_hip_int8_linear(*p(self.out, self.w8, self.scales), None, self.logits.data_ptr(), BF16, tokens, self.wide, self.vocab, self.rooms[1].data_ptr(), self.need[1], stream))
+        check_(lib.limn_hip_sample(*p(self.logits, self.u), None, None, self.top_p.data_ptr(), None, *p(self.drawn, self.logs), BF16, tokens, self.vocab, self.vocab,
+                                   self.rooms[2].data_ptr(), self.need[2], stream))
+
+    def change(self, seed):
+        """Other inputs in the same buffers."""
+        g = torch.Generator(device="cuda").manual_seed(seed)
+        for t in (self.q, self.k, self.v):
+            t.normal_(generator=g)
+        self.u.uniform_(generator=g)
+        self.lengths.copy_((self.lengths * 7 + seed) % (self.sizes[6] * self.sizes[7] - 3) + 3)
+        self.table.copy_(self.table.flip(0))
+
+    def clear(self):
+        for t in (self.out, self.logits, self.drawn, self.logs):
+            t.zero_()
+
+    def results(self):
+        return [t.clone() for t in (self.out, self.logits, self.drawn, self.logs, *self.pools)]
+
+
+SHAPES = [((1, 1, 1), 300), ((1,) * 40, 3000), ((200, 1, 70), 700)]
+
+
+@pytest.mark.parametrize("counts,most", SHAPES, ids=["few", "parts", "tiles"])
+def test_a_stream_of_the_callers(hipdev, counts, most):
+    step = Step(hipdev.lib, 1, counts, most)
+    pools = [t.clone() for t in step.pools]
+    step.run(None)
+    torch.cuda.synchronize()
+    want = step.results()
+    for t, old in zip(step.pools, pools):
+        t.copy_(old)
+    step.clear()
+    stream = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    step.run(ctypes.c_void_p(stream.cuda_stream))
+    stream.synchronize()
+    for a, b in zip(step.results(), want):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("counts,most", SHAPES, ids=["few", "parts", "tiles"])
+def test_two_graphs_replayed_in_turn(hipdev, counts, most):
+    steps = [Step(hipdev.lib, s, counts, most) for s in (1, 2)]
+    stream, graphs = torch.cuda.Stream(), []
+    for step in steps:
+        step.run(ctypes.c_void_p(stream.cuda_stream))
+        stream.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            step.run(ctypes.c_void_p(torch.cuda.current_stream().cuda_stream))
+        graphs.append(graph)
+    for turn in range(5):
+        for step, graph in zip(steps, graphs):
+            step.change(turn)
+            pools = [t.clone() for t in step.pools]
+            step.clear()
+            graph.replay()
+            got = step.results()
+            for t, old in zip(step.pools, pools):
+                t.copy_(old)
+            step.clear()
+            torch.cuda.synchronize()
+            step.run(None)
+            torch.cuda.synchronize()
+            for a, b in zip(got, step.results()):
+                assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("steps", [1, 4, 64])
+@pytest.mark.parametrize("top_p", [0.05, 0.5, 0.9, 0.999])
+def test_borders_among_equal_logits(hipdev, dtype, steps, top_p):
+    """Logits of few values, some with more members than a sorted list: draws in the border's own bin, in the one beside it, in the first."""
+    rng = np.random.default_rng(steps)
+    rows, vocab = 48, 9000
+    logits = storage_values((np.round(rng.standard_normal((rows, vocab)) * 1.5 * steps) / steps).astype(np.float32), DTYPES[dtype])
+    u = np.concatenate([[0.0, 1e-7, 0.5, 1 - 2.0**-24], rng.random(rows - 4)]).astype(np.float32)
+    check(hipdev, logits, u, dtype, top_p=top_p)
+    check(hipdev, logits, u, dtype, top_p=top_p, min_p=0.3)
+    check(hipdev, logits, u, dtype, top_p=top_p, temperature=np.geomspace(0.05, 50, rows).astype(np.float32))
+    check(hipdev, logits, u, dtype, top_p=top_p, top_k=np.geomspace(1, vocab, rows).astype(np.int32))
+
+
+def test_the_largest_vocabulary(hipdev):
+    """2^24 logits. Their masses are off by sqrt(2^24) half units of 2^-38 of the largest weight, 4e-9 of it; a drawn token's is
+    some 1e-3 of it, so a border moves past one in a case of 10^5."""
+    rng = np.random.default_rng(3)
+    logits, u = (rng.standard_normal((1, 1 << 24)) * 2.5).astype(np.float32), np.array([0.37], np.float32)
+    check(hipdev, logits, u, "float32", top_p=0.8)
+    with pytest.raises(NotImplementedError):
+        called(hipdev, np.zeros((1, (1 << 24) + 1), np.float32), u, "float32")
