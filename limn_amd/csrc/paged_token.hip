@@ -98,8 +98,8 @@ struct Operands<F32, W> {
   }
 };
 
-template <typename T, int D, int NR, int waves>
-__global__ __launch_bounds__(64 * waves, waves == 4 ? 2 : 1) void paged_token(PagedFast a, PagedView v) {
+template <typename T, int D, int NR, int waves, int blocks>
+__global__ __launch_bounds__(64 * waves, blocks) void paged_token(PagedFast a, PagedView v) {
 #if defined(__HIP_DEVICE_COMPILE__)  // the host pass needs the stub alone
   constexpr int W = D / 16;
   typedef Operands<T, W> O;
@@ -334,6 +334,11 @@ __global__ __launch_bounds__(64 * waves, waves == 4 ? 2 : 1) void paged_token(Pa
 // Waves of a workgroup that has a row tile to itself: as many as its registers allow without spills.
 template <typename T, int D, int NR>
 constexpr int LONE_WAVES = std::is_same<T, F32>::value ? (D == 64 && NR == 1 ? 8 : 4) : (D == 64 && NR == 1 ? 16 : 8);
+// Workgroups of 4 waves that share a CU. Two wide float32 row tiles (2 x 8 tokens, up to 4000 positions, 55 us with two, 37 with one)
+// and a workgroup that is alone anyway (8 x 2000 positions of 128 dims 79 and 68) spill in half of the registers; one row tile
+// spills less than a second workgroup gives (32 x 8192 positions 326 and 342).
+template <typename T, int D, int NR>
+constexpr int SHARING = std::is_same<T, F32>::value && D == 128 && NR == 2 ? 1 : 2;
 
 template <typename T, int D, int NR>
 int launch_token(const PagedArgs& a, const PagedFast& f, bool lone) {
@@ -341,10 +346,10 @@ int launch_token(const PagedArgs& a, const PagedFast& f, bool lone) {
   const int64_t blocks = paged_slots(a, 16 * NR) * a.kv_heads * f.parts;
   if (blocks > 0x7fffffff) return fail(LIMN_HIP_EUNSUPPORTED, "attend_paged: %lld workgroups exceed one launch", (long long)blocks);
   constexpr int LONE = LONE_WAVES<T, D, NR>;
-  if (LONE == 4 || !lone)
-    hipLaunchKernelGGL((paged_token<T, D, NR, 4>), dim3((unsigned)blocks), dim3(256), 0, a.stream, f, v);
+  if (lone)
+    hipLaunchKernelGGL((paged_token<T, D, NR, LONE, 1>), dim3((unsigned)blocks), dim3(64 * LONE), 0, a.stream, f, v);
   else
-    hipLaunchKernelGGL((paged_token<T, D, NR, LONE>), dim3((unsigned)blocks), dim3(64 * LONE), 0, a.stream, f, v);
+    hipLaunchKernelGGL((paged_token<T, D, NR, 4, SHARING<T, D, NR>>), dim3((unsigned)blocks), dim3(256), 0, a.stream, f, v);
   return check_hip(hipGetLastError(), "launching attention of few tokens over a paged cache");
 }
 
