@@ -10,10 +10,14 @@
 // Rows of up to 1024 logits are sorted whole. A bin with more than 1024 members (rows of equal logits) is taken apart by the bits
 // of x instead, 11, 11 and 10 at a time.
 //
+// A few long rows are split over workgroups, a launch for each of the three readings (sample_largest, sample_spread,
+// sample_members) and a last one that sorts and draws; what they pass on lies in the workspace. Whole numbers make the parts' sums
+// the row's, in any order.
+//
 // What bounds it: 256 rows of 131072 float32 logits, a workgroup a CU, take 130 us: 19 for the largest (the 134 MB come once from
 // memory and then from the last cache), 48 for the masses, which is the rate of 64-bit atomics on shared memory (48 cycles for 64
-// of them), 24 for the members, 20 for sorting and placing. 64 rows of 65536 bfloat16 with a top-k take 29 us, one row of 50257 40,
-// chains of small steps; 32 rows of 256 10. (Tried for a top-k and no faster: the kth of every four threads' largest as a bound
+// of them), 24 for the members, 20 for sorting and placing. 64 rows of 65536 bfloat16 with a top-k take 29 us, one row of 50257 28
+// in four launches of 3, 7, 9 and 9, chains of small steps; 32 rows of 256 10. (Tried for a top-k and no faster: the kth of every four threads' largest as a bound
 // in place of the counts, 28 us.)
 //
 // Masses are whole numbers, w 2^F rounded with F such that a row's sum stays below 2^63: sums of them do not depend on
@@ -25,6 +29,7 @@
 
 #include <math.h>
 
+#include <algorithm>
 #include <type_traits>
 
 namespace limn {
@@ -73,15 +78,33 @@ struct Shared {
   unsigned found_bin, found_count, listed, word;
   double powers[64];  // 2^(F + i / 64)
 };
+// The logits of three bins: a border's, and the draw's two (the second one empty where they are the same).
+struct Three {
+  float least[3], most[3];
+  __device__ __forceinline__ bool in(int j, float v) const { return v >= least[j] && v <= most[j]; }
+  // a list of the draw's that v is in, 0 if it is only in the border's, -1
+  __device__ __forceinline__ int list(float v) const { return in(2, v) ? 2 : in(1, v) ? 1 : in(0, v) ? 0 : -1; }
+};
 template <int TH>
 struct Bins {
   uint64_t mass0[BINS], mass[BINS];
   unsigned count0[BINS], count[BINS];  // count0: where a top-k asks for it
-  uint64_t list[2][TH];
-  unsigned listed[2];
-  float least[3], most[3];  // the logits of three bins
+  alignas(16) uint64_t list[3][TH];
+  unsigned listed[3];
+  Three at;
 };
 struct Nothing {};
+
+// What a row over several workgroups keeps between its launches.
+constexpr int LISTED = 1024, MOST_PARTS = 64;
+struct SplitRow {
+  uint64_t mass[BINS];         // of the histogram: masses, or counts where there is a top-k
+  uint64_t lists[3][LISTED];   // elements of the border's bin and of the draw's two, or of all bins that a top-k keeps
+  uint64_t m[3], total, kept;  // the masses before those bins; of all; of those that reach min_p
+  unsigned listed[3];
+  int found;  // whether the lists are of use
+  float best[MOST_PARTS];
+};
 
 // What a search looks for: a number of elements, or a mass.
 struct Target {
@@ -89,6 +112,18 @@ struct Target {
   uint64_t least;
   __device__ __forceinline__ bool reached(uint64_t mass, unsigned count) const { return (counts ? (uint64_t)count : mass) >= least; }
 };
+
+// The first mass of a beginning that reaches p of the whole: the last one kept is the first with which it does; the first element
+// always is kept.
+__device__ __forceinline__ uint64_t least_mass(float p, uint64_t total) {
+  const double want = ceil(fmax((double)p, 0.0) * (double)total);
+  return want > 1.0 ? (uint64_t)want : 1;
+}
+// The mass before the drawn token, at most: u of the kept mass, and below the whole of it.
+__device__ __forceinline__ uint64_t mass_before(float u, uint64_t total) {
+  const double share = u > 0.f ? (double)u * (double)total : u == u ? 0.0 : (double)total;
+  return share < (double)total ? min((uint64_t)share, total - 1) : total - 1;
+}
 
 // A row of logits, seen by a workgroup of TH threads.
 template <typename T, int TH>
@@ -105,6 +140,17 @@ struct Row {
   __device__ __forceinline__ Row(const S* x_, int vocab_, int bits_, Shared<TH>& sh_) : x(x_), vocab(vocab_), bits(bits_), least(-__builtin_inff()), most(__builtin_inff()), top(0.f), inv(0.f), top64(0.0), scale(0.0), sh(sh_) {
     head = min(vocab, (int)((16 - ((uintptr_t)x & 15)) & 15) / (int)sizeof(S));
     chunks = (vocab - head) / PER;
+  }
+
+  __device__ __forceinline__ void set(float best, float t) {
+    if (best == __builtin_inff()) {
+      least = best;
+      most = best = __FLT_MAX__;
+    }
+    top = best;
+    top64 = (double)top;
+    inv = 64.f / t;
+    scale = 64.0 * 1.4426950408889634 / (double)t;
   }
 
   __device__ __forceinline__ float seen(float v) const { return v >= least ? fminf(v, most) : -__builtin_inff(); }
@@ -161,6 +207,19 @@ struct Row {
   __device__ __forceinline__ uint64_t whole(float v) const { return whole64(weight(exponent(v))); }
   // 64 bins an e-fold of the weight; monotone in v: each step rounds, none turns the order round
   __device__ __forceinline__ int bin(float v) const { return v == top ? 0 : (int)fminf((top - v) * inv, (float)(BINS - 1)); }
+
+  __device__ __forceinline__ float largest_of() const {
+    float best = -__builtin_inff();
+    each([&](float v, int) __attribute__((always_inline)) { best = fmaxf(best, v); });
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) best = fmaxf(best, __shfl_xor(best, o));
+    if ((threadIdx.x & 63) == 0) sh.counts[threadIdx.x >> 6] = __float_as_uint(best);
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < WAVES; w++) best = fmaxf(best, __uint_as_float(sh.counts[w]));
+    __syncthreads();
+    return best;
+  }
 
   __device__ __forceinline__ uint64_t sum(uint64_t v) const {
 #pragma unroll
@@ -255,6 +314,25 @@ struct Row {
     return b;
   }
 
+  // The masses into the bins, what reaches least_weight summed in kept; of the last bin, which may have most of the elements, in
+  // registers.
+  __device__ __forceinline__ void masses(uint64_t* mass, bool some, double least_weight, uint64_t& kept) const {
+    uint64_t rest = 0;
+    each([&](float v, int) __attribute__((always_inline)) {
+      const double w = weight(exponent(v));
+      const uint64_t m = whole64(w);
+      const int b = bin(v);
+      if (some) kept += w >= least_weight ? m : 0;
+      if (b < BINS - 1)
+        atomicAdd((unsigned long long*)&mass[b], (unsigned long long)m);
+      else
+        rest += m;
+    });
+    rest = sum(rest);
+    if (threadIdx.x == 0) mass[BINS - 1] = rest;
+    __syncthreads();
+  }
+
   __device__ __forceinline__ void clear(uint64_t* mass, unsigned* count) const {
     __syncthreads();
     for (int b = threadIdx.x; b < BINS; b += TH) {
@@ -277,6 +355,36 @@ struct Row {
       hi = least;
     }
     return of_key(hi);
+  }
+
+  // The bins of a top-p's border and of the draw's ends, whatever the border's place in its bin, and the masses before them, from
+  // this thread's two of the histogram `mass`. Whether no bin between the draw's two has a mass.
+  __device__ __forceinline__ bool windows(const uint64_t (&two)[2], const uint64_t* mass, uint64_t total, uint64_t kept, float p, float u, Three& at, uint64_t (&m)[3]) const {
+    uint64_t bm = 0;
+    unsigned c = 0;
+    before(two[0] + two[1], 0u, bm, c);
+    int b[3] = {-1, 0, 0};
+    uint64_t lo = min(total, kept), hi = lo;
+    if (p < 1.f) {
+      b[0] = bin_at(bm, two[0], two[1], least_mass(p, total), m[0]);
+      lo = min(m[0] + 1, kept);
+      hi = min(m[0] + mass[b[0]], kept);
+    }
+    b[1] = bin_at(bm, two[0], two[1], mass_before(u, lo) + 1, m[1]);
+    b[2] = bin_at(bm, two[0], two[1], mass_before(u, hi) + 1, m[2]);
+    const bool same = b[1] == b[2], next = same || m[1] + mass[b[1]] == m[2];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    if (wave < 6) {  // each edge by a wave of its own
+      const int j = wave >> 1, mine = j == 0 ? b[0] : j == 1 ? b[1] : b[2];
+      const bool upper = wave & 1, none = j == 0 ? !(p < 1.f) : j == 2 && same;
+      float x = upper ? -__builtin_inff() : __builtin_inff();
+      if (!none) x = upper && mine == 0 ? __builtin_inff() : edge(mine - upper);
+      if (!none && upper && mine > 0) x = of_key(key_of(x) - 1);
+      if ((threadIdx.x & 63) == 0) (upper ? at.most : at.least)[j] = x;
+    }
+    if (same) m[2] = ~0ull;  // nothing lies behind it
+    __syncthreads();
+    return next;
   }
 
   // ... and the largest of bin b
@@ -420,21 +528,17 @@ struct Row {
   }
 };
 
-// The first mass of a beginning that reaches p of the whole: the last one kept is the first with which it does; the first element
-// always is kept.
-__device__ __forceinline__ uint64_t least_mass(float p, uint64_t total) {
-  const double want = ceil(fmax((double)p, 0.0) * (double)total);
-  return want > 1.0 ? (uint64_t)want : 1;
-}
-// The mass before the drawn token, at most: u of the kept mass, and below the whole of it.
-__device__ __forceinline__ uint64_t mass_before(float u, uint64_t total) {
-  const double share = u > 0.f ? (double)u * (double)total : u == u ? 0.0 : (double)total;
-  return share < (double)total ? min((uint64_t)share, total - 1) : total - 1;
+// the largest logit of a split row, for a whole wave
+__device__ __forceinline__ float row_best(const SplitRow& s, int parts) {
+  float best = (int)(threadIdx.x & 63) < parts ? s.best[threadIdx.x & 63] : -__builtin_inff();
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) best = fmaxf(best, __shfl_xor(best, o));
+  return best;
 }
 
-// WHOLE: rows of up to TH logits.
-template <typename T, int TH, bool WHOLE>
-__global__ __launch_bounds__(TH) void sample_rows(const typename T::Storage* __restrict__ logits, SampleArgs a) {
+// WHOLE: rows of up to TH logits. SPLIT: the last launch of split rows.
+template <typename T, int TH, bool WHOLE, bool SPLIT>
+__global__ __launch_bounds__(TH) void sample_rows(const typename T::Storage* __restrict__ logits, SampleArgs a, const SplitRow* split, int parts) {
   __shared__ Shared<TH> sh;
   __shared__ std::conditional_t<WHOLE, Nothing, Bins<TH>> bins;
   const int64_t n = blockIdx.x;
@@ -443,15 +547,8 @@ __global__ __launch_bounds__(TH) void sample_rows(const typename T::Storage* __r
   const int k = a.top_k != nullptr ? a.top_k[n] : 0;
   if (threadIdx.x < 64) sh.powers[threadIdx.x] = exp2(a.bits + threadIdx.x * 0.015625);
   Row<T, TH> row(logits + n * a.row_stride, vocab, a.bits, sh);
-  float best = -__builtin_inff();
-  row.each([&](float v, int) __attribute__((always_inline)) { best = fmaxf(best, v); });
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) best = fmaxf(best, __shfl_xor(best, o));
-  if ((threadIdx.x & 63) == 0) sh.counts[threadIdx.x >> 6] = __float_as_uint(best);
-  __syncthreads();
-#pragma unroll
-  for (int w = 0; w < TH / 64; w++) best = fmaxf(best, __uint_as_float(sh.counts[w]));
-  __syncthreads();
+  const SplitRow* given = SPLIT ? split + n : nullptr;
+  const float best = SPLIT ? row_best(*given, parts) : row.largest_of();
   auto give = [&](int token, float logprob) {
     if (threadIdx.x != 0) return;
     a.tokens[n] = token;
@@ -473,26 +570,25 @@ __global__ __launch_bounds__(TH) void sample_rows(const typename T::Storage* __r
     give((int)sh.word, 0.f);
     return;
   }
-  if (best == __builtin_inff()) {
-    row.least = best;
-    row.most = best = __FLT_MAX__;
-  }
-  row.top = best;
-  row.top64 = (double)row.top;
-  row.inv = 64.f / t;
-  row.scale = 64.0 * 1.4426950408889634 / (double)t;
+  row.set(best, t);
 
   const double one = ldexp(1.0, a.bits);  // the largest weight
   const bool few = k > 0 && k < vocab;
   // either all that is kept, sorted, or a histogram
   bool whole = WHOLE;
+  const bool lists = SPLIT && given->found != 0 && max(given->listed[0], max(given->listed[1], given->listed[2])) <= LISTED;
   uint64_t e = ~0ull, total = 0, kept = 0;
   const double least_weight = (double)q * one;
   if constexpr (WHOLE) {
     e = row.sorted([](float) __attribute__((always_inline)) { return true; }, whole);
   } else {
-    row.clear(bins.mass0, bins.count0);
-    if (few) {
+    if (!lists) row.clear(bins.mass0, bins.count0);
+    if (lists && few) {
+      if (threadIdx.x < given->listed[0]) sh.list[threadIdx.x] = given->lists[0][threadIdx.x];
+      __syncthreads();
+      e = row.arranged(sh.list, (int)given->listed[0]);
+      whole = true;
+    } else if (few) {
       row.each([&](float v, int) __attribute__((always_inline)) { atomicAdd(&bins.count0[row.bin(v)], 1u); });
       __syncthreads();
       uint64_t m = 0;
@@ -503,22 +599,15 @@ __global__ __launch_bounds__(TH) void sample_rows(const typename T::Storage* __r
         e = row.sorted([=](float v) __attribute__((always_inline)) { return v >= lo; }, whole);
       }
     }
-    if (!whole) {  // the masses; of the last bin, which may have most of the elements, in registers
-      uint64_t rest = 0;
-      const bool least = q > 0.f;
-      row.each([&](float v, int) __attribute__((always_inline)) {
-        const double w = row.weight(row.exponent(v));
-        const uint64_t m = row.whole64(w);
-        const int b = row.bin(v);
-        if (least) kept += w >= least_weight ? m : 0;
-        if (b < BINS - 1)
-          atomicAdd((unsigned long long*)&bins.mass0[b], (unsigned long long)m);
-        else
-          rest += m;
-      });
-      rest = row.sum(rest);
-      if (threadIdx.x == 0) bins.mass0[BINS - 1] = rest;
+    if (!whole && !lists && SPLIT && !few) {  // the lists did not hold what they have to: the histogram is there
+      for (int b = threadIdx.x; b < BINS; b += TH) {
+        bins.mass0[b] = given->mass[b];
+        total += given->mass[b];
+      }
+      if (threadIdx.x == 0) kept = given->kept;
       __syncthreads();
+    } else if (!whole && !lists) {
+      row.masses(bins.mass0, q > 0.f, least_weight, kept);
       for (int b = threadIdx.x; b < BINS; b += TH) total += bins.mass0[b];
     }
   }
@@ -530,62 +619,51 @@ __global__ __launch_bounds__(TH) void sample_rows(const typename T::Storage* __r
     unsigned c = 0;
     row.before(w, 0u, m, c);
   }
-  total = row.sum(total);
-  kept = q > 1.f ? row.whole(row.top) : q > 0.f ? row.sum(kept) : total;  // past 1: the first alone
+  total = lists && !few ? given->total : row.sum(total);
+  kept = q > 1.f ? row.whole(row.top) : !(q > 0.f) ? total : lists && !few ? given->kept : row.sum(kept);  // past 1: the first alone
   Border end = {0u, 0xffffffffu, 0x7fffffff, 0}, b;
   bool drawn = false;
   if constexpr (!WHOLE) {
     // The border of a top-p lies in one bin, and the draw, whatever the border's place in it, in one or in two others most often:
     // one reading for the members of all three, where one for each border took 16 us more for 256 rows of 131072.
-    if (!whole && !few && p < 1.f) {
-      uint64_t mp = 0, m1 = 0, m2 = 0;  // the masses before the border's bin and the draw's two
-      const Target border = {false, least_mass(p, total)};
+    uint64_t ms[3] = {0, 0, 0};
+    if (lists && !few) {
+      ms[0] = given->m[0], ms[1] = given->m[1], ms[2] = given->m[2];
+      drawn = true;
+    } else if (!whole && !few && !SPLIT && p < 1.f) {
       const uint64_t two[2] = {bins.mass0[2 * threadIdx.x], bins.mass0[2 * threadIdx.x + 1]};
-      static_assert(BINS == 2 * TH, "two bins for a thread");
-      uint64_t bm = 0;
-      unsigned c = 0;
-      row.before(two[0] + two[1], 0u, bm, c);
-      const int bp = row.bin_at(bm, two[0], two[1], border.least, mp);
-      const int b1 = row.bin_at(bm, two[0], two[1], mass_before(u, min(mp + 1, kept)) + 1, m1);
-      const int b2 = row.bin_at(bm, two[0], two[1], mass_before(u, min(mp + bins.mass0[bp], kept)) + 1, m2);
-      if (b1 == b2 || m1 + bins.mass0[b1] == m2) {  // nothing between the two
-        const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-        if (wave < 3) {  // each edge by a wave of its own
-          const int b = wave == 0 ? bp : wave == 1 ? b1 : b2;
-          const float l = row.edge(b), h = row.largest(b);
-          if ((threadIdx.x & 63) == 0) {
-            bins.least[wave] = l;
-            bins.most[wave] = wave == 2 && b1 == b2 ? -__builtin_inff() : h;
-          }
-        }
-        if (threadIdx.x == 0) sh.listed = bins.listed[0] = bins.listed[1] = 0;
+      if (row.windows(two, bins.mass0, total, kept, p, u, bins.at, ms)) {
+        if (threadIdx.x < 3) bins.listed[threadIdx.x] = 0;
         __syncthreads();
-        const float lop = bins.least[0], hip = bins.most[0], lo1 = bins.least[1], hi1 = bins.most[1], lo2 = bins.least[2], hi2 = bins.most[2];
+        const Three at = bins.at;
         row.each([&](float v, int i) __attribute__((always_inline)) {
-          const bool in = v >= lop && v <= hip, in1 = v >= lo1 && v <= hi1, in2 = v >= lo2 && v <= hi2;
-          if (in | in1 | in2) {
-            if (in) row.append(sh.list, sh.listed, v, i);
-            if (in1 | in2) row.append(bins.list[in2], bins.listed[in2], v, i);
+          const int j = at.list(v);
+          if (j >= 0) {
+            if (at.in(0, v)) row.append(bins.list[0], bins.listed[0], v, i);
+            if (j > 0) row.append(bins.list[j], bins.listed[j], v, i);
           }
         });
         __syncthreads();
-        drawn = max(sh.listed, max(bins.listed[0], bins.listed[1])) <= TH;
+        drawn = max(bins.listed[0], max(bins.listed[1], bins.listed[2])) <= TH;
       }
-      if (drawn) {
-        Target target = border;
-        uint64_t* list = sh.list;
-        unsigned listed = sh.listed;
+    }
+    if (drawn) {
+      Target target = {false, least_mass(p, total)};
 #pragma unroll 1
-        for (int step = 0; step < 2; step++) {
-          b = row.reaches(row.arranged(list, (int)listed), target, mp, 0);
-          if (step == 1) break;
-          total = min(b.mass, kept);
+      for (int j = p < 1.f ? 0 : 3;;) {  // the border's list, then one of the draw's
+        if (j == 3) {
+          total = min(total, kept);
           target.least = mass_before(u, total) + 1;
-          const int other = b1 != b2 && target.least > m2;
-          list = bins.list[other];
-          listed = bins.listed[other];
-          mp = other ? m2 : m1;
+          j = target.least > ms[2] ? 2 : 1;
         }
+        uint64_t* list = bins.list[j];
+        int listed = (int)(lists ? given->listed[j] : bins.listed[j]);
+        if (lists && (int)threadIdx.x < listed) list[threadIdx.x] = given->lists[j][threadIdx.x];
+        __syncthreads();
+        b = row.reaches(row.arranged(list, listed), target, ms[j], 0);
+        if (j > 0) break;
+        total = b.mass;
+        j = 3;
       }
     }
   }
@@ -608,16 +686,147 @@ __global__ __launch_bounds__(TH) void sample_rows(const typename T::Storage* __r
   give(i, (float)log(row.weight(row.exponent(of_key(b.key))) / (double)total));
 }
 
+// A split row's launches. A part's elements, and its row's settings.
+template <typename T, int TH>
+struct Part {
+  int64_t n;
+  int begin, count, k;
+  float t, p, q, u;
+  bool few;
+  __device__ __forceinline__ Part(const SampleArgs& a, int each) {
+    n = blockIdx.y;
+    begin = min((int)a.vocab, (int)blockIdx.x * each);
+    count = min((int)a.vocab - begin, each);
+    t = a.temperature != nullptr ? a.temperature[n] : 1.f, p = a.top_p != nullptr ? a.top_p[n] : 1.f, q = a.min_p != nullptr ? a.min_p[n] : 0.f, u = a.uniforms[n];
+    k = a.top_k != nullptr ? a.top_k[n] : 0;
+    few = k > 0 && k < a.vocab;
+  }
+};
+
+// The parts' largest logits; and the row's numbers cleared.
+template <typename T, int TH>
+__global__ __launch_bounds__(TH) void sample_largest(const typename T::Storage* __restrict__ logits, SampleArgs a, SplitRow* split, int each) {
+  __shared__ Shared<TH> sh;
+  const Part<T, TH> at(a, each);
+  SplitRow& s = split[at.n];
+  const Row<T, TH> row(logits + at.n * a.row_stride + at.begin, at.count, a.bits, sh);
+  const float best = row.largest_of();
+  if (threadIdx.x == 0) s.best[blockIdx.x] = best;
+  for (int b = blockIdx.x * TH + threadIdx.x; b < BINS; b += gridDim.x * TH) s.mass[b] = 0;
+  if (blockIdx.x == 0 && threadIdx.x < 3) s.listed[threadIdx.x] = 0;
+  if (blockIdx.x == 0 && threadIdx.x == 0) s.kept = 0;
+}
+
+// The histogram: of counts where there is a top-k.
+template <typename T, int TH>
+__global__ __launch_bounds__(TH) void sample_spread(const typename T::Storage* __restrict__ logits, SampleArgs a, SplitRow* split, int each) {
+  __shared__ Shared<TH> sh;
+  __shared__ uint64_t mass[BINS];
+  const Part<T, TH> at(a, each);
+  SplitRow& s = split[at.n];
+  const float best = row_best(s, gridDim.x);
+  if (best == -__builtin_inff() || !(at.t > 0.f)) return;
+  if (threadIdx.x < 64) sh.powers[threadIdx.x] = exp2(a.bits + threadIdx.x * 0.015625);
+  Row<T, TH> row(logits + at.n * a.row_stride + at.begin, at.count, a.bits, sh);
+  row.set(best, at.t);
+  for (int b = threadIdx.x; b < BINS; b += TH) mass[b] = 0;
+  __syncthreads();
+  if (at.few) {
+    row.each([&](float v, int) __attribute__((always_inline)) { atomicAdd((unsigned long long*)&mass[row.bin(v)], 1ull); });
+    __syncthreads();
+  } else {
+    uint64_t kept = 0;
+    row.masses(mass, at.q > 0.f, (double)at.q * ldexp(1.0, a.bits), kept);
+    if (at.q > 0.f) kept = row.sum(kept);
+    if (threadIdx.x == 0 && kept != 0) atomicAdd((unsigned long long*)&s.kept, (unsigned long long)kept);
+  }
+  for (int b = threadIdx.x; b < BINS; b += TH)
+    if (mass[b] != 0) atomicAdd((unsigned long long*)&s.mass[b], (unsigned long long)mass[b]);
+}
+
+// The members of the bins that matter. Every part finds those bins for itself.
+template <typename T, int TH>
+__global__ __launch_bounds__(TH) void sample_members(const typename T::Storage* __restrict__ logits, SampleArgs a, SplitRow* split, int each) {
+  __shared__ Shared<TH> sh;
+  __shared__ Three three;
+  __shared__ uint64_t lists[3][TH];  // of this part
+  __shared__ unsigned listed[3], place[3];
+  const Part<T, TH> at(a, each);
+  SplitRow& s = split[at.n];
+  const float best = row_best(s, gridDim.x);
+  if (best == -__builtin_inff() || !(at.t > 0.f)) return;
+  Row<T, TH> row(logits + at.n * a.row_stride + at.begin, at.count, a.bits, sh);
+  row.set(best, at.t);
+  const uint64_t two[2] = {s.mass[2 * threadIdx.x], s.mass[2 * threadIdx.x + 1]};
+  uint64_t m[3] = {0, 0, 0}, total = 0, kept = 0;
+  bool found;
+  if (at.few) {
+    uint64_t bm = 0;
+    unsigned c = 0;
+    row.before(two[0] + two[1], 0u, bm, c);
+    const int last = row.bin_at(bm, two[0], two[1], (uint64_t)at.k, m[0]);
+    found = m[0] + s.mass[last] <= LISTED;
+    const float lo = row.edge(last);
+    if (threadIdx.x < 3) {
+      three.least[threadIdx.x] = threadIdx.x == 0 ? lo : __builtin_inff();
+      three.most[threadIdx.x] = threadIdx.x == 0 ? __builtin_inff() : -__builtin_inff();
+    }
+    __syncthreads();
+  } else {
+    total = row.sum(two[0] + two[1]);
+    kept = at.q > 1.f ? (uint64_t)1 << a.bits : at.q > 0.f ? s.kept : total;
+    found = row.windows(two, s.mass, total, kept, at.p, at.u, three, m);
+  }
+  if (blockIdx.x == 0 && threadIdx.x == 0) {
+    s.found = found;
+    s.total = total;
+    for (int j = 0; j < 3; j++) s.m[j] = m[j];
+  }
+  if (!found) return;
+  if (threadIdx.x < 3) listed[threadIdx.x] = 0;
+  __syncthreads();
+  const Three in = three;
+  row.each([&](float v, int i) __attribute__((always_inline)) {
+    const int j = in.list(v);
+    if (j >= 0) {
+      if (in.in(0, v)) row.append(lists[0], listed[0], v, at.begin + i);
+      if (j > 0) row.append(lists[j], listed[j], v, at.begin + i);
+    }
+  });
+  __syncthreads();
+  if (threadIdx.x < 3) place[threadIdx.x] = listed[threadIdx.x] > 0 ? atomicAdd(&s.listed[threadIdx.x], listed[threadIdx.x]) : 0;
+  __syncthreads();
+  for (int j = 0; j < 3; j++)  // past the end: not all of them fit, and the last launch takes the row from its beginning
+    if (threadIdx.x < listed[j] && place[j] + threadIdx.x < LISTED) s.lists[j][place[j] + threadIdx.x] = lists[j][threadIdx.x];
+}
+
+// Parts of a row: some 4096 logits each, and a workgroup for each CU in all; from seven on. (One workgroup a row and parts, with a
+// top-p and with a top-k: 1 x 16384 23 and 27 us, 18 and 24; 1 x 32000 36 and 27, 24 and 24; 1 x 131072 77 and 27, 40 and 25; 32 x 32000
+// 41 and 33, 25 and 27; 32 x 131072 97 and 50, 41 and 31; 64 x 50257 53 and 75, 26 and 30.)
+int parts_of(int64_t rows, int64_t vocab) {
+  const int64_t n = std::min(std::min((int64_t)MOST_PARTS, 256 / rows), vocab / 4096);
+  return n < 7 ? 1 : (int)n;
+}
+
 template <typename T>
-int sample_of(const void* logits, const SampleArgs& a, hipStream_t stream) {
+int sample_of(const void* logits, const SampleArgs& a, SplitRow* split, hipStream_t stream) {
   typedef typename T::Storage S;
   const dim3 grid((unsigned)a.rows);
+  if (const int parts = parts_of(a.rows, a.vocab); parts > 1) {
+    const dim3 many((unsigned)parts, (unsigned)a.rows), block(1024);
+    const int each = (int)(((a.vocab + parts - 1) / parts + 7) / 8 * 8);
+    hipLaunchKernelGGL((sample_largest<T, 1024>), many, block, 0, stream, (const S*)logits, a, split, each);
+    hipLaunchKernelGGL((sample_spread<T, 1024>), many, block, 0, stream, (const S*)logits, a, split, each);
+    hipLaunchKernelGGL((sample_members<T, 1024>), many, block, 0, stream, (const S*)logits, a, split, each);
+    hipLaunchKernelGGL((sample_rows<T, 1024, false, true>), grid, block, 0, stream, (const S*)logits, a, (const SplitRow*)split, parts);
+    return check_hip(hipGetLastError(), "launching sampling");
+  }
   if (a.vocab <= 256)
-    hipLaunchKernelGGL((sample_rows<T, 256, true>), grid, dim3(256), 0, stream, (const S*)logits, a);
+    hipLaunchKernelGGL((sample_rows<T, 256, true, false>), grid, dim3(256), 0, stream, (const S*)logits, a, nullptr, 1);
   else if (a.vocab <= 1024)
-    hipLaunchKernelGGL((sample_rows<T, 1024, true>), grid, dim3(1024), 0, stream, (const S*)logits, a);
+    hipLaunchKernelGGL((sample_rows<T, 1024, true, false>), grid, dim3(1024), 0, stream, (const S*)logits, a, nullptr, 1);
   else
-    hipLaunchKernelGGL((sample_rows<T, 1024, false>), grid, dim3(1024), 0, stream, (const S*)logits, a);
+    hipLaunchKernelGGL((sample_rows<T, 1024, false, false>), grid, dim3(1024), 0, stream, (const S*)logits, a, nullptr, 1);
   return check_hip(hipGetLastError(), "launching sampling");
 }
 
@@ -626,7 +835,9 @@ int sample_of(const void* logits, const SampleArgs& a, hipStream_t stream) {
 
 using namespace limn;
 
-extern "C" int64_t limn_hip_sample_workspace(int dtype, int64_t rows, int64_t vocab) { return 0; }
+extern "C" int64_t limn_hip_sample_workspace(int dtype, int64_t rows, int64_t vocab) {
+  return rows > 0 && vocab > 0 && parts_of(rows, vocab) > 1 ? rows * (int64_t)sizeof(SplitRow) : 0;
+}
 
 extern "C" int limn_hip_sample(const void* logits, const void* uniforms, const void* temperature, const void* top_k, const void* top_p, const void* min_p,
                                void* tokens, void* logprobs, int dtype, int64_t rows, int64_t vocab, int64_t row_stride, void* workspace,
@@ -641,10 +852,14 @@ extern "C" int limn_hip_sample(const void* logits, const void* uniforms, const v
   if ((uintptr_t)logits % size != 0 || words % 4 != 0) return fail(LIMN_HIP_EINVAL, "sample: buffers must be aligned to their element size");
   if (workspace_bytes < 0) return fail(LIMN_HIP_EINVAL, "sample: negative workspace size");
   if (rows > 0x7fffffff || vocab > (1 << 24)) return fail(LIMN_HIP_EUNSUPPORTED, "sample: sizes out of range");
+  const int64_t need = limn_hip_sample_workspace(dtype, rows, vocab);
+  if (need > 0 && (workspace == nullptr || (uintptr_t)workspace % 16 != 0 || workspace_bytes < need))
+    return fail(LIMN_HIP_EINVAL, "sample: needs a workspace of %lld bytes, 16-byte aligned", (long long)need);
   int log2v = 0;
   while (((int64_t)1 << log2v) < vocab) log2v++;
   const SampleArgs a = {(const float*)uniforms, (const float*)temperature, (const int*)top_k, (const float*)top_p, (const float*)min_p, (int*)tokens,
                         (float*)logprobs, rows, vocab, row_stride, 62 - log2v < 52 ? 62 - log2v : 52};
   const hipStream_t s = (hipStream_t)stream;
-  return dtype == LIMN_HIP_FLOAT32 ? sample_of<F32>(logits, a, s) : dtype == LIMN_HIP_FLOAT16 ? sample_of<F16>(logits, a, s) : sample_of<BF16>(logits, a, s);
+  SplitRow* split = (SplitRow*)workspace;
+  return dtype == LIMN_HIP_FLOAT32 ? sample_of<F32>(logits, a, split, s) : dtype == LIMN_HIP_FLOAT16 ? sample_of<F16>(logits, a, split, s) : sample_of<BF16>(logits, a, split, s);
 }

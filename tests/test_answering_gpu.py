@@ -10,10 +10,14 @@ import numpy as np
 import pytest
 import torch
 
-from conftest import DTYPES, storage_values
+from conftest import DTYPES, storage_values, upload
 from limn_amd.dtypes import ABI_CODE
 from limn_amd.hip import runtime
-from limn_amd.seam import bfloat16
+from limn_amd.sampling import sample
+from limn_amd.seam import Tensor, bfloat16, capture, realize, use_device
+from oracle.attend import within
+from oracle.serving import sample as oracle
+from serving import logit_rows
 from test_sample_gpu import TYPES, called, check
 
 pytestmark = pytest.mark.gpu
@@ -71,12 +75,12 @@ class Step:
         return [t.clone() for t in (self.out, self.logits, self.drawn, self.logs, *self.pools)]
 
 
-SHAPES = [((1, 1, 1), 300), ((1,) * 40, 3000), ((200, 1, 70), 700)]
+SHAPES = [((1, 1, 1), 300, 1500), ((1,) * 40, 3000, 1500), ((200, 1, 70), 700, 1500), ((1, 2, 1), 300, 40001)]
 
 
-@pytest.mark.parametrize("counts,most", SHAPES, ids=["few", "parts", "tiles"])
-def test_a_stream_of_the_callers(hipdev, counts, most):
-    step = Step(hipdev.lib, 1, counts, most)
+@pytest.mark.parametrize("counts,most,vocab", SHAPES, ids=["few", "parts", "tiles", "split-rows"])
+def test_a_stream_of_the_callers(hipdev, counts, most, vocab):
+    step = Step(hipdev.lib, 1, counts, most, vocab=vocab)
     pools = [t.clone() for t in step.pools]
     step.run(None)
     torch.cuda.synchronize()
@@ -92,9 +96,9 @@ def test_a_stream_of_the_callers(hipdev, counts, most):
         assert torch.equal(a, b)
 
 
-@pytest.mark.parametrize("counts,most", SHAPES, ids=["few", "parts", "tiles"])
-def test_two_graphs_replayed_in_turn(hipdev, counts, most):
-    steps = [Step(hipdev.lib, s, counts, most) for s in (1, 2)]
+@pytest.mark.parametrize("counts,most,vocab", SHAPES, ids=["few", "parts", "tiles", "split-rows"])
+def test_two_graphs_replayed_in_turn(hipdev, counts, most, vocab):
+    steps = [Step(hipdev.lib, s, counts, most, vocab=vocab) for s in (1, 2)]
     stream, graphs = torch.cuda.Stream(), []
     for step in steps:
         step.run(ctypes.c_void_p(stream.cuda_stream))
@@ -135,6 +139,32 @@ def test_borders_among_equal_logits(hipdev, dtype, steps, top_p):
     check(hipdev, logits, u, dtype, top_p=top_p, top_k=np.geomspace(1, vocab, rows).astype(np.int32))
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,vocab,apart", [(1, 28672, 0), (36, 28675, 3), (5, 30011, 0), (2, 70001, 7), (1, 300001, 0)])
+def test_rows_over_workgroups(hipdev, dtype, rows, vocab, apart):
+    """Every setting at once and alone, rows that end before all others among them: nothing above minus infinity, a largest one without a
+    draw, infinities, equal logits, masks that leave few."""
+    rng = np.random.default_rng(rows + vocab)
+    logits = storage_values((rng.standard_normal((rows, vocab)) * 3).astype(np.float32), DTYPES[dtype])
+    u = rng.random(rows).astype(np.float32)
+    for rules in (dict(), dict(top_p=0.9), dict(top_k=40), dict(top_k=3000), dict(min_p=0.1), dict(temperature=0.8, top_k=100, top_p=0.9, min_p=0.01), dict(top_p=0.8, min_p=0.2),
+                  dict(top_p=0.8, min_p=1.5), dict(temperature=40.0, top_p=0.5)):
+        check(hipdev, logits, u, dtype, apart, **rules)
+    mixed = logits.copy()
+    for r in range(rows):
+        if r % 5 == 0:
+            mixed[r] = [-np.inf, np.nan, 1.0][r // 5 % 3]
+        elif r % 5 == 1:
+            mixed[r, [7, vocab - 1]] = np.inf
+        elif r % 5 == 2:
+            mixed[r, 3:-2] = -np.inf
+        elif r % 5 == 3:
+            mixed[r] = np.round(mixed[r])
+    warm = np.where(np.arange(rows) % 4 == 3, 0.0, 0.9).astype(np.float32)
+    for rules in (dict(), dict(top_p=0.9), dict(top_k=50), dict(top_k=2, top_p=0.5)):
+        check(hipdev, mixed, u, dtype, apart, temperature=warm, **rules)
+
+
 def test_the_largest_vocabulary(hipdev):
     """2^24 logits. Their masses are off by sqrt(2^24) half units of 2^-38 of the largest weight, 4e-9 of it; a drawn token's is
     some 1e-3 of it, so a border moves past one in a case of 10^5."""
@@ -143,3 +173,25 @@ def test_the_largest_vocabulary(hipdev):
     check(hipdev, logits, u, "float32", top_p=0.8)
     with pytest.raises(NotImplementedError):
         called(hipdev, np.zeros((1, (1 << 24) + 1), np.float32), u, "float32")
+
+
+def test_split_rows_captured_through_the_tensor_api(hipdev):
+    """The workspace that a replay holds is the device's own, and other calls use it between two replays."""
+    use_device(hipdev)
+    logits, u, rng = logit_rows(7, 6, 40001, "bfloat16")
+    t = Tensor.from_node(upload(hipdev, logits, DTYPES["bfloat16"]))
+
+    def step(x, u):
+        got = sample(x, u, temperature=0.8, top_p=0.9) + sample(x, u, top_k=30)
+        realize(*got)
+        return got
+
+    run, full = capture(step), lambda value, kind=np.float32: np.full(6, value, kind)
+    for turn in range(6):
+        u = rng.random(6).astype(np.float32)
+        got = run(t, Tensor(u).realize())
+        for (tokens, logs), rules in ((got[:2], dict(temperature=full(0.8), top_p=full(0.9))), (got[2:], dict(top_k=full(30, np.int32)))):
+            want, (lp, bound) = oracle(logits, u, **rules)
+            np.testing.assert_array_equal(tokens.numpy(), want)
+            within(logs.numpy(), lp, bound, "logprob")
+        sample(t, Tensor(1 - u), top_p=0.5)[0].numpy()
