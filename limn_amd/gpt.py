@@ -161,7 +161,7 @@ class Block:
         qkv, kv = mixed(self.qkv, normed(self.ln1, x)), cfg.key_heads * hd
         q, k, v = (part.reshape(n, -1, hd) for part in (qkv[:, :c], qkv[:, c : c + kv], qkv[:, c + kv :]))
         att = attend_paged(q, k, v, *pages, *where, softcap=cfg.softcap, slopes=slopes)
-        x = materialized(x + mixed(self.proj, att.reshape(n, c)))
+        x = materialized(x + mixed(self.proj, att.cast(x.dtype).reshape(n, c)))
         return materialized(x + mixed(self.down, gelu(mixed(self.up, normed(self.ln2, x)))))
 
 

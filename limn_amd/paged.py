@@ -50,7 +50,7 @@ def attend_paged(q: Tensor, k: Tensor | None, v: Tensor | None, key_pages: Tenso
     width = key_pages.dtype
     if width not in FLOATS or value_pages.dtype != width:
         raise ValueError(f"attend_paged needs pages of one float dtype, got {key_pages.dtype} and {value_pages.dtype}")
-    if key_pages.node is value_pages.node or any(t.node.op is not Op.BUFFER for t in (key_pages, value_pages)):
+    if any(t.node.op is not Op.BUFFER for t in (key_pages, value_pages)) or key_pages.node.arg is value_pages.node.arg:
         raise ValueError("attend_paged writes its pages in place: they must be two realized buffers")
     if (k is None) != (v is None):
         raise ValueError("attend_paged: new keys and new values go together")

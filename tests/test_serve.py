@@ -9,7 +9,7 @@ import numpy as np
 import pytest
 
 from limn_amd.gpt import GPT, GPTConfig, Held
-from limn_amd.seam import Tensor, float32, int8, int32, no_grad, set_seed
+from limn_amd.seam import Tensor, bfloat16, float32, int8, int32, no_grad, set_seed
 from limn_amd.seam import device as limn_device
 from limn_amd.serve import Cache, generate, held, prefill
 from serving import PROMPTS, whole_logits
@@ -50,6 +50,20 @@ def test_prompts_in_parts_are_the_whole_model(cfg, part, small):
         got = prefill(model, cache, range(len(PROMPTS)), PROMPTS, cache.table(range(len(PROMPTS))), part).numpy()
         want = np.stack([whole_logits(model, p)[-1] for p in PROMPTS])
     assert np.abs(got - want).max() <= (WORST_INT8 if small else WORST) * np.abs(want).max()
+
+
+def test_a_cache_of_a_wider_type():
+    """bfloat16 rows over float32 pages: queries, keys and values are cast to the pages' type, the stream stays the model's."""
+    cfg = replace(EVERY, dtype=bfloat16)
+    with no_grad():
+        model = held(model_of(cfg))
+        cache = Cache(model, 3, 8, dtype=float32)
+        cache.reserve(0, 11)
+        got = prefill(model, cache, [0], [PROMPTS[2]], cache.table([0]), 5)
+        assert got.dtype == bfloat16 and cache.layers[0][0].dtype == float32
+        want = whole_logits(model, PROMPTS[2])[-1]
+    # bfloat16 nodes on the oracle: some 30 roundings of up to 2^-8 between the two, 6 2^-8 as they go both ways
+    assert np.abs(got.numpy()[0] - want).max() <= 3e-2 * np.abs(want).max()
 
 
 @pytest.mark.parametrize("cfg", [PLAIN, EVERY], ids=["plain", "every"])

@@ -237,6 +237,8 @@ def call(entry, workspace=FAKE, room=1 << 40, **kw):
         ("sample", dict(uniforms=None), 1, "null"),
         ("sample", dict(logits=ODD), 1, "aligned"),
         ("sample", dict(room=-1), 1, "workspace"),
+        ("sample", dict(vocab=1 << 16, stride=1 << 16, workspace=None), 1, "workspace"),
+        ("sample", dict(vocab=1 << 16, stride=1 << 16, room=1000), 1, "workspace"),
         ("quantize", dict(dtype=5), 2, "float32, float16 or bfloat16"),
         ("quantize", dict(width=0), 1, "positive"),
         ("quantize", dict(s=None), 1, "null"),
