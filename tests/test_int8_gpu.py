@@ -51,7 +51,7 @@ def check(dev, x, w, scales, bias, dtype, **kw):
 
 
 SIZES = [(1, 1, 1), (1, 64, 64), (3, 24, 17), (1, 760, 1000), (16, 512, 1536), (17, 128, 33), (32, 1000, 300), (33, 257, 65), (64, 4096, 128), (65, 130, 513), (130, 96, 1025), (257, 777, 129),
-         (300, 1536, 512), (1021, 48, 257), (5, 20000, 40), (2100, 300, 2049)]
+         (300, 1536, 512), (1021, 48, 257), (5, 20000, 40), (2100, 300, 2049), (4100, 70, 4099)]
 
 
 @pytest.mark.parametrize("dtype", TYPES)
