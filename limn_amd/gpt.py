@@ -157,10 +157,8 @@ class Block:
         """The rows x (tokens, dim) of new tokens through the block, over `pages` of the keys and values before them; `where`:
         starts, lengths and table, as `attend_paged` takes them."""
         n, c = x.shape
-        cfg, hd = self.cfg, self.cfg.dim // self.heads
-        qkv, kv = mixed(self.qkv, normed(self.ln1, x)), cfg.key_heads * hd
-        q, k, v = (part.reshape(n, -1, hd) for part in (qkv[:, :c], qkv[:, c : c + kv], qkv[:, c + kv :]))
-        att = attend_paged(q, k, v, *pages, *where, softcap=cfg.softcap, slopes=slopes)
+        qkv = mixed(self.qkv, normed(self.ln1, x))
+        att = attend_paged(qkv, None, None, *pages, *where, softcap=self.cfg.softcap, slopes=slopes, heads=self.heads)
         x = materialized(x + mixed(self.proj, att.cast(x.dtype).reshape(n, c)))
         return materialized(x + mixed(self.down, gelu(mixed(self.up, normed(self.ln2, x)))))
 

@@ -678,27 +678,29 @@ class HipDevice(CompiledDevice):
     def _paged_runner(self, node: Node) -> Runner:
         """CUSTOM attend_paged (srcs q, the new k and v if given, both pools of pages, starts, lengths, table, slopes if given),
         bound to limn_hip_attend_paged. It writes the pools, which are sources, in place. params: (scale, softcap, whether k
-        and v are given, whether slopes are)."""
-        name, (scale, softcap, fresh, sloped) = node.arg.name, node.arg.params
+        and v are given, whether slopes are, whether q holds each token's queries, keys and values)."""
+        name, (scale, softcap, fresh, sloped, together) = node.arg.name, node.arg.params
         if len(node.srcs) != 6 + 2 * fresh + sloped:
             raise ValueError(f"{name}: expected {6 + 2 * fresh + sloped} srcs, got {len(node.srcs)}")
         q, news, (keys, values, starts, lengths, table), slopes = node.srcs[0], node.srcs[1 : 1 + 2 * fresh], node.srcs[1 + 2 * fresh : 6 + 2 * fresh], node.srcs[6 + 2 * fresh :]
         if q.dtype not in ABI_CODE or q.dtype not in FLOATS or any(s.dtype != q.dtype for s in (*news, keys, values)):
             raise NotImplementedError(f"{name}: no kernel for dtypes {[s.dtype for s in (q, *news, keys, values)]}")
-        if len(q.shape) != 3 or len(keys.shape) != 4 or len(table.shape) != 2:
+        if len(q.shape) != (2 if together else 3) or len(keys.shape) != 4 or len(table.shape) != 2 or (together and fresh):
             raise ValueError(f"{name} shape mismatch: {[s.shape for s in node.srcs]}")
-        (tokens, heads, hd), (pages, kv_heads, page, _), (sequences, table_pages) = q.shape, keys.shape, table.shape
-        if (keys.shape[-1] != hd or values.shape != keys.shape or any(s.shape != (tokens, kv_heads, hd) for s in news) or starts.shape != (sequences + 1,)
+        tokens, (pages, kv_heads, page, hd), (sequences, table_pages) = q.shape[0], keys.shape, table.shape
+        heads = q.shape[1] // hd - 2 * kv_heads if together else q.shape[1]
+        if (q.shape[1:] != (((heads + 2 * kv_heads) * hd,) if together else (heads, hd)) or values.shape != keys.shape or any(s.shape != (tokens, kv_heads, hd) for s in news) or starts.shape != (sequences + 1,)
                 or lengths.shape != (sequences,) or any(s.shape != (heads,) or s.dtype != float32 for s in slopes) or any(s.dtype != int32 for s in (starts, lengths, table))):
             raise ValueError(f"{name} shape mismatch: {[(s.shape, s.dtype) for s in node.srcs]}")
         code, sizes = ABI_CODE[q.dtype], (tokens, sequences, heads, kv_heads, hd, pages, page, table_pages)
-        rows, scale, softcap = (heads * hd, kv_heads * hd, kv_heads * hd), float(scale), float(softcap)
+        rows, scale, softcap = (q.shape[1],) * 3 if together else (heads * hd, kv_heads * hd, kv_heads * hd), float(scale), float(softcap)
+        behind = tuple(n * hd * q.dtype.itemsize for n in (heads, heads + kv_heads))
         need = int(self.lib.limn_hip_attend_paged_workspace(code, *sizes))
         cap_bits = ctypes.c_int64.from_buffer_copy(ctypes.c_double(softcap)).value
 
         def run(inputs: list[Buffer], outs: list[Buffer]) -> None:
             ptrs = [b.ptr for b in inputs]
-            args = (ptrs[0], *(ptrs[1:3] if fresh else (None, None)), *ptrs[1 + 2 * fresh : 6 + 2 * fresh], ptrs[-1] if sloped else None, outs[0].ptr, code, *sizes, *rows)
+            args = (ptrs[0], *(ptrs[1:3] if fresh else [ptrs[0] + b for b in behind] if together else (None, None)), *ptrs[1 + 2 * fresh : 6 + 2 * fresh], ptrs[-1] if sloped else None, outs[0].ptr, code, *sizes, *rows)
             ws, room = self._scratch(need)
             check_limn(self.lib.limn_hip_attend_paged(*args, scale, softcap, ws, room, None))
             if self.tape is not None:

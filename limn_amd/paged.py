@@ -24,7 +24,7 @@ ATTEND_PAGED = "attend_paged"
 
 
 def attend_paged(q: Tensor, k: Tensor | None, v: Tensor | None, key_pages: Tensor, value_pages: Tensor, starts: Tensor, lengths: Tensor, table: Tensor,
-                 *, softcap: float = 0.0, slopes: Tensor | None = None, scale: float | None = None) -> Tensor:
+                 *, softcap: float = 0.0, slopes: Tensor | None = None, scale: float | None = None, heads: int = 0) -> Tensor:
     """Attention of packed new tokens q (tokens, heads, hd) over a paged cache, which takes up their k and v (tokens, kv_heads, hd).
 
     - `key_pages`, `value_pages` (pages, kv_heads, page, hd): the cache, realized buffers; written in place when the result
@@ -37,13 +37,19 @@ def attend_paged(q: Tensor, k: Tensor | None, v: Tensor | None, key_pages: Tenso
       anything. Keys of a page number that is not in the cache are not there: nothing is written, and no query sees them.
       Sequences may share pages that none of them writes to in this call; a page that is written stands in the table once.
     - `slopes` (heads,) float32, `softcap`, `scale`: as in `attend`.
+    - `heads`: q holds all that is new, each token's queries, keys and values one behind another, (tokens, (heads + 2 kv_heads) hd), as
+      a layer's one product gives them; k and v are None then, and nothing is copied apart.
+
+    The result is (tokens, heads, hd).
 
     There is no gradient: the call is for answering (under `no_grad`, or on tensors that need none).
     """
-    if q.ndim != 3 or key_pages.ndim != 4:
-        raise ValueError(f"attend_paged needs (tokens, heads, hd) queries and (pages, kv_heads, page, hd) pages, got {q.shape} and {key_pages.shape}")
-    (tokens, heads, hd), (pages, kv_heads, page, _) = q.shape, key_pages.shape
-    if key_pages.shape[-1] != hd or value_pages.shape != key_pages.shape:
+    together = heads > 0
+    if heads < 0 or q.ndim != (2 if together else 3) or key_pages.ndim != 4:
+        raise ValueError(f"attend_paged needs (tokens, heads, hd) queries, or all in one with `heads`, and (pages, kv_heads, page, hd) pages, got {q.shape} and {key_pages.shape}")
+    (pages, kv_heads, page, hd), tokens = key_pages.shape, q.shape[0]
+    heads = heads or q.shape[1]
+    if q.shape[1:] != (((heads + 2 * kv_heads) * hd,) if together else (heads, hd)) or value_pages.shape != key_pages.shape:
         raise ValueError(f"attend_paged shape mismatch: {q.shape}, {key_pages.shape}, {value_pages.shape}")
     if heads % kv_heads:
         raise ValueError(f"attend_paged: {heads} query heads do not share {kv_heads} key heads evenly")
@@ -52,8 +58,8 @@ def attend_paged(q: Tensor, k: Tensor | None, v: Tensor | None, key_pages: Tenso
         raise ValueError(f"attend_paged needs pages of one float dtype, got {key_pages.dtype} and {value_pages.dtype}")
     if any(t.node.op is not Op.BUFFER for t in (key_pages, value_pages)) or key_pages.node.arg is value_pages.node.arg:
         raise ValueError("attend_paged writes its pages in place: they must be two realized buffers")
-    if (k is None) != (v is None):
-        raise ValueError("attend_paged: new keys and new values go together")
+    if (k is None) != (v is None) or (together and k is not None):
+        raise ValueError("attend_paged: new keys and new values go together, and not beside queries that hold them")
     fresh = () if k is None else (k, v)
     if any(t.shape != (tokens, kv_heads, hd) for t in fresh):
         raise ValueError(f"attend_paged: new keys and values must be {(tokens, kv_heads, hd)}, got {k.shape} and {v.shape}")
@@ -77,12 +83,15 @@ def attend_paged(q: Tensor, k: Tensor | None, v: Tensor | None, key_pages: Tenso
         raise ValueError("attend_paged has no gradient: call it under no_grad, or on tensors that need none")
     q, *fresh = (t.cast(width) for t in (q, *fresh))
     if width == float64 or hd > 256 or not active_device().has_custom(ATTEND_PAGED):
+        if together:
+            at, kv = heads * hd, kv_heads * hd
+            q, *fresh = (t.reshape(tokens, -1, hd) for t in (q[:, :at], q[:, at : at + kv], q[:, at + kv :]))
         return _composed(q, *(fresh or (None, None)), key_pages, value_pages, starts, lengths, table, slopes, scale, softcap)
     if any(isinstance(t.node.arg, np.ndarray) for t in (key_pages, value_pages)):
         raise ValueError("attend_paged writes its pages in place: they must lie on the device")
     given = (starts, lengths, table) + (() if slopes is None else (slopes,))
     srcs = tuple(contiguous(t).node for t in (q, *fresh, key_pages, value_pages, *given))
-    (out,) = custom(ATTEND_PAGED, srcs, (scale, softcap, bool(fresh), slopes is not None), ((width, q.shape),))
+    (out,) = custom(ATTEND_PAGED, srcs, (scale, softcap, bool(fresh), slopes is not None, together), ((width, (tokens, heads, hd)),))
     return Tensor.from_node(out)
 
 

@@ -13,11 +13,12 @@ import torch
 from conftest import DTYPES, storage_values, upload
 from limn_amd.dtypes import ABI_CODE
 from limn_amd.hip import runtime
+from limn_amd.paged import attend_paged
 from limn_amd.sampling import sample
-from limn_amd.seam import Tensor, bfloat16, capture, realize, use_device
+from limn_amd.seam import Tensor, bfloat16, capture, int32, realize, use_device
 from oracle.attend import within
 from oracle.serving import sample as oracle
-from serving import logit_rows
+from serving import logit_rows, paged_inputs
 from test_sample_gpu import TYPES, called, check
 
 pytestmark = pytest.mark.gpu
@@ -195,3 +196,29 @@ def test_split_rows_captured_through_the_tensor_api(hipdev):
             np.testing.assert_array_equal(tokens.numpy(), want)
             within(logs.numpy(), lp, bound, "logprob")
         sample(t, Tensor(1 - u), top_p=0.5)[0].numpy()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("counts,lengths,heads,kv_heads,hd", [((1, 1, 1), (40, 9, 300), 8, 2, 64), ((1,), (5,), 3, 1, 33), ((130, 2), (200, 64), 4, 4, 80), ((2, 5), (9, 70), 2, 2, 200)])
+def test_queries_keys_and_values_in_one(hipdev, dtype, counts, lengths, heads, kv_heads, hd):
+    """The bits of the call with each apart, through the Tensor API, captured too."""
+    use_device(hipdev)
+    x = paged_inputs(3, dtype=dtype, counts=counts, lengths=lengths, heads=heads, kv_heads=kv_heads, hd=hd, page=16, spare=1)
+    t = DTYPES[dtype]
+    on = lambda a, kind=t: Tensor.from_node(upload(hipdev, a, kind))  # noqa: E731
+    where = [on(x[n], int32) for n in ("starts", "lengths", "table")]
+    apart, one = ([on(x[n]) for n in ("key_pages", "value_pages")] for _ in range(2))
+    together = on(np.concatenate([x[n].reshape(len(x["q"]), -1) for n in ("q", "k", "v")], 1))
+
+    def step(qkv):
+        out = attend_paged(qkv, None, None, *one, *where, softcap=5.0, heads=heads)
+        realize(out)
+        return out
+
+    want = attend_paged(*(on(x[n]) for n in ("q", "k", "v")), *apart, *where, softcap=5.0).numpy()
+    run = capture(step)
+    for _ in range(4):
+        np.testing.assert_array_equal(run(together).numpy(), want)
+        for a, b in zip(one, apart):
+            np.testing.assert_array_equal(a.numpy(), b.numpy())
+        assert (Tensor(np.ones(1000)) * 3.0).sum().item() == 3000.0

@@ -256,3 +256,21 @@ def call(entry, workspace=FAKE, room=1 << 40, **kw):
 def test_the_abi_refuses_with_a_reason(entry, kw, code, message):
     assert call(entry, **kw) == code
     assert message in runtime.kernels().limn_hip_last_error().decode()
+
+
+def test_paged_queries_keys_and_values_in_one():
+    x = paged_inputs(5, counts=(2, 1), lengths=(7, 3), heads=4, kv_heads=2, hd=8, spare=1)
+    tokens = len(x["q"])
+    on = lambda n: Tensor(x[n])  # noqa: E731
+    where = lambda: [Tensor(x[n], dtype=int32) for n in ("starts", "lengths", "table")]  # noqa: E731
+    apart, one = ([on("key_pages"), on("value_pages")] for _ in range(2))
+    want = attend_paged(on("q"), on("k"), on("v"), *apart, *where()).numpy()
+    qkv = np.concatenate([x[n].reshape(tokens, -1) for n in ("q", "k", "v")], 1)
+    np.testing.assert_array_equal(attend_paged(Tensor(qkv), None, None, *one, *where(), heads=4).numpy(), want)
+    for a, b in zip(one, apart):
+        np.testing.assert_array_equal(a.numpy(), b.numpy())
+    for bad, heads, match in ((qkv, 3, "mismatch"), (qkv[:, :-1], 4, "mismatch"), (x["q"], 4, "all in one"), (qkv, -1, "all in one"), (qkv, 0, "all in one")):
+        with pytest.raises(ValueError, match=match):
+            attend_paged(Tensor(bad), None, None, *one, *where(), heads=heads)
+    with pytest.raises(ValueError, match="beside"):
+        attend_paged(Tensor(qkv), on("k"), on("v"), *one, *where(), heads=4)
