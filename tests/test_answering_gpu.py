@@ -222,3 +222,19 @@ def test_queries_keys_and_values_in_one(hipdev, dtype, counts, lengths, heads, k
         for a, b in zip(one, apart):
             np.testing.assert_array_equal(a.numpy(), b.numpy())
         assert (Tensor(np.ones(1000)) * 3.0).sum().item() == 3000.0
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("few", [False, True], ids=["every", "few-values"])
+def test_settings_of_every_split_row(hipdev, dtype, few):
+    rng = np.random.default_rng(9)
+    rows, vocab = 36, 30011
+    logits = storage_values((rng.standard_normal((rows, vocab)) * 2.5).astype(np.float32), DTYPES[dtype])
+    if few:
+        logits = np.round(logits) * rng.choice([-0.0, 0.0, 1.0], (rows, vocab)).astype(np.float32)  # both zeros are equal
+    for _ in range(3):
+        u = rng.choice([-1.0, 0.0, 0.3, 0.999999, 1.0, 7.0, np.nan, -1.0, 0.5], rows).astype(np.float32)
+        check(hipdev, logits, u, dtype, temperature=rng.choice([-1.0, 0.0, 1e-30, 0.01, 0.5, 1.0, 2.0, 1e30, np.nan, np.inf], rows).astype(np.float32),
+              top_k=rng.choice([-3, 0, 1, 2, 10, 2000, vocab - 1, vocab, 2**31 - 1], rows).astype(np.int32), top_p=rng.choice([-1.0, 0.0, 1e-9, 0.3, 0.99, 1.0, 2.0, np.nan], rows).astype(np.float32),
+              min_p=rng.choice([-1.0, 0.0, 1e-9, 0.1, 1.0, 5.0, np.nan], rows).astype(np.float32))
+        check(hipdev, logits, u, dtype, top_p=rng.choice([-1.0, 0.0, 1e-9, 0.3, 0.99, 1.0, 2.0, np.nan], rows).astype(np.float32), min_p=rng.choice([-1.0, 0.0, 1e-9, 0.1, 1.0, 5.0, np.nan], rows).astype(np.float32))
