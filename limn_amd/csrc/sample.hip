@@ -155,9 +155,13 @@ struct Row {
 
   __device__ __forceinline__ float seen(float v) const { return v >= least ? fminf(v, most) : -__builtin_inff(); }
 
-  // f(logit, index) for every element, some of them by this thread
-  template <typename F>
+  // f(logit, index) for every element, some of them by this thread; WHOLE: one at most
+  template <bool WHOLE = false, typename F>
   __device__ __forceinline__ void each(F f) const {
+    if constexpr (WHOLE) {
+      if ((int)threadIdx.x < vocab) f(seen(T::load(x, threadIdx.x)), (int)threadIdx.x);
+      return;
+    }
     const u32x4* body = (const u32x4*)(x + head);
     int c = threadIdx.x;
     constexpr int U = 4;
@@ -208,9 +212,10 @@ struct Row {
   // 64 bins an e-fold of the weight; monotone in v: each step rounds, none turns the order round
   __device__ __forceinline__ int bin(float v) const { return v == top ? 0 : (int)fminf((top - v) * inv, (float)(BINS - 1)); }
 
+  template <bool WHOLE = false>
   __device__ __forceinline__ float largest_of() const {
     float best = -__builtin_inff();
-    each([&](float v, int) __attribute__((always_inline)) { best = fmaxf(best, v); });
+    each<WHOLE>([&](float v, int) __attribute__((always_inline)) { best = fmaxf(best, v); });
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) best = fmaxf(best, __shfl_xor(best, o));
     if ((threadIdx.x & 63) == 0) sh.counts[threadIdx.x >> 6] = __float_as_uint(best);
@@ -548,7 +553,7 @@ __global__ __launch_bounds__(TH) void sample_rows(const typename T::Storage* __r
   if (threadIdx.x < 64) sh.powers[threadIdx.x] = exp2(a.bits + threadIdx.x * 0.015625);
   Row<T, TH> row(logits + n * a.row_stride, vocab, a.bits, sh);
   const SplitRow* given = SPLIT ? split + n : nullptr;
-  const float best = SPLIT ? row_best(*given, parts) : row.largest_of();
+  const float best = SPLIT ? row_best(*given, parts) : row.template largest_of<WHOLE>();
   auto give = [&](int token, float logprob) {
     if (threadIdx.x != 0) return;
     a.tokens[n] = token;
@@ -562,7 +567,7 @@ __global__ __launch_bounds__(TH) void sample_rows(const typename T::Storage* __r
     if (threadIdx.x == 0) sh.word = 0xffffffffu;
     __syncthreads();
     unsigned first = 0xffffffffu;
-    row.each([&](float v, int i) __attribute__((always_inline)) {
+    row.template each<WHOLE>([&](float v, int i) __attribute__((always_inline)) {
       if (v == best) first = min(first, (unsigned)i);
     });
     if (first != 0xffffffffu) atomicMin(&sh.word, first);
@@ -580,7 +585,9 @@ __global__ __launch_bounds__(TH) void sample_rows(const typename T::Storage* __r
   uint64_t e = ~0ull, total = 0, kept = 0;
   const double least_weight = (double)q * one;
   if constexpr (WHOLE) {
-    e = row.sorted([](float) __attribute__((always_inline)) { return true; }, whole);
+    row.template each<true>([&](float v, int i) __attribute__((always_inline)) { sh.list[i] = ((uint64_t)~key_of(v) << 32) | (unsigned)i; });
+    __syncthreads();
+    e = row.arranged(sh.list, vocab);
   } else {
     if (!lists) row.clear(bins.mass0, bins.count0);
     if (lists && few) {
