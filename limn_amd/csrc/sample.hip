@@ -36,6 +36,7 @@ namespace limn {
 namespace {
 
 constexpr int BINS = 2048;
+constexpr int PAD = 16;  // room behind a list
 
 struct SampleArgs {
   const float* uniforms;
@@ -72,7 +73,8 @@ __device__ __forceinline__ bool shorter(const Border& a, const Border& b) {
 
 template <int TH>
 struct Shared {
-  uint64_t list[TH], sums[TH / 64];  // list: of elements, see Row::append
+  alignas(16) uint64_t list[TH + PAD];  // of elements, see Row::append
+  uint64_t sums[TH / 64];
   unsigned counts[TH / 64];
   uint64_t found_mass, found_element;
   unsigned found_bin, found_count, listed, word;
@@ -89,7 +91,7 @@ template <int TH>
 struct Bins {
   uint64_t mass0[BINS], mass[BINS];
   unsigned count0[BINS], count[BINS];  // count0: where a top-k asks for it
-  alignas(16) uint64_t list[3][TH];
+  alignas(16) uint64_t list[3][TH + PAD];
   unsigned listed[3];
   Three at;
 };
@@ -421,10 +423,17 @@ struct Row {
     uint64_t e = (int)threadIdx.x < n ? list[threadIdx.x] : ~0ull;
     const int wave0 = (int)(threadIdx.x & ~63u);
     if (n <= 512) {  // the place of each is the number of those before it: n reads that all lanes share; a sorting network of 36 steps took 6 us for 256
+      if (threadIdx.x < PAD) list[n + threadIdx.x] = ~0ull;
+      __syncthreads();
       int rank = 0;
       if (wave0 < n) {
-#pragma unroll 8
-        for (int j = 0; j < n; j++) rank += list[j] < e;
+        for (int j = 0; j < n; j += PAD) {
+          ulonglong2 o[PAD / 2];
+#pragma unroll
+          for (int i = 0; i < PAD / 2; i++) o[i] = *(const ulonglong2*)(list + j + 2 * i);
+#pragma unroll
+          for (int i = 0; i < PAD / 2; i++) rank += (int)(o[i].x < e) + (int)(o[i].y < e);
+        }
       }
       __syncthreads();
       if ((int)threadIdx.x < n) list[rank] = e;
