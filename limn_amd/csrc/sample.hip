@@ -16,8 +16,8 @@
 //
 // What bounds it: 256 rows of 131072 float32 logits, a workgroup a CU, take 130 us: 19 for the largest (the 134 MB come once from
 // memory and then from the last cache), 48 for the masses, which is the rate of 64-bit atomics on shared memory (48 cycles for 64
-// of them), 24 for the members, 20 for sorting and placing. 64 rows of 65536 bfloat16 with a top-k take 29 us, one row of 50257 28
-// in four launches of 3, 7, 9 and 9, chains of small steps; 32 rows of 256 10. (Tried for a top-k and no faster: the kth of every four threads' largest as a bound
+// of them), 24 for the members, 20 for sorting and placing. 64 rows of 65536 bfloat16 with a top-k take 28 us, one row of 50257 28
+// in four launches of 3, 7, 9 and 9, chains of small steps; 32 rows of 256 9. (Tried for a top-k and no faster: the kth of every four threads' largest as a bound
 // in place of the counts, 28 us.)
 //
 // Masses are whole numbers, w 2^F rounded with F such that a row's sum stays below 2^63: sums of them do not depend on
@@ -83,9 +83,7 @@ struct Shared {
 // The logits of three bins: a border's, and the draw's two (the second one empty where they are the same).
 struct Three {
   float least[3], most[3];
-  __device__ __forceinline__ bool in(int j, float v) const { return v >= least[j] && v <= most[j]; }
-  // a list of the draw's that v is in, 0 if it is only in the border's, -1
-  __device__ __forceinline__ int list(float v) const { return in(2, v) ? 2 : in(1, v) ? 1 : in(0, v) ? 0 : -1; }
+  __device__ __forceinline__ bool has(int j, float v) const { return v >= least[j] && v <= most[j]; }
 };
 template <int TH>
 struct Bins {
@@ -653,10 +651,10 @@ __global__ __launch_bounds__(TH) void sample_rows(const typename T::Storage* __r
         __syncthreads();
         const Three at = bins.at;
         row.each([&](float v, int i) __attribute__((always_inline)) {
-          const int j = at.list(v);
-          if (j >= 0) {
-            if (at.in(0, v)) row.append(bins.list[0], bins.listed[0], v, i);
-            if (j > 0) row.append(bins.list[j], bins.listed[j], v, i);
+          const bool border = at.has(0, v), one = at.has(1, v), two = at.has(2, v);
+          if (border | one | two) {
+            if (border) row.append(bins.list[0], bins.listed[0], v, i);
+            if (one | two) row.append(bins.list[1 + two], bins.listed[1 + two], v, i);
           }
         });
         __syncthreads();
@@ -803,10 +801,10 @@ __global__ __launch_bounds__(TH) void sample_members(const typename T::Storage* 
   __syncthreads();
   const Three in = three;
   row.each([&](float v, int i) __attribute__((always_inline)) {
-    const int j = in.list(v);
-    if (j >= 0) {
-      if (in.in(0, v)) row.append(lists[0], listed[0], v, at.begin + i);
-      if (j > 0) row.append(lists[j], listed[j], v, at.begin + i);
+    const bool border = in.has(0, v), one = in.has(1, v), two = in.has(2, v);
+    if (border | one | two) {
+      if (border) row.append(lists[0], listed[0], v, at.begin + i);
+      if (one | two) row.append(lists[1 + two], listed[1 + two], v, at.begin + i);
     }
   });
   __syncthreads();
