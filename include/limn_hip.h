@@ -335,7 +335,8 @@ int limn_hip_quantize_rows(const void* x, void* values, void* scales, int dtype,
  * A linear layer in 8-bit integers: x (rows, width) brought to 8 bits as limn_hip_quantize_rows does, x8 with scales s, then
  *   out[r][n] = (sum_i x8[r][i] weight[n][i]) s[r] weight_scales[n] + bias[n]
  * with weight (outputs, width) int8, weight_scales (outputs) float32, bias (outputs) of x's type or NULL, out (rows, outputs) of x's
- * type. The sums are exact; their products with the scales and the sum with the bias are float32, rounded once to out's type.
+ * type. The sums are exact; their products with the scales and the sum with the bias are float32, rounded once to out's type: a row's
+ * bits do not depend on the rows beside it.
  * width up to 2^17. Workspace as above, of limn_hip_int8_linear_workspace(...) bytes. No counterpart in the reference.
  */
 int limn_hip_int8_linear(const void* x, const void* weight, const void* weight_scales, const void* bias, void* out, int dtype,

@@ -14,7 +14,8 @@
 // step ahead, the last one's of a stage in the next stage, which has landed by then.
 //
 // int8_few (up to 16 rows; bound by reading the weight once): a wave has 16 outputs and a part of the width, its bytes read from
-// memory straight into operands of v_mfma_i32_16x16x64_i8; the waves of a workgroup add their sums in LDS.
+// memory straight into operands of v_mfma_i32_16x16x64_i8; the waves of a workgroup add their sums in LDS. A few inputs are brought
+// to 8 bits by every workgroup, while its weights are on their way.
 
 #include "common.h"
 
@@ -69,6 +70,25 @@ struct Eight<F32> {
   __device__ __forceinline__ float at(int i) const { return i < 4 ? lo[i & 3] : hi[i & 3]; }
 };
 
+// A row's scale, from its largest magnitude (an infinity where the row has one or a NaN), and its numbers.
+struct Rounding {
+  float s;
+  bool fine;
+  __device__ __forceinline__ explicit Rounding(float top) : s(fmaxf(top / 127.f, 0x1p-126f)), fine(top < __builtin_inff()) {}
+  __device__ __forceinline__ float scale() const { return fine ? s : __builtin_nanf(""); }
+  __device__ __forceinline__ int operator()(float v) const { return fine ? (int)rintf(v / s) : 0; }
+  template <typename E>
+  __device__ __forceinline__ uint2 eight(const E& x) const {
+    unsigned lo = 0, hi = 0;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      lo |= ((unsigned)(*this)(x.at(i)) & 255u) << (8 * i);
+      hi |= ((unsigned)(*this)(x.at(4 + i)) & 255u) << (8 * i);
+    }
+    return make_uint2(lo, hi);
+  }
+};
+
 constexpr int HELD = 4;  // eights a thread of quantize_rows holds between its two uses: 8192 elements a row
 
 // A workgroup a row: its largest magnitude, then its numbers, `stride` bytes a row, zeros behind the width. A row with an
@@ -117,22 +137,12 @@ __global__ __launch_bounds__(256) void quantize_rows(const typename T::Storage* 
   if ((threadIdx.x & 63) == 0) tops[threadIdx.x >> 6] = top;
   __syncthreads();
   top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
-  const bool fine = top < __builtin_inff();
-  const float s = fmaxf(top / 127.f, 0x1p-126f);
-  if (threadIdx.x == 0) scales[blockIdx.x] = fine ? s : __builtin_nanf("");
-  auto round8 = [&](float v) __attribute__((always_inline)) { return fine ? (int)rintf(v / s) : 0; };
+  const Rounding by(top);
+  if (threadIdx.x == 0) scales[blockIdx.x] = by.scale();
 #pragma unroll
   for (int h = 0; h < HELD; h++)
-    if (h * 256 + threadIdx.x < eights) {
-      unsigned lo = 0, hi = 0;
-#pragma unroll
-      for (int i = 0; i < 4; i++) {
-        lo |= ((unsigned)round8(held[h].at(i)) & 255u) << (8 * i);
-        hi |= ((unsigned)round8(held[h].at(4 + i)) & 255u) << (8 * i);
-      }
-      *(uint2*)(o + (h * 256 + threadIdx.x) * 8) = make_uint2(lo, hi);
-    }
-  for (int64_t i = (vec ? HELD * 2048 : 0) + threadIdx.x; i < width; i += 256) o[i] = (signed char)round8(T::load(row, i));
+    if (h * 256 + threadIdx.x < eights) *(uint2*)(o + (h * 256 + threadIdx.x) * 8) = by.eight(held[h]);
+  for (int64_t i = (vec ? HELD * 2048 : 0) + threadIdx.x; i < width; i += 256) o[i] = (signed char)by(T::load(row, i));
   for (int64_t i = width + threadIdx.x; i < stride; i += 256) o[i] = 0;
 }
 
@@ -171,9 +181,12 @@ struct Tile {
   static __device__ __forceinline__ i32x4 operand(const char* tile, int at, int t) { return *(const i32x4*)(tile + at + t * 32 * STAGE); }
 };
 
-// A sum times the weight's scale, then times the scale of x, which may be as large as x.
-__device__ __forceinline__ float scaled(int sum, float w_scale, float x_scale) {
-  return (float)sum * w_scale * x_scale;
+// A sum times the weight's scale, then times the scale of x, which may be as large as x, and the bias or 0. Every kernel gives the
+// same bits: one operation by name, and a float32 before it is rounded to float16 (an instruction that does both rounds but once).
+__device__ __forceinline__ float scaled(int sum, float w_scale, float x_scale, float bias) {
+  float y = fmaf((float)sum * w_scale, x_scale, bias);
+  asm("" : "+v"(y));
+  return y;
 }
 
 template <typename T, int BM, int STAGE>
@@ -308,8 +321,8 @@ __global__ __launch_bounds__(256, BM * STAGE > 8192 ? 1 : 2) void int8_tiles(con
         for (int r0 = 0; r0 < 32; r0 += 64 / SPAN) {
           const int r = r0 + lane / SPAN;
           const int64_t row = m0 + wm * WT + i * 32 + r;
-          const float v = scaled(*(const int*)(region + r * WT * 4 + ((in >> 2) ^ (r & 7)) * 16 + (in & 3) * 4), w, __shfl(xs[i], r));
-          if (row < a.rows && c < a.outputs) T::store(out, row * a.outputs + c, bias != nullptr ? v + b : v);
+          const float v = scaled(*(const int*)(region + r * WT * 4 + ((in >> 2) ^ (r & 7)) * 16 + (in & 3) * 4), w, __shfl(xs[i], r), b);
+          if (row < a.rows && c < a.outputs) T::store(out, row * a.outputs + c, v);
         }
       }
       __builtin_amdgcn_wave_barrier();
@@ -325,10 +338,7 @@ __global__ __launch_bounds__(256, BM * STAGE > 8192 ? 1 : 2) void int8_tiles(con
       for (int half = 0; half < 2; half++) {
         const i32x4 c = *(const i32x4*)(region + r * WT * 4 + ((2 * (lane % LPR) + half) ^ (r & 7)) * 16);
 #pragma unroll
-        for (int e = 0; e < 4; e++) {
-          const float v = scaled(c[e], ws[4 * half + e], s);
-          y[4 * half + e] = bias != nullptr ? v + bs[4 * half + e] : v;
-        }
+        for (int e = 0; e < 4; e++) y[4 * half + e] = scaled(c[e], ws[4 * half + e], s, bs[4 * half + e]);
       }
       if constexpr (sizeof(S) == 2)
         if (!wide) {  // over the row's sums, which all of its lanes have read
@@ -375,8 +385,15 @@ __global__ __launch_bounds__(256, BM * STAGE > 8192 ? 1 : 2) void int8_tiles(con
 #endif
 }
 
-// 16 outputs of up to 16 rows; the width in pairs of 64 bytes, 4 of a wave's in flight while 4 are multiplied.
-template <typename T>
+// Inputs that every workgroup of int8_few brings to 8 bits for itself, in place of a launch before it: up to 8192 bytes for up to 1024
+// workgroups. (By itself and by a launch: 1 x 4096 x 4096 8.9 and 11.8 us, 2 x 4096 x 8192 10.1 and 11.9, 16 x 512 x 2048 9.0 and 12.1; 4 x
+// 4096 x 8192 14.0 and 11.9, 1 x 1024 x 50000 15.9 and 15.1, 4 x 1024 x 50000 19.7 and 16.2.)
+constexpr int OWN_BYTES = 8192, OWN_OUTPUTS = 16384;
+constexpr int OWN_ROW = 16;  // bytes between two rows, to part their banks
+
+// 16 outputs of up to 16 rows; the width in pairs of 64 bytes, 4 of a wave's in flight while 4 are multiplied. OWN: x is not in 8 bits
+// yet (rows of whole aligned eights, rows * padded at most OWN_BYTES).
+template <typename T, bool OWN>
 __global__ __launch_bounds__(256) void int8_few(const signed char* __restrict__ x8, const float* __restrict__ scales, const signed char* __restrict__ w8, int64_t w_stride, Int8Args a) {
 #if defined(__HIP_DEVICE_COMPILE__)  // the host pass needs the stub alone
   constexpr int U = 4, STEP = 4 * U;  // pairs of a wave, and of the workgroup, in a batch
@@ -388,6 +405,8 @@ __global__ __launch_bounds__(256) void int8_few(const signed char* __restrict__ 
   const __amdgpu_buffer_rsrc_t rw = __builtin_amdgcn_make_buffer_rsrc((void*)(w8 + n0 * w_stride), (short)0, (int)(left < 0x7fffffff ? left : 0x7fffffff), 0x00020000);
   const __amdgpu_buffer_rsrc_t rx = __builtin_amdgcn_make_buffer_rsrc((void*)x8, (short)0, (int)(a.rows * padded), 0x00020000);
   const int wv = (int)(n * w_stride) + 16 * g, xv = (int)(n * padded) + 16 * g;
+  __shared__ __attribute__((aligned(16))) signed char own[OWN ? OWN_BYTES + 16 * OWN_ROW : 16];
+  __shared__ float own_scales[16], tops[4];
   i32x4 acc = {0, 0, 0, 0};
   struct Batch {
     i32x4 w[2 * U], x[2 * U];
@@ -399,7 +418,16 @@ __global__ __launch_bounds__(256) void int8_few(const signed char* __restrict__ 
       for (int k = 0; k < 2; k++) {
         const int p = p0 + 4 * u, off = p * 128 + k * 64;  // past the width: zeros, and nothing of the next row is read
         b.w[2 * u + k] = __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(rw, p < pairs ? wv + off : 0x7ffffff0, 0, 0));
-        b.x[2 * u + k] = __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(rx, p < pairs ? xv + off : 0x7ffffff0, 0, 0));
+        if (!OWN) b.x[2 * u + k] = __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(rx, p < pairs ? xv + off : 0x7ffffff0, 0, 0));
+      }
+  };
+  auto from_own = [&](Batch& b, int p0) __attribute__((always_inline)) {
+#pragma unroll
+    for (int u = 0; u < U; u++)
+#pragma unroll
+      for (int k = 0; k < 2; k++) {
+        const int p = p0 + 4 * u;
+        b.x[2 * u + k] = p < pairs && n < a.rows ? *(const i32x4*)(own + n * (padded + OWN_ROW) + p * 128 + k * 64 + 16 * g) : i32x4{0, 0, 0, 0};
       }
   };
   auto multiply = [&](const Batch& b) __attribute__((always_inline)) {
@@ -408,11 +436,51 @@ __global__ __launch_bounds__(256) void int8_few(const signed char* __restrict__ 
   };
   Batch b0, b1;
   load(b0, wave);
+  if constexpr (OWN) {  // as quantize_rows does, by one, two or four waves a row
+    const int share = a.rows == 1 ? 4 : a.rows == 2 ? 2 : 1, at_once = 4 / share, eights = (int)(a.width / 8);
+    for (int r0 = 0; r0 < a.rows; r0 += at_once) {
+      const int r = r0 + wave / share, first = (wave % share) * 64 + lane;
+      const typename T::Storage* row = (const typename T::Storage*)a.x + r * a.width;
+      float top = 0.f, odd = 0.f;
+      if (r < a.rows)
+        for (int i = first; i < eights; i += share * 64) {
+          Eight<T> x;
+          x.load(row + i * 8);
+#pragma unroll
+          for (int e = 0; e < 8; e++) {
+            top = fmaxf(top, fabsf(x.at(e)));
+            odd = fmaf(x.at(e), 0.f, odd);
+          }
+        }
+      if (odd != odd) top = __builtin_inff();
+#pragma unroll
+      for (int m = 1; m < 64; m <<= 1) top = fmaxf(top, __shfl_xor(top, m));
+      if (lane == 0) tops[wave] = top;
+      __syncthreads();
+      for (int w = 0; w < share; w++) top = fmaxf(top, tops[wave / share * share + w]);
+      const Rounding by(top);
+      if (r < a.rows) {
+        if (first == 0) own_scales[r] = by.scale();
+        for (int i = first; i < (int)(padded / 8); i += share * 64) {
+          uint2 y = {0u, 0u};
+          if (i < eights) {
+            Eight<T> x;
+            x.load(row + i * 8);
+            y = by.eight(x);
+          }
+          *(uint2*)(own + r * (padded + OWN_ROW) + i * 8) = y;
+        }
+      }
+      __syncthreads();
+    }
+  }
   for (int p = wave; p < pairs; p += 2 * STEP) {
     if (p + STEP < pairs) load(b1, p + STEP);
+    if (OWN) from_own(b0, p);
     multiply(b0);
     if (p + STEP >= pairs) break;
     if (p + 2 * STEP < pairs) load(b0, p + 2 * STEP);
+    if (OWN) from_own(b1, p + STEP);
     multiply(b1);
   }
   *(i32x4*)&sums[(wave * 16 + n) * 16 + 4 * g] = acc;  // row n, outputs 4 g .. + 3
@@ -423,9 +491,7 @@ __global__ __launch_bounds__(256) void int8_few(const signed char* __restrict__ 
   const int sum = (sums[i] + sums[256 + i]) + (sums[512 + i] + sums[768 + i]);
   const int64_t row = i >> 4, col = n0 + (i & 15);
   if (row >= a.rows || col >= a.outputs) return;
-  float y = scaled(sum, a.w_scales[col], scales[row]);
-  if (bias != nullptr) y += T::load(bias, col);
-  T::store((S*)a.out, row * a.outputs + col, y);
+  T::store((S*)a.out, row * a.outputs + col, scaled(sum, a.w_scales[col], OWN ? own_scales[row] : scales[row], bias != nullptr ? T::load(bias, col) : 0.f));
 #endif
 }
 
@@ -437,9 +503,9 @@ int tiles_of(const Int8Args& a, const signed char* x8, const float* scales, cons
   return check_hip(hipGetLastError(), "launching the 8-bit product");
 }
 
-template <typename T>
+template <typename T, bool OWN>
 int few_of(const Int8Args& a, const signed char* x8, const float* scales, const signed char* w8, int64_t w_stride) {
-  hipLaunchKernelGGL((int8_few<T>), dim3((unsigned)((a.outputs + 15) / 16)), dim3(256), 0, a.stream, x8, scales, w8, w_stride, a);
+  hipLaunchKernelGGL((int8_few<T, OWN>), dim3((unsigned)((a.outputs + 15) / 16)), dim3(256), 0, a.stream, x8, scales, w8, w_stride, a);
   return check_hip(hipGetLastError(), "launching the 8-bit product of few rows");
 }
 
@@ -473,13 +539,14 @@ int linear(const Int8Args& a) {
   const signed char* w8 = (const signed char*)a.w;
   int64_t w_stride = a.width;
   signed char* copy = needs_copy(a.w, a.width) ? (signed char*)scales + align256(a.rows * 4) : nullptr;
+  if (a.rows <= FEW && a.rows * padded <= OWN_BYTES && a.outputs <= OWN_OUTPUTS && copy == nullptr && (uintptr_t)a.x % 16 == 0) return few_of<T, true>(a, x8, scales, w8, w_stride);
   const int rc = quantize(a.dtype, a.x, x8, scales, a.rows, a.width, padded, a.w, copy, a.outputs, a.stream);
   if (rc != LIMN_HIP_OK) return rc;
   if (copy != nullptr) {
     w8 = copy;
     w_stride = padded;
   }
-  if (a.rows <= FEW) return few_of<T>(a, x8, scales, w8, w_stride);
+  if (a.rows <= FEW) return few_of<T, false>(a, x8, scales, w8, w_stride);
   // The largest tiles where they give every CU a workgroup, the middle ones where they do more than half (1024 x 760 x 2288, 144 of
   // them: 16.0 us, 16.9 in the small ones; 512 x 4096 x 4096, 128: 25.5 and 23.2).
   const auto tiles = [&](int64_t m) { return ((a.rows + m - 1) / m) * ((a.outputs + m - 1) / m); };

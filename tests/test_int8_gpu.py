@@ -51,7 +51,7 @@ def check(dev, x, w, scales, bias, dtype, **kw):
 
 
 SIZES = [(1, 1, 1), (1, 64, 64), (3, 24, 17), (1, 760, 1000), (16, 512, 1536), (17, 128, 33), (32, 1000, 300), (33, 257, 65), (64, 4096, 128), (65, 130, 513), (130, 96, 1025), (257, 777, 129),
-         (300, 1536, 512), (1021, 48, 257), (5, 20000, 40), (2100, 300, 2049), (4100, 70, 4099)]
+         (300, 1536, 512), (1021, 48, 257), (5, 20000, 40), (2100, 300, 2049), (4100, 70, 4099), (1, 512, 300), (2, 4096, 64), (3, 1024, 1000), (16, 512, 33), (2, 8192, 40), (1, 8192, 17), (5, 1536, 16385), (7, 48, 2048)]
 
 
 @pytest.mark.parametrize("dtype", TYPES)
@@ -133,3 +133,18 @@ def test_through_the_tensor_api_captured(hipdev):
         y = run(Tensor.from_node(upload(hipdev, x, t)))
         within(y.numpy().reshape(30, 500), *oracle(x.reshape(30, 256), w, s, b, "bfloat16"), "y")
         assert (Tensor(np.ones(1000)) * 3.0).sum().item() == 3000.0
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,width,outputs", [(1, 512, 300), (2, 1024, 77), (3, 320, 64), (7, 1040, 33), (16, 512, 1000)])
+def test_few_rows_have_the_bits_of_many(hipdev, rows, width, outputs, dtype):
+    """Rows alone and among forty, rows of zeros, infinities, NaN, the least and the largest numbers among them."""
+    x, w, s, b = layer(11, dtype, 40, width, outputs, bias=True)
+    t = np.float16 if dtype == "float16" else np.float32
+    for r, value in enumerate([None, 0.0, np.inf, np.nan, None, float(np.finfo(t).max) / 2, float(np.finfo(t).tiny), -np.inf]):
+        if value is not None:
+            x[r, : width if value == 0 else 3] = value
+    many = called(hipdev, x, w, s, b, dtype)
+    for first in (0, 1, 2, 5):
+        got = called(hipdev, x[first : first + rows], w, s, b, dtype)
+        np.testing.assert_array_equal(got, many[first : first + rows])
