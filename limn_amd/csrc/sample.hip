@@ -634,7 +634,7 @@ __global__ __launch_bounds__(TH) void sample_rows(const typename T::Storage* __r
     row.before(w, 0u, m, c);
   }
   total = lists && !few ? given->total : row.sum(total);
-  kept = q > 1.f ? row.whole(row.top) : !(q > 0.f) ? total : lists && !few ? given->kept : row.sum(kept);  // past 1: the first alone
+  kept = q > 1.f ? (uint64_t)1 << a.bits : !(q > 0.f) ? total : lists && !few ? given->kept : row.sum(kept);  // past 1: the first alone
   Border end = {0u, 0xffffffffu, 0x7fffffff, 0}, b;
   bool drawn = false;
   if constexpr (!WHOLE) {
