@@ -17,11 +17,12 @@ from limn_amd.attend import contiguous
 from limn_amd.seam import FLOATS, Tensor, active_device, custom, float32, float64, int32
 
 SAMPLE = "sample"
+MOST_TOKENS = 1 << 24
 
 
 def sample(logits: Tensor, uniforms: Tensor, *, temperature: float | Tensor = 1.0, top_k: int | Tensor = 0, top_p: float | Tensor = 1.0,
            min_p: float | Tensor = 0.0) -> tuple[Tensor, Tensor]:
-    """Tokens (...) int32 drawn from logits (..., vocab) by uniforms (...) float32 in [0, 1), and the logarithms (...) float32
+    """Tokens (...) int32 drawn from logits (..., vocab), vocab up to 2^24, by uniforms (...) float32 in [0, 1), and the logarithms (...) float32
     of their shares of the kept mass.
 
     The settings are numbers, or tensors (...) with one for each row (float32, top_k int32):
@@ -34,6 +35,8 @@ def sample(logits: Tensor, uniforms: Tensor, *, temperature: float | Tensor = 1.
     """
     if logits.ndim < 1 or logits.dtype not in FLOATS:
         raise ValueError(f"sample needs float logits (..., vocab), got {logits.shape} {logits.dtype}")
+    if logits.shape[-1] > MOST_TOKENS:
+        raise ValueError(f"sample: a vocabulary of at most {MOST_TOKENS}, not {logits.shape[-1]}")
     rows = logits.shape[:-1]
     if uniforms.shape != rows or uniforms.dtype != float32:
         raise ValueError(f"sample: uniforms must be {rows} float32, got {uniforms.shape} {uniforms.dtype}")

@@ -79,7 +79,8 @@ class Cache:
 
 def prefill(model: GPT, cache: Cache, sequences: Sequence[int], prompts: Sequence[Sequence[int]], table: Tensor, part: int = 4096) -> Tensor:
     """The prompts through the model, their keys and values into the cache: the logits (sequences, vocab) behind each one's last token.
-    Parts hold at most `part` tokens and end anywhere; each sequence goes on in the next one where it ended."""
+    Parts hold at most `part` tokens and end anywhere; each sequence goes on in the next one where it ended. For answering: under
+    `no_grad`, with pages reserved for the prompts."""
     todo, done = [list(p) for p in prompts], [0] * len(prompts)
     logits: Tensor | None = None
     while any(at < len(p) for at, p in zip(done, todo)):

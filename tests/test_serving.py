@@ -274,3 +274,9 @@ def test_paged_queries_keys_and_values_in_one():
             attend_paged(Tensor(bad), None, None, *one, *where(), heads=heads)
     with pytest.raises(ValueError, match="beside"):
         attend_paged(Tensor(qkv), on("k"), on("v"), *one, *where(), heads=4)
+
+
+def test_a_vocabulary_past_the_kernels_is_refused():
+    logits = Tensor(np.zeros(1), dtype=float32).expand((1 << 24) + 1)
+    with pytest.raises(ValueError, match="vocabulary"):
+        sample(logits, Tensor(np.float32(0.5), dtype=float32))
