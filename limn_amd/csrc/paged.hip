@@ -2,6 +2,7 @@
 // values into their pages; and the kernel that serves every type, head dim and alignment.
 
 #include "paged_fast.h"
+#include "paged_reads.h"
 
 #include <math.h>
 
@@ -203,7 +204,7 @@ int join_of(const PagedArgs& a, const PagedFast& f) {
 
 // Sizes that the tiled kernels serve: rows of whole 16-byte chunks; places counted in 32 bits.
 bool fast_sizes(const PagedArgs& a) {
-  return a.hd <= 128 && a.hd % (a.dtype == LIMN_HIP_FLOAT32 ? 4 : 8) == 0 && a.pages < (int64_t)0xffffffff / a.kv_heads / a.page;
+  return paged_dim(a.hd, a.dtype == LIMN_HIP_FLOAT32 ? 4 : 2) && a.pages < (int64_t)0xffffffff / a.kv_heads / a.page;
 }
 // A call of such sizes goes to them where every buffer and row is 16-byte aligned, and its constants stay normal numbers.
 bool fast_call(const PagedArgs& a) {

@@ -6,7 +6,7 @@
 //    and values are read once for all of them;
 //  - a wave takes 32 keys at a time and reads them from memory straight into matrix operands, no LDS and no barrier in the
 //    loop. K: lane (n = lane % 16, g = lane / 16) reads 16 bytes of keys n and 16 + n at a time; V: W = D / 16 dims from W n
-//    on of keys 4 g + j and 16 + 4 g + j. S^T = K Q^T leaves exactly those keys' weights in the lane, so they are the second
+//    on (value_dim) of keys 4 g + j and 16 + 4 g + j. S^T = K Q^T leaves exactly those keys' weights in the lane, so they are the second
 //    product's operand as they stand. Half widths multiply by v_mfma_f32_16x16x32, float32 by v_mfma_f32_16x16x4_f32;
 //  - a lane looks up the place of one key of 32 in the table, a tile ahead, and gets the places of the keys it reads from
 //    the other lanes: pages of any size cost the same;
@@ -18,6 +18,7 @@
 // with keys that some rows do not see are looked over (see give_back).
 
 #include "paged_fast.h"
+#include "paged_reads.h"
 
 namespace limn {
 namespace {
@@ -187,7 +188,7 @@ __global__ __launch_bounds__(64 * waves, blocks) void paged_token(PagedFast a, P
   };
   auto load_v = [&](int kt, unsigned rows_) __attribute__((always_inline)) {
     const bool old = kt < old_tiles;
-    const uint64_t base = (uint64_t)(old ? pool_v : fresh_v + (q.row0 + begin_of(kt) - q.off) * v.v_row) + sizeof(typename O::Values) * n;
+    const uint64_t base = (uint64_t)(old ? pool_v : fresh_v + (q.row0 + begin_of(kt) - q.off) * v.v_row) + sizeof(S) * value_dim(n, W, v.hd);
     const unsigned stride = (unsigned)(old ? v.hd : v.v_row) * (unsigned)sizeof(S);
 #pragma unroll
     for (int j = 0; j < 8; j++) {
@@ -309,13 +310,13 @@ __global__ __launch_bounds__(64 * waves, blocks) void paged_token(PagedFast a, P
     for (int e = 0; e < W; e++) {
       __syncthreads();
 #pragma unroll
-      for (int i = 0; i < 4; i++) lds[(wave * 16 + 4 * g + i) * 17 + n] = acc[t][e][i] * factor;  // dim W (4 g + i) + e
+      for (int i = 0; i < 4; i++) lds[(wave * 16 + 4 * g + i) * 17 + n] = acc[t][e][i] * factor;  // the e-th dim of lane 4 g + i
       __syncthreads();
       if (wave < 4) {  // 16 dims x 16 rows: wave w takes dims 4 w + g of row n
-        const int dd = 4 * wave + g, d = W * dd + e;
+        const int dd = 4 * wave + g, d = value_dim(dd, W, v.hd) + e;
         float x = 0.f;
         for (int w = 0; w < waves; w++) x += lds[(w * 16 + dd) * 17 + n];
-        if (there[t] && d < v.hd) {
+        if (there[t] && W * dd < v.hd && d >= W * dd) {  // (a dim of the lane before is that one's to store)
           if (!alone)
             a.totals[(part * rows_all + at[t]) * v.hd + d] = x;
           else
@@ -355,7 +356,7 @@ int launch_token(const PagedArgs& a, const PagedFast& f, bool lone) {
 
 template <typename T>
 int launch_token_type(const PagedArgs& a, const PagedFast& f, bool lone) {
-  if (a.hd <= 64) return f.rows == 16 ? launch_token<T, 64, 1>(a, f, lone) : launch_token<T, 64, 2>(a, f, lone);
+  if (token_width(a.hd) == 64) return f.rows == 16 ? launch_token<T, 64, 1>(a, f, lone) : launch_token<T, 64, 2>(a, f, lone);
   return f.rows == 16 ? launch_token<T, 128, 1>(a, f, lone) : launch_token<T, 128, 2>(a, f, lone);
 }
 
