@@ -289,7 +289,8 @@ int64_t limn_hip_xent_workspace(int dtype, int64_t rows, int64_t width, int64_t 
  * a key that a query does not see holds, infinities and NaN among them, changes nothing in its row; an infinite value that it
  * sees gives an infinity, or NaN where its weight is below float32's least number (float16's, 2^-31). Pages that this
  * call writes to belong to one sequence; others may be shared. q, k, v and out do not overlap the pages.
- * hd at most 256; scale between -2^120 and 2^120; softcap 0 for none, else from 2^-120 to 2^120.
+ * hd at most 256; scale between -2^120 and 2^120; softcap 0 for none, else from 2^-120 to 2^120. A call whose
+ * launches would have 2^32 threads is refused before anything is written.
  * `workspace` must hold limn_hip_attend_paged_workspace(...) bytes, 16-byte aligned, for this call alone, as for
  * limn_hip_attend_fwd. Results are deterministic; sums and statistics are float32. Half widths multiply on 16-bit matrix cores
  * where hd is a multiple of 8 up to 128 and every buffer and row 16-byte aligned: the weights are rounded to the half width
@@ -314,7 +315,7 @@ int64_t limn_hip_attend_paged_workspace(int dtype, int64_t tokens, int64_t seque
  * A temperature of 0 or below, or NaN, takes the first of the order with a logprob of 0. top_k outside [1, vocab), top_p of 1
  * or more or NaN, and min_p of 0 or below or NaN keep everything. A u outside [0, 1) is taken as the nearest end (NaN: the
  * last one kept). NaN among the logits counts as minus infinity; a row without anything above that gives -1 and minus
- * infinity; an infinite logit has all of the mass. vocab up to 2^24.
+ * infinity; an infinite logit has all of the mass. vocab up to 2^24, fewer than 2^22 rows (2^24 of up to 256 logits).
  * Weights and masses are computed in 64 bits; results are deterministic. Workspace as above, of limn_hip_sample_workspace(...)
  * bytes. No counterpart in the reference (its training example draws from a softmax on the host, examples/train_stories.py).
  */
@@ -327,7 +328,7 @@ int64_t limn_hip_sample_workspace(int dtype, int64_t rows, int64_t vocab);
 /*
  * Rows x (rows, width) of float32, float16 or bfloat16 brought to 8 bits: scales[r] = max(max |x[r]| / 127, 2^-126) and
  * values[r][i] = round(x[r][i] / scales[r]), ties to even, in float32 arithmetic. A row with an infinity or a NaN gets the scale NaN
- * and zeros. No counterpart in the reference.
+ * and zeros. Fewer than 2^24 rows. No counterpart in the reference.
  */
 int limn_hip_quantize_rows(const void* x, void* values, void* scales, int dtype, int64_t rows, int64_t width, void* stream);
 

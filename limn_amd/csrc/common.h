@@ -105,4 +105,7 @@ namespace limn {
 void set_error(const char* fmt, ...);
 int fail(int code, const char* fmt, ...);
 int check_hip(hipError_t err, const char* doing);
+
+// Whether HIP takes a launch of so many workgroups: it counts their threads in 32 bits.
+inline bool one_launch(int64_t workgroups, int64_t threads) { return workgroups <= (int64_t)0xffffffff / threads; }
 }  // namespace limn

@@ -495,11 +495,11 @@ __global__ __launch_bounds__(256) void int8_few(const signed char* __restrict__ 
 #endif
 }
 
+int64_t tiles(const Int8Args& a, int64_t m) { return ((a.rows + m - 1) / m) * ((a.outputs + m - 1) / m); }
+
 template <typename T, int BM, int STAGE>
 int tiles_of(const Int8Args& a, const signed char* x8, const float* scales, const signed char* w8, int64_t w_stride) {
-  const int64_t blocks = ((a.rows + BM - 1) / BM) * ((a.outputs + BM - 1) / BM);
-  if (blocks > 0x7fffffff) return fail(LIMN_HIP_EUNSUPPORTED, "int8_linear: %lld workgroups exceed one launch", (long long)blocks);
-  hipLaunchKernelGGL((int8_tiles<T, BM, STAGE>), dim3((unsigned)blocks), dim3(256), 0, a.stream, x8, scales, w8, w_stride, a);
+  hipLaunchKernelGGL((int8_tiles<T, BM, STAGE>), dim3((unsigned)tiles(a, BM)), dim3(256), 0, a.stream, x8, scales, w8, w_stride, a);
   return check_hip(hipGetLastError(), "launching the 8-bit product");
 }
 
@@ -515,7 +515,7 @@ int quantize_of(const void* x, void* values, float* scales, int64_t rows, int64_
   typedef typename T::Storage S;
   const int vec = width % 8 == 0 && (uintptr_t)x % 16 == 0 && (uintptr_t)values % 8 == 0 && stride % 8 == 0;
   const int64_t copies = w_out == nullptr ? 0 : outputs < 1024 ? outputs : 1024;
-  if (rows + copies > 0x7fffffff) return fail(LIMN_HIP_EUNSUPPORTED, "quantize_rows: %lld rows exceed one launch", (long long)rows);
+  if (!one_launch(rows + copies, 256)) return fail(LIMN_HIP_EUNSUPPORTED, "quantize_rows: %lld rows are out of range, they exceed one launch", (long long)rows);
   hipLaunchKernelGGL((quantize_rows<T>), dim3((unsigned)(rows + copies)), dim3(256), 0, stream, (const S*)x, (signed char*)values, scales, rows, width, stride, vec,
                      (const signed char*)w, (signed char*)w_out, outputs);
   return check_hip(hipGetLastError(), "launching the rounding of rows to 8 bits");
@@ -540,6 +540,11 @@ int linear(const Int8Args& a) {
   int64_t w_stride = a.width;
   signed char* copy = needs_copy(a.w, a.width) ? (signed char*)scales + align256(a.rows * 4) : nullptr;
   if (a.rows <= FEW && a.rows * padded <= OWN_BYTES && a.outputs <= OWN_OUTPUTS && copy == nullptr && (uintptr_t)a.x % 16 == 0) return few_of<T, true>(a, x8, scales, w8, w_stride);
+  // The largest tiles where they give every CU a workgroup, the middle ones where they do more than half (1024 x 760 x 2288, 144 of
+  // them: 16.0 us, 16.9 in the small ones; 512 x 4096 x 4096, 128: 25.5 and 23.2).
+  const int m = tiles(a, 256) >= 256 ? 256 : tiles(a, 128) > 128 ? 128 : 64;
+  const int64_t blocks = a.rows <= FEW ? (a.outputs + 15) / 16 : tiles(a, m);
+  if (!one_launch(blocks, 256)) return fail(LIMN_HIP_EUNSUPPORTED, "int8_linear: sizes out of range, %lld workgroups exceed one launch", (long long)blocks);
   const int rc = quantize(a.dtype, a.x, x8, scales, a.rows, a.width, padded, a.w, copy, a.outputs, a.stream);
   if (rc != LIMN_HIP_OK) return rc;
   if (copy != nullptr) {
@@ -547,11 +552,8 @@ int linear(const Int8Args& a) {
     w_stride = padded;
   }
   if (a.rows <= FEW) return few_of<T, false>(a, x8, scales, w8, w_stride);
-  // The largest tiles where they give every CU a workgroup, the middle ones where they do more than half (1024 x 760 x 2288, 144 of
-  // them: 16.0 us, 16.9 in the small ones; 512 x 4096 x 4096, 128: 25.5 and 23.2).
-  const auto tiles = [&](int64_t m) { return ((a.rows + m - 1) / m) * ((a.outputs + m - 1) / m); };
-  if (tiles(256) >= 256) return tiles_of<T, 256, 64>(a, x8, scales, w8, w_stride);
-  if (tiles(128) > 128) return tiles_of<T, 128, 128>(a, x8, scales, w8, w_stride);
+  if (m == 256) return tiles_of<T, 256, 64>(a, x8, scales, w8, w_stride);
+  if (m == 128) return tiles_of<T, 128, 128>(a, x8, scales, w8, w_stride);
   return tiles_of<T, 64, 128>(a, x8, scales, w8, w_stride);
 }
 
@@ -577,7 +579,7 @@ extern "C" int limn_hip_quantize_rows(const void* x, void* values, void* scales,
   if (x == nullptr || values == nullptr || scales == nullptr) return fail(LIMN_HIP_EINVAL, "%s: null buffer", name);
   if ((uintptr_t)x % (dtype == LIMN_HIP_FLOAT32 ? 4 : 2) != 0 || (uintptr_t)scales % 4 != 0)
     return fail(LIMN_HIP_EINVAL, "%s: buffers must be aligned to their element size", name);
-  if (rows > 0x7fffffff || width > ((int64_t)1 << 40) / rows) return fail(LIMN_HIP_EUNSUPPORTED, "%s: sizes out of range", name);
+  if (!one_launch(rows, 256) || width > ((int64_t)1 << 40) / rows) return fail(LIMN_HIP_EUNSUPPORTED, "%s: sizes out of range", name);
   return quantize(dtype, x, values, (float*)scales, rows, width, width, nullptr, nullptr, 0, (hipStream_t)stream);
 }
 

@@ -93,11 +93,13 @@ __global__ __launch_bounds__(256) void paged_rows(PagedView v, const typename T:
     if (c * 64 + lane < v.hd) T::store(out, ((int64_t)row * v.heads + head) * v.hd + c * 64 + lane, acc[c] * inv);
 }
 
+// a wave a token and head, in fours
+int64_t row_blocks(const PagedArgs& a) { return (a.tokens * a.heads + 3) / 4; }
+
 template <typename T>
 int rows_of(const PagedArgs& a) {
   typedef typename T::Storage S;
-  const int64_t blocks = (a.tokens * a.heads + 3) / 4;
-  hipLaunchKernelGGL((paged_rows<T>), dim3((unsigned)blocks), dim3(256), 0, a.stream, paged_view(a), (const S*)a.q, (const S*)a.key_pages,
+  hipLaunchKernelGGL((paged_rows<T>), dim3((unsigned)row_blocks(a)), dim3(256), 0, a.stream, paged_view(a), (const S*)a.q, (const S*)a.key_pages,
                      (const S*)a.value_pages, (S*)a.out);
   return check_hip(hipGetLastError(), "launching attention over a paged cache");
 }
@@ -198,7 +200,7 @@ int check_buffers(const PagedArgs& a) {
 
 template <typename T>
 int join_of(const PagedArgs& a, const PagedFast& f) {
-  hipLaunchKernelGGL((paged_join<T>), dim3((unsigned)((a.tokens * a.heads + 3) / 4)), dim3(256), 0, a.stream, f, paged_view(a));
+  hipLaunchKernelGGL((paged_join<T>), dim3((unsigned)row_blocks(a)), dim3(256), 0, a.stream, f, paged_view(a));
   return check_hip(hipGetLastError(), "joining the parts of attention over a paged cache");
 }
 
@@ -307,6 +309,8 @@ extern "C" int limn_hip_attend_paged(const void* q, const void* k, const void* v
   if (need > 0 && (workspace == nullptr || (uintptr_t)workspace % 16 != 0 || workspace_bytes < need))
     return fail(LIMN_HIP_EINVAL, "attend_paged: needs a workspace of %lld bytes, 16-byte aligned", (long long)need);
   if (fast_call(a)) return launch_fast(a);
+  const int64_t blocks = row_blocks(a) > tokens ? row_blocks(a) : tokens;  // before anything is written
+  if (!one_launch(blocks, 256)) return fail(LIMN_HIP_EUNSUPPORTED, "attend_paged: sizes out of range, %lld workgroups exceed one launch", (long long)blocks);
   rc = dtype == LIMN_HIP_FLOAT32 ? write_of<float>(a) : write_of<u16>(a);
   if (rc != LIMN_HIP_OK) return rc;
   return dtype == LIMN_HIP_FLOAT32 ? rows_of<F32>(a) : dtype == LIMN_HIP_FLOAT16 ? rows_of<F16>(a) : rows_of<BF16>(a);

@@ -330,7 +330,7 @@ __global__ __launch_bounds__(THREADS, 2) void paged_tiles(PagedFast a, PagedView
 template <typename T, int D, Cap CAP, bool BIAS>
 int launch_tiles_as(const PagedArgs& a, const PagedFast& f) {
   const int64_t slots = paged_slots(a, ATT_ROWS), blocks = slots * a.kv_heads * f.parts;
-  if (blocks > 0x7fffffff) return fail(LIMN_HIP_EUNSUPPORTED, "attend_paged: %lld workgroups exceed one launch", (long long)blocks);
+  if (!one_launch(blocks, THREADS)) return fail(LIMN_HIP_EUNSUPPORTED, "attend_paged: sizes out of range, %lld workgroups exceed one launch", (long long)blocks);
   hipLaunchKernelGGL((paged_tiles<T, D, CAP, BIAS>), dim3((unsigned)blocks), dim3(THREADS), 0, a.stream, f, paged_view(a), (int)slots);
   return check_hip(hipGetLastError(), "launching attention over a paged cache");
 }

@@ -345,8 +345,8 @@ template <typename T, int D, int NR>
 int launch_token(const PagedArgs& a, const PagedFast& f, bool lone) {
   const PagedView v = paged_view(a);
   const int64_t blocks = paged_slots(a, 16 * NR) * a.kv_heads * f.parts;
-  if (blocks > 0x7fffffff) return fail(LIMN_HIP_EUNSUPPORTED, "attend_paged: %lld workgroups exceed one launch", (long long)blocks);
   constexpr int LONE = LONE_WAVES<T, D, NR>;
+  if (!one_launch(blocks, lone ? 64 * LONE : 256)) return fail(LIMN_HIP_EUNSUPPORTED, "attend_paged: sizes out of range, %lld workgroups exceed one launch", (long long)blocks);
   if (lone)
     hipLaunchKernelGGL((paged_token<T, D, NR, LONE, 1>), dim3((unsigned)blocks), dim3(64 * LONE), 0, a.stream, f, v);
   else

@@ -822,6 +822,9 @@ int parts_of(int64_t rows, int64_t vocab) {
   return n < 7 ? 1 : (int)n;
 }
 
+// of a row's workgroup
+int threads_of(int64_t vocab) { return vocab <= 256 ? 256 : 1024; }
+
 template <typename T>
 int sample_of(const void* logits, const SampleArgs& a, SplitRow* split, hipStream_t stream) {
   typedef typename T::Storage S;
@@ -835,7 +838,7 @@ int sample_of(const void* logits, const SampleArgs& a, SplitRow* split, hipStrea
     hipLaunchKernelGGL((sample_rows<T, 1024, false, true>), grid, block, 0, stream, (const S*)logits, a, (const SplitRow*)split, parts);
     return check_hip(hipGetLastError(), "launching sampling");
   }
-  if (a.vocab <= 256)
+  if (threads_of(a.vocab) == 256)
     hipLaunchKernelGGL((sample_rows<T, 256, true, false>), grid, dim3(256), 0, stream, (const S*)logits, a, nullptr, 1);
   else if (a.vocab <= 1024)
     hipLaunchKernelGGL((sample_rows<T, 1024, true, false>), grid, dim3(1024), 0, stream, (const S*)logits, a, nullptr, 1);
@@ -865,7 +868,7 @@ extern "C" int limn_hip_sample(const void* logits, const void* uniforms, const v
   const uintptr_t words = (uintptr_t)uniforms | (uintptr_t)temperature | (uintptr_t)top_k | (uintptr_t)top_p | (uintptr_t)min_p | (uintptr_t)tokens | (uintptr_t)logprobs;
   if ((uintptr_t)logits % size != 0 || words % 4 != 0) return fail(LIMN_HIP_EINVAL, "sample: buffers must be aligned to their element size");
   if (workspace_bytes < 0) return fail(LIMN_HIP_EINVAL, "sample: negative workspace size");
-  if (rows > 0x7fffffff || vocab > (1 << 24)) return fail(LIMN_HIP_EUNSUPPORTED, "sample: sizes out of range");
+  if (vocab > (1 << 24) || !one_launch(rows, threads_of(vocab))) return fail(LIMN_HIP_EUNSUPPORTED, "sample: sizes out of range");
   const int64_t need = limn_hip_sample_workspace(dtype, rows, vocab);
   if (need > 0 && (workspace == nullptr || (uintptr_t)workspace % 16 != 0 || workspace_bytes < need))
     return fail(LIMN_HIP_EINVAL, "sample: needs a workspace of %lld bytes, 16-byte aligned", (long long)need);
