@@ -99,8 +99,8 @@ class Program:
     @functools.cached_property
     def launches(self) -> int:
         """Kernel launches of the list, as they count for the choice between a graph and its steps: a contraction
-        given a workspace may fold k slices, one of half widths copy its operands as well; LAUNCHES has the other
-        kinds of several. It is an estimate for those: a cross entropy's for one piece of the vocabulary, attention's
+        given a workspace may fold k slices, one of half widths copy its operands as well; sampling given one splits its
+        rows, in four launches; LAUNCHES has the other kinds of several. It is an estimate for those: a cross entropy's for one piece of the vocabulary, attention's
         without documents (one more a pass) and parts (one more in the backward), so that one attention and its
         gradients go launch by launch, which is faster with documents too (8 x 12 heads x 1021 x 80, a prefix: 230 us
         against 241 as a graph; 2 x 4 x 256 x 64 float32, documents and every other rule: 133 against 147)."""
@@ -111,6 +111,8 @@ class Program:
                 total += 1 + (value(19 if kind == STEP_MATMUL else 26) > 0)
             elif kind == STEP_CONTRACT:
                 total += 1 + (value(26) > 0) * (1 if value(3) == 1 else 2)
+            elif kind == STEP_SAMPLE:
+                total += 4 if value(13) > 0 else 1
             else:
                 total += LAUNCHES.get(kind, 1)
         return total

@@ -200,3 +200,18 @@ def test_launches_count_what_a_step_issues():
         dev, plan = replaying(lib)
         dev._replay(plan, prog, {0: dev._alloc(16)})
         assert (lib.graph_calls, lib.list_calls) == ((1, 0) if 4 * n > replay.SHORT_LIST else (0, 1))
+
+
+def test_a_sample_of_split_rows_counts_its_four_launches():
+    """Rows are split exactly where the call has a workspace; two such steps are no short list."""
+    def sampled(room):
+        return replay.Launch(replay.STEP_SAMPLE, (0x1000,) * 8 + (1, 6, 40001, 40001, 0x2000 if room else 0, room))
+
+    for room, each in ((0, 1), (4096, 4)):
+        for n in (1, 2, 7, 8):
+            steps, args = replay.bind([sampled(room)] * n, [])
+            lib, prog = StubLib(graph_status=0), replay.Program(steps, args, (), (), (), 1)
+            assert prog.launches == each * n
+            dev, plan = replaying(lib)
+            dev._replay(plan, prog, {0: dev._alloc(16)})
+            assert (lib.graph_calls, lib.list_calls) == ((1, 0) if each * n > replay.SHORT_LIST else (0, 1))
