@@ -338,7 +338,9 @@ int limn_hip_quantize_rows(const void* x, void* values, void* scales, int dtype,
  * with weight (outputs, width) int8, weight_scales (outputs) float32, bias (outputs) of x's type or NULL, out (rows, outputs) of x's
  * type. The sums are exact; their products with the scales and the sum with the bias are float32, rounded once to out's type: a row's
  * bits do not depend on the rows beside it.
- * width up to 2^17. Workspace as above, of limn_hip_int8_linear_workspace(...) bytes. No counterpart in the reference.
+ * width up to 2^17. Workspace as above, of limn_hip_int8_linear_workspace(...) bytes: the rows in 8 bits, and of a weight of some 64 MB
+ * at most the room for a copy whose rows are aligned, used where it does not begin at 16 bytes; for widths that are no multiple of 16 the
+ * whole copy, made in every call. No counterpart in the reference.
  */
 int limn_hip_int8_linear(const void* x, const void* weight, const void* weight_scales, const void* bias, void* out, int dtype,
                          int64_t rows, int64_t width, int64_t outputs, void* workspace, int64_t workspace_bytes, void* stream);

@@ -21,6 +21,7 @@
 
 #include <math.h>
 
+#include <algorithm>
 #include <type_traits>
 
 namespace limn {
@@ -42,7 +43,7 @@ struct Int8Args {
   const void* bias;  // of x's type, or nullptr
   void* out;
   int dtype;
-  int64_t rows, width, outputs;
+  int64_t rows, width, outputs, out_row;  // out_row: outputs between rows of out, more than `outputs` where a call goes in slabs
   void* workspace;
   hipStream_t stream;
   int64_t padded() const { return (width + PAD - 1) / PAD * PAD; }
@@ -52,6 +53,15 @@ constexpr int64_t align256(int64_t bytes) { return (bytes + 255) / 256 * 256; }
 
 // The copy of the weight with aligned rows that a call needs where its rows are not.
 bool needs_copy(const void* w, int64_t width) { return width % 16 != 0 || (uintptr_t)w % 16 != 0; }
+
+// Outputs that there is room to copy at a time. Of a width whose rows may be aligned a whole weight may not be spared for a start that
+// is not: such a call goes in slabs of some 64 MB, whole tiles each (300 x 4096 x 50000, four of them: 259 us, 240 in one; slabs of 16 MB
+// 331).
+int64_t copied_outputs(int64_t width, int64_t outputs) {
+  if (width % 16 != 0) return outputs;
+  const int64_t padded = (width + PAD - 1) / PAD * PAD, slab = std::max<int64_t>(((int64_t)1 << 26) / padded / 256, 1) * 256;
+  return std::min(outputs, slab);
+}
 
 // 8 consecutive elements
 template <typename T>
@@ -292,7 +302,7 @@ __global__ __launch_bounds__(256, BM * STAGE > 8192 ? 1 : 2) void int8_tiles(con
   S* out = (S*)a.out;
   const S* bias = (const S*)a.bias;
   const int64_t col = n0 + wn * WT + (lane % LPR) * 8;
-  const bool wide = a.outputs % 8 == 0 && ((uintptr_t)out & 15) == 0;
+  const bool wide = a.out_row % 8 == 0 && ((uintptr_t)out & 15) == 0;
   float ws[8], bs[8];
 #pragma unroll
   for (int e = 0; e < 8; e++) {
@@ -322,7 +332,7 @@ __global__ __launch_bounds__(256, BM * STAGE > 8192 ? 1 : 2) void int8_tiles(con
           const int r = r0 + lane / SPAN;
           const int64_t row = m0 + wm * WT + i * 32 + r;
           const float v = scaled(*(const int*)(region + r * WT * 4 + ((in >> 2) ^ (r & 7)) * 16 + (in & 3) * 4), w, __shfl(xs[i], r), b);
-          if (row < a.rows && c < a.outputs) T::store(out, row * a.outputs + c, v);
+          if (row < a.rows && c < a.outputs) T::store(out, row * a.out_row + c, v);
         }
       }
       __builtin_amdgcn_wave_barrier();
@@ -346,7 +356,7 @@ __global__ __launch_bounds__(256, BM * STAGE > 8192 ? 1 : 2) void int8_tiles(con
           continue;
         }
       if (row >= a.rows || col >= a.outputs) continue;
-      S* o = out + row * a.outputs + col;
+      S* o = out + row * a.out_row + col;
       if constexpr (std::is_same<T, F32>::value) {
         *(f32x4*)o = f32x4{y[0], y[1], y[2], y[3]};
         *(f32x4*)(o + 4) = f32x4{y[4], y[5], y[6], y[7]};
@@ -365,7 +375,7 @@ __global__ __launch_bounds__(256, BM * STAGE > 8192 ? 1 : 2) void int8_tiles(con
           const int64_t row = m0 + wm * WT + i * 32 + r;
           const char* const from = region + r * WT * 4;
           auto word = [&](int w) __attribute__((always_inline)) { return *(const unsigned*)(from + (((w >> 2) & (LPR - 1)) ^ (r % LPR)) * 16 + (w & 3) * 4); };
-          S* o = out + row * a.outputs + c0;
+          S* o = out + row * a.out_row + c0;
           const int before = (int)((16 - ((uintptr_t)o & 15)) & 15) / 2, at = before + 8 * j;  // the outputs before the first boundary
           unsigned w[5];
 #pragma unroll
@@ -491,7 +501,7 @@ __global__ __launch_bounds__(256) void int8_few(const signed char* __restrict__ 
   const int sum = (sums[i] + sums[256 + i]) + (sums[512 + i] + sums[768 + i]);
   const int64_t row = i >> 4, col = n0 + (i & 15);
   if (row >= a.rows || col >= a.outputs) return;
-  T::store((S*)a.out, row * a.outputs + col, scaled(sum, a.w_scales[col], OWN ? own_scales[row] : scales[row], bias != nullptr ? T::load(bias, col) : 0.f));
+  T::store((S*)a.out, row * a.out_row + col, scaled(sum, a.w_scales[col], OWN ? own_scales[row] : scales[row], bias != nullptr ? T::load(bias, col) : 0.f));
 #endif
 }
 
@@ -531,30 +541,47 @@ int quantize(int dtype, const void* x, void* values, float* scales, int64_t rows
 // and 14.3 us; 16 x 4096 x 2048 11.2 and 13.4; 32 x 4096 x 8192, two operands a wave, 17.3 and 14.9.)
 constexpr int64_t FEW = 16;
 
+// The largest tiles where they give every CU a workgroup, the middle ones where they do more than half (1024 x 760 x 2288, 144 of
+// them: 16.0 us, 16.9 in the small ones; 512 x 4096 x 4096, 128: 25.5 and 23.2).
+int tile_of(const Int8Args& a) { return tiles(a, 256) >= 256 ? 256 : tiles(a, 128) > 128 ? 128 : 64; }
+
 template <typename T>
-int linear(const Int8Args& a) {
-  const int64_t padded = a.padded();
-  signed char* x8 = (signed char*)a.workspace;
-  float* scales = (float*)(x8 + align256(a.rows * padded));
-  const signed char* w8 = (const signed char*)a.w;
-  int64_t w_stride = a.width;
-  signed char* copy = needs_copy(a.w, a.width) ? (signed char*)scales + align256(a.rows * 4) : nullptr;
-  if (a.rows <= FEW && a.rows * padded <= OWN_BYTES && a.outputs <= OWN_OUTPUTS && copy == nullptr && (uintptr_t)a.x % 16 == 0) return few_of<T, true>(a, x8, scales, w8, w_stride);
-  // The largest tiles where they give every CU a workgroup, the middle ones where they do more than half (1024 x 760 x 2288, 144 of
-  // them: 16.0 us, 16.9 in the small ones; 512 x 4096 x 4096, 128: 25.5 and 23.2).
-  const int m = tiles(a, 256) >= 256 ? 256 : tiles(a, 128) > 128 ? 128 : 64;
-  const int64_t blocks = a.rows <= FEW ? (a.outputs + 15) / 16 : tiles(a, m);
-  if (!one_launch(blocks, 256)) return fail(LIMN_HIP_EUNSUPPORTED, "int8_linear: sizes out of range, %lld workgroups exceed one launch", (long long)blocks);
-  const int rc = quantize(a.dtype, a.x, x8, scales, a.rows, a.width, padded, a.w, copy, a.outputs, a.stream);
-  if (rc != LIMN_HIP_OK) return rc;
-  if (copy != nullptr) {
-    w8 = copy;
-    w_stride = padded;
-  }
+int product(const Int8Args& a, const signed char* x8, const float* scales, const signed char* w8, int64_t w_stride) {
   if (a.rows <= FEW) return few_of<T, false>(a, x8, scales, w8, w_stride);
+  const int m = tile_of(a);
   if (m == 256) return tiles_of<T, 256, 64>(a, x8, scales, w8, w_stride);
   if (m == 128) return tiles_of<T, 128, 128>(a, x8, scales, w8, w_stride);
   return tiles_of<T, 64, 128>(a, x8, scales, w8, w_stride);
+}
+
+template <typename T>
+int linear(const Int8Args& a) {
+  typedef typename T::Storage S;
+  const int64_t padded = a.padded();
+  signed char* x8 = (signed char*)a.workspace;
+  float* scales = (float*)(x8 + align256(a.rows * padded));
+  const signed char* w = (const signed char*)a.w;
+  const bool copied = needs_copy(w, a.width);
+  if (a.rows <= FEW && a.rows * padded <= OWN_BYTES && a.outputs <= OWN_OUTPUTS && !copied && (uintptr_t)a.x % 16 == 0) return few_of<T, true>(a, x8, scales, w, a.width);
+  const int64_t blocks = a.rows <= FEW ? (a.outputs + 15) / 16 : tiles(a, tile_of(a));
+  if (!one_launch(blocks, 256)) return fail(LIMN_HIP_EUNSUPPORTED, "int8_linear: sizes out of range, %lld workgroups exceed one launch", (long long)blocks);
+  if (!copied) {
+    const int rc = quantize(a.dtype, a.x, x8, scales, a.rows, a.width, padded, nullptr, nullptr, 0, a.stream);
+    return rc != LIMN_HIP_OK ? rc : product<T>(a, x8, scales, w, a.width);
+  }
+  signed char* const copy = (signed char*)scales + align256(a.rows * 4);
+  const int64_t most = copied_outputs(a.width, a.outputs);
+  for (int64_t n = 0; n < a.outputs; n += most) {  // the rows' rounding with the first slab's copy
+    Int8Args slab = a;
+    slab.outputs = std::min(most, a.outputs - n);
+    slab.w_scales = a.w_scales + n;
+    slab.bias = a.bias == nullptr ? nullptr : (const S*)a.bias + n;
+    slab.out = (S*)a.out + n;
+    int rc = quantize(a.dtype, a.x, x8, scales, n == 0 ? a.rows : 0, a.width, padded, w + n * a.width, copy, slab.outputs, a.stream);
+    if (rc == LIMN_HIP_OK) rc = product<T>(slab, x8, scales, copy, padded);
+    if (rc != LIMN_HIP_OK) return rc;
+  }
+  return LIMN_HIP_OK;
 }
 
 int check_sizes(const char* name, int dtype, int64_t rows, int64_t width, int64_t outputs) {
@@ -586,7 +613,7 @@ extern "C" int limn_hip_quantize_rows(const void* x, void* values, void* scales,
 extern "C" int64_t limn_hip_int8_linear_workspace(int dtype, int64_t rows, int64_t width, int64_t outputs) {
   if (rows < 1 || width < 1 || width > WIDEST || outputs < 1 || rows > 0x7fffffff || outputs > 0x7fffffff) return 0;
   const int64_t padded = (width + PAD - 1) / PAD * PAD;
-  return align256(rows * padded) + align256(rows * 4) + outputs * padded;  // the copy too: a weight's rows may be aligned, its start not
+  return align256(rows * padded) + align256(rows * 4) + copied_outputs(width, outputs) * padded;  // the copy too: a weight's rows may be aligned, its start not
 }
 
 extern "C" int limn_hip_int8_linear(const void* x, const void* weight, const void* weight_scales, const void* bias, void* out, int dtype, int64_t rows,
@@ -603,6 +630,6 @@ extern "C" int limn_hip_int8_linear(const void* x, const void* weight, const voi
   if (workspace_bytes < 0) return fail(LIMN_HIP_EINVAL, "%s: negative workspace size", name);
   if (workspace == nullptr || (uintptr_t)workspace % 16 != 0 || workspace_bytes < limn_hip_int8_linear_workspace(dtype, rows, width, outputs))
     return fail(LIMN_HIP_EINVAL, "%s: needs a workspace of %lld bytes, 16-byte aligned", name, (long long)limn_hip_int8_linear_workspace(dtype, rows, width, outputs));
-  const Int8Args a = {x, weight, (const float*)weight_scales, bias, out, dtype, rows, width, outputs, workspace, (hipStream_t)stream};
+  const Int8Args a = {x, weight, (const float*)weight_scales, bias, out, dtype, rows, width, outputs, outputs, workspace, (hipStream_t)stream};
   return dtype == LIMN_HIP_FLOAT32 ? linear<F32>(a) : dtype == LIMN_HIP_FLOAT16 ? linear<F16>(a) : linear<BF16>(a);
 }

@@ -280,3 +280,11 @@ def test_a_vocabulary_past_the_kernels_is_refused():
     logits = Tensor(np.zeros(1), dtype=float32).expand((1 << 24) + 1)
     with pytest.raises(ValueError, match="vocabulary"):
         sample(logits, Tensor(np.float32(0.5), dtype=float32))
+
+
+def test_an_aligned_weight_asks_for_no_copy_of_its_size():
+    """Of a width whose rows are aligned, the copy for a start that is not goes in slabs; other widths are copied whole."""
+    lib = runtime.kernels()
+    need = lambda width, outputs: lib.limn_hip_int8_linear_workspace(3, 16, width, outputs) - 16 * -(-width // 256) * 256 - 256  # noqa: E731
+    assert need(4096, 131072) <= 1 << 26 and need(1 << 17, 1 << 16) <= 1 << 26
+    assert need(512, 1000) == 512 * 1000 and need(4097, 8192) == 4352 * 8192
