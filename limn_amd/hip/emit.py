@@ -1800,7 +1800,7 @@ def bias_cast(nests: list[LoopNest], bias: Node, reader: int, kept: set) -> int 
     nothing; launched alone, each such cast cost a 4-5 us launch in the GPT step."""
     if bias in kept:
         return None
-    makers = [p for p, n in enumerate(nests) if n.kernel.target is bias]
+    makers = [p for p, n in enumerate(nests) if n.kernel.ast is bias]
     if len(makers) != 1 or makers[0] >= reader:
         return None
     p = makers[0]
@@ -1826,6 +1826,12 @@ INLINE_WHOLE = 48  # ... and with the producers evaluated in it: a float32 resid
 # (a training step of 4 float32 layers, 1 x 64 x 512: 8670 us without this bound, 3530 at 96, 2230 at 48; 5 other small steps, bfloat16, the same)
 
 
+def outputs(nest: LoopNest) -> set[Node]:
+    """The nodes by which later nests are known to read a nest's output: its root, as which an ASSIGN's new value is read too;
+    and an ASSIGN's target, whose readers get the old value from the buffer and go behind the nest without need."""
+    return {nest.kernel.ast, nest.kernel.target}
+
+
 class InlineSet:
     """Producers evaluated inside their readers, by nest index, and the buffers each reader
     then needs: every producer it reaches (directly or through another inlined producer) hands
@@ -1834,7 +1840,7 @@ class InlineSet:
     def __init__(self, nests: list[LoopNest], producers: set[int]):
         self.nests = nests
         self.producers = producers
-        self.by_target = {nests[j].kernel.target: j for j in producers}
+        self.by_target = {nests[j].kernel.ast: j for j in producers}
 
     def reached(self, nest: LoopNest) -> list[int]:
         seen: set[int] = set()
@@ -1914,7 +1920,7 @@ def inline_producers(nests: list[LoopNest], plans: list[Planned], kept: set | No
     """Small elementwise nests to evaluate inside their readers instead of launching: the
     scheduler realizes every broadcast value (a row's max, 1/sum, a LayerNorm scale) as its own
     kernel (reference limn/schedule.py:46-141), a launch of a few microseconds for a few
-    kilobytes. A producer qualifies when its output is not kept (a sink or a CUSTOM input;
+    kilobytes. A producer qualifies when its output is not kept (a sink, a CUSTOM input or an ASSIGN's;
     `kept` None inlines nothing), it has at most INLINE_CELLS cells and INLINE_BODY
     instructions (INLINE_WHOLE with those of the producers evaluated in it), and every reader is an emitted nest (not a contraction, not a relu epilogue)
     that reads it by plain loads. Its inputs stay valid for the whole plan: the executor keeps
@@ -1929,8 +1935,10 @@ def inline_producers(nests: list[LoopNest], plans: list[Planned], kept: set | No
     chosen: set[int] = set()
     whole: dict = {}  # a chosen producer's output -> the instructions of its body and of those evaluated in it
     for j, (nest, plan) in enumerate(zip(nests, plans)):
-        target = nest.kernel.target
+        target = nest.kernel.ast
         if not plan.notes.get("elementwise") or j in fused or target in kept or target not in readers:
+            continue
+        if target.op is Op.ASSIGN:  # stored for its commit
             continue
         if math.prod(target.shape) > INLINE_CELLS or len(read_nest(nest).body) > INLINE_BODY:
             continue
@@ -2029,7 +2037,7 @@ def merge_runs(nests: list[LoopNest], plans: list[Planned], custom_inputs: set |
         size[target][0] += grid
         size[target][1] += params
         deps[target] |= hit
-        owner[nest.kernel.target] = target
+        owner.update(dict.fromkeys(outputs(nest), target))
     launch_at: list[int] = []
     for g, members in enumerate(groups):
         launch_at.append(max([members[-1]] + [launch_at[d] for d in deps[g]]))
@@ -2263,7 +2271,7 @@ def _loads(body) -> list[Instr]:
 def _reads_rows_only(nest: LoopNest, member: RowMember, made: set, inlined: "InlineSet") -> bool:
     """Whether every read of a value `made` earlier in the program, by the nest or by a producer
     it evaluates in place, is a plain load of this row's value."""
-    producers = {inlined.nests[j].kernel.target: j for j in inlined.reached(nest)}
+    producers = {inlined.nests[j].kernel.ast: j for j in inlined.reached(nest)}
     # producers whose value depends on something made in the program (directly or through another)
     tainted: set = set()
     changed = True
@@ -2338,9 +2346,9 @@ def row_chains(nests: list[LoopNest], plans: list[Planned], custom_inputs: set |
             fits = m.rows == key["rows"] and (m.col is None or key["cols"] in (None, m.col[1]))
             fits = fits and (m.group is None or key["group"] in (None, m.group))
             if fits and _reads_rows_only(nest, m, made, inlined) and all(
-                    row_member(nests[p], plans[p]).kind != "cells" for p in run if nests[p].kernel.target in reads(c)):
+                    row_member(nests[p], plans[p]).kind != "cells" for p in run if outputs(nests[p]) & reads(c)):
                 run.append(c)
-                made.add(nest.kernel.target)
+                made |= outputs(nest)
                 key["cols"] = key["cols"] if m.col is None else m.col[1]
                 key["group"] = key["group"] if m.group is None else m.group
                 continue
@@ -2348,7 +2356,7 @@ def row_chains(nests: list[LoopNest], plans: list[Planned], custom_inputs: set |
             close()
         if m is not None:
             run.append(c)
-            made.add(nest.kernel.target)
+            made |= outputs(nest)
             key.update(rows=m.rows, cols=None if m.col is None else m.col[1], group=m.group)
     close()
     return chains
@@ -2538,13 +2546,13 @@ def row_source(name: str, nests: list[LoopNest], plans: list[Planned], run: list
             out_ref = f"out[{render_index(shape.out_index, wide)}]"
             lines.append(f"      if ({tid} == 0) {out_ref} = {store_expr(out_dtype, 'acc')};")
             lines.append(f"      {var} = (float)acc;")
-            values[kernel.target] = (var, out_dtype)
+            values[kernel.ast] = (var, out_dtype)
         elif m.kind == "scalar":
             lines += ["      " + value_line(i, bufs) for i in shape.body]
             write = shape.write
             lines.append(f"      if ({tid} == 0) out[{render_index(write.arg[1], wide)}] = {store_expr(out_dtype, write.srcs[0])};")
             lines.append(f"      {var} = (float){write.srcs[0]};")
-            values[kernel.target] = (var, out_dtype)
+            values[kernel.ast] = (var, out_dtype)
         else:
             col_var, extent = m.col
             vec = setup[s_][1]
@@ -2593,7 +2601,7 @@ def streamed_outputs(nests: list[LoopNest], kept: set | None, custom_inputs: set
             continue
         if math.prod(target.shape) * target.dtype.itemsize < STREAM_BYTES:
             continue
-        if any(src is target for later in nests[k + 1:] for src in later.kernel.inputs):
+        if any(src in outputs(nest) for later in nests[k + 1:] for src in later.kernel.inputs):
             continue
         out.add(k)
     return out
