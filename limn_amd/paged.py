@@ -40,7 +40,7 @@ def attend_paged(q: Tensor, k: Tensor | None, v: Tensor | None, key_pages: Tenso
     - `heads`: q holds all that is new, each token's queries, keys and values one behind another, (tokens, (heads + 2 kv_heads) hd), as
       a layer's one product gives them; k and v are None then, and nothing is copied apart.
 
-    The result is (tokens, heads, hd).
+    The result is (tokens, heads, hd). What a key that a query does not see holds, infinities and NaN among them, changes nothing in its row.
 
     There is no gradient: the call is for answering (under `no_grad`, or on tensors that need none).
     """
@@ -140,4 +140,5 @@ def _composed(q, k, v, key_pages, value_pages, starts, lengths, table, slopes, s
     e = seen.where((s - s.max(-1, keepdim=True)).exp(), 0.0)
     total = e.sum(axis=-1, keepdim=True)
     weights = e * (total + total.eq(0.0)).reciprocal()
+    values = seen.transpose(-2, -1).where(values, 0.0)  # an infinity or a NaN times a weight of 0 is NaN
     return (weights @ values).reshape(tokens, heads, hd).cast(q.dtype)
