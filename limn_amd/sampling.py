@@ -13,6 +13,9 @@ min_p; the first always. The token is the first one whose mass with all before i
 
 from __future__ import annotations
 
+import math
+import sys
+
 from limn_amd.attend import contiguous
 from limn_amd.seam import FLOATS, Tensor, active_device, custom, float32, float64, int32
 
@@ -31,7 +34,8 @@ def sample(logits: Tensor, uniforms: Tensor, *, temperature: float | Tensor = 1.
     - `top_p`: 1 or more for no limit; - `min_p`: 0 or below for none.
 
     A NaN among the logits counts as minus infinity; a row without anything above that gives token -1 and minus infinity. An
-    infinite logit has all of the mass. A uniform number outside [0, 1) takes the nearest end. No gradient flows.
+    infinite logit has all of the mass. A uniform number outside [0, 1) takes the nearest end, NaN the last token kept. Of tensors, a
+    temperature of NaN counts as 0, and a top_p or min_p of NaN is no limit. No gradient flows.
     """
     if logits.ndim < 1 or logits.dtype not in FLOATS:
         raise ValueError(f"sample needs float logits (..., vocab), got {logits.shape} {logits.dtype}")
@@ -65,13 +69,15 @@ def _composed(logits: Tensor, uniforms: Tensor, temperature, top_k, top_p, min_p
     rows, vocab = logits.shape[:-1], logits.shape[-1]
     ones = (1,) * len(rows)
     column = lambda t: t.reshape(*rows, 1)  # noqa: E731
-    x = logits.cast(float64).maximum(-1e300)  # minus infinity, and a NaN (which is not below anything), as far down as numbers go
-    x = (x <= 1e308).where(x, 1e300)
+    x = logits.cast(float64)
+    infinite = (x > sys.float_info.max).cast(float64)
+    there = infinite.max(-1, keepdim=True).where(infinite, x > -math.inf)  # not minus infinity, NaN (which is above nothing), or beside an infinity
+    x = there.where((infinite > 0).where(0.0, x), -math.inf)
     top = x.max(-1, keepdim=True)
-    some = (top > -1e300).reshape(*rows)
+    some = (top > -math.inf).reshape(*rows)
     warm = Tensor.full(rows, 1.0) if temperature is None else temperature
     heat = column((warm > 0).where(warm, 1.0).cast(float64))
-    w = ((x - top) / heat).exp()
+    w = there.where(((x - top) / heat).exp(), 0.0)
     mine, other = x.reshape(*rows, vocab, 1), x.reshape(*rows, 1, vocab)
     index = Tensor.arange(vocab)
     sooner = (index.reshape(*ones, 1, vocab) < index.reshape(*ones, vocab, 1)).cast(float64)
@@ -83,14 +89,17 @@ def _composed(logits: Tensor, uniforms: Tensor, temperature, top_k, top_p, min_p
         kept = rank < column(((top_k > 0) * (top_k < vocab)).where(top_k, vocab).cast(float64))
     if top_p is not None:
         p = column(top_p.cast(float64))
-        kept = kept * ((before < p * (kept * w).sum(-1, keepdim=True)) + (p >= 1.0) > 0)
+        kept = kept * (p < 1.0).where(before < p * (kept * w).sum(-1, keepdim=True), 1.0)
     if min_p is not None:
-        kept = kept * (w >= column(min_p.cast(float64)))
+        kept = kept * (1.0 - (w < column(min_p.cast(float64))))
     kept = (kept + rank.eq(0.0)) > 0
     mass = (kept * w).sum(-1, keepdim=True)
-    short = (kept * ((before + w) <= column(uniforms.cast(float64)) * mass)).sum(-1)
-    place = (warm > 0).cast(float64) * short.minimum(kept.sum(-1) - 1.0)
+    # past the end, NaN too: the last one kept whose mass is one, as the kernels' whole numbers have it
+    u = uniforms.cast(float64)
+    short = (u < 1.0).where((kept * ((before + w) <= column(u) * mass)).sum(-1), vocab)
+    heavy = w > 2.0 ** -(1 + min(52, 62 - (vocab - 1).bit_length()))
+    place = (warm > 0).cast(float64) * short.minimum((kept * heavy).sum(-1) - 1.0)
     hit = rank.eq(column(place))
     token = (hit * index.cast(float64).reshape(*ones, vocab)).sum(-1).cast(int32)
     share = (warm > 0).cast(float64).where((hit * w).sum(-1) / mass.reshape(*rows), 1.0)
-    return some.cast(int32).where(token, -1), some.where(share.log(), float("-inf")).cast(float32)
+    return some.cast(int32).where(token, -1), some.where(share.log(), -math.inf).cast(float32)
