@@ -47,7 +47,7 @@ def sample(logits: Tensor, uniforms: Tensor, *, temperature: float | Tensor = 1.
     rules: list[Tensor | None] = []
     for name, rule, off, dtype in (("temperature", temperature, 1.0, float32), ("top_k", top_k, 0, int32), ("top_p", top_p, 1.0, float32), ("min_p", min_p, 0.0, float32)):
         if not isinstance(rule, Tensor):
-            number = int(rule) if dtype == int32 else float(rule)
+            number = int(rule) if dtype == int32 and math.isfinite(rule) else float(rule)
             if number != rule or abs(number) > 2**31 - 1:
                 raise ValueError(f"sample: {name} must be a finite {'whole ' if dtype == int32 else ''}number, got {rule}")
             rules.append(None if number == off else Tensor.full(rows, number, dtype=dtype))

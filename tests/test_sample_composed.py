@@ -78,3 +78,11 @@ def test_an_infinite_temperature_draws_evenly_from_what_is_there():
     tokens, logs = sample(Tensor(logits), Tensor(u), temperature=Tensor(np.full(4, np.inf, np.float32)))
     np.testing.assert_array_equal(tokens.numpy(), [0, 4, 2, 5])
     np.testing.assert_allclose(logs.numpy(), np.log(0.25), rtol=2.0**-23)
+
+
+@pytest.mark.parametrize("value", [float("inf"), float("-inf"), float("nan")])
+def test_numbers_that_are_no_numbers_are_refused(value):
+    logits, u, _ = logit_rows(3, 2, 5)
+    for name in KINDS:
+        with pytest.raises(ValueError, match="finite"):
+            sample(Tensor(logits), Tensor(u), **{name: value})
