@@ -23,7 +23,7 @@ WIDEST = 1 << 17  # products of 127 * 128 whose sum a 32-bit integer holds
 
 def quantize_rows(x: Tensor) -> tuple[Tensor, Tensor]:
     """x (..., width) as int8 (..., width) and a float32 scale for each row (...). A row with an infinity or a NaN has the scale NaN
-    and zeros (composed of primitives, whatever that makes of it)."""
+    and zeros."""
     if x.ndim < 1 or x.dtype not in FLOATS:
         raise ValueError(f"quantize_rows needs a float tensor (..., width), got {x.shape} {x.dtype}")
     x = x.detach()
@@ -72,5 +72,6 @@ def _rounded(x: Tensor) -> tuple[Tensor, Tensor]:
     """Rows as whole float32 numbers from -127 to 127, and their scales (..., 1)."""
     x = x.cast(float32)
     scales = (x.maximum(-x).max(-1, keepdim=True) / 127.0).maximum(2.0**-126)
+    fine = scales < math.inf
     magic = 1.5 * 2.0**23  # a float32 this large has no bits below 1: adding it rounds to whole numbers, ties to even
-    return ((x * scales.reciprocal()) + magic) - magic, scales
+    return fine.where(((x * scales.reciprocal()) + magic) - magic, 0.0), fine.where(scales, math.nan)

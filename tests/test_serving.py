@@ -288,3 +288,18 @@ def test_an_aligned_weight_asks_for_no_copy_of_its_size():
     need = lambda width, outputs: lib.limn_hip_int8_linear_workspace(3, 16, width, outputs) - 16 * -(-width // 256) * 256 - 256  # noqa: E731
     assert need(4096, 131072) <= 1 << 26 and need(1 << 17, 1 << 16) <= 1 << 26
     assert need(512, 1000) == 512 * 1000 and need(4097, 8192) == 4352 * 8192
+
+
+@pytest.mark.parametrize("dtype", ["float32", "float64"])
+def test_rows_with_infinities_and_nan_in_8_bits(dtype):
+    """Composed of primitives as in the kernels: zeros and the scale NaN, results of NaN, and no other row's."""
+    x = np.random.default_rng(6).standard_normal((6, 20)).astype(dtype)
+    x[1, 3], x[2, 19], x[4, 0] = np.inf, np.nan, -np.inf
+    kind = DTYPES[dtype]
+    with np.errstate(invalid="ignore"):
+        values, scales = quantize_rows(Tensor(x, dtype=kind))
+        y = int8_linear(Tensor(x, dtype=kind), Tensor(np.eye(5, 20), dtype=int8), Tensor(np.ones(5), dtype=float32)).numpy()
+        values, scales = values.numpy(), scales.numpy()
+    odd = np.isin(np.arange(6), [1, 2, 4])
+    assert (values[odd] == 0).all() and np.isnan(scales[odd]).all() and np.isnan(y[odd]).all()
+    assert np.isfinite(scales[~odd]).all() and np.isfinite(y[~odd]).all()
