@@ -58,11 +58,10 @@ class Cache:
 
     def reserve(self, sequence: int, length: int) -> None:
         """Pages for the first `length` positions of a sequence, those it has first."""
-        own = self.tables.setdefault(sequence, [])
-        more = -(-length // self.page) - len(own)
+        more = -(-length // self.page) - len(self.tables.get(sequence, ()))
         if more > len(self.free):
             raise ValueError(f"Cache: {length} positions of sequence {sequence} take {more} more pages, {len(self.free)} are free")
-        own.extend(self.free.pop() for _ in range(more))
+        self.tables.setdefault(sequence, []).extend(self.free.pop() for _ in range(more))
 
     def drop(self, sequence: int) -> None:
         """The sequence is over: its pages are free."""
@@ -71,6 +70,8 @@ class Cache:
     def table(self, sequences: Sequence[int]) -> Tensor:
         """The sequences' pages (sequences, the most that one has) int32, -1 behind the last."""
         rows = [self.tables[s] for s in sequences]
+        if not rows:
+            raise ValueError("Cache: a table is of at least one sequence")
         out = np.full((len(rows), max(1, *(len(r) for r in rows))), -1, dtype=np.int32)
         for to, row in zip(out, rows):
             to[: len(row)] = row

@@ -148,3 +148,12 @@ def test_a_model_that_records_is_refused():
     cache.reserve(0, 2)
     with pytest.raises(ValueError, match="no gradient"):
         prefill(model, cache, [0], [[1, 2]], cache.table([0]))
+
+
+def test_a_table_of_no_sequences_and_a_reservation_that_fails():
+    cache = Cache(model_of(PLAIN), 3, 4)
+    with pytest.raises(ValueError, match="at least one"):
+        cache.table([])
+    with pytest.raises(ValueError, match="free"):
+        cache.reserve(2, 13)
+    assert cache.tables == {} and len(cache.free) == 3
