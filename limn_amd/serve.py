@@ -78,10 +78,26 @@ class Cache:
         return Tensor(out, dtype=int32)
 
 
+def in_vocabulary(name: str, model: GPT, prompts: Sequence[Sequence[int]]) -> None:
+    if any(not 0 <= t < model.cfg.vocab for p in prompts for t in p):
+        raise ValueError(f"{name}: tokens must lie in [0, {model.cfg.vocab})")
+
+
 def prefill(model: GPT, cache: Cache, sequences: Sequence[int], prompts: Sequence[Sequence[int]], table: Tensor, part: int = 4096) -> Tensor:
     """The prompts through the model, their keys and values into the cache: the logits (sequences, vocab) behind each one's last token.
     Parts hold at most `part` tokens and end anywhere; each sequence goes on in the next one where it ended. For answering: under
-    `no_grad`, with pages reserved for the prompts."""
+    `no_grad`, with pages reserved for the prompts, at least one token each."""
+    if part < 1 or not prompts or len(sequences) != len(prompts) or any(len(p) == 0 for p in prompts):
+        raise ValueError(f"prefill needs a part of at least 1 and a prompt of at least one token for each sequence, got {part}, {len(sequences)} sequences and prompts of {[len(p) for p in prompts]}")
+    longest = max(len(p) for p in prompts)
+    in_vocabulary("prefill", model, prompts)
+    if not model.cfg.distance and longest > model.cfg.ctx:
+        raise ValueError(f"prefill: learned positions end at {model.cfg.ctx}, a prompt of {longest} tokens does not fit")
+    short = [s for s, p in zip(sequences, prompts) if len(cache.tables.get(s, ())) * cache.page < len(p)]
+    if short:
+        raise ValueError(f"prefill: the prompts of the sequences {short} have more positions than pages are reserved for")
+    if table.ndim != 2 or table.shape[0] != len(prompts) or table.shape[1] * cache.page < longest:
+        raise ValueError(f"prefill: a table of {table.shape} does not hold {len(prompts)} prompts of up to {longest} tokens in pages of {cache.page}")
     todo, done = [list(p) for p in prompts], [0] * len(prompts)
     logits: Tensor | None = None
     while any(at < len(p) for at, p in zip(done, todo)):
@@ -112,8 +128,7 @@ def generate(model: GPT, prompts: Sequence[Sequence[int]], count: int, *, temper
     cfg, n = model.cfg, len(prompts)
     if n == 0 or count < 1 or part < 1 or page < 1 or any(len(p) == 0 for p in prompts):
         raise ValueError("generate needs prompts of at least one token, and a count, part and page of at least 1")
-    if any(not 0 <= t < cfg.vocab for p in prompts for t in p):
-        raise ValueError(f"generate: tokens must lie in [0, {cfg.vocab})")
+    in_vocabulary("generate", model, prompts)
     if not cfg.distance and max(len(p) for p in prompts) + count > cfg.ctx + 1:
         raise ValueError(f"generate: learned positions end at {cfg.ctx}, a prompt of {max(len(p) for p in prompts)} tokens and {count} more do not fit")
     rules = dict(temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)

@@ -150,6 +150,36 @@ def test_a_model_that_records_is_refused():
         prefill(model, cache, [0], [[1, 2]], cache.table([0]))
 
 
+@pytest.mark.parametrize(
+    "change, match",
+    [
+        (dict(part=0), "part"),
+        (dict(prompts=[[1, 2], []]), "at least one"),
+        (dict(prompts=[]), "at least one"),
+        (dict(sequences=[0]), "at least one"),
+        (dict(prompts=[[1, 2], [37]]), "must lie"),
+        (dict(prompts=[[1, 2], [-1]]), "must lie"),
+        (dict(prompts=[[1, 2], [3] * 9]), "reserved"),
+        (dict(sequences=[0, 5]), "reserved"),
+        (dict(prompts=[list(range(25)), [1]]), "positions end"),
+        (dict(table=[[0, 1]]), "table"),
+        (dict(table=[[0], [1]]), "table"),
+    ],
+    ids=str,
+)
+def test_prefill_refuses(change, match):
+    """A part of nothing would never end; tokens and positions outside the model's tables would be read there."""
+    with no_grad():
+        model = held(model_of(PLAIN))
+        cache = Cache(model, 12, 4)
+        cache.reserve(0, 25)
+        cache.reserve(1, 8)
+        a = {**dict(sequences=[0, 1], prompts=[[1, 2, 3, 4, 5], [3]], part=3), **change}
+        table = Tensor(np.array(a["table"], dtype=np.int32), dtype=int32) if "table" in a else cache.table([0, 1])
+        with pytest.raises(ValueError, match=match):
+            prefill(model, cache, a["sequences"], a["prompts"], table, a["part"])
+
+
 def test_a_table_of_no_sequences_and_a_reservation_that_fails():
     cache = Cache(model_of(PLAIN), 3, 4)
     with pytest.raises(ValueError, match="at least one"):
