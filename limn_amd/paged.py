@@ -106,7 +106,8 @@ def _composed(q, k, v, key_pages, value_pages, starts, lengths, table, slopes, s
     length = lengths.maximum(0).minimum(places).reshape(1, sequences)
     known = mine.sum(-1)
     at = (mine * (length - end)).sum(-1) + row  # p, where known
-    own = table.gather_rows((mine * seq.reshape(1, sequences)).sum(-1))  # (tokens, table_pages)
+    # (rows are gathered by numbers that lie inside whatever the tensors hold)
+    own = table.gather_rows((mine * seq.reshape(1, sequences)).sum(-1).minimum(sequences - 1))  # (tokens, table_pages)
     inside = (own >= 0) * (own < pages)
     own = inside.where(own, 0)
     pools = []
@@ -118,7 +119,7 @@ def _composed(q, k, v, key_pages, value_pages, starts, lengths, table, slopes, s
             slot = (here * (own * page + (at.reshape(tokens, 1) - of * page) + 1)).sum(-1) - 1  # -1: none
             cell = Tensor.arange(pages * page).reshape(pages * page, 1)
             writes = cell.eq(slot.reshape(1, tokens))
-            writer = (writes * row.reshape(1, tokens)).sum(-1)
+            writer = (writes * row.reshape(1, tokens)).sum(-1).minimum(tokens - 1)
             new = fresh.reshape(tokens, kv_heads * hd).gather_rows(writer).reshape(pages, page, kv_heads, hd).permute(0, 2, 1, 3)
             hit = writes.sum(-1).reshape(pages, 1, page, 1)
             pool.assign(contiguous(hit.where(new, Tensor.from_node(pool.node))))

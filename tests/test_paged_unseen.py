@@ -58,3 +58,15 @@ def test_later_tokens(dtype):
     x["v"][3, :, ::3], x["v"][4], x["k"][4] = np.inf, np.nan, np.nan
     got = check(x, dtype)
     assert np.isfinite(got[:3]).all() and not np.isfinite(got[3:]).all()
+
+
+def test_no_row_is_gathered_from_outside():
+    """A page that two sequences write to, and starts that do not ascend: nobody's promise, and no read past a tensor."""
+    set_device("numpy")
+    x = paged_inputs(5, counts=(3, 2, 4, 3, 1), lengths=(5, 6, 4, 9, 3))
+    t = tensors({**x, "table": np.repeat(x["table"][3:4], 5, 0)}, "float32")
+    assert attend_paged(**t).numpy().shape == x["q"].shape
+    t = tensors({**x, "starts": np.array([0, 13, 0, 13, 0, 13], np.int32)}, "float32")
+    assert attend_paged(**t).numpy().shape == x["q"].shape
+    t = tensors({**x, "starts": np.array([-9, 13, -2, 99, 5, 2**31 - 1], np.int32), "lengths": np.array([-5, 2**31 - 1, 0, 7, -(2**31)], np.int32)}, "float32")
+    assert attend_paged(**t).numpy().shape == x["q"].shape
