@@ -8,9 +8,11 @@ import pytest
 
 from conftest import DTYPES, download
 from limn_amd.paged import attend_paged
+from limn_amd.sampling import sample
 from limn_amd.seam import Tensor, capture, realize, set_device, use_device
 from oracle.attend import within
 from oracle.serving import paged
+from oracle.serving import sample as sample_oracle
 from serving import paged_inputs
 from test_paged_gpu import tensors
 
@@ -80,3 +82,34 @@ def test_attend_paged_composed(hipdev, dtype, hd):
         np.testing.assert_array_equal(t["key_pages"].numpy(), keys)
         np.testing.assert_array_equal(t["value_pages"].numpy(), values)
         x["key_pages"], x["value_pages"] = keys, values
+
+
+@pytest.mark.parametrize("captured", [False, True])
+def test_calls_of_kernels_read_what_was_assigned(hipdev, captured):
+    """Lengths that a step moves on itself, and numbers that it halves, in one batch with the calls that take them."""
+    use_device(hipdev)
+    x = paged_inputs(6, dtype="bfloat16", counts=(1, 1, 1), lengths=(20, 3, 9), heads=4, kv_heads=2, hd=64, page=8, table_pages=4)
+    x["table"][:] = np.arange(12).reshape(3, 4)
+    t = tensors(hipdev, x, "bfloat16")
+    logits = np.random.default_rng(7).standard_normal((3, 500)).astype(np.float32)
+    u, z = Tensor(np.array([0.9, 0.7, 0.99], np.float32)).realize(), Tensor(logits).realize()
+
+    def step():
+        t["lengths"].assign(t["lengths"].detach() + 1)
+        u.assign(u.detach() * 0.5)
+        out = attend_paged(**t)
+        tokens, logs = sample(z, u.detach())
+        realize(out, tokens, logs)
+        return out, tokens, logs
+
+    run, share = capture(step) if captured else step, np.array([0.9, 0.7, 0.99], np.float32)
+    for turn in range(6):
+        out, tokens, logs = run()
+        x["lengths"], share = x["lengths"] + 1, share * np.float32(0.5)
+        (want, bound), x["key_pages"], x["value_pages"] = paged(**x, dtype="bfloat16")
+        within(out.numpy(), want, bound, f"turn {turn}")
+        drawn, (lp, b) = sample_oracle(logits, share)
+        np.testing.assert_array_equal(tokens.numpy(), drawn)
+        within(logs.numpy(), lp, b, "logprob")
+        np.testing.assert_array_equal(t["lengths"].numpy(), x["lengths"])
+        assert (Tensor(np.ones(1000)) * 3.0).sum().item() == 3000.0
