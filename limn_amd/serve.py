@@ -87,7 +87,7 @@ def prefill(model: GPT, cache: Cache, sequences: Sequence[int], prompts: Sequenc
     """The prompts through the model, their keys and values into the cache: the logits (sequences, vocab) behind each one's last token.
     Parts hold at most `part` tokens and end anywhere; each sequence goes on in the next one where it ended. For answering: under
     `no_grad`, with pages reserved for the prompts, at least one token each."""
-    if part < 1 or not prompts or len(sequences) != len(prompts) or any(len(p) == 0 for p in prompts):
+    if part < 1 or len(prompts) == 0 or len(sequences) != len(prompts) or any(len(p) == 0 for p in prompts):
         raise ValueError(f"prefill needs a part of at least 1 and a prompt of at least one token for each sequence, got {part}, {len(sequences)} sequences and prompts of {[len(p) for p in prompts]}")
     longest = max(len(p) for p in prompts)
     in_vocabulary("prefill", model, prompts)

@@ -187,3 +187,10 @@ def test_a_table_of_no_sequences_and_a_reservation_that_fails():
     with pytest.raises(ValueError, match="free"):
         cache.reserve(2, 13)
     assert cache.tables == {} and len(cache.free) == 3
+
+
+def test_prompts_in_an_array():
+    model = model_of(EVERY)
+    prompts = np.array([[1, 2, 3], [4, 5, 6]])
+    for a, b in zip(generate(model, prompts, 3, seed=1), generate(model, prompts.tolist(), 3, seed=1)):
+        np.testing.assert_array_equal(a, b)
