@@ -241,7 +241,12 @@ Plan plan_of(const PagedArgs& a, bool tiled) {
   const int64_t places = a.table_pages * a.page, all = a.tokens * a.group(), each = (a.tokens + a.sequences - 1) / a.sequences * a.group();
   p.tiled = tiled && a.dtype != LIMN_HIP_FLOAT32 && a.tokens > a.sequences && all > FEW_ROWS;
   p.lone = false;
-  if (p.tiled) {  // (24 single tokens beside two parts of 500, in parts for 256, 512, 768 and 1024 workgroups: 96, 70, 53 and 63 us)
+  // In parts for 256, 512, 768, 1024 and 1536 workgroups, us: 24 single tokens beside two parts of 500 96, 72, 52, 57 and 56; 8 beside one of
+  // 1000, one key head, 16000 positions 171, 93, 78, 95, 86; a part alone of 256 tokens against 8192 positions, 8 key heads 96, 67, 81, 79,
+  // 76; of 2048, 2 key heads 244, 123, 129, 117, 121; of 128 against 32768, 8 key heads of 64 dims 59, 44, 44, 44, 44; of 512 against 16384,
+  // one key head 56, 55, 55, 55, 54. Two workgroups share a CU, so 512 is one round of equal workgroups, which a part alone has; in a
+  // mixed batch most slots are short or empty, and 768 even them out. What a batch holds is known on the device alone.
+  if (p.tiled) {
     p.rows = 128;
     cut(p, (places + 63) / 64 + 1, (a.sequences + all / 128) * a.kv_heads, 768);
     return p;

@@ -42,7 +42,8 @@ def attend_paged(q: Tensor, k: Tensor | None, v: Tensor | None, key_pages: Tenso
 
     The result is (tokens, heads, hd). What a key that a query does not see holds, infinities and NaN among them, changes nothing in its row.
 
-    There is no gradient: the call is for answering (under `no_grad`, or on tensors that need none).
+    There is no gradient: the call is for answering (under `no_grad`, or on tensors that need none). Nothing else of the batch that
+    realizes the result may read the pages, or write what it reads: the order between them is not set.
     """
     together = heads > 0
     if heads < 0 or q.ndim != (2 if together else 3) or key_pages.ndim != 4:
